@@ -375,6 +375,180 @@ int q3h_codec_back(q3h_codec *c, const float *x, int frames, float *pcm);
 int64_t q3h_codec_bytes(const q3h_codec *c);
 int q3h_codec_destroy(q3h_codec *c);
 
+/* ---- drafted continuations: a cache of its own, the rotary forms, attention
+   over a tree of drafted rows, scores of given tokens (no reference
+   counterpart; the reference decodes one token at a time over an f32 or f16
+   cache) ----
+
+   These four operators work on device memory of the caller, of the GPU of
+   their handle, in the order of a stream of the caller (hipStream_t as void *;
+   NULL: the default stream). They only enqueue kernels: no allocation, no
+   copy, no wait, so they can be captured into a graph (a captured call's
+   kernels hold the pointers it was given). The caller's current device is as
+   it was when they return. Arguments that the host can see are checked
+   (Q3H_E_ARG, Q3H_E_CAPACITY, nothing enqueued); what only the device holds
+   (lengths, counts, parents, tokens) is checked there, and what is out of range
+   never reads or writes outside the tensors: the rows concerned come out as
+   NaN. Calls on one cache may run at once where none writes rows that another
+   reads or writes.
+
+   A call covers the first `sequences` sequences of a cache, each with `rows`
+   drafted rows: tensors are [sequences][rows][...], row r of sequence b at row
+   b * rows + r, rows ld* floats apart. lens [sequences]: the positions each
+   sequence held before the draft; its row r goes to (is) position lens[b] + r
+   of the cache. counts [sequences] (nullable: all rows): how many of the rows
+   there are, taken into [0, rows]; the others are neither read nor written.
+   parents [sequences][rows] (nullable): the row that row r continues, below r,
+   or -1 for one that continues the sequence itself; for at most
+   Q3H_TREE_MAX_ROWS rows. A row sees the positions before the draft, the rows on
+   its path and itself, and its rotary position is lens[b] plus its depth.
+   NULL: a chain, row r after row r - 1, of any length (a prompt, or one new
+   token). */
+#define Q3H_KV_F32 0
+#define Q3H_KV_F16 1
+/* a byte per element and one f32 scale per position and kv head: scale =
+   max |x| / 127 rounded to f32, byte = x / scale rounded to even, both from 64
+   bits. A row with an infinity or NaN reads as NaN. */
+#define Q3H_KV_Q8 2
+#define Q3H_TREE_MAX_ROWS 64
+#define Q3H_TOP_MAX 64
+
+typedef struct q3h_rope q3h_rope;
+typedef struct q3h_cache q3h_cache;
+
+/* rotary positions: the first rot_dim elements of a head turn in pairs i by
+   position * f(i), in 64 bits; f(i) = theta ^ (-2 i / rot_dim), then
+   - Q3H_ROPE_PLAIN: as it is;
+   - Q3H_ROPE_LINEAR: / factor;
+   - Q3H_ROPE_YARN: / factor where a pair turns less than beta_slow times over
+     original_positions, as it is where more than beta_fast times, in between a
+     ramp over the pair number (its ends rounded outwards to whole pairs);
+   - Q3H_ROPE_BANDS: / factor where a pair turns less than low_turns times over
+     original_positions, as it is where more than high_turns times, in between
+     mixed by its turns. */
+#define Q3H_ROPE_PLAIN 0
+#define Q3H_ROPE_LINEAR 1
+#define Q3H_ROPE_YARN 2
+#define Q3H_ROPE_BANDS 3
+typedef struct {
+  int32_t head_dim;      /* 64 or 128 */
+  int32_t rot_dim;       /* even, 2 .. head_dim; the other elements stay */
+  int32_t interleaved;   /* pair i: elements 2i, 2i + 1; 0: i, i + rot_dim / 2 */
+  int32_t max_positions; /* positions of the table (16 bytes a pair each) */
+  float theta;
+  int32_t scaling;            /* Q3H_ROPE_* */
+  float factor;               /* all but PLAIN: > 0 */
+  int32_t original_positions; /* YARN, BANDS: > 0 */
+  float beta_fast, beta_slow; /* YARN: beta_fast > beta_slow > 0 */
+  float low_turns, high_turns; /* BANDS: high_turns > low_turns > 0 */
+  float magnitude; /* on cosine and sine; 0: 0.1 ln(factor) + 1 for YARN with a
+                      factor above 1, else 1 */
+} q3h_rope_config;
+int q3h_rope_create(q3h_device *dev, const q3h_rope_config *cfg, q3h_rope **out);
+int q3h_rope_destroy(q3h_rope *r);
+
+/* a K/V cache of several sequences: per sequence keys, then values
+   [layers][kv_heads][max_positions][head_dim] in the format (Q3H_KV_*), the
+   layout of a context's cache, then for Q3H_KV_Q8 the scales of the keys and
+   of the values [layers][kv_heads][max_positions]; zeros at first */
+typedef struct {
+  int32_t sequences, layers, kv_heads, head_dim; /* head_dim 64 or 128 */
+  int32_t max_positions, format;
+} q3h_cache_config;
+int q3h_cache_create(q3h_device *dev, const q3h_cache_config *cfg, q3h_cache **out);
+int64_t q3h_cache_bytes(const q3h_cache *c);
+int q3h_cache_destroy(q3h_cache *c);
+
+/* The drafted rows' keys and values into the cache: k and v [..][kv_heads]
+   [head_dim], and with heads > 0 the queries q [..][heads][head_dim] to q_out.
+   Queries and keys are RMS-normed over the head (q_norm, k_norm [head_dim],
+   nullable: not normed) and turned (rope, nullable: not turned; its
+   max_positions not below the cache's), in 64 bits and rounded once to f32;
+   then k and v are rounded to the format. q_out may be q itself (the same
+   pointer and row distance) and overlap nothing else. A sequence whose rows would pass its positions, or of
+   negative length, gets no rows and NaN queries, and so does a row on whose
+   path a parent is not below its row. */
+typedef struct {
+  int32_t layer, sequences, rows, heads;
+  const float *q, *k, *v;
+  int64_t ldq, ldk, ldv;
+  float *q_out;
+  int64_t ld_out;
+  const float *q_norm, *k_norm;
+  float eps;
+  const q3h_rope *rope;
+  const int32_t *lens, *counts, *parents;
+} q3h_append_args;
+int q3h_cache_append(q3h_cache *c, const q3h_append_args *a, void *stream);
+
+/* positions starts[b] .. + counts[b] - 1 of a layer (starts nullable: 0) as
+   the f32 values that the cache holds: k and v (either nullable)
+   [sequences][rows][kv_heads][head_dim], contiguous */
+int q3h_cache_read(q3h_cache *c, int layer, int sequences, int rows, const int32_t *starts,
+                   const int32_t *counts, float *k, float *v, void *stream);
+
+/* out = softmax(scale q . K + mask) V for the drafted rows, whose keys and
+   values the cache holds already (q3h_cache_append): q and out
+   [..][heads][head_dim], heads a multiple of kv_heads, query head h on kv head
+   h / (heads / kv_heads). max_len: no length in lens is above it (the host's
+   bound, it sizes the launch; a longer or negative one: NaN rows). scale: 0 for
+   1 / sqrt(head_dim). Products and sums keep f32's precision in every format.
+   Infinities and NaN at positions a row does not see do not reach it. workspace:
+   q3h_cache_attend_workspace bytes for the same sequences, rows, heads and max_len
+   (of the caller, 256-byte aligned, one for each call that may run at once;
+   nullable where that is 0). out may be q itself. */
+typedef struct {
+  int32_t layer, sequences, rows, heads, max_len;
+  float scale;
+  const float *q;
+  int64_t ldq;
+  float *out;
+  int64_t ld_out;
+  const int32_t *lens, *counts, *parents;
+  void *workspace;
+  int64_t workspace_bytes;
+} q3h_attend_args;
+/* negative: a Q3H_E* code */
+int64_t q3h_cache_attend_workspace(const q3h_cache *c, int sequences, int rows, int heads,
+                                   int max_len);
+int q3h_cache_attend(q3h_cache *c, const q3h_attend_args *a, void *stream);
+
+/* The drafted rows that are kept, moved to the front: kept [sequences][rows]
+   holds kept_counts[b] row numbers, each above the one before (a path from a
+   root down); row kept[b][i], at position lens[b] + kept[b][i], goes to
+   position lens[b] + i, in every layer. The caller's lengths grow by
+   kept_counts. A list that is not of that form leaves its sequence as it is. */
+int q3h_cache_keep(q3h_cache *c, int sequences, int rows, const int32_t *lens,
+                   const int32_t *kept, const int32_t *kept_counts, void *stream);
+
+/* Scores of rows of logits [rows][vocab] (dtype Q3H_F32 or Q3H_BF16, rows ld
+   elements apart), computed in f32 from one read of them: with lse = log sum
+   exp of a row,
+   - logprobs [rows][tokens_per_row]: logit - lse of the given tokens (tokens
+     [rows][tokens_per_row]; a token outside [0, vocab): NaN);
+   - entropy [rows] (nullable): lse - sum p logit, logits of -infinity adding
+     nothing;
+   - top_ids, top_logprobs [rows][top_k] (top_k 0: none; at most Q3H_TOP_MAX and
+     vocab): the largest logits from the top, of equal ones the lowest token
+     first, NaN last.
+   A row with a NaN or +infinity, or of -infinity alone, has NaN scores.
+   workspace: q3h_token_logprobs_workspace bytes for the same rows, vocab and
+   top_k, as q3h_cache_attend's. */
+typedef struct {
+  const void *logits;
+  int64_t ld;
+  int32_t dtype, rows, vocab;
+  int32_t tokens_per_row, top_k;
+  const int32_t *tokens;
+  float *logprobs, *entropy;
+  int32_t *top_ids;
+  float *top_logprobs;
+  void *workspace;
+  int64_t workspace_bytes;
+} q3h_score_args;
+int64_t q3h_token_logprobs_workspace(int rows, int vocab, int top_k);
+int q3h_token_logprobs(q3h_device *dev, const q3h_score_args *a, void *stream);
+
 /* ---- helpers ---- */
 
 /* ggml quantize_row_q8_0_ref (InferQuantizeRowQ8_0Ref, lm.pas:265-267) on the

@@ -1,0 +1,603 @@
+// q3h_cache.hip - a K/V cache of several sequences: rotary tables, the append
+// of drafted rows (norm, rotation, rounding to the cache's format), reading
+// back, and moving the kept rows to the front.
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+#include <string>
+#include <vector>
+
+#include "q3h.h"
+#include "q3h_api_internal.h"
+#include "q3h_draft.h"
+#include "q3h_wave.h"
+
+namespace q3h {
+
+namespace {
+
+constexpr int kThreads = 256;
+
+// table [positions][pairs] of (cos, sin) * mag at position * freq, in 64 bits
+__global__ void k_rope_table(const double *freq, double mag, int pairs, size_t n, double2 *table) {
+  const size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= n) return;
+  double s, c;
+  sincos((double)(i / pairs) * freq[i % pairs], &s, &c);
+  table[i] = make_double2(c * mag, s * mag);
+}
+
+// sum over the G lanes (32 or 64) of a head, in every lane
+template <int G>
+__device__ __forceinline__ double head_sum(double v) {
+  if constexpr (G == 64) {
+    return wave_sum_dpp_d(v);
+  } else {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+  }
+}
+template <int G>
+__device__ __forceinline__ float head_max(float v) {
+  if constexpr (G == 64) return wave_max_dpp(v);
+  return half_max_dpp(v);
+}
+
+// One head of one row per HD / 2 lanes, a pair of elements each: those that
+// turn together, or two neighbours of the part that does not turn. Everything
+// up to the f32 row is in 64 bits, so that a byte of the int8 format is that of
+// the definition and not of a rounding before it.
+template <int FMT, int HD>
+__global__ __launch_bounds__(kThreads) void k_cache_append(AppendRows a) {
+  constexpr int G = HD / 2;
+  const int lane = threadIdx.x & 63, sub = lane & (G - 1);
+  const int row = blockIdx.x, b = row / a.kv.rows, t = row - b * a.kv.rows;
+  const KvSeq s = kv_sequence(a.kv, b);
+  if (t >= s.count) return;
+  int depth = t;
+  bool bad = s.len < 0 || s.len > s.max_pos - s.count;
+  if (a.parents) {
+    const Path path = tree_path(a.parents + (size_t)b * a.kv.rows, a.kv.rows);
+    depth = __shfl(path.depth, t);
+    bad = bad || __shfl((int)path.bad, t) != 0;
+  }
+  const int kvh = a.kv.kvh, all = a.heads + 2 * kvh;
+  const int half = a.rot_dim >> 1;
+  const bool turns = a.table && sub < half;
+  int e0 = 2 * sub, e1 = e0 + 1;
+  if (a.table && !a.interleaved) {
+    e0 = turns ? sub : a.rot_dim + 2 * (sub - half);
+    e1 = turns ? sub + half : e0 + 1;
+  }
+  double2 cs = make_double2(1.0, 0.0);
+  if (turns && !bad) cs = a.table[(size_t)(s.len + depth) * half + sub];
+  const int waves = gridDim.y * (kThreads / 64) * (64 / G);
+  for (int j = (blockIdx.y * (kThreads / 64) + (threadIdx.x >> 6)) * (64 / G) + lane / G; j < all;
+       j += waves) {
+    const int part = j < a.heads ? 0 : j < a.heads + kvh ? 1 : 2;
+    const int g = part == 0 ? j : part == 1 ? j - a.heads : j - a.heads - kvh;
+    const float *src = part == 0   ? a.q + (size_t)row * a.ldq
+                       : part == 1 ? a.k + (size_t)row * a.ldk
+                                   : a.v + (size_t)row * a.ldv;
+    float x0 = src[(size_t)g * HD + e0], x1 = src[(size_t)g * HD + e1];
+    const float *w = part == 0 ? a.q_norm : part == 1 ? a.k_norm : nullptr;
+    if (part < 2) {
+      double y0 = x0, y1 = x1;
+      if (w) {
+        const double ss = head_sum<G>(y0 * y0 + y1 * y1);
+        const double inv = 1.0 / sqrt(ss / HD + (double)a.eps);
+        y0 = y0 * inv * (double)w[e0];
+        y1 = y1 * inv * (double)w[e1];
+      }
+      if (turns) {
+        const double r0 = y0 * cs.x - y1 * cs.y;
+        y1 = y1 * cs.x + y0 * cs.y;
+        y0 = r0;
+      }
+      x0 = (float)y0;
+      x1 = (float)y1;
+    }
+    if (part == 0) {
+      float *o = a.q_out + (size_t)row * a.ld_out + (size_t)g * HD;
+      o[e0] = bad ? NAN : x0;
+      o[e1] = bad ? NAN : x1;
+      continue;
+    }
+    if (bad) continue;
+    const int64_t at = kv_row(a.kv, s, part - 1, g, s.len + t);
+    if constexpr (FMT == Q3H_KV_Q8) {
+      // (fmaxf drops a NaN: it is found by its comparison)
+      const bool finite = fabsf(x0) < INFINITY && fabsf(x1) < INFINITY;
+      const float m = head_max<G>(finite ? fmaxf(fabsf(x0), fabsf(x1)) : INFINITY);
+      float d = (float)((double)m / 127.0);
+      int q0 = 0, q1 = 0;
+      if (m == INFINITY) {
+        d = NAN;
+      } else if (d > 0.f) {
+        q0 = min(127, max(-127, (int)rint((double)x0 / (double)d)));
+        q1 = min(127, max(-127, (int)rint((double)x1 / (double)d)));
+      }
+      int8_t *o = reinterpret_cast<int8_t *>(s.k0) + at * HD;
+      o[e0] = (int8_t)q0;
+      o[e1] = (int8_t)q1;
+      if (sub == 0) kv_scales(a.kv, s, HD)[at] = d;
+    } else {
+      using KV = std::conditional_t<FMT == Q3H_KV_F16, _Float16, float>;
+      KV *o = reinterpret_cast<KV *>(s.k0) + at * HD;
+      o[e0] = to_cache<KV>(x0);
+      o[e1] = to_cache<KV>(x1);
+    }
+  }
+}
+
+// 8 elements of a row per thread
+template <int FMT, int HD>
+__global__ __launch_bounds__(kThreads) void k_cache_read(KvView kv, const int32_t *starts,
+                                                         float *k, float *v) {
+  constexpr int PER = HD / 8;
+  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  const int e = (int)(i % PER) * 8;
+  const int64_t r = i / PER;  // (sequence, row, kv head)
+  const int g = (int)(r % kv.kvh);
+  const int64_t row = r / kv.kvh;
+  if (row >= (int64_t)kv.sequences * kv.rows) return;
+  const int b = (int)(row / kv.rows), t = (int)(row - (int64_t)b * kv.rows);
+  KvSeq s;
+  s.k0 = kv.base + b * kv.seq_bytes;
+  s.max_pos = kv.max_pos;
+  s.len = starts ? starts[b] : 0;
+  s.count = kv.counts ? min(max(kv.counts[b], 0), kv.rows) : kv.rows;
+  if (t >= s.count) return;
+  const bool bad = s.len < 0 || s.len > s.max_pos - s.count;
+#pragma unroll
+  for (int part = 0; part < 2; part++) {
+    float *dst = part ? v : k;
+    if (!dst) continue;
+    float o[8];
+    if (bad) {
+      for (int x = 0; x < 8; x++) o[x] = NAN;
+    } else {
+      const int64_t at = kv_row(kv, s, part, g, s.len + t);
+      if constexpr (FMT == Q3H_KV_Q8) {
+        const int8_t *p = reinterpret_cast<const int8_t *>(s.k0) + at * HD + e;
+        const float d = kv_scales(kv, s, HD)[at];
+        for (int x = 0; x < 8; x++) o[x] = (float)p[x] * d;
+      } else {
+        using KV = std::conditional_t<FMT == Q3H_KV_F16, _Float16, float>;
+        const KV *p = reinterpret_cast<const KV *>(s.k0) + at * HD + e;
+        for (int x = 0; x < 8; x++) o[x] = (float)p[x];
+      }
+    }
+    float *y = dst + r * HD + e;
+    for (int x = 0; x < 8; x++) y[x] = o[x];
+  }
+}
+
+// One workgroup per (sequence, layer, kv head, keys or values): the kept rows
+// in ascending order, each to a position at or before its own that no later
+// row comes from, so one row after another is enough; a 4-byte word of a row a
+// thread (HD = 64 int8: 16 words), the rest of the threads on the scale.
+template <int FMT, int HD>
+__global__ __launch_bounds__(128) void k_cache_keep(KvView kv, const int32_t *kept) {
+  constexpr int WORDS = HD * (FMT == Q3H_KV_F32 ? 4 : FMT == Q3H_KV_F16 ? 2 : 1) / 4;
+  const int b = blockIdx.x, tid = threadIdx.x;
+  const KvSeq s = kv_sequence(kv, b);
+  const int n = kv.counts[b];
+  if (n < 1 || n > kv.rows || s.len < 0) return;
+  const int32_t *list = kept + (size_t)b * kv.rows;
+  // the list's form: ascending, in [0, rows), the last position inside the cache
+  int last = -1;
+  for (int i = 0; i < n; i++) {
+    const int r = list[i];
+    if (r <= last || r >= kv.rows) return;
+    last = r;
+  }
+  if (s.len >= s.max_pos - last) return;
+  const int layer = blockIdx.y / (2 * kv.kvh), lg = blockIdx.y - layer * 2 * kv.kvh;
+  const int part = lg / kv.kvh, g = lg - part * kv.kvh;
+  KvView at = kv;
+  at.layer = layer;
+  const int64_t first = kv_row(at, s, part, g, s.len);
+  uint32_t *words = reinterpret_cast<uint32_t *>(s.k0) + first * WORDS;
+  float *scales = kv_scales(at, s, HD) + first;
+  for (int i = 0; i < n; i++) {
+    const int r = list[i];
+    if (r == i) continue;
+    if (tid < WORDS) words[(int64_t)i * WORDS + tid] = words[(int64_t)r * WORDS + tid];
+    if (FMT == Q3H_KV_Q8 && tid == WORDS) scales[i] = scales[r];
+  }
+}
+
+template <template <int, int> class F, class... A>
+void by_format(int hd, int fmt, A &&...args) {
+  if (hd == 64) {
+    if (fmt == Q3H_KV_F32) F<Q3H_KV_F32, 64>::go(args...);
+    else if (fmt == Q3H_KV_F16) F<Q3H_KV_F16, 64>::go(args...);
+    else F<Q3H_KV_Q8, 64>::go(args...);
+  } else {
+    if (fmt == Q3H_KV_F32) F<Q3H_KV_F32, 128>::go(args...);
+    else if (fmt == Q3H_KV_F16) F<Q3H_KV_F16, 128>::go(args...);
+    else F<Q3H_KV_Q8, 128>::go(args...);
+  }
+}
+
+template <int FMT, int HD>
+struct GoAppend {
+  static void go(const AppendRows &a, hipStream_t st) {
+    const int per = (kThreads / 64) * (128 / HD), all = a.heads + 2 * a.kv.kvh;
+    const dim3 grid(a.kv.sequences * a.kv.rows, (all + per - 1) / per);
+    hipLaunchKernelGGL((k_cache_append<FMT, HD>), grid, dim3(kThreads), 0, st, a);
+  }
+};
+template <int FMT, int HD>
+struct GoRead {
+  static void go(const KvView &kv, const int32_t *starts, float *k, float *v, hipStream_t st) {
+    const int64_t n = (int64_t)kv.sequences * kv.rows * kv.kvh * (HD / 8);
+    hipLaunchKernelGGL((k_cache_read<FMT, HD>), dim3((unsigned)((n + kThreads - 1) / kThreads)),
+                       dim3(kThreads), 0, st, kv, starts, k, v);
+  }
+};
+template <int FMT, int HD>
+struct GoKeep {
+  static void go(const KvView &kv, const int32_t *kept, hipStream_t st) {
+    hipLaunchKernelGGL((k_cache_keep<FMT, HD>), dim3(kv.sequences, kv.layers * 2 * kv.kvh),
+                       dim3(128), 0, st, kv, kept);
+  }
+};
+
+// the pairs' angles per position, and the factor on cosine and sine
+std::vector<double> rope_frequencies(const q3h_rope_config &c, double &mag) {
+  const double pi = 3.14159265358979323846;
+  const int pairs = c.rot_dim / 2;
+  const double theta = c.theta, factor = c.factor, span = c.original_positions;
+  std::vector<double> f(pairs);
+  mag = 1.0;
+  if (c.scaling == Q3H_ROPE_YARN && factor > 1.0) mag = 0.1 * std::log(factor) + 1.0;
+  if (c.magnitude != 0.f) mag = c.magnitude;
+  // the pair that turns `turns` times over the span
+  auto pair_of = [&](double turns) {
+    return c.rot_dim * std::log(span / (turns * 2.0 * pi)) / (2.0 * std::log(theta));
+  };
+  for (int i = 0; i < pairs; i++) {
+    const double g = std::pow(theta, -2.0 * i / c.rot_dim);
+    double own = 1.0;  // share of the unscaled frequency
+    if (c.scaling == Q3H_ROPE_LINEAR) {
+      own = 0.0;
+    } else if (c.scaling == Q3H_ROPE_YARN) {
+      const double lo = std::max(0.0, std::floor(pair_of(c.beta_fast)));
+      const double hi = std::min(c.rot_dim - 1.0, std::ceil(pair_of(c.beta_slow)));
+      own = 1.0 - std::min(1.0, std::max(0.0, (i - lo) / std::max(hi - lo, 0.001)));
+    } else if (c.scaling == Q3H_ROPE_BANDS) {
+      const double turns = span * g / (2.0 * pi);
+      own = std::min(1.0, std::max(0.0, (turns - c.low_turns) / ((double)c.high_turns -
+                                                                 (double)c.low_turns)));
+    }
+    f[i] = c.scaling == Q3H_ROPE_PLAIN ? g : g * own + g / factor * (1.0 - own);
+  }
+  return f;
+}
+
+// rows of pointers and row distances that every drafted-row call has
+void check_rows(const q3h_cache *c, int layer, int sequences, int rows, const char *who) {
+  const std::string w(who);
+  require(layer >= 0 && layer < c->cfg.layers, Q3H_E_ARG, w + ": no layer " + std::to_string(layer));
+  require(sequences >= 0 && sequences <= c->cfg.sequences, Q3H_E_ARG,
+          w + ": " + std::to_string(sequences) + " sequences of a cache of " +
+              std::to_string(c->cfg.sequences));
+  require(rows >= 0, Q3H_E_ARG, w + ": negative rows");
+  require(rows <= c->cfg.max_positions, Q3H_E_CAPACITY,
+          w + ": " + std::to_string(rows) + " rows in a cache of " +
+              std::to_string(c->cfg.max_positions) + " positions");
+}
+
+KvView view_of(const q3h_cache *c, int layer, int sequences, int rows, const int32_t *lens,
+               const int32_t *counts) {
+  KvView v{};
+  v.base = c->data;
+  v.seq_bytes = (int64_t)c->seq_bytes;
+  v.lens = lens;
+  v.counts = counts;
+  v.layers = c->cfg.layers;
+  v.kvh = c->cfg.kv_heads;
+  v.max_pos = c->cfg.max_positions;
+  v.layer = layer;
+  v.sequences = sequences;
+  v.rows = rows;
+  return v;
+}
+
+}  // namespace
+
+DeviceScope::DeviceScope(int ordinal) {
+  int now = -1;
+  check_hip(hipGetDevice(&now), "hipGetDevice");
+  if (now == ordinal) return;
+  check_hip(hipSetDevice(ordinal), "hipSetDevice");
+  before_ = now;
+}
+
+DeviceScope::~DeviceScope() {
+  if (before_ >= 0) (void)hipSetDevice(before_);
+}
+
+void launch_cache_append(const AppendRows &a, int hd, int fmt, hipStream_t st) {
+  by_format<GoAppend>(hd, fmt, a, st);
+}
+
+}  // namespace q3h
+
+using namespace q3h;
+
+// ---------------------------------------------------------------------------
+// rotary tables
+
+extern "C" int q3h_rope_create(q3h_device *dev, const q3h_rope_config *cfg, q3h_rope **out) {
+  q3h_rope *r = nullptr;
+  double *freq = nullptr;
+  int rc = guard([&] {
+    require(dev && cfg && out, Q3H_E_ARG, "q3h_rope_create: NULL argument");
+    *out = nullptr;
+    const q3h_rope_config &c = *cfg;
+    require(c.head_dim == 64 || c.head_dim == 128, Q3H_E_ARG,
+            "q3h_rope_create: head_dim must be 64 or 128");
+    require(c.rot_dim >= 2 && c.rot_dim <= c.head_dim && c.rot_dim % 2 == 0, Q3H_E_ARG,
+            "q3h_rope_create: rot_dim must be even and in [2, head_dim]");
+    require(c.interleaved == 0 || c.interleaved == 1, Q3H_E_ARG,
+            "q3h_rope_create: interleaved must be 0 or 1");
+    require(c.max_positions > 0 && c.max_positions <= (1 << 24), Q3H_E_ARG,
+            "q3h_rope_create: max_positions must be in [1, 2^24]");
+    require(c.theta > 1.f && std::isfinite(c.theta), Q3H_E_ARG,
+            "q3h_rope_create: theta must be above 1");
+    require(c.scaling >= Q3H_ROPE_PLAIN && c.scaling <= Q3H_ROPE_BANDS, Q3H_E_ARG,
+            "q3h_rope_create: no scaling " + std::to_string(c.scaling));
+    require(c.scaling == Q3H_ROPE_PLAIN || (c.factor > 0.f && std::isfinite(c.factor)), Q3H_E_ARG,
+            "q3h_rope_create: factor must be above 0");
+    require(c.scaling < Q3H_ROPE_YARN || c.original_positions > 0, Q3H_E_ARG,
+            "q3h_rope_create: original_positions must be above 0");
+    require(c.scaling != Q3H_ROPE_YARN ||
+                (c.beta_fast > c.beta_slow && c.beta_slow > 0.f && std::isfinite(c.beta_fast)),
+            Q3H_E_ARG, "q3h_rope_create: beta_fast > beta_slow > 0 is needed");
+    require(c.scaling != Q3H_ROPE_BANDS ||
+                (c.high_turns > c.low_turns && c.low_turns > 0.f && std::isfinite(c.high_turns)),
+            Q3H_E_ARG, "q3h_rope_create: high_turns > low_turns > 0 is needed");
+    require(std::isfinite(c.magnitude) && c.magnitude >= 0.f, Q3H_E_ARG,
+            "q3h_rope_create: magnitude must not be negative");
+    DeviceScope scope(dev->ordinal);
+    r = new q3h_rope();
+    r->dev = dev;
+    r->cfg = c;
+    double mag = 1.0;
+    const std::vector<double> f = rope_frequencies(c, mag);
+    const size_t n = (size_t)c.max_positions * f.size();
+    freq = (double *)dev_alloc(sizeof(double) * f.size());
+    check_hip(hipMemcpy(freq, f.data(), sizeof(double) * f.size(), hipMemcpyHostToDevice),
+              "upload frequencies");
+    r->table = (double2 *)dev_alloc(sizeof(double2) * n);
+    hipLaunchKernelGGL(k_rope_table, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, nullptr,
+                       freq, mag, (int)f.size(), n, r->table);
+    check_hip(hipGetLastError(), "rope table kernel");
+    check_hip(hipStreamSynchronize(nullptr), "rope table sync");
+    r->bytes = (int64_t)(sizeof(double2) * n);
+    dev->bytes += r->bytes;
+    dev->stacks++;
+    *out = r;
+  });
+  dev_free(freq);
+  if (rc != 0 && r) {
+    dev_free(r->table);
+    delete r;
+  }
+  return rc;
+}
+
+extern "C" int q3h_rope_destroy(q3h_rope *r) {
+  return guard([&] {
+    require(r != nullptr, Q3H_E_ARG, "q3h_rope_destroy: NULL table");
+    DeviceScope scope(r->dev->ordinal);
+    dev_free(r->table);
+    r->dev->bytes -= r->bytes;
+    r->dev->stacks--;
+    delete r;
+  });
+}
+
+// ---------------------------------------------------------------------------
+// caches
+
+extern "C" int q3h_cache_create(q3h_device *dev, const q3h_cache_config *cfg, q3h_cache **out) {
+  q3h_cache *c = nullptr;
+  int rc = guard([&] {
+    require(dev && cfg && out, Q3H_E_ARG, "q3h_cache_create: NULL argument");
+    *out = nullptr;
+    require(cfg->sequences > 0 && cfg->layers > 0 && cfg->kv_heads > 0 && cfg->max_positions > 0,
+            Q3H_E_ARG, "q3h_cache_create: non-positive dimension");
+    require(cfg->sequences <= 65535 && cfg->kv_heads <= 1024 && cfg->layers <= 1024 &&
+                cfg->max_positions <= (1 << 24) && (int64_t)cfg->layers * cfg->kv_heads <= 32767,
+            Q3H_E_ARG, "q3h_cache_create: too many sequences, layers, heads or positions");
+    require(cfg->head_dim == 64 || cfg->head_dim == 128, Q3H_E_ARG,
+            "q3h_cache_create: head_dim must be 64 or 128");
+    require(cfg->format >= Q3H_KV_F32 && cfg->format <= Q3H_KV_Q8, Q3H_E_ARG,
+            "q3h_cache_create: format must be Q3H_KV_F32, Q3H_KV_F16 or Q3H_KV_Q8");
+    DeviceScope scope(dev->ordinal);
+    c = new q3h_cache();
+    c->dev = dev;
+    c->cfg = *cfg;
+    const size_t need = kv_bytes(cfg->format, cfg->layers, cfg->kv_heads, cfg->max_positions,
+                                 cfg->head_dim);
+    c->seq_bytes = (need + 255) & ~(size_t)255;
+    const size_t all = c->seq_bytes * cfg->sequences;
+    c->data = (char *)dev_alloc(all);
+    check_hip(hipMemset(c->data, 0, all), "zero cache");
+    check_hip(hipStreamSynchronize(nullptr), "zero cache sync");
+    c->bytes = (int64_t)all;
+    dev->bytes += c->bytes;
+    dev->stacks++;
+    *out = c;
+  });
+  if (rc != 0 && c) {
+    dev_free(c->data);
+    delete c;
+  }
+  return rc;
+}
+
+extern "C" int64_t q3h_cache_bytes(const q3h_cache *c) { return c ? c->bytes : 0; }
+
+extern "C" int q3h_cache_destroy(q3h_cache *c) {
+  return guard([&] {
+    require(c != nullptr, Q3H_E_ARG, "q3h_cache_destroy: NULL cache");
+    DeviceScope scope(c->dev->ordinal);
+    dev_free(c->data);
+    c->dev->bytes -= c->bytes;
+    c->dev->stacks--;
+    delete c;
+  });
+}
+
+extern "C" int q3h_cache_append(q3h_cache *c, const q3h_append_args *p, void *stream) {
+  return guard([&] {
+    require(c && p, Q3H_E_ARG, "q3h_cache_append: NULL argument");
+    const q3h_cache_config &cf = c->cfg;
+    check_rows(c, p->layer, p->sequences, p->rows, "q3h_cache_append");
+    require(p->heads >= 0 && p->heads <= 4096, Q3H_E_ARG, "q3h_cache_append: bad heads");
+    if (p->sequences == 0 || p->rows == 0) return;
+    require(p->k && p->v && p->lens, Q3H_E_ARG, "q3h_cache_append: NULL k, v or lens");
+    require(p->heads == 0 || (p->q && p->q_out), Q3H_E_ARG, "q3h_cache_append: NULL q or q_out");
+    const int64_t wq = (int64_t)p->heads * cf.head_dim, wk = (int64_t)cf.kv_heads * cf.head_dim;
+    require(p->ldk >= wk && p->ldv >= wk && (p->heads == 0 || (p->ldq >= wq && p->ld_out >= wq)),
+            Q3H_E_ARG, "q3h_cache_append: rows overlap (a row distance below the row's width)");
+    require(p->heads == 0 || p->q_out != p->q || p->ldq == p->ld_out, Q3H_E_ARG,
+            "q3h_cache_append: in place with another row distance");
+    require((p->q_norm == nullptr && p->k_norm == nullptr) || p->eps >= 0.f, Q3H_E_ARG,
+            "q3h_cache_append: eps must not be negative");
+    require(!p->parents || p->rows <= Q3H_TREE_MAX_ROWS, Q3H_E_CAPACITY,
+            "q3h_cache_append: a tree has at most " + std::to_string(Q3H_TREE_MAX_ROWS) + " rows");
+    require((int64_t)p->sequences * p->rows <= INT32_MAX, Q3H_E_CAPACITY,
+            "q3h_cache_append: too many rows");
+    if (p->rope) {
+      require(p->rope->dev->ordinal == c->dev->ordinal, Q3H_E_ARG,
+              "q3h_cache_append: rope of another device");
+      require(p->rope->cfg.head_dim == cf.head_dim, Q3H_E_ARG,
+              "q3h_cache_append: rope of another head_dim");
+      require(p->rope->cfg.max_positions >= cf.max_positions, Q3H_E_ARG,
+              "q3h_cache_append: the rope table has fewer positions than the cache");
+    }
+    DeviceScope scope(c->dev->ordinal);
+    AppendRows a{};
+    a.kv = view_of(c, p->layer, p->sequences, p->rows, p->lens, p->counts);
+    a.heads = p->heads;
+    a.q = p->q;
+    a.k = p->k;
+    a.v = p->v;
+    a.ldq = p->ldq;
+    a.ldk = p->ldk;
+    a.ldv = p->ldv;
+    a.q_out = p->q_out;
+    a.ld_out = p->ld_out;
+    a.q_norm = p->q_norm;
+    a.k_norm = p->k_norm;
+    a.eps = p->eps;
+    if (p->rope) {
+      a.table = p->rope->table;
+      a.rot_dim = p->rope->cfg.rot_dim;
+      a.interleaved = p->rope->cfg.interleaved;
+    }
+    a.parents = p->parents;
+    launch_cache_append(a, cf.head_dim, cf.format, (hipStream_t)stream);
+    check_hip(hipGetLastError(), "cache append kernel");
+  });
+}
+
+extern "C" int q3h_cache_read(q3h_cache *c, int layer, int sequences, int rows,
+                              const int32_t *starts, const int32_t *counts, float *k, float *v,
+                              void *stream) {
+  return guard([&] {
+    require(c != nullptr, Q3H_E_ARG, "q3h_cache_read: NULL cache");
+    check_rows(c, layer, sequences, rows, "q3h_cache_read");
+    if (sequences == 0 || rows == 0 || (!k && !v)) return;
+    require((int64_t)sequences * rows <= INT32_MAX / 16 / c->cfg.kv_heads * 16, Q3H_E_CAPACITY,
+            "q3h_cache_read: too many rows");
+    DeviceScope scope(c->dev->ordinal);
+    by_format<GoRead>(c->cfg.head_dim, c->cfg.format,
+                      view_of(c, layer, sequences, rows, nullptr, counts), starts, k, v,
+                      (hipStream_t)stream);
+    check_hip(hipGetLastError(), "cache read kernel");
+  });
+}
+
+extern "C" int q3h_cache_keep(q3h_cache *c, int sequences, int rows, const int32_t *lens,
+                              const int32_t *kept, const int32_t *kept_counts, void *stream) {
+  return guard([&] {
+    require(c != nullptr, Q3H_E_ARG, "q3h_cache_keep: NULL cache");
+    check_rows(c, 0, sequences, rows, "q3h_cache_keep");
+    if (sequences == 0 || rows == 0) return;
+    require(lens && kept && kept_counts, Q3H_E_ARG, "q3h_cache_keep: NULL argument");
+    DeviceScope scope(c->dev->ordinal);
+    by_format<GoKeep>(c->cfg.head_dim, c->cfg.format,
+                      view_of(c, 0, sequences, rows, lens, kept_counts), kept,
+                      (hipStream_t)stream);
+    check_hip(hipGetLastError(), "cache keep kernel");
+  });
+}
+
+extern "C" int64_t q3h_cache_attend_workspace(const q3h_cache *c, int sequences, int rows,
+                                              int heads, int max_len) {
+  int64_t bytes = 0;
+  const int rc = guard([&] {
+    require(c != nullptr, Q3H_E_ARG, "q3h_cache_attend_workspace: NULL cache");
+    check_rows(c, 0, sequences, rows, "q3h_cache_attend_workspace");
+    require(heads > 0 && heads <= 4096 && heads % c->cfg.kv_heads == 0, Q3H_E_ARG,
+            "q3h_cache_attend_workspace: heads must be a multiple of the cache's");
+    require(max_len >= 0 && max_len <= c->cfg.max_positions, Q3H_E_ARG,
+            "q3h_cache_attend_workspace: max_len beyond the cache");
+    if (sequences > 0 && rows > 0)
+      bytes = (int64_t)attend_part_bytes(sequences, rows, heads, c->cfg.kv_heads,
+                                         c->cfg.head_dim, max_len);
+  });
+  return rc ? rc : bytes;
+}
+
+extern "C" int q3h_cache_attend(q3h_cache *c, const q3h_attend_args *p, void *stream) {
+  return guard([&] {
+    require(c && p, Q3H_E_ARG, "q3h_cache_attend: NULL argument");
+    const q3h_cache_config &cf = c->cfg;
+    check_rows(c, p->layer, p->sequences, p->rows, "q3h_cache_attend");
+    require(p->heads > 0 && p->heads <= 4096 && p->heads % cf.kv_heads == 0, Q3H_E_ARG,
+            "q3h_cache_attend: heads must be a multiple of the cache's");
+    require(p->max_len >= 0 && p->max_len <= cf.max_positions, Q3H_E_ARG,
+            "q3h_cache_attend: max_len beyond the cache");
+    if (p->sequences == 0 || p->rows == 0) return;
+    require(p->q && p->out && p->lens, Q3H_E_ARG, "q3h_cache_attend: NULL q, out or lens");
+    const int64_t w = (int64_t)p->heads * cf.head_dim;
+    require(p->ldq >= w && p->ld_out >= w, Q3H_E_ARG,
+            "q3h_cache_attend: rows overlap (a row distance below the row's width)");
+    require(p->out != p->q || p->ldq == p->ld_out, Q3H_E_ARG,
+            "q3h_cache_attend: in place with another row distance");
+    require(!p->parents || p->rows <= Q3H_TREE_MAX_ROWS, Q3H_E_CAPACITY,
+            "q3h_cache_attend: a tree has at most " + std::to_string(Q3H_TREE_MAX_ROWS) + " rows");
+    require((int64_t)p->sequences * p->rows <= INT32_MAX, Q3H_E_CAPACITY,
+            "q3h_cache_attend: too many rows");
+    require(std::isfinite(p->scale), Q3H_E_ARG, "q3h_cache_attend: scale is not finite");
+    const size_t need = attend_part_bytes(p->sequences, p->rows, p->heads, cf.kv_heads,
+                                          cf.head_dim, p->max_len);
+    require(need == 0 || (p->workspace && p->workspace_bytes >= (int64_t)need &&
+                          (uintptr_t)p->workspace % 256 == 0),
+            Q3H_E_ARG, "q3h_cache_attend: a workspace of " + std::to_string(need) +
+                           " bytes, 256-byte aligned, is needed");
+    DeviceScope scope(c->dev->ordinal);
+    AttendRows a{};
+    a.kv = view_of(c, p->layer, p->sequences, p->rows, p->lens, p->counts);
+    a.heads = p->heads;
+    a.max_len = p->max_len;
+    a.scale = p->scale != 0.f ? p->scale : 1.0f / std::sqrt((float)cf.head_dim);
+    a.q = p->q;
+    a.ldq = p->ldq;
+    a.out = p->out;
+    a.ld_out = p->ld_out;
+    a.parents = p->parents;
+    a.part = (float *)p->workspace;
+    launch_cache_attend(a, cf.head_dim, cf.format, (hipStream_t)stream);
+    check_hip(hipGetLastError(), "cache attention kernels");
+  });
+}

@@ -25,6 +25,17 @@ const
   Q3H_Q8_0 = 1;
   Q3H_BF16 = 2;
 
+  // formats of a K/V cache, rotary scalings, limits of the drafted rows
+  Q3H_KV_F32 = 0;
+  Q3H_KV_F16 = 1;
+  Q3H_KV_Q8 = 2;
+  Q3H_ROPE_PLAIN = 0;
+  Q3H_ROPE_LINEAR = 1;
+  Q3H_ROPE_YARN = 2;
+  Q3H_ROPE_BANDS = 3;
+  Q3H_TREE_MAX_ROWS = 64;
+  Q3H_TOP_MAX = 64;
+
   Q3H_OK = 0;
   Q3H_E_ARG = -1;
   Q3H_E_HIP = -2;
@@ -45,6 +56,8 @@ type
   q3h_frame = pointer;
   q3h_text_proj = pointer;
   q3h_codec = pointer;
+  q3h_rope = pointer;
+  q3h_cache = pointer;
   Pq3h_context = ^q3h_context;
 
   /// TDecoderConfig + KvF16 + the numerics of the Q8_0 products
@@ -121,6 +134,62 @@ type
     out_alpha, out_beta, out_w, out_b: PSingle;
   end;
   Pq3h_codec_weights = ^q3h_codec_weights;
+
+  /// the operators around drafted rows: pointers to device memory of the
+  // caller, enqueued on a stream of the caller (nil: the default stream)
+  q3h_rope_config = record
+    head_dim, rot_dim, interleaved, max_positions: integer;
+    theta: single;
+    scaling: integer;            // Q3H_ROPE_*
+    factor: single;
+    original_positions: integer;
+    beta_fast, beta_slow, low_turns, high_turns, magnitude: single;
+  end;
+  Pq3h_rope_config = ^q3h_rope_config;
+
+  q3h_cache_config = record
+    sequences, layers, kv_heads, head_dim, max_positions, format: integer;
+  end;
+  Pq3h_cache_config = ^q3h_cache_config;
+
+  q3h_append_args = record
+    layer, sequences, rows, heads: integer;
+    q, k, v: PSingle;
+    ldq, ldk, ldv: Int64;
+    q_out: PSingle;
+    ld_out: Int64;
+    q_norm, k_norm: PSingle;
+    eps: single;
+    rope: pointer; // q3h_rope, nil: not turned
+    lens, counts, parents: PInteger;
+  end;
+  Pq3h_append_args = ^q3h_append_args;
+
+  q3h_attend_args = record
+    layer, sequences, rows, heads, max_len: integer;
+    scale: single;
+    q: PSingle;
+    ldq: Int64;
+    out: PSingle;
+    ld_out: Int64;
+    lens, counts, parents: PInteger;
+    workspace: pointer;
+    workspace_bytes: Int64;
+  end;
+  Pq3h_attend_args = ^q3h_attend_args;
+
+  q3h_score_args = record
+    logits: pointer;
+    ld: Int64;
+    dtype, rows, vocab, tokens_per_row, top_k: integer;
+    tokens: PInteger;
+    logprobs, entropy: PSingle;
+    top_ids: PInteger;
+    top_logprobs: PSingle;
+    workspace: pointer;
+    workspace_bytes: Int64;
+  end;
+  Pq3h_score_args = ^q3h_score_args;
 
 { device: TQwenVulkan (lm.pas:44-62, 202-222) }
 function q3h_device_available: integer; cdecl; external LIBQ3H;
@@ -208,6 +277,31 @@ function q3h_codec_back(c: q3h_codec; x: PSingle; frames: integer;
   pcm: PSingle): integer; cdecl; external LIBQ3H;
 function q3h_codec_bytes(c: q3h_codec): Int64; cdecl; external LIBQ3H;
 function q3h_codec_destroy(c: q3h_codec): integer; cdecl; external LIBQ3H;
+
+{ drafted rows: caches, rotary forms, attention over a tree, token scores }
+function q3h_rope_create(dev: q3h_device; cfg: Pq3h_rope_config;
+  out rope: q3h_rope): integer; cdecl; external LIBQ3H;
+function q3h_rope_destroy(r: q3h_rope): integer; cdecl; external LIBQ3H;
+function q3h_cache_create(dev: q3h_device; cfg: Pq3h_cache_config;
+  out cache: q3h_cache): integer; cdecl; external LIBQ3H;
+function q3h_cache_bytes(c: q3h_cache): Int64; cdecl; external LIBQ3H;
+function q3h_cache_destroy(c: q3h_cache): integer; cdecl; external LIBQ3H;
+function q3h_cache_append(c: q3h_cache; a: Pq3h_append_args;
+  stream: pointer): integer; cdecl; external LIBQ3H;
+function q3h_cache_read(c: q3h_cache; layer, sequences, rows: integer;
+  starts, counts: PInteger; k, v: PSingle; stream: pointer): integer;
+  cdecl; external LIBQ3H;
+function q3h_cache_attend_workspace(c: q3h_cache; sequences, rows, heads,
+  max_len: integer): Int64; cdecl; external LIBQ3H;
+function q3h_cache_attend(c: q3h_cache; a: Pq3h_attend_args;
+  stream: pointer): integer; cdecl; external LIBQ3H;
+function q3h_cache_keep(c: q3h_cache; sequences, rows: integer;
+  lens, kept, kept_counts: PInteger; stream: pointer): integer;
+  cdecl; external LIBQ3H;
+function q3h_token_logprobs_workspace(rows, vocab, top_k: integer): Int64;
+  cdecl; external LIBQ3H;
+function q3h_token_logprobs(dev: q3h_device; a: Pq3h_score_args;
+  stream: pointer): integer; cdecl; external LIBQ3H;
 
 { helpers }
 function q3h_quantize_row_q8_0(x: PSingle; y: pointer; k: Int64): integer;

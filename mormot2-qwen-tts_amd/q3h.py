@@ -22,6 +22,13 @@ F32 = 0
 Q8_0 = 1
 BF16 = 2
 
+# formats of a K/V cache (Q3H_KV_*)
+KV_F32, KV_F16, KV_Q8 = 0, 1, 2
+# rotary scalings (Q3H_ROPE_*)
+ROPE_SCALING = {"plain": 0, "linear": 1, "yarn": 2, "bands": 3}
+TREE_MAX_ROWS = 64  # Q3H_TREE_MAX_ROWS
+TOP_MAX = 64  # Q3H_TOP_MAX
+
 E_ARG, E_HIP, E_CAPACITY, E_STATE, E_NODEV = -1, -2, -3, -4, -5
 NOALLOC_MAX_ROWS = 64  # Q3H_NOALLOC_MAX_ROWS
 NOALLOC_SCRATCH_BYTES = 16 << 20  # Q3H_NOALLOC_SCRATCH_BYTES
@@ -123,6 +130,47 @@ class StartIds(ctypes.Structure):
                 ("tts_bos", "tts_eos", "tts_pad", "codec_pad", "codec_bos")]
 
 
+class RopeConfig(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in
+                ("head_dim", "rot_dim", "interleaved", "max_positions")] + [
+        ("theta", ctypes.c_float), ("scaling", ctypes.c_int32), ("factor", ctypes.c_float),
+        ("original_positions", ctypes.c_int32), ("beta_fast", ctypes.c_float),
+        ("beta_slow", ctypes.c_float), ("low_turns", ctypes.c_float),
+        ("high_turns", ctypes.c_float), ("magnitude", ctypes.c_float)]
+
+
+class CacheConfig(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in
+                ("sequences", "layers", "kv_heads", "head_dim", "max_positions", "format")]
+
+
+class AppendArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("layer", "sequences", "rows", "heads")] + \
+        [(n, ctypes.c_void_p) for n in ("q", "k", "v")] + \
+        [(n, ctypes.c_int64) for n in ("ldq", "ldk", "ldv")] + [
+        ("q_out", ctypes.c_void_p), ("ld_out", ctypes.c_int64), ("q_norm", ctypes.c_void_p),
+        ("k_norm", ctypes.c_void_p), ("eps", ctypes.c_float), ("rope", ctypes.c_void_p)] + \
+        [(n, ctypes.c_void_p) for n in ("lens", "counts", "parents")]
+
+
+class AttendArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in
+                ("layer", "sequences", "rows", "heads", "max_len")] + [
+        ("scale", ctypes.c_float), ("q", ctypes.c_void_p), ("ldq", ctypes.c_int64),
+        ("out", ctypes.c_void_p), ("ld_out", ctypes.c_int64)] + \
+        [(n, ctypes.c_void_p) for n in ("lens", "counts", "parents", "workspace")] + \
+        [("workspace_bytes", ctypes.c_int64)]
+
+
+class ScoreArgs(ctypes.Structure):
+    _fields_ = [("logits", ctypes.c_void_p), ("ld", ctypes.c_int64)] + \
+        [(n, ctypes.c_int32) for n in
+         ("dtype", "rows", "vocab", "tokens_per_row", "top_k")] + \
+        [(n, ctypes.c_void_p) for n in
+         ("tokens", "logprobs", "entropy", "top_ids", "top_logprobs", "workspace")] + \
+        [("workspace_bytes", ctypes.c_int64)]
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _FP = ctypes.POINTER(ctypes.c_float)
@@ -172,6 +220,18 @@ SIGNATURES = {
     "q3h_codec_bytes": (ctypes.c_int64, [_P]),
     "q3h_codec_destroy": (_I, [_P]),
     "q3h_frame_start_text": (_I, [_P, _I, _P, ctypes.POINTER(StartIds), _IP, _I, _IP, _I, _I]),
+    "q3h_rope_create": (_I, [_P, ctypes.POINTER(RopeConfig), ctypes.POINTER(_P)]),
+    "q3h_rope_destroy": (_I, [_P]),
+    "q3h_cache_create": (_I, [_P, ctypes.POINTER(CacheConfig), ctypes.POINTER(_P)]),
+    "q3h_cache_bytes": (ctypes.c_int64, [_P]),
+    "q3h_cache_destroy": (_I, [_P]),
+    "q3h_cache_append": (_I, [_P, ctypes.POINTER(AppendArgs), _P]),
+    "q3h_cache_read": (_I, [_P, _I, _I, _I, _P, _P, _P, _P, _P]),
+    "q3h_cache_attend_workspace": (ctypes.c_int64, [_P, _I, _I, _I, _I]),
+    "q3h_cache_attend": (_I, [_P, ctypes.POINTER(AttendArgs), _P]),
+    "q3h_cache_keep": (_I, [_P, _I, _I, _P, _P, _P, _P]),
+    "q3h_token_logprobs_workspace": (ctypes.c_int64, [_I, _I, _I]),
+    "q3h_token_logprobs": (_I, [_P, ctypes.POINTER(ScoreArgs), _P]),
     "q3h_quantize_row_q8_0": (_I, [_FP, _P, ctypes.c_int64]),
     "q3h_stack_time_gemv": (_I, [_P, _I, _I, _I, _FP, ctypes.POINTER(_I),
                                  ctypes.POINTER(ctypes.c_int64)]),
@@ -228,6 +288,7 @@ class Device:
         h = _P()
         _check(lib().q3h_device_open(ordinal, ctypes.byref(h)))
         self.h = h
+        self.ordinal = ordinal
 
     @property
     def name(self):
@@ -611,3 +672,254 @@ class Frame:
         if self.h:
             _check(lib().q3h_frame_destroy(self.h))
             self.h = None
+
+
+# ---------------------------------------------------------------------------
+# operators on device memory: torch tensors of the handle's device, in the order
+# of torch's current stream there (no copies, no waits; they can be captured)
+
+
+def _bad(msg):
+    raise Q3HError(E_ARG, msg)
+
+
+def _ptr(t, ordinal, dtype, name):
+    """The address of a tensor of this dtype ("float32", ...) on the device."""
+    d = t.device
+    if d.type != "cuda" or (d.index or 0) != ordinal:
+        _bad(f"{name} is on {d}, not on device {ordinal}")
+    if str(t.dtype) != "torch." + dtype:
+        _bad(f"{name} is {t.dtype}, not {dtype}")
+    return t.data_ptr()
+
+
+def _rows(t, n, rows, heads, hd, ordinal, name):
+    """(address, floats between rows) of f32 rows [n][rows][heads][hd], or
+    [n][rows][heads * hd], contiguous within a row."""
+    shape, stride = tuple(t.shape), t.stride()
+    if shape == (n, rows, heads, hd):
+        if stride[3] != 1 or (heads > 1 and stride[2] != hd):
+            _bad(f"{name}: the heads of a row are not side by side")
+    elif shape == (n, rows, heads * hd):
+        if stride[2] != 1:
+            _bad(f"{name}: the elements of a row are not side by side")
+    else:
+        _bad(f"{name} is {list(shape)}, not {[n, rows, heads, hd]}")
+    ld = stride[1] if rows > 1 else stride[0] if n > 1 else heads * hd
+    if rows > 1 and n > 1 and stride[0] != rows * ld:
+        _bad(f"{name}: the sequences' rows are not evenly spaced")
+    return _ptr(t, ordinal, "float32", name), ld
+
+
+def _whole(t, shape, ordinal, dtype, name):
+    """The address of a contiguous tensor of this shape and dtype; None for None."""
+    if t is None:
+        return None
+    if tuple(t.shape) != shape or not t.is_contiguous():
+        _bad(f"{name} is {list(t.shape)}, not contiguous {list(shape)}")
+    return _ptr(t, ordinal, dtype, name)
+
+
+def _stream(ordinal):
+    import torch
+    return torch.cuda.current_stream(ordinal).cuda_stream
+
+
+class Rope:
+    """A rotary table (q3h_rope_*): the first rot_dim elements of a head turned
+    in neighbouring pairs (interleaved) or in pairs half of them apart. scaling:
+    None, dict(kind="linear", factor=), dict(kind="yarn", factor=, original=,
+    beta_fast=32, beta_slow=1), dict(kind="bands", factor=, original=, low=1,
+    high=4); magnitude: on cosine and sine (0: the scaling's own)."""
+
+    h = None
+
+    def __init__(self, dev, head_dim, max_positions, theta, rot_dim=None, interleaved=False,
+                 scaling=None, magnitude=0.0):
+        s = dict(scaling or {"kind": "plain"})
+        kind = s.pop("kind")
+        if kind not in ROPE_SCALING:
+            _bad(f"no rotary scaling {kind!r}")
+        cfg = RopeConfig(head_dim, head_dim if rot_dim is None else rot_dim, int(interleaved),
+                         max_positions, theta, ROPE_SCALING[kind], s.pop("factor", 1.0),
+                         s.pop("original", 0), s.pop("beta_fast", 32.0), s.pop("beta_slow", 1.0),
+                         s.pop("low", 1.0), s.pop("high", 4.0), magnitude)
+        if s:
+            _bad(f"unknown rotary settings {sorted(s)}")
+        h = _P()
+        _check(lib().q3h_rope_create(dev.h, ctypes.byref(cfg), ctypes.byref(h)))
+        self.dev = dev
+        self.h = h
+
+    def destroy(self):
+        if self.h:
+            _check(lib().q3h_rope_destroy(self.h))
+            self.h = None
+
+    def __del__(self):
+        if self.h and self.dev.h:
+            lib().q3h_rope_destroy(self.h)
+
+
+class Cache:
+    """A K/V cache of several sequences (q3h_cache_*), in f32, f16 or one byte
+    per element with a scale per position and head (KV_F32, KV_F16, KV_Q8).
+    Calls take rows [sequences][rows][heads][head_dim] for the first sequences of
+    the cache; lens, counts [sequences] and parents [sequences][rows] are int32
+    tensors on the device."""
+
+    h = None
+
+    def __init__(self, dev, sequences, kv_heads, head_dim, max_positions, fmt=KV_F32, layers=1):
+        cfg = CacheConfig(sequences, layers, kv_heads, head_dim, max_positions, fmt)
+        h = _P()
+        _check(lib().q3h_cache_create(dev.h, ctypes.byref(cfg), ctypes.byref(h)))
+        self.dev = dev
+        self.h = h
+        self.kv_heads, self.head_dim = kv_heads, head_dim
+
+    @property
+    def bytes(self):
+        return lib().q3h_cache_bytes(self.h)
+
+    def append(self, k, v, lens, counts=None, parents=None, q=None, q_out=None, rope=None,
+               q_norm=None, k_norm=None, eps=1e-6, layer=0):
+        """Writes the drafted rows k, v at positions lens[b] + row, keys and
+        queries normed (q_norm, k_norm) and turned (rope) first. Returns the
+        queries (q_out, made when it is None; rows beyond counts as they were),
+        None without q. parents: the row each row continues (-1: the sequence
+        itself); None: a chain."""
+        o, hd = self.dev.ordinal, self.head_dim
+        n, rows = k.shape[0], k.shape[1]
+        a = AppendArgs()
+        a.layer, a.sequences, a.rows = layer, n, rows
+        a.k, a.ldk = _rows(k, n, rows, self.kv_heads, hd, o, "k")
+        a.v, a.ldv = _rows(v, n, rows, self.kv_heads, hd, o, "v")
+        if q is not None:
+            heads = q.shape[2] if q.dim() == 4 else q.shape[2] // hd
+            if q_out is None:
+                q_out = q.new_empty((n, rows, heads, hd))
+            a.heads = heads
+            a.q, a.ldq = _rows(q, n, rows, heads, hd, o, "q")
+            a.q_out, a.ld_out = _rows(q_out, n, rows, heads, hd, o, "q_out")
+            a.q_norm = _whole(q_norm, (hd,), o, "float32", "q_norm")
+        a.k_norm = _whole(k_norm, (hd,), o, "float32", "k_norm")
+        a.eps = eps
+        a.rope = rope.h if rope is not None else None
+        a.lens = _whole(lens, (n,), o, "int32", "lens")
+        a.counts = _whole(counts, (n,), o, "int32", "counts")
+        a.parents = _whole(parents, (n, rows), o, "int32", "parents")
+        _check(lib().q3h_cache_append(self.h, ctypes.byref(a), _stream(o)))
+        return q_out
+
+    def read(self, k, v, starts=None, counts=None, layer=0):
+        """Positions starts[b] .. + counts[b] - 1 of the first sequences into k
+        and v (either None) [sequences][rows][kv_heads][head_dim] as f32; rows
+        beyond counts stay as they were."""
+        o = self.dev.ordinal
+        like = k if k is not None else v
+        n, rows = like.shape[0], like.shape[1]
+        shape = (n, rows, self.kv_heads, self.head_dim)
+        _check(lib().q3h_cache_read(
+            self.h, layer, n, rows, _whole(starts, (n,), o, "int32", "starts"),
+            _whole(counts, (n,), o, "int32", "counts"), _whole(k, shape, o, "float32", "k"),
+            _whole(v, shape, o, "float32", "v"), _stream(o)))
+
+    def attend(self, q, lens, max_len, out=None, counts=None, parents=None, scale=0.0, layer=0,
+               workspace=None):
+        """Attention of the drafted rows q over the cache, which holds their keys
+        and values already; max_len: no length in lens is above it. Returns out
+        (made when it is None; rows beyond counts as they were). scale 0: 1 /
+        sqrt(head_dim). workspace: a uint8 tensor of attend_workspace bytes (made
+        when it is None)."""
+        o, hd = self.dev.ordinal, self.head_dim
+        n, rows = q.shape[0], q.shape[1]
+        heads = q.shape[2] if q.dim() == 4 else q.shape[2] // hd
+        if out is None:
+            out = q.new_empty((n, rows, heads, hd))
+        a = AttendArgs()
+        a.layer, a.sequences, a.rows, a.heads, a.max_len = layer, n, rows, heads, max_len
+        a.scale = scale
+        a.q, a.ldq = _rows(q, n, rows, heads, hd, o, "q")
+        a.out, a.ld_out = _rows(out, n, rows, heads, hd, o, "out")
+        a.lens = _whole(lens, (n,), o, "int32", "lens")
+        a.counts = _whole(counts, (n,), o, "int32", "counts")
+        a.parents = _whole(parents, (n, rows), o, "int32", "parents")
+        need = self.attend_workspace(n, rows, heads, max_len)
+        if need:
+            workspace = _space(workspace, need, q, o)
+            a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
+        _check(lib().q3h_cache_attend(self.h, ctypes.byref(a), _stream(o)))
+        return out
+
+    def attend_workspace(self, sequences, rows, heads, max_len):
+        need = lib().q3h_cache_attend_workspace(self.h, sequences, rows, heads, max_len)
+        if need < 0:
+            _check(need)
+        return need
+
+    def keep(self, lens, kept, kept_counts):
+        """Moves the rows kept [sequences][rows] (ascending row numbers, the first
+        kept_counts of each sequence) to positions lens[b], lens[b] + 1, ... in
+        every layer. The caller's lengths then grow by kept_counts."""
+        o = self.dev.ordinal
+        n, rows = kept.shape
+        _check(lib().q3h_cache_keep(
+            self.h, n, rows, _whole(lens, (n,), o, "int32", "lens"),
+            _whole(kept, (n, rows), o, "int32", "kept"),
+            _whole(kept_counts, (n,), o, "int32", "kept_counts"), _stream(o)))
+
+    def destroy(self):
+        if self.h:
+            _check(lib().q3h_cache_destroy(self.h))
+            self.h = None
+
+    def __del__(self):
+        if self.h and self.dev.h:
+            lib().q3h_cache_destroy(self.h)
+
+
+def _space(workspace, need, like, ordinal):
+    """A uint8 tensor of at least need bytes on the device."""
+    if workspace is None:
+        import torch
+        return torch.empty(need, dtype=torch.uint8, device=like.device)
+    _ptr(workspace, ordinal, "uint8", "workspace")
+    if not workspace.is_contiguous():
+        _bad("workspace is not contiguous")
+    return workspace
+
+
+def token_logprobs(dev, logits, tokens, top_k=0, workspace=None):
+    """Scores of logits [rows][vocab] (f32 or bf16) at tokens [rows][m] (int32):
+    dict of logprobs [rows][m], entropy [rows] and, with top_k, top_ids and
+    top_logprobs [rows][top_k] (largest first, of equal ones the lowest token)."""
+    o = dev.ordinal
+    rows, vocab = logits.shape
+    bf16 = str(logits.dtype) == "torch.bfloat16"
+    if vocab > 1 and logits.stride(1) != 1:
+        _bad("logits: the elements of a row are not side by side")
+    a = ScoreArgs()
+    a.logits = _ptr(logits, o, "bfloat16" if bf16 else "float32", "logits")
+    a.ld = logits.stride(0) if rows > 1 else vocab
+    a.dtype, a.rows, a.vocab, a.top_k = BF16 if bf16 else F32, rows, vocab, top_k
+    m = tokens.shape[1]
+    a.tokens_per_row = m
+    a.tokens = _whole(tokens, (rows, m), o, "int32", "tokens")
+    like = dict(device=logits.device)
+    import torch
+    res = {"logprobs": torch.empty((rows, m), **like), "entropy": torch.empty(rows, **like)}
+    a.logprobs, a.entropy = res["logprobs"].data_ptr(), res["entropy"].data_ptr()
+    if top_k > 0:
+        res["top_ids"] = torch.empty((rows, top_k), dtype=torch.int32, **like)
+        res["top_logprobs"] = torch.empty((rows, top_k), **like)
+        a.top_ids = res["top_ids"].data_ptr()
+        a.top_logprobs = res["top_logprobs"].data_ptr()
+    need = lib().q3h_token_logprobs_workspace(rows, vocab, top_k)
+    if need < 0:
+        _check(need)
+    if need:
+        workspace = _space(workspace, need, logits, o)
+        a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
+    _check(lib().q3h_token_logprobs(dev.h, ctypes.byref(a), _stream(o)))
+    return res
