@@ -1,6 +1,27 @@
 // q3h_tree.hip - attention of drafted rows over a K/V cache: each row sees the
 // positions before the draft and its own path among the drafted rows.
+//
+// One pass over the cache with the running maximum and sum of a softmax, on
+// the matrix cores, without a trip through LDS. The query rows of a kv head
+// (drafted row x query head of the group) go in tiles of 16, the positions in
+// tiles of 32 (f32: 16):
+//   S^T = K Q^T: keys are the rows of the product, queries its columns, so a
+//     lane gets scores of one query (lane % 16) for 4 keys of each 16;
+//   O^T = V^T P^T: the same lane holds exactly those scores' weights as a
+//     column of P^T, where the order of positions along the product's inner
+//     dimension is free: V is read in the order the scores have. V^T's rows are
+//     the head's elements, dealt so that a lane reads HD / 16 neighbouring ones
+//     of a position (whole rows per load instruction) and is left with HD / 4
+//     neighbouring elements of its query's output.
+// Precision is that of f32 products in every format: f16 and int8 elements are
+// exact in f16, queries and weights go in as two f16 parts (22 bits; queries
+// scaled to 2^13 .. 2^14 by a power of two per row, weights to at most 2^14, so
+// that the second part stays normal), f32 caches use the f32 matrix
+// instructions. An int8 row's scale is a factor of the position: it multiplies
+// the score, and the weight that the values are summed with.
 #include <hip/hip_runtime.h>
+
+#include <algorithm>
 
 #include "q3h_draft.h"
 #include "q3h_wave.h"
@@ -9,106 +30,736 @@ namespace q3h {
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kWaves = 4, kThreads = 64 * kWaves;
 
-template <int FMT, int HD>
-__device__ __forceinline__ float kv_value(const KvView &kv, const KvSeq &s, int64_t at, int e) {
-  if constexpr (FMT == Q3H_KV_Q8)
-    return (float)reinterpret_cast<const int8_t *>(s.k0)[at * HD + e] * kv_scales(kv, s, HD)[at];
-  else if constexpr (FMT == Q3H_KV_F16)
-    return (float)reinterpret_cast<const _Float16 *>(s.k0)[at * HD + e];
-  else
-    return reinterpret_cast<const float *>(s.k0)[at * HD + e];
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef float f2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u4e __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+
+template <typename T>
+__device__ __forceinline__ T load(const char *p, int64_t off) {
+  return *reinterpret_cast<const __attribute__((address_space(1))) T *>(
+      reinterpret_cast<uintptr_t>(p) + off);
 }
 
-// One workgroup per (query head, row, sequence): a position a thread for the
-// scores, an element a thread for the values, with the softmax's running
-// maximum and sum over blocks of 256 positions.
-template <int FMT, int HD>
-__global__ __launch_bounds__(kThreads) void k_attend(AttendRows a) {
-  __shared__ float q[HD], p[kThreads], red[kThreads / 64], o[kThreads];
-  const int h = blockIdx.y, t = blockIdx.x, b = blockIdx.z, tid = threadIdx.x;
-  const KvSeq s = kv_sequence(a.kv, b);
-  if (t >= s.count) return;
-  const size_t row = (size_t)b * a.kv.rows + t;
-  const int g = h / (a.heads / a.kv.kvh);
-  uint64_t path = 0;
-  bool bad = s.len < 0 || s.len > a.max_len || s.len > s.max_pos - s.count;
-  if (a.parents) {
-    const Path x = tree_path(a.parents + (size_t)b * a.kv.rows, a.kv.rows);
-    path = __shfl(x.rows, t);
-    bad = bad || __shfl((int)x.bad, t) != 0;
-  }
-  float *out = a.out + row * a.ld_out + (size_t)h * HD;
-  if (bad) {
-    if (tid < HD) out[tid] = NAN;
-    return;
-  }
-  if (tid < HD) q[tid] = a.q[row * a.ldq + (size_t)h * HD + tid] * a.scale;
-  __syncthreads();
-  const int end = s.len + t + 1;  // (a path's rows are below its own)
-  constexpr int PARTS = kThreads / HD;
-  const int e = tid % HD, half = tid / HD;
-  float m = -INFINITY, l = 0.f, acc = 0.f;
-  for (int j0 = 0; j0 < end; j0 += kThreads) {
-    const int j = j0 + tid;
-    const bool sees = j < end && (j < s.len || !a.parents || (path >> (j - s.len) & 1));
-    float x = -INFINITY;
-    if (sees) {
-      const int64_t at = kv_row(a.kv, s, 0, g, j);
-      x = 0.f;
-      for (int i = 0; i < HD; i++) x = fmaf(q[i], kv_value<FMT, HD>(a.kv, s, at, i), x);
-    }
-    const float wm = wave_max_dpp(x);
-    __syncthreads();
-    if ((tid & 63) == 0) red[tid >> 6] = wm;
-    __syncthreads();
-    float mn = m;
-    for (int i = 0; i < kThreads / 64; i++) mn = fmaxf(mn, red[i]);
-    const float base = mn == -INFINITY ? 0.f : mn;
-    const float f = expf(m - base);
-    const float w = sees ? expf(x - base) : 0.f;
-    p[tid] = sees ? w : -1.f;  // (negative: not seen)
-    const float ws = wave_sum_dpp(w);
-    __syncthreads();
-    if ((tid & 63) == 0) red[tid >> 6] = ws;
-    __syncthreads();
-    l *= f;
-    for (int i = 0; i < kThreads / 64; i++) l += red[i];
-    acc *= f;
-    m = mn;
-    for (int i = half; i < kThreads && j0 + i < end; i += PARTS)
-      if (!(p[i] < 0.f))
-        acc = fmaf(p[i], kv_value<FMT, HD>(a.kv, s, kv_row(a.kv, s, 1, g, j0 + i), e), acc);
-  }
-  o[tid] = acc;
-  __syncthreads();
-  if (tid < HD) {
-    for (int i = 1; i < PARTS; i++) acc += o[i * HD + tid];
-    out[tid] = acc / l;
-  }
+// positions of a tile, and how a format's operands are laid out
+template <int FMT>
+constexpr int kTile = FMT == Q3H_KV_F32 ? 16 : 32;
+
+// where the positions of a row group are cut: tiles in all, tiles a split
+struct Cut {
+  int full;   // positions that all the group's rows see
+  int end;    // positions that some row of it sees
+  int tiles, per;
+};
+__device__ __forceinline__ Cut cut_of(const AttendRows &a, const KvSeq &s, int t0, int t1,
+                                      int splits, int tile) {
+  Cut c;
+  c.full = s.len + (a.parents ? 0 : t0 + 1);
+  c.end = s.len + t1 + 1;
+  c.tiles = (c.end + tile - 1) / tile;
+  c.per = (c.tiles + splits - 1) / splits;
+  return c;
 }
+
+// two floats rounded to f16 and what is left of them
+__device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t &lo) {
+  const h2 h = __builtin_convertvector((f2){x, y}, h2);
+  const h2 l = __builtin_convertvector((f2){x - (float)h[0], y - (float)h[1]}, h2);
+  hi = __builtin_bit_cast(uint32_t, h);
+  lo = __builtin_bit_cast(uint32_t, l);
+}
+
+// bytes a, b of a pair of int8 words (biased by 128) as two exact f16
+__device__ __forceinline__ uint32_t bytes_f16(uint32_t w, uint32_t sel) {
+  // 0x6400 | u is 1024 + u
+  const uint32_t x = __builtin_amdgcn_perm(0x64646464u, w, sel);
+  const h2 v = __builtin_bit_cast(h2, x) + (h2){(_Float16)-1152.f, (_Float16)-1152.f};
+  return __builtin_bit_cast(uint32_t, v);
+}
+
+template <int FMT, int HD>
+struct Raw;  // a tile's keys and values as loaded
 
 template <int HD>
-void launch(const AttendRows &a, int fmt, hipStream_t st) {
-  const dim3 grid(a.kv.rows, a.heads, a.kv.sequences);
-  if (fmt == Q3H_KV_F32)
-    hipLaunchKernelGGL((k_attend<Q3H_KV_F32, HD>), grid, dim3(kThreads), 0, st, a);
-  else if (fmt == Q3H_KV_F16)
-    hipLaunchKernelGGL((k_attend<Q3H_KV_F16, HD>), grid, dim3(kThreads), 0, st, a);
+struct Raw<Q3H_KV_F16, HD> {
+  u4 k[2][HD / 32];
+  u4 v[8 * HD / 128];  // 8 positions of HD / 16 halves
+};
+template <int HD>
+struct Raw<Q3H_KV_Q8, HD> {
+  u4 k[2][HD / 64];
+  u2 v[8 * HD / 128];  // 8 positions of HD / 16 bytes
+  f4 ks[2], vs[2];
+};
+template <int HD>
+struct Raw<Q3H_KV_F32, HD> {
+  f4 k[HD / 16];
+  f4 v[4][HD / 64];
+};
+
+// One workgroup per (split, kv head, sequence, group of WQ * NQ query tiles):
+// WQ waves side by side over the query tiles, 4 / WQ waves over the positions.
+// NQ tiles a wave share its loads and conversions of K and V.
+template <int FMT, int HD, int NQ, int WQ>
+__global__ __launch_bounds__(kThreads) void k_attend(AttendRows a, int splits) {
+  constexpr int T = kTile<FMT>, WK = kWaves / WQ;
+  constexpr int GROUP = 16 * NQ * WQ;  // query rows of the workgroup
+  constexpr int C = HD / 16;           // output tiles; neighbouring elements a lane reads
+  constexpr bool F32 = FMT == Q3H_KV_F32, Q8 = FMT == Q3H_KV_Q8;
+  constexpr int NS = F32 ? 1 : 2;  // key tiles of 16 in a tile
+  __shared__ float sm_acc[WK > 1 ? kWaves * NQ * 16 * HD : 1];
+  __shared__ float sm_m[kWaves][NQ * 16], sm_l[kWaves][NQ * 16];
+  __shared__ float sm_w[F32 || FMT == Q3H_KV_F16 ? kWaves : 1][NQ * 16][T];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int n16 = lane & 15, g4 = lane >> 4;
+  const int wq = wave % WQ, wk = wave / WQ;
+  const int split = blockIdx.x % splits, rest = blockIdx.x / splits;
+  const int g = rest % a.kv.kvh, b = (rest / a.kv.kvh) % a.kv.sequences,
+            group = rest / a.kv.kvh / a.kv.sequences;
+  const int per_kv = a.heads / a.kv.kvh;
+  const KvSeq s = kv_sequence(a.kv, b);
+  const int rows_in = s.count * per_kv;  // query rows of the sequence's kv head
+  const int first = group * GROUP;
+  if (first >= rows_in) return;
+  const size_t row0 = (size_t)b * a.kv.rows;
+  const bool bad = s.len < 0 || s.len > a.max_len || s.len > s.max_pos - s.count;
+  if (bad) {
+    if (split > 0 || splits > 1) return;  // (the merge writes it)
+    for (int i = tid; i < GROUP * HD; i += kThreads) {
+      const int r = first + i / HD;
+      if (r < rows_in)
+        a.out[(row0 + r / per_kv) * a.ld_out + (size_t)(g * per_kv + r % per_kv) * HD + i % HD] =
+            NAN;
+    }
+    return;
+  }
+  const int t1 = (std::min(first + GROUP, rows_in) - 1) / per_kv;
+  const Cut cut = cut_of(a, s, first / per_kv, t1, splits, T);
+  const int tile0 = split * cut.per, tile1 = std::min(cut.tiles, tile0 + cut.per);
+  if (tile0 >= tile1) return;
+  const int last = cut.end - 1;  // no row behind it is read
+
+  // the wave's queries: dims of (step, lane group) as the keys' loads have them
+  int qrow[NQ];
+  bool live[NQ];
+  f4 qf[F32 ? NQ : 1][HD / 16];
+  uint32_t qh[F32 ? 1 : NQ][HD / 32][4], ql[F32 ? 1 : NQ][HD / 32][4];
+  float sfac[NQ];
+#pragma unroll
+  for (int q = 0; q < NQ; q++) {
+    const int r = first + (wq * NQ + q) * 16 + n16;
+    live[q] = r < rows_in;
+    qrow[q] = std::min(r, rows_in - 1);
+    const float *p = a.q + (row0 + qrow[q] / per_kv) * a.ldq +
+                     (size_t)(g * per_kv + qrow[q] % per_kv) * HD;
+    constexpr float kLog2e = 1.44269504088896340736f;
+    if constexpr (F32) {
+#pragma unroll
+      for (int i = 0; i < HD / 16; i++) qf[q][i] = load<f4u>((const char *)p, 4 * (16 * i + 4 * g4));
+      sfac[q] = a.scale * kLog2e;
+    } else {
+      float x[HD / 32][8];
+      float m = 0.f;
+      bool odd = false;
+#pragma unroll
+      for (int i = 0; i < HD / 32; i++) {
+        const int d = Q8 ? (i >> 1) * 64 + g4 * 16 + (i & 1) * 8 : i * 32 + g4 * 8;
+        const f4 u = load<f4u>((const char *)p, 4 * d), w = load<f4u>((const char *)p, 4 * d + 16);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          x[i][e] = u[e];
+          x[i][4 + e] = w[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          m = fmaxf(m, fabsf(x[i][e]));
+          odd = odd || !(fabsf(x[i][e]) < INFINITY);
+        }
+      }
+      m = rows4_max(odd ? INFINITY : m);
+      // m * 2^k in [2^13, 2^14); infinities and NaN stay what they are
+      int k = m > 0.f && m < INFINITY ? 14 - (ilogbf(m) + 1) : 0;
+#pragma unroll
+      for (int i = 0; i < HD / 32; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          split2(ldexpf(x[i][2 * e], k), ldexpf(x[i][2 * e + 1], k), qh[q][i][e], ql[q][i][e]);
+      sfac[q] = ldexpf(a.scale * kLog2e, -k);
+    }
+  }
+
+  const char *kbase = s.k0 + kv_row(a.kv, s, 0, g, 0) * (HD * (F32 ? 4 : Q8 ? 1 : 2));
+  const char *vbase = s.k0 + kv_row(a.kv, s, 1, g, 0) * (HD * (F32 ? 4 : Q8 ? 1 : 2));
+  const char *ksc = nullptr, *vsc = nullptr;
+  if constexpr (Q8) {
+    ksc = reinterpret_cast<const char *>(kv_scales(a.kv, s, HD) + kv_row(a.kv, s, 0, g, 0));
+    vsc = reinterpret_cast<const char *>(kv_scales(a.kv, s, HD) + kv_row(a.kv, s, 1, g, 0));
+  }
+  constexpr int ROW = HD * (F32 ? 4 : Q8 ? 1 : 2);  // bytes
+
+  Raw<FMT, HD> raw;
+  auto load_k = [&](int tile) {
+    const int j0 = tile * T;
+#pragma unroll
+    for (int t = 0; t < NS; t++) {
+      const int64_t at = (int64_t)std::min(j0 + 16 * t + n16, last) * ROW;
+      if constexpr (F32) {
+#pragma unroll
+        for (int i = 0; i < HD / 16; i++) raw.k[i] = load<f4>(kbase, at + 64 * i + 16 * g4);
+      } else if constexpr (Q8) {
+#pragma unroll
+        for (int i = 0; i < HD / 64; i++) raw.k[t][i] = load<u4>(kbase, at + 64 * i + 16 * g4);
+      } else {
+#pragma unroll
+        for (int i = 0; i < HD / 32; i++) raw.k[t][i] = load<u4>(kbase, at + 64 * i + 16 * g4);
+      }
+    }
+    if constexpr (Q8) {
+#pragma unroll
+      for (int t = 0; t < 2; t++) {
+        const int j = j0 + 16 * t + 4 * g4;
+        if (j0 + T <= cut.end) {
+          raw.ks[t] = load<f4u>(ksc, 4 * (int64_t)j);
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; r++)
+            raw.ks[t][r] = load<float>(ksc, 4 * (int64_t)std::min(j + r, last));
+        }
+      }
+    }
+  };
+  auto load_v = [&](int tile) {
+    const int j0 = tile * T;
+#pragma unroll
+    for (int i = 0; i < (F32 ? 4 : 8); i++) {
+      const int j = j0 + (F32 ? 4 * g4 + i : (i >> 2) * 16 + 4 * g4 + (i & 3));
+      const int64_t at = (int64_t)std::min(j, last) * ROW + n16 * (ROW / 16);
+      if constexpr (F32) {
+#pragma unroll
+        for (int e = 0; e < HD / 64; e++) raw.v[i][e] = load<f4>(vbase, at + 16 * e);
+      } else if constexpr (Q8) {
+        if constexpr (HD == 128) raw.v[i] = load<u2>(vbase, at);
+        else raw.v[i / 2][i & 1] = load<uint32_t>(vbase, at);
+      } else {
+        if constexpr (HD == 128) {
+          raw.v[i] = load<u4>(vbase, at);
+        } else {
+          const u2 x = load<u2>(vbase, at);
+          raw.v[i / 2][2 * (i & 1)] = x[0];
+          raw.v[i / 2][2 * (i & 1) + 1] = x[1];
+        }
+      }
+    }
+    if constexpr (Q8) {
+#pragma unroll
+      for (int t = 0; t < 2; t++) {
+        const int j = j0 + 16 * t + 4 * g4;
+        if (j0 + T <= cut.end) {
+          raw.vs[t] = load<f4u>(vsc, 4 * (int64_t)j);
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; r++)
+            raw.vs[t][r] = load<float>(vsc, 4 * (int64_t)std::min(j + r, last));
+        }
+      }
+    }
+  };
+  // word w of the HD / 16 elements of position i of the loaded values
+  auto vword = [&](int i, int w) -> uint32_t {
+    if constexpr (FMT == Q3H_KV_F16)
+      return HD == 128 ? raw.v[i][w] : raw.v[i / 2][2 * (i & 1) + w];
+    else if constexpr (Q8)
+      return HD == 128 ? raw.v[i][w] : raw.v[i / 2][i & 1];
+    else
+      return 0;
+  };
+
+  f4 acc[NQ][C];
+  float m[NQ], l[NQ];
+  int ev;  // int8: the values' scales are below 2^ev so far
+  uint64_t path[NQ];
+  bool broken[NQ], paths = false;
+#pragma unroll
+  for (int q = 0; q < NQ; q++) path[q] = 0, broken[q] = false;
+  // An infinity times one of the parts that a query or a weight is split in is
+  // NaN where the product itself is not. A wave that ends with a NaN goes over
+  // its positions again with care: such products one by one, in f32.
+  for (bool careful = false;; careful = true) {
+#pragma unroll
+  for (int q = 0; q < NQ; q++) {
+    m[q] = -INFINITY;
+    l[q] = 0.f;
+#pragma unroll
+    for (int c = 0; c < C; c++) acc[q][c] = (f4){0.f, 0.f, 0.f, 0.f};
+  }
+  ev = -100;
+  int tile = tile0 + wk;
+  if (tile < tile1) {
+    load_k(tile);
+    load_v(tile);
+  }
+  for (; tile < tile1; tile += WK) {
+    const int j0 = tile * T;
+    const bool tail = j0 + T > cut.full;
+    // scores
+    f4 st[NQ][NS];
+#pragma unroll
+    for (int q = 0; q < NQ; q++)
+#pragma unroll
+      for (int t = 0; t < NS; t++) st[q][t] = (f4){0.f, 0.f, 0.f, 0.f};
+    if constexpr (F32) {
+#pragma unroll
+      for (int i = 0; i < HD / 16; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+#pragma unroll
+          for (int q = 0; q < NQ; q++)
+            st[q][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(raw.k[i][e], qf[q][i][e], st[q][0], 0,
+                                                            0, 0);
+    } else {
+#pragma unroll
+      for (int t = 0; t < NS; t++)
+#pragma unroll
+        for (int i = 0; i < HD / 32; i++) {
+          u4 ka;
+          if constexpr (Q8) {
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+              const uint32_t w = raw.k[t][i >> 1][2 * (i & 1) + e] ^ 0x80808080u;
+              ka[2 * e] = bytes_f16(w, 0x04010400u);
+              ka[2 * e + 1] = bytes_f16(w, 0x04030402u);
+            }
+          } else {
+            ka = raw.k[t][i];
+          }
+          const h8 A = __builtin_bit_cast(h8, ka);
+#pragma unroll
+          for (int q = 0; q < NQ; q++) {
+            const u4 bl = {ql[q][i][0], ql[q][i][1], ql[q][i][2], ql[q][i][3]};
+            const u4 bh = {qh[q][i][0], qh[q][i][1], qh[q][i][2], qh[q][i][3]};
+            st[q][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, __builtin_bit_cast(h8, bl),
+                                                              st[q][t], 0, 0, 0);
+            st[q][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, __builtin_bit_cast(h8, bh),
+                                                              st[q][t], 0, 0, 0);
+          }
+        }
+    }
+    f4 ks[2], vs[2];
+    if constexpr (Q8) {
+#pragma unroll
+      for (int t = 0; t < 2; t++) {
+        ks[t] = raw.ks[t];
+        vs[t] = raw.vs[t];
+      }
+    }
+    if (tile + WK < tile1) load_k(tile + WK);
+
+    // which positions the rows see (the tile of the drafted rows and behind)
+    uint32_t sees[NQ];
+#pragma unroll
+    for (int q = 0; q < NQ; q++) sees[q] = 0xff;
+    if (tail) {
+      if (a.parents && !paths) {
+        paths = true;
+        const Path p = tree_path(a.parents + row0, a.kv.rows);
+#pragma unroll
+        for (int q = 0; q < NQ; q++) {
+          path[q] = __shfl(p.rows, qrow[q] / per_kv);
+          broken[q] = __shfl((int)p.bad, qrow[q] / per_kv) != 0;
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < NQ; q++) {
+        const int t = qrow[q] / per_kv;
+        sees[q] = 0;
+#pragma unroll
+        for (int i = 0; i < 4 * NS; i++) {
+          const int d = j0 + (i >> 2) * 16 + 4 * g4 + (i & 3) - s.len;
+          const bool ok = d < 0 || (d <= t && (!a.parents || (path[q] >> d & 1)));
+          sees[q] |= (ok ? 1u : 0u) << i;
+        }
+      }
+    }
+    float vfac = 16384.f;
+    int ev_new = ev;
+    if constexpr (Q8) {
+      float x = 0.f;
+#pragma unroll
+      for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) x = fmaxf(x, vs[t][r]);
+      x = rows4_max(x);
+      ev_new = std::max(ev, (int)(__float_as_uint(x) >> 23) - 126);
+      vfac = ldexpf(1.f, 14 - ev_new);
+    }
+    float w[NQ][4 * NS];
+#pragma unroll
+    for (int q = 0; q < NQ; q++) {
+      float mx = m[q];
+#pragma unroll
+      for (int i = 0; i < 4 * NS; i++) {
+        float x = st[q][i >> 2][i & 3] * sfac[q];
+        if constexpr (Q8) x *= ks[i >> 2][i & 3];
+        if (careful && x != x) {
+          const float *p = a.q + (row0 + qrow[q] / per_kv) * a.ldq +
+                           (size_t)(g * per_kv + qrow[q] % per_kv) * HD;
+          const int64_t at = (int64_t)std::min(j0 + (i >> 2) * 16 + 4 * g4 + (i & 3), last) * ROW;
+          x = 0.f;
+          for (int e = 0; e < HD; e++) {
+            float k;
+            if constexpr (F32) k = load<float>(kbase, at + 4 * e);
+            else if constexpr (Q8) k = (float)load<int8_t>(kbase, at + e);
+            else k = (float)load<_Float16>(kbase, at + 2 * e);
+            x = fmaf(p[e], k, x);
+          }
+          x *= a.scale * 1.44269504088896340736f;
+          if constexpr (Q8) x *= ks[i >> 2][i & 3];
+        }
+        if (tail) {
+          x = sees[q] >> i & 1 ? x : -INFINITY;
+          // a row whose path is broken: NaN at itself, and so in all of it
+          if (broken[q] && j0 + (i >> 2) * 16 + 4 * g4 + (i & 3) - s.len == qrow[q] / per_kv)
+            x = NAN;
+        }
+        w[q][i] = x;
+        mx = fmaxf(mx, x);
+      }
+      mx = rows4_max(mx);
+      const float base = mx == -INFINITY ? 0.f : mx;
+      if (__any(mx > m[q] || ev_new > ev)) {
+        const float f = __builtin_amdgcn_exp2f(m[q] - base);
+        l[q] *= f;
+        const float fa = Q8 ? ldexpf(f, ev - ev_new) : f;
+#pragma unroll
+        for (int c = 0; c < C; c++) acc[q][c] *= fa;
+        m[q] = mx;
+      }
+#pragma unroll
+      for (int i = 0; i < 4 * NS; i++) {
+        const float p = __builtin_amdgcn_exp2f(w[q][i] - base);
+        l[q] += p;
+        if constexpr (Q8) {
+          w[q][i] = p * (vs[i >> 2][i & 3] * vfac);
+          if (tail) w[q][i] = sees[q] >> i & 1 ? w[q][i] : 0.f;
+        } else if constexpr (F32) {
+          w[q][i] = p;
+        } else {
+          w[q][i] = p * vfac;
+        }
+      }
+    }
+    ev = ev_new;
+
+    // values: an infinity or NaN in a drafted row reaches only the rows that
+    // see it: such elements (and everything behind the last row) go in as 0, and
+    // are added by hand
+    bool odd = false;
+    const int guard0 = careful ? 0 : s.len;  // positions from here on are looked at
+    if constexpr (!Q8) {
+      if (tail || careful) {
+#pragma unroll
+        for (int i = 0; i < 4 * NS; i++) {
+          const int j = j0 + (i >> 2) * 16 + 4 * g4 + (i & 3);
+          if constexpr (F32) {
+#pragma unroll
+            for (int e = 0; e < C; e++)
+              if (j >= guard0) {
+                const float x = raw.v[i][e >> 2][e & 3];
+                const bool fin = fabsf(x) < INFINITY;
+                odd = odd || !fin;
+                raw.v[i][e >> 2][e & 3] = fin ? x : 0.f;
+              }
+          } else {
+#pragma unroll
+            for (int e = 0; e < C / 2; e++)
+              if (j >= guard0) {
+                const uint32_t x = vword(i, e);
+                const bool lo = (x & 0x7c00u) != 0x7c00u, hi = (x & 0x7c000000u) != 0x7c000000u;
+                odd = odd || !lo || !hi;
+                const uint32_t y = x & ((lo ? 0xffffu : 0u) | (hi ? 0xffff0000u : 0u));
+                if constexpr (HD == 128) raw.v[i][e] = y;
+                else raw.v[i / 2][2 * (i & 1) + e] = y;
+              }
+          }
+        }
+        odd = __any(odd);
+      }
+    }
+    if constexpr (F32) {
+#pragma unroll
+      for (int r = 0; r < 4; r++)
+#pragma unroll
+        for (int c = 0; c < C; c++)
+#pragma unroll
+          for (int q = 0; q < NQ; q++)
+            acc[q][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(raw.v[r][c >> 2][c & 3], w[q][r],
+                                                             acc[q][c], 0, 0, 0);
+    } else {
+      u4 ph[NQ], pl[NQ];
+#pragma unroll
+      for (int q = 0; q < NQ; q++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          uint32_t hi, lo;
+          split2(w[q][2 * e], w[q][2 * e + 1], hi, lo);
+          ph[q][e] = hi;
+          pl[q][e] = lo;
+        }
+#pragma unroll
+      for (int c = 0; c < C; c++) {
+        u4 va;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          if constexpr (Q8) {
+            // bytes c of positions 2e and 2e + 1
+            const uint32_t x = vword(2 * e, c >> 2), y = vword(2 * e + 1, c >> 2);
+            const uint32_t sel = 0x0c0c0000u | ((4u + (c & 3)) << 8) | (c & 3);
+            const uint32_t z = __builtin_amdgcn_perm(y, x, sel) ^ 0x00008080u;
+            va[e] = bytes_f16(z, 0x04010400u);
+          } else {
+            const uint32_t x = vword(2 * e, c >> 1), y = vword(2 * e + 1, c >> 1);
+            va[e] = __builtin_amdgcn_perm(y, x, c & 1 ? 0x07060302u : 0x05040100u);
+          }
+        }
+        const h8 A = __builtin_bit_cast(h8, va);
+#pragma unroll
+        for (int q = 0; q < NQ; q++) {
+          acc[q][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, __builtin_bit_cast(h8, pl[q]),
+                                                             acc[q][c], 0, 0, 0);
+          acc[q][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, __builtin_bit_cast(h8, ph[q]),
+                                                             acc[q][c], 0, 0, 0);
+        }
+      }
+    }
+    if constexpr (!Q8) {
+      if (odd) {
+        // weights of the tile by query, negative where the row does not see it
+#pragma unroll
+        for (int q = 0; q < NQ; q++)
+#pragma unroll
+          for (int i = 0; i < 4 * NS; i++)
+            sm_w[wave][q * 16 + n16][(i >> 2) * 16 + 4 * g4 + (i & 3)] =
+                sees[q] >> i & 1 ? w[q][i] : -1.f;
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        for (int j = std::max(j0, guard0); j <= std::min(j0 + T - 1, last); j++) {
+#pragma unroll
+          for (int c = 0; c < C; c++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+              const int e = C * (4 * g4 + r) + c;
+              float x;
+              if constexpr (F32) x = load<float>(vbase, (int64_t)j * ROW + 4 * e);
+              else x = (float)load<_Float16>(vbase, (int64_t)j * ROW + 2 * e);
+              if (fabsf(x) < INFINITY) continue;
+#pragma unroll
+              for (int q = 0; q < NQ; q++) {
+                const float p = sm_w[wave][q * 16 + n16][j - j0];
+                if (!(p < 0.f)) acc[q][c][r] += p * x;
+              }
+            }
+        }
+      }
+    }
+    if (tile + WK < tile1) load_v(tile + WK);
+  }
+  if (careful) break;
+  bool nan = false;
+#pragma unroll
+  for (int q = 0; q < NQ; q++) {
+    nan = nan || l[q] != l[q];
+#pragma unroll
+    for (int c = 0; c < C; c++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) nan = nan || acc[q][c][r] != acc[q][c][r];
+  }
+  if (!__any(nan)) break;
+  }
+
+  // the waves over the positions together
+  constexpr int Q16 = NQ * 16;
+#pragma unroll
+  for (int q = 0; q < NQ; q++) {
+    l[q] = rows4_sum(l[q]);
+    if (WK > 1 && g4 == 0) {
+      sm_m[wave][q * 16 + n16] = m[q];
+      sm_l[wave][q * 16 + n16] = l[q];
+    }
+  }
+  if (WK > 1) __syncthreads();
+  float *part = a.part;
+  const size_t part_rows = (size_t)a.kv.rows * per_kv;
+  const size_t part0 = ((size_t)(b * a.kv.kvh + g) * splits + split) * part_rows;
+  float *part_ml = part + (size_t)a.kv.sequences * a.kv.kvh * splits * part_rows * HD;
+#pragma unroll
+  for (int q = 0; q < NQ; q++) {
+    float M = m[q], L = l[q], f = 1.f;
+    if constexpr (WK > 1) {
+      M = -INFINITY;
+      for (int i = 0; i < WK; i++) M = fmaxf(M, sm_m[i * WQ + wq][q * 16 + n16]);
+      const float base = M == -INFINITY ? 0.f : M;
+      L = 0.f;
+      for (int i = 0; i < WK; i++)
+        L += sm_l[i * WQ + wq][q * 16 + n16] *
+             __builtin_amdgcn_exp2f(sm_m[i * WQ + wq][q * 16 + n16] - base);
+      f = __builtin_amdgcn_exp2f(m[q] - base);
+    }
+    // out of the weights' scale; with one split also the softmax's sum
+    if constexpr (Q8) f = ldexpf(f, ev - 14);
+    else if constexpr (!F32) f *= 1.f / 16384.f;
+    if (splits == 1) f /= L;
+    if (splits > 1 && wk == 0 && g4 == 0 && live[q]) {
+      part_ml[2 * (part0 + qrow[q])] = M;
+      part_ml[2 * (part0 + qrow[q]) + 1] = L;
+    }
+    if constexpr (WK > 1) {
+#pragma unroll
+      for (int c = 0; c < C; c++)
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+          sm_acc[(wave * Q16 + q * 16 + n16) * HD + C * (4 * g4 + r) + c] = acc[q][c][r] * f;
+    } else if (live[q]) {
+      float *o = splits > 1 ? part + (part0 + qrow[q]) * HD
+                            : a.out + (row0 + qrow[q] / per_kv) * a.ld_out +
+                                  (size_t)(g * per_kv + qrow[q] % per_kv) * HD;
+#pragma unroll
+      for (int r = 0; r < 4; r++)
+#pragma unroll
+        for (int c = 0; c < C; c++) o[C * (4 * g4 + r) + c] = acc[q][c][r] * f;
+    }
+  }
+  if constexpr (WK > 1) {
+    __syncthreads();
+    for (int i = tid; i < GROUP * HD; i += kThreads) {
+      const int r = i / HD, e = i % HD;  // row of the group
+      const int row = first + r;
+      if (row >= rows_in) break;
+      float x = 0.f;
+      for (int k = 0; k < WK; k++)
+        x += sm_acc[((k * WQ + r / Q16) * Q16 + r % Q16) * HD + e];
+      if (splits > 1)
+        part[(part0 + row) * HD + e] = x;
+      else
+        a.out[(row0 + row / per_kv) * a.ld_out + (size_t)(g * per_kv + row % per_kv) * HD + e] = x;
+    }
+  }
+}
+
+// The splits' parts of a query row together: one row a wave.
+template <int HD>
+__global__ __launch_bounds__(kThreads) void k_attend_merge(AttendRows a, int splits, int tile,
+                                                           int group_rows) {
+  const int lane = threadIdx.x & 63;
+  const int per_kv = a.heads / a.kv.kvh;
+  const int64_t id = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
+  const int part_rows = a.kv.rows * per_kv;
+  const int row = (int)(id % part_rows);
+  const int64_t bg = id / part_rows;
+  const int g = (int)(bg % a.kv.kvh), b = (int)(bg / a.kv.kvh);
+  if (b >= a.kv.sequences) return;
+  const KvSeq s = kv_sequence(a.kv, b);
+  const int rows_in = s.count * per_kv;
+  if (row >= rows_in) return;
+  float *out = a.out + ((size_t)b * a.kv.rows + row / per_kv) * a.ld_out +
+               (size_t)(g * per_kv + row % per_kv) * HD;
+  if (s.len < 0 || s.len > a.max_len || s.len > s.max_pos - s.count) {
+    for (int e = lane; e < HD; e += 64) out[e] = NAN;
+    return;
+  }
+  const int first = row / group_rows * group_rows;
+  const Cut cut = cut_of(a, s, first / per_kv,
+                         (std::min(first + group_rows, rows_in) - 1) / per_kv, splits, tile);
+  const int n = (cut.tiles + cut.per - 1) / cut.per;  // splits that hold anything
+  const size_t base = (size_t)bg * splits * part_rows + row;
+  const float *ml = a.part + (size_t)a.kv.sequences * a.kv.kvh * splits * part_rows * HD;
+  float M = -INFINITY;
+  for (int i = lane; i < n; i += 64) M = fmaxf(M, ml[2 * (base + (size_t)i * part_rows)]);
+  M = wave_max_dpp(M);
+  const float top = M == -INFINITY ? 0.f : M;
+  float L = 0.f;
+  for (int i = lane; i < n; i += 64)
+    L += ml[2 * (base + (size_t)i * part_rows) + 1] *
+         __builtin_amdgcn_exp2f(ml[2 * (base + (size_t)i * part_rows)] - top);
+  L = wave_sum_dpp(L);
+  float x[HD / 64] = {};
+  for (int i = 0; i < n; i++) {
+    const float f = __builtin_amdgcn_exp2f(ml[2 * (base + (size_t)i * part_rows)] - top);
+#pragma unroll
+    for (int e = 0; e < HD / 64; e++)
+      x[e] += f * a.part[(base + (size_t)i * part_rows) * HD + 64 * e + lane];
+  }
+#pragma unroll
+  for (int e = 0; e < HD / 64; e++) out[64 * e + lane] = x[e] / L;
+}
+
+// How a call is laid out: NQ query tiles a wave, WQ waves side by side over
+// the query tiles (the others over the positions), splits of the positions.
+struct Shape {
+  int nq, wq, splits;
+  int group() const { return 16 * nq * wq; }
+};
+Shape shape_of(int sequences, int rows, int heads, int kvh, int max_len) {
+  const int q_rows = rows * (heads / kvh);
+  Shape s;
+  s.nq = q_rows > 16 ? 2 : 1;
+  s.wq = q_rows > 64 ? 4 : q_rows > 32 ? 2 : 1;
+  const int64_t units = (int64_t)sequences * kvh * ((q_rows + s.group() - 1) / s.group());
+  const int tiles = (max_len + rows + 31) / 32;
+  const int64_t want = std::max<int64_t>(1, 512 / units);
+  const int most = std::max(1, tiles / (2 * (kWaves / s.wq)));
+  s.splits = (int)std::min<int64_t>(want, most);
+  return s;
+}
+
+template <int FMT, int HD>
+void launch(const AttendRows &a, hipStream_t st) {
+  const Shape s = shape_of(a.kv.sequences, a.kv.rows, a.heads, a.kv.kvh, a.max_len);
+  const int q_rows = a.kv.rows * (a.heads / a.kv.kvh);
+  const unsigned blocks = (unsigned)((int64_t)s.splits * a.kv.kvh * a.kv.sequences *
+                                     ((q_rows + s.group() - 1) / s.group()));
+  if (s.nq == 1)
+    hipLaunchKernelGGL((k_attend<FMT, HD, 1, 1>), dim3(blocks), dim3(kThreads), 0, st, a,
+                       s.splits);
+  else if (s.wq == 1)
+    hipLaunchKernelGGL((k_attend<FMT, HD, 2, 1>), dim3(blocks), dim3(kThreads), 0, st, a,
+                       s.splits);
+  else if (s.wq == 2)
+    hipLaunchKernelGGL((k_attend<FMT, HD, 2, 2>), dim3(blocks), dim3(kThreads), 0, st, a,
+                       s.splits);
   else
-    hipLaunchKernelGGL((k_attend<Q3H_KV_Q8, HD>), grid, dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL((k_attend<FMT, HD, 2, 4>), dim3(blocks), dim3(kThreads), 0, st, a,
+                       s.splits);
+  if (s.splits > 1) {
+    const int64_t rows = (int64_t)a.kv.sequences * a.kv.kvh * q_rows;
+    hipLaunchKernelGGL((k_attend_merge<HD>), dim3((unsigned)((rows + kWaves - 1) / kWaves)),
+                       dim3(kThreads), 0, st, a, s.splits, kTile<FMT>, s.group());
+  }
 }
 
 }  // namespace
 
-size_t attend_part_bytes(int, int, int, int, int, int) { return 0; }
+size_t attend_part_bytes(int sequences, int rows, int heads, int kvh, int hd, int max_len) {
+  const Shape s = shape_of(sequences, rows, heads, kvh, max_len);
+  if (s.splits == 1) return 0;
+  return sizeof(float) * (size_t)sequences * heads * rows * s.splits * (hd + 2);
+}
 
 void launch_cache_attend(const AttendRows &a, int hd, int fmt, hipStream_t st) {
-  if (hd == 64)
-    launch<64>(a, fmt, st);
-  else
-    launch<128>(a, fmt, st);
+  if (hd == 64) {
+    if (fmt == Q3H_KV_F32) launch<Q3H_KV_F32, 64>(a, st);
+    else if (fmt == Q3H_KV_F16) launch<Q3H_KV_F16, 64>(a, st);
+    else launch<Q3H_KV_Q8, 64>(a, st);
+  } else {
+    if (fmt == Q3H_KV_F32) launch<Q3H_KV_F32, 128>(a, st);
+    else if (fmt == Q3H_KV_F16) launch<Q3H_KV_F16, 128>(a, st);
+    else launch<Q3H_KV_Q8, 128>(a, st);
+  }
 }
 
 }  // namespace q3h
