@@ -118,9 +118,9 @@ __global__ __launch_bounds__(kThreads) void k_cache_append(AppendRows a) {
         q0 = min(127, max(-127, (int)rint((double)x0 / (double)d)));
         q1 = min(127, max(-127, (int)rint((double)x1 / (double)d)));
       }
-      int8_t *o = reinterpret_cast<int8_t *>(s.k0) + at * HD;
-      o[e0] = (int8_t)q0;
-      o[e1] = (int8_t)q1;
+      uint8_t *o = reinterpret_cast<uint8_t *>(s.k0) + at * HD;
+      o[e0] = (uint8_t)(q0 < 0 ? 128 - q0 : q0);
+      o[e1] = (uint8_t)(q1 < 0 ? 128 - q1 : q1);
       if (sub == 0) kv_scales(a.kv, s, HD)[at] = d;
     } else {
       using KV = std::conditional_t<FMT == Q3H_KV_F16, _Float16, float>;
@@ -160,9 +160,9 @@ __global__ __launch_bounds__(kThreads) void k_cache_read(KvView kv, const int32_
     } else {
       const int64_t at = kv_row(kv, s, part, g, s.len + t);
       if constexpr (FMT == Q3H_KV_Q8) {
-        const int8_t *p = reinterpret_cast<const int8_t *>(s.k0) + at * HD + e;
+        const uint8_t *p = reinterpret_cast<const uint8_t *>(s.k0) + at * HD + e;
         const float d = kv_scales(kv, s, HD)[at];
-        for (int x = 0; x < 8; x++) o[x] = (float)p[x] * d;
+        for (int x = 0; x < 8; x++) o[x] = kv_byte(p[x]) * d;
       } else {
         using KV = std::conditional_t<FMT == Q3H_KV_F16, _Float16, float>;
         const KV *p = reinterpret_cast<const KV *>(s.k0) + at * HD + e;

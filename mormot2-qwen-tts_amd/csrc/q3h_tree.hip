@@ -38,7 +38,6 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef float f2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u4e __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 
 template <typename T>
@@ -47,14 +46,16 @@ __device__ __forceinline__ T load(const char *p, int64_t off) {
       reinterpret_cast<uintptr_t>(p) + off);
 }
 
-// positions of a tile, and how a format's operands are laid out
+// positions of a tile
 template <int FMT>
 constexpr int kTile = FMT == Q3H_KV_F32 ? 16 : 32;
 
+constexpr float kLog2e = 1.44269504088896340736f;
+
 // where the positions of a row group are cut: tiles in all, tiles a split
 struct Cut {
-  int full;   // positions that all the group's rows see
-  int end;    // positions that some row of it sees
+  int full;  // positions that all the group's rows see
+  int end;   // positions that some row of it sees
   int tiles, per;
 };
 __device__ __forceinline__ Cut cut_of(const AttendRows &a, const KvSeq &s, int t0, int t1,
@@ -75,12 +76,10 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t 
   lo = __builtin_bit_cast(uint32_t, l);
 }
 
-// bytes a, b of a pair of int8 words (biased by 128) as two exact f16
-__device__ __forceinline__ uint32_t bytes_f16(uint32_t w, uint32_t sel) {
-  // 0x6400 | u is 1024 + u
-  const uint32_t x = __builtin_amdgcn_perm(0x64646464u, w, sel);
-  const h2 v = __builtin_bit_cast(h2, x) + (h2){(_Float16)-1152.f, (_Float16)-1152.f};
-  return __builtin_bit_cast(uint32_t, v);
+// two bytes (sel: each twice) of an int8 cache as f16: sign and 7 bits of
+// magnitude, which as a subnormal are 2^-24 times it, exactly
+__device__ __forceinline__ uint32_t bytes_f16(uint32_t y, uint32_t x, uint32_t sel) {
+  return __builtin_amdgcn_perm(y, x, sel) & 0x807f807fu;
 }
 
 template <int FMT, int HD>
@@ -107,16 +106,17 @@ struct Raw<Q3H_KV_F32, HD> {
 // WQ waves side by side over the query tiles, 4 / WQ waves over the positions.
 // NQ tiles a wave share its loads and conversions of K and V.
 template <int FMT, int HD, int NQ, int WQ>
-__global__ __launch_bounds__(kThreads) void k_attend(AttendRows a, int splits) {
+__global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, int splits) {
   constexpr int T = kTile<FMT>, WK = kWaves / WQ;
   constexpr int GROUP = 16 * NQ * WQ;  // query rows of the workgroup
   constexpr int C = HD / 16;           // output tiles; neighbouring elements a lane reads
   constexpr bool F32 = FMT == Q3H_KV_F32, Q8 = FMT == Q3H_KV_Q8;
-  constexpr int NS = F32 ? 1 : 2;  // key tiles of 16 in a tile
+  constexpr int NS = F32 ? 1 : 2;                // key tiles of 16 in a tile
+  constexpr int ROW = HD * (F32 ? 4 : Q8 ? 1 : 2);  // bytes
   __shared__ float sm_acc[WK > 1 ? kWaves * NQ * 16 * HD : 1];
   __shared__ float sm_m[kWaves][NQ * 16], sm_l[kWaves][NQ * 16];
-  __shared__ float sm_w[F32 || FMT == Q3H_KV_F16 ? kWaves : 1][NQ * 16][T];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n16 = lane & 15, g4 = lane >> 4;
   const int wq = wave % WQ, wk = wave / WQ;
   const int split = blockIdx.x % splits, rest = blockIdx.x / splits;
@@ -130,7 +130,7 @@ __global__ __launch_bounds__(kThreads) void k_attend(AttendRows a, int splits) {
   const size_t row0 = (size_t)b * a.kv.rows;
   const bool bad = s.len < 0 || s.len > a.max_len || s.len > s.max_pos - s.count;
   if (bad) {
-    if (split > 0 || splits > 1) return;  // (the merge writes it)
+    if (splits > 1) return;  // (the merge writes it)
     for (int i = tid; i < GROUP * HD; i += kThreads) {
       const int r = first + i / HD;
       if (r < rows_in)
@@ -145,23 +145,103 @@ __global__ __launch_bounds__(kThreads) void k_attend(AttendRows a, int splits) {
   if (tile0 >= tile1) return;
   const int last = cut.end - 1;  // no row behind it is read
 
+  const char *kbase = s.k0 + kv_row(a.kv, s, 0, g, 0) * ROW;
+  const char *vbase = s.k0 + kv_row(a.kv, s, 1, g, 0) * ROW;
+  const char *ksc = nullptr, *vsc = nullptr;
+  if constexpr (Q8) {
+    ksc = reinterpret_cast<const char *>(kv_scales(a.kv, s, HD) + kv_row(a.kv, s, 0, g, 0));
+    vsc = reinterpret_cast<const char *>(kv_scales(a.kv, s, HD) + kv_row(a.kv, s, 1, g, 0));
+  }
+
+  Raw<FMT, HD> raw;
+  auto load_scales = [&](const char *sc, int j0, f4(&d)[2]) {
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+      const int j = j0 + 16 * t + 4 * g4;
+      if (j0 + T <= cut.end) {
+        d[t] = load<f4u>(sc + 4 * (int64_t)j0, (uint32_t)(64 * t + 16 * g4));
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; r++) d[t][r] = load<float>(sc, 4 * (int64_t)std::min(j + r, last));
+      }
+    }
+  };
+  auto load_k = [&](int tile) {
+    const int j0 = tile * T;
+    const char *p = kbase + (int64_t)j0 * ROW;
+#pragma unroll
+    for (int t = 0; t < NS; t++) {
+      const uint32_t at = (uint32_t)(std::min(16 * t + n16, last - j0) * ROW + 16 * g4);
+      if constexpr (F32) {
+#pragma unroll
+        for (int i = 0; i < HD / 16; i++) raw.k[i] = load<f4>(p, at + 64 * i);
+      } else if constexpr (Q8) {
+#pragma unroll
+        for (int i = 0; i < HD / 64; i++) raw.k[t][i] = load<u4>(p, at + 64 * i);
+      } else {
+#pragma unroll
+        for (int i = 0; i < HD / 32; i++) raw.k[t][i] = load<u4>(p, at + 64 * i);
+      }
+    }
+    if constexpr (Q8) load_scales(ksc, j0, raw.ks);
+  };
+  auto load_v = [&](int tile) {
+    const int j0 = tile * T;
+    const char *p = vbase + (int64_t)j0 * ROW;
+#pragma unroll
+    for (int i = 0; i < (F32 ? 4 : 8); i++) {
+      const int j = F32 ? 4 * g4 + i : (i >> 2) * 16 + 4 * g4 + (i & 3);
+      const uint32_t at = (uint32_t)(std::min(j, last - j0) * ROW + n16 * (ROW / 16));
+      if constexpr (F32) {
+#pragma unroll
+        for (int e = 0; e < HD / 64; e++) raw.v[i][e] = load<f4>(p, at + 16 * e);
+      } else if constexpr (Q8) {
+        if constexpr (HD == 128) raw.v[i] = load<u2>(p, at);
+        else raw.v[i / 2][i & 1] = load<uint32_t>(p, at);
+      } else {
+        if constexpr (HD == 128) {
+          raw.v[i] = load<u4>(p, at);
+        } else {
+          const u2 x = load<u2>(p, at);
+          raw.v[i / 2][2 * (i & 1)] = x[0];
+          raw.v[i / 2][2 * (i & 1) + 1] = x[1];
+        }
+      }
+    }
+    if constexpr (Q8) load_scales(vsc, j0, raw.vs);
+  };
+  // word w of the HD / 16 elements of position i of the loaded values
+  auto vword = [&](int i, int w) -> uint32_t {
+    if constexpr (FMT == Q3H_KV_F16)
+      return HD == 128 ? raw.v[i][w] : raw.v[i / 2][2 * (i & 1) + w];
+    else if constexpr (Q8)
+      return HD == 128 ? raw.v[i][w] : raw.v[i / 2][i & 1];
+    else
+      return 0;
+  };
+
+  int tile = tile0 + wk;
+  if (tile < tile1) {
+    load_k(tile);
+    load_v(tile);
+  }
+
   // the wave's queries: dims of (step, lane group) as the keys' loads have them
   int qrow[NQ];
   bool live[NQ];
   f4 qf[F32 ? NQ : 1][HD / 16];
-  uint32_t qh[F32 ? 1 : NQ][HD / 32][4], ql[F32 ? 1 : NQ][HD / 32][4];
-  float sfac[NQ];
+  u4 qh[F32 ? 1 : NQ][HD / 32], ql[F32 ? 1 : NQ][HD / 32];
+  float sfac[NQ];  // a score in powers of two: product * sfac (* the key's scale)
 #pragma unroll
   for (int q = 0; q < NQ; q++) {
     const int r = first + (wq * NQ + q) * 16 + n16;
     live[q] = r < rows_in;
     qrow[q] = std::min(r, rows_in - 1);
-    const float *p = a.q + (row0 + qrow[q] / per_kv) * a.ldq +
-                     (size_t)(g * per_kv + qrow[q] % per_kv) * HD;
-    constexpr float kLog2e = 1.44269504088896340736f;
+    const char *p = reinterpret_cast<const char *>(
+        a.q + (row0 + qrow[q] / per_kv) * a.ldq + (size_t)(g * per_kv + qrow[q] % per_kv) * HD);
     if constexpr (F32) {
 #pragma unroll
-      for (int i = 0; i < HD / 16; i++) qf[q][i] = load<f4u>((const char *)p, 4 * (16 * i + 4 * g4));
+      for (int i = 0; i < HD / 16; i++) qf[q][i] = load<f4u>(p, 4 * (16 * i + 4 * g4));
       sfac[q] = a.scale * kLog2e;
     } else {
       float x[HD / 32][8];
@@ -170,7 +250,7 @@ __global__ __launch_bounds__(kThreads) void k_attend(AttendRows a, int splits) {
 #pragma unroll
       for (int i = 0; i < HD / 32; i++) {
         const int d = Q8 ? (i >> 1) * 64 + g4 * 16 + (i & 1) * 8 : i * 32 + g4 * 8;
-        const f4 u = load<f4u>((const char *)p, 4 * d), w = load<f4u>((const char *)p, 4 * d + 16);
+        const f4 u = load<f4u>(p, 4 * d), w = load<f4u>(p, 4 * d + 16);
 #pragma unroll
         for (int e = 0; e < 4; e++) {
           x[i][e] = u[e];
@@ -184,126 +264,38 @@ __global__ __launch_bounds__(kThreads) void k_attend(AttendRows a, int splits) {
       }
       m = rows4_max(odd ? INFINITY : m);
       // m * 2^k in [2^13, 2^14); infinities and NaN stay what they are
-      int k = m > 0.f && m < INFINITY ? 14 - (ilogbf(m) + 1) : 0;
+      const int k = m > 0.f && m < INFINITY ? 13 - ilogbf(m) : 0;
 #pragma unroll
       for (int i = 0; i < HD / 32; i++)
 #pragma unroll
-        for (int e = 0; e < 4; e++)
-          split2(ldexpf(x[i][2 * e], k), ldexpf(x[i][2 * e + 1], k), qh[q][i][e], ql[q][i][e]);
-      sfac[q] = ldexpf(a.scale * kLog2e, -k);
+        for (int e = 0; e < 4; e++) {
+          uint32_t hi, lo;
+          split2(ldexpf(x[i][2 * e], k), ldexpf(x[i][2 * e + 1], k), hi, lo);
+          qh[q][i][e] = hi;
+          ql[q][i][e] = lo;
+        }
+      sfac[q] = ldexpf(a.scale * kLog2e, Q8 ? 24 - k : -k);
     }
   }
-
-  const char *kbase = s.k0 + kv_row(a.kv, s, 0, g, 0) * (HD * (F32 ? 4 : Q8 ? 1 : 2));
-  const char *vbase = s.k0 + kv_row(a.kv, s, 1, g, 0) * (HD * (F32 ? 4 : Q8 ? 1 : 2));
-  const char *ksc = nullptr, *vsc = nullptr;
-  if constexpr (Q8) {
-    ksc = reinterpret_cast<const char *>(kv_scales(a.kv, s, HD) + kv_row(a.kv, s, 0, g, 0));
-    vsc = reinterpret_cast<const char *>(kv_scales(a.kv, s, HD) + kv_row(a.kv, s, 1, g, 0));
-  }
-  constexpr int ROW = HD * (F32 ? 4 : Q8 ? 1 : 2);  // bytes
-
-  Raw<FMT, HD> raw;
-  auto load_k = [&](int tile) {
-    const int j0 = tile * T;
-#pragma unroll
-    for (int t = 0; t < NS; t++) {
-      const int64_t at = (int64_t)std::min(j0 + 16 * t + n16, last) * ROW;
-      if constexpr (F32) {
-#pragma unroll
-        for (int i = 0; i < HD / 16; i++) raw.k[i] = load<f4>(kbase, at + 64 * i + 16 * g4);
-      } else if constexpr (Q8) {
-#pragma unroll
-        for (int i = 0; i < HD / 64; i++) raw.k[t][i] = load<u4>(kbase, at + 64 * i + 16 * g4);
-      } else {
-#pragma unroll
-        for (int i = 0; i < HD / 32; i++) raw.k[t][i] = load<u4>(kbase, at + 64 * i + 16 * g4);
-      }
-    }
-    if constexpr (Q8) {
-#pragma unroll
-      for (int t = 0; t < 2; t++) {
-        const int j = j0 + 16 * t + 4 * g4;
-        if (j0 + T <= cut.end) {
-          raw.ks[t] = load<f4u>(ksc, 4 * (int64_t)j);
-        } else {
-#pragma unroll
-          for (int r = 0; r < 4; r++)
-            raw.ks[t][r] = load<float>(ksc, 4 * (int64_t)std::min(j + r, last));
-        }
-      }
-    }
-  };
-  auto load_v = [&](int tile) {
-    const int j0 = tile * T;
-#pragma unroll
-    for (int i = 0; i < (F32 ? 4 : 8); i++) {
-      const int j = j0 + (F32 ? 4 * g4 + i : (i >> 2) * 16 + 4 * g4 + (i & 3));
-      const int64_t at = (int64_t)std::min(j, last) * ROW + n16 * (ROW / 16);
-      if constexpr (F32) {
-#pragma unroll
-        for (int e = 0; e < HD / 64; e++) raw.v[i][e] = load<f4>(vbase, at + 16 * e);
-      } else if constexpr (Q8) {
-        if constexpr (HD == 128) raw.v[i] = load<u2>(vbase, at);
-        else raw.v[i / 2][i & 1] = load<uint32_t>(vbase, at);
-      } else {
-        if constexpr (HD == 128) {
-          raw.v[i] = load<u4>(vbase, at);
-        } else {
-          const u2 x = load<u2>(vbase, at);
-          raw.v[i / 2][2 * (i & 1)] = x[0];
-          raw.v[i / 2][2 * (i & 1) + 1] = x[1];
-        }
-      }
-    }
-    if constexpr (Q8) {
-#pragma unroll
-      for (int t = 0; t < 2; t++) {
-        const int j = j0 + 16 * t + 4 * g4;
-        if (j0 + T <= cut.end) {
-          raw.vs[t] = load<f4u>(vsc, 4 * (int64_t)j);
-        } else {
-#pragma unroll
-          for (int r = 0; r < 4; r++)
-            raw.vs[t][r] = load<float>(vsc, 4 * (int64_t)std::min(j + r, last));
-        }
-      }
-    }
-  };
-  // word w of the HD / 16 elements of position i of the loaded values
-  auto vword = [&](int i, int w) -> uint32_t {
-    if constexpr (FMT == Q3H_KV_F16)
-      return HD == 128 ? raw.v[i][w] : raw.v[i / 2][2 * (i & 1) + w];
-    else if constexpr (Q8)
-      return HD == 128 ? raw.v[i][w] : raw.v[i / 2][i & 1];
-    else
-      return 0;
-  };
 
   f4 acc[NQ][C];
   float m[NQ], l[NQ];
-  int ev;  // int8: the values' scales are below 2^ev so far
+  int ev = -100;  // int8: the values' scales are below 2^ev so far
   uint64_t path[NQ];
   bool broken[NQ], paths = false;
 #pragma unroll
-  for (int q = 0; q < NQ; q++) path[q] = 0, broken[q] = false;
-  // An infinity times one of the parts that a query or a weight is split in is
-  // NaN where the product itself is not. A wave that ends with a NaN goes over
-  // its positions again with care: such products one by one, in f32.
-  for (bool careful = false;; careful = true) {
-#pragma unroll
   for (int q = 0; q < NQ; q++) {
+    path[q] = 0;
+    broken[q] = false;
     m[q] = -INFINITY;
     l[q] = 0.f;
 #pragma unroll
     for (int c = 0; c < C; c++) acc[q][c] = (f4){0.f, 0.f, 0.f, 0.f};
   }
-  ev = -100;
-  int tile = tile0 + wk;
-  if (tile < tile1) {
-    load_k(tile);
-    load_v(tile);
-  }
+  // whether query tile q's row sees drafted row d (d < 0: a position before the draft)
+  auto sees = [&](int q, int d) {
+    return d < 0 || (d <= qrow[q] / per_kv && (!a.parents || (path[q] >> d & 1)));
+  };
   for (; tile < tile1; tile += WK) {
     const int j0 = tile * T;
     const bool tail = j0 + T > cut.full;
@@ -324,16 +316,16 @@ __global__ __launch_bounds__(kThreads) void k_attend(AttendRows a, int splits) {
                                                             0, 0);
     } else {
 #pragma unroll
-      for (int t = 0; t < NS; t++)
+      for (int i = 0; i < HD / 32; i++)
 #pragma unroll
-        for (int i = 0; i < HD / 32; i++) {
+        for (int t = 0; t < NS; t++) {
           u4 ka;
           if constexpr (Q8) {
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-              const uint32_t w = raw.k[t][i >> 1][2 * (i & 1) + e] ^ 0x80808080u;
-              ka[2 * e] = bytes_f16(w, 0x04010400u);
-              ka[2 * e + 1] = bytes_f16(w, 0x04030402u);
+              const uint32_t w = raw.k[t][i >> 1][2 * (i & 1) + e];
+              ka[2 * e] = bytes_f16(w, w, 0x01010000u);
+              ka[2 * e + 1] = bytes_f16(w, w, 0x03030202u);
             }
           } else {
             ka = raw.k[t][i];
@@ -341,62 +333,42 @@ __global__ __launch_bounds__(kThreads) void k_attend(AttendRows a, int splits) {
           const h8 A = __builtin_bit_cast(h8, ka);
 #pragma unroll
           for (int q = 0; q < NQ; q++) {
-            const u4 bl = {ql[q][i][0], ql[q][i][1], ql[q][i][2], ql[q][i][3]};
-            const u4 bh = {qh[q][i][0], qh[q][i][1], qh[q][i][2], qh[q][i][3]};
-            st[q][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, __builtin_bit_cast(h8, bl),
-                                                              st[q][t], 0, 0, 0);
-            st[q][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, __builtin_bit_cast(h8, bh),
-                                                              st[q][t], 0, 0, 0);
+            st[q][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                A, __builtin_bit_cast(h8, ql[q][i]), st[q][t], 0, 0, 0);
+            st[q][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                A, __builtin_bit_cast(h8, qh[q][i]), st[q][t], 0, 0, 0);
           }
         }
     }
     f4 ks[2], vs[2];
     if constexpr (Q8) {
 #pragma unroll
-      for (int t = 0; t < 2; t++) {
-        ks[t] = raw.ks[t];
-        vs[t] = raw.vs[t];
-      }
+      for (int t = 0; t < 2; t++) ks[t] = raw.ks[t];
     }
     if (tile + WK < tile1) load_k(tile + WK);
 
-    // which positions the rows see (the tile of the drafted rows and behind)
-    uint32_t sees[NQ];
-#pragma unroll
-    for (int q = 0; q < NQ; q++) sees[q] = 0xff;
-    if (tail) {
-      if (a.parents && !paths) {
-        paths = true;
-        const Path p = tree_path(a.parents + row0, a.kv.rows);
-#pragma unroll
-        for (int q = 0; q < NQ; q++) {
-          path[q] = __shfl(p.rows, qrow[q] / per_kv);
-          broken[q] = __shfl((int)p.bad, qrow[q] / per_kv) != 0;
-        }
-      }
-#pragma unroll
-      for (int q = 0; q < NQ; q++) {
-        const int t = qrow[q] / per_kv;
-        sees[q] = 0;
-#pragma unroll
-        for (int i = 0; i < 4 * NS; i++) {
-          const int d = j0 + (i >> 2) * 16 + 4 * g4 + (i & 3) - s.len;
-          const bool ok = d < 0 || (d <= t && (!a.parents || (path[q] >> d & 1)));
-          sees[q] |= (ok ? 1u : 0u) << i;
-        }
-      }
-    }
-    float vfac = 16384.f;
+    float fv = 16384.f;
     int ev_new = ev;
     if constexpr (Q8) {
       float x = 0.f;
 #pragma unroll
       for (int t = 0; t < 2; t++)
 #pragma unroll
-        for (int r = 0; r < 4; r++) x = fmaxf(x, vs[t][r]);
+        for (int r = 0; r < 4; r++) x = fmaxf(x, raw.vs[t][r]);
       x = rows4_max(x);
       ev_new = std::max(ev, (int)(__float_as_uint(x) >> 23) - 126);
-      vfac = ldexpf(1.f, 14 - ev_new);
+      fv = ldexpf(1.f, 14 - ev_new);
+#pragma unroll
+      for (int t = 0; t < 2; t++) vs[t] = raw.vs[t] * fv;
+    }
+    if (tail && a.parents && !paths) {
+      paths = true;
+      const Path p = tree_path(a.parents + row0, a.kv.rows);
+#pragma unroll
+      for (int q = 0; q < NQ; q++) {
+        path[q] = __shfl(p.rows, qrow[q] / per_kv);
+        broken[q] = __shfl((int)p.bad, qrow[q] / per_kv) != 0;
+      }
     }
     float w[NQ][4 * NS];
 #pragma unroll
@@ -404,28 +376,16 @@ __global__ __launch_bounds__(kThreads) void k_attend(AttendRows a, int splits) {
       float mx = m[q];
 #pragma unroll
       for (int i = 0; i < 4 * NS; i++) {
-        float x = st[q][i >> 2][i & 3] * sfac[q];
-        if constexpr (Q8) x *= ks[i >> 2][i & 3];
-        if (careful && x != x) {
-          const float *p = a.q + (row0 + qrow[q] / per_kv) * a.ldq +
-                           (size_t)(g * per_kv + qrow[q] % per_kv) * HD;
-          const int64_t at = (int64_t)std::min(j0 + (i >> 2) * 16 + 4 * g4 + (i & 3), last) * ROW;
-          x = 0.f;
-          for (int e = 0; e < HD; e++) {
-            float k;
-            if constexpr (F32) k = load<float>(kbase, at + 4 * e);
-            else if constexpr (Q8) k = (float)load<int8_t>(kbase, at + e);
-            else k = (float)load<_Float16>(kbase, at + 2 * e);
-            x = fmaf(p[e], k, x);
-          }
-          x *= a.scale * 1.44269504088896340736f;
-          if constexpr (Q8) x *= ks[i >> 2][i & 3];
-        }
+        float x;
+        if constexpr (Q8)
+          x = st[q][i >> 2][i & 3] * sfac[q] * ks[i >> 2][i & 3];
+        else
+          x = st[q][i >> 2][i & 3] * sfac[q];
         if (tail) {
-          x = sees[q] >> i & 1 ? x : -INFINITY;
+          const int d = j0 + (i >> 2) * 16 + 4 * g4 + (i & 3) - s.len;
+          x = sees(q, d) ? x : -INFINITY;
           // a row whose path is broken: NaN at itself, and so in all of it
-          if (broken[q] && j0 + (i >> 2) * 16 + 4 * g4 + (i & 3) - s.len == qrow[q] / per_kv)
-            x = NAN;
+          if (broken[q] && d == qrow[q] / per_kv) x = NAN;
         }
         w[q][i] = x;
         mx = fmaxf(mx, x);
@@ -445,52 +405,18 @@ __global__ __launch_bounds__(kThreads) void k_attend(AttendRows a, int splits) {
         const float p = __builtin_amdgcn_exp2f(w[q][i] - base);
         l[q] += p;
         if constexpr (Q8) {
-          w[q][i] = p * (vs[i >> 2][i & 3] * vfac);
-          if (tail) w[q][i] = sees[q] >> i & 1 ? w[q][i] : 0.f;
+          float v = vs[i >> 2][i & 3];
+          if (tail) v = sees(q, j0 + (i >> 2) * 16 + 4 * g4 + (i & 3) - s.len) ? v : 0.f;
+          w[q][i] = p * v;
         } else if constexpr (F32) {
           w[q][i] = p;
         } else {
-          w[q][i] = p * vfac;
+          w[q][i] = p * fv;
         }
       }
     }
     ev = ev_new;
 
-    // values: an infinity or NaN in a drafted row reaches only the rows that
-    // see it: such elements (and everything behind the last row) go in as 0, and
-    // are added by hand
-    bool odd = false;
-    const int guard0 = careful ? 0 : s.len;  // positions from here on are looked at
-    if constexpr (!Q8) {
-      if (tail || careful) {
-#pragma unroll
-        for (int i = 0; i < 4 * NS; i++) {
-          const int j = j0 + (i >> 2) * 16 + 4 * g4 + (i & 3);
-          if constexpr (F32) {
-#pragma unroll
-            for (int e = 0; e < C; e++)
-              if (j >= guard0) {
-                const float x = raw.v[i][e >> 2][e & 3];
-                const bool fin = fabsf(x) < INFINITY;
-                odd = odd || !fin;
-                raw.v[i][e >> 2][e & 3] = fin ? x : 0.f;
-              }
-          } else {
-#pragma unroll
-            for (int e = 0; e < C / 2; e++)
-              if (j >= guard0) {
-                const uint32_t x = vword(i, e);
-                const bool lo = (x & 0x7c00u) != 0x7c00u, hi = (x & 0x7c000000u) != 0x7c000000u;
-                odd = odd || !lo || !hi;
-                const uint32_t y = x & ((lo ? 0xffffu : 0u) | (hi ? 0xffff0000u : 0u));
-                if constexpr (HD == 128) raw.v[i][e] = y;
-                else raw.v[i / 2][2 * (i & 1) + e] = y;
-              }
-          }
-        }
-        odd = __any(odd);
-      }
-    }
     if constexpr (F32) {
 #pragma unroll
       for (int r = 0; r < 4; r++)
@@ -501,16 +427,20 @@ __global__ __launch_bounds__(kThreads) void k_attend(AttendRows a, int splits) {
             acc[q][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(raw.v[r][c >> 2][c & 3], w[q][r],
                                                              acc[q][c], 0, 0, 0);
     } else {
-      u4 ph[NQ], pl[NQ];
+      h8 ph[NQ], pl[NQ];
 #pragma unroll
-      for (int q = 0; q < NQ; q++)
+      for (int q = 0; q < NQ; q++) {
+        u4 hi4, lo4;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
           uint32_t hi, lo;
           split2(w[q][2 * e], w[q][2 * e + 1], hi, lo);
-          ph[q][e] = hi;
-          pl[q][e] = lo;
+          hi4[e] = hi;
+          lo4[e] = lo;
         }
+        ph[q] = __builtin_bit_cast(h8, hi4);
+        pl[q] = __builtin_bit_cast(h8, lo4);
+      }
 #pragma unroll
       for (int c = 0; c < C; c++) {
         u4 va;
@@ -518,10 +448,8 @@ __global__ __launch_bounds__(kThreads) void k_attend(AttendRows a, int splits) {
         for (int e = 0; e < 4; e++) {
           if constexpr (Q8) {
             // bytes c of positions 2e and 2e + 1
-            const uint32_t x = vword(2 * e, c >> 2), y = vword(2 * e + 1, c >> 2);
-            const uint32_t sel = 0x0c0c0000u | ((4u + (c & 3)) << 8) | (c & 3);
-            const uint32_t z = __builtin_amdgcn_perm(y, x, sel) ^ 0x00008080u;
-            va[e] = bytes_f16(z, 0x04010400u);
+            va[e] = bytes_f16(vword(2 * e + 1, c >> 2), vword(2 * e, c >> 2),
+                              0x04040000u + 0x01010101u * (c & 3));
           } else {
             const uint32_t x = vword(2 * e, c >> 1), y = vword(2 * e + 1, c >> 1);
             va[e] = __builtin_amdgcn_perm(y, x, c & 1 ? 0x07060302u : 0x05040100u);
@@ -530,69 +458,86 @@ __global__ __launch_bounds__(kThreads) void k_attend(AttendRows a, int splits) {
         const h8 A = __builtin_bit_cast(h8, va);
 #pragma unroll
         for (int q = 0; q < NQ; q++) {
-          acc[q][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, __builtin_bit_cast(h8, pl[q]),
-                                                             acc[q][c], 0, 0, 0);
-          acc[q][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, __builtin_bit_cast(h8, ph[q]),
-                                                             acc[q][c], 0, 0, 0);
-        }
-      }
-    }
-    if constexpr (!Q8) {
-      if (odd) {
-        // weights of the tile by query, negative where the row does not see it
-#pragma unroll
-        for (int q = 0; q < NQ; q++)
-#pragma unroll
-          for (int i = 0; i < 4 * NS; i++)
-            sm_w[wave][q * 16 + n16][(i >> 2) * 16 + 4 * g4 + (i & 3)] =
-                sees[q] >> i & 1 ? w[q][i] : -1.f;
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        for (int j = std::max(j0, guard0); j <= std::min(j0 + T - 1, last); j++) {
-#pragma unroll
-          for (int c = 0; c < C; c++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-              const int e = C * (4 * g4 + r) + c;
-              float x;
-              if constexpr (F32) x = load<float>(vbase, (int64_t)j * ROW + 4 * e);
-              else x = (float)load<_Float16>(vbase, (int64_t)j * ROW + 2 * e);
-              if (fabsf(x) < INFINITY) continue;
-#pragma unroll
-              for (int q = 0; q < NQ; q++) {
-                const float p = sm_w[wave][q * 16 + n16][j - j0];
-                if (!(p < 0.f)) acc[q][c][r] += p * x;
-              }
-            }
+          acc[q][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, pl[q], acc[q][c], 0, 0, 0);
+          acc[q][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, ph[q], acc[q][c], 0, 0, 0);
         }
       }
     }
     if (tile + WK < tile1) load_v(tile + WK);
   }
-  if (careful) break;
+
+  // out of the weights' scale
   bool nan = false;
 #pragma unroll
   for (int q = 0; q < NQ; q++) {
-    nan = nan || l[q] != l[q];
+    const float f = F32 ? 1.f : Q8 ? ldexpf(0x1p24f, ev - 14) : 1.f / 16384.f;
+    l[q] = rows4_sum(l[q]);
+    nan = nan || (l[q] != l[q] && !broken[q]);
 #pragma unroll
     for (int c = 0; c < C; c++)
 #pragma unroll
-      for (int r = 0; r < 4; r++) nan = nan || acc[q][c][r] != acc[q][c][r];
+      for (int r = 0; r < 4; r++) {
+        acc[q][c][r] *= f;
+        nan = nan || (acc[q][c][r] != acc[q][c][r] && !broken[q]);
+      }
   }
-  if (!__any(nan)) break;
+  // An infinity times one of the parts that a query or a weight is split in is
+  // NaN where the product itself is not, and so is an infinity that a row does
+  // not see times its weight 0. A wave that ends with a NaN goes over its
+  // positions again one by one, each lane on its query and its HD / 4 elements.
+  if (__any(nan)) {
+#pragma unroll
+    for (int q = 0; q < NQ; q++) {
+      const float *p = a.q + (row0 + qrow[q] / per_kv) * a.ldq +
+                       (size_t)(g * per_kv + qrow[q] % per_kv) * HD + C * 4 * g4;
+      float ms = -INFINITY, ls = 0.f;
+#pragma unroll
+      for (int c = 0; c < C; c++) acc[q][c] = (f4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+      for (int at = tile0 + wk; at < tile1; at += WK)
+#pragma unroll 1
+        for (int j = at * T; j < std::min(at * T + T, cut.end); j++) {
+          const float kd = Q8 ? load<float>(ksc, 4 * (int64_t)j) : 1.f;
+          const float vd = Q8 ? load<float>(vsc, 4 * (int64_t)j) : 1.f;
+          auto value = [&](const char *base, int e) {
+            const int64_t off = (int64_t)j * ROW;
+            if constexpr (F32) return load<float>(base, off + 4 * e);
+            else if constexpr (Q8) return kv_byte(load<uint8_t>(base, off + e));
+            else return (float)load<_Float16>(base, off + 2 * e);
+          };
+          float x = 0.f;
+#pragma unroll 1
+          for (int e = 0; e < HD / 4; e++) x = fmaf(p[e], value(kbase, C * 4 * g4 + e), x);
+          x = rows4_sum(x) * kd * a.scale * kLog2e;
+          if (!sees(q, j - s.len)) continue;
+          if (broken[q]) x = NAN;
+          const float mn = fmaxf(ms, x), base = mn == -INFINITY ? 0.f : mn;
+          const float f = __builtin_amdgcn_exp2f(ms - base), w = __builtin_amdgcn_exp2f(x - base);
+          ls = fmaf(ls, f, w);
+#pragma unroll
+          for (int c = 0; c < C; c++)
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+              acc[q][c][r] = fmaf(acc[q][c][r], f, w * (value(vbase, C * (4 * g4 + r) + c) * vd));
+          ms = mn;
+        }
+      m[q] = ms;
+      l[q] = ls;
+    }
   }
 
   // the waves over the positions together
   constexpr int Q16 = NQ * 16;
+  if constexpr (WK > 1) {
+    if (g4 == 0) {
 #pragma unroll
-  for (int q = 0; q < NQ; q++) {
-    l[q] = rows4_sum(l[q]);
-    if (WK > 1 && g4 == 0) {
-      sm_m[wave][q * 16 + n16] = m[q];
-      sm_l[wave][q * 16 + n16] = l[q];
+      for (int q = 0; q < NQ; q++) {
+        sm_m[wave][q * 16 + n16] = m[q];
+        sm_l[wave][q * 16 + n16] = l[q];
+      }
     }
+    __syncthreads();
   }
-  if (WK > 1) __syncthreads();
   float *part = a.part;
   const size_t part_rows = (size_t)a.kv.rows * per_kv;
   const size_t part0 = ((size_t)(b * a.kv.kvh + g) * splits + split) * part_rows;
@@ -610,19 +555,16 @@ __global__ __launch_bounds__(kThreads) void k_attend(AttendRows a, int splits) {
              __builtin_amdgcn_exp2f(sm_m[i * WQ + wq][q * 16 + n16] - base);
       f = __builtin_amdgcn_exp2f(m[q] - base);
     }
-    // out of the weights' scale; with one split also the softmax's sum
-    if constexpr (Q8) f = ldexpf(f, ev - 14);
-    else if constexpr (!F32) f *= 1.f / 16384.f;
-    if (splits == 1) f /= L;
+    if (splits == 1) f /= L;  // the softmax's sum
     if (splits > 1 && wk == 0 && g4 == 0 && live[q]) {
       part_ml[2 * (part0 + qrow[q])] = M;
       part_ml[2 * (part0 + qrow[q]) + 1] = L;
     }
     if constexpr (WK > 1) {
 #pragma unroll
-      for (int c = 0; c < C; c++)
+      for (int r = 0; r < 4; r++)
 #pragma unroll
-        for (int r = 0; r < 4; r++)
+        for (int c = 0; c < C; c++)
           sm_acc[(wave * Q16 + q * 16 + n16) * HD + C * (4 * g4 + r) + c] = acc[q][c][r] * f;
     } else if (live[q]) {
       float *o = splits > 1 ? part + (part0 + qrow[q]) * HD
