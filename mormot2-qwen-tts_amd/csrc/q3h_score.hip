@@ -13,113 +13,273 @@ namespace q3h {
 
 namespace {
 
+constexpr int kMaxVocab = 1 << 20;
+
 constexpr int kThreads = 256, kWaves = kThreads / 64;
+constexpr float kLog2e = 1.44269504088896340736f;
 
-template <bool BF16>
-__device__ __forceinline__ float logit(const void *p, size_t i) {
-  if constexpr (BF16)
-    return __uint_as_float((uint32_t) static_cast<const uint16_t *>(p)[i] << 16);
-  else
-    return static_cast<const float *>(p)[i];
+// A logit and its token as one number that orders them from the top: larger
+// logits first, of equal ones (0 and -0 among them) the lower token, NaN last.
+// Never 0, and no two alike.
+__device__ __forceinline__ uint64_t top_key(float x, int i) {
+  const uint32_t b = __float_as_uint(x + 0.f);
+  const uint32_t v = x != x ? 1u : b & 0x80000000u ? ~b : b | 0x80000000u;
+  return (uint64_t)v << 32 | (uint32_t)~i;
 }
-
-// whether (x, i) comes before (y, j) from the top: larger first, of equal ones
-// the lower token, NaN last (among themselves by token)
-__device__ __forceinline__ bool before(float x, int i, float y, int j) {
-  const bool nx = x != x, ny = y != y;
-  if (nx != ny) return ny;
-  if (!nx && x != y) return x > y;
-  return i < j;
+__device__ __forceinline__ float key_logit(uint64_t k) {
+  const uint32_t v = (uint32_t)(k >> 32);
+  if (v == 1u) return NAN;
+  return __uint_as_float(v & 0x80000000u ? v & 0x7fffffffu : ~v);
 }
+__device__ __forceinline__ int key_token(uint64_t k) { return (int)~(uint32_t)k; }
 
-// One workgroup per row: the maximum, then the sums of e^(x - max) and of
-// (x - max) e^(x - max), then the top tokens one by one.
-template <bool BF16>
-__global__ __launch_bounds__(kThreads) void k_score(ScoreRows a) {
-  __shared__ float rv[kWaves], rs[kWaves], rt[kWaves];
-  __shared__ int ri[kWaves];
-  const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const void *x = static_cast<const char *>(a.logits) + (size_t)r * a.ld * (BF16 ? 2 : 4);
-  float m = -INFINITY;
-  for (int i = tid; i < a.vocab; i += kThreads) m = fmaxf(m, logit<BF16>(x, i));
-  m = wave_max_dpp(m);
-  if (lane == 0) rv[wave] = m;
-  __syncthreads();
-  for (int i = 0; i < kWaves; i++) m = fmaxf(m, rv[i]);
-  float s = 0.f, u = 0.f;
-  for (int i = tid; i < a.vocab; i += kThreads) {
-    const float d = logit<BF16>(x, i) - m, e = expf(d);
-    s += e;
-    if (e != 0.f) u += d * e;
-  }
-  s = wave_sum_dpp(s);
-  u = wave_sum_dpp(u);
-  if (lane == 0) {
-    rs[wave] = s;
-    rt[wave] = u;
+// The k largest of the workgroup's keys (at most E a thread, key(e); 0: none),
+// k <= 64: the k-th largest of the threads' own maxima is not above the k-th
+// largest key, and only k threads hold keys from it on, so at most k E keys are
+// left; each of those counts the ones above it. emit(rank, key) once for
+// every rank below min(k, keys).
+template <int E>
+struct TopSpace {
+  uint64_t top[kThreads];
+  uint64_t list[Q3H_TOP_MAX * E];
+  uint64_t bound;
+  int n;
+};
+template <int E, class Key, class Emit>
+__device__ __forceinline__ void block_top(TopSpace<E> &sm, int k, Key &&key, Emit &&emit) {
+  const int tid = threadIdx.x;
+  uint64_t best = 0;
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    const uint64_t x = key(e);
+    best = x > best ? x : best;
   }
   __syncthreads();
-  s = u = 0.f;
-  for (int i = 0; i < kWaves; i++) {
-    s += rs[i];
-    u += rt[i];
+  sm.top[tid] = best;
+  if (tid == 0) {
+    sm.n = 0;
+    sm.bound = 1;
   }
-  const float ls = logf(s);
-  for (int i = tid; i < a.tokens_per_row; i += kThreads) {
-    const int t = a.tokens[(size_t)r * a.tokens_per_row + i];
-    a.logprobs[(size_t)r * a.tokens_per_row + i] =
-        t >= 0 && t < a.vocab ? logit<BF16>(x, t) - m - ls : NAN;
-  }
-  if (tid == 0 && a.entropy) a.entropy[r] = ls - u / s;
-  float lv = 0.f;
-  int li = -1;
-  for (int k = 0; k < a.top_k; k++) {
-    float bv = NAN;
-    int bi = INT32_MAX;
-    for (int i = tid; i < a.vocab; i += kThreads) {
-      const float v = logit<BF16>(x, i);
-      if ((li < 0 || before(lv, li, v, i)) && before(v, i, bv, bi)) {
-        bv = v;
-        bi = i;
-      }
-    }
-    for (int o = 32; o > 0; o >>= 1) {
-      const float v2 = __shfl_xor(bv, o);
-      const int i2 = __shfl_xor(bi, o);
-      if (before(v2, i2, bv, bi)) {
-        bv = v2;
-        bi = i2;
-      }
-    }
-    __syncthreads();
-    if (lane == 0) {
-      rv[wave] = bv;
-      ri[wave] = bi;
-    }
-    __syncthreads();
-    lv = rv[0];
-    li = ri[0];
-    for (int i = 1; i < kWaves; i++)
-      if (before(rv[i], ri[i], lv, li)) {
-        lv = rv[i];
-        li = ri[i];
-      }
-    if (tid == 0) {
-      a.top_ids[(size_t)r * a.top_k + k] = li;
-      a.top_logprobs[(size_t)r * a.top_k + k] = lv - m - ls;
+  __syncthreads();
+  int above = 0;
+#pragma unroll 16
+  for (int i = 0; i < kThreads; i++) above += sm.top[i] > best;
+  if (best && above == k - 1) sm.bound = best;  // (one thread at most: no two keys alike)
+  __syncthreads();
+  const uint64_t bound = sm.bound;
+  if (best >= bound) {
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      const uint64_t x = key(e);
+      if (x >= bound) sm.list[atomicAdd(&sm.n, 1)] = x;
     }
   }
+  __syncthreads();
+  const int n = sm.n;
+  for (int c = tid; c < n; c += kThreads) {
+    const uint64_t x = sm.list[c];
+    int rank = 0;
+    for (int i = 0; i < n; i++) rank += sm.list[i] > x;
+    if (rank < k) emit(rank, x);
+  }
+}
+
+// A row's sums: the maximum, and over the logits' distances d from it the sums
+// of e^d and of d e^d.
+struct Sums {
+  float m, s, u;
+};
+
+// what a row's sums and top tokens come to
+__device__ __forceinline__ void finish_row(const ScoreRows &a, int r, const Sums &t, float ls) {
+  for (int i = threadIdx.x; i < a.tokens_per_row; i += kThreads) {
+    const int c = a.tokens[(size_t)r * a.tokens_per_row + i];
+    float v = NAN;
+    if (c >= 0 && c < a.vocab) {
+      const size_t at = (size_t)r * a.ld + c;
+      const float x =
+          a.bf16 ? __uint_as_float((uint32_t) static_cast<const uint16_t *>(a.logits)[at] << 16)
+                 : static_cast<const float *>(a.logits)[at];
+      v = x - t.m - ls;
+    }
+    a.logprobs[(size_t)r * a.tokens_per_row + i] = v;
+  }
+  if (threadIdx.x == 0 && a.entropy) a.entropy[r] = ls - t.u / t.s;
+}
+
+// what a split of a row leaves for the merge: its sums, then top_k keys (0: none)
+struct Space {
+  Sums *sums;      // [rows][splits]
+  uint64_t *keys;  // [rows][splits][top_k]
+};
+__host__ __device__ __forceinline__ size_t sums_bytes(int rows, int splits) {
+  return ((size_t)rows * splits * sizeof(Sums) + 255) / 256 * 256;
+}
+__device__ __forceinline__ Space space_of(const ScoreRows &a, int splits) {
+  Space s;
+  s.sums = static_cast<Sums *>(a.work);
+  s.keys = reinterpret_cast<uint64_t *>(static_cast<char *>(a.work) + sums_bytes(a.rows, splits));
+  return s;
+}
+
+// One workgroup per (row, split of kThreads * E logits), the logits read once,
+// 16 bytes a load, and kept in registers: the maximum, the sums, the top. Loads
+// are at 16-byte boundaries whatever the row's: the row begins `skew` elements
+// into its first.
+template <bool BF16, int E>
+__global__ __launch_bounds__(kThreads) void k_score(ScoreRows a, int splits) {
+  constexpr int VEC = BF16 ? 8 : 4, SIZE = BF16 ? 2 : 4;
+  __shared__ TopSpace<E> sm;
+  __shared__ float red[3][kWaves];
+  const int r = blockIdx.x / splits, split = blockIdx.x - r * splits, tid = threadIdx.x;
+  const char *row = static_cast<const char *>(a.logits) + (size_t)r * a.ld * SIZE;
+  const int skew = (int)(reinterpret_cast<uintptr_t>(row) & 15) / SIZE;
+  const int first = split * kThreads * E - skew + tid * VEC;  // the thread's first token
+  float x[E];
+  typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+  for (int v = 0; v < E / VEC; v++) {
+    const int i = first + v * kThreads * VEC;
+    float *y = x + v * VEC;
+    if (i >= 0 && i + VEC <= a.vocab) {
+      const u4 w = *reinterpret_cast<const u4 *>(row + (int64_t)i * SIZE);
+#pragma unroll
+      for (int e = 0; e < VEC; e++)
+        y[e] = __uint_as_float(!BF16 ? w[e] : e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; e++) {
+        y[e] = -INFINITY;
+        if (i + e >= 0 && i + e < a.vocab)
+          y[e] = BF16 ? __uint_as_float((uint32_t) reinterpret_cast<const uint16_t *>(row)[i + e]
+                                        << 16)
+                      : reinterpret_cast<const float *>(row)[i + e];
+      }
+    }
+  }
+  Sums t;
+  t.m = -INFINITY;
+#pragma unroll
+  for (int e = 0; e < E; e++) t.m = fmaxf(t.m, x[e]);
+  t.m = wave_max_dpp(t.m);
+  if ((tid & 63) == 0) red[0][tid >> 6] = t.m;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kWaves; i++) t.m = fmaxf(t.m, red[0][i]);
+  const float base = t.m == -INFINITY ? 0.f : t.m;
+  t.s = t.u = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    const float d = x[e] - base, w = __builtin_amdgcn_exp2f(d * kLog2e);
+    t.s += w;
+    t.u += w != 0.f ? d * w : 0.f;
+  }
+  t.s = wave_sum_dpp(t.s);
+  t.u = wave_sum_dpp(t.u);
+  if ((tid & 63) == 0) {
+    red[1][tid >> 6] = t.s;
+    red[2][tid >> 6] = t.u;
+  }
+  __syncthreads();
+  t.s = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+  t.u = (red[2][0] + red[2][1]) + (red[2][2] + red[2][3]);
+  const Space out = space_of(a, splits);
+  const float ls = logf(t.s);
+  if (splits == 1) finish_row(a, r, t, ls);
+  else if (tid == 0) out.sums[blockIdx.x] = t;
+  if (a.top_k == 0) return;
+  uint64_t *keys = out.keys + (size_t)blockIdx.x * a.top_k;
+  if (splits > 1 && tid < a.top_k && tid >= a.vocab - (split * kThreads * E - skew)) keys[tid] = 0;
+  block_top<E>(
+      sm, a.top_k,
+      [&](int e) -> uint64_t {
+        const int i = first + e / VEC * kThreads * VEC + e % VEC;
+        return i >= 0 && i < a.vocab ? top_key(x[e], i) : 0;
+      },
+      [&](int rank, uint64_t k) {
+        if (splits == 1) {
+          a.top_ids[(size_t)r * a.top_k + rank] = key_token(k);
+          a.top_logprobs[(size_t)r * a.top_k + rank] = key_logit(k) - t.m - ls;
+        } else {
+          keys[rank] = k;
+        }
+      });
+}
+
+// the splits of a row together
+constexpr int kMergeKeys = 32;  // a thread
+__global__ __launch_bounds__(kThreads) void k_score_merge(ScoreRows a, int splits) {
+  __shared__ TopSpace<kMergeKeys> sm;
+  const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  const Space in = space_of(a, splits);
+  const Sums *sums = in.sums + (size_t)r * splits;
+  Sums t{-INFINITY, 0.f, 0.f};
+  for (int i = lane; i < splits; i += 64) t.m = fmaxf(t.m, sums[i].m);
+  t.m = wave_max_dpp(t.m);
+  const float base = t.m == -INFINITY ? 0.f : t.m;
+  for (int i = lane; i < splits; i += 64) {
+    const Sums p = sums[i];
+    const float d = p.m - base, f = __builtin_amdgcn_exp2f(d * kLog2e);
+    if (p.s != 0.f) {  // (none: logits of -infinity alone)
+      t.s += f * p.s;
+      if (f != 0.f) t.u += f * (p.u + d * p.s);
+    }
+  }
+  t.s = wave_sum_dpp(t.s);
+  t.u = wave_sum_dpp(t.u);
+  const float ls = logf(t.s);
+  finish_row(a, r, t, ls);
+  if (a.top_k == 0) return;
+  const int n = splits * a.top_k;
+  const uint64_t *keys = in.keys + (size_t)r * n;
+  uint64_t mine[kMergeKeys];
+#pragma unroll
+  for (int e = 0; e < kMergeKeys; e++)
+    mine[e] = e * kThreads + tid < n ? keys[e * kThreads + tid] : 0;
+  block_top<kMergeKeys>(
+      sm, a.top_k, [&](int e) { return mine[e]; },
+      [&](int rank, uint64_t k) {
+        a.top_ids[(size_t)r * a.top_k + rank] = key_token(k);
+        a.top_logprobs[(size_t)r * a.top_k + rank] = key_logit(k) - t.m - ls;
+      });
+}
+
+// Logits a thread: as few as cover the row with one workgroup, at most 40 (the
+// registers of two workgroups a SIMD). A row that does not begin at a 16-byte
+// boundary takes up to 7 more.
+int score_width(int vocab) {
+  return vocab + 7 <= kThreads * 8 ? 8 : vocab + 7 <= kThreads * 16 ? 16 : 40;
+}
+int score_splits(int vocab) {
+  const int per = kThreads * score_width(vocab);
+  return (vocab + 7 + per - 1) / per;
+}
+static_assert((kMaxVocab + 7 + kThreads * 40 - 1) / (kThreads * 40) * Q3H_TOP_MAX <=
+                  kMergeKeys * kThreads,
+              "the merge holds every split's keys");
+
+template <bool BF16>
+void launch(const ScoreRows &a, hipStream_t st) {
+  const int splits = score_splits(a.vocab), width = score_width(a.vocab);
+  const dim3 grid((unsigned)((int64_t)a.rows * splits));
+  if (width == 8) hipLaunchKernelGGL((k_score<BF16, 8>), grid, dim3(kThreads), 0, st, a, splits);
+  else if (width == 16) hipLaunchKernelGGL((k_score<BF16, 16>), grid, dim3(kThreads), 0, st, a, splits);
+  else hipLaunchKernelGGL((k_score<BF16, 40>), grid, dim3(kThreads), 0, st, a, splits);
+  if (splits > 1)
+    hipLaunchKernelGGL(k_score_merge, dim3(a.rows), dim3(kThreads), 0, st, a, splits);
 }
 
 }  // namespace
 
-size_t score_work_bytes(int, int, int) { return 0; }
+size_t score_work_bytes(int rows, int vocab, int top_k) {
+  const int splits = score_splits(vocab);
+  if (splits == 1) return 0;
+  return sums_bytes(rows, splits) + (size_t)rows * splits * top_k * sizeof(uint64_t);
+}
 
 void launch_token_scores(const ScoreRows &a, hipStream_t st) {
-  if (a.bf16)
-    hipLaunchKernelGGL(k_score<true>, dim3(a.rows), dim3(kThreads), 0, st, a);
-  else
-    hipLaunchKernelGGL(k_score<false>, dim3(a.rows), dim3(kThreads), 0, st, a);
+  if (a.bf16) launch<true>(a, st);
+  else launch<false>(a, st);
 }
 
 }  // namespace q3h
@@ -129,7 +289,7 @@ using namespace q3h;
 extern "C" int64_t q3h_token_logprobs_workspace(int rows, int vocab, int top_k) {
   int64_t bytes = 0;
   const int rc = guard([&] {
-    require(rows >= 0 && vocab > 0 && top_k >= 0 && top_k <= Q3H_TOP_MAX && top_k <= vocab,
+    require(rows >= 0 && vocab > 0 && vocab <= kMaxVocab && top_k >= 0 && top_k <= Q3H_TOP_MAX && top_k <= vocab,
             Q3H_E_ARG, "q3h_token_logprobs_workspace: invalid argument");
     if (rows > 0) bytes = (int64_t)score_work_bytes(rows, vocab, top_k);
   });
@@ -139,8 +299,8 @@ extern "C" int64_t q3h_token_logprobs_workspace(int rows, int vocab, int top_k) 
 extern "C" int q3h_token_logprobs(q3h_device *dev, const q3h_score_args *p, void *stream) {
   return guard([&] {
     require(dev && p, Q3H_E_ARG, "q3h_token_logprobs: NULL argument");
-    require(p->rows >= 0 && p->vocab > 0 && p->vocab <= (1 << 30), Q3H_E_ARG,
-            "q3h_token_logprobs: bad rows or vocab");
+    require(p->rows >= 0 && p->vocab > 0 && p->vocab <= kMaxVocab, Q3H_E_ARG,
+            "q3h_token_logprobs: rows must not be negative, vocab in [1, 2^20]");
     require(p->dtype == Q3H_F32 || p->dtype == Q3H_BF16, Q3H_E_ARG,
             "q3h_token_logprobs: dtype must be Q3H_F32 or Q3H_BF16");
     require(p->tokens_per_row >= 0, Q3H_E_ARG, "q3h_token_logprobs: negative tokens_per_row");
@@ -149,6 +309,10 @@ extern "C" int q3h_token_logprobs(q3h_device *dev, const q3h_score_args *p, void
                 ")]");
     if (p->rows == 0) return;
     require(p->logits != nullptr, Q3H_E_ARG, "q3h_token_logprobs: NULL logits");
+    require((uintptr_t)p->logits % (p->dtype == Q3H_BF16 ? 2 : 4) == 0, Q3H_E_ARG,
+            "q3h_token_logprobs: logits between elements");
+    require((int64_t)p->rows * 128 <= INT32_MAX, Q3H_E_CAPACITY,
+            "q3h_token_logprobs: too many rows");
     require(p->ld >= p->vocab, Q3H_E_ARG, "q3h_token_logprobs: rows overlap (ld below vocab)");
     require(p->tokens_per_row == 0 || (p->tokens && p->logprobs), Q3H_E_ARG,
             "q3h_token_logprobs: NULL tokens or logprobs");
