@@ -44,14 +44,31 @@ __device__ __forceinline__ float head_max(float v) {
   return half_max_dpp(v);
 }
 
+typedef float f2u __attribute__((ext_vector_type(2), aligned(4)));
+
+// rint(x / d) for the bytes of a row: the quotient by the reciprocal, by the
+// division itself where a reciprocal's error could cross a half
+__device__ __forceinline__ int byte_of(float x, float d, double inv) {
+  double y = (double)x * inv, q = rint(y);
+  if (fabs(y - q) > 0.5 - 1e-6) q = rint((double)x / (double)d);
+  const int v = min(127, max(-127, (int)q));
+  return v < 0 ? 128 - v : v;
+}
+
 // One head of one row per HD / 2 lanes, a pair of elements each: those that
-// turn together, or two neighbours of the part that does not turn. Everything
-// up to the f32 row is in 64 bits, so that a byte of the int8 format is that of
-// the definition and not of a rounding before it.
+// turn together, or two neighbours of the part that does not turn. A wave takes
+// kHeads heads of a row at a time (their loads and sums side by side, one
+// square root and division for all of them) and goes over the row's heads with
+// the same turning angles. Everything up to the f32 row is in 64 bits, so that a
+// byte of the int8 format is that of the definition and not of a rounding
+// before it.
+constexpr int kHeads = 4;
 template <int FMT, int HD>
 __global__ __launch_bounds__(kThreads) void k_cache_append(AppendRows a) {
-  constexpr int G = HD / 2;
-  const int lane = threadIdx.x & 63, sub = lane & (G - 1);
+  constexpr int G = HD / 2, SIDE = 64 / G;  // lanes of a head, heads side by side
+  constexpr int PER = kHeads * SIDE;        // heads of a wave at a time
+  const int lane = threadIdx.x & 63, sub = lane & (G - 1), side = lane / G;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int row = blockIdx.x, b = row / a.kv.rows, t = row - b * a.kv.rows;
   const KvSeq s = kv_sequence(a.kv, b);
   if (t >= s.count) return;
@@ -62,7 +79,7 @@ __global__ __launch_bounds__(kThreads) void k_cache_append(AppendRows a) {
     depth = __shfl(path.depth, t);
     bad = bad || __shfl((int)path.bad, t) != 0;
   }
-  const int kvh = a.kv.kvh, all = a.heads + 2 * kvh;
+  const int kvh = a.kv.kvh, turned = a.heads + kvh;
   const int half = a.rot_dim >> 1;
   const bool turns = a.table && sub < half;
   int e0 = 2 * sub, e1 = e0 + 1;
@@ -72,61 +89,113 @@ __global__ __launch_bounds__(kThreads) void k_cache_append(AppendRows a) {
   }
   double2 cs = make_double2(1.0, 0.0);
   if (turns && !bad) cs = a.table[(size_t)(s.len + depth) * half + sub];
-  const int waves = gridDim.y * (kThreads / 64) * (64 / G);
-  for (int j = (blockIdx.y * (kThreads / 64) + (threadIdx.x >> 6)) * (64 / G) + lane / G; j < all;
-       j += waves) {
-    const int part = j < a.heads ? 0 : j < a.heads + kvh ? 1 : 2;
-    const int g = part == 0 ? j : part == 1 ? j - a.heads : j - a.heads - kvh;
-    const float *src = part == 0   ? a.q + (size_t)row * a.ldq
-                       : part == 1 ? a.k + (size_t)row * a.ldk
-                                   : a.v + (size_t)row * a.ldv;
-    float x0 = src[(size_t)g * HD + e0], x1 = src[(size_t)g * HD + e1];
-    const float *w = part == 0 ? a.q_norm : part == 1 ? a.k_norm : nullptr;
-    if (part < 2) {
-      double y0 = x0, y1 = x1;
-      if (w) {
-        const double ss = head_sum<G>(y0 * y0 + y1 * y1);
-        const double inv = 1.0 / sqrt(ss / HD + (double)a.eps);
-        y0 = y0 * inv * (double)w[e0];
-        y1 = y1 * inv * (double)w[e1];
+  const float *src_q = a.q + (size_t)row * a.ldq, *src_k = a.k + (size_t)row * a.ldk,
+              *src_v = a.v + (size_t)row * a.ldv;
+  const int groups = (turned + PER - 1) / PER, all = groups + (kvh + PER - 1) / PER;
+  for (int group = blockIdx.y * (kThreads / 64) + wave; group < all;
+       group += gridDim.y * (kThreads / 64)) {
+    const bool values = group >= groups;
+    const int first = (values ? group - groups : group) * PER + side;
+    const int heads = values ? kvh : turned;
+    float x0[kHeads], x1[kHeads];
+#pragma unroll
+    for (int u = 0; u < kHeads; u++) {
+      const int j = min(first + u * SIDE, heads - 1);
+      const float *p = values ? src_v + (size_t)j * HD
+                       : j < a.heads ? src_q + (size_t)j * HD
+                                     : src_k + (size_t)(j - a.heads) * HD;
+      if (values) {
+        const f2u w = *reinterpret_cast<const f2u *>(p + 2 * sub);
+        x0[u] = w[0];
+        x1[u] = w[1];
+      } else {
+        x0[u] = p[e0];
+        x1[u] = p[e1];
       }
-      if (turns) {
-        const double r0 = y0 * cs.x - y1 * cs.y;
-        y1 = y1 * cs.x + y0 * cs.y;
-        y0 = r0;
+    }
+    if (!values) {
+      double y0[kHeads], y1[kHeads];
+#pragma unroll
+      for (int u = 0; u < kHeads; u++) y0[u] = x0[u], y1[u] = x1[u];
+      if (a.q_norm || a.k_norm) {
+        double ss[kHeads];
+#pragma unroll
+        for (int u = 0; u < kHeads; u++) ss[u] = head_sum<G>(y0[u] * y0[u] + y1[u] * y1[u]);
+        // lane u of a head does the u-th one's root
+        double mine = ss[0];
+#pragma unroll
+        for (int u = 1; u < kHeads; u++) mine = sub == u ? ss[u] : mine;
+        const double inv = 1.0 / sqrt(mine / HD + (double)a.eps);
+#pragma unroll
+        for (int u = 0; u < kHeads; u++) {
+          const double f = __shfl(inv, side * G + u);
+          const float *w = min(first + u * SIDE, heads - 1) < a.heads ? a.q_norm : a.k_norm;
+          if (w) {
+            y0[u] = y0[u] * f * (double)w[e0];
+            y1[u] = y1[u] * f * (double)w[e1];
+          }
+        }
       }
-      x0 = (float)y0;
-      x1 = (float)y1;
+#pragma unroll
+      for (int u = 0; u < kHeads; u++) {
+        if (turns) {
+          const double r0 = y0[u] * cs.x - y1[u] * cs.y;
+          y1[u] = y1[u] * cs.x + y0[u] * cs.y;
+          y0[u] = r0;
+        }
+        x0[u] = (float)y0[u];
+        x1[u] = (float)y1[u];
+      }
     }
-    if (part == 0) {
-      float *o = a.q_out + (size_t)row * a.ld_out + (size_t)g * HD;
-      o[e0] = bad ? NAN : x0;
-      o[e1] = bad ? NAN : x1;
-      continue;
-    }
-    if (bad) continue;
-    const int64_t at = kv_row(a.kv, s, part - 1, g, s.len + t);
+    // the int8 format: the heads' scales
+    float d[kHeads] = {};
+    double inv[kHeads] = {};
     if constexpr (FMT == Q3H_KV_Q8) {
-      // (fmaxf drops a NaN: it is found by its comparison)
-      const bool finite = fabsf(x0) < INFINITY && fabsf(x1) < INFINITY;
-      const float m = head_max<G>(finite ? fmaxf(fabsf(x0), fabsf(x1)) : INFINITY);
-      float d = (float)((double)m / 127.0);
-      int q0 = 0, q1 = 0;
-      if (m == INFINITY) {
-        d = NAN;
-      } else if (d > 0.f) {
-        q0 = min(127, max(-127, (int)rint((double)x0 / (double)d)));
-        q1 = min(127, max(-127, (int)rint((double)x1 / (double)d)));
+      if (values || first + (kHeads - 1) * SIDE >= a.heads) {
+        float m[kHeads];
+#pragma unroll
+        for (int u = 0; u < kHeads; u++) {
+          // (fmaxf drops a NaN: it is found by its comparison)
+          const bool finite = fabsf(x0[u]) < INFINITY && fabsf(x1[u]) < INFINITY;
+          m[u] = head_max<G>(finite ? fmaxf(fabsf(x0[u]), fabsf(x1[u])) : INFINITY);
+        }
+        float mine = m[0];
+#pragma unroll
+        for (int u = 1; u < kHeads; u++) mine = sub == u ? m[u] : mine;
+        const float dm = (float)((double)mine / 127.0);
+        const double im = 1.0 / (double)dm;
+#pragma unroll
+        for (int u = 0; u < kHeads; u++) {
+          d[u] = m[u] == INFINITY ? NAN : __shfl(dm, side * G + u);
+          inv[u] = __shfl(im, side * G + u);
+        }
       }
-      uint8_t *o = reinterpret_cast<uint8_t *>(s.k0) + at * HD;
-      o[e0] = (uint8_t)(q0 < 0 ? 128 - q0 : q0);
-      o[e1] = (uint8_t)(q1 < 0 ? 128 - q1 : q1);
-      if (sub == 0) kv_scales(a.kv, s, HD)[at] = d;
-    } else {
-      using KV = std::conditional_t<FMT == Q3H_KV_F16, _Float16, float>;
-      KV *o = reinterpret_cast<KV *>(s.k0) + at * HD;
-      o[e0] = to_cache<KV>(x0);
-      o[e1] = to_cache<KV>(x1);
+    }
+    const int e_0 = values ? 2 * sub : e0, e_1 = values ? 2 * sub + 1 : e1;
+#pragma unroll
+    for (int u = 0; u < kHeads; u++) {
+      const int j = first + u * SIDE;
+      if (j >= heads) continue;
+      if (!values && j < a.heads) {
+        float *o = a.q_out + (size_t)row * a.ld_out + (size_t)j * HD;
+        o[e_0] = bad ? NAN : x0[u];
+        o[e_1] = bad ? NAN : x1[u];
+        continue;
+      }
+      if (bad) continue;
+      const int64_t at = kv_row(a.kv, s, values, values ? j : j - a.heads, s.len + t);
+      if constexpr (FMT == Q3H_KV_Q8) {
+        uint8_t *o = reinterpret_cast<uint8_t *>(s.k0) + at * HD;
+        const bool some = d[u] > 0.f;  // (not NaN, not 0)
+        o[e_0] = some ? byte_of(x0[u], d[u], inv[u]) : 0;
+        o[e_1] = some ? byte_of(x1[u], d[u], inv[u]) : 0;
+        if (sub == 0) kv_scales(a.kv, s, HD)[at] = d[u];
+      } else {
+        using KV = std::conditional_t<FMT == Q3H_KV_F16, _Float16, float>;
+        KV *o = reinterpret_cast<KV *>(s.k0) + at * HD;
+        o[e_0] = to_cache<KV>(x0[u]);
+        o[e_1] = to_cache<KV>(x1[u]);
+      }
     }
   }
 }
@@ -169,8 +238,10 @@ __global__ __launch_bounds__(kThreads) void k_cache_read(KvView kv, const int32_
         for (int x = 0; x < 8; x++) o[x] = (float)p[x];
       }
     }
+    typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
     float *y = dst + r * HD + e;
-    for (int x = 0; x < 8; x++) y[x] = o[x];
+    __builtin_nontemporal_store((f4){o[0], o[1], o[2], o[3]}, reinterpret_cast<f4 *>(y));
+    __builtin_nontemporal_store((f4){o[4], o[5], o[6], o[7]}, reinterpret_cast<f4 *>(y + 4));
   }
 }
 
@@ -225,8 +296,13 @@ void by_format(int hd, int fmt, A &&...args) {
 template <int FMT, int HD>
 struct GoAppend {
   static void go(const AppendRows &a, hipStream_t st) {
-    const int per = (kThreads / 64) * (128 / HD), all = a.heads + 2 * a.kv.kvh;
-    const dim3 grid(a.kv.sequences * a.kv.rows, (all + per - 1) / per);
+    const int per = kHeads * (128 / HD);  // heads of a wave at a time
+    const int groups = (a.heads + a.kv.kvh + per - 1) / per + (a.kv.kvh + per - 1) / per;
+    // few rows: a wave for each group of heads; many: one workgroup a row, its
+    // waves going over the heads with one load of the angles
+    const int rows = a.kv.sequences * a.kv.rows;
+    const int side = rows >= 1024 ? 1 : (groups + kThreads / 64 - 1) / (kThreads / 64);
+    const dim3 grid(rows, side);
     hipLaunchKernelGGL((k_cache_append<FMT, HD>), grid, dim3(kThreads), 0, st, a);
   }
 };

@@ -18,13 +18,12 @@ constexpr int kMaxVocab = 1 << 20;
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr float kLog2e = 1.44269504088896340736f;
 
-// A logit and its token as one number that orders them from the top: larger
-// logits first, of equal ones (0 and -0 among them) the lower token, NaN last.
-// Never 0, and no two alike.
-__device__ __forceinline__ uint64_t top_key(float x, int i) {
+// A logit as a number that orders it from the top: larger logits above, 0 and -0
+// alike, NaN last; never 0. With its token's complement below it, as one 64-bit
+// key, of equal logits the lower token is above, and no two keys are alike.
+__device__ __forceinline__ uint32_t top_value(float x) {
   const uint32_t b = __float_as_uint(x + 0.f);
-  const uint32_t v = x != x ? 1u : b & 0x80000000u ? ~b : b | 0x80000000u;
-  return (uint64_t)v << 32 | (uint32_t)~i;
+  return x != x ? 1u : b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float key_logit(uint64_t k) {
   const uint32_t v = (uint32_t)(k >> 32);
@@ -34,52 +33,62 @@ __device__ __forceinline__ float key_logit(uint64_t k) {
 __device__ __forceinline__ int key_token(uint64_t k) { return (int)~(uint32_t)k; }
 
 // The k largest of the workgroup's keys (at most E a thread, key(e); 0: none),
-// k <= 64: the k-th largest of the threads' own maxima is not above the k-th
-// largest key, and only k threads hold keys from it on, so at most k E keys are
-// left; each of those counts the ones above it. emit(rank, key) once for
-// every rank below min(k, keys).
-template <int E>
+// k <= 64: the k-th largest of the maxima of 64 groups of 4 threads is not
+// above the k-th largest key, and only k groups hold keys from it on, so at
+// most 4 k E keys are left (24 of 10240 on average for k = 20, 270 for 64); each
+// of those counts the ones above it. emit(rank, key) once for every rank below
+// min(k, keys).
 struct TopSpace {
   uint64_t top[kThreads];
-  uint64_t list[Q3H_TOP_MAX * E];
   uint64_t bound;
   int n;
 };
+// (the keys left: top_bytes of dynamic LDS)
+inline size_t top_bytes(int k, int per_thread) {
+  return (size_t)4 * k * per_thread * sizeof(uint64_t);
+}
 template <int E, class Key, class Emit>
-__device__ __forceinline__ void block_top(TopSpace<E> &sm, int k, Key &&key, Emit &&emit) {
-  const int tid = threadIdx.x;
+__device__ __forceinline__ void block_top(TopSpace &sm, uint64_t *list, int k, Key &&key, Emit &&emit) {
+  const int tid = threadIdx.x, lane = tid & 63;
   uint64_t best = 0;
 #pragma unroll
   for (int e = 0; e < E; e++) {
     const uint64_t x = key(e);
     best = x > best ? x : best;
   }
-  __syncthreads();
   sm.top[tid] = best;
-  if (tid == 0) {
-    sm.n = 0;
-    sm.bound = 1;
-  }
+  if (tid == 0) sm.n = 0;
   __syncthreads();
-  int above = 0;
-#pragma unroll 16
-  for (int i = 0; i < kThreads; i++) above += sm.top[i] > best;
-  if (best && above == k - 1) sm.bound = best;  // (one thread at most: no two keys alike)
+  if (tid < 64) {
+    uint64_t g = best;
+#pragma unroll
+    for (int i = 1; i < kWaves; i++) g = sm.top[64 * i + lane] > g ? sm.top[64 * i + lane] : g;
+    int above = 0;
+#pragma unroll
+    for (int i = 0; i < 64; i++) {
+      const uint64_t o = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(g >> 32), i) << 32 |
+                         (uint32_t)__builtin_amdgcn_readlane((int)g, i);
+      above += o > g;
+    }
+    // (one lane at most: no two keys alike)
+    const uint64_t hit = __ballot(g && above == k - 1);
+    if (hit == 0 ? lane == 0 : (hit >> lane & 1)) sm.bound = hit == 0 ? 1 : g;
+  }
   __syncthreads();
   const uint64_t bound = sm.bound;
   if (best >= bound) {
 #pragma unroll
     for (int e = 0; e < E; e++) {
       const uint64_t x = key(e);
-      if (x >= bound) sm.list[atomicAdd(&sm.n, 1)] = x;
+      if (x >= bound) list[atomicAdd(&sm.n, 1)] = x;
     }
   }
   __syncthreads();
   const int n = sm.n;
   for (int c = tid; c < n; c += kThreads) {
-    const uint64_t x = sm.list[c];
+    const uint64_t x = list[c];
     int rank = 0;
-    for (int i = 0; i < n; i++) rank += sm.list[i] > x;
+    for (int i = 0; i < n; i++) rank += list[i] > x;
     if (rank < k) emit(rank, x);
   }
 }
@@ -129,7 +138,8 @@ __device__ __forceinline__ Space space_of(const ScoreRows &a, int splits) {
 template <bool BF16, int E>
 __global__ __launch_bounds__(kThreads) void k_score(ScoreRows a, int splits) {
   constexpr int VEC = BF16 ? 8 : 4, SIZE = BF16 ? 2 : 4;
-  __shared__ TopSpace<E> sm;
+  __shared__ TopSpace sm;
+  extern __shared__ uint64_t list[];
   __shared__ float red[3][kWaves];
   const int r = blockIdx.x / splits, split = blockIdx.x - r * splits, tid = threadIdx.x;
   const char *row = static_cast<const char *>(a.logits) + (size_t)r * a.ld * SIZE;
@@ -190,11 +200,17 @@ __global__ __launch_bounds__(kThreads) void k_score(ScoreRows a, int splits) {
   if (a.top_k == 0) return;
   uint64_t *keys = out.keys + (size_t)blockIdx.x * a.top_k;
   if (splits > 1 && tid < a.top_k && tid >= a.vocab - (split * kThreads * E - skew)) keys[tid] = 0;
+  uint32_t v[E];
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    const int i = first + e / VEC * kThreads * VEC + e % VEC;
+    v[e] = i >= 0 && i < a.vocab ? top_value(x[e]) : 0;
+  }
   block_top<E>(
-      sm, a.top_k,
+      sm, list, a.top_k,
       [&](int e) -> uint64_t {
         const int i = first + e / VEC * kThreads * VEC + e % VEC;
-        return i >= 0 && i < a.vocab ? top_key(x[e], i) : 0;
+        return v[e] ? (uint64_t)v[e] << 32 | (uint32_t)~i : 0;
       },
       [&](int rank, uint64_t k) {
         if (splits == 1) {
@@ -209,7 +225,8 @@ __global__ __launch_bounds__(kThreads) void k_score(ScoreRows a, int splits) {
 // the splits of a row together
 constexpr int kMergeKeys = 32;  // a thread
 __global__ __launch_bounds__(kThreads) void k_score_merge(ScoreRows a, int splits) {
-  __shared__ TopSpace<kMergeKeys> sm;
+  __shared__ TopSpace sm;
+  extern __shared__ uint64_t list[];
   const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
   const Space in = space_of(a, splits);
   const Sums *sums = in.sums + (size_t)r * splits;
@@ -237,7 +254,7 @@ __global__ __launch_bounds__(kThreads) void k_score_merge(ScoreRows a, int split
   for (int e = 0; e < kMergeKeys; e++)
     mine[e] = e * kThreads + tid < n ? keys[e * kThreads + tid] : 0;
   block_top<kMergeKeys>(
-      sm, a.top_k, [&](int e) { return mine[e]; },
+      sm, list, a.top_k, [&](int e) { return mine[e]; },
       [&](int rank, uint64_t k) {
         a.top_ids[(size_t)r * a.top_k + rank] = key_token(k);
         a.top_logprobs[(size_t)r * a.top_k + rank] = key_logit(k) - t.m - ls;
@@ -262,11 +279,16 @@ template <bool BF16>
 void launch(const ScoreRows &a, hipStream_t st) {
   const int splits = score_splits(a.vocab), width = score_width(a.vocab);
   const dim3 grid((unsigned)((int64_t)a.rows * splits));
-  if (width == 8) hipLaunchKernelGGL((k_score<BF16, 8>), grid, dim3(kThreads), 0, st, a, splits);
-  else if (width == 16) hipLaunchKernelGGL((k_score<BF16, 16>), grid, dim3(kThreads), 0, st, a, splits);
-  else hipLaunchKernelGGL((k_score<BF16, 40>), grid, dim3(kThreads), 0, st, a, splits);
+  const size_t lds = top_bytes(a.top_k, width);
+  if (width == 8)
+    hipLaunchKernelGGL((k_score<BF16, 8>), grid, dim3(kThreads), lds, st, a, splits);
+  else if (width == 16)
+    hipLaunchKernelGGL((k_score<BF16, 16>), grid, dim3(kThreads), lds, st, a, splits);
+  else
+    hipLaunchKernelGGL((k_score<BF16, 40>), grid, dim3(kThreads), lds, st, a, splits);
   if (splits > 1)
-    hipLaunchKernelGGL(k_score_merge, dim3(a.rows), dim3(kThreads), 0, st, a, splits);
+    hipLaunchKernelGGL(k_score_merge, dim3(a.rows), dim3(kThreads),
+                       top_bytes(a.top_k, kMergeKeys), st, a, splits);
 }
 
 }  // namespace

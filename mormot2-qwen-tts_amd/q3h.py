@@ -683,12 +683,23 @@ def _bad(msg):
     raise Q3HError(E_ARG, msg)
 
 
+_torch = None
+
+
+def _use_torch():
+    """torch, imported with the first handle that takes its tensors."""
+    global _torch
+    if _torch is None:
+        import torch
+        _torch = torch
+    return _torch
+
+
 def _ptr(t, ordinal, dtype, name):
-    """The address of a tensor of this dtype ("float32", ...) on the device."""
-    d = t.device
-    if d.type != "cuda" or (d.index or 0) != ordinal:
-        _bad(f"{name} is on {d}, not on device {ordinal}")
-    if str(t.dtype) != "torch." + dtype:
+    """The address of a tensor of this dtype on the device."""
+    if t.get_device() != ordinal:
+        _bad(f"{name} is on {t.device}, not on device {ordinal}")
+    if t.dtype is not dtype:
         _bad(f"{name} is {t.dtype}, not {dtype}")
     return t.data_ptr()
 
@@ -696,7 +707,7 @@ def _ptr(t, ordinal, dtype, name):
 def _rows(t, n, rows, heads, hd, ordinal, name):
     """(address, floats between rows) of f32 rows [n][rows][heads][hd], or
     [n][rows][heads * hd], contiguous within a row."""
-    shape, stride = tuple(t.shape), t.stride()
+    shape, stride = t.shape, t.stride()
     if shape == (n, rows, heads, hd):
         if stride[3] != 1 or (heads > 1 and stride[2] != hd):
             _bad(f"{name}: the heads of a row are not side by side")
@@ -708,21 +719,20 @@ def _rows(t, n, rows, heads, hd, ordinal, name):
     ld = stride[1] if rows > 1 else stride[0] if n > 1 else heads * hd
     if rows > 1 and n > 1 and stride[0] != rows * ld:
         _bad(f"{name}: the sequences' rows are not evenly spaced")
-    return _ptr(t, ordinal, "float32", name), ld
+    return _ptr(t, ordinal, _torch.float32, name), ld
 
 
 def _whole(t, shape, ordinal, dtype, name):
     """The address of a contiguous tensor of this shape and dtype; None for None."""
     if t is None:
         return None
-    if tuple(t.shape) != shape or not t.is_contiguous():
+    if t.shape != shape or not t.is_contiguous():
         _bad(f"{name} is {list(t.shape)}, not contiguous {list(shape)}")
     return _ptr(t, ordinal, dtype, name)
 
 
 def _stream(ordinal):
-    import torch
-    return torch.cuda.current_stream(ordinal).cuda_stream
+    return _torch.cuda.current_stream(ordinal).cuda_stream
 
 
 class Rope:
@@ -773,10 +783,15 @@ class Cache:
     def __init__(self, dev, sequences, kv_heads, head_dim, max_positions, fmt=KV_F32, layers=1):
         cfg = CacheConfig(sequences, layers, kv_heads, head_dim, max_positions, fmt)
         h = _P()
-        _check(lib().q3h_cache_create(dev.h, ctypes.byref(cfg), ctypes.byref(h)))
+        L = lib()
+        _check(L.q3h_cache_create(dev.h, ctypes.byref(cfg), ctypes.byref(h)))
+        _use_torch()
         self.dev = dev
         self.h = h
         self.kv_heads, self.head_dim = kv_heads, head_dim
+        self._append, self._read, self._attend = \
+            L.q3h_cache_append, L.q3h_cache_read, L.q3h_cache_attend
+        self._workspace = L.q3h_cache_attend_workspace
 
     @property
     def bytes(self):
@@ -789,41 +804,38 @@ class Cache:
         queries (q_out, made when it is None; rows beyond counts as they were),
         None without q. parents: the row each row continues (-1: the sequence
         itself); None: a chain."""
-        o, hd = self.dev.ordinal, self.head_dim
+        o, hd, i32, f32 = self.dev.ordinal, self.head_dim, _torch.int32, _torch.float32
         n, rows = k.shape[0], k.shape[1]
-        a = AppendArgs()
-        a.layer, a.sequences, a.rows = layer, n, rows
-        a.k, a.ldk = _rows(k, n, rows, self.kv_heads, hd, o, "k")
-        a.v, a.ldv = _rows(v, n, rows, self.kv_heads, hd, o, "v")
+        pk, ldk = _rows(k, n, rows, self.kv_heads, hd, o, "k")
+        pv, ldv = _rows(v, n, rows, self.kv_heads, hd, o, "v")
+        heads, pq, ldq, po, ldo, qn = 0, None, 0, None, 0, None
         if q is not None:
             heads = q.shape[2] if q.dim() == 4 else q.shape[2] // hd
             if q_out is None:
                 q_out = q.new_empty((n, rows, heads, hd))
-            a.heads = heads
-            a.q, a.ldq = _rows(q, n, rows, heads, hd, o, "q")
-            a.q_out, a.ld_out = _rows(q_out, n, rows, heads, hd, o, "q_out")
-            a.q_norm = _whole(q_norm, (hd,), o, "float32", "q_norm")
-        a.k_norm = _whole(k_norm, (hd,), o, "float32", "k_norm")
-        a.eps = eps
-        a.rope = rope.h if rope is not None else None
-        a.lens = _whole(lens, (n,), o, "int32", "lens")
-        a.counts = _whole(counts, (n,), o, "int32", "counts")
-        a.parents = _whole(parents, (n, rows), o, "int32", "parents")
-        _check(lib().q3h_cache_append(self.h, ctypes.byref(a), _stream(o)))
+            pq, ldq = _rows(q, n, rows, heads, hd, o, "q")
+            po, ldo = _rows(q_out, n, rows, heads, hd, o, "q_out")
+            qn = _whole(q_norm, (hd,), o, f32, "q_norm")
+        a = AppendArgs(layer, n, rows, heads, pq, pk, pv, ldq, ldk, ldv, po, ldo, qn,
+                       _whole(k_norm, (hd,), o, f32, "k_norm"), eps,
+                       rope.h if rope is not None else None, _whole(lens, (n,), o, i32, "lens"),
+                       _whole(counts, (n,), o, i32, "counts"),
+                       _whole(parents, (n, rows), o, i32, "parents"))
+        _check(self._append(self.h, a, _stream(o)))
         return q_out
 
     def read(self, k, v, starts=None, counts=None, layer=0):
         """Positions starts[b] .. + counts[b] - 1 of the first sequences into k
         and v (either None) [sequences][rows][kv_heads][head_dim] as f32; rows
         beyond counts stay as they were."""
-        o = self.dev.ordinal
+        o, i32, f32 = self.dev.ordinal, _torch.int32, _torch.float32
         like = k if k is not None else v
         n, rows = like.shape[0], like.shape[1]
         shape = (n, rows, self.kv_heads, self.head_dim)
-        _check(lib().q3h_cache_read(
-            self.h, layer, n, rows, _whole(starts, (n,), o, "int32", "starts"),
-            _whole(counts, (n,), o, "int32", "counts"), _whole(k, shape, o, "float32", "k"),
-            _whole(v, shape, o, "float32", "v"), _stream(o)))
+        _check(self._read(
+            self.h, layer, n, rows, _whole(starts, (n,), o, i32, "starts"),
+            _whole(counts, (n,), o, i32, "counts"), _whole(k, shape, o, f32, "k"),
+            _whole(v, shape, o, f32, "v"), _stream(o)))
 
     def attend(self, q, lens, max_len, out=None, counts=None, parents=None, scale=0.0, layer=0,
                workspace=None):
@@ -832,28 +844,26 @@ class Cache:
         (made when it is None; rows beyond counts as they were). scale 0: 1 /
         sqrt(head_dim). workspace: a uint8 tensor of attend_workspace bytes (made
         when it is None)."""
-        o, hd = self.dev.ordinal, self.head_dim
+        o, hd, i32 = self.dev.ordinal, self.head_dim, _torch.int32
         n, rows = q.shape[0], q.shape[1]
         heads = q.shape[2] if q.dim() == 4 else q.shape[2] // hd
         if out is None:
             out = q.new_empty((n, rows, heads, hd))
-        a = AttendArgs()
-        a.layer, a.sequences, a.rows, a.heads, a.max_len = layer, n, rows, heads, max_len
-        a.scale = scale
-        a.q, a.ldq = _rows(q, n, rows, heads, hd, o, "q")
-        a.out, a.ld_out = _rows(out, n, rows, heads, hd, o, "out")
-        a.lens = _whole(lens, (n,), o, "int32", "lens")
-        a.counts = _whole(counts, (n,), o, "int32", "counts")
-        a.parents = _whole(parents, (n, rows), o, "int32", "parents")
-        need = self.attend_workspace(n, rows, heads, max_len)
+        pq, ldq = _rows(q, n, rows, heads, hd, o, "q")
+        po, ldo = _rows(out, n, rows, heads, hd, o, "out")
+        need, space = self.attend_workspace(n, rows, heads, max_len), None
         if need:
             workspace = _space(workspace, need, q, o)
-            a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
-        _check(lib().q3h_cache_attend(self.h, ctypes.byref(a), _stream(o)))
+            space, need = workspace.data_ptr(), workspace.numel()
+        a = AttendArgs(layer, n, rows, heads, max_len, scale, pq, ldq, po, ldo,
+                       _whole(lens, (n,), o, i32, "lens"),
+                       _whole(counts, (n,), o, i32, "counts"),
+                       _whole(parents, (n, rows), o, i32, "parents"), space, need)
+        _check(self._attend(self.h, a, _stream(o)))
         return out
 
     def attend_workspace(self, sequences, rows, heads, max_len):
-        need = lib().q3h_cache_attend_workspace(self.h, sequences, rows, heads, max_len)
+        need = self._workspace(self.h, sequences, rows, heads, max_len)
         if need < 0:
             _check(need)
         return need
@@ -862,12 +872,12 @@ class Cache:
         """Moves the rows kept [sequences][rows] (ascending row numbers, the first
         kept_counts of each sequence) to positions lens[b], lens[b] + 1, ... in
         every layer. The caller's lengths then grow by kept_counts."""
-        o = self.dev.ordinal
+        o, i32 = self.dev.ordinal, _torch.int32
         n, rows = kept.shape
         _check(lib().q3h_cache_keep(
-            self.h, n, rows, _whole(lens, (n,), o, "int32", "lens"),
-            _whole(kept, (n, rows), o, "int32", "kept"),
-            _whole(kept_counts, (n,), o, "int32", "kept_counts"), _stream(o)))
+            self.h, n, rows, _whole(lens, (n,), o, i32, "lens"),
+            _whole(kept, (n, rows), o, i32, "kept"),
+            _whole(kept_counts, (n,), o, i32, "kept_counts"), _stream(o)))
 
     def destroy(self):
         if self.h:
@@ -882,9 +892,8 @@ class Cache:
 def _space(workspace, need, like, ordinal):
     """A uint8 tensor of at least need bytes on the device."""
     if workspace is None:
-        import torch
-        return torch.empty(need, dtype=torch.uint8, device=like.device)
-    _ptr(workspace, ordinal, "uint8", "workspace")
+        return _torch.empty(need, dtype=_torch.uint8, device=like.device)
+    _ptr(workspace, ordinal, _torch.uint8, "workspace")
     if not workspace.is_contiguous():
         _bad("workspace is not contiguous")
     return workspace
@@ -894,32 +903,33 @@ def token_logprobs(dev, logits, tokens, top_k=0, workspace=None):
     """Scores of logits [rows][vocab] (f32 or bf16) at tokens [rows][m] (int32):
     dict of logprobs [rows][m], entropy [rows] and, with top_k, top_ids and
     top_logprobs [rows][top_k] (largest first, of equal ones the lowest token)."""
-    o = dev.ordinal
+    torch, L, o = _use_torch(), lib(), dev.ordinal
+    f32, i32 = torch.float32, torch.int32
     rows, vocab = logits.shape
-    bf16 = str(logits.dtype) == "torch.bfloat16"
-    if vocab > 1 and logits.stride(1) != 1:
+    bf16 = logits.dtype is torch.bfloat16
+    stride = logits.stride()
+    if vocab > 1 and stride[1] != 1:
         _bad("logits: the elements of a row are not side by side")
-    a = ScoreArgs()
-    a.logits = _ptr(logits, o, "bfloat16" if bf16 else "float32", "logits")
-    a.ld = logits.stride(0) if rows > 1 else vocab
-    a.dtype, a.rows, a.vocab, a.top_k = BF16 if bf16 else F32, rows, vocab, top_k
+    at = _ptr(logits, o, torch.bfloat16 if bf16 else f32, "logits")
     m = tokens.shape[1]
-    a.tokens_per_row = m
-    a.tokens = _whole(tokens, (rows, m), o, "int32", "tokens")
-    like = dict(device=logits.device)
-    import torch
-    res = {"logprobs": torch.empty((rows, m), **like), "entropy": torch.empty(rows, **like)}
-    a.logprobs, a.entropy = res["logprobs"].data_ptr(), res["entropy"].data_ptr()
-    if top_k > 0:
-        res["top_ids"] = torch.empty((rows, top_k), dtype=torch.int32, **like)
-        res["top_logprobs"] = torch.empty((rows, top_k), **like)
-        a.top_ids = res["top_ids"].data_ptr()
-        a.top_logprobs = res["top_logprobs"].data_ptr()
-    need = lib().q3h_token_logprobs_workspace(rows, vocab, top_k)
+    pt = _whole(tokens, (rows, m), o, i32, "tokens")
+    need, space = L.q3h_token_logprobs_workspace(rows, vocab, top_k), None
     if need < 0:
         _check(need)
     if need:
         workspace = _space(workspace, need, logits, o)
-        a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
-    _check(lib().q3h_token_logprobs(dev.h, ctypes.byref(a), _stream(o)))
+        space, need = workspace.data_ptr(), workspace.numel()
+    like = logits.device
+    logprobs = torch.empty((rows, m), dtype=f32, device=like)
+    entropy = torch.empty(rows, dtype=f32, device=like)
+    res = {"logprobs": logprobs, "entropy": entropy}
+    ids = top = None
+    if top_k > 0:
+        res["top_ids"] = ids = torch.empty((rows, top_k), dtype=i32, device=like)
+        res["top_logprobs"] = top = torch.empty((rows, top_k), dtype=f32, device=like)
+    a = ScoreArgs(at, stride[0] if rows > 1 else vocab, BF16 if bf16 else F32, rows, vocab, m,
+                  top_k, pt, logprobs.data_ptr(), entropy.data_ptr(),
+                  ids.data_ptr() if top_k > 0 else None, top.data_ptr() if top_k > 0 else None,
+                  space, need)
+    _check(L.q3h_token_logprobs(dev.h, a, _stream(o)))
     return res
