@@ -629,7 +629,7 @@ extern "C" int64_t q3h_cache_attend_workspace(const q3h_cache *c, int sequences,
             "q3h_cache_attend_workspace: max_len beyond the cache");
     if (sequences > 0 && rows > 0)
       bytes = (int64_t)attend_part_bytes(sequences, rows, heads, c->cfg.kv_heads,
-                                         c->cfg.head_dim, max_len);
+                                         c->cfg.head_dim, c->cfg.format, max_len);
   });
   return rc ? rc : bytes;
 }
@@ -654,9 +654,11 @@ extern "C" int q3h_cache_attend(q3h_cache *c, const q3h_attend_args *p, void *st
             "q3h_cache_attend: a tree has at most " + std::to_string(Q3H_TREE_MAX_ROWS) + " rows");
     require((int64_t)p->sequences * p->rows <= INT32_MAX, Q3H_E_CAPACITY,
             "q3h_cache_attend: too many rows");
+    require((int64_t)p->sequences * p->rows * p->heads <= (1 << 29), Q3H_E_CAPACITY,
+            "q3h_cache_attend: too many rows and heads");
     require(std::isfinite(p->scale), Q3H_E_ARG, "q3h_cache_attend: scale is not finite");
     const size_t need = attend_part_bytes(p->sequences, p->rows, p->heads, cf.kv_heads,
-                                          cf.head_dim, p->max_len);
+                                          cf.head_dim, cf.format, p->max_len);
     require(need == 0 || (p->workspace && p->workspace_bytes >= (int64_t)need &&
                           (uintptr_t)p->workspace % 256 == 0),
             Q3H_E_ARG, "q3h_cache_attend: a workspace of " + std::to_string(need) +

@@ -129,7 +129,8 @@ struct AttendRows {
   const int32_t *parents;
   float *part;  // attend_part_bytes
 };
-size_t attend_part_bytes(int sequences, int rows, int heads, int kvh, int hd, int max_len);
+size_t attend_part_bytes(int sequences, int rows, int heads, int kvh, int hd, int fmt,
+                         int max_len);
 void launch_cache_attend(const AttendRows &a, int hd, int fmt, hipStream_t st);
 
 struct ScoreRows {

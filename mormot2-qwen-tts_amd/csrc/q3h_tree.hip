@@ -52,19 +52,35 @@ constexpr int kTile = FMT == Q3H_KV_F32 ? 16 : 32;
 
 constexpr float kLog2e = 1.44269504088896340736f;
 
-// where the positions of a row group are cut: tiles in all, tiles a split
-struct Cut {
-  int full;  // positions that all the group's rows see
-  int end;   // positions that some row of it sees
-  int tiles, per;
+// How a call is laid out: query tiles of 16 rows a wave (nq), rows of a
+// workgroup (group), tiles of positions a wave goes over (per_wave: the same for
+// all, so that a long sequence has more splits and not longer ones), splits at
+// most.
+struct Shape {
+  int nq, group, per_wave, splits;
 };
-__device__ __forceinline__ Cut cut_of(const AttendRows &a, const KvSeq &s, int t0, int t1,
-                                      int splits, int tile) {
+
+// A row group's share of the work: waves side by side over its query tiles (wq)
+// and over the positions (wk), and its positions.
+struct Cut {
+  int here;    // rows of the group
+  int wq, wk;
+  int full;    // positions that all its rows see
+  int end;     // positions that some row of it sees
+  int tiles, per, splits;  // tiles that hold them, tiles a split, splits
+};
+__device__ __forceinline__ Cut cut_of(const AttendRows &a, const KvSeq &s, const Shape &shape,
+                                      int first, int rows_in, int tile) {
+  const int per_kv = a.heads / a.kv.kvh;
   Cut c;
-  c.full = s.len + (a.parents ? 0 : t0 + 1);
-  c.end = s.len + t1 + 1;
+  c.here = std::min(shape.group, rows_in - first);
+  c.wq = c.here > 32 * shape.nq ? 4 : c.here > 16 * shape.nq ? 2 : 1;
+  c.wk = kWaves / c.wq;
+  c.full = s.len + (a.parents ? 0 : first / per_kv + 1);
+  c.end = s.len + (first + c.here - 1) / per_kv + 1;
   c.tiles = (c.end + tile - 1) / tile;
-  c.per = (c.tiles + splits - 1) / splits;
+  c.per = shape.per_wave * c.wk;
+  c.splits = (c.tiles + c.per - 1) / c.per;
   return c;
 }
 
@@ -102,23 +118,30 @@ struct Raw<Q3H_KV_F32, HD> {
   f4 v[4][HD / 64];
 };
 
-// One workgroup per (split, kv head, sequence, group of WQ * NQ query tiles):
-// WQ waves side by side over the query tiles, 4 / WQ waves over the positions.
-// NQ tiles a wave share its loads and conversions of K and V.
-template <int FMT, int HD, int NQ, int WQ>
-__global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, int splits) {
-  constexpr int T = kTile<FMT>, WK = kWaves / WQ;
-  constexpr int GROUP = 16 * NQ * WQ;  // query rows of the workgroup
+// One workgroup per (split, kv head, sequence, group of query rows): as many
+// waves side by side as the rows it has need (1, 2 or 4), NQ query tiles each,
+// the others over the positions. NQ tiles a wave share its loads and
+// conversions of K and V; a wave of one tile has the registers for two tiles of
+// positions on their way.
+template <int FMT, int HD, int NQ>
+__global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shape) {
+  constexpr int T = kTile<FMT>;
   constexpr int C = HD / 16;           // output tiles; neighbouring elements a lane reads
   constexpr bool F32 = FMT == Q3H_KV_F32, Q8 = FMT == Q3H_KV_Q8;
   constexpr int NS = F32 ? 1 : 2;                // key tiles of 16 in a tile
   constexpr int ROW = HD * (F32 ? 4 : Q8 ? 1 : 2);  // bytes
-  __shared__ float sm_acc[WK > 1 ? kWaves * NQ * 16 * HD : 1];
+  constexpr int LD = HD + 4;  // (rows 4 banks apart)
+  // the waves' outputs; before that, with two query tiles a wave, its queries as
+  // operands (64 registers: two waves a SIMD would not have them)
+  constexpr bool QLDS = NQ > 1 && !F32;
+  constexpr int QW = NQ * (HD / 32) * 2 * 256;  // words of a wave's queries
+  __shared__ __align__(16) float
+      sm_acc[QLDS && QW > NQ * 16 * LD ? kWaves * QW : kWaves * NQ * 16 * LD];
   __shared__ float sm_m[kWaves][NQ * 16], sm_l[kWaves][NQ * 16];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n16 = lane & 15, g4 = lane >> 4;
-  const int wq = wave % WQ, wk = wave / WQ;
+  const int splits = shape.splits, GROUP = shape.group;
   const int split = blockIdx.x % splits, rest = blockIdx.x / splits;
   const int g = rest % a.kv.kvh, b = (rest / a.kv.kvh) % a.kv.sequences,
             group = rest / a.kv.kvh / a.kv.sequences;
@@ -139,11 +162,12 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, int splits
     }
     return;
   }
-  const int t1 = (std::min(first + GROUP, rows_in) - 1) / per_kv;
-  const Cut cut = cut_of(a, s, first / per_kv, t1, splits, T);
+  const Cut cut = cut_of(a, s, shape, first, rows_in, T);
   const int tile0 = split * cut.per, tile1 = std::min(cut.tiles, tile0 + cut.per);
   if (tile0 >= tile1) return;
   const int last = cut.end - 1;  // no row behind it is read
+  const int here = cut.here, WQ = cut.wq, WK = cut.wk;
+  const int wq = wave & (WQ - 1), wk = wave / WQ;
 
   const char *kbase = s.k0 + kv_row(a.kv, s, 0, g, 0) * ROW;
   const char *vbase = s.k0 + kv_row(a.kv, s, 1, g, 0) * ROW;
@@ -153,7 +177,6 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, int splits
     vsc = reinterpret_cast<const char *>(kv_scales(a.kv, s, HD) + kv_row(a.kv, s, 1, g, 0));
   }
 
-  Raw<FMT, HD> raw;
   auto load_scales = [&](const char *sc, int j0, f4(&d)[2]) {
 #pragma unroll
     for (int t = 0; t < 2; t++) {
@@ -166,7 +189,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, int splits
       }
     }
   };
-  auto load_k = [&](int tile) {
+  auto load_k = [&](Raw<FMT, HD> &raw, int tile) {
     const int j0 = tile * T;
     const char *p = kbase + (int64_t)j0 * ROW;
 #pragma unroll
@@ -185,7 +208,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, int splits
     }
     if constexpr (Q8) load_scales(ksc, j0, raw.ks);
   };
-  auto load_v = [&](int tile) {
+  auto load_v = [&](Raw<FMT, HD> &raw, int tile) {
     const int j0 = tile * T;
     const char *p = vbase + (int64_t)j0 * ROW;
 #pragma unroll
@@ -211,7 +234,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, int splits
     if constexpr (Q8) load_scales(vsc, j0, raw.vs);
   };
   // word w of the HD / 16 elements of position i of the loaded values
-  auto vword = [&](int i, int w) -> uint32_t {
+  auto vword = [](const Raw<FMT, HD> &raw, int i, int w) -> uint32_t {
     if constexpr (FMT == Q3H_KV_F16)
       return HD == 128 ? raw.v[i][w] : raw.v[i / 2][2 * (i & 1) + w];
     else if constexpr (Q8)
@@ -220,33 +243,44 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, int splits
       return 0;
   };
 
+  Raw<FMT, HD> raw;
   int tile = tile0 + wk;
   if (tile < tile1) {
-    load_k(tile);
-    load_v(tile);
+    load_k(raw, tile);
+    load_v(raw, tile);
   }
 
   // the wave's queries: dims of (step, lane group) as the keys' loads have them
-  int qrow[NQ];
+  int qrow[NQ], qt[NQ];  // the lane's query row, and the drafted row that it is of
   bool live[NQ];
   f4 qf[F32 ? NQ : 1][HD / 16];
-  u4 qh[F32 ? 1 : NQ][HD / 32], ql[F32 ? 1 : NQ][HD / 32];
-  float sfac[NQ];  // a score in powers of two: product * sfac (* the key's scale)
+  u4 qh[F32 || QLDS ? 1 : NQ][HD / 32], ql[F32 || QLDS ? 1 : NQ][HD / 32];
+  u4 *const qs = reinterpret_cast<u4 *>(sm_acc) + wave * (QW / 4) + lane;
+  // the two parts of step i of query tile q
+  auto query = [&](int q, int i, int part) -> h8 {
+    if constexpr (QLDS) return __builtin_bit_cast(h8, qs[((q * (HD / 32) + i) * 2 + part) * 64]);
+    else return __builtin_bit_cast(h8, part ? ql[q][i] : qh[q][i]);
+  };
+  // a score in powers of two: product (* the key's scale) * sfac, which is not
+  // negative (the queries have the scale's sign): the maximum is the products'
+  float sfac[NQ];
+  const float sign = a.scale < 0.f ? -1.f : 1.f;
 #pragma unroll
   for (int q = 0; q < NQ; q++) {
     const int r = first + (wq * NQ + q) * 16 + n16;
     live[q] = r < rows_in;
     qrow[q] = std::min(r, rows_in - 1);
+    qt[q] = qrow[q] / per_kv;
     const char *p = reinterpret_cast<const char *>(
-        a.q + (row0 + qrow[q] / per_kv) * a.ldq + (size_t)(g * per_kv + qrow[q] % per_kv) * HD);
+        a.q + (row0 + qt[q]) * a.ldq + (size_t)(g * per_kv + qrow[q] - qt[q] * per_kv) * HD);
     if constexpr (F32) {
 #pragma unroll
-      for (int i = 0; i < HD / 16; i++) qf[q][i] = load<f4u>(p, 4 * (16 * i + 4 * g4));
-      sfac[q] = a.scale * kLog2e;
+      for (int i = 0; i < HD / 16; i++)
+        qf[q][i] = load<f4u>(p, 4 * (16 * i + 4 * g4)) * sign;
+      sfac[q] = fabsf(a.scale) * kLog2e;
     } else {
       float x[HD / 32][8];
       float m = 0.f;
-      bool odd = false;
 #pragma unroll
       for (int i = 0; i < HD / 32; i++) {
         const int d = Q8 ? (i >> 1) * 64 + g4 * 16 + (i & 1) * 8 : i * 32 + g4 * 8;
@@ -257,24 +291,32 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, int splits
           x[i][4 + e] = w[e];
         }
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-          m = fmaxf(m, fabsf(x[i][e]));
-          odd = odd || !(fabsf(x[i][e]) < INFINITY);
-        }
+        for (int e = 0; e < 8; e++) m = fmaxf(m, fabsf(x[i][e]));
       }
-      m = rows4_max(odd ? INFINITY : m);
-      // m * 2^k in [2^13, 2^14); infinities and NaN stay what they are
-      const int k = m > 0.f && m < INFINITY ? 13 - ilogbf(m) : 0;
+      m = rows4_max(m);
+      // m * 2^k in [2^13, 2^14) (rows below 2^-113: less); infinities and NaN stay
+      // what they are
+      const int k = m > 0.f && m < INFINITY ? std::min(126, 140 - (int)(__float_as_uint(m) >> 23)) : 0;
+      const float up = sign * __uint_as_float((uint32_t)(127 + k) << 23);
 #pragma unroll
-      for (int i = 0; i < HD / 32; i++)
+      for (int i = 0; i < HD / 32; i++) {
+        u4 h, l;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
           uint32_t hi, lo;
-          split2(ldexpf(x[i][2 * e], k), ldexpf(x[i][2 * e + 1], k), hi, lo);
-          qh[q][i][e] = hi;
-          ql[q][i][e] = lo;
+          split2(x[i][2 * e] * up, x[i][2 * e + 1] * up, hi, lo);
+          h[e] = hi;
+          l[e] = lo;
         }
-      sfac[q] = ldexpf(a.scale * kLog2e, Q8 ? 24 - k : -k);
+        if constexpr (QLDS) {
+          qs[(q * (HD / 32) + i) * 2 * 64] = h;
+          qs[((q * (HD / 32) + i) * 2 + 1) * 64] = l;
+        } else {
+          qh[q][i] = h;
+          ql[q][i] = l;
+        }
+      }
+      sfac[q] = ldexpf(fabsf(a.scale) * kLog2e, Q8 ? 24 - k : -k);
     }
   }
 
@@ -294,10 +336,12 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, int splits
   }
   // whether query tile q's row sees drafted row d (d < 0: a position before the draft)
   auto sees = [&](int q, int d) {
-    return d < 0 || (d <= qrow[q] / per_kv && (!a.parents || (path[q] >> d & 1)));
+    return d < 0 || (d <= qt[q] && (!a.parents || (path[q] >> d & 1)));
   };
-  for (; tile < tile1; tile += WK) {
-    const int j0 = tile * T;
+  auto step = [&](Raw<FMT, HD> &raw, int tile) {
+    const int j0 = tile * T, next = tile + WK;
+    // (the queries stay in LDS: not read once for all tiles)
+    if constexpr (QLDS) asm volatile("" ::: "memory");
     const bool tail = j0 + T > cut.full;
     // scores
     f4 st[NQ][NS];
@@ -333,10 +377,10 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, int splits
           const h8 A = __builtin_bit_cast(h8, ka);
 #pragma unroll
           for (int q = 0; q < NQ; q++) {
-            st[q][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                A, __builtin_bit_cast(h8, ql[q][i]), st[q][t], 0, 0, 0);
-            st[q][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                A, __builtin_bit_cast(h8, qh[q][i]), st[q][t], 0, 0, 0);
+            st[q][t] =
+                __builtin_amdgcn_mfma_f32_16x16x32_f16(A, query(q, i, 1), st[q][t], 0, 0, 0);
+            st[q][t] =
+                __builtin_amdgcn_mfma_f32_16x16x32_f16(A, query(q, i, 0), st[q][t], 0, 0, 0);
           }
         }
     }
@@ -345,9 +389,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, int splits
 #pragma unroll
       for (int t = 0; t < 2; t++) ks[t] = raw.ks[t];
     }
-    if (tile + WK < tile1) load_k(tile + WK);
+    if (next < tile1) load_k(raw, next);
 
-    float fv = 16384.f;
     int ev_new = ev;
     if constexpr (Q8) {
       float x = 0.f;
@@ -357,7 +400,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, int splits
         for (int r = 0; r < 4; r++) x = fmaxf(x, raw.vs[t][r]);
       x = rows4_max(x);
       ev_new = std::max(ev, (int)(__float_as_uint(x) >> 23) - 126);
-      fv = ldexpf(1.f, 14 - ev_new);
+      const float fv = ldexpf(1.f, 14 - ev_new);
 #pragma unroll
       for (int t = 0; t < 2; t++) vs[t] = raw.vs[t] * fv;
     }
@@ -366,34 +409,34 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, int splits
       const Path p = tree_path(a.parents + row0, a.kv.rows);
 #pragma unroll
       for (int q = 0; q < NQ; q++) {
-        path[q] = __shfl(p.rows, qrow[q] / per_kv);
-        broken[q] = __shfl((int)p.bad, qrow[q] / per_kv) != 0;
+        path[q] = __shfl(p.rows, qt[q]);
+        broken[q] = __shfl((int)p.bad, qt[q]) != 0;
       }
     }
     float w[NQ][4 * NS];
 #pragma unroll
     for (int q = 0; q < NQ; q++) {
-      float mx = m[q];
+      float mx = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 4 * NS; i++) {
-        float x;
-        if constexpr (Q8)
-          x = st[q][i >> 2][i & 3] * sfac[q] * ks[i >> 2][i & 3];
-        else
-          x = st[q][i >> 2][i & 3] * sfac[q];
+        float x = st[q][i >> 2][i & 3];
+        if constexpr (Q8) x *= ks[i >> 2][i & 3];
         if (tail) {
           const int d = j0 + (i >> 2) * 16 + 4 * g4 + (i & 3) - s.len;
           x = sees(q, d) ? x : -INFINITY;
           // a row whose path is broken: NaN at itself, and so in all of it
-          if (broken[q] && d == qrow[q] / per_kv) x = NAN;
+          if (broken[q] && d == qt[q]) x = NAN;
         }
         w[q][i] = x;
         mx = fmaxf(mx, x);
       }
+      // (a row that sees none of these, or whose queries are 0: no NaN from inf * 0)
       mx = rows4_max(mx);
-      const float base = mx == -INFINITY ? 0.f : mx;
+      mx = fmaxf(m[q], mx == -INFINITY ? mx : mx * sfac[q]);
+      // f16: weights to 2^14
+      const float base = mx == -INFINITY ? 0.f : mx - (FMT == Q3H_KV_F16 ? 14.f : 0.f);
       if (__any(mx > m[q] || ev_new > ev)) {
-        const float f = __builtin_amdgcn_exp2f(m[q] - base);
+        const float f = __builtin_amdgcn_exp2f(m[q] - (mx == -INFINITY ? 0.f : mx));
         l[q] *= f;
         const float fa = Q8 ? ldexpf(f, ev - ev_new) : f;
 #pragma unroll
@@ -402,7 +445,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, int splits
       }
 #pragma unroll
       for (int i = 0; i < 4 * NS; i++) {
-        const float p = __builtin_amdgcn_exp2f(w[q][i] - base);
+        float p = __builtin_amdgcn_exp2f(fmaf(w[q][i], sfac[q], -base));
+        if (tail) p = w[q][i] == -INFINITY ? 0.f : p;
         l[q] += p;
         if constexpr (Q8) {
           float v = vs[i >> 2][i & 3];
@@ -411,7 +455,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, int splits
         } else if constexpr (F32) {
           w[q][i] = p;
         } else {
-          w[q][i] = p * fv;
+          w[q][i] = p;
         }
       }
     }
@@ -448,10 +492,10 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, int splits
         for (int e = 0; e < 4; e++) {
           if constexpr (Q8) {
             // bytes c of positions 2e and 2e + 1
-            va[e] = bytes_f16(vword(2 * e + 1, c >> 2), vword(2 * e, c >> 2),
+            va[e] = bytes_f16(vword(raw, 2 * e + 1, c >> 2), vword(raw, 2 * e, c >> 2),
                               0x04040000u + 0x01010101u * (c & 3));
           } else {
-            const uint32_t x = vword(2 * e, c >> 1), y = vword(2 * e + 1, c >> 1);
+            const uint32_t x = vword(raw, 2 * e, c >> 1), y = vword(raw, 2 * e + 1, c >> 1);
             va[e] = __builtin_amdgcn_perm(y, x, c & 1 ? 0x07060302u : 0x05040100u);
           }
         }
@@ -463,23 +507,24 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, int splits
         }
       }
     }
-    if (tile + WK < tile1) load_v(tile + WK);
-  }
+    if (next < tile1) load_v(raw, next);
+  };
+  for (; tile < tile1; tile += WK) step(raw, tile);
 
-  // out of the weights' scale
+  // what the outputs are still to be multiplied with; whether any is NaN (or, as
+  // good, infinite)
+  float scale[NQ];
   bool nan = false;
 #pragma unroll
   for (int q = 0; q < NQ; q++) {
-    const float f = F32 ? 1.f : Q8 ? ldexpf(0x1p24f, ev - 14) : 1.f / 16384.f;
-    l[q] = rows4_sum(l[q]);
-    nan = nan || (l[q] != l[q] && !broken[q]);
+    scale[q] = F32 ? 1.f : Q8 ? ldexpf(0x1p24f, ev - 14) : 1.f / 16384.f;
+    l[q] = rows4_sum(l[q]) * (FMT == Q3H_KV_F16 ? 1.f / 16384.f : 1.f);
+    float zero = 0.f * l[q];
 #pragma unroll
     for (int c = 0; c < C; c++)
 #pragma unroll
-      for (int r = 0; r < 4; r++) {
-        acc[q][c][r] *= f;
-        nan = nan || (acc[q][c][r] != acc[q][c][r] && !broken[q]);
-      }
+      for (int r = 0; r < 4; r++) zero = fmaf(acc[q][c][r], 0.f, zero);
+    nan = nan || (zero != 0.f && !broken[q]);
   }
   // An infinity times one of the parts that a query or a weight is split in is
   // NaN where the product itself is not, and so is an infinity that a row does
@@ -488,8 +533,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, int splits
   if (__any(nan)) {
 #pragma unroll
     for (int q = 0; q < NQ; q++) {
-      const float *p = a.q + (row0 + qrow[q] / per_kv) * a.ldq +
-                       (size_t)(g * per_kv + qrow[q] % per_kv) * HD + C * 4 * g4;
+      const float *p = a.q + (row0 + qt[q]) * a.ldq +
+                       (size_t)(g * per_kv + qrow[q] - qt[q] * per_kv) * HD + C * 4 * g4;
       float ms = -INFINITY, ls = 0.f;
 #pragma unroll
       for (int c = 0; c < C; c++) acc[q][c] = (f4){0.f, 0.f, 0.f, 0.f};
@@ -523,12 +568,13 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, int splits
         }
       m[q] = ms;
       l[q] = ls;
+      scale[q] = 1.f;
     }
   }
 
   // the waves over the positions together
   constexpr int Q16 = NQ * 16;
-  if constexpr (WK > 1) {
+  if (WK > 1) {
     if (g4 == 0) {
 #pragma unroll
       for (int q = 0; q < NQ; q++) {
@@ -545,7 +591,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, int splits
 #pragma unroll
   for (int q = 0; q < NQ; q++) {
     float M = m[q], L = l[q], f = 1.f;
-    if constexpr (WK > 1) {
+    if (WK > 1) {
       M = -INFINITY;
       for (int i = 0; i < WK; i++) M = fmaxf(M, sm_m[i * WQ + wq][q * 16 + n16]);
       const float base = M == -INFINITY ? 0.f : M;
@@ -555,139 +601,155 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, int splits
              __builtin_amdgcn_exp2f(sm_m[i * WQ + wq][q * 16 + n16] - base);
       f = __builtin_amdgcn_exp2f(m[q] - base);
     }
+    f *= scale[q];
     if (splits == 1) f /= L;  // the softmax's sum
     if (splits > 1 && wk == 0 && g4 == 0 && live[q]) {
       part_ml[2 * (part0 + qrow[q])] = M;
       part_ml[2 * (part0 + qrow[q]) + 1] = L;
     }
-    if constexpr (WK > 1) {
+    if (!live[q]) continue;
+    float *o = WK > 1 ? sm_acc + (wave * Q16 + q * 16 + n16) * LD
+               : splits > 1
+                   ? part + (part0 + qrow[q]) * HD
+                   : a.out + (row0 + qt[q]) * a.ld_out +
+                         (size_t)(g * per_kv + qrow[q] - qt[q] * per_kv) * HD;
 #pragma unroll
-      for (int r = 0; r < 4; r++)
+    for (int r = 0; r < 4; r++)
 #pragma unroll
-        for (int c = 0; c < C; c++)
-          sm_acc[(wave * Q16 + q * 16 + n16) * HD + C * (4 * g4 + r) + c] = acc[q][c][r] * f;
-    } else if (live[q]) {
-      float *o = splits > 1 ? part + (part0 + qrow[q]) * HD
-                            : a.out + (row0 + qrow[q] / per_kv) * a.ld_out +
-                                  (size_t)(g * per_kv + qrow[q] % per_kv) * HD;
-#pragma unroll
-      for (int r = 0; r < 4; r++)
-#pragma unroll
-        for (int c = 0; c < C; c++) o[C * (4 * g4 + r) + c] = acc[q][c][r] * f;
-    }
+      for (int c = 0; c < C; c += 4) {
+        const f4 x = {acc[q][c][r] * f, acc[q][c + 1][r] * f, acc[q][c + 2][r] * f,
+                      acc[q][c + 3][r] * f};
+        if (WK > 1) *reinterpret_cast<f4 *>(o + C * (4 * g4 + r) + c) = x;
+        else *reinterpret_cast<f4u *>(o + C * (4 * g4 + r) + c) = x;
+      }
   }
-  if constexpr (WK > 1) {
+  if (WK > 1) {
     __syncthreads();
-    for (int i = tid; i < GROUP * HD; i += kThreads) {
-      const int r = i / HD, e = i % HD;  // row of the group
+    for (int i = tid; i < here * (HD / 4); i += kThreads) {
+      const int r = i / (HD / 4), e = i % (HD / 4) * 4;  // row of the group
       const int row = first + r;
-      if (row >= rows_in) break;
-      float x = 0.f;
+      f4 x = {0.f, 0.f, 0.f, 0.f};
       for (int k = 0; k < WK; k++)
-        x += sm_acc[((k * WQ + r / Q16) * Q16 + r % Q16) * HD + e];
-      if (splits > 1)
-        part[(part0 + row) * HD + e] = x;
-      else
-        a.out[(row0 + row / per_kv) * a.ld_out + (size_t)(g * per_kv + row % per_kv) * HD + e] = x;
+        x += *reinterpret_cast<const f4 *>(
+            sm_acc + ((k * WQ + r / Q16) * Q16 + r % Q16) * LD + e);
+      float *o = part + (part0 + row) * HD;
+      if (splits == 1) {
+        const int t = row / per_kv;
+        o = a.out + (row0 + t) * a.ld_out + (size_t)(g * per_kv + row - t * per_kv) * HD;
+      }
+      *reinterpret_cast<f4u *>(o + e) = x;
     }
   }
 }
 
-// The splits' parts of a query row together: one row a wave.
+// The splits' parts of a query row together: `side` waves a row (1 or 4), each
+// over every side-th split, four parts on their way at a time.
+constexpr int kMaxSplits = 64;
 template <int HD>
-__global__ __launch_bounds__(kThreads) void k_attend_merge(AttendRows a, int splits, int tile,
-                                                           int group_rows) {
+__global__ __launch_bounds__(kThreads) void k_attend_merge(AttendRows a, Shape shape, int tile,
+                                                           int side) {
+  constexpr int E = HD / 64, AHEAD = 4;
+  typedef float fe __attribute__((ext_vector_type(E)));
+  __shared__ fe sm[kWaves][64];
   const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int per_kv = a.heads / a.kv.kvh;
-  const int64_t id = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
   const int part_rows = a.kv.rows * per_kv;
-  const int row = (int)(id % part_rows);
-  const int64_t bg = id / part_rows;
-  const int g = (int)(bg % a.kv.kvh), b = (int)(bg / a.kv.kvh);
+  const int id = side == 1 ? blockIdx.x * kWaves + wave : blockIdx.x;
+  const int row = id % part_rows, bg = id / part_rows;
+  const int g = bg % a.kv.kvh, b = bg / a.kv.kvh;
   if (b >= a.kv.sequences) return;
   const KvSeq s = kv_sequence(a.kv, b);
   const int rows_in = s.count * per_kv;
   if (row >= rows_in) return;
-  float *out = a.out + ((size_t)b * a.kv.rows + row / per_kv) * a.ld_out +
-               (size_t)(g * per_kv + row % per_kv) * HD;
+  const int t = row / per_kv;
+  typedef float feu __attribute__((ext_vector_type(E), aligned(4)));
+  feu *out = reinterpret_cast<feu *>(a.out + ((size_t)b * a.kv.rows + t) * a.ld_out +
+                                     (size_t)(g * per_kv + row - t * per_kv) * HD) +
+             lane;
+  const bool writes = side == 1 || wave == 0;
   if (s.len < 0 || s.len > a.max_len || s.len > s.max_pos - s.count) {
-    for (int e = lane; e < HD; e += 64) out[e] = NAN;
+    if (writes) *out = (fe)NAN;
     return;
   }
-  const int first = row / group_rows * group_rows;
-  const Cut cut = cut_of(a, s, first / per_kv,
-                         (std::min(first + group_rows, rows_in) - 1) / per_kv, splits, tile);
-  const int n = (cut.tiles + cut.per - 1) / cut.per;  // splits that hold anything
-  const size_t base = (size_t)bg * splits * part_rows + row;
-  const float *ml = a.part + (size_t)a.kv.sequences * a.kv.kvh * splits * part_rows * HD;
-  float M = -INFINITY;
-  for (int i = lane; i < n; i += 64) M = fmaxf(M, ml[2 * (base + (size_t)i * part_rows)]);
-  M = wave_max_dpp(M);
-  const float top = M == -INFINITY ? 0.f : M;
-  float L = 0.f;
-  for (int i = lane; i < n; i += 64)
-    L += ml[2 * (base + (size_t)i * part_rows) + 1] *
-         __builtin_amdgcn_exp2f(ml[2 * (base + (size_t)i * part_rows)] - top);
-  L = wave_sum_dpp(L);
-  float x[HD / 64] = {};
-  for (int i = 0; i < n; i++) {
-    const float f = __builtin_amdgcn_exp2f(ml[2 * (base + (size_t)i * part_rows)] - top);
-#pragma unroll
-    for (int e = 0; e < HD / 64; e++)
-      x[e] += f * a.part[(base + (size_t)i * part_rows) * HD + 64 * e + lane];
+  const int n = cut_of(a, s, shape, row / shape.group * shape.group, rows_in, tile).splits;
+  const size_t base = (size_t)bg * shape.splits * part_rows + row;
+  const float *ml = a.part + (size_t)a.kv.sequences * a.kv.kvh * shape.splits * part_rows * HD;
+  // a split's maximum and sum a lane
+  float m = -INFINITY, l = 0.f;
+  if (lane < n) {
+    const float2 x = *reinterpret_cast<const float2 *>(ml + 2 * (base + (size_t)lane * part_rows));
+    m = x.x;
+    l = x.y;
   }
+  const float M = wave_max_dpp(m), top = M == -INFINITY ? 0.f : M;
+  const float f = __builtin_amdgcn_exp2f(m - top);
+  const float L = wave_sum_dpp(lane < n ? l * f : 0.f);
+  fe x = 0.f;
+  const int step = side == 1 ? 1 : kWaves;
+  for (int i0 = side == 1 ? 0 : wave; i0 < n; i0 += AHEAD * step) {
+    fe y[AHEAD];
 #pragma unroll
-  for (int e = 0; e < HD / 64; e++) out[64 * e + lane] = x[e] / L;
+    for (int i = 0; i < AHEAD; i++)
+      y[i] = reinterpret_cast<const fe *>(
+          a.part + (base + (size_t)min(i0 + i * step, n - 1) * part_rows) * HD)[lane];
+#pragma unroll
+    for (int i = 0; i < AHEAD; i++)
+      if (i0 + i * step < n) x += lane_f(f, i0 + i * step) * y[i];
+  }
+  if (side > 1) {
+    sm[wave][lane] = x;
+    __syncthreads();
+    x = (sm[0][lane] + sm[1][lane]) + (sm[2][lane] + sm[3][lane]);
+  }
+  if (writes) *out = x / L;
 }
 
-// How a call is laid out: NQ query tiles a wave, WQ waves side by side over
-// the query tiles (the others over the positions), splits of the positions.
-struct Shape {
-  int nq, wq, splits;
-  int group() const { return 16 * nq * wq; }
-};
-Shape shape_of(int sequences, int rows, int heads, int kvh, int max_len) {
+Shape shape_of(int sequences, int rows, int heads, int kvh, int max_len, int tile) {
   const int q_rows = rows * (heads / kvh);
   Shape s;
   s.nq = q_rows > 16 ? 2 : 1;
-  s.wq = q_rows > 64 ? 4 : q_rows > 32 ? 2 : 1;
-  const int64_t units = (int64_t)sequences * kvh * ((q_rows + s.group() - 1) / s.group());
-  const int tiles = (max_len + rows + 31) / 32;
-  const int64_t want = std::max<int64_t>(1, 512 / units);
-  const int most = std::max(1, tiles / (2 * (kWaves / s.wq)));
-  s.splits = (int)std::min<int64_t>(want, most);
+  const int waves = q_rows > 32 * s.nq ? 4 : q_rows > 16 * s.nq ? 2 : 1;
+  s.group = 16 * s.nq * waves;
+  const int64_t units = (int64_t)sequences * kvh * ((q_rows + s.group - 1) / s.group);
+  const int tiles = (max_len + rows + tile - 1) / tile;
+  // the work as tiles of one wave, over 8192 waves (four times what the chip
+  // holds: sequences and groups differ), but 8 or 4 tiles a wave at least (a
+  // workgroup begins and ends in the time of 3 to 6 of them, and parts cost a
+  // second launch, 4 us)
+  const int64_t work = units * waves * tiles;
+  const int wk = kWaves / waves;
+  s.per_wave = (int)std::max<int64_t>((work + 8191) / 8192, s.nq == 1 ? 8 : 4);
+  s.per_wave = std::max(s.per_wave, (tiles + kMaxSplits - 1) / kMaxSplits);
+  // (groups of fewer rows have more waves over the positions, and fewer splits)
+  s.splits = (tiles + s.per_wave * wk - 1) / (s.per_wave * wk);
   return s;
 }
 
 template <int FMT, int HD>
 void launch(const AttendRows &a, hipStream_t st) {
-  const Shape s = shape_of(a.kv.sequences, a.kv.rows, a.heads, a.kv.kvh, a.max_len);
+  const Shape s = shape_of(a.kv.sequences, a.kv.rows, a.heads, a.kv.kvh, a.max_len, kTile<FMT>);
   const int q_rows = a.kv.rows * (a.heads / a.kv.kvh);
   const unsigned blocks = (unsigned)((int64_t)s.splits * a.kv.kvh * a.kv.sequences *
-                                     ((q_rows + s.group() - 1) / s.group()));
+                                     ((q_rows + s.group - 1) / s.group));
   if (s.nq == 1)
-    hipLaunchKernelGGL((k_attend<FMT, HD, 1, 1>), dim3(blocks), dim3(kThreads), 0, st, a,
-                       s.splits);
-  else if (s.wq == 1)
-    hipLaunchKernelGGL((k_attend<FMT, HD, 2, 1>), dim3(blocks), dim3(kThreads), 0, st, a,
-                       s.splits);
-  else if (s.wq == 2)
-    hipLaunchKernelGGL((k_attend<FMT, HD, 2, 2>), dim3(blocks), dim3(kThreads), 0, st, a,
-                       s.splits);
+    hipLaunchKernelGGL((k_attend<FMT, HD, 1>), dim3(blocks), dim3(kThreads), 0, st, a, s);
   else
-    hipLaunchKernelGGL((k_attend<FMT, HD, 2, 4>), dim3(blocks), dim3(kThreads), 0, st, a,
-                       s.splits);
+    hipLaunchKernelGGL((k_attend<FMT, HD, 2>), dim3(blocks), dim3(kThreads), 0, st, a, s);
   if (s.splits > 1) {
     const int64_t rows = (int64_t)a.kv.sequences * a.kv.kvh * q_rows;
-    hipLaunchKernelGGL((k_attend_merge<HD>), dim3((unsigned)((rows + kWaves - 1) / kWaves)),
-                       dim3(kThreads), 0, st, a, s.splits, kTile<FMT>, s.group());
+    const int side = rows >= 4096 ? 1 : kWaves;
+    hipLaunchKernelGGL((k_attend_merge<HD>),
+                       dim3((unsigned)(side == 1 ? (rows + kWaves - 1) / kWaves : rows)),
+                       dim3(kThreads), 0, st, a, s, kTile<FMT>, side);
   }
 }
 
 }  // namespace
 
-size_t attend_part_bytes(int sequences, int rows, int heads, int kvh, int hd, int max_len) {
-  const Shape s = shape_of(sequences, rows, heads, kvh, max_len);
+size_t attend_part_bytes(int sequences, int rows, int heads, int kvh, int hd, int fmt,
+                         int max_len) {
+  const Shape s = shape_of(sequences, rows, heads, kvh, max_len, fmt == Q3H_KV_F32 ? 16 : 32);
   if (s.splits == 1) return 0;
   return sizeof(float) * (size_t)sequences * heads * rows * s.splits * (hd + 2);
 }

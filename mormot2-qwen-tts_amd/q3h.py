@@ -732,7 +732,7 @@ def _whole(t, shape, ordinal, dtype, name):
 
 
 def _stream(ordinal):
-    return _torch.cuda.current_stream(ordinal).cuda_stream
+    return _torch._C._cuda_getCurrentRawStream(ordinal)
 
 
 class Rope:
