@@ -53,7 +53,10 @@ typedef struct {
   int32_t layers, hidden, heads, kv_heads, head_dim, intermediate;
   float rms_eps, rope_theta;
   int32_t dtype;         /* storage: Q3H_F32 or Q3H_Q8_0 (weights and heads) */
-  int32_t kv_f16;        /* K/V cache in half floats (lm.pas:128-130) */
+  int32_t kv_f16;        /* K/V cache in half floats (lm.pas:128-130): 0 or 1; or
+                            Q3H_KV_Q8 (2; no reference counterpart): a byte per
+                            element and a scale per position and head, f32
+                            activations only */
   int32_t act_q8;        /* Q8_0 only: 1 = activations quantized per 32-block
                             (int8 products, ggml vec_dot_q8_0_q8_0); 0 = f32
                             activations times dequantized weights */
@@ -548,6 +551,45 @@ typedef struct {
 } q3h_score_args;
 int64_t q3h_token_logprobs_workspace(int rows, int vocab, int top_k);
 int q3h_token_logprobs(q3h_device *dev, const q3h_score_args *a, void *stream);
+
+/* The same operators on a context, whose rows go through the stack's layers;
+   all pointers are host memory, the calls block as q3h_forward_embeds does. */
+
+/* other rotary positions than the whole head's unscaled halves, for every
+   context of a stack with f32 activations: before the first context or frame
+   (Q3H_E_STATE); head_dim and max_positions as the stack's. rope_theta of the
+   stack's configuration is not used then. Contexts of such a stack, and of one
+   with an int8 cache, take the same calls as any other (prompts of
+   q3h_frame_start_batch each by itself; not q3h_context_time_attention). */
+int q3h_stack_set_rope(q3h_stack *s, const q3h_rope_config *cfg);
+
+/* scores of every row of a forward, as q3h_token_logprobs gives them; entropy
+   nullable, tokens and logprobs [rows][tokens_per_row] */
+typedef struct {
+  int32_t tokens_per_row, top_k;
+  const int32_t *tokens;
+  float *logprobs, *entropy;
+  int32_t *top_ids;
+  float *top_logprobs;
+} q3h_row_scores;
+
+/* A tree of drafted rows: x [rows][hidden], at most Q3H_TREE_MAX_ROWS, row r
+   after row parents[r] (below r; -1: after the context's last position). Every
+   row's logits [rows][head rows], normed state [rows][hidden] and scores
+   (each nullable; scores need a head). The context's length stays; the rows
+   wait behind it for q3h_context_keep, until another call writes to the
+   context. f32 activations. rows <= 0 does nothing. */
+int q3h_forward_tree(q3h_context *c, const float *x, int rows, const int32_t *parents, int head,
+                     const q3h_row_scores *scores, float *logits, float *normed);
+/* The rows kept [n] of the last q3h_forward_tree, a path from a root down (each
+   row the parent of the next), become the context's next n positions; the
+   others are dropped (n 0: all). Q3H_E_STATE when there is no tree. */
+int q3h_context_keep(q3h_context *c, const int32_t *kept, int n);
+/* q3h_forward_embeds of rows whose every position is scored, the logits (of
+   every row, nullable) staying on the device otherwise; normed [rows][hidden]
+   nullable. Any stack. */
+int q3h_forward_score(q3h_context *c, const float *x, int rows, int head,
+                      const q3h_row_scores *scores, float *logits, float *normed);
 
 /* ---- helpers ---- */
 

@@ -10,6 +10,7 @@
 
 #include "q3h.h"
 #include "q3h_api_internal.h"
+#include "q3h_draft.h"
 
 using namespace q3h;
 
@@ -101,16 +102,29 @@ void Work::ensure(const q3h_stack *s, int rows, int splits, int head_rows) {
   gen++;
 }
 
-bool work_carve(const q3h_stack *s, int rows, int splits, int head_rows, void *base, size_t cap,
-                Work &w) {
+void Work::ensure_tree(size_t bytes) {
+  if (bytes <= tree_bytes) return;
+  dev_free(tree);
+  tree = nullptr;
+  tree_bytes = 0;
+  tree = (float *)dev_alloc(bytes);
+  tree_bytes = bytes;
+  gen++;
+}
+
+bool work_carve(const q3h_stack *s, int rows, int splits, int head_rows, size_t tree_bytes,
+                void *base, size_t cap, Work &w) {
   size_t off = 0;
   bool fits = true;
-  work_fields(s, rows, splits, head_rows, w, [&](void **slot, size_t bytes) {
+  auto carve = [&](void **slot, size_t bytes) {
     off = (off + 255) & ~(size_t)255;
     fits = fits && off + bytes <= cap;
     *slot = fits ? (char *)base + off : nullptr;
     off += bytes;
-  });
+  };
+  work_fields(s, rows, splits, head_rows, w, carve);
+  if (tree_bytes) carve((void **)&w.tree, tree_bytes);
+  w.tree_bytes = tree_bytes;
   w.rows_cap = rows;
   w.splits_cap = splits;
   w.head_cap = head_rows;
@@ -130,6 +144,9 @@ void Work::release() {
   dev_free(xa.q);
   dev_free(xb.q);
   dev_free(gpart);
+  dev_free(tree);
+  tree = nullptr;
+  tree_bytes = 0;
   x3n = x3a = nullptr;
   xa = QAct{};
   xb = QAct{};
@@ -141,11 +158,19 @@ void Work::release() {
 }
 
 int attention_splits(const q3h_stack *s, int positions) {
-  return attn_splits(positions, s->cfg.kv_f16 != 0);
+  return s->ext ? 0 : attn_splits(positions, s->cfg.kv_f16 != 0);
 }
 
 int attention_splits_upto(const q3h_stack *s, int positions) {
-  return attn_splits_upto(positions, s->cfg.kv_f16 != 0);
+  return s->ext ? 0 : attn_splits_upto(positions, s->cfg.kv_f16 != 0);
+}
+
+size_t tree_bytes(const q3h_stack *s, int n, int rows, int positions, bool drafted) {
+  const q3h_stack_config &c = s->cfg;
+  if (!s->ext && !drafted) return 0;
+  // single rows: of any length (a captured launch serves many)
+  if (rows == 1) return sizeof(float) * (size_t)n * c.heads * kAttendSplits * (c.head_dim + 2);
+  return attend_part_bytes(n, rows, c.heads, c.kv_heads, c.head_dim, c.kv_f16, positions);
 }
 
 void linear(const q3h_stack *s, Work &w, const Mat &W, const float *x, int ldx, int M,
@@ -199,6 +224,59 @@ static void prompt_attn_x(const q3h_stack *s, Work &w, AttnArgs &at, int M, int 
       launch_attn_x_prompt(at, M, positions, c.kv_f16 != 0, w.xa, st))
     return;
   launch_attn_x(at, M, fused, c.kv_f16 != 0, 0, w.xa, c.max_positions, st);
+}
+
+// Layer l's keys and values of the M rows of w.qkv written to the cache and its
+// attention to w.att by the kernels of drafted rows: stacks with an int8 cache
+// or rotary positions of their own, and drafted trees on any stack.
+static void attend_drafted(const q3h_stack *s, Work &w, int l, int M, int positions, bool fused,
+                           const LayerIO &io, hipStream_t st) {
+  const q3h_stack_config &c = s->cfg;
+  const Layer &L = s->layers[l];
+  const int hd = c.head_dim, NQ = c.heads * hd, NKV = c.kv_heads * hd, ldq = NQ + 2 * NKV;
+  const int rows = fused ? 1 : io.single_context ? M : io.rows_each;
+  require(rows > 0 && M % rows == 0, Q3H_E_ARG, "rows of several contexts on this stack");
+  AppendRows a{};
+  a.kv.rd = w.rd;
+  a.kv.layers = c.layers;
+  a.kv.kvh = c.kv_heads;
+  a.kv.layer = l;
+  a.kv.sequences = M / rows;
+  a.kv.rows = rows;
+  a.heads = c.heads;
+  a.q = w.qkv;
+  a.k = w.qkv + NQ;
+  a.v = w.qkv + NQ + NKV;
+  a.ldq = a.ldk = a.ldv = a.ld_out = ldq;
+  a.q_out = w.qkv;
+  a.q_norm = L.q_norm;
+  a.k_norm = L.k_norm;
+  a.eps = c.rms_eps;
+  a.rot_dim = hd;
+  if (s->rope) {
+    a.table = s->rope->table;
+    a.rot_dim = s->rope->cfg.rot_dim;
+    a.interleaved = s->rope->cfg.interleaved;
+  } else {
+    a.table32 = reinterpret_cast<const float2 *>(s->rope_cs);
+  }
+  a.parents = io.parents;
+  launch_cache_append(a, hd, c.kv_f16, st);
+  AttendRows t{};
+  t.kv = a.kv;
+  t.heads = c.heads;
+  t.max_len = positions;
+  t.scale = 1.0f / std::sqrt((float)hd);
+  t.q = w.qkv;
+  t.ldq = ldq;
+  t.out = w.att;
+  t.ld_out = NQ;
+  t.parents = io.parents;
+  t.part = w.tree;
+  require(attend_part_bytes(M / rows, rows, c.heads, c.kv_heads, hd, c.kv_f16, positions) <=
+              w.tree_bytes,
+          Q3H_E_HIP, "the attention's parts have no room");
+  launch_cache_attend(t, hd, c.kv_f16, st);
 }
 
 // The int8 path over M <= kPartialRows rows: every product leaves its chunk
@@ -296,7 +374,8 @@ static void run_layers_x3(const q3h_stack *s, Work &w, int M, int positions, boo
   for (int l = 0; l < c.layers; l++) {
     const Layer &L = s->layers[l];
     launch_gemm_x3(L.qkv, w.x3n, M, w.qkv, ldq, st);
-    if (!fused)
+    const bool drafted = s->ext || io.parents;
+    if (!fused && !drafted)
       launch_qk_rope_append(w.qkv, ldq, w.rd, M, l, c.heads, c.kv_heads, hd, L.q_norm, L.k_norm,
                             eps, s->rope_cs, kv16, st);
     AttnArgs at{};
@@ -313,7 +392,10 @@ static void run_layers_x3(const q3h_stack *s, Work &w, int M, int positions, boo
     at.tiles = io.tiles;
     at.n_tiles = io.n_tiles;
     at.tile_rows = io.tile_rows;
-    if (!fused && (io.tiles || io.single_context)) {
+    if (drafted) {
+      attend_drafted(s, w, l, M, positions, fused, io, st);
+      launch_x3_rows(w.att, NQ, M, NQ, w.x3a, cut, st);
+    } else if (!fused && (io.tiles || io.single_context)) {
       at.out3 = w.x3a;
       at.cut3 = cut;
       launch_attn_prefill(at, M, kv16, st);
@@ -343,14 +425,15 @@ static void run_layers_f32(const q3h_stack *s, Work &w, int M, int positions, bo
   for (int l = 0; l < c.layers; l++) {
     const Layer &L = s->layers[l];
     // q/k/v as K slices (Q8_0, 17-64 rows of a prefill) added by the append
-    const int qs = fused ? 0 : q8x_slices(L.qkv, M);
+    const bool drafted = s->ext || io.parents;
+    const int qs = fused || drafted ? 0 : q8x_slices(L.qkv, M);
     if (qs > 0 && qs <= kRopeMaxSlices) {
       launch_gemm_f32_part(L.qkv, w.normed, H, M, w.gpart, st);
       launch_qk_rope_append(w.qkv, ldq, w.rd, M, l, c.heads, c.kv_heads, hd, L.q_norm,
                             L.k_norm, eps, s->rope_cs, kv16, st, w.gpart, qs);
     } else {
       launch_gemm_f32(L.qkv, w.normed, H, M, EPI_STORE, w.qkv, ldq, st);
-      if (!fused)
+      if (!fused && !drafted)
         launch_qk_rope_append(w.qkv, ldq, w.rd, M, l, c.heads, c.kv_heads, hd, L.q_norm,
                               L.k_norm, eps, s->rope_cs, kv16, st);
     }
@@ -365,7 +448,9 @@ static void run_layers_f32(const q3h_stack *s, Work &w, int M, int positions, bo
     at.rope_cs = reinterpret_cast<const float2 *>(s->rope_cs);
     at.out = w.att;
     at.part = w.part;
-    if (!fused && single_context && M >= kPrefillRows)
+    if (drafted)
+      attend_drafted(s, w, l, M, positions, fused, io, st);
+    else if (!fused && single_context && M >= kPrefillRows)
       launch_attn_prefill(at, M, kv16, st);
     else
       launch_attn(at, M, positions, fused, kv16, st);
@@ -429,7 +514,8 @@ void run_layers(const q3h_stack *s, Work &w, int M, int positions, bool fused, h
       continue;
     }
     // QK-norm, RoPE, K/V append (in the attention prologue when fused)
-    if (!fused)
+    const bool drafted = s->ext || io.parents;
+    if (!fused && !drafted)
       launch_qk_rope_append(w.qkv, ldq, w.rd, M, l, c.heads, c.kv_heads, hd, L.q_norm,
                             L.k_norm, c.rms_eps, s->rope_cs, kv16, st);
     // GQA attention
@@ -445,7 +531,9 @@ void run_layers(const q3h_stack *s, Work &w, int M, int positions, bool fused, h
     at.out = w.att;
     at.part = w.part;
     at.layers = c.layers;  // decode: the next layer's cache rows loaded one launch ahead
-    if (!fused && io.single_context && M >= kPrefillRows) {
+    if (drafted) {
+      attend_drafted(s, w, l, M, positions, fused, io, st);
+    } else if (!fused && io.single_context && M >= kPrefillRows) {
       launch_attn_prefill(at, M, kv16, st);
     } else if (attn_merge_o_supported(at, L.o, M, positions, kv16)) {
       // one decode row over a split context: the splits' merge in the o_proj
@@ -729,6 +817,7 @@ void destroy_stack(q3h_stack *s) {
   for (auto &h : s->heads) free_mat(h);
   dev_free(s->final_norm);
   dev_free(s->rope_cs);
+  if (s->rope) (void)q3h_rope_destroy(s->rope);
   if (s->stream) (void)hipStreamDestroy(s->stream);
 }
 
@@ -761,9 +850,13 @@ extern "C" int q3h_stack_create(q3h_device *dev, const q3h_stack_config *cfg,
     require(c.dtype == Q3H_Q8_0 || w->src_dtype != Q3H_Q8_0, Q3H_E_ARG,
             "q3h_stack_create: an f32 stack takes f32 or BF16 weights");
     require(c.max_positions > 0, Q3H_E_ARG, "q3h_stack_create: max_positions <= 0");
-    require(c.max_positions <= attn_max_positions(c.kv_f16 != 0), Q3H_E_ARG,
-            "q3h_stack_create: max_positions above " +
-                std::to_string(attn_max_positions(c.kv_f16 != 0)));
+    require(c.kv_f16 >= Q3H_KV_F32 && c.kv_f16 <= Q3H_KV_Q8, Q3H_E_ARG,
+            "q3h_stack_create: kv_f16 must be Q3H_KV_F32, Q3H_KV_F16 or Q3H_KV_Q8");
+    require(c.kv_f16 != Q3H_KV_Q8 || !c.act_q8, Q3H_E_ARG,
+            "q3h_stack_create: act_q8 takes an f32 or f16 cache");
+    const int most = attn_max_positions(c.kv_f16 != Q3H_KV_F32);
+    require(c.max_positions <= most, Q3H_E_ARG,
+            "q3h_stack_create: max_positions above " + std::to_string(most));
     require(c.act_q8 == 0 || c.dtype == Q3H_Q8_0, Q3H_E_ARG,
             "q3h_stack_create: act_q8 needs Q8_0 weights");
     require(c.act_q8 == 0 ||
@@ -784,6 +877,7 @@ extern "C" int q3h_stack_create(q3h_device *dev, const q3h_stack_config *cfg,
     s = new q3h_stack();
     s->dev = dev;
     s->cfg = c;
+    s->ext = c.kv_f16 == Q3H_KV_Q8;
     check_hip(hipStreamCreateWithFlags(&s->stream, hipStreamNonBlocking), "hipStreamCreate");
     const int H = c.hidden, hd = c.head_dim, NQ = c.heads * hd, NKV = c.kv_heads * hd;
     const int I = c.intermediate;
@@ -903,6 +997,26 @@ extern "C" int q3h_stack_add_head(q3h_stack *s, const void *w, int rows, int src
   });
 }
 
+extern "C" int q3h_stack_set_rope(q3h_stack *s, const q3h_rope_config *cfg) {
+  return guard([&] {
+    require(s && cfg, Q3H_E_ARG, "q3h_stack_set_rope: NULL argument");
+    require(!s->cfg.act_q8, Q3H_E_ARG,
+            "q3h_stack_set_rope: a stack with f32 activations is required");
+    require(cfg->head_dim == s->cfg.head_dim, Q3H_E_ARG,
+            "q3h_stack_set_rope: head_dim is not the stack's");
+    require(cfg->max_positions == s->cfg.max_positions, Q3H_E_ARG,
+            "q3h_stack_set_rope: max_positions is not the stack's");
+    require(s->contexts.load() == 0, Q3H_E_STATE,
+            "q3h_stack_set_rope: contexts or frames already use this stack");
+    q3h_rope *r = nullptr;
+    const int rc = q3h_rope_create(s->dev, cfg, &r);
+    if (rc != 0) throw Error{rc, g_last_error};
+    if (s->rope) (void)q3h_rope_destroy(s->rope);
+    s->rope = r;
+    s->ext = true;
+  });
+}
+
 extern "C" int64_t q3h_stack_bytes(const q3h_stack *s) { return s ? s->bytes : 0; }
 
 extern "C" int q3h_stack_destroy(q3h_stack *s) {
@@ -931,13 +1045,14 @@ q3h_context *new_context(q3h_stack *s, int max_positions) {
   try {
     check_hip(hipStreamCreateWithFlags(&ctx->stream, hipStreamNonBlocking), "hipStreamCreate");
     const size_t n = (size_t)c.layers * c.kv_heads * max_positions * c.head_dim;
-    const size_t esz = c.kv_f16 ? 2 : 4;
-    // keys then values in one allocation: v = k + n elements
-    ctx->k = dev_alloc(2 * n * esz);
+    const size_t esz = kv_elem_bytes(c.kv_f16);
+    const size_t bytes = kv_bytes(c.kv_f16, c.layers, c.kv_heads, max_positions, c.head_dim);
+    // keys then values in one allocation: v = k + n elements (int8: then the scales)
+    ctx->k = dev_alloc(bytes);
     ctx->v = static_cast<char *>(ctx->k) + n * esz;
     // zeros: a position is finite before it is first written (the long-context
     // attention reads rows past the context with weight 0)
-    check_hip(hipMemset(ctx->k, 0, 2 * n * esz), "zero K/V");
+    check_hip(hipMemset(ctx->k, 0, bytes), "zero K/V");
     ctx->dev = (CtxDev *)dev_alloc(sizeof(CtxDev));
     ctx->dev_arr = (CtxDev **)dev_alloc(sizeof(CtxDev *));
     CtxDev h{ctx->k, ctx->v, max_positions, 0};
@@ -962,6 +1077,7 @@ void free_context(q3h_context *ctx) {
   ctx->w.release();
   if (ctx->pin) (void)hipHostFree(ctx->pin);
   dev_free(ctx->probe);
+  dev_free(ctx->draft);
   dev_free(ctx->k);  // the values share this allocation
   dev_free(ctx->dev);
   dev_free(ctx->dev_arr);
@@ -974,6 +1090,7 @@ void set_len(q3h_context *c, int len, hipStream_t st) {
             "set length");
   check_hip(hipStreamSynchronize(st), "set length sync");
   c->len = len;
+  c->drafted.clear();
 }
 
 }  // namespace q3h
@@ -1031,8 +1148,12 @@ extern "C" int q3h_context_fill_kv(q3h_context *c, const float *k, const float *
           check_hip(hipMemcpyAsync(st, which ? v : k, n * sizeof(float), hipMemcpyHostToDevice,
                                    c->stream),
                     "fill kv upload");
-          launch_kv_fill(st, cf.layers, cf.kv_heads, len, cf.head_dim, which ? c->v : c->k,
-                         c->max_pos, cf.kv_f16 != 0, c->stream);
+          if (cf.kv_f16 == Q3H_KV_Q8)
+            launch_q8_fill(st, (char *)c->k, which, cf.layers, cf.kv_heads, len, cf.head_dim,
+                           c->max_pos, c->stream);
+          else
+            launch_kv_fill(st, cf.layers, cf.kv_heads, len, cf.head_dim, which ? c->v : c->k,
+                           c->max_pos, cf.kv_f16 != 0, c->stream);
           check_hip(hipGetLastError(), "kv fill kernel");
           check_hip(hipStreamSynchronize(c->stream), "fill kv sync");
         }
@@ -1057,8 +1178,12 @@ extern "C" int q3h_context_read_kv(q3h_context *c, int layer, float *k, float *v
     float *st = (float *)dev_alloc(n * sizeof(float));
     try {
       for (int which = 0; which < 2; which++) {
-        launch_kv_read(which ? c->v : c->k, layer, cf.kv_heads, c->len, cf.head_dim, c->max_pos,
-                       cf.kv_f16 != 0, st, c->stream);
+        if (cf.kv_f16 == Q3H_KV_Q8)
+          launch_q8_read((const char *)c->k, which, cf.layers, layer, cf.kv_heads, c->len,
+                         cf.head_dim, c->max_pos, st, c->stream);
+        else
+          launch_kv_read(which ? c->v : c->k, layer, cf.kv_heads, c->len, cf.head_dim, c->max_pos,
+                         cf.kv_f16 != 0, st, c->stream);
         check_hip(hipGetLastError(), "kv read kernel");
         check_hip(hipMemcpyAsync(which ? v : k, st, n * sizeof(float), hipMemcpyDeviceToHost,
                                  c->stream),
@@ -1085,6 +1210,9 @@ extern "C" int q3h_context_time_attention(q3h_context *c, int iters, float *us_p
     const q3h_stack_config &cf = s->cfg;
     require(!cf.act_q8, Q3H_E_ARG,
             "q3h_context_time_attention: a stack with f32 activations is required");
+    require(!s->ext, Q3H_E_ARG,
+            "q3h_context_time_attention: an f32 or f16 cache and the stack's own rotary "
+            "positions are required");
     require(c->len + 1 <= c->max_pos, Q3H_E_CAPACITY, "q3h_context_time_attention: context full");
     check_hip(hipSetDevice(s->dev->ordinal), "hipSetDevice");
     const int positions = c->len + 1;
@@ -1173,7 +1301,7 @@ int forward_positions(const q3h_context *c, int rows) {
 // kPrefillRows rows or more (the causal prefill attention), else those of the
 // decode attention over forward_positions
 int forward_splits(const q3h_context *c, int rows) {
-  if (c->s->cfg.act_q8 || rows >= kPrefillRows) return 0;
+  if (c->s->cfg.act_q8 || c->s->ext || rows >= kPrefillRows) return 0;
   return attention_splits(c->s, forward_positions(c, rows));
 }
 
@@ -1267,6 +1395,7 @@ void forward_rows(q3h_context *c, Work &w, const float *x, int rows, int head, f
   const int head_rows = head >= 0 ? s->heads[head].N : 0;
   const int positions = forward_positions(c, rows);
   hipStream_t st = c->stream;
+  c->drafted.clear();
   // results (and a single row) are copied through pinned host memory where the
   // call may allocate it (a pageable copy is staged by the runtime, which waits
   // for the stream at each: 10 us a copy)
@@ -1343,6 +1472,7 @@ extern "C" int q3h_forward_embeds(q3h_context *c, const float *x, int rows, int 
     check_hip(hipSetDevice(s->dev->ordinal), "hipSetDevice");
     const int head_rows = head >= 0 ? s->heads[head].N : 0;
     c->w.ensure(s, rows, forward_splits(c, rows), head_rows);
+    c->w.ensure_tree(tree_bytes(s, 1, rows, forward_positions(c, rows)));
     // one row (a decode step): the forward replayed from a captured graph; a
     // prompt's results through pinned memory where the context has it, or from
     // its second prompt on (the first does not pay for the allocation)
@@ -1361,6 +1491,7 @@ extern "C" int q3h_forward_embeds_probe(q3h_context *c, const float *x, int rows
     check_hip(hipSetDevice(s->dev->ordinal), "hipSetDevice");
     const int head_rows = head >= 0 ? s->heads[head].N : 0;
     c->w.ensure(s, rows, forward_splits(c, rows), head_rows);
+    c->w.ensure_tree(tree_bytes(s, 1, rows, forward_positions(c, rows)));
     forward_rows(c, c->w, x, rows, head, logits, normed_last, layer_out, false, normed_rows);
   });
 }
@@ -1379,7 +1510,8 @@ extern "C" int q3h_forward_embeds_noalloc(q3h_context *c, const float *x, int ro
     const int head_rows = head >= 0 ? s->heads[head].N : 0;
     Work w;  // a view of the array: owns nothing
     require(work_carve(s, rows, forward_splits(c, rows), head_rows,
-                       dev->scratch, Q3H_NOALLOC_SCRATCH_BYTES, w),
+                       tree_bytes(s, 1, rows, forward_positions(c, rows)), dev->scratch,
+                       Q3H_NOALLOC_SCRATCH_BYTES, w),
             Q3H_E_CAPACITY,
             "q3h_forward_embeds_noalloc: the work buffers of " + std::to_string(rows) +
                 " rows at " + std::to_string(c->len + rows) + " positions exceed the " +
@@ -1438,6 +1570,8 @@ extern "C" int q3h_forward_embeds_batch(q3h_context *const *ctxs, int n, const f
     const int positions = cover ? graph_cover(maxlen, c0->max_pos) : maxlen;
     Work &w = c0->w;
     w.ensure(s, n, attention_splits(s, positions), head_rows);
+    w.ensure_tree(tree_bytes(s, n, 1, positions));
+    for (int i = 0; i < n; i++) ctxs[i]->drafted.clear();
     hipStream_t st = c0->stream;
     auto enqueue = [&] {
       launch_prep(w.ctx_arr, nullptr, n, 1, w.rd, st);
@@ -1487,6 +1621,188 @@ extern "C" int q3h_forward_embeds_batch(q3h_context *const *ctxs, int n, const f
     if (exec && normed) std::memcpy(normed, nm, sizeof(float) * nx);
     if (exec && logits && heads) std::memcpy(logits, lg, sizeof(float) * nl);
     for (int i = 0; i < n; i++) ctxs[i]->len += 1;
+  });
+}
+
+// ---------------------------------------------------------------------------
+// drafted trees, and rows scored on the device
+
+namespace {
+
+// bytes of c's device memory for trees and scores (c's stream idle)
+char *draft_space(q3h_context *c, size_t bytes) {
+  if (c->draft_bytes < bytes) {
+    dev_free(c->draft);
+    c->draft = nullptr;
+    c->draft_bytes = 0;
+    c->draft = (char *)dev_alloc(bytes);
+    c->draft_bytes = bytes;
+  }
+  return c->draft;
+}
+
+void check_scores(const q3h_context *c, int head, const q3h_row_scores *sc, const char *who) {
+  if (!sc) return;
+  const std::string w(who);
+  require(head >= 0, Q3H_E_ARG, w + ": scores need a head");
+  require(sc->tokens_per_row >= 0 && sc->tokens_per_row <= 4096, Q3H_E_ARG,
+          w + ": tokens_per_row in [0, 4096]");
+  require(sc->tokens_per_row == 0 || (sc->tokens && sc->logprobs), Q3H_E_ARG,
+          w + ": NULL tokens or logprobs");
+  require(sc->top_k >= 0 && sc->top_k <= Q3H_TOP_MAX && sc->top_k <= c->s->heads[head].N,
+          Q3H_E_ARG, w + ": top_k in [0, min(head rows, " + std::to_string(Q3H_TOP_MAX) + ")]");
+  require(sc->top_k == 0 || (sc->top_ids && sc->top_logprobs), Q3H_E_ARG,
+          w + ": NULL top_ids or top_logprobs");
+}
+
+// x's rows through the layers of c (parents: a drafted tree, whose rows stay
+// behind the context's length), the final norm and the head of every row, its
+// scores; blocks until the outputs are in host memory
+void forward_all_rows(q3h_context *c, const float *x, int rows, const int32_t *parents, int head,
+                      const q3h_row_scores *sc, float *logits, float *normed) {
+  q3h_stack *s = c->s;
+  const int H = s->cfg.hidden, V = head >= 0 ? s->heads[head].N : 0;
+  hipStream_t st = c->stream;
+  const int positions = parents ? c->len + rows : forward_positions(c, rows);
+  Work &w = c->w;
+  w.ensure(s, rows, parents ? 0 : forward_splits(c, rows), V);
+  w.ensure_tree(tree_bytes(s, 1, rows, positions, parents != nullptr));
+  // the call's device memory: parents; tokens, scores, their workspace
+  size_t need = 0;
+  auto take = [&](size_t bytes) {
+    const size_t at = need;
+    need += (bytes + 255) / 256 * 256;
+    return at;
+  };
+  const int m = sc ? sc->tokens_per_row : 0, k = sc ? sc->top_k : 0;
+  const size_t cells = (size_t)rows * m, tops = (size_t)rows * k;
+  const size_t work = sc ? score_work_bytes(rows, V, k) : 0;
+  const size_t at_parents = take(sizeof(int32_t) * rows), at_tokens = take(4 * cells),
+               at_logp = take(4 * cells), at_entropy = take(4 * (size_t)rows),
+               at_ids = take(4 * tops), at_top = take(4 * tops), at_work = take(work);
+  char *const mem = draft_space(c, need);
+  c->drafted.clear();
+  check_hip(hipMemcpyAsync(w.h, x, sizeof(float) * rows * H, hipMemcpyHostToDevice, st),
+            "upload x");
+  if (parents)
+    check_hip(hipMemcpyAsync(mem + at_parents, parents, sizeof(int32_t) * rows,
+                             hipMemcpyHostToDevice, st),
+              "upload parents");
+  if (cells)
+    check_hip(hipMemcpyAsync(mem + at_tokens, sc->tokens, 4 * cells, hipMemcpyHostToDevice, st),
+              "upload tokens");
+  LayerIO io;
+  io.single_context = true;
+  if (parents) io.parents = reinterpret_cast<const int32_t *>(mem + at_parents);
+  launch_prep(c->dev_arr, nullptr, 1, rows, w.rd, st);
+  run_layers(s, w, rows, positions, rows == 1 && !parents, st, io);
+  launch_rmsnorm_rows(w.h, H, rows, H, s->final_norm, s->cfg.rms_eps, w.normed, H, st);
+  if (normed)
+    check_hip(hipMemcpyAsync(normed, w.normed, sizeof(float) * rows * H, hipMemcpyDeviceToHost,
+                             st),
+              "download states");
+  if (head >= 0 && (logits || sc))
+    linear(s, w, s->heads[head], w.normed, H, rows, nullptr, w.logits, V, EPI_STORE, nullptr, st);
+  if (sc) {
+    ScoreRows a{};
+    a.logits = w.logits;
+    a.ld = V;
+    a.rows = rows;
+    a.vocab = V;
+    a.tokens_per_row = m;
+    a.top_k = k;
+    a.tokens = reinterpret_cast<const int32_t *>(mem + at_tokens);
+    a.logprobs = reinterpret_cast<float *>(mem + at_logp);
+    a.entropy = reinterpret_cast<float *>(mem + at_entropy);
+    a.top_ids = reinterpret_cast<int32_t *>(mem + at_ids);
+    a.top_logprobs = reinterpret_cast<float *>(mem + at_top);
+    a.work = mem + at_work;
+    launch_token_scores(a, st);
+  }
+  if (!parents) launch_advance(c->dev_arr, nullptr, 1, rows, st);
+  check_hip(hipGetLastError(), "forward kernels");
+  auto down = [&](void *to, const void *from, size_t bytes) {
+    if (to && bytes)
+      check_hip(hipMemcpyAsync(to, from, bytes, hipMemcpyDeviceToHost, st), "download scores");
+  };
+  if (head >= 0) down(logits, w.logits, sizeof(float) * rows * V);
+  if (sc) {
+    down(sc->logprobs, mem + at_logp, 4 * cells);
+    down(sc->entropy, mem + at_entropy, 4 * (size_t)rows);
+    down(sc->top_ids, mem + at_ids, 4 * tops);
+    down(sc->top_logprobs, mem + at_top, 4 * tops);
+  }
+  check_hip(hipStreamSynchronize(st), "forward sync");
+  if (parents) c->drafted.assign(parents, parents + rows);
+  else c->len += rows;
+}
+
+}  // namespace
+
+extern "C" int q3h_forward_tree(q3h_context *c, const float *x, int rows, const int32_t *parents,
+                                int head, const q3h_row_scores *scores, float *logits,
+                                float *normed) {
+  return guard([&] {
+    if (!forward_args(c, x, rows, head, "q3h_forward_tree")) return;
+    require(!c->s->cfg.act_q8, Q3H_E_ARG,
+            "q3h_forward_tree: a stack with f32 activations is required");
+    require(parents != nullptr, Q3H_E_ARG, "q3h_forward_tree: parents is NULL");
+    require(rows <= Q3H_TREE_MAX_ROWS, Q3H_E_CAPACITY,
+            "q3h_forward_tree: a tree has at most " + std::to_string(Q3H_TREE_MAX_ROWS) + " rows");
+    for (int r = 0; r < rows; r++)
+      require(parents[r] >= -1 && parents[r] < r, Q3H_E_ARG,
+              "q3h_forward_tree: the parent of row " + std::to_string(r) + " is not below it");
+    check_scores(c, head, scores, "q3h_forward_tree");
+    check_hip(hipSetDevice(c->s->dev->ordinal), "hipSetDevice");
+    forward_all_rows(c, x, rows, parents, head, scores, logits, normed);
+  });
+}
+
+extern "C" int q3h_context_keep(q3h_context *c, const int32_t *kept, int n) {
+  return guard([&] {
+    require(c != nullptr && n >= 0 && (n == 0 || kept), Q3H_E_ARG,
+            "q3h_context_keep: invalid argument");
+    require(!c->drafted.empty(), Q3H_E_STATE,
+            "q3h_context_keep: no tree since the context was last written");
+    const int rows = (int)c->drafted.size();
+    for (int i = 0; i < n; i++)
+      require(kept[i] >= 0 && kept[i] < rows && c->drafted[kept[i]] == (i ? kept[i - 1] : -1),
+              Q3H_E_ARG, "q3h_context_keep: the kept rows are not a path from a root of the tree");
+    check_hip(hipSetDevice(c->s->dev->ordinal), "hipSetDevice");
+    if (n > 0 && kept[n - 1] != n - 1) {
+      const q3h_stack_config &cf = c->s->cfg;
+      // [kept | their count] (the space of the tree's own call is larger)
+      std::vector<int32_t> v(Q3H_TREE_MAX_ROWS + 1, 0);
+      std::copy(kept, kept + n, v.begin());
+      v[Q3H_TREE_MAX_ROWS] = n;
+      int32_t *const d = reinterpret_cast<int32_t *>(draft_space(c, sizeof(int32_t) * v.size()));
+      check_hip(hipMemcpyAsync(d, v.data(), sizeof(int32_t) * v.size(), hipMemcpyHostToDevice,
+                               c->stream),
+                "upload kept rows");
+      KvView view{};
+      view.base = static_cast<char *>(c->k);
+      view.lens = &c->dev->len;
+      view.counts = d + Q3H_TREE_MAX_ROWS;
+      view.layers = cf.layers;
+      view.kvh = cf.kv_heads;
+      view.max_pos = c->max_pos;
+      view.sequences = 1;
+      view.rows = rows;
+      launch_cache_keep(view, d, cf.head_dim, cf.kv_f16, c->stream);
+      check_hip(hipGetLastError(), "keep kernel");
+    }
+    set_len(c, c->len + n, c->stream);
+  });
+}
+
+extern "C" int q3h_forward_score(q3h_context *c, const float *x, int rows, int head,
+                                 const q3h_row_scores *scores, float *logits, float *normed) {
+  return guard([&] {
+    if (!forward_args(c, x, rows, head, "q3h_forward_score")) return;
+    require(scores != nullptr, Q3H_E_ARG, "q3h_forward_score: scores is NULL");
+    check_scores(c, head, scores, "q3h_forward_score");
+    check_hip(hipSetDevice(c->s->dev->ordinal), "hipSetDevice");
+    forward_all_rows(c, x, rows, nullptr, head, scores, logits, normed);
   });
 }
 

@@ -173,6 +173,10 @@ struct Work {
   // activations): the normed rows, and the attention / SwiGLU outputs; the
   // memory of att and act, which that path needs at other times only
   uint16_t *x3n = nullptr, *x3a = nullptr;
+  // parts of the attention over drafted rows (q3h_draft.h)
+  float *tree = nullptr;
+  size_t tree_bytes = 0;
+  void ensure_tree(size_t bytes);
   void ensure(const struct ::q3h_stack *s, int rows, int splits, int head_rows);
   void release();
 };
@@ -180,8 +184,12 @@ struct Work {
 // w's buffers for (rows, splits, head_rows) carved from [base, base + cap),
 // each at a 256-byte boundary (w owns nothing: never release it); false when
 // they do not fit
-bool work_carve(const struct ::q3h_stack *s, int rows, int splits, int head_rows, void *base,
-                size_t cap, Work &w);
+bool work_carve(const struct ::q3h_stack *s, int rows, int splits, int head_rows,
+                size_t tree_bytes, void *base, size_t cap, Work &w);
+// the bytes of Work::tree for a forward of n contexts, rows rows each, over up to
+// `positions` positions: those of stacks whose every attention is that over
+// drafted rows, or of a drafted tree
+size_t tree_bytes(const struct ::q3h_stack *s, int n, int rows, int positions, bool drafted = false);
 
 // attention splits (the partial buffer) for contexts of up to `positions`
 int attention_splits(const struct ::q3h_stack *s, int positions);
@@ -232,6 +240,11 @@ struct LayerIO {
   // the rows come in pairs, row 2i + 1 at the position after row 2i's in the
   // same context (the int8 path over few rows then runs the fused attention)
   bool row_pairs = false;
+  // stacks whose every attention is that over drafted rows (q3h_stack::ext): rows
+  // of each context, when there are several of several
+  int rows_each = 0;
+  // the rows are a tree of drafted rows of one context: their parents (device)
+  const int32_t *parents = nullptr;
 };
 // whether run_layers takes the int8 partial-product path for M rows of stack s
 bool partial_path(const struct ::q3h_stack *s, int M);
@@ -254,6 +267,10 @@ struct q3h_stack {
   std::vector<q3h::Layer> layers;
   float *final_norm = nullptr;
   float *rope_cs = nullptr;  // [max_positions][head_dim / 2] (cos, sin)
+  // an int8 cache or other rotary positions than rope_cs: keys and values are
+  // written and attended by the kernels of drafted rows (q3h_draft.h)
+  bool ext = false;
+  struct ::q3h_rope *rope = nullptr;
   std::vector<q3h::Mat> heads;
   int64_t bytes = 0, head_bytes = 0;
   int64_t aux_bytes = 0;  // the split-bf16 planes of f32 layers (not in StackBytes)
@@ -286,6 +303,11 @@ struct q3h_context {
   float *pin = nullptr;
   size_t pin_floats = 0;
   bool prompted = false;  // a forward of several rows has run
+  // the tree of the last q3h_forward_tree, its rows behind len, until another call
+  // writes there; device memory for trees and scores
+  std::vector<int32_t> drafted;
+  char *draft = nullptr;
+  size_t draft_bytes = 0;
 };
 
 // the text projection (q3h_text.hip)

@@ -81,14 +81,23 @@ __global__ __launch_bounds__(kThreads) void k_cache_append(AppendRows a) {
   }
   const int kvh = a.kv.kvh, turned = a.heads + kvh;
   const int half = a.rot_dim >> 1;
-  const bool turns = a.table && sub < half;
+  const bool rotary = a.table || a.table32;
+  const bool turns = rotary && sub < half;
   int e0 = 2 * sub, e1 = e0 + 1;
-  if (a.table && !a.interleaved) {
+  if (rotary && !a.interleaved) {
     e0 = turns ? sub : a.rot_dim + 2 * (sub - half);
     e1 = turns ? sub + half : e0 + 1;
   }
   double2 cs = make_double2(1.0, 0.0);
-  if (turns && !bad) cs = a.table[(size_t)(s.len + depth) * half + sub];
+  if (turns && !bad) {
+    const size_t at = (size_t)(s.len + depth) * half + sub;
+    if (a.table) {
+      cs = a.table[at];
+    } else {
+      const float2 c = a.table32[at];
+      cs = make_double2(c.x, c.y);
+    }
+  }
   const float *src_q = a.q + (size_t)row * a.ldq, *src_k = a.k + (size_t)row * a.ldk,
               *src_v = a.v + (size_t)row * a.ldv;
   const int groups = (turned + PER - 1) / PER, all = groups + (kvh + PER - 1) / PER;
@@ -280,6 +289,46 @@ __global__ __launch_bounds__(128) void k_cache_keep(KvView kv, const int32_t *ke
   }
 }
 
+// int8 rows from and to f32 [layers][kvh][len][HD], a wave a row
+template <int HD>
+__global__ void k_q8_fill(const float *src, char *k0, int part, int layers, int kvh, int len,
+                          int max_pos) {
+  const int lane = threadIdx.x & 63;
+  const int64_t r = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
+  if (r >= (int64_t)layers * kvh * len) return;
+  const int64_t lg = r / len, at = ((int64_t)part * layers * kvh + lg) * max_pos + (r - lg * len);
+  float x[HD / 64], m = 0.f;
+  bool finite = true;
+#pragma unroll
+  for (int e = 0; e < HD / 64; e++) {
+    x[e] = src[r * HD + 64 * e + lane];
+    finite = finite && fabsf(x[e]) < INFINITY;
+    m = fmaxf(m, fabsf(x[e]));
+  }
+  m = wave_max_dpp(finite ? m : INFINITY);
+  const float d = m == INFINITY ? NAN : (float)((double)m / 127.0);
+  const double inv = 1.0 / (double)d;
+#pragma unroll
+  for (int e = 0; e < HD / 64; e++)
+    reinterpret_cast<uint8_t *>(k0)[at * HD + 64 * e + lane] = d > 0.f ? byte_of(x[e], d, inv) : 0;
+  if (lane == 0)
+    reinterpret_cast<float *>(k0 + 2 * (int64_t)layers * kvh * max_pos * HD)[at] = d;
+}
+template <int HD>
+__global__ void k_q8_read(const char *k0, int part, int layers, int layer, int kvh, int len,
+                          int max_pos, float *dst) {
+  const int lane = threadIdx.x & 63;
+  const int64_t r = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
+  if (r >= (int64_t)kvh * len) return;
+  const int64_t g = r / len;
+  const int64_t at = (((int64_t)part * layers + layer) * kvh + g) * max_pos + (r - g * len);
+  const float d = reinterpret_cast<const float *>(k0 + 2 * (int64_t)layers * kvh * max_pos * HD)[at];
+#pragma unroll
+  for (int e = 0; e < HD / 64; e++)
+    dst[r * HD + 64 * e + lane] =
+        kv_byte(reinterpret_cast<const uint8_t *>(k0)[at * HD + 64 * e + lane]) * d;
+}
+
 template <template <int, int> class F, class... A>
 void by_format(int hd, int fmt, A &&...args) {
   if (hd == 64) {
@@ -399,6 +448,32 @@ DeviceScope::~DeviceScope() {
 
 void launch_cache_append(const AppendRows &a, int hd, int fmt, hipStream_t st) {
   by_format<GoAppend>(hd, fmt, a, st);
+}
+
+void launch_cache_keep(const KvView &v, const int32_t *kept, int hd, int fmt, hipStream_t st) {
+  by_format<GoKeep>(hd, fmt, v, kept, st);
+}
+
+void launch_q8_fill(const float *src, char *k0, bool values, int layers, int kvh, int len, int hd,
+                    int max_pos, hipStream_t st) {
+  const dim3 grid((unsigned)(((int64_t)layers * kvh * len + 3) / 4));
+  if (hd == 64)
+    hipLaunchKernelGGL(k_q8_fill<64>, grid, dim3(kThreads), 0, st, src, k0, values, layers, kvh,
+                       len, max_pos);
+  else
+    hipLaunchKernelGGL(k_q8_fill<128>, grid, dim3(kThreads), 0, st, src, k0, values, layers, kvh,
+                       len, max_pos);
+}
+
+void launch_q8_read(const char *k0, bool values, int layers, int layer, int kvh, int len, int hd,
+                    int max_pos, float *dst, hipStream_t st) {
+  const dim3 grid((unsigned)(((int64_t)kvh * len + 3) / 4));
+  if (hd == 64)
+    hipLaunchKernelGGL(k_q8_read<64>, grid, dim3(kThreads), 0, st, k0, values, layers, layer, kvh,
+                       len, max_pos, dst);
+  else
+    hipLaunchKernelGGL(k_q8_read<128>, grid, dim3(kThreads), 0, st, k0, values, layers, layer,
+                       kvh, len, max_pos, dst);
 }
 
 }  // namespace q3h
@@ -610,9 +685,8 @@ extern "C" int q3h_cache_keep(q3h_cache *c, int sequences, int rows, const int32
     if (sequences == 0 || rows == 0) return;
     require(lens && kept && kept_counts, Q3H_E_ARG, "q3h_cache_keep: NULL argument");
     DeviceScope scope(c->dev->ordinal);
-    by_format<GoKeep>(c->cfg.head_dim, c->cfg.format,
-                      view_of(c, 0, sequences, rows, lens, kept_counts), kept,
-                      (hipStream_t)stream);
+    launch_cache_keep(view_of(c, 0, sequences, rows, lens, kept_counts), kept, c->cfg.head_dim,
+                      c->cfg.format, (hipStream_t)stream);
     check_hip(hipGetLastError(), "cache keep kernel");
   });
 }

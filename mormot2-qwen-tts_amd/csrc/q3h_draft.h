@@ -110,8 +110,10 @@ struct AppendRows {
   int64_t ld_out;
   const float *q_norm, *k_norm;  // nullable
   float eps;
-  // rotary table [position][rot_dim / 2] of (cos, sin) in 64 bits, nullable
+  // rotary table [position][rot_dim / 2] of (cos, sin) in 64 bits, or a stack's in
+  // 32; at most one of them
   const double2 *table;
+  const float2 *table32;
   int rot_dim, interleaved;
   const int32_t *parents;  // nullable
 };
@@ -132,6 +134,16 @@ struct AttendRows {
 size_t attend_part_bytes(int sequences, int rows, int heads, int kvh, int hd, int fmt,
                          int max_len);
 void launch_cache_attend(const AttendRows &a, int hd, int fmt, hipStream_t st);
+constexpr int kAttendSplits = 64;  // the most parts of a query row
+// kept rows to the front of the drafted ones, every layer of v: kept [sequences][rows],
+// v.counts of them
+void launch_cache_keep(const KvView &v, const int32_t *kept, int hd, int fmt, hipStream_t st);
+// positions [0, len) of an int8 cache of one sequence (k0: its keys, values behind
+// them) from or to f32 [layers][kvh][len][hd]
+void launch_q8_fill(const float *src, char *k0, bool values, int layers, int kvh, int len, int hd,
+                    int max_pos, hipStream_t st);
+void launch_q8_read(const char *k0, bool values, int layers, int layer, int kvh, int len, int hd,
+                    int max_pos, float *dst, hipStream_t st);
 
 struct ScoreRows {
   const void *logits;

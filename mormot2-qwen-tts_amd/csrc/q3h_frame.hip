@@ -880,7 +880,7 @@ void enqueue_step(q3h_frame *f, FrameSlice &sl, int positions, hipStream_t st) {
   // one stream on the Qwen3-TTS shapes: step 0 runs the fused two-row path,
   // steps 1.. the fused single-row path (positions are fixed: step g adds
   // position g + 1)
-  const bool fused = n == 1 && cp_fused_supported(cp->cfg) && cctx0->max_pos == 16;
+  const bool fused = n == 1 && !cp->ext && cp_fused_supported(cp->cfg) && cctx0->max_pos == 16;
   // greedy on that path: the argmax of head g and the next input row are taken
   // by the first product of forward g + 1 (one launch fewer per group)
   const bool code_in_product =
@@ -913,7 +913,9 @@ void enqueue_step(q3h_frame *f, FrameSlice &sl, int positions, hipStream_t st) {
       run_cp_fused(cp, cw, cctx0, g + 1, st, code_in_product ? &src : nullptr);
     } else {
       launch_prep(c_arr, fd.alive, n, R, cw.rd, st);
-      run_layers(cp, cw, n * R, c.groups, R == 1, st);
+      LayerIO io;
+      io.rows_each = R;
+      run_layers(cp, cw, n * R, c.groups, R == 1, st, io);
       launch_advance(c_arr, fd.alive, n, R, st);
     }
     // final norm of each stream's last row + head g, one launch
@@ -1024,6 +1026,9 @@ extern "C" int q3h_frame_create(q3h_stack *talker, q3h_stack *cp, const q3h_fram
       check_hip(hipStreamCreateWithFlags(&sl.stream, hipStreamNonBlocking), "hipStreamCreate");
       sl.tw.ensure(talker, sl.n, attention_splits_upto(talker, c.max_positions), c.vocab);
       sl.cw.ensure(cp, 2 * sl.n, 1, c.cp_vocab);
+      sl.tw.ensure_tree(tree_bytes(talker, sl.n, 1, c.max_positions));
+      sl.cw.ensure_tree(std::max(tree_bytes(cp, sl.n, 1, c.groups),
+                                 tree_bytes(cp, sl.n, 2, c.groups)));
     }
     f->codec_emb = falloc<float>(f, (size_t)c.vocab * H);
     check_hip(hipMemcpy(f->codec_emb, codec_emb, sizeof(float) * c.vocab * H,
@@ -1131,6 +1136,7 @@ void start_enqueue(q3h_frame *f, int stream, int rows, int trailing_rows, uint64
   q3h_stack *s = f->talker;
   Work &w = tc->w;
   w.ensure(s, rows, attention_splits(s, rows), c.vocab);
+  w.ensure_tree(tree_bytes(s, 1, rows, rows));
   hipStream_t st = tc->stream;
   FrameDev &d = f->fd;
   fill(w.h, d.trailing + (size_t)stream * c.max_frames * H, st);
@@ -1182,7 +1188,7 @@ constexpr int kStartRows = 8192;
 // count (more than kManyRows rows), so the pass gives the bits of one
 // q3h_frame_start per stream.
 bool start_joins(const q3h_stack *s, int rows) {
-  return rows <= kStartRows && (s->cfg.act_q8 || x3_path(s, rows));
+  return rows <= kStartRows && !s->ext && (s->cfg.act_q8 || x3_path(s, rows));
 }
 
 // The prompts args[0 .. n - 1] (start_joins, kStartRows rows in all) through

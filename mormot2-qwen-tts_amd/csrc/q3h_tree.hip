@@ -121,8 +121,7 @@ struct Raw<Q3H_KV_F32, HD> {
 // One workgroup per (split, kv head, sequence, group of query rows): as many
 // waves side by side as the rows it has need (1, 2 or 4), NQ query tiles each,
 // the others over the positions. NQ tiles a wave share its loads and
-// conversions of K and V; a wave of one tile has the registers for two tiles of
-// positions on their way.
+// conversions of K and V.
 template <int FMT, int HD, int NQ>
 __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shape) {
   constexpr int T = kTile<FMT>;
@@ -644,7 +643,6 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
 
 // The splits' parts of a query row together: `side` waves a row (1 or 4), each
 // over every side-th split, four parts on their way at a time.
-constexpr int kMaxSplits = 64;
 template <int HD>
 __global__ __launch_bounds__(kThreads) void k_attend_merge(AttendRows a, Shape shape, int tile,
                                                            int side) {
@@ -714,13 +712,14 @@ Shape shape_of(int sequences, int rows, int heads, int kvh, int max_len, int til
   const int64_t units = (int64_t)sequences * kvh * ((q_rows + s.group - 1) / s.group);
   const int tiles = (max_len + rows + tile - 1) / tile;
   // the work as tiles of one wave, over 8192 waves (four times what the chip
-  // holds: sequences and groups differ), but 8 or 4 tiles a wave at least (a
-  // workgroup begins and ends in the time of 3 to 6 of them, and parts cost a
-  // second launch, 4 us)
+  // holds: sequences and groups differ; a prompt's rows, whose groups alone are
+  // many, over 2048), but 8 or 4 tiles a wave at least (a workgroup begins and
+  // ends in the time of 3 to 6 of them, and parts cost a second launch, 4 us)
   const int64_t work = units * waves * tiles;
+  const int64_t want = rows > Q3H_TREE_MAX_ROWS ? 2048 : 8192;
   const int wk = kWaves / waves;
-  s.per_wave = (int)std::max<int64_t>((work + 8191) / 8192, s.nq == 1 ? 8 : 4);
-  s.per_wave = std::max(s.per_wave, (tiles + kMaxSplits - 1) / kMaxSplits);
+  s.per_wave = (int)std::max<int64_t>((work + want - 1) / want, s.nq == 1 ? 8 : 4);
+  s.per_wave = std::max(s.per_wave, (tiles + kAttendSplits - 1) / kAttendSplits);
   // (groups of fewer rows have more waves over the positions, and fewer splits)
   s.splits = (tiles + s.per_wave * wk - 1) / (s.per_wave * wk);
   return s;

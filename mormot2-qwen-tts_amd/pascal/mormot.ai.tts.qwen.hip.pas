@@ -65,7 +65,7 @@ type
     layers, hidden, heads, kv_heads, head_dim, intermediate: integer;
     rms_eps, rope_theta: single;
     dtype: integer;         // Q3H_F32 or Q3H_Q8_0
-    kv_f16: integer;        // K/V cache in half floats (lm.pas:128-130)
+    kv_f16: integer;        // K/V cache in half floats (lm.pas:128-130), or Q3H_KV_Q8
     act_q8: integer;        // Q8_0 only: activations quantized per 32-block
     max_positions: integer;
   end;
@@ -191,6 +191,16 @@ type
   end;
   Pq3h_score_args = ^q3h_score_args;
 
+  /// scores of every row of a forward (host memory)
+  q3h_row_scores = record
+    tokens_per_row, top_k: integer;
+    tokens: PInteger;
+    logprobs, entropy: PSingle;
+    top_ids: PInteger;
+    top_logprobs: PSingle;
+  end;
+  Pq3h_row_scores = ^q3h_row_scores;
+
 { device: TQwenVulkan (lm.pas:44-62, 202-222) }
 function q3h_device_available: integer; cdecl; external LIBQ3H;
 function q3h_device_open(ordinal: integer; out dev: q3h_device): integer;
@@ -302,6 +312,18 @@ function q3h_token_logprobs_workspace(rows, vocab, top_k: integer): Int64;
   cdecl; external LIBQ3H;
 function q3h_token_logprobs(dev: q3h_device; a: Pq3h_score_args;
   stream: pointer): integer; cdecl; external LIBQ3H;
+
+{ the same on a context: host memory, blocking }
+function q3h_stack_set_rope(s: q3h_stack; cfg: Pq3h_rope_config): integer;
+  cdecl; external LIBQ3H;
+function q3h_forward_tree(c: q3h_context; x: PSingle; rows: integer;
+  parents: PInteger; head: integer; scores: Pq3h_row_scores;
+  logits, normed: PSingle): integer; cdecl; external LIBQ3H;
+function q3h_context_keep(c: q3h_context; kept: PInteger; n: integer): integer;
+  cdecl; external LIBQ3H;
+function q3h_forward_score(c: q3h_context; x: PSingle; rows, head: integer;
+  scores: Pq3h_row_scores; logits, normed: PSingle): integer;
+  cdecl; external LIBQ3H;
 
 { helpers }
 function q3h_quantize_row_q8_0(x: PSingle; y: pointer; k: Int64): integer;

@@ -171,6 +171,12 @@ class ScoreArgs(ctypes.Structure):
         [("workspace_bytes", ctypes.c_int64)]
 
 
+class RowScores(ctypes.Structure):
+    _fields_ = [("tokens_per_row", ctypes.c_int32), ("top_k", ctypes.c_int32)] + \
+        [(n, ctypes.c_void_p) for n in
+         ("tokens", "logprobs", "entropy", "top_ids", "top_logprobs")]
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _FP = ctypes.POINTER(ctypes.c_float)
@@ -232,6 +238,10 @@ SIGNATURES = {
     "q3h_cache_keep": (_I, [_P, _I, _I, _P, _P, _P, _P]),
     "q3h_token_logprobs_workspace": (ctypes.c_int64, [_I, _I, _I]),
     "q3h_token_logprobs": (_I, [_P, ctypes.POINTER(ScoreArgs), _P]),
+    "q3h_stack_set_rope": (_I, [_P, ctypes.POINTER(RopeConfig)]),
+    "q3h_forward_tree": (_I, [_P, _FP, _I, _IP, _I, ctypes.POINTER(RowScores), _FP, _FP]),
+    "q3h_context_keep": (_I, [_P, _IP, _I]),
+    "q3h_forward_score": (_I, [_P, _FP, _I, _I, ctypes.POINTER(RowScores), _FP, _FP]),
     "q3h_quantize_row_q8_0": (_I, [_FP, _P, ctypes.c_int64]),
     "q3h_stack_time_gemv": (_I, [_P, _I, _I, _I, _FP, ctypes.POINTER(_I),
                                  ctypes.POINTER(ctypes.c_int64)]),
@@ -340,6 +350,12 @@ class Stack:
         self.head_rows.append(rows)
         return idx.value
 
+    def set_rope(self, theta, rot_dim=None, interleaved=False, scaling=None, magnitude=0.0):
+        """Rotary positions of every context made from now on (as Rope's)."""
+        cfg = _rope_config(self.cfg["head_dim"], self.cfg["max_positions"], theta, rot_dim,
+                           interleaved, scaling, magnitude)
+        _check(lib().q3h_stack_set_rope(self.h, ctypes.byref(cfg)))
+
     @property
     def bytes(self):
         return lib().q3h_stack_bytes(self.h)
@@ -416,6 +432,62 @@ class Context:
         _check(lib().q3h_forward_embeds_probe(self.h, _fp(x), rows, head, _fp(logits),
                                               _fp(normed), _fp(lo), _fp(nr)))
         return logits, normed, lo, nr
+
+    def _scored(self, rows, head, tokens, top_k):
+        """(the structure of a call's scores, their arrays by name)."""
+        t = np.zeros((rows, 0), np.int32) if tokens is None else \
+            np.ascontiguousarray(tokens, dtype=np.int32).reshape(rows, -1)
+        res = {"logprobs": np.empty(t.shape, np.float32), "entropy": np.empty(rows, np.float32)}
+        sc = RowScores(t.shape[1], top_k, t.ctypes.data, res["logprobs"].ctypes.data,
+                       res["entropy"].ctypes.data)
+        if top_k > 0:
+            res["top_ids"] = np.empty((rows, top_k), np.int32)
+            res["top_logprobs"] = np.empty((rows, top_k), np.float32)
+            sc.top_ids = res["top_ids"].ctypes.data
+            sc.top_logprobs = res["top_logprobs"].ctypes.data
+        sc.keep = t
+        return sc, res
+
+    def _all_rows(self, x, head, tokens, top_k, want_logits, want_normed, want_scores, call):
+        x = _f32(x)
+        rows, hidden = x.shape
+        known = 0 <= head < len(self.stack.head_rows)
+        logits = np.empty((rows, self.stack.head_rows[head]), np.float32) \
+            if known and want_logits else None
+        normed = np.empty((rows, hidden), np.float32) if want_normed else None
+        sc, res = self._scored(rows, head, tokens, top_k) if want_scores else (None, {})
+        _check(call(x, rows, ctypes.byref(sc) if sc is not None else None, logits, normed))
+        if logits is not None:
+            res["logits"] = logits
+        if normed is not None:
+            res["normed"] = normed
+        return res
+
+    def forward_tree(self, x, parents, head=-1, tokens=None, top_k=0, want_logits=True,
+                     want_normed=True, want_scores=False):
+        """A tree of drafted rows x [rows][hidden], row r after row parents[r] (-1:
+        after the context's last position): dict of logits [rows][head rows],
+        normed [rows][hidden] and, with want_scores, those of token_logprobs (of
+        tokens [rows][m]). The length stays; keep() takes a path of them over."""
+        p = np.ascontiguousarray(parents, dtype=np.int32)
+        return self._all_rows(
+            x, head, tokens, top_k, want_logits, want_normed, want_scores,
+            lambda a, n, sc, lg, nm: lib().q3h_forward_tree(
+                self.h, _fp(a), n, p.ctypes.data_as(_IP), head, sc, _fp(lg), _fp(nm)))
+
+    def keep(self, kept):
+        """The rows kept of the last forward_tree, a path from a root down, become
+        the context's next positions."""
+        k = np.ascontiguousarray(kept, dtype=np.int32)
+        _check(lib().q3h_context_keep(self.h, k.ctypes.data_as(_IP), len(k)))
+
+    def forward_score(self, x, head, tokens=None, top_k=0, want_logits=False, want_normed=False):
+        """forward() of rows x, every position scored: dict as token_logprobs gives
+        it (of tokens [rows][m]), with logits and normed of every row when wanted."""
+        return self._all_rows(
+            x, head, tokens, top_k, want_logits, want_normed, True,
+            lambda a, n, sc, lg, nm: lib().q3h_forward_score(
+                self.h, _fp(a), n, head, sc, _fp(lg), _fp(nm)))
 
     def fill_kv(self, k, v):
         """k, v: float32 [layers][kv_heads][len][head_dim]."""
@@ -735,6 +807,20 @@ def _stream(ordinal):
     return _torch._C._cuda_getCurrentRawStream(ordinal)
 
 
+def _rope_config(head_dim, max_positions, theta, rot_dim, interleaved, scaling, magnitude):
+    s = dict(scaling or {"kind": "plain"})
+    kind = s.pop("kind")
+    if kind not in ROPE_SCALING:
+        _bad(f"no rotary scaling {kind!r}")
+    cfg = RopeConfig(head_dim, head_dim if rot_dim is None else rot_dim, int(interleaved),
+                     max_positions, theta, ROPE_SCALING[kind], s.pop("factor", 1.0),
+                     s.pop("original", 0), s.pop("beta_fast", 32.0), s.pop("beta_slow", 1.0),
+                     s.pop("low", 1.0), s.pop("high", 4.0), magnitude)
+    if s:
+        _bad(f"unknown rotary settings {sorted(s)}")
+    return cfg
+
+
 class Rope:
     """A rotary table (q3h_rope_*): the first rot_dim elements of a head turned
     in neighbouring pairs (interleaved) or in pairs half of them apart. scaling:
@@ -746,16 +832,8 @@ class Rope:
 
     def __init__(self, dev, head_dim, max_positions, theta, rot_dim=None, interleaved=False,
                  scaling=None, magnitude=0.0):
-        s = dict(scaling or {"kind": "plain"})
-        kind = s.pop("kind")
-        if kind not in ROPE_SCALING:
-            _bad(f"no rotary scaling {kind!r}")
-        cfg = RopeConfig(head_dim, head_dim if rot_dim is None else rot_dim, int(interleaved),
-                         max_positions, theta, ROPE_SCALING[kind], s.pop("factor", 1.0),
-                         s.pop("original", 0), s.pop("beta_fast", 32.0), s.pop("beta_slow", 1.0),
-                         s.pop("low", 1.0), s.pop("high", 4.0), magnitude)
-        if s:
-            _bad(f"unknown rotary settings {sorted(s)}")
+        cfg = _rope_config(head_dim, max_positions, theta, rot_dim, interleaved, scaling,
+                           magnitude)
         h = _P()
         _check(lib().q3h_rope_create(dev.h, ctypes.byref(cfg), ctypes.byref(h)))
         self.dev = dev
