@@ -779,19 +779,20 @@ def _ptr(t, ordinal, dtype, name):
 def _rows(t, n, rows, heads, hd, ordinal, name):
     """(address, floats between rows) of f32 rows [n][rows][heads][hd], or
     [n][rows][heads * hd], contiguous within a row."""
-    shape, stride = t.shape, t.stride()
-    if shape == (n, rows, heads, hd):
-        if stride[3] != 1 or (heads > 1 and stride[2] != hd):
-            _bad(f"{name}: the heads of a row are not side by side")
-    elif shape == (n, rows, heads * hd):
-        if stride[2] != 1:
-            _bad(f"{name}: the elements of a row are not side by side")
-    else:
+    shape, width = t.shape, heads * hd
+    if shape != (n, rows, heads, hd) and shape != (n, rows, width):
         _bad(f"{name} is {list(shape)}, not {[n, rows, heads, hd]}")
-    ld = stride[1] if rows > 1 else stride[0] if n > 1 else heads * hd
+    if t.get_device() != ordinal or t.dtype is not _torch.float32:
+        _ptr(t, ordinal, _torch.float32, name)
+    if t.is_contiguous():
+        return t.data_ptr(), width
+    stride = t.stride()
+    if stride[-1] != 1 or (len(shape) == 4 and heads > 1 and stride[2] != hd):
+        _bad(f"{name}: the heads of a row are not side by side")
+    ld = stride[1] if rows > 1 else stride[0] if n > 1 else width
     if rows > 1 and n > 1 and stride[0] != rows * ld:
         _bad(f"{name}: the sequences' rows are not evenly spaced")
-    return _ptr(t, ordinal, _torch.float32, name), ld
+    return t.data_ptr(), ld
 
 
 def _whole(t, shape, ordinal, dtype, name):
@@ -800,7 +801,9 @@ def _whole(t, shape, ordinal, dtype, name):
         return None
     if t.shape != shape or not t.is_contiguous():
         _bad(f"{name} is {list(t.shape)}, not contiguous {list(shape)}")
-    return _ptr(t, ordinal, dtype, name)
+    if t.get_device() != ordinal or t.dtype is not dtype:
+        _ptr(t, ordinal, dtype, name)
+    return t.data_ptr()
 
 
 def _stream(ordinal):
@@ -835,18 +838,20 @@ class Rope:
         cfg = _rope_config(head_dim, max_positions, theta, rot_dim, interleaved, scaling,
                            magnitude)
         h = _P()
-        _check(lib().q3h_rope_create(dev.h, ctypes.byref(cfg), ctypes.byref(h)))
+        L = lib()
+        _check(L.q3h_rope_create(dev.h, ctypes.byref(cfg), ctypes.byref(h)))
         self.dev = dev
         self.h = h
+        self._destroy = L.q3h_rope_destroy
 
     def destroy(self):
         if self.h:
-            _check(lib().q3h_rope_destroy(self.h))
+            _check(self._destroy(self.h))
             self.h = None
 
     def __del__(self):
         if self.h and self.dev.h:
-            lib().q3h_rope_destroy(self.h)
+            self._destroy(self.h)
 
 
 class Cache:
@@ -870,6 +875,7 @@ class Cache:
         self._append, self._read, self._attend = \
             L.q3h_cache_append, L.q3h_cache_read, L.q3h_cache_attend
         self._workspace = L.q3h_cache_attend_workspace
+        self._destroy = L.q3h_cache_destroy
 
     @property
     def bytes(self):
@@ -959,12 +965,12 @@ class Cache:
 
     def destroy(self):
         if self.h:
-            _check(lib().q3h_cache_destroy(self.h))
+            _check(self._destroy(self.h))
             self.h = None
 
     def __del__(self):
         if self.h and self.dev.h:
-            lib().q3h_cache_destroy(self.h)
+            self._destroy(self.h)
 
 
 def _space(workspace, need, like, ordinal):
@@ -997,14 +1003,13 @@ def token_logprobs(dev, logits, tokens, top_k=0, workspace=None):
     if need:
         workspace = _space(workspace, need, logits, o)
         space, need = workspace.data_ptr(), workspace.numel()
-    like = logits.device
-    logprobs = torch.empty((rows, m), dtype=f32, device=like)
-    entropy = torch.empty(rows, dtype=f32, device=like)
+    new = logits.new_empty if not bf16 else lambda shape: logits.new_empty(shape, dtype=f32)
+    logprobs, entropy = new((rows, m)), new((rows,))
     res = {"logprobs": logprobs, "entropy": entropy}
     ids = top = None
     if top_k > 0:
-        res["top_ids"] = ids = torch.empty((rows, top_k), dtype=i32, device=like)
-        res["top_logprobs"] = top = torch.empty((rows, top_k), dtype=f32, device=like)
+        res["top_ids"] = ids = tokens.new_empty((rows, top_k))
+        res["top_logprobs"] = top = new((rows, top_k))
     a = ScoreArgs(at, stride[0] if rows > 1 else vocab, BF16 if bf16 else F32, rows, vocab, m,
                   top_k, pt, logprobs.data_ptr(), entropy.data_ptr(),
                   ids.data_ptr() if top_k > 0 else None, top.data_ptr() if top_k > 0 else None,
