@@ -169,7 +169,7 @@ size_t tree_bytes(const q3h_stack *s, int n, int rows, int positions, bool draft
   const q3h_stack_config &c = s->cfg;
   if (!s->ext && !drafted) return 0;
   // single rows: of any length (a captured launch serves many)
-  if (rows == 1) return sizeof(float) * (size_t)n * c.heads * kAttendSplits * (c.head_dim + 2);
+  if (rows == 1) positions = c.max_positions;
   return attend_part_bytes(n, rows, c.heads, c.kv_heads, c.head_dim, c.kv_f16, positions);
 }
 

@@ -728,8 +728,9 @@ extern "C" int q3h_cache_attend(q3h_cache *c, const q3h_attend_args *p, void *st
             "q3h_cache_attend: a tree has at most " + std::to_string(Q3H_TREE_MAX_ROWS) + " rows");
     require((int64_t)p->sequences * p->rows <= INT32_MAX, Q3H_E_CAPACITY,
             "q3h_cache_attend: too many rows");
-    require((int64_t)p->sequences * p->rows * p->heads <= (1 << 29), Q3H_E_CAPACITY,
-            "q3h_cache_attend: too many rows and heads");
+    require((int64_t)p->sequences * p->rows * p->heads <= (1 << 29) &&
+                attend_fits(p->sequences, p->rows, p->heads, cf.kv_heads, cf.format, p->max_len),
+            Q3H_E_CAPACITY, "q3h_cache_attend: too many rows, heads and positions");
     require(std::isfinite(p->scale), Q3H_E_ARG, "q3h_cache_attend: scale is not finite");
     const size_t need = attend_part_bytes(p->sequences, p->rows, p->heads, cf.kv_heads,
                                           cf.head_dim, cf.format, p->max_len);

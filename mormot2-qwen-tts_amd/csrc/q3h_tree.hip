@@ -52,37 +52,116 @@ constexpr int kTile = FMT == Q3H_KV_F32 ? 16 : 32;
 
 constexpr float kLog2e = 1.44269504088896340736f;
 
-// How a call is laid out: query tiles of 16 rows a wave (nq), rows of a
-// workgroup (group), tiles of positions a wave goes over (per_wave: the same for
-// all, so that a long sequence has more splits and not longer ones), splits at
-// most.
+// How a call is laid out. The query rows of a (sequence, kv head) go in groups of
+// `group`, 16 * nq a wave; the waves that a group does not need side by side (wq)
+// go over its positions together (wk of them, a tile each: a step). A group's
+// steps are cut into shares of about the same length in all groups , a
+// workgroup each, so that long and short sequences, full and small groups end
+// together; the shares of a group that has several leave parts, which a second
+// kernel joins. shares: of a short call no group is cut; blocks: workgroups, of
+// shares those that they may come to.
 struct Shape {
-  int nq, group, per_wave, splits;
+  int nq, group, blocks;
+  bool shares;
+  int per_kv;       // query heads of a kv head
+  uint32_t by_kv;   // ceil(2^32 / per_kv)
+  // x / per_kv (attend_fits: x * per_kv < 2^32)
+  __device__ __forceinline__ int drafted(int x) const {
+    return per_kv == 1 ? x : (int)__umulhi((uint32_t)x, by_kv);
+  }
 };
 
-// A row group's share of the work: waves side by side over its query tiles (wq)
-// and over the positions (wk), and its positions.
 struct Cut {
   int here;    // rows of the group
   int wq, wk;
   int full;    // positions that all its rows see
   int end;     // positions that some row of it sees
-  int tiles, per, splits;  // tiles that hold them, tiles a split, splits
+  int tiles, steps;
 };
 __device__ __forceinline__ Cut cut_of(const AttendRows &a, const KvSeq &s, const Shape &shape,
                                       int first, int rows_in, int tile) {
-  const int per_kv = a.heads / a.kv.kvh;
   Cut c;
   c.here = std::min(shape.group, rows_in - first);
-  c.wq = c.here > 32 * shape.nq ? 4 : c.here > 16 * shape.nq ? 2 : 1;
-  c.wk = kWaves / c.wq;
-  c.full = s.len + (a.parents ? 0 : first / per_kv + 1);
-  c.end = s.len + (first + c.here - 1) / per_kv + 1;
+  const int turn = c.here > 32 * shape.nq ? 2 : c.here > 16 * shape.nq ? 1 : 0;
+  c.wq = 1 << turn;
+  c.wk = kWaves >> turn;
+  c.full = s.len + (a.parents ? 0 : shape.drafted(first) + 1);
+  c.end = s.len + shape.drafted(first + c.here - 1) + 1;
   c.tiles = (c.end + tile - 1) / tile;
-  c.per = shape.per_wave * c.wk;
-  c.splits = (c.tiles + c.per - 1) / c.per;
+  c.steps = (c.tiles + c.wk - 1) >> (2 - turn);
   return c;
 }
+__device__ __forceinline__ bool bad_length(const AttendRows &a, const KvSeq &s) {
+  return s.len < 0 || s.len > a.max_len || s.len > s.max_pos - s.count;
+}
+// steps of group `first` (of a sequence of a bad length: one, which writes NaN)
+__device__ __forceinline__ int group_steps(const AttendRows &a, const KvSeq &s, const Shape &shape,
+                                           int first, int rows_in, int tile) {
+  return bad_length(a, s) ? 1 : cut_of(a, s, shape, first, rows_in, tile).steps;
+}
+// a sequence's groups of one kv head: how many, their steps, and their shares of up
+// to `most` steps
+struct Head {
+  int groups, steps, shares;
+};
+__device__ __forceinline__ Head head_of(const AttendRows &a, const KvSeq &s, const Shape &shape,
+                                        int tile, int most) {
+  const int rows_in = s.count * shape.per_kv;
+  Head h{0, 0, 0};
+  for (int first = 0; first < rows_in; first += shape.group) {
+    const int n = group_steps(a, s, shape, first, rows_in, tile);
+    h.groups++;
+    h.steps += n;
+    h.shares += (n + most - 1) / most;
+  }
+  return h;
+}
+// The steps of a share at most, from all heads' groups and steps. Rounding up
+// costs half a share a group: the shares come to about two for each CU, what it
+// holds, and to no more than shape.blocks. Of little work one for each CU: a
+// second one on some of the CUs would take them as long as a longer one on all.
+constexpr int kMinSteps = 6, kWorkers = 512;
+__device__ __forceinline__ int share_steps(uint32_t groups, uint32_t steps) {
+  const uint32_t w = steps <= kWorkers / 2 * 8 ? kWorkers / 2 : kWorkers;
+  const uint32_t n = std::max(w - std::min(groups / 2, w / 2), w / 2);
+  return (int)std::max<uint32_t>(kMinSteps, (steps + n - 1) / n);
+}
+__device__ __forceinline__ KvSeq lane_sequence(const KvSeq &x, int l) {
+  KvSeq s;
+  const uint64_t p = reinterpret_cast<uint64_t>(x.k0);
+  s.k0 = reinterpret_cast<char *>(
+      global_ptr(reinterpret_cast<char *>((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(p >> 32), l) << 32 |
+                                          (uint32_t)__builtin_amdgcn_readlane((int)p, l))));
+  s.max_pos = __builtin_amdgcn_readlane(x.max_pos, l);
+  s.len = __builtin_amdgcn_readlane(x.len, l);
+  s.count = __builtin_amdgcn_readlane(x.count, l);
+  return s;
+}
+
+// The workspace of a call: a part for each workgroup, [group][HD] outputs and
+// [group] (maximum, sum); the shares before each sequence, and of one of its
+// heads; the steps of a share.
+struct Parts {
+  float *out;
+  float2 *ml;
+  int32_t *before, *head, *most;  // [sequences], [sequences], [1]
+};
+inline size_t parts_bytes(const Shape &s, int sequences, int hd) {
+  if (!s.shares) return 0;
+  return sizeof(float) * s.blocks * s.group * (hd + 2) + sizeof(int32_t) * (2 * (size_t)sequences + 1);
+}
+__device__ __forceinline__ Parts parts_of(const AttendRows &a, const Shape &s, int hd) {
+  Parts p;
+  const size_t rows = (size_t)s.blocks * s.group;
+  p.out = a.part;
+  p.ml = reinterpret_cast<float2 *>(a.part + rows * hd);
+  p.before = reinterpret_cast<int32_t *>(p.ml + rows);
+  p.head = p.before + a.kv.sequences;
+  p.most = p.head + a.kv.sequences;
+  return p;
+}
+// inclusive sums over the lanes
+__device__ __forceinline__ int lane_sums(int x) { return wave_prefix_sum_i(x); }
 
 // two floats rounded to f16 and what is left of them
 __device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t &lo) {
@@ -118,10 +197,7 @@ struct Raw<Q3H_KV_F32, HD> {
   f4 v[4][HD / 64];
 };
 
-// One workgroup per (split, kv head, sequence, group of query rows): as many
-// waves side by side as the rows it has need (1, 2 or 4), NQ query tiles each,
-// the others over the positions. NQ tiles a wave share its loads and
-// conversions of K and V.
+// NQ query tiles a wave share its loads and conversions of K and V.
 template <int FMT, int HD, int NQ>
 __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shape) {
   constexpr int T = kTile<FMT>;
@@ -136,24 +212,83 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
   constexpr int QW = NQ * (HD / 32) * 2 * 256;  // words of a wave's queries
   __shared__ __align__(16) float
       sm_acc[QLDS && QW > NQ * 16 * LD ? kWaves * QW : kWaves * NQ * 16 * LD];
-  __shared__ float sm_m[kWaves][NQ * 16], sm_l[kWaves][NQ * 16];
-  const int tid = threadIdx.x, lane = tid & 63;
+  __shared__ float2 sm_ml[kWaves][NQ * 16];
+  const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int per_kv = shape.per_kv;
+  const int lane = tid & 63;
+  // the workgroup's share: steps step0 .. step1 - 1 of group `first` of kv head g
+  // of sequence b; whole: all of the group's
+  int b, g, first, step0 = 0, step1 = 0;
+  KvSeq s;
+  bool whole = true;
+  const int n = a.kv.sequences;
+  if (!shape.shares) {
+    g = blockIdx.x % a.kv.kvh;
+    const int bg = blockIdx.x / a.kv.kvh;
+    b = bg % n;
+    first = bg / n * shape.group;
+    s = kv_sequence(a.kv, b);
+  } else {
+    // each wave finds it by itself, 64 sequences at a time
+    KvSeq mine;
+    auto head_at = [&](int i, int most) {
+      if (most == 1 || n > 64) mine = kv_sequence(a.kv, std::min(i, n - 1));
+      return i < n ? head_of(a, mine, shape, T, most) : Head{0, 0, 0};
+    };
+    Head h{0, 0, 0};
+    int groups = 0, steps = 0;
+    for (int base = 0; base < n; base += 64) {
+      h = head_at(base + lane, 1);
+      groups += __builtin_amdgcn_readlane(lane_sums(h.groups), 63) * a.kv.kvh;
+      steps += __builtin_amdgcn_readlane(lane_sums(h.steps), 63) * a.kv.kvh;
+    }
+    const int most = share_steps(groups, steps), worker = blockIdx.x;
+    int sum = 0, at = 0, shares = 1;
+    b = -1;
+    for (int base = 0; base < n && (b < 0 || worker == 0); base += 64) {
+      h = head_at(base + lane, most);
+      const int upto = sum + lane_sums(h.shares) * a.kv.kvh, before = upto - h.shares * a.kv.kvh;
+      if (worker == 0 && tid < 64 && base + lane < n) {
+        const Parts p = parts_of(a, shape, HD);
+        p.before[base + lane] = before;
+        p.head[base + lane] = h.shares;
+        *p.most = most;
+      }
+      const uint64_t hit = __ballot(upto > worker);
+      if (b < 0 && hit) {
+        const int f = __builtin_ctzll(hit);
+        b = base + f;
+        at = worker - __builtin_amdgcn_readlane(before, f);
+        shares = __builtin_amdgcn_readlane(h.shares, f);
+        s = lane_sequence(mine, f);
+      }
+      sum = __builtin_amdgcn_readlane(upto, 63);
+    }
+    // (no share is left; lengths that change while the kernel runs lead nowhere else)
+    if (b < 0) return;
+    g = at / shares;
+    at -= g * shares;
+    const int rows_in = s.count * per_kv;
+    for (first = 0; first < rows_in; first += shape.group) {
+      const int own = group_steps(a, s, shape, first, rows_in, T), k = (own + most - 1) / most;
+      if (at < k) {
+        // k shares that differ by a step at most
+        const int q = own / k, longer = own - q * k;
+        step0 = at * q + std::min(at, longer);
+        step1 = step0 + q + (at < longer);
+        whole = k == 1;
+        break;
+      }
+      at -= k;
+    }
+  }
+  if (first >= s.count * per_kv) return;
   const int n16 = lane & 15, g4 = lane >> 4;
-  const int splits = shape.splits, GROUP = shape.group;
-  const int split = blockIdx.x % splits, rest = blockIdx.x / splits;
-  const int g = rest % a.kv.kvh, b = (rest / a.kv.kvh) % a.kv.sequences,
-            group = rest / a.kv.kvh / a.kv.sequences;
-  const int per_kv = a.heads / a.kv.kvh;
-  const KvSeq s = kv_sequence(a.kv, b);
   const int rows_in = s.count * per_kv;  // query rows of the sequence's kv head
-  const int first = group * GROUP;
-  if (first >= rows_in) return;
   const size_t row0 = (size_t)b * a.kv.rows;
-  const bool bad = s.len < 0 || s.len > a.max_len || s.len > s.max_pos - s.count;
-  if (bad) {
-    if (splits > 1) return;  // (the merge writes it)
-    for (int i = tid; i < GROUP * HD; i += kThreads) {
+  if (bad_length(a, s)) {
+    for (int i = tid; i < shape.group * HD; i += kThreads) {
       const int r = first + i / HD;
       if (r < rows_in)
         a.out[(row0 + r / per_kv) * a.ld_out + (size_t)(g * per_kv + r % per_kv) * HD + i % HD] =
@@ -162,8 +297,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
     return;
   }
   const Cut cut = cut_of(a, s, shape, first, rows_in, T);
-  const int tile0 = split * cut.per, tile1 = std::min(cut.tiles, tile0 + cut.per);
-  if (tile0 >= tile1) return;
+  const int tile0 = step0 * cut.wk, tile1 = whole ? cut.tiles : std::min(cut.tiles, step1 * cut.wk);
   const int last = cut.end - 1;  // no row behind it is read
   const int here = cut.here, WQ = cut.wq, WK = cut.wk;
   const int wq = wave & (WQ - 1), wk = wave / WQ;
@@ -242,13 +376,6 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
       return 0;
   };
 
-  Raw<FMT, HD> raw;
-  int tile = tile0 + wk;
-  if (tile < tile1) {
-    load_k(raw, tile);
-    load_v(raw, tile);
-  }
-
   // the wave's queries: dims of (step, lane group) as the keys' loads have them
   int qrow[NQ], qt[NQ];  // the lane's query row, and the drafted row that it is of
   bool live[NQ];
@@ -260,38 +387,46 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
     if constexpr (QLDS) return __builtin_bit_cast(h8, qs[((q * (HD / 32) + i) * 2 + part) * 64]);
     else return __builtin_bit_cast(h8, part ? ql[q][i] : qh[q][i]);
   };
-  // a score in powers of two: product (* the key's scale) * sfac, which is not
-  // negative (the queries have the scale's sign): the maximum is the products'
+  // a score in powers of two: product (* the key's scale) * sfac, which is above 0
+  // (the queries have the scale's sign): the maximum is the products'
   float sfac[NQ];
-  const float sign = a.scale < 0.f ? -1.f : 1.f;
+  const float sign = a.scale < 0.f ? -1.f : 1.f, factor = fabsf(a.scale) * kLog2e;
+  f4 qx[NQ][HD / 16];  // as loaded, before the keys and values are on their way
 #pragma unroll
   for (int q = 0; q < NQ; q++) {
     const int r = first + (wq * NQ + q) * 16 + n16;
     live[q] = r < rows_in;
     qrow[q] = std::min(r, rows_in - 1);
-    qt[q] = qrow[q] / per_kv;
+    qt[q] = shape.drafted(qrow[q]);
     const char *p = reinterpret_cast<const char *>(
         a.q + (row0 + qt[q]) * a.ldq + (size_t)(g * per_kv + qrow[q] - qt[q] * per_kv) * HD);
+#pragma unroll
+    for (int i = 0; i < HD / 16; i++) {
+      const int d = F32 ? 16 * i + 4 * g4
+                    : Q8 ? (i >> 2) * 64 + g4 * 16 + (i & 3) * 4
+                         : (i >> 1) * 32 + g4 * 8 + (i & 1) * 4;
+      qx[q][i] = load<f4u>(p, 4 * d);
+    }
+  }
+  Raw<FMT, HD> raw;
+  int tile = tile0 + wk;
+  if (tile < tile1) {
+    load_k(raw, tile);
+    load_v(raw, tile);
+  }
+
+#pragma unroll
+  for (int q = 0; q < NQ; q++) {
     if constexpr (F32) {
 #pragma unroll
-      for (int i = 0; i < HD / 16; i++)
-        qf[q][i] = load<f4u>(p, 4 * (16 * i + 4 * g4)) * sign;
-      sfac[q] = fabsf(a.scale) * kLog2e;
+      for (int i = 0; i < HD / 16; i++) qf[q][i] = qx[q][i] * sign;
+      sfac[q] = factor;
     } else {
-      float x[HD / 32][8];
       float m = 0.f;
 #pragma unroll
-      for (int i = 0; i < HD / 32; i++) {
-        const int d = Q8 ? (i >> 1) * 64 + g4 * 16 + (i & 1) * 8 : i * 32 + g4 * 8;
-        const f4 u = load<f4u>(p, 4 * d), w = load<f4u>(p, 4 * d + 16);
+      for (int i = 0; i < HD / 16; i++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          x[i][e] = u[e];
-          x[i][4 + e] = w[e];
-        }
-#pragma unroll
-        for (int e = 0; e < 8; e++) m = fmaxf(m, fabsf(x[i][e]));
-      }
+        for (int e = 0; e < 4; e++) m = fmaxf(m, fabsf(qx[q][i][e]));
       m = rows4_max(m);
       // m * 2^k in [2^13, 2^14) (rows below 2^-113: less); infinities and NaN stay
       // what they are
@@ -302,8 +437,9 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
         u4 h, l;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
+          const f4 x = qx[q][2 * i + (e >> 1)];
           uint32_t hi, lo;
-          split2(x[i][2 * e] * up, x[i][2 * e + 1] * up, hi, lo);
+          split2(x[2 * (e & 1)] * up, x[2 * (e & 1) + 1] * up, hi, lo);
           h[e] = hi;
           l[e] = lo;
         }
@@ -315,13 +451,16 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
           ql[q][i] = l;
         }
       }
-      sfac[q] = ldexpf(fabsf(a.scale) * kLog2e, Q8 ? 24 - k : -k);
+      sfac[q] = ldexpf(factor, Q8 ? 24 - k : -k);
     }
   }
 
   f4 acc[NQ][C];
-  float m[NQ], l[NQ];
-  int ev = -100;  // int8: the values' scales are below 2^ev so far
+  // The running maximum, and the sum: weights are 2^(score - m). It is less than
+  // the scores' maximum by 14 where weights go in as f16, and by 14 - ev of
+  // int8 values whose scales are below 2^ev, which are multiplied into the weights:
+  // a maximum of scores + ev, so that what goes in is at most 2^14.
+  float m[NQ], l[NQ], vmax[NQ];
   uint64_t path[NQ];
   bool broken[NQ], paths = false;
 #pragma unroll
@@ -329,7 +468,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
     path[q] = 0;
     broken[q] = false;
     m[q] = -INFINITY;
-    l[q] = 0.f;
+    l[q] = vmax[q] = 0.f;
 #pragma unroll
     for (int c = 0; c < C; c++) acc[q][c] = (f4){0.f, 0.f, 0.f, 0.f};
   }
@@ -386,23 +525,13 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
     f4 ks[2], vs[2];
     if constexpr (Q8) {
 #pragma unroll
-      for (int t = 0; t < 2; t++) ks[t] = raw.ks[t];
+      for (int t = 0; t < 2; t++) {
+        ks[t] = raw.ks[t];
+        vs[t] = raw.vs[t];
+      }
     }
     if (next < tile1) load_k(raw, next);
 
-    int ev_new = ev;
-    if constexpr (Q8) {
-      float x = 0.f;
-#pragma unroll
-      for (int t = 0; t < 2; t++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) x = fmaxf(x, raw.vs[t][r]);
-      x = rows4_max(x);
-      ev_new = std::max(ev, (int)(__float_as_uint(x) >> 23) - 126);
-      const float fv = ldexpf(1.f, 14 - ev_new);
-#pragma unroll
-      for (int t = 0; t < 2; t++) vs[t] = raw.vs[t] * fv;
-    }
     if (tail && a.parents && !paths) {
       paths = true;
       const Path p = tree_path(a.parents + row0, a.kv.rows);
@@ -412,53 +541,59 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
         broken[q] = __shfl((int)p.bad, qt[q]) != 0;
       }
     }
-    float w[NQ][4 * NS];
+    float w[NQ][4 * NS], top = 0.f;
+    if constexpr (Q8) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) top = fmaxf(top, vs[i >> 2][i & 3]);
+    }
 #pragma unroll
     for (int q = 0; q < NQ; q++) {
-      float mx = -INFINITY;
+      float mx = -INFINITY, vx = top;
 #pragma unroll
-      for (int i = 0; i < 4 * NS; i++) {
-        float x = st[q][i >> 2][i & 3];
-        if constexpr (Q8) x *= ks[i >> 2][i & 3];
-        if (tail) {
+      for (int i = 0; i < 4 * NS; i++)
+        w[q][i] = Q8 ? st[q][i >> 2][i & 3] * ks[i >> 2][i & 3] : st[q][i >> 2][i & 3];
+      if (tail) {
+        asm volatile("");  // (a branch, so that the other tiles have no selects)
+        vx = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4 * NS; i++) {
           const int d = j0 + (i >> 2) * 16 + 4 * g4 + (i & 3) - s.len;
-          x = sees(q, d) ? x : -INFINITY;
+          const bool see = sees(q, d);
+          w[q][i] = see ? w[q][i] : -INFINITY;
           // a row whose path is broken: NaN at itself, and so in all of it
-          if (broken[q] && d == qt[q]) x = NAN;
+          if (broken[q] && d == qt[q]) w[q][i] = NAN;
+          if (Q8 && see) vx = fmaxf(vx, vs[i >> 2][i & 3]);
         }
-        w[q][i] = x;
-        mx = fmaxf(mx, x);
       }
-      // (a row that sees none of these, or whose queries are 0: no NaN from inf * 0)
-      mx = rows4_max(mx);
-      mx = fmaxf(m[q], mx == -INFINITY ? mx : mx * sfac[q]);
-      // f16: weights to 2^14
-      const float base = mx == -INFINITY ? 0.f : mx - (FMT == Q3H_KV_F16 ? 14.f : 0.f);
-      if (__any(mx > m[q] || ev_new > ev)) {
-        const float f = __builtin_amdgcn_exp2f(m[q] - (mx == -INFINITY ? 0.f : mx));
-        l[q] *= f;
-        const float fa = Q8 ? ldexpf(f, ev - ev_new) : f;
 #pragma unroll
-        for (int c = 0; c < C; c++) acc[q][c] *= fa;
+      for (int i = 0; i < 4 * NS; i++) mx = fmaxf(mx, w[q][i]);
+      mx = rows4_max(mx);
+      float off = F32 ? 0.f : -14.f;
+      if constexpr (Q8) {
+        // (of 2^-40 .. 2^50: further apart, the factor between two tiles' sums
+        // would leave f32. Weights of larger scales leave f16 and become NaN, a wave
+        // whose scales are all far smaller is known by the largest: both are done
+        // again below)
+        vx = rows4_max(vx);
+        vmax[q] = fmaxf(vmax[q], vx);
+        off += (float)std::min(50, std::max(-40, (int)(__float_as_uint(vx) >> 23) - 126));
+      }
+      mx = fmaxf(m[q], fmaf(mx, sfac[q], off));
+      const float base = mx == -INFINITY ? 0.f : mx;
+      if (__any(mx > m[q])) {
+        const float f = __builtin_amdgcn_exp2f(m[q] - base);
+        l[q] *= f;
+#pragma unroll
+        for (int c = 0; c < C; c++) acc[q][c] *= f;
         m[q] = mx;
       }
 #pragma unroll
       for (int i = 0; i < 4 * NS; i++) {
-        float p = __builtin_amdgcn_exp2f(fmaf(w[q][i], sfac[q], -base));
-        if (tail) p = w[q][i] == -INFINITY ? 0.f : p;
+        const float p = __builtin_amdgcn_exp2f(fmaf(w[q][i], sfac[q], -base));
         l[q] += p;
-        if constexpr (Q8) {
-          float v = vs[i >> 2][i & 3];
-          if (tail) v = sees(q, j0 + (i >> 2) * 16 + 4 * g4 + (i & 3) - s.len) ? v : 0.f;
-          w[q][i] = p * v;
-        } else if constexpr (F32) {
-          w[q][i] = p;
-        } else {
-          w[q][i] = p;
-        }
+        w[q][i] = Q8 ? p * vs[i >> 2][i & 3] : p;
       }
     }
-    ev = ev_new;
 
     if constexpr (F32) {
 #pragma unroll
@@ -516,14 +651,14 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
   bool nan = false;
 #pragma unroll
   for (int q = 0; q < NQ; q++) {
-    scale[q] = F32 ? 1.f : Q8 ? ldexpf(0x1p24f, ev - 14) : 1.f / 16384.f;
-    l[q] = rows4_sum(l[q]) * (FMT == Q3H_KV_F16 ? 1.f / 16384.f : 1.f);
+    scale[q] = Q8 ? 0x1p24f : 1.f;
+    l[q] = rows4_sum(l[q]);
     float zero = 0.f * l[q];
 #pragma unroll
     for (int c = 0; c < C; c++)
 #pragma unroll
       for (int r = 0; r < 4; r++) zero = fmaf(acc[q][c][r], 0.f, zero);
-    nan = nan || (zero != 0.f && !broken[q]);
+    nan = nan || (zero != 0.f && !broken[q]) || (Q8 && vmax[q] > 0.f && vmax[q] < 0x1p-56f);
   }
   // An infinity times one of the parts that a query or a weight is split in is
   // NaN where the product itself is not, and so is an infinity that a row does
@@ -577,39 +712,36 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
     if (g4 == 0) {
 #pragma unroll
       for (int q = 0; q < NQ; q++) {
-        sm_m[wave][q * 16 + n16] = m[q];
-        sm_l[wave][q * 16 + n16] = l[q];
+        sm_ml[wave][q * 16 + n16] = make_float2(m[q], l[q]);
       }
     }
     __syncthreads();
   }
-  float *part = a.part;
-  const size_t part_rows = (size_t)a.kv.rows * per_kv;
-  const size_t part0 = ((size_t)(b * a.kv.kvh + g) * splits + split) * part_rows;
-  float *part_ml = part + (size_t)a.kv.sequences * a.kv.kvh * splits * part_rows * HD;
+  const Parts parts = parts_of(a, shape, HD);
+  const size_t part0 = (size_t)blockIdx.x * shape.group - first;
 #pragma unroll
   for (int q = 0; q < NQ; q++) {
     float M = m[q], L = l[q], f = 1.f;
     if (WK > 1) {
-      M = -INFINITY;
-      for (int i = 0; i < WK; i++) M = fmaxf(M, sm_m[i * WQ + wq][q * 16 + n16]);
+      // (of two waves each twice: the maximum stays, and a sum counts half)
+      float2 o[kWaves];
+#pragma unroll
+      for (int i = 0; i < kWaves; i++) o[i] = sm_ml[(i * WQ + wq) & (kWaves - 1)][q * 16 + n16];
+      M = fmaxf(fmaxf(o[0].x, o[1].x), fmaxf(o[2].x, o[3].x));
       const float base = M == -INFINITY ? 0.f : M;
       L = 0.f;
-      for (int i = 0; i < WK; i++)
-        L += sm_l[i * WQ + wq][q * 16 + n16] *
-             __builtin_amdgcn_exp2f(sm_m[i * WQ + wq][q * 16 + n16] - base);
+#pragma unroll
+      for (int i = 0; i < kWaves; i++) L += o[i].y * __builtin_amdgcn_exp2f(o[i].x - base);
+      if (WK == 2) L *= 0.5f;
       f = __builtin_amdgcn_exp2f(m[q] - base);
     }
     f *= scale[q];
-    if (splits == 1) f /= L;  // the softmax's sum
-    if (splits > 1 && wk == 0 && g4 == 0 && live[q]) {
-      part_ml[2 * (part0 + qrow[q])] = M;
-      part_ml[2 * (part0 + qrow[q]) + 1] = L;
-    }
+    if (whole) f /= L;  // the softmax's sum
+    if (!whole && wk == 0 && g4 == 0 && live[q]) parts.ml[part0 + qrow[q]] = make_float2(M, L);
     if (!live[q]) continue;
     float *o = WK > 1 ? sm_acc + (wave * Q16 + q * 16 + n16) * LD
-               : splits > 1
-                   ? part + (part0 + qrow[q]) * HD
+               : !whole
+                   ? parts.out + (part0 + qrow[q]) * HD
                    : a.out + (row0 + qt[q]) * a.ld_out +
                          (size_t)(g * per_kv + qrow[q] - qt[q] * per_kv) * HD;
 #pragma unroll
@@ -631,9 +763,9 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
       for (int k = 0; k < WK; k++)
         x += *reinterpret_cast<const f4 *>(
             sm_acc + ((k * WQ + r / Q16) * Q16 + r % Q16) * LD + e);
-      float *o = part + (part0 + row) * HD;
-      if (splits == 1) {
-        const int t = row / per_kv;
+      float *o = parts.out + (part0 + row) * HD;
+      if (whole) {
+        const int t = shape.drafted(row);
         o = a.out + (row0 + t) * a.ld_out + (size_t)(g * per_kv + row - t * per_kv) * HD;
       }
       *reinterpret_cast<f4u *>(o + e) = x;
@@ -641,87 +773,96 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
   }
 }
 
-// The splits' parts of a query row together: `side` waves a row (1 or 4), each
-// over every side-th split, four parts on their way at a time.
+// The parts of the rows whose group has several shares, joined: a row a wave, or
+// four waves a row, each over every fourth part (side 4).
 template <int HD>
-__global__ __launch_bounds__(kThreads) void k_attend_merge(AttendRows a, Shape shape, int tile,
-                                                           int side) {
+__global__ __launch_bounds__(kThreads) void k_attend_join(AttendRows a, Shape shape, int tile,
+                                                          int side) {
   constexpr int E = HD / 64, AHEAD = 4;
   typedef float fe __attribute__((ext_vector_type(E)));
+  typedef float feu __attribute__((ext_vector_type(E), aligned(4)));
   __shared__ fe sm[kWaves][64];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int per_kv = a.heads / a.kv.kvh;
-  const int part_rows = a.kv.rows * per_kv;
+  const int per_kv = shape.per_kv;
+  const int q_rows = a.kv.rows * per_kv;
   const int id = side == 1 ? blockIdx.x * kWaves + wave : blockIdx.x;
-  const int row = id % part_rows, bg = id / part_rows;
+  const int row = id % q_rows, bg = id / q_rows;
   const int g = bg % a.kv.kvh, b = bg / a.kv.kvh;
   if (b >= a.kv.sequences) return;
   const KvSeq s = kv_sequence(a.kv, b);
   const int rows_in = s.count * per_kv;
   if (row >= rows_in) return;
-  const int t = row / per_kv;
-  typedef float feu __attribute__((ext_vector_type(E), aligned(4)));
-  feu *out = reinterpret_cast<feu *>(a.out + ((size_t)b * a.kv.rows + t) * a.ld_out +
-                                     (size_t)(g * per_kv + row - t * per_kv) * HD) +
-             lane;
-  const bool writes = side == 1 || wave == 0;
-  if (s.len < 0 || s.len > a.max_len || s.len > s.max_pos - s.count) {
-    if (writes) *out = (fe)NAN;
-    return;
+  const Parts parts = parts_of(a, shape, HD);
+  const int most = *parts.most, mine = row / shape.group * shape.group;
+  int start = parts.before[b] + g * parts.head[b], n = 0;
+  for (int first = 0; first <= mine; first += shape.group) {
+    start += n;
+    n = (group_steps(a, s, shape, first, rows_in, tile) + most - 1) / most;
   }
-  const int n = cut_of(a, s, shape, row / shape.group * shape.group, rows_in, tile).splits;
-  const size_t base = (size_t)bg * shape.splits * part_rows + row;
-  const float *ml = a.part + (size_t)a.kv.sequences * a.kv.kvh * shape.splits * part_rows * HD;
-  // a split's maximum and sum a lane
-  float m = -INFINITY, l = 0.f;
-  if (lane < n) {
-    const float2 x = *reinterpret_cast<const float2 *>(ml + 2 * (base + (size_t)lane * part_rows));
-    m = x.x;
-    l = x.y;
-  }
-  const float M = wave_max_dpp(m), top = M == -INFINITY ? 0.f : M;
-  const float f = __builtin_amdgcn_exp2f(m - top);
-  const float L = wave_sum_dpp(lane < n ? l * f : 0.f);
+  if (n <= 1 || start < 0 || start + n > shape.blocks) return;  // (one share: written as it is)
+  auto part = [&](int i) { return (size_t)(start + i) * shape.group + (row - mine); };
+  float M = -INFINITY;
+  for (int i = lane; i < n; i += 64) M = fmaxf(M, parts.ml[part(i)].x);
+  M = wave_max_dpp(M);
+  const float top = M == -INFINITY ? 0.f : M;
+  float L = 0.f;
   fe x = 0.f;
   const int step = side == 1 ? 1 : kWaves;
-  for (int i0 = side == 1 ? 0 : wave; i0 < n; i0 += AHEAD * step) {
-    fe y[AHEAD];
+  for (int base = 0; base < n; base += 64) {
+    float f = 0.f, l = 0.f;
+    if (base + lane < n) {
+      const float2 p = parts.ml[part(base + lane)];
+      f = __builtin_amdgcn_exp2f(p.x - top);
+      l = p.y * f;
+    }
+    L += wave_sum_dpp(l);
+    const int end = min(n, base + 64);
+    for (int i0 = base + (side == 1 ? 0 : wave); i0 < end; i0 += AHEAD * step) {
+      fe y[AHEAD];
 #pragma unroll
-    for (int i = 0; i < AHEAD; i++)
-      y[i] = reinterpret_cast<const fe *>(
-          a.part + (base + (size_t)min(i0 + i * step, n - 1) * part_rows) * HD)[lane];
+      for (int i = 0; i < AHEAD; i++)
+        y[i] = reinterpret_cast<const fe *>(parts.out + part(min(i0 + i * step, end - 1)) * HD)[lane];
 #pragma unroll
-    for (int i = 0; i < AHEAD; i++)
-      if (i0 + i * step < n) x += lane_f(f, i0 + i * step) * y[i];
+      for (int i = 0; i < AHEAD; i++)
+        if (i0 + i * step < end) x += lane_f(f, i0 + i * step - base) * y[i];
+    }
   }
   if (side > 1) {
     sm[wave][lane] = x;
     __syncthreads();
+    if (wave > 0) return;
     x = (sm[0][lane] + sm[1][lane]) + (sm[2][lane] + sm[3][lane]);
   }
-  if (writes) *out = x / L;
+  const int t = shape.drafted(row);
+  *(reinterpret_cast<feu *>(a.out + ((size_t)b * a.kv.rows + t) * a.ld_out +
+                            (size_t)(g * per_kv + row - t * per_kv) * HD) +
+    lane) = x / L;
+}
+
+// steps of a call at most
+int64_t steps_upto(int sequences, int rows, int heads, int kvh, int max_len, int tile) {
+  return ((int64_t)rows * (heads / kvh) + 15) / 16 * sequences * kvh *
+         ((max_len + rows + tile - 1) / tile);
 }
 
 Shape shape_of(int sequences, int rows, int heads, int kvh, int max_len, int tile) {
-  const int q_rows = rows * (heads / kvh);
   Shape s;
+  s.per_kv = heads / kvh;
+  s.by_kv = (uint32_t)(((1ull << 32) + s.per_kv - 1) / s.per_kv);
+  const int q_rows = rows * s.per_kv;
   s.nq = q_rows > 16 ? 2 : 1;
   const int waves = q_rows > 32 * s.nq ? 4 : q_rows > 16 * s.nq ? 2 : 1;
   s.group = 16 * s.nq * waves;
-  const int64_t units = (int64_t)sequences * kvh * ((q_rows + s.group - 1) / s.group);
-  const int tiles = (max_len + rows + tile - 1) / tile;
-  // the work as tiles of one wave, over 8192 waves (four times what the chip
-  // holds: sequences and groups differ; a prompt's rows, whose groups alone are
-  // many, over 2048), but 8 or 4 tiles a wave at least (a workgroup begins and
-  // ends in the time of 3 to 6 of them, and parts cost a second launch, 4 us)
-  const int64_t work = units * waves * tiles;
-  const int64_t want = rows > Q3H_TREE_MAX_ROWS ? 2048 : 8192;
+  const int64_t groups = (int64_t)sequences * kvh * ((q_rows + s.group - 1) / s.group);
   const int wk = kWaves / waves;
-  s.per_wave = (int)std::max<int64_t>((work + want - 1) / want, s.nq == 1 ? 8 : 4);
-  s.per_wave = std::max(s.per_wave, (tiles + kAttendSplits - 1) / kAttendSplits);
-  // (groups of fewer rows have more waves over the positions, and fewer splits)
-  s.splits = (tiles + s.per_wave * wk - 1) / (s.per_wave * wk);
+  const int64_t steps = ((max_len + rows + tile - 1) / tile + wk - 1) / wk;
+  // no share is shorter than six steps (a workgroup begins and ends in the time of
+  // four, and parts cost a second launch, 4 us); two on every CU, what it holds
+  s.shares = steps > kMinSteps;
+  s.blocks = (int)(s.shares ? std::min(std::max<int64_t>(kWorkers - groups / 2, kWorkers / 2) + groups,
+                                       (groups * steps + kMinSteps - 1) / kMinSteps + groups)
+                            : groups);
   return s;
 }
 
@@ -729,16 +870,15 @@ template <int FMT, int HD>
 void launch(const AttendRows &a, hipStream_t st) {
   const Shape s = shape_of(a.kv.sequences, a.kv.rows, a.heads, a.kv.kvh, a.max_len, kTile<FMT>);
   const int q_rows = a.kv.rows * (a.heads / a.kv.kvh);
-  const unsigned blocks = (unsigned)((int64_t)s.splits * a.kv.kvh * a.kv.sequences *
-                                     ((q_rows + s.group - 1) / s.group));
+  const unsigned blocks = s.blocks;
   if (s.nq == 1)
     hipLaunchKernelGGL((k_attend<FMT, HD, 1>), dim3(blocks), dim3(kThreads), 0, st, a, s);
   else
     hipLaunchKernelGGL((k_attend<FMT, HD, 2>), dim3(blocks), dim3(kThreads), 0, st, a, s);
-  if (s.splits > 1) {
+  if (s.shares) {
     const int64_t rows = (int64_t)a.kv.sequences * a.kv.kvh * q_rows;
     const int side = rows >= 4096 ? 1 : kWaves;
-    hipLaunchKernelGGL((k_attend_merge<HD>),
+    hipLaunchKernelGGL((k_attend_join<HD>),
                        dim3((unsigned)(side == 1 ? (rows + kWaves - 1) / kWaves : rows)),
                        dim3(kThreads), 0, st, a, s, kTile<FMT>, side);
   }
@@ -748,9 +888,14 @@ void launch(const AttendRows &a, hipStream_t st) {
 
 size_t attend_part_bytes(int sequences, int rows, int heads, int kvh, int hd, int fmt,
                          int max_len) {
-  const Shape s = shape_of(sequences, rows, heads, kvh, max_len, fmt == Q3H_KV_F32 ? 16 : 32);
-  if (s.splits == 1) return 0;
-  return sizeof(float) * (size_t)sequences * heads * rows * s.splits * (hd + 2);
+  return parts_bytes(shape_of(sequences, rows, heads, kvh, max_len, fmt == Q3H_KV_F32 ? 16 : 32),
+                     sequences, hd);
+}
+
+bool attend_fits(int sequences, int rows, int heads, int kvh, int fmt, int max_len) {
+  const int64_t per_kv = heads / kvh;
+  return rows * per_kv * per_kv < (int64_t)1 << 32 &&
+         steps_upto(sequences, rows, heads, kvh, max_len, fmt == Q3H_KV_F32 ? 16 : 32) <= 1 << 30;
 }
 
 void launch_cache_attend(const AttendRows &a, int hd, int fmt, hipStream_t st) {

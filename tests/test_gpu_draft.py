@@ -287,6 +287,73 @@ def test_unseen_rows_do_not_reach_a_row(device, fmt, heads):
     assert np.isfinite(out[0, :2]).all() and np.isnan(out[0, 2:]).all()
 
 
+@pytest.mark.parametrize("fmt", [F, H, Q])
+@pytest.mark.parametrize("heads", [2, 24])
+def test_large_values_of_siblings_cost_no_precision(device, fmt, heads):
+    """Siblings whose values are larger by up to 2^100, and positions before the
+    draft whose values are smaller by 2^30, leave a row's precision as it is."""
+    rng = np.random.default_rng(24)
+    hd, rows, P, length = 64, 7, 200, 150
+    k = rng.standard_normal((1, P, 1, hd)).astype(np.float32)
+    v = rng.standard_normal((1, P, 1, hd)).astype(np.float32)
+    v[0, :100] *= 2.0 ** (-10 if fmt == H else -30)
+    parents = np.array([[-1, -1, 0, 1, 2, 3, 4]], np.int32)
+    for r in (1, 3, 5):  # a branch of its own
+        v[0, length + r] *= 2.0 ** (12 if fmt == H else 33 * (r + 1) // 2)
+    k[0, length:] *= 0.1
+    q = rng.standard_normal((1, rows, heads, hd)).astype(np.float32)
+    cache = q3h.Cache(device, 1, 1, hd, P, fmt)
+    fill(cache, k, v, [length + rows])
+    out = host(cache.attend(dev_f(q), dev_i([length]), length, parents=dev_i(parents)))
+    held = ref.stored(k, fmt).astype(np.float64), ref.stored(v, fmt).astype(np.float64)
+    want, bound = ref.attention(q.astype(np.float64), *held, [length], [rows], parents, hd ** -0.5)
+    assert np.isfinite(want).all()
+    ratio = np.abs(out - want) / bound
+    print(ratio.max(axis=(0, 2, 3)), flush=True)
+    assert (ratio <= 1).all()
+
+
+@pytest.mark.parametrize("size", [2.0 ** -110, 2.0 ** -70, 2.0 ** -50, 2.0 ** 45, 2.0 ** 70, 2.0 ** 110])
+@pytest.mark.parametrize("heads", [1, 20])
+def test_attend_int8_values_of_any_size(device, size, heads):
+    rng = np.random.default_rng(26)
+    hd, rows, P, length = 128, 3, 300, 290
+    k = rng.standard_normal((1, P, 1, hd)).astype(np.float32)
+    v = (rng.standard_normal((1, P, 1, hd)) * size).astype(np.float32)
+    v[0, 64:96] = 0
+    v[0, 200:240] *= 2.0 ** -16
+    q = rng.standard_normal((1, rows, heads, hd)).astype(np.float32)
+    cache = q3h.Cache(device, 1, 1, hd, P, Q)
+    fill(cache, k, v, [length + rows])
+    held = ref.stored(k, Q).astype(np.float64), ref.stored(v, Q).astype(np.float64)
+    want, bound = ref.attention(q.astype(np.float64), *held, [length], [rows], None, hd ** -0.5)
+    out = host(cache.attend(dev_f(q), dev_i([length]), length))
+    ratio = np.abs(out - want) / bound
+    print(ratio.max(), flush=True)
+    assert (ratio <= 1).all()
+
+
+@pytest.mark.parametrize("fmt", [F, H, Q])
+def test_attend_with_other_scales(device, fmt):
+    """A scale so small that every position counts the same, one that takes the
+    queries' products out of f32's normal numbers, a negative one."""
+    rng = np.random.default_rng(25)
+    hd, rows, P, length = 128, 5, 90, 61
+    k = rng.standard_normal((2, P, 2, hd)).astype(np.float32)
+    v = rng.standard_normal((2, P, 2, hd)).astype(np.float32)
+    q = rng.standard_normal((2, rows, 4, hd)).astype(np.float32)
+    parents = random_tree(rng, 2, rows)
+    cache = q3h.Cache(device, 2, 2, hd, P, fmt)
+    fill(cache, k, v, [P, P])
+    held = ref.stored(k, fmt).astype(np.float64), ref.stored(v, fmt).astype(np.float64)
+    for scale in (1e-20, 1e-40, -0.11):
+        want, bound = ref.attention(q.astype(np.float64), *held, [length, 3], [rows] * 2, parents,
+                                    scale)
+        out = host(cache.attend(dev_f(q), dev_i([length, 3]), length, parents=dev_i(parents),
+                                scale=scale))
+        assert (np.abs(out - want) <= bound).all()
+
+
 def test_infinite_values_seen_stay_infinite(device):
     """An infinity among the values a row sees comes out in its element, as in
     the sum that defines it, and in no other."""
