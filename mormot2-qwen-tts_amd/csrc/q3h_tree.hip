@@ -773,59 +773,85 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
   }
 }
 
-// The parts of the rows whose group has several shares, joined: a row a wave, or
-// four waves a row, each over every fourth part (side 4).
+// The parts of the rows whose group has several shares, joined. A wave takes
+// neighbouring rows of a group, HD / 4 lanes each, so that it finds its parts once
+// for 256 / HD rows and asks for them in 16 bytes a lane; or four waves do, each
+// over every fourth part (side 4).
 template <int HD>
 __global__ __launch_bounds__(kThreads) void k_attend_join(AttendRows a, Shape shape, int tile,
                                                           int side) {
-  constexpr int E = HD / 64, AHEAD = 4;
-  typedef float fe __attribute__((ext_vector_type(E)));
-  typedef float feu __attribute__((ext_vector_type(E), aligned(4)));
-  __shared__ fe sm[kWaves][64];
+  constexpr int R = 256 / HD, AHEAD = 4;
+  __shared__ f4 sm[kWaves][64];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int per_kv = shape.per_kv;
-  const int q_rows = a.kv.rows * per_kv;
+  const int sets = (a.kv.rows * per_kv + R - 1) / R;
   const int id = side == 1 ? blockIdx.x * kWaves + wave : blockIdx.x;
-  const int row = id % q_rows, bg = id / q_rows;
-  const int g = bg % a.kv.kvh, b = bg / a.kv.kvh;
+  const int bg = id / sets, row0 = (id - bg * sets) * R;
+  const int b = bg / a.kv.kvh, g = bg - b * a.kv.kvh;
   if (b >= a.kv.sequences) return;
   const KvSeq s = kv_sequence(a.kv, b);
-  const int rows_in = s.count * per_kv;
-  if (row >= rows_in) return;
   const Parts parts = parts_of(a, shape, HD);
-  const int most = *parts.most, mine = row / shape.group * shape.group;
+  const int most = *parts.most;
   int start = parts.before[b] + g * parts.head[b], n = 0;
+  const int rows_in = s.count * per_kv;
+  if (row0 >= rows_in) return;
+  const int mine = row0 / shape.group * shape.group;
   for (int first = 0; first <= mine; first += shape.group) {
     start += n;
     n = (group_steps(a, s, shape, first, rows_in, tile) + most - 1) / most;
   }
   if (n <= 1 || start < 0 || start + n > shape.blocks) return;  // (one share: written as it is)
-  auto part = [&](int i) { return (size_t)(start + i) * shape.group + (row - mine); };
-  float M = -INFINITY;
-  for (int i = lane; i < n; i += 64) M = fmaxf(M, parts.ml[part(i)].x);
-  M = wave_max_dpp(M);
-  const float top = M == -INFINITY ? 0.f : M;
-  float L = 0.f;
-  fe x = 0.f;
+  const int sub = lane / (HD / 4), e = lane % (HD / 4) * 4;
+  auto part = [&](int i, int r) {
+    return (size_t)(start + i) * shape.group + (std::min(row0 + r, rows_in - 1) - mine);
+  };
+  float M[R], L[R];
+  float2 head[R];  // of the first 64 parts
+#pragma unroll
+  for (int r = 0; r < R; r++) {
+    head[r] = lane < n ? parts.ml[part(lane, r)] : make_float2(-INFINITY, 0.f);
+    M[r] = head[r].x;
+    L[r] = 0.f;
+  }
+  for (int i = lane + 64; i < n; i += 64)
+#pragma unroll
+    for (int r = 0; r < R; r++) M[r] = fmaxf(M[r], parts.ml[part(i, r)].x);
+#pragma unroll
+  for (int r = 0; r < R; r++) {
+    M[r] = wave_max_dpp(M[r]);
+    if (M[r] == -INFINITY) M[r] = 0.f;
+  }
+  f4 x = {0.f, 0.f, 0.f, 0.f};
   const int step = side == 1 ? 1 : kWaves;
   for (int base = 0; base < n; base += 64) {
-    float f = 0.f, l = 0.f;
-    if (base + lane < n) {
-      const float2 p = parts.ml[part(base + lane)];
-      f = __builtin_amdgcn_exp2f(p.x - top);
-      l = p.y * f;
+    float f[R];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      float2 p = head[r];
+      if (base > 0)
+        p = base + lane < n ? parts.ml[part(base + lane, r)] : make_float2(-INFINITY, 0.f);
+      f[r] = __builtin_amdgcn_exp2f(p.x - M[r]);
+      L[r] += wave_sum_dpp(p.y * f[r]);
     }
-    L += wave_sum_dpp(l);
     const int end = min(n, base + 64);
     for (int i0 = base + (side == 1 ? 0 : wave); i0 < end; i0 += AHEAD * step) {
-      fe y[AHEAD];
+      f4 y[AHEAD];
 #pragma unroll
       for (int i = 0; i < AHEAD; i++)
-        y[i] = reinterpret_cast<const fe *>(parts.out + part(min(i0 + i * step, end - 1)) * HD)[lane];
+        y[i] = *reinterpret_cast<const f4 *>(
+            parts.out + part(min(i0 + i * step, end - 1), sub) * HD + e);
 #pragma unroll
       for (int i = 0; i < AHEAD; i++)
-        if (i0 + i * step < end) x += lane_f(f, i0 + i * step - base) * y[i];
+        if (i0 + i * step < end) {
+          float k = lane_f(f[0], i0 + i * step - base);
+#pragma unroll
+          for (int r = 1; r < R; r++) {
+            const float other = lane_f(f[r], i0 + i * step - base);
+            k = sub == r ? other : k;
+          }
+          x += k * y[i];
+        }
     }
   }
   if (side > 1) {
@@ -834,10 +860,14 @@ __global__ __launch_bounds__(kThreads) void k_attend_join(AttendRows a, Shape sh
     if (wave > 0) return;
     x = (sm[0][lane] + sm[1][lane]) + (sm[2][lane] + sm[3][lane]);
   }
+  float sum = L[0];
+#pragma unroll
+  for (int r = 1; r < R; r++) sum = sub == r ? L[r] : sum;
+  const int row = row0 + sub;
+  if (row >= rows_in) return;
   const int t = shape.drafted(row);
-  *(reinterpret_cast<feu *>(a.out + ((size_t)b * a.kv.rows + t) * a.ld_out +
-                            (size_t)(g * per_kv + row - t * per_kv) * HD) +
-    lane) = x / L;
+  *reinterpret_cast<f4u *>(a.out + ((size_t)b * a.kv.rows + t) * a.ld_out +
+                           (size_t)(g * per_kv + row - t * per_kv) * HD + e) = x / sum;
 }
 
 // steps of a call at most
@@ -876,10 +906,11 @@ void launch(const AttendRows &a, hipStream_t st) {
   else
     hipLaunchKernelGGL((k_attend<FMT, HD, 2>), dim3(blocks), dim3(kThreads), 0, st, a, s);
   if (s.shares) {
-    const int64_t rows = (int64_t)a.kv.sequences * a.kv.kvh * q_rows;
-    const int side = rows >= 4096 ? 1 : kWaves;
+    constexpr int R = 256 / HD;
+    const int64_t sets = (int64_t)a.kv.sequences * a.kv.kvh * ((q_rows + R - 1) / R);
+    const int side = sets >= 2048 ? 1 : kWaves;
     hipLaunchKernelGGL((k_attend_join<HD>),
-                       dim3((unsigned)(side == 1 ? (rows + kWaves - 1) / kWaves : rows)),
+                       dim3((unsigned)(side == 1 ? (sets + kWaves - 1) / kWaves : sets)),
                        dim3(kThreads), 0, st, a, s, kTile<FMT>, side);
   }
 }
