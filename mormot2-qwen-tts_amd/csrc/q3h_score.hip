@@ -39,13 +39,26 @@ __device__ __forceinline__ int key_token(uint64_t k) { return (int)~(uint32_t)k;
 // of those counts the ones above it. emit(rank, key) once for every rank below
 // min(k, keys).
 struct TopSpace {
-  uint64_t top[kThreads];
+  union {
+    uint64_t top[kThreads];
+    float best[kThreads];
+  };
   uint64_t bound;
+  float value;
   int n;
 };
 // (the keys left: top_bytes of dynamic LDS)
 inline size_t top_bytes(int k, int per_thread) {
   return (size_t)4 * k * per_thread * sizeof(uint64_t);
+}
+template <class Emit>
+__device__ __forceinline__ void rank_list(const uint64_t *list, int n, int k, Emit &&emit) {
+  for (int c = threadIdx.x; c < n; c += kThreads) {
+    const uint64_t x = list[c];
+    int rank = 0;
+    for (int i = 0; i < n; i++) rank += list[i] > x;
+    if (rank < k) emit(rank, x);
+  }
 }
 template <int E, class Key, class Emit>
 __device__ __forceinline__ void block_top(TopSpace &sm, uint64_t *list, int k, Key &&key, Emit &&emit) {
@@ -84,13 +97,53 @@ __device__ __forceinline__ void block_top(TopSpace &sm, uint64_t *list, int k, K
     }
   }
   __syncthreads();
-  const int n = sm.n;
-  for (int c = tid; c < n; c += kThreads) {
-    const uint64_t x = list[c];
-    int rank = 0;
-    for (int i = 0; i < n; i++) rank += list[i] > x;
-    if (rank < k) emit(rank, x);
+  rank_list(list, sm.n, k, emit);
+}
+
+// The same for logits x(e), first by their values alone: the largest value that k
+// of the 64 groups reach bounds the row's k-th from below, one comparison a logit.
+// Where that leaves more than `list` holds (many logits alike) or bounds nothing
+// (NaN, -infinity), by whole keys. best: the thread's largest logit.
+template <int E, class Logit, class Key, class Emit>
+__device__ __forceinline__ void block_top_logits(TopSpace &sm, uint64_t *list, int k, float best,
+                                                 Logit &&x, Key &&key, Emit &&emit) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  sm.best[tid] = best;
+  if (tid == 0) sm.n = 0;
+  __syncthreads();
+  if (tid < 64) {
+    float g = best;
+#pragma unroll
+    for (int i = 1; i < kWaves; i++) g = fmaxf(g, sm.best[64 * i + lane]);
+    int reach = 0;  // groups that reach this one's largest
+#pragma unroll
+    for (int i = 0; i < 64; i++) reach += lane_f(g, i) >= g;
+    const float bound = wave_max_dpp(reach >= k ? g : -INFINITY);
+    if (lane == 0) sm.value = bound;
   }
+  __syncthreads();
+  const float bound = sm.value;
+  if (bound > -INFINITY) {
+    if (best >= bound) {
+      int n = 0;
+#pragma unroll
+      for (int e = 0; e < E; e++) n += x(e) >= bound;
+      int at = atomicAdd(&sm.n, n);
+      if (at + n <= 4 * k * E) {
+#pragma unroll
+        for (int e = 0; e < E; e++)
+          if (x(e) >= bound) list[at++] = key(e);
+      }
+    }
+    __syncthreads();
+    const int n = sm.n;
+    if (n <= 4 * k * E) {
+      rank_list(list, n, k, emit);
+      return;
+    }
+    __syncthreads();  // (sm.n is written again)
+  }
+  block_top<E>(sm, list, k, key, emit);
 }
 
 // A row's sums: the maximum, and over the logits' distances d from it the sums
@@ -171,6 +224,7 @@ __global__ __launch_bounds__(kThreads) void k_score(ScoreRows a, int splits) {
   t.m = -INFINITY;
 #pragma unroll
   for (int e = 0; e < E; e++) t.m = fmaxf(t.m, x[e]);
+  const float best = t.m;
   t.m = wave_max_dpp(t.m);
   if ((tid & 63) == 0) red[0][tid >> 6] = t.m;
   __syncthreads();
@@ -182,7 +236,7 @@ __global__ __launch_bounds__(kThreads) void k_score(ScoreRows a, int splits) {
   for (int e = 0; e < E; e++) {
     const float d = x[e] - base, w = __builtin_amdgcn_exp2f(d * kLog2e);
     t.s += w;
-    t.u += w != 0.f ? d * w : 0.f;
+    t.u = fmaf(fmaxf(d, -200.f), w, t.u);  // (w is 0 there, and not 0 * -infinity)
   }
   t.s = wave_sum_dpp(t.s);
   t.u = wave_sum_dpp(t.u);
@@ -200,17 +254,11 @@ __global__ __launch_bounds__(kThreads) void k_score(ScoreRows a, int splits) {
   if (a.top_k == 0) return;
   uint64_t *keys = out.keys + (size_t)blockIdx.x * a.top_k;
   if (splits > 1 && tid < a.top_k && tid >= a.vocab - (split * kThreads * E - skew)) keys[tid] = 0;
-  uint32_t v[E];
-#pragma unroll
-  for (int e = 0; e < E; e++) {
-    const int i = first + e / VEC * kThreads * VEC + e % VEC;
-    v[e] = i >= 0 && i < a.vocab ? top_value(x[e]) : 0;
-  }
-  block_top<E>(
-      sm, list, a.top_k,
+  block_top_logits<E>(
+      sm, list, a.top_k, best, [&](int e) { return x[e]; },
       [&](int e) -> uint64_t {
         const int i = first + e / VEC * kThreads * VEC + e % VEC;
-        return v[e] ? (uint64_t)v[e] << 32 | (uint32_t)~i : 0;
+        return i >= 0 && i < a.vocab ? (uint64_t)top_value(x[e]) << 32 | (uint32_t)~i : 0;
       },
       [&](int rank, uint64_t k) {
         if (splits == 1) {
@@ -223,7 +271,8 @@ __global__ __launch_bounds__(kThreads) void k_score(ScoreRows a, int splits) {
 }
 
 // the splits of a row together
-constexpr int kMergeKeys = 32;  // a thread
+constexpr int kMergeKeys = 32;  // a thread, at most
+template <int E>
 __global__ __launch_bounds__(kThreads) void k_score_merge(ScoreRows a, int splits) {
   __shared__ TopSpace sm;
   extern __shared__ uint64_t list[];
@@ -249,11 +298,11 @@ __global__ __launch_bounds__(kThreads) void k_score_merge(ScoreRows a, int split
   if (a.top_k == 0) return;
   const int n = splits * a.top_k;
   const uint64_t *keys = in.keys + (size_t)r * n;
-  uint64_t mine[kMergeKeys];
+  uint64_t mine[E];
 #pragma unroll
-  for (int e = 0; e < kMergeKeys; e++)
+  for (int e = 0; e < E; e++)
     mine[e] = e * kThreads + tid < n ? keys[e * kThreads + tid] : 0;
-  block_top<kMergeKeys>(
+  block_top<E>(
       sm, list, a.top_k, [&](int e) { return mine[e]; },
       [&](int rank, uint64_t k) {
         a.top_ids[(size_t)r * a.top_k + rank] = key_token(k);
@@ -286,9 +335,15 @@ void launch(const ScoreRows &a, hipStream_t st) {
     hipLaunchKernelGGL((k_score<BF16, 16>), grid, dim3(kThreads), lds, st, a, splits);
   else
     hipLaunchKernelGGL((k_score<BF16, 40>), grid, dim3(kThreads), lds, st, a, splits);
-  if (splits > 1)
-    hipLaunchKernelGGL(k_score_merge, dim3(a.rows), dim3(kThreads),
-                       top_bytes(a.top_k, kMergeKeys), st, a, splits);
+  if (splits > 1) {
+    const int keys = (splits * a.top_k + kThreads - 1) / kThreads;
+    if (keys <= 2)
+      hipLaunchKernelGGL((k_score_merge<2>), dim3(a.rows), dim3(kThreads), top_bytes(a.top_k, 2),
+                         st, a, splits);
+    else
+      hipLaunchKernelGGL((k_score_merge<kMergeKeys>), dim3(a.rows), dim3(kThreads),
+                         top_bytes(a.top_k, kMergeKeys), st, a, splits);
+  }
 }
 
 }  // namespace
