@@ -27,24 +27,23 @@ __global__ void k_rope_table(const double *freq, double mag, int pairs, size_t n
   table[i] = make_double2(c * mag, s * mag);
 }
 
-// sum over the G lanes (32 or 64) of a head, in every lane
-template <int G>
+// sum and maximum over the L lanes (8 or 16, a row of lanes or half of one) of a
+// head, in every lane
+template <int L>
 __device__ __forceinline__ double head_sum(double v) {
-  if constexpr (G == 64) {
-    return wave_sum_dpp_d(v);
-  } else {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    return v;
-  }
+  for (int i = 0; i < (L == 16 ? 4 : 3); i++) v += dpp_d_step(v, i);
+  return v;
 }
-template <int G>
+template <int L>
 __device__ __forceinline__ float head_max(float v) {
-  if constexpr (G == 64) return wave_max_dpp(v);
-  return half_max_dpp(v);
+  v = fmaxf(v, dpp_f_keep<kQuadXor1>(v));
+  v = fmaxf(v, dpp_f_keep<kQuadXor2>(v));
+  v = fmaxf(v, dpp_f_keep<kHalfMirror>(v));
+  return L == 16 ? fmaxf(v, dpp_f_keep<kRowMirror>(v)) : v;
 }
 
-typedef float f2u __attribute__((ext_vector_type(2), aligned(4)));
+typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
 
 // rint(x / d) for the bytes of a row: the quotient by the reciprocal, by the
 // division itself where a reciprocal's error could cross a half
@@ -55,17 +54,19 @@ __device__ __forceinline__ int byte_of(float x, float d, double inv) {
   return v < 0 ? 128 - v : v;
 }
 
-// One head of one row per HD / 2 lanes, a pair of elements each: those that
-// turn together, or two neighbours of the part that does not turn. A wave takes
-// kHeads heads of a row at a time (their loads and sums side by side, one
-// square root and division for all of them) and goes over the row's heads with
-// the same turning angles. Everything up to the f32 row is in 64 bits, so that a
+// One head of one row per HD / 8 lanes, 8 elements each: a[i] and b[i] of four
+// pairs that turn together (halves), a's and b's neighbours (interleaved pairs),
+// or elements that do not turn. A wave has 512 / HD heads of a row side by side,
+// kHeads of them one after another with one square root and division for all,
+// and goes over the row's heads with the same turning angles; loads and stores
+// are of 16 bytes a lane (f16: 8, int8: 4). ODD: pairs that are not a multiple of
+// four, element by element. Everything up to the f32 row is in 64 bits, so that a
 // byte of the int8 format is that of the definition and not of a rounding
 // before it.
-constexpr int kHeads = 4;
-template <int FMT, int HD>
+constexpr int kHeads = 2;
+template <int FMT, int HD, bool ODD>
 __global__ __launch_bounds__(kThreads) void k_cache_append(AppendRows a) {
-  constexpr int G = HD / 2, SIDE = 64 / G;  // lanes of a head, heads side by side
+  constexpr int G = HD / 8, SIDE = 64 / G;  // lanes of a head, heads side by side
   constexpr int PER = kHeads * SIDE;        // heads of a wave at a time
   const int lane = threadIdx.x & 63, sub = lane & (G - 1), side = lane / G;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -80,24 +81,52 @@ __global__ __launch_bounds__(kThreads) void k_cache_append(AppendRows a) {
     bad = bad || __shfl((int)path.bad, t) != 0;
   }
   const int kvh = a.kv.kvh, turned = a.heads + kvh;
-  const int half = a.rot_dim >> 1;
   const bool rotary = a.table || a.table32;
-  const bool turns = rotary && sub < half;
-  int e0 = 2 * sub, e1 = e0 + 1;
-  if (rotary && !a.interleaved) {
-    e0 = turns ? sub : a.rot_dim + 2 * (sub - half);
-    e1 = turns ? sub + half : e0 + 1;
+  const int half = rotary ? a.rot_dim >> 1 : 0;
+  // the lane's elements: four from ea, four from eb (ODD: e[i] and e[4 + i])
+  const bool turns = 4 * sub < half, split = rotary && !a.interleaved;
+  int ea = 8 * sub, eb = ea + 4;
+  if (split) {
+    ea = turns ? 4 * sub : a.rot_dim + 2 * (4 * sub - half);
+    eb = turns ? half + 4 * sub : ea + 4;
   }
-  double2 cs = make_double2(1.0, 0.0);
-  if (turns && !bad) {
-    const size_t at = (size_t)(s.len + depth) * half + sub;
-    if (a.table) {
-      cs = a.table[at];
-    } else {
-      const float2 c = a.table32[at];
-      cs = make_double2(c.x, c.y);
+  int e[ODD ? 8 : 1];
+  if constexpr (ODD) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int p = 4 * sub + i;
+      e[i] = !split ? 2 * p : p < half ? p : a.rot_dim + 2 * (p - half);
+      e[4 + i] = split && p < half ? half + p : e[i] + 1;
     }
   }
+  double2 cs[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    cs[i] = make_double2(1.0, 0.0);
+    if (4 * sub + i < half && !bad) {
+      const size_t at = (size_t)(s.len + depth) * half + 4 * sub + i;
+      if (a.table) {
+        cs[i] = a.table[at];
+      } else {
+        const float2 c = a.table32[at];
+        cs[i] = make_double2(c.x, c.y);
+      }
+    }
+  }
+  auto load8 = [&](const float *p, float (&x)[8], bool values) {
+    if (ODD && !values) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) x[i] = p[e[ODD ? i : 0]];
+    } else {
+      const f4u w0 = *reinterpret_cast<const f4u *>(p + (values ? 8 * sub : ea));
+      const f4u w1 = *reinterpret_cast<const f4u *>(p + (values ? 8 * sub + 4 : eb));
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        x[i] = w0[i];
+        x[4 + i] = w1[i];
+      }
+    }
+  };
   const float *src_q = a.q + (size_t)row * a.ldq, *src_k = a.k + (size_t)row * a.ldk,
               *src_v = a.v + (size_t)row * a.ldv;
   const int groups = (turned + PER - 1) / PER, all = groups + (kvh + PER - 1) / PER;
@@ -106,30 +135,30 @@ __global__ __launch_bounds__(kThreads) void k_cache_append(AppendRows a) {
     const bool values = group >= groups;
     const int first = (values ? group - groups : group) * PER + side;
     const int heads = values ? kvh : turned;
-    float x0[kHeads], x1[kHeads];
+    float x[kHeads][8];
 #pragma unroll
     for (int u = 0; u < kHeads; u++) {
       const int j = min(first + u * SIDE, heads - 1);
-      const float *p = values ? src_v + (size_t)j * HD
-                       : j < a.heads ? src_q + (size_t)j * HD
-                                     : src_k + (size_t)(j - a.heads) * HD;
-      if (values) {
-        const f2u w = *reinterpret_cast<const f2u *>(p + 2 * sub);
-        x0[u] = w[0];
-        x1[u] = w[1];
-      } else {
-        x0[u] = p[e0];
-        x1[u] = p[e1];
-      }
+      load8(values ? src_v + (size_t)j * HD
+                   : j < a.heads ? src_q + (size_t)j * HD
+                                 : src_k + (size_t)(j - a.heads) * HD,
+            x[u], values);
     }
     if (!values) {
-      double y0[kHeads], y1[kHeads];
+      double y[kHeads][8];
 #pragma unroll
-      for (int u = 0; u < kHeads; u++) y0[u] = x0[u], y1[u] = x1[u];
+      for (int u = 0; u < kHeads; u++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) y[u][i] = x[u][i];
       if (a.q_norm || a.k_norm) {
         double ss[kHeads];
 #pragma unroll
-        for (int u = 0; u < kHeads; u++) ss[u] = head_sum<G>(y0[u] * y0[u] + y1[u] * y1[u]);
+        for (int u = 0; u < kHeads; u++) {
+          ss[u] = 0.0;
+#pragma unroll
+          for (int i = 0; i < 8; i++) ss[u] += y[u][i] * y[u][i];
+          ss[u] = head_sum<G>(ss[u]);
+        }
         // lane u of a head does the u-th one's root
         double mine = ss[0];
 #pragma unroll
@@ -140,33 +169,54 @@ __global__ __launch_bounds__(kThreads) void k_cache_append(AppendRows a) {
           const double f = __shfl(inv, side * G + u);
           const float *w = min(first + u * SIDE, heads - 1) < a.heads ? a.q_norm : a.k_norm;
           if (w) {
-            y0[u] = y0[u] * f * (double)w[e0];
-            y1[u] = y1[u] * f * (double)w[e1];
+            float wx[8];
+            load8(w, wx, false);
+#pragma unroll
+            for (int i = 0; i < 8; i++) y[u][i] = y[u][i] * f * (double)wx[i];
           }
         }
       }
 #pragma unroll
       for (int u = 0; u < kHeads; u++) {
-        if (turns) {
-          const double r0 = y0[u] * cs.x - y1[u] * cs.y;
-          y1[u] = y1[u] * cs.x + y0[u] * cs.y;
-          y0[u] = r0;
+        auto turn = [&](double &y0, double &y1, int i) {
+          const double r0 = y0 * cs[i].x - y1 * cs[i].y;
+          y1 = y1 * cs[i].x + y0 * cs[i].y;
+          y0 = r0;
+        };
+        if constexpr (ODD) {
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            if (4 * sub + i < half) turn(y[u][i], y[u][4 + i], i);
+        } else if (turns) {
+          if (split) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) turn(y[u][i], y[u][4 + i], i);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) turn(y[u][2 * i], y[u][2 * i + 1], i);
+          }
         }
-        x0[u] = (float)y0[u];
-        x1[u] = (float)y1[u];
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[u][i] = (float)y[u][i];
       }
     }
     // the int8 format: the heads' scales
     float d[kHeads] = {};
     double inv[kHeads] = {};
     if constexpr (FMT == Q3H_KV_Q8) {
-      if (values || first + (kHeads - 1) * SIDE >= a.heads) {
+      if (values || (group + 1) * PER > a.heads) {
         float m[kHeads];
 #pragma unroll
         for (int u = 0; u < kHeads; u++) {
           // (fmaxf drops a NaN: it is found by its comparison)
-          const bool finite = fabsf(x0[u]) < INFINITY && fabsf(x1[u]) < INFINITY;
-          m[u] = head_max<G>(finite ? fmaxf(fabsf(x0[u]), fabsf(x1[u])) : INFINITY);
+          float most = 0.f;
+          bool finite = true;
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            finite = finite && fabsf(x[u][i]) < INFINITY;
+            most = fmaxf(most, fabsf(x[u][i]));
+          }
+          m[u] = head_max<G>(finite ? most : INFINITY);
         }
         float mine = m[0];
 #pragma unroll
@@ -180,15 +230,30 @@ __global__ __launch_bounds__(kThreads) void k_cache_append(AppendRows a) {
         }
       }
     }
-    const int e_0 = values ? 2 * sub : e0, e_1 = values ? 2 * sub + 1 : e1;
+    const int e_a = values ? 8 * sub : ea, e_b = values ? 8 * sub + 4 : eb;
 #pragma unroll
     for (int u = 0; u < kHeads; u++) {
       const int j = first + u * SIDE;
       if (j >= heads) continue;
+      // four(element, values' index) or one(...) of the row
+      auto put = [&](auto &&four, auto &&one) {
+        if (ODD && !values) {
+#pragma unroll
+          for (int i = 0; i < 8; i++) one(e[ODD ? i : 0], i);
+        } else {
+          four(e_a, 0);
+          four(e_b, 4);
+        }
+      };
       if (!values && j < a.heads) {
         float *o = a.q_out + (size_t)row * a.ld_out + (size_t)j * HD;
-        o[e_0] = bad ? NAN : x0[u];
-        o[e_1] = bad ? NAN : x1[u];
+        if (bad) {
+#pragma unroll
+          for (int i = 0; i < 8; i++) x[u][i] = NAN;
+        }
+        put([&](int at, int i) {
+          *reinterpret_cast<f4u *>(o + at) = (f4u){x[u][i], x[u][i + 1], x[u][i + 2], x[u][i + 3]};
+        }, [&](int at, int i) { o[at] = x[u][i]; });
         continue;
       }
       if (bad) continue;
@@ -196,14 +261,23 @@ __global__ __launch_bounds__(kThreads) void k_cache_append(AppendRows a) {
       if constexpr (FMT == Q3H_KV_Q8) {
         uint8_t *o = reinterpret_cast<uint8_t *>(s.k0) + at * HD;
         const bool some = d[u] > 0.f;  // (not NaN, not 0)
-        o[e_0] = some ? byte_of(x0[u], d[u], inv[u]) : 0;
-        o[e_1] = some ? byte_of(x1[u], d[u], inv[u]) : 0;
+        uint32_t y[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) y[i] = some ? byte_of(x[u][i], d[u], inv[u]) : 0;
+        put([&](int at, int i) {
+          *reinterpret_cast<uint32_t *>(o + at) =
+              y[i] | y[i + 1] << 8 | y[i + 2] << 16 | y[i + 3] << 24;
+        }, [&](int at, int i) { o[at] = y[i]; });
         if (sub == 0) kv_scales(a.kv, s, HD)[at] = d[u];
       } else {
         using KV = std::conditional_t<FMT == Q3H_KV_F16, _Float16, float>;
+        typedef KV kv4 __attribute__((ext_vector_type(4)));
         KV *o = reinterpret_cast<KV *>(s.k0) + at * HD;
-        o[e_0] = to_cache<KV>(x0[u]);
-        o[e_1] = to_cache<KV>(x1[u]);
+        put([&](int at, int i) {
+          *reinterpret_cast<kv4 *>(o + at) =
+              (kv4){to_cache<KV>(x[u][i]), to_cache<KV>(x[u][i + 1]), to_cache<KV>(x[u][i + 2]),
+                    to_cache<KV>(x[u][i + 3])};
+        }, [&](int at, int i) { o[at] = to_cache<KV>(x[u][i]); });
       }
     }
   }
@@ -345,14 +419,17 @@ void by_format(int hd, int fmt, A &&...args) {
 template <int FMT, int HD>
 struct GoAppend {
   static void go(const AppendRows &a, hipStream_t st) {
-    const int per = kHeads * (128 / HD);  // heads of a wave at a time
+    const int per = kHeads * (512 / HD);  // heads of a wave at a time
     const int groups = (a.heads + a.kv.kvh + per - 1) / per + (a.kv.kvh + per - 1) / per;
     // few rows: a wave for each group of heads; many: one workgroup a row, its
     // waves going over the heads with one load of the angles
     const int rows = a.kv.sequences * a.kv.rows;
     const int side = rows >= 1024 ? 1 : (groups + kThreads / 64 - 1) / (kThreads / 64);
     const dim3 grid(rows, side);
-    hipLaunchKernelGGL((k_cache_append<FMT, HD>), grid, dim3(kThreads), 0, st, a);
+    if ((a.table || a.table32) && a.rot_dim % 8 != 0)
+      hipLaunchKernelGGL((k_cache_append<FMT, HD, true>), grid, dim3(kThreads), 0, st, a);
+    else
+      hipLaunchKernelGGL((k_cache_append<FMT, HD, false>), grid, dim3(kThreads), 0, st, a);
   }
 };
 template <int FMT, int HD>
