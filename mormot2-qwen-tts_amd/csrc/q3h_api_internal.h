@@ -39,6 +39,9 @@ extern thread_local std::string g_last_error;
 
 void check_hip(hipError_t e, const char *what);
 void require(bool cond, int code, const std::string &msg);
+inline void require(bool cond, int code, const char *msg) {
+  if (!cond) require(false, code, std::string(msg));
+}
 void *dev_alloc(size_t bytes);
 void dev_free(void *p);
 

@@ -482,16 +482,21 @@ std::vector<double> rope_frequencies(const q3h_rope_config &c, double &mag) {
 
 // rows of pointers and row distances that every drafted-row call has
 void check_rows(const q3h_cache *c, int layer, int sequences, int rows, const char *who) {
-  const std::string w(who);
-  require(layer >= 0 && layer < c->cfg.layers, Q3H_E_ARG, w + ": no layer " + std::to_string(layer));
-  require(sequences >= 0 && sequences <= c->cfg.sequences, Q3H_E_ARG,
-          w + ": " + std::to_string(sequences) + " sequences of a cache of " +
-              std::to_string(c->cfg.sequences));
-  require(rows >= 0, Q3H_E_ARG, w + ": negative rows");
-  require(rows <= c->cfg.max_positions, Q3H_E_CAPACITY,
-          w + ": " + std::to_string(rows) + " rows in a cache of " +
-              std::to_string(c->cfg.max_positions) + " positions");
+  const q3h_cache_config &f = c->cfg;
+  if (layer < 0 || layer >= f.layers || sequences < 0 || sequences > f.sequences || rows < 0)
+    require(false, Q3H_E_ARG,
+            std::string(who) + ": layer " + std::to_string(layer) + ", " +
+                std::to_string(sequences) + " sequences, " + std::to_string(rows) +
+                " rows of a cache of " + std::to_string(f.layers) + " layers, " +
+                std::to_string(f.sequences) + " sequences");
+  if (rows > f.max_positions)
+    require(false, Q3H_E_CAPACITY,
+            std::string(who) + ": " + std::to_string(rows) + " rows in a cache of " +
+                std::to_string(f.max_positions) + " positions");
 }
+
+// threads of a launch, below what a grid takes
+bool launch_fits(int64_t blocks) { return blocks * kThreads < (int64_t)1 << 32; }
 
 KvView view_of(const q3h_cache *c, int layer, int sequences, int rows, const int32_t *lens,
                const int32_t *counts) {
@@ -700,8 +705,8 @@ extern "C" int q3h_cache_append(q3h_cache *c, const q3h_append_args *p, void *st
     require((p->q_norm == nullptr && p->k_norm == nullptr) || p->eps >= 0.f, Q3H_E_ARG,
             "q3h_cache_append: eps must not be negative");
     require(!p->parents || p->rows <= Q3H_TREE_MAX_ROWS, Q3H_E_CAPACITY,
-            "q3h_cache_append: a tree has at most " + std::to_string(Q3H_TREE_MAX_ROWS) + " rows");
-    require((int64_t)p->sequences * p->rows <= INT32_MAX, Q3H_E_CAPACITY,
+            "q3h_cache_append: a tree has at most 64 rows");
+    require(launch_fits((int64_t)p->sequences * p->rows), Q3H_E_CAPACITY,
             "q3h_cache_append: too many rows");
     if (p->rope) {
       require(p->rope->dev->ordinal == c->dev->ordinal, Q3H_E_ARG,
@@ -744,8 +749,9 @@ extern "C" int q3h_cache_read(q3h_cache *c, int layer, int sequences, int rows,
     require(c != nullptr, Q3H_E_ARG, "q3h_cache_read: NULL cache");
     check_rows(c, layer, sequences, rows, "q3h_cache_read");
     if (sequences == 0 || rows == 0 || (!k && !v)) return;
-    require((int64_t)sequences * rows <= INT32_MAX / 16 / c->cfg.kv_heads * 16, Q3H_E_CAPACITY,
-            "q3h_cache_read: too many rows");
+    const int64_t width = (int64_t)c->cfg.kv_heads * (c->cfg.head_dim / 8);  // threads a row
+    require(launch_fits(((int64_t)sequences * rows * width + kThreads - 1) / kThreads),
+            Q3H_E_CAPACITY, "q3h_cache_read: too many rows");
     DeviceScope scope(c->dev->ordinal);
     by_format<GoRead>(c->cfg.head_dim, c->cfg.format,
                       view_of(c, layer, sequences, rows, nullptr, counts), starts, k, v,
@@ -778,9 +784,12 @@ extern "C" int64_t q3h_cache_attend_workspace(const q3h_cache *c, int sequences,
             "q3h_cache_attend_workspace: heads must be a multiple of the cache's");
     require(max_len >= 0 && max_len <= c->cfg.max_positions, Q3H_E_ARG,
             "q3h_cache_attend_workspace: max_len beyond the cache");
-    if (sequences > 0 && rows > 0)
-      bytes = (int64_t)attend_part_bytes(sequences, rows, heads, c->cfg.kv_heads,
-                                         c->cfg.head_dim, c->cfg.format, max_len);
+    if (sequences == 0 || rows == 0) return;
+    require(attend_fits(sequences, rows, heads, c->cfg.kv_heads, c->cfg.head_dim, c->cfg.format,
+                        max_len),
+            Q3H_E_CAPACITY, "q3h_cache_attend_workspace: too many rows, heads and positions");
+    bytes = (int64_t)attend_part_bytes(sequences, rows, heads, c->cfg.kv_heads, c->cfg.head_dim,
+                                       c->cfg.format, max_len);
   });
   return rc ? rc : bytes;
 }
@@ -802,19 +811,17 @@ extern "C" int q3h_cache_attend(q3h_cache *c, const q3h_attend_args *p, void *st
     require(p->out != p->q || p->ldq == p->ld_out, Q3H_E_ARG,
             "q3h_cache_attend: in place with another row distance");
     require(!p->parents || p->rows <= Q3H_TREE_MAX_ROWS, Q3H_E_CAPACITY,
-            "q3h_cache_attend: a tree has at most " + std::to_string(Q3H_TREE_MAX_ROWS) + " rows");
-    require((int64_t)p->sequences * p->rows <= INT32_MAX, Q3H_E_CAPACITY,
-            "q3h_cache_attend: too many rows");
-    require((int64_t)p->sequences * p->rows * p->heads <= (1 << 29) &&
-                attend_fits(p->sequences, p->rows, p->heads, cf.kv_heads, cf.format, p->max_len),
+            "q3h_cache_attend: a tree has at most 64 rows");
+    require(attend_fits(p->sequences, p->rows, p->heads, cf.kv_heads, cf.head_dim, cf.format,
+                        p->max_len),
             Q3H_E_CAPACITY, "q3h_cache_attend: too many rows, heads and positions");
     require(std::isfinite(p->scale), Q3H_E_ARG, "q3h_cache_attend: scale is not finite");
     const size_t need = attend_part_bytes(p->sequences, p->rows, p->heads, cf.kv_heads,
                                           cf.head_dim, cf.format, p->max_len);
-    require(need == 0 || (p->workspace && p->workspace_bytes >= (int64_t)need &&
-                          (uintptr_t)p->workspace % 256 == 0),
-            Q3H_E_ARG, "q3h_cache_attend: a workspace of " + std::to_string(need) +
-                           " bytes, 256-byte aligned, is needed");
+    if (need > 0 && (!p->workspace || p->workspace_bytes < (int64_t)need ||
+                     (uintptr_t)p->workspace % 256 != 0))
+      require(false, Q3H_E_ARG, "q3h_cache_attend: a workspace of " + std::to_string(need) +
+                                    " bytes, 256-byte aligned, is needed");
     DeviceScope scope(c->dev->ordinal);
     AttendRows a{};
     a.kv = view_of(c, p->layer, p->sequences, p->rows, p->lens, p->counts);

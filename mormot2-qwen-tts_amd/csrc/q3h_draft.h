@@ -134,7 +134,7 @@ struct AttendRows {
 size_t attend_part_bytes(int sequences, int rows, int heads, int kvh, int hd, int fmt,
                          int max_len);
 // whether a call's work can be counted in 32 bits (2^30 tiles of 16 rows)
-bool attend_fits(int sequences, int rows, int heads, int kvh, int fmt, int max_len);
+bool attend_fits(int sequences, int rows, int heads, int kvh, int hd, int fmt, int max_len);
 void launch_cache_attend(const AttendRows &a, int hd, int fmt, hipStream_t st);
 // kept rows to the front of the drafted ones, every layer of v: kept [sequences][rows],
 // v.counts of them

@@ -382,8 +382,7 @@ extern "C" int q3h_token_logprobs(q3h_device *dev, const q3h_score_args *p, void
             "q3h_token_logprobs: dtype must be Q3H_F32 or Q3H_BF16");
     require(p->tokens_per_row >= 0, Q3H_E_ARG, "q3h_token_logprobs: negative tokens_per_row");
     require(p->top_k >= 0 && p->top_k <= Q3H_TOP_MAX && p->top_k <= p->vocab, Q3H_E_ARG,
-            "q3h_token_logprobs: top_k must be in [0, min(vocab, " + std::to_string(Q3H_TOP_MAX) +
-                ")]");
+            "q3h_token_logprobs: top_k must be in [0, min(vocab, 64)]");
     if (p->rows == 0) return;
     require(p->logits != nullptr, Q3H_E_ARG, "q3h_token_logprobs: NULL logits");
     require((uintptr_t)p->logits % (p->dtype == Q3H_BF16 ? 2 : 4) == 0, Q3H_E_ARG,
@@ -396,10 +395,10 @@ extern "C" int q3h_token_logprobs(q3h_device *dev, const q3h_score_args *p, void
     require(p->top_k == 0 || (p->top_ids && p->top_logprobs), Q3H_E_ARG,
             "q3h_token_logprobs: NULL top_ids or top_logprobs");
     const size_t need = score_work_bytes(p->rows, p->vocab, p->top_k);
-    require(need == 0 || (p->workspace && p->workspace_bytes >= (int64_t)need &&
-                          (uintptr_t)p->workspace % 256 == 0),
-            Q3H_E_ARG, "q3h_token_logprobs: a workspace of " + std::to_string(need) +
-                           " bytes, 256-byte aligned, is needed");
+    if (need > 0 && (!p->workspace || p->workspace_bytes < (int64_t)need ||
+                     (uintptr_t)p->workspace % 256 != 0))
+      require(false, Q3H_E_ARG, "q3h_token_logprobs: a workspace of " + std::to_string(need) +
+                                    " bytes, 256-byte aligned, is needed");
     DeviceScope scope(dev->ordinal);
     ScoreRows a{};
     a.logits = p->logits;

@@ -870,9 +870,9 @@ __global__ __launch_bounds__(kThreads) void k_attend_join(AttendRows a, Shape sh
                            (size_t)(g * per_kv + row - t * per_kv) * HD + e) = x / sum;
 }
 
-// steps of a call at most
-int64_t steps_upto(int sequences, int rows, int heads, int kvh, int max_len, int tile) {
-  return ((int64_t)rows * (heads / kvh) + 15) / 16 * sequences * kvh *
+// steps of a call at most (a product that can leave 64 bits)
+double steps_upto(int sequences, int rows, int heads, int kvh, int max_len, int tile) {
+  return (double)(((int64_t)rows * (heads / kvh) + 15) / 16) * sequences * kvh *
          ((max_len + rows + tile - 1) / tile);
 }
 
@@ -896,18 +896,22 @@ Shape shape_of(int sequences, int rows, int heads, int kvh, int max_len, int til
   return s;
 }
 
+// sets of rows that k_attend_join has a wave for
+int64_t join_sets(int sequences, int rows, int heads, int kvh, int hd) {
+  const int64_t per = 256 / hd;
+  return (int64_t)sequences * kvh * (((int64_t)rows * (heads / kvh) + per - 1) / per);
+}
+
 template <int FMT, int HD>
 void launch(const AttendRows &a, hipStream_t st) {
   const Shape s = shape_of(a.kv.sequences, a.kv.rows, a.heads, a.kv.kvh, a.max_len, kTile<FMT>);
-  const int q_rows = a.kv.rows * (a.heads / a.kv.kvh);
   const unsigned blocks = s.blocks;
   if (s.nq == 1)
     hipLaunchKernelGGL((k_attend<FMT, HD, 1>), dim3(blocks), dim3(kThreads), 0, st, a, s);
   else
     hipLaunchKernelGGL((k_attend<FMT, HD, 2>), dim3(blocks), dim3(kThreads), 0, st, a, s);
   if (s.shares) {
-    constexpr int R = 256 / HD;
-    const int64_t sets = (int64_t)a.kv.sequences * a.kv.kvh * ((q_rows + R - 1) / R);
+    const int64_t sets = join_sets(a.kv.sequences, a.kv.rows, a.heads, a.kv.kvh, HD);
     const int side = sets >= 2048 ? 1 : kWaves;
     hipLaunchKernelGGL((k_attend_join<HD>),
                        dim3((unsigned)(side == 1 ? (sets + kWaves - 1) / kWaves : sets)),
@@ -923,10 +927,16 @@ size_t attend_part_bytes(int sequences, int rows, int heads, int kvh, int hd, in
                      sequences, hd);
 }
 
-bool attend_fits(int sequences, int rows, int heads, int kvh, int fmt, int max_len) {
-  const int64_t per_kv = heads / kvh;
-  return rows * per_kv * per_kv < (int64_t)1 << 32 &&
-         steps_upto(sequences, rows, heads, kvh, max_len, fmt == Q3H_KV_F32 ? 16 : 32) <= 1 << 30;
+bool attend_fits(int sequences, int rows, int heads, int kvh, int hd, int fmt, int max_len) {
+  const int64_t per_kv = heads / kvh, most = (int64_t)1 << 32;  // threads of a launch: below
+  const int tile = fmt == Q3H_KV_F32 ? 16 : 32;
+  // (steps in 32 bits, and with them groups and shares)
+  if (rows * per_kv * per_kv >= most ||
+      steps_upto(sequences, rows, heads, kvh, max_len, tile) > 0x1p30)
+    return false;
+  const Shape s = shape_of(sequences, rows, heads, kvh, max_len, tile);
+  return (int64_t)s.blocks * kThreads < most &&
+         (!s.shares || join_sets(sequences, rows, heads, kvh, hd) * 64 + kThreads < most);
 }
 
 void launch_cache_attend(const AttendRows &a, int hd, int fmt, hipStream_t st) {

@@ -48,6 +48,38 @@ int main() {
   rope.cfg.rot_dim = 64;
   rope.cfg.max_positions = 100;
 
+  // more than a launch or 32-bit counts hold
+  {
+    q3h_cache wide = c;
+    wide.cfg = {65535, 1, 1024, 64, 1 << 24, Q3H_KV_Q8};
+    q3h_append_args a{};
+    a.sequences = 65535, a.rows = 257;
+    a.k = a.v = mem, a.lens = ints;
+    a.ldk = a.ldv = 65536;
+    expect("append: 2^24 rows", Q3H_E_CAPACITY, q3h_cache_append(&wide, &a, nullptr));
+    expect("read: 2^32 threads", Q3H_E_CAPACITY,
+           q3h_cache_read(&wide, 0, 65535, 9, ints, ints, mem, mem, nullptr));
+    for (int rows : {1, 100, 1 << 20, 1 << 24})
+      for (int heads : {1024, 4096})
+        for (int len : {100, 1 << 24}) {
+          q3h_attend_args t{};
+          t.sequences = 65535, t.rows = rows, t.heads = heads, t.max_len = len;
+          t.q = mem, t.ldq = 64 * heads, t.out = mem + 64, t.ld_out = 64 * heads;
+          t.lens = ints;
+          expect("attend: 2^32 threads", Q3H_E_CAPACITY, q3h_cache_attend(&wide, &t, nullptr));
+          expect("workspace: 2^32 threads", Q3H_E_CAPACITY,
+                 q3h_cache_attend_workspace(&wide, 65535, rows, heads, len));
+        }
+    // one long prompt of many heads, as far as the counts go
+    wide.cfg = {1, 1, 1, 128, 1 << 24, Q3H_KV_F16};
+    expect("workspace: a prompt of 2^24", Q3H_E_CAPACITY,
+           q3h_cache_attend_workspace(&wide, 1, 1 << 24, 64, 0));
+    if (q3h_cache_attend_workspace(&wide, 1, 1 << 16, 64, 1 << 10) <= 0) {
+      std::printf("workspace: a prompt of 2^16: %s\n", q3h_last_error());
+      bad++;
+    }
+  }
+
   // append
   q3h_append_args a{};
   a.layer = 1, a.sequences = 4, a.rows = 10, a.heads = 4;
