@@ -54,12 +54,8 @@ __device__ __forceinline__ KvSeq kv_sequence(const KvView &v, int b) {
   if (v.counts) s.count = min(max(v.counts[b], 0), s.count);
   return s;
 }
-// The int8 format keeps sign and magnitude (the two in their places of an f16
-// are 2^-24 times the value, exactly: the products take it like that).
-__device__ __forceinline__ float kv_byte(uint8_t b) {
-  const float m = (float)(b & 127);
-  return b & 128 ? -m : m;
-}
+// a byte of the int8 format: the value + 128
+__device__ __forceinline__ float kv_byte(uint8_t b) { return (float)((int)b - 128); }
 // the row of (part: 0 keys, 1 values; kv head g; position p) in rows of the
 // sequence's allocation: elements at row * HD, int8 scales at
 // 2 rows_in_all * HD bytes + 4 row

@@ -171,10 +171,14 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t 
   lo = __builtin_bit_cast(uint32_t, l);
 }
 
-// two bytes (sel: each twice) of an int8 cache as f16: sign and 7 bits of
-// magnitude, which as a subnormal are 2^-24 times it, exactly
+// Two bytes (sel: each under a byte of zeros) of an int8 cache as f16, 2^-9 times
+// what they hold, exactly: as subnormals they are 2^-24 times it + 128. (Taken as
+// subnormals, sign and magnitude, the matrix instructions lose what is below
+// 2^-24 of a normal number: 2^-14 of the smallest byte a product.)
 __device__ __forceinline__ uint32_t bytes_f16(uint32_t y, uint32_t x, uint32_t sel) {
-  return __builtin_amdgcn_perm(y, x, sel) & 0x807f807fu;
+  const h2 b = __builtin_bit_cast(h2, __builtin_amdgcn_perm(y, x, sel));
+  const h2 up = {(_Float16)32768.f, (_Float16)32768.f}, off = {(_Float16)-0.25f, (_Float16)-0.25f};
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(b, up, off));
 }
 
 template <int FMT, int HD>
@@ -451,7 +455,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
           ql[q][i] = l;
         }
       }
-      sfac[q] = ldexpf(factor, Q8 ? 24 - k : -k);
+      sfac[q] = ldexpf(factor, Q8 ? 9 - k : -k);
     }
   }
 
@@ -506,8 +510,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
 #pragma unroll
             for (int e = 0; e < 2; e++) {
               const uint32_t w = raw.k[t][i >> 1][2 * (i & 1) + e];
-              ka[2 * e] = bytes_f16(w, w, 0x01010000u);
-              ka[2 * e + 1] = bytes_f16(w, w, 0x03030202u);
+              ka[2 * e] = bytes_f16(w, w, 0x0c010c00u);
+              ka[2 * e + 1] = bytes_f16(w, w, 0x0c030c02u);
             }
           } else {
             ka = raw.k[t][i];
@@ -627,7 +631,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
           if constexpr (Q8) {
             // bytes c of positions 2e and 2e + 1
             va[e] = bytes_f16(vword(raw, 2 * e + 1, c >> 2), vword(raw, 2 * e, c >> 2),
-                              0x04040000u + 0x01010101u * (c & 3));
+                              0x0c040c00u + 0x00010001u * (c & 3));
           } else {
             const uint32_t x = vword(raw, 2 * e, c >> 1), y = vword(raw, 2 * e + 1, c >> 1);
             va[e] = __builtin_amdgcn_perm(y, x, c & 1 ? 0x07060302u : 0x05040100u);
@@ -651,7 +655,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
   bool nan = false;
 #pragma unroll
   for (int q = 0; q < NQ; q++) {
-    scale[q] = Q8 ? 0x1p24f : 1.f;
+    scale[q] = Q8 ? 0x1p9f : 1.f;
     l[q] = rows4_sum(l[q]);
     float zero = 0.f * l[q];
 #pragma unroll

@@ -893,6 +893,9 @@ class Cache:
         pk, ldk = _rows(k, n, rows, self.kv_heads, hd, o, "k")
         pv, ldv = _rows(v, n, rows, self.kv_heads, hd, o, "v")
         heads, pq, ldq, po, ldo, qn = 0, None, 0, None, 0, None
+        turn = None
+        if rope is not None:
+            turn = rope.h or _bad("the rotary table is destroyed")
         if q is not None:
             heads = q.shape[2] if q.dim() == 4 else q.shape[2] // hd
             if q_out is None:
@@ -902,7 +905,7 @@ class Cache:
             qn = _whole(q_norm, (hd,), o, f32, "q_norm")
         a = AppendArgs(layer, n, rows, heads, pq, pk, pv, ldq, ldk, ldv, po, ldo, qn,
                        _whole(k_norm, (hd,), o, f32, "k_norm"), eps,
-                       rope.h if rope is not None else None, _whole(lens, (n,), o, i32, "lens"),
+                       turn, _whole(lens, (n,), o, i32, "lens"),
                        _whole(counts, (n,), o, i32, "counts"),
                        _whole(parents, (n, rows), o, i32, "parents"))
         _check(self._append(self.h, a, _stream(o)))
@@ -914,6 +917,8 @@ class Cache:
         beyond counts stay as they were."""
         o, i32, f32 = self.dev.ordinal, _torch.int32, _torch.float32
         like = k if k is not None else v
+        if like is None:
+            _bad("neither k nor v")
         n, rows = like.shape[0], like.shape[1]
         shape = (n, rows, self.kv_heads, self.head_dim)
         _check(self._read(

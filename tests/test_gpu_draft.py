@@ -53,6 +53,7 @@ ROPES = {
     "pairs_of_six": dict(rot=6, interleaved=True, scaling=dict(kind="bands", factor=8.0,
                                                              original=512)),
     "yarn": dict(scaling=dict(kind="yarn", factor=4.0, original=1024)),
+    "halves_of_ten": dict(rot=20, scaling=dict(kind="linear", factor=3.0)),
     "none": None,
 }
 
@@ -716,3 +717,142 @@ def test_refusals_of_tensors(device):
     table = q3h.Rope(device, 64, 4, 1e4)
     with pytest.raises(q3h.Q3HError):
         cache.append(k, k, lens, rope=table)  # fewer positions than the cache
+
+
+def test_destroyed_handles_are_refused(device):
+    """A destroyed table is not taken for none, a destroyed cache for any."""
+    cache = q3h.Cache(device, 1, 1, 64, 16)
+    table = q3h.Rope(device, 64, 16, 1e4)
+    rows, lens = torch.ones(1, 2, 1, 64, device="cuda"), dev_i([0])
+    cache.append(rows, rows, lens, rope=table)
+    table.destroy()
+    with pytest.raises(Exception, match="destroyed"):
+        cache.append(rows, rows, lens, rope=table)
+    with pytest.raises(Exception, match="neither"):
+        cache.read(None, None)
+    cache.destroy()
+    for call in (lambda: cache.append(rows, rows, lens), lambda: cache.attend(rows, lens, 0),
+                 lambda: cache.read(rows, None)):
+        with pytest.raises(q3h.Q3HError):
+            call()
+
+
+@pytest.mark.parametrize("fmt", [F, H, Q])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_append_of_any_heads_and_distances(device, fmt, hd):
+    """Heads that fill a wave, part of one and several, none of the queries',
+    rows that begin between 16-byte boundaries."""
+    rng = np.random.default_rng(33 + hd + fmt)
+    freq, mag = ref.frequencies(hd, 1e4)
+    table = q3h.Rope(device, hd, 50, 1e4)
+    qn, kn = [(1 + 0.2 * rng.standard_normal(hd)).astype(np.float32) for _ in range(2)]
+    eps = float(np.float32(1e-6))
+
+    def place(x, ld):  # rows ld floats apart, from an odd float on
+        n, rows = x.shape[:2]
+        buf = torch.full((n * rows * ld + 1,), 9.0, device="cuda")
+        t = buf[1:].as_strided((n, rows, x.shape[2] * hd), (rows * ld, ld, 1), 1)
+        t.copy_(dev_f(x).reshape(n, rows, -1))
+        return t
+
+    for heads, kvh in ((0, 1), (1, 1), (5, 1), (28, 4), (7, 7), (48, 8), (12, 9)):
+        print("heads", heads, kvh, flush=True)
+        n, rows, P, lens = 2, 3, 50, [0, 41]
+        cache = q3h.Cache(device, n, kvh, hd, P, fmt)
+        q = rng.standard_normal((n, rows, heads, hd)).astype(np.float32)
+        k = rng.standard_normal((n, rows, kvh, hd)).astype(np.float32)
+        v = rng.standard_normal((n, rows, kvh, hd)).astype(np.float32)
+        tq = place(q, heads * hd + 3) if heads else None
+        got = cache.append(place(k, kvh * hd + 1), place(v, kvh * hd + 5), dev_i(lens), q=tq,
+                           q_out=tq, rope=table, q_norm=dev_f(qn) if heads else None,
+                           k_norm=dev_f(kn))
+        back = [torch.empty((n, rows, kvh, hd), device="cuda") for _ in range(2)]
+        cache.read(*back, starts=dev_i(lens))
+        for s in range(n):
+            for i in range(rows):
+                k0 = ref.turned(ref.normed(k[s, i].astype(np.float64), kn, eps), lens[s] + i, hd,
+                                False, freq, mag)
+                np.testing.assert_array_equal(host(back[0][s, i]),
+                                              ref.stored(k0.astype(np.float32), fmt))
+                np.testing.assert_array_equal(host(back[1][s, i]), ref.stored(v[s, i], fmt))
+                if heads:
+                    q0 = ref.turned(ref.normed(q[s, i].astype(np.float64), qn, eps), lens[s] + i,
+                                    hd, False, freq, mag)
+                    tol = U * np.abs(q0) + 1e-13 * np.abs(q0).max()
+                    assert (np.abs(host(got[s, i]).reshape(heads, hd) - q0) <= tol).all()
+
+
+@pytest.mark.parametrize("fmt", [F, Q])
+def test_attend_of_many_sequences(device, fmt):
+    """More sequences than lanes: long ones, empty ones, ones without rows, one
+    whose length is beyond the bound, one that is none."""
+    rng = np.random.default_rng(34)
+    n, rows, heads, kvh, hd, P = 150, 3, 4, 2, 64, 900
+    lens = rng.integers(0, 300, n)
+    lens[[7, 70, 149]] = 890, 850, 870
+    lens[[0, 64]] = 0
+    counts = rng.integers(0, rows + 1, n)
+    counts[[0, 7, 70, 149, 30, 31]] = rows
+    parents = random_tree(rng, n, rows)
+    k, v = [(rng.standard_normal((n, P, kvh, hd))).astype(np.float32) for _ in range(2)]
+    q = rng.standard_normal((n, rows, heads, hd)).astype(np.float32)
+    cache = q3h.Cache(device, n, kvh, hd, P, fmt)
+    fill(cache, k, v, [P] * n)
+    asked = lens.copy()
+    asked[30], asked[31] = 896, -1
+    out = torch.full((n, rows, heads, hd), 7.0, device="cuda")
+    cache.attend(dev_f(q), dev_i(asked), 895, out=out, counts=dev_i(counts),
+                 parents=dev_i(parents))
+    out = host(out)
+    for b in (30, 31):
+        assert np.isnan(out[b]).all()
+    good = [b for b in range(n) if b not in (30, 31)]
+    held = ref.stored(k, fmt).astype(np.float64), ref.stored(v, fmt).astype(np.float64)
+    want, bound = ref.attention(q.astype(np.float64), *held, lens, counts, parents, hd ** -0.5)
+    for b in good:
+        assert (out[b, counts[b]:] == 7).all()
+        off = np.abs(out - want)[b, :counts[b]]
+        if not (off <= bound[b, :counts[b]]).all():
+            at = np.argwhere(off > bound[b, :counts[b]])
+            print("sequence", b, lens[b], counts[b], parents[b], len(at), at[:8].tolist(),
+                  [(out[b][tuple(i)], want[b][tuple(i)], bound[b][tuple(i)]) for i in at[:8]])
+        assert (off <= bound[b, :counts[b]]).all()
+
+
+def test_graphs_that_share_a_workspace(device):
+    """Two captured calls of different shapes over one workspace, replayed in
+    turn with eager calls between."""
+    rng = np.random.default_rng(35)
+    n, kvh, hd, P = 3, 2, 128, 2100
+    cache = q3h.Cache(device, n, kvh, hd, P, H)
+    base = rng.standard_normal((n, 2000, kvh, hd)).astype(np.float32)
+    fill(cache, base, base, [2000, 1990, 700])
+    lens = dev_i([1900, 1700, 600])
+    calls = []
+    need = max(cache.attend_workspace(n, 1, 8, 2000), cache.attend_workspace(n, 17, 16, 2000))
+    space = torch.empty(need, dtype=torch.uint8, device="cuda")
+    for rows, heads in ((1, 8), (17, 16)):
+        q = dev_f(rng.standard_normal((n, rows, heads, hd)))
+        out = torch.zeros_like(q)
+        parents = dev_i(random_tree(rng, n, rows))
+
+        def call(q=q, out=out, parents=parents):
+            cache.attend(q, lens, 2000, out=out, parents=parents, workspace=space)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            call()
+        calls.append((g, q, out, call))
+    for turn in range(4):
+        want = []
+        for g, q, out, call in calls:
+            q.copy_(dev_f(rng.standard_normal(tuple(q.shape))))
+            call()
+            want.append(out.clone())
+            out.zero_()
+        torch.cuda.synchronize()
+        for g, q, out, call in calls[::1 if turn % 2 else -1]:
+            g.replay()
+        torch.cuda.synchronize()
+        for (g, q, out, call), w in zip(calls, want):
+            assert torch.equal(out, w)
+        lens += 20
