@@ -188,6 +188,15 @@ __device__ __forceinline__ Space space_of(const ScoreRows &a, int splits) {
 // 16 bytes a load, and kept in registers: the maximum, the sums, the top. Loads
 // are at 16-byte boundaries whatever the row's: the row begins `skew` elements
 // into its first.
+//
+// m = max x, s = sum e^(x - m), u = sum (x - m) e^(x - m): logprob = x - m - ln s,
+// entropy = ln s - u / s. Bound by what a thread does with its logits (an
+// exponential, two sums, two comparisons each) behind one round of loads, as
+// all workgroups are on the chip at once: 1021 rows of 8191 bf16 logits, 16.8 MB,
+// 12 us (17 with whole 64-bit keys compared for the top); 40 rows of 151936 f32
+// logits, 24.3 MB in 600 workgroups, 12 us and the merge's 4.5; one row of 2048 4.4.
+// 16 logits a thread for long rows were 5 % faster there and have three times the
+// keys to merge: not kept.
 template <bool BF16, int E>
 __global__ __launch_bounds__(kThreads) void k_score(ScoreRows a, int splits) {
   constexpr int VEC = BF16 ? 8 : 4, SIZE = BF16 ? 2 : 4;
@@ -270,7 +279,8 @@ __global__ __launch_bounds__(kThreads) void k_score(ScoreRows a, int splits) {
       });
 }
 
-// the splits of a row together
+// The splits of a row together, a workgroup a row: 40 rows of 15 splits 4.5 us, a
+// launch and three trips to memory (sums, keys, the given tokens' logits).
 constexpr int kMergeKeys = 32;  // a thread, at most
 template <int E>
 __global__ __launch_bounds__(kThreads) void k_score_merge(ScoreRows a, int splits) {

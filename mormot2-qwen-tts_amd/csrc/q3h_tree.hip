@@ -18,7 +18,22 @@
 // scaled to 2^13 .. 2^14 by a power of two per row, weights to at most 2^14, so
 // that the second part stays normal), f32 caches use the f32 matrix
 // instructions. An int8 row's scale is a factor of the position: it multiplies
-// the score, and the weight that the values are summed with.
+// the score, and the weight that the values are summed with. (One f16 part of
+// each would be half the products; the sums were then 2^-12 off instead of 2^-21.)
+//
+// What bounds it, by how much a share has to do (heads of 128):
+// - one row over 171 positions of an f32 cache, 8 workgroups of 2 or 3 tiles a wave:
+//   9.0 us, a launch and the round trips of one workgroup (lengths, rows, the waves'
+//   meeting);
+// - 32 sequences of one row, 41000 positions of int8 in all, 87 MB: 23.5 us + 4.2 for
+//   the parts, 432 shares of 8 steps, where a workgroup takes 10 us to find its
+//   share, have its first tiles and join its waves, and 1.45 a step. Shares of fewer
+//   steps, or three workgroups a CU at 168 registers (27 us), were slower;
+// - a tree of 27 rows over 12289 positions of f16, 51 MB: 22 us + 5.2, 224 shares of 7;
+// - 12 trees, 420 rows, 32 query heads over 8, 60000 positions of int8, 141 MB: 129 us
+//   + 11.4, VALU bound: of a tile's 390 instructions a wave and 64 products 128
+//   make f16 of its bytes, 16 scores a lane take 9 each. 260 TFLOP/s of the
+//   definition's operations, twice that in products.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
