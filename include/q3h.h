@@ -468,9 +468,9 @@ int q3h_cache_destroy(q3h_cache *c);
    nullable: not normed) and turned (rope, nullable: not turned; its
    max_positions not below the cache's), in 64 bits and rounded once to f32;
    then k and v are rounded to the format. q_out may be q itself (the same
-   pointer and row distance) and overlap nothing else. A sequence whose rows would pass its positions, or of
-   negative length, gets no rows and NaN queries, and so does a row on whose
-   path a parent is not below its row. */
+   pointer and row distance) and overlap nothing else. A sequence whose rows
+   would pass its positions, or of negative length, gets no rows and NaN queries,
+   and so does a row on whose path a parent is not below its row. */
 typedef struct {
   int32_t layer, sequences, rows, heads;
   const float *q, *k, *v;
@@ -495,7 +495,8 @@ int q3h_cache_read(q3h_cache *c, int layer, int sequences, int rows, const int32
    [..][heads][head_dim], heads a multiple of kv_heads, query head h on kv head
    h / (heads / kv_heads). max_len: no length in lens is above it (the host's
    bound, it sizes the launch; a longer or negative one: NaN rows). scale: 0 for
-   1 / sqrt(head_dim). Products and sums keep f32's precision in every format.
+   1 / sqrt(head_dim). Products and sums keep f32's precision in every format (an
+   f16 cache's elements below 2^-14 count to 2^-38).
    Infinities and NaN at positions a row does not see do not reach it. workspace:
    q3h_cache_attend_workspace bytes for the same sequences, rows, heads and max_len
    (of the caller, 256-byte aligned, one for each call that may run at once;
@@ -525,8 +526,8 @@ int q3h_cache_keep(q3h_cache *c, int sequences, int rows, const int32_t *lens,
                    const int32_t *kept, const int32_t *kept_counts, void *stream);
 
 /* Scores of rows of logits [rows][vocab] (dtype Q3H_F32 or Q3H_BF16, rows ld
-   elements apart, at most 2^20 tokens), computed in f32 from one read of them: with lse = log sum
-   exp of a row,
+   elements apart, at most 2^20 tokens), computed in f32 from one read of them:
+   with lse = log sum exp of a row,
    - logprobs [rows][tokens_per_row]: logit - lse of the given tokens (tokens
      [rows][tokens_per_row]; a token outside [0, vocab): NaN);
    - entropy [rows] (nullable): lse - sum p logit, logits of -infinity adding

@@ -70,7 +70,7 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // How a call is laid out. The query rows of a (sequence, kv head) go in groups of
 // `group`, 16 * nq a wave; the waves that a group does not need side by side (wq)
 // go over its positions together (wk of them, a tile each: a step). A group's
-// steps are cut into shares of about the same length in all groups , a
+// steps are cut into shares of about the same length in all groups, a
 // workgroup each, so that long and short sequences, full and small groups end
 // together; the shares of a group that has several leave parts, which a second
 // kernel joins. shares: of a short call no group is cut; blocks: workgroups, of

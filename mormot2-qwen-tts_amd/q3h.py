@@ -436,7 +436,11 @@ class Context:
     def _scored(self, rows, head, tokens, top_k):
         """(the structure of a call's scores, their arrays by name)."""
         t = np.zeros((rows, 0), np.int32) if tokens is None else \
-            np.ascontiguousarray(tokens, dtype=np.int32).reshape(rows, -1)
+            np.ascontiguousarray(tokens, dtype=np.int32)
+        if t.ndim == 1:
+            t = t[:, None]
+        if t.ndim != 2 or t.shape[0] != rows:
+            _bad(f"tokens are {list(t.shape)}, not of {rows} rows")
         res = {"logprobs": np.empty(t.shape, np.float32), "entropy": np.empty(rows, np.float32)}
         sc = RowScores(t.shape[1], top_k, t.ctypes.data, res["logprobs"].ctypes.data,
                        res["entropy"].ctypes.data)
@@ -450,6 +454,8 @@ class Context:
 
     def _all_rows(self, x, head, tokens, top_k, want_logits, want_normed, want_scores, call):
         x = _f32(x)
+        if x.ndim != 2 or x.shape[1] != self.stack.cfg["hidden"]:
+            _bad(f"x is {list(x.shape)}, not [rows][{self.stack.cfg['hidden']}]")
         rows, hidden = x.shape
         known = 0 <= head < len(self.stack.head_rows)
         logits = np.empty((rows, self.stack.head_rows[head]), np.float32) \
@@ -470,6 +476,8 @@ class Context:
         normed [rows][hidden] and, with want_scores, those of token_logprobs (of
         tokens [rows][m]). The length stays; keep() takes a path of them over."""
         p = np.ascontiguousarray(parents, dtype=np.int32)
+        if p.shape != (len(x),):
+            _bad(f"{list(p.shape)} parents of {len(x)} rows")
         return self._all_rows(
             x, head, tokens, top_k, want_logits, want_normed, want_scores,
             lambda a, n, sc, lg, nm: lib().q3h_forward_tree(

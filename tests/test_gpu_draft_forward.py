@@ -387,3 +387,25 @@ def test_refusals(device):
         assert code(q3h.Stack, device, dict(DIMS, dtype=q3h.Q8_0, kv_f16=kv, act_q8=act,
                                             max_positions=64), layers, final,
                     q3h.Q8_0) == q3h.E_ARG
+
+
+def test_arrays_that_do_not_fit_are_refused(device):
+    """Before a pointer to them is handed on."""
+    s = Setup(device)
+    c = s.context(60)
+    x = rows_of(1, 4)
+    for call in (lambda: c.forward_tree(x, [-1, 0, 0]),
+                 lambda: c.forward_tree(x, [[-1, 0, 0, 0]]),
+                 lambda: c.forward_tree(x[:, :-1], [-1, 0, 0, 0]),
+                 lambda: c.forward_tree(x, [-1, 0, 0, 0], s.head, tokens=[[1, 2, 3, 4]] * 2,
+                                        want_scores=True),
+                 lambda: c.forward_score(x[0], s.head),
+                 lambda: c.forward_score(x, s.head, tokens=[1, 2])):
+        with pytest.raises(q3h.Q3HError) as e:
+            call()
+        assert e.value.code == q3h.E_ARG
+    assert c.length == 0
+    got = c.forward_score(x, s.head, tokens=[1, 2, 3, 4])
+    assert got["logprobs"].shape == (4, 1) and c.length == 4
+    c.destroy()
+    s.destroy()
