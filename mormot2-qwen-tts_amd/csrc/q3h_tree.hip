@@ -31,12 +31,14 @@
 //   steps, or three workgroups a CU at 168 registers (27 us), were slower;
 // - a tree of 27 rows over 12289 positions of f16, 51 MB: 22 us + 5.2, 224 shares of 7;
 // - 12 trees, 420 rows, 32 query heads over 8, 60000 positions of int8, 141 MB: 129 us
-//   + 11.4, VALU bound: of a tile's 390 instructions a wave and 64 products 128
-//   make f16 of its bytes, 16 scores a lane take 9 each. 260 TFLOP/s of the
-//   definition's operations, twice that in products.
+//   + 11.4, where VALU (300 instructions a wave and tile, 16 scores a lane taking 9
+//   each) and matrix instructions (64) take turns more than they overlap: 69 % and
+//   34 % of the time. 260 TFLOP/s of the definition's operations, twice that in
+//   products.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "q3h_draft.h"
 #include "q3h_wave.h"
@@ -229,9 +231,14 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
   // operands (64 registers: two waves a SIMD would not have them)
   constexpr bool QLDS = NQ > 1 && !F32;
   constexpr int QW = NQ * (HD / 32) * 2 * 256;  // words of a wave's queries
-  __shared__ __align__(16) float
-      sm_acc[QLDS && QW > NQ * 16 * LD ? kWaves * QW : kWaves * NQ * 16 * LD];
-  __shared__ float2 sm_ml[kWaves][NQ * 16];
+  // with four waves side by side also a tile's keys and values as operands, each
+  // wave's quarter
+  constexpr int ACC = kWaves * NQ * 16 * LD * 4, QB = QLDS ? kWaves * QW * 4 : 0,
+                KVB = QLDS ? T * HD * 2 * 2 : 0, MLB = kWaves * NQ * 16 * 8,
+                ML_AT = ACC > QB + KVB - MLB ? ACC : QB + KVB - MLB;  // (not beside a tile)
+  __shared__ __align__(16) char sm[ML_AT + MLB];
+  float *const sm_acc = reinterpret_cast<float *>(sm);
+  float2(*const sm_ml)[NQ * 16] = reinterpret_cast<float2(*)[NQ * 16]>(sm + ML_AT);
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int per_kv = shape.per_kv;
@@ -395,6 +402,84 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
       return 0;
   };
 
+  // Four waves side by side (more than 64 rows): each loads and converts a quarter
+  // of a tile's operands, all take them from LDS (12 trees of up to 64 rows x 4
+  // heads, int8: 149 -> 143.6 us; 2 x 1500 rows of a prompt, f16: 105 -> 101.4).
+  constexpr int KI = HD / 32, KN = QLDS ? 2 * KI / kWaves : 1, VN = QLDS ? C / kWaves : 1;
+  const bool shared = QLDS && WK == 1;
+  u4 *const sm_k = reinterpret_cast<u4 *>(sm + QB) + lane, *const sm_v = sm_k + 2 * KI * 64;
+  struct Quarter {
+    u4 k[Q8 ? 1 : KN];
+    uint32_t v[8];
+    f4 ks[2], vs[2];
+  };
+  auto load_quarter = [&](Quarter &raw, int tile) {
+    const int j0 = tile * T;
+    const int t = wave >> 1, i = (wave & 1) * KN;
+    const char *p = kbase + (int64_t)j0 * ROW;
+    const uint32_t at = (uint32_t)(std::min(16 * t + n16, last - j0) * ROW + 16 * g4);
+    if constexpr (Q8) {
+      if constexpr (KN == 2) {
+        raw.k[0] = load<u4>(p, at + 32 * i);
+      } else {
+        const u2 x = load<u2>(p, at + 8 * i);
+        raw.k[0][0] = x[0];
+        raw.k[0][1] = x[1];
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < KN; u++) raw.k[u] = load<u4>(p, at + 64 * (i + u));
+    }
+    p = vbase + (int64_t)j0 * ROW;
+    const int word = VN * wave >> (Q8 ? 2 : 1);
+#pragma unroll
+    for (int u = 0; u < 8; u++) {
+      const int j = (u >> 2) * 16 + 4 * g4 + (u & 3);
+      raw.v[u] = load<uint32_t>(
+          p, (uint32_t)(std::min(j, last - j0) * ROW + n16 * (ROW / 16) + 4 * word));
+    }
+    if constexpr (Q8) {
+      load_scales(ksc, j0, raw.ks);
+      load_scales(vsc, j0, raw.vs);
+    }
+  };
+  auto store_quarter = [&](const Quarter &raw) {
+#pragma unroll
+    for (int u = 0; u < KN; u++) {
+      u4 x;
+      if constexpr (Q8) {
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          const uint32_t w = raw.k[0][2 * u + e];
+          x[2 * e] = bytes_f16(w, w, 0x0c010c00u);
+          x[2 * e + 1] = bytes_f16(w, w, 0x0c030c02u);
+        }
+      } else {
+        x = raw.k[u];
+      }
+      sm_k[(wave * KN + u) * 64] = x;
+    }
+#pragma unroll
+    for (int u = 0; u < VN; u++) {
+      const int c = VN * wave + u;
+      // (byte or half c of the words)
+      const uint32_t sel = Q8 ? 0x0c040c00u + 0x00010001u * (uint32_t)(c & 3)
+                              : c & 1 ? 0x07060302u : 0x05040100u;
+      u4 x;
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        if constexpr (Q8) x[e] = bytes_f16(raw.v[2 * e + 1], raw.v[2 * e], sel);
+        else x[e] = __builtin_amdgcn_perm(raw.v[2 * e + 1], raw.v[2 * e], sel);
+      }
+      sm_v[c * 64] = x;
+    }
+  };
+  auto barrier = [&] {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+  };
+
   // the wave's queries: dims of (step, lane group) as the keys' loads have them
   int qrow[NQ], qt[NQ];  // the lane's query row, and the drafted row that it is of
   bool live[NQ];
@@ -428,10 +513,15 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
     }
   }
   Raw<FMT, HD> raw;
+  Quarter quarter;
   int tile = tile0 + wk;
   if (tile < tile1) {
-    load_k(raw, tile);
-    load_v(raw, tile);
+    if (shared) {
+      load_quarter(quarter, tile);
+    } else {
+      load_k(raw, tile);
+      load_v(raw, tile);
+    }
   }
 
 #pragma unroll
@@ -495,7 +585,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
   auto sees = [&](int q, int d) {
     return d < 0 || (d <= qt[q] && (!a.parents || (path[q] >> d & 1)));
   };
-  auto step = [&](Raw<FMT, HD> &raw, int tile) {
+  auto step = [&](auto &raw, int tile, auto share) {
+    constexpr bool SHARE = decltype(share)::value;
     const int j0 = tile * T, next = tile + WK;
     // (the queries stay in LDS: not read once for all tiles)
     if constexpr (QLDS) asm volatile("" ::: "memory");
@@ -520,8 +611,14 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
       for (int i = 0; i < HD / 32; i++)
 #pragma unroll
         for (int t = 0; t < NS; t++) {
+          // int8: the wave at its products goes first, so that the two of a SIMD
+          // move apart, one's products beside the other's softmax (143.6 -> 140.1
+          // us, the prompt in int8 109.6 -> 111.7; f16 trees slower by 0.5 %)
+          if (Q8 && i == 0 && t == 0) __builtin_amdgcn_s_setprio(1);
           u4 ka;
-          if constexpr (Q8) {
+          if constexpr (SHARE) {
+            ka = sm_k[(t * KI + i) * 64];
+          } else if constexpr (Q8) {
 #pragma unroll
             for (int e = 0; e < 2; e++) {
               const uint32_t w = raw.k[t][i >> 1][2 * (i & 1) + e];
@@ -541,6 +638,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
           }
         }
     }
+    if constexpr (Q8) __builtin_amdgcn_s_setprio(0);
     f4 ks[2], vs[2];
     if constexpr (Q8) {
 #pragma unroll
@@ -549,7 +647,11 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
         vs[t] = raw.vs[t];
       }
     }
-    if (next < tile1) load_k(raw, next);
+    if constexpr (SHARE) {
+      if (next < tile1) load_quarter(raw, next);
+    } else {
+      if (next < tile1) load_k(raw, next);
+    }
 
     if (tail && a.parents && !paths) {
       paths = true;
@@ -640,10 +742,13 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
       }
 #pragma unroll
       for (int c = 0; c < C; c++) {
+        if (Q8 && c == 0) __builtin_amdgcn_s_setprio(1);
         u4 va;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          if constexpr (Q8) {
+          if constexpr (SHARE) {
+            // (below)
+          } else if constexpr (Q8) {
             // bytes c of positions 2e and 2e + 1
             va[e] = bytes_f16(vword(raw, 2 * e + 1, c >> 2), vword(raw, 2 * e, c >> 2),
                               0x0c040c00u + 0x00010001u * (c & 3));
@@ -652,6 +757,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
             va[e] = __builtin_amdgcn_perm(y, x, c & 1 ? 0x07060302u : 0x05040100u);
           }
         }
+        if constexpr (SHARE) va = sm_v[c * 64];
         const h8 A = __builtin_bit_cast(h8, va);
 #pragma unroll
         for (int q = 0; q < NQ; q++) {
@@ -660,9 +766,23 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
         }
       }
     }
-    if (next < tile1) load_v(raw, next);
+    if constexpr (Q8) __builtin_amdgcn_s_setprio(0);
+    if constexpr (!SHARE) {
+      if (next < tile1) load_v(raw, next);
+    }
   };
-  for (; tile < tile1; tile += WK) step(raw, tile);
+  if (shared) {
+    if constexpr (QLDS) {
+      for (; tile < tile1; tile++) {
+        store_quarter(quarter);
+        barrier();
+        step(quarter, tile, std::true_type());
+        barrier();
+      }
+    }
+  } else {
+    for (; tile < tile1; tile += WK) step(raw, tile, std::false_type());
+  }
 
   // what the outputs are still to be multiplied with; whether any is NaN (or, as
   // good, infinite)
