@@ -137,11 +137,11 @@ __device__ __forceinline__ Head head_of(const AttendRows &a, const KvSeq &s, con
 // costs half a share a group: the shares come to about two for each CU, what it
 // holds, and to no more than shape.blocks. Of little work one for each CU: a
 // second one on some of the CUs would take them as long as a longer one on all.
-constexpr int kMinSteps = 6, kWorkers = 512;
+constexpr int kWholeSteps = 6, kWorkers = 512;
 __device__ __forceinline__ int share_steps(uint32_t groups, uint32_t steps) {
   const uint32_t w = steps <= kWorkers / 2 * 8 ? kWorkers / 2 : kWorkers;
   const uint32_t n = std::max(w - std::min(groups / 2, w / 2), w / 2);
-  return (int)std::max<uint32_t>(kMinSteps, (steps + n - 1) / n);
+  return (int)std::max(1u, (steps + n - 1) / n);
 }
 __device__ __forceinline__ KvSeq lane_sequence(const KvSeq &x, int l) {
   KvSeq s;
@@ -1026,11 +1026,13 @@ Shape shape_of(int sequences, int rows, int heads, int kvh, int max_len, int til
   const int64_t groups = (int64_t)sequences * kvh * ((q_rows + s.group - 1) / s.group);
   const int wk = kWaves / waves;
   const int64_t steps = ((max_len + rows + tile - 1) / tile + wk - 1) / wk;
-  // no share is shorter than six steps (a workgroup begins and ends in the time of
-  // four, and parts cost a second launch, 4 us); two on every CU, what it holds
-  s.shares = steps > kMinSteps;
+  // Up to six steps no group is cut: parts cost a second launch, 4 us (one row over
+  // 640 positions of f16: 11.1 us whole, 12.5 cut; 900: 14.4 and 11.9). Beyond, the
+  // more workgroups the better, down to one step each (8000 positions: 18.5 us with
+  // six steps at least, 15.4 with one or two).
+  s.shares = steps > kWholeSteps;
   s.blocks = (int)(s.shares ? std::min(std::max<int64_t>(kWorkers - groups / 2, kWorkers / 2) + groups,
-                                       (groups * steps + kMinSteps - 1) / kMinSteps + groups)
+                                       groups * steps)
                             : groups);
   return s;
 }
