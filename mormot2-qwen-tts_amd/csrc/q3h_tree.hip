@@ -135,11 +135,14 @@ __device__ __forceinline__ Head head_of(const AttendRows &a, const KvSeq &s, con
 }
 // The steps of a share at most, from all heads' groups and steps. Rounding up
 // costs half a share a group: the shares come to about two for each CU, what it
-// holds, and to no more than shape.blocks. Of little work one for each CU: a
-// second one on some of the CUs would take them as long as a longer one on all.
+// holds, and to no more than shape.blocks. Of little work one for each CU, as the
+// join has twice the parts otherwise and some of the CUs a second share: one row
+// over 8000 positions of 8 heads 15.4 us, with two 17.3; a tree of 27 over 12289
+// (1544 steps) 26.5 and 29.8; but four rows, 20000 positions in all (1250 steps, 32
+// groups) 20.0 and 18.6, four trees 33 and 29.4.
 constexpr int kWholeSteps = 6, kWorkers = 512;
 __device__ __forceinline__ int share_steps(uint32_t groups, uint32_t steps) {
-  const uint32_t w = steps <= kWorkers / 2 * 8 ? kWorkers / 2 : kWorkers;
+  const uint32_t w = steps <= kWorkers / 2 * (groups < 16 ? 7 : 4) ? kWorkers / 2 : kWorkers;
   const uint32_t n = std::max(w - std::min(groups / 2, w / 2), w / 2);
   return (int)std::max(1u, (steps + n - 1) / n);
 }
