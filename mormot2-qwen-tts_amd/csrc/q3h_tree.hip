@@ -76,9 +76,9 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // workgroup each, so that long and short sequences, full and small groups end
 // together; the shares of a group that has several leave parts, which a second
 // kernel joins. shares: of a short call no group is cut; blocks: workgroups, of
-// shares those that they may come to.
+// shares those that they may come to; parts: that they may leave.
 struct Shape {
-  int nq, group, blocks;
+  int nq, group, blocks, parts;
   bool shares;
   int per_kv;       // query heads of a kv head
   uint32_t by_kv;   // ceil(2^32 / per_kv)
@@ -116,20 +116,22 @@ __device__ __forceinline__ int group_steps(const AttendRows &a, const KvSeq &s, 
                                            int first, int rows_in, int tile) {
   return bad_length(a, s) ? 1 : cut_of(a, s, shape, first, rows_in, tile).steps;
 }
-// a sequence's groups of one kv head: how many, their steps, and their shares of up
-// to `most` steps
+// a sequence's groups of one kv head: how many, their steps, their shares of up to
+// `most` steps, and those of them that leave parts
 struct Head {
-  int groups, steps, shares;
+  int groups, steps, shares, parts;
 };
 __device__ __forceinline__ Head head_of(const AttendRows &a, const KvSeq &s, const Shape &shape,
                                         int tile, int most) {
   const int rows_in = s.count * shape.per_kv;
-  Head h{0, 0, 0};
+  Head h{0, 0, 0, 0};
   for (int first = 0; first < rows_in; first += shape.group) {
     const int n = group_steps(a, s, shape, first, rows_in, tile);
     h.groups++;
     h.steps += n;
-    h.shares += (n + most - 1) / most;
+    const int k = (n + most - 1) / most;
+    h.shares += k;
+    h.parts += k > 1 ? k : 0;
   }
   return h;
 }
@@ -158,9 +160,10 @@ __device__ __forceinline__ KvSeq lane_sequence(const KvSeq &x, int l) {
   return s;
 }
 
-// The workspace of a call: a part for each workgroup, [group][HD] outputs and
-// [group] (maximum, sum); the shares before each sequence, and of one of its
-// heads; the steps of a share.
+// The workspace of a call: for each part [group][HD] outputs and [group] (maximum,
+// sum); the parts before each sequence, and of one of its heads; the steps of a
+// share. (A group of k > 1 shares has more than half of k times a share's steps, so
+// parts are less than twice the shares that all steps come to.)
 struct Parts {
   float *out;
   float2 *ml;
@@ -168,11 +171,11 @@ struct Parts {
 };
 inline size_t parts_bytes(const Shape &s, int sequences, int hd) {
   if (!s.shares) return 0;
-  return sizeof(float) * s.blocks * s.group * (hd + 2) + sizeof(int32_t) * (2 * (size_t)sequences + 1);
+  return sizeof(float) * s.parts * s.group * (hd + 2) + sizeof(int32_t) * (2 * (size_t)sequences + 1);
 }
 __device__ __forceinline__ Parts parts_of(const AttendRows &a, const Shape &s, int hd) {
   Parts p;
-  const size_t rows = (size_t)s.blocks * s.group;
+  const size_t rows = (size_t)s.parts * s.group;
   p.out = a.part;
   p.ml = reinterpret_cast<float2 *>(a.part + rows * hd);
   p.before = reinterpret_cast<int32_t *>(p.ml + rows);
@@ -247,8 +250,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
   const int per_kv = shape.per_kv;
   const int lane = tid & 63;
   // the workgroup's share: steps step0 .. step1 - 1 of group `first` of kv head g
-  // of sequence b; whole: all of the group's
-  int b, g, first, step0 = 0, step1 = 0;
+  // of sequence b; whole: all of the group's, else they leave part `slot`
+  int b, g, first, step0 = 0, step1 = 0, slot = 0;
   KvSeq s;
   bool whole = true;
   const int n = a.kv.sequences;
@@ -263,9 +266,9 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
     KvSeq mine;
     auto head_at = [&](int i, int most) {
       if (most == 1 || n > 64) mine = kv_sequence(a.kv, std::min(i, n - 1));
-      return i < n ? head_of(a, mine, shape, T, most) : Head{0, 0, 0};
+      return i < n ? head_of(a, mine, shape, T, most) : Head{0, 0, 0, 0};
     };
-    Head h{0, 0, 0};
+    Head h{0, 0, 0, 0};
     int groups = 0, steps = 0;
     for (int base = 0; base < n; base += 64) {
       h = head_at(base + lane, 1);
@@ -273,15 +276,17 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
       steps += __builtin_amdgcn_readlane(lane_sums(h.steps), 63) * a.kv.kvh;
     }
     const int most = share_steps(groups, steps), worker = blockIdx.x;
-    int sum = 0, at = 0, shares = 1;
+    int sum = 0, sum_parts = 0, at = 0, shares = 1, head_parts = 0;
     b = -1;
     for (int base = 0; base < n && (b < 0 || worker == 0); base += 64) {
       h = head_at(base + lane, most);
       const int upto = sum + lane_sums(h.shares) * a.kv.kvh, before = upto - h.shares * a.kv.kvh;
+      const int parts_upto = sum_parts + lane_sums(h.parts) * a.kv.kvh,
+                parts_before = parts_upto - h.parts * a.kv.kvh;
       if (worker == 0 && tid < 64 && base + lane < n) {
         const Parts p = parts_of(a, shape, HD);
-        p.before[base + lane] = before;
-        p.head[base + lane] = h.shares;
+        p.before[base + lane] = parts_before;
+        p.head[base + lane] = h.parts;
         *p.most = most;
       }
       const uint64_t hit = __ballot(upto > worker);
@@ -290,14 +295,18 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
         b = base + f;
         at = worker - __builtin_amdgcn_readlane(before, f);
         shares = __builtin_amdgcn_readlane(h.shares, f);
+        slot = __builtin_amdgcn_readlane(parts_before, f);
+        head_parts = __builtin_amdgcn_readlane(h.parts, f);
         s = lane_sequence(mine, f);
       }
       sum = __builtin_amdgcn_readlane(upto, 63);
+      sum_parts = __builtin_amdgcn_readlane(parts_upto, 63);
     }
     // (no share is left; lengths that change while the kernel runs lead nowhere else)
     if (b < 0) return;
     g = at / shares;
     at -= g * shares;
+    slot += g * head_parts;
     const int rows_in = s.count * per_kv;
     for (first = 0; first < rows_in; first += shape.group) {
       const int own = group_steps(a, s, shape, first, rows_in, T), k = (own + most - 1) / most;
@@ -307,12 +316,15 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
         step0 = at * q + std::min(at, longer);
         step1 = step0 + q + (at < longer);
         whole = k == 1;
+        slot += at;
         break;
       }
       at -= k;
+      slot += k > 1 ? k : 0;
     }
   }
-  if (first >= s.count * per_kv) return;
+  // (as for no share: lengths that change meanwhile)
+  if (first >= s.count * per_kv || (!whole && slot >= shape.parts)) return;
   const int n16 = lane & 15, g4 = lane >> 4;
   const int rows_in = s.count * per_kv;  // query rows of the sequence's kv head
   const size_t row0 = (size_t)b * a.kv.rows;
@@ -860,7 +872,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
     __syncthreads();
   }
   const Parts parts = parts_of(a, shape, HD);
-  const size_t part0 = (size_t)blockIdx.x * shape.group - first;
+  const size_t part0 = (size_t)slot * shape.group - first;
 #pragma unroll
   for (int q = 0; q < NQ; q++) {
     float M = m[q], L = l[q], f = 1.f;
@@ -935,15 +947,15 @@ __global__ __launch_bounds__(kThreads) void k_attend_join(AttendRows a, Shape sh
   const KvSeq s = kv_sequence(a.kv, b);
   const Parts parts = parts_of(a, shape, HD);
   const int most = *parts.most;
-  int start = parts.before[b] + g * parts.head[b], n = 0;
+  int start = parts.before[b] + g * parts.head[b], n = 1;
   const int rows_in = s.count * per_kv;
   if (row0 >= rows_in) return;
   const int mine = row0 / shape.group * shape.group;
   for (int first = 0; first <= mine; first += shape.group) {
-    start += n;
+    start += n > 1 ? n : 0;
     n = (group_steps(a, s, shape, first, rows_in, tile) + most - 1) / most;
   }
-  if (n <= 1 || start < 0 || start + n > shape.blocks) return;  // (one share: written as it is)
+  if (n <= 1 || start < 0 || start + n > shape.parts) return;  // (one share: written as it is)
   const int sub = lane / (HD / 4), e = lane % (HD / 4) * 4;
   auto part = [&](int i, int r) {
     return (size_t)(start + i) * shape.group + (std::min(row0 + r, rows_in - 1) - mine);
@@ -1034,9 +1046,13 @@ Shape shape_of(int sequences, int rows, int heads, int kvh, int max_len, int til
   // more workgroups the better, down to one step each (8000 positions: 18.5 us with
   // six steps at least, 15.4 with one or two).
   s.shares = steps > kWholeSteps;
-  s.blocks = (int)(s.shares ? std::min(std::max<int64_t>(kWorkers - groups / 2, kWorkers / 2) + groups,
-                                       groups * steps)
-                            : groups);
+  const int64_t n = std::max<int64_t>(kWorkers - groups / 2, kWorkers / 2);
+  s.blocks = (int)(s.shares ? std::min(n + groups, groups * steps) : groups);
+  // n shares of whole steps and one more a group, or twice n: the most of any number
+  // of groups up to these is at a third of 2 kWorkers
+  s.parts = s.shares ? (int)std::min<int64_t>(
+                           kWorkers + std::min<int64_t>(groups, 2 * kWorkers / 3) / 2 + 2, s.blocks)
+                     : 0;
   return s;
 }
 
