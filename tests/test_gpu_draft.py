@@ -216,6 +216,9 @@ ATTEND = [
     (Q, 128, 2, 1, 1, [4100, 2000], False),
     (H, 128, 2, 1, 9, [4500], True),
     (F, 64, 2, 1, 2, [3333, 4097], False),
+    (H, 64, 8, 2, 300, [900, 350, 0], False),
+    (Q, 128, 8, 8, 2, [900 - 13 * i for i in range(50)], True),
+    (H, 128, 4, 1, 64, [2000, 100, 1500, 30], True),
 ]
 
 
