@@ -12,6 +12,7 @@ to a CPU path: loading fails loudly when libq3h.so is missing.
 """
 import ctypes
 import os
+import struct
 
 import numpy as np
 
@@ -144,31 +145,12 @@ class CacheConfig(ctypes.Structure):
                 ("sequences", "layers", "kv_heads", "head_dim", "max_positions", "format")]
 
 
-class AppendArgs(ctypes.Structure):
-    _fields_ = [(n, ctypes.c_int32) for n in ("layer", "sequences", "rows", "heads")] + \
-        [(n, ctypes.c_void_p) for n in ("q", "k", "v")] + \
-        [(n, ctypes.c_int64) for n in ("ldq", "ldk", "ldv")] + [
-        ("q_out", ctypes.c_void_p), ("ld_out", ctypes.c_int64), ("q_norm", ctypes.c_void_p),
-        ("k_norm", ctypes.c_void_p), ("eps", ctypes.c_float), ("rope", ctypes.c_void_p)] + \
-        [(n, ctypes.c_void_p) for n in ("lens", "counts", "parents")]
-
-
-class AttendArgs(ctypes.Structure):
-    _fields_ = [(n, ctypes.c_int32) for n in
-                ("layer", "sequences", "rows", "heads", "max_len")] + [
-        ("scale", ctypes.c_float), ("q", ctypes.c_void_p), ("ldq", ctypes.c_int64),
-        ("out", ctypes.c_void_p), ("ld_out", ctypes.c_int64)] + \
-        [(n, ctypes.c_void_p) for n in ("lens", "counts", "parents", "workspace")] + \
-        [("workspace_bytes", ctypes.c_int64)]
-
-
-class ScoreArgs(ctypes.Structure):
-    _fields_ = [("logits", ctypes.c_void_p), ("ld", ctypes.c_int64)] + \
-        [(n, ctypes.c_int32) for n in
-         ("dtype", "rows", "vocab", "tokens_per_row", "top_k")] + \
-        [(n, ctypes.c_void_p) for n in
-         ("tokens", "logprobs", "entropy", "top_ids", "top_logprobs", "workspace")] + \
-        [("workspace_bytes", ctypes.c_int64)]
+# q3h_append_args, q3h_attend_args and q3h_score_args, field by field in the
+# header's order with C's alignment: packed for each call, which takes a quarter of
+# the time that a ctypes structure does (2 us of a call's 8)
+APPEND_ARGS = struct.Struct("4i3P3qPqPPfPPPP")
+ATTEND_ARGS = struct.Struct("5ifPqPqPPPPq")
+SCORE_ARGS = struct.Struct("Pq5iPPPPPPq")
 
 
 class RowScores(ctypes.Structure):
@@ -231,13 +213,13 @@ SIGNATURES = {
     "q3h_cache_create": (_I, [_P, ctypes.POINTER(CacheConfig), ctypes.POINTER(_P)]),
     "q3h_cache_bytes": (ctypes.c_int64, [_P]),
     "q3h_cache_destroy": (_I, [_P]),
-    "q3h_cache_append": (_I, [_P, ctypes.POINTER(AppendArgs), _P]),
+    "q3h_cache_append": (_I, [_P, _P, _P]),
     "q3h_cache_read": (_I, [_P, _I, _I, _I, _P, _P, _P, _P, _P]),
     "q3h_cache_attend_workspace": (ctypes.c_int64, [_P, _I, _I, _I, _I]),
-    "q3h_cache_attend": (_I, [_P, ctypes.POINTER(AttendArgs), _P]),
+    "q3h_cache_attend": (_I, [_P, _P, _P]),
     "q3h_cache_keep": (_I, [_P, _I, _I, _P, _P, _P, _P]),
     "q3h_token_logprobs_workspace": (ctypes.c_int64, [_I, _I, _I]),
-    "q3h_token_logprobs": (_I, [_P, ctypes.POINTER(ScoreArgs), _P]),
+    "q3h_token_logprobs": (_I, [_P, _P, _P]),
     "q3h_stack_set_rope": (_I, [_P, ctypes.POINTER(RopeConfig)]),
     "q3h_forward_tree": (_I, [_P, _FP, _I, _IP, _I, ctypes.POINTER(RowScores), _FP, _FP]),
     "q3h_context_keep": (_I, [_P, _IP, _I]),
@@ -804,9 +786,9 @@ def _rows(t, n, rows, heads, hd, ordinal, name):
 
 
 def _whole(t, shape, ordinal, dtype, name):
-    """The address of a contiguous tensor of this shape and dtype; None for None."""
+    """The address of a contiguous tensor of this shape and dtype; 0 for None."""
     if t is None:
-        return None
+        return 0
     if t.shape != shape or not t.is_contiguous():
         _bad(f"{name} is {list(t.shape)}, not contiguous {list(shape)}")
     if t.get_device() != ordinal or t.dtype is not dtype:
@@ -900,10 +882,9 @@ class Cache:
         n, rows = k.shape[0], k.shape[1]
         pk, ldk = _rows(k, n, rows, self.kv_heads, hd, o, "k")
         pv, ldv = _rows(v, n, rows, self.kv_heads, hd, o, "v")
-        heads, pq, ldq, po, ldo, qn = 0, None, 0, None, 0, None
-        turn = None
+        heads = pq = ldq = po = ldo = qn = turn = 0
         if rope is not None:
-            turn = rope.h or _bad("the rotary table is destroyed")
+            turn = rope.h.value if rope.h else _bad("the rotary table is destroyed")
         if q is not None:
             heads = q.shape[2] if q.dim() == 4 else q.shape[2] // hd
             if q_out is None:
@@ -911,11 +892,11 @@ class Cache:
             pq, ldq = _rows(q, n, rows, heads, hd, o, "q")
             po, ldo = _rows(q_out, n, rows, heads, hd, o, "q_out")
             qn = _whole(q_norm, (hd,), o, f32, "q_norm")
-        a = AppendArgs(layer, n, rows, heads, pq, pk, pv, ldq, ldk, ldv, po, ldo, qn,
-                       _whole(k_norm, (hd,), o, f32, "k_norm"), eps,
-                       turn, _whole(lens, (n,), o, i32, "lens"),
-                       _whole(counts, (n,), o, i32, "counts"),
-                       _whole(parents, (n, rows), o, i32, "parents"))
+        a = APPEND_ARGS.pack(
+            layer, n, rows, heads, pq, pk, pv, ldq, ldk, ldv, po, ldo, qn,
+            _whole(k_norm, (hd,), o, f32, "k_norm"), eps, turn,
+            _whole(lens, (n,), o, i32, "lens"), _whole(counts, (n,), o, i32, "counts"),
+            _whole(parents, (n, rows), o, i32, "parents"))
         _check(self._append(self.h, a, _stream(o)))
         return q_out
 
@@ -948,14 +929,14 @@ class Cache:
             out = q.new_empty((n, rows, heads, hd))
         pq, ldq = _rows(q, n, rows, heads, hd, o, "q")
         po, ldo = _rows(out, n, rows, heads, hd, o, "out")
-        need, space = self.attend_workspace(n, rows, heads, max_len), None
+        need, space = self.attend_workspace(n, rows, heads, max_len), 0
         if need:
             workspace = _space(workspace, need, q, o)
             space, need = workspace.data_ptr(), workspace.numel()
-        a = AttendArgs(layer, n, rows, heads, max_len, scale, pq, ldq, po, ldo,
-                       _whole(lens, (n,), o, i32, "lens"),
-                       _whole(counts, (n,), o, i32, "counts"),
-                       _whole(parents, (n, rows), o, i32, "parents"), space, need)
+        a = ATTEND_ARGS.pack(
+            layer, n, rows, heads, max_len, scale, pq, ldq, po, ldo,
+            _whole(lens, (n,), o, i32, "lens"), _whole(counts, (n,), o, i32, "counts"),
+            _whole(parents, (n, rows), o, i32, "parents"), space, need)
         _check(self._attend(self.h, a, _stream(o)))
         return out
 
@@ -1010,7 +991,7 @@ def token_logprobs(dev, logits, tokens, top_k=0, workspace=None):
     at = _ptr(logits, o, torch.bfloat16 if bf16 else f32, "logits")
     m = tokens.shape[1]
     pt = _whole(tokens, (rows, m), o, i32, "tokens")
-    need, space = L.q3h_token_logprobs_workspace(rows, vocab, top_k), None
+    need, space = L.q3h_token_logprobs_workspace(rows, vocab, top_k), 0
     if need < 0:
         _check(need)
     if need:
@@ -1023,9 +1004,9 @@ def token_logprobs(dev, logits, tokens, top_k=0, workspace=None):
     if top_k > 0:
         res["top_ids"] = ids = tokens.new_empty((rows, top_k))
         res["top_logprobs"] = top = new((rows, top_k))
-    a = ScoreArgs(at, stride[0] if rows > 1 else vocab, BF16 if bf16 else F32, rows, vocab, m,
-                  top_k, pt, logprobs.data_ptr(), entropy.data_ptr(),
-                  ids.data_ptr() if top_k > 0 else None, top.data_ptr() if top_k > 0 else None,
-                  space, need)
+    a = SCORE_ARGS.pack(
+        at, stride[0] if rows > 1 else vocab, BF16 if bf16 else F32, rows, vocab, m, top_k, pt,
+        logprobs.data_ptr(), entropy.data_ptr(), ids.data_ptr() if top_k > 0 else 0,
+        top.data_ptr() if top_k > 0 else 0, space, need)
     _check(L.q3h_token_logprobs(dev.h, a, _stream(o)))
     return res

@@ -4,6 +4,7 @@ hand (no device is opened), every call with one argument wrong. Nothing here
 launches: a call that passed its checks would fail for want of a device, with
 another code."""
 import os
+import struct
 import subprocess
 
 import pytest
@@ -14,6 +15,7 @@ HIPCC = "/opt/rocm/bin/hipcc"
 
 SOURCE = r"""
 #include <cmath>
+#include <cstddef>
 #include <cstdio>
 #include <functional>
 
@@ -33,6 +35,11 @@ static void expect(const char *what, int want, long long got) {
 }
 
 int main() {
+  // what the binding packs
+  std::printf("sizes %zu %zu %zu %zu %zu %zu\n", sizeof(q3h_append_args),
+              offsetof(q3h_append_args, rope), sizeof(q3h_attend_args),
+              offsetof(q3h_attend_args, lens), sizeof(q3h_score_args),
+              offsetof(q3h_score_args, tokens));
   q3h_device dev, other;
   dev.ordinal = 0;
   other.ordinal = 1;
@@ -310,3 +317,8 @@ def test_host_checks(tmp_path, q3h):
                     "-L" + PKG, "-l:libq3h.so", "-Wl,-rpath," + PKG, "-o", exe], check=True)
     r = subprocess.run([exe], capture_output=True, text=True, timeout=60)
     assert r.returncode == 0, r.stdout + r.stderr
+    # the binding's formats have the header's sizes and places
+    sizes = [int(x) for x in r.stdout.split("\n")[0].split()[1:]]
+    assert sizes == [q3h.APPEND_ARGS.size, struct.calcsize("4i3P3qPqPPf0P"),
+                     q3h.ATTEND_ARGS.size, struct.calcsize("5ifPqPq"),
+                     q3h.SCORE_ARGS.size, struct.calcsize("Pq5i0P")]
