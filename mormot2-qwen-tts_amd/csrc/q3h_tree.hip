@@ -927,6 +927,132 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
   }
 }
 
+// One or two query rows of a kv head over an f32 cache, uncut: the f32 matrix
+// instructions would spend 14 of their 16 columns on nothing (2048 cycles a tile of
+// 16 positions; here 220 instructions). A wave's tile: a score per lane (position
+// lane % 16, summed over four lanes of HD / 4 elements each), then the values with
+// HD / 64 elements a lane, their weights broadcast. Bound by its round trips
+// (lengths, rows and queries, the waves' meeting): 171 positions, 16 heads over 8,
+// 8.1 us (8.9 on the matrix instructions; 8.6 with four waves, 8.2 with eight), 64
+// such sequences 14.1 (16.5).
+template <int HD>
+__global__ __launch_bounds__(384) void k_attend_few(AttendRows a, int per_kv) {
+  constexpr int R = 2, W = 6, E = HD / 64;
+  typedef float fe __attribute__((ext_vector_type(E)));
+  __shared__ fe sm_acc[W][R][64];
+  __shared__ float2 sm_ml[W][R];
+  auto row_max = [](float v) {  // of the lane's row of 16
+    v = quad_max_dpp(v);
+    v = fmaxf(v, dpp_f_keep<kHalfMirror>(v));
+    return fmaxf(v, dpp_f_keep<kRowMirror>(v));
+  };
+  auto row_sum = [](float v) {
+    v += dpp_f<kQuadXor1>(v);
+    v += dpp_f<kQuadXor2>(v);
+    v += dpp_f<kHalfMirror>(v);
+    return v + dpp_f<kRowMirror>(v);
+  };
+  const int lane = threadIdx.x & 63, n16 = lane & 15, g4 = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int b = blockIdx.x / a.kv.kvh, g = blockIdx.x - b * a.kv.kvh;
+  const KvSeq s = kv_sequence(a.kv, b);
+  const int rows_in = s.count * per_kv;
+  if (rows_in < 1) return;
+  const size_t row0 = (size_t)b * a.kv.rows;
+  // query row r: drafted row r / per_kv (0 or r)
+  auto drafted = [&](int r) { return per_kv == 1 ? r : 0; };
+  auto out = [&](int r) {
+    return a.out + (row0 + drafted(r)) * a.ld_out + (size_t)(g * per_kv + r - drafted(r) * per_kv) * HD;
+  };
+  if (bad_length(a, s)) {
+    for (int i = threadIdx.x; i < rows_in * HD; i += 64 * W) out(i / HD)[i % HD] = NAN;
+    return;
+  }
+  const int end = s.len + s.count, last = end - 1;
+  const char *kbase = s.k0 + kv_row(a.kv, s, 0, g, 0) * (HD * 4);
+  const char *vbase = s.k0 + kv_row(a.kv, s, 1, g, 0) * (HD * 4);
+  f4 q[R][HD / 16];
+#pragma unroll
+  for (int r = 0; r < R; r++) {
+    const int at = std::min(r, rows_in - 1), t = drafted(at);
+    const char *p = reinterpret_cast<const char *>(
+        a.q + (row0 + t) * a.ldq + (size_t)(g * per_kv + at - t * per_kv) * HD);
+#pragma unroll
+    for (int i = 0; i < HD / 16; i++) q[r][i] = load<f4u>(p, 4 * (16 * i + 4 * g4));
+  }
+  // the second of two drafted rows sees the first one if it continues it
+  const int parent = a.parents && s.count > 1 ? a.parents[row0 + 1] : 0;
+  const int root = a.parents ? a.parents[row0] : -1;
+  const float factor = a.scale * kLog2e;
+  float m[R] = {-INFINITY, -INFINITY}, l[R] = {0.f, 0.f};
+  fe acc[R] = {};
+  for (int tile = wave; tile * 16 < end; tile += W) {
+    const int j0 = tile * 16;
+    const char *kp = kbase + (int64_t)j0 * (HD * 4), *vp = vbase + (int64_t)j0 * (HD * 4);
+    f4 k[HD / 16];
+    fe v[16];
+#pragma unroll
+    for (int i = 0; i < HD / 16; i++)
+      k[i] = load<f4>(kp, (uint32_t)(std::min(n16, last - j0) * HD * 4 + 64 * i + 16 * g4));
+#pragma unroll
+    for (int j = 0; j < 16; j++)
+      v[j] = load<fe>(vp, (uint32_t)(std::min(j, last - j0) * HD * 4 + 4 * E * lane));
+    float w[R];
+    uint32_t seen[R];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      float x = 0.f;
+#pragma unroll
+      for (int i = 0; i < HD / 16; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) x = fmaf(k[i][e], q[r][i][e], x);
+      x = rows4_sum(x) * factor;
+      const int d = j0 + n16 - s.len, t = drafted(r);
+      const bool see = d < 0 || d == t || (t == 1 && d == 0 && parent == 0);
+      seen[r] = (uint32_t)__ballot(see) & 0xffffu;
+      x = see ? x : -INFINITY;
+      const float mx = fmaxf(m[r], row_max(x)), base = mx == -INFINITY ? 0.f : mx;
+      const float f = __builtin_amdgcn_exp2f(m[r] - base);
+      w[r] = __builtin_amdgcn_exp2f(x - base);
+      l[r] = fmaf(l[r], f, w[r]);
+      acc[r] *= f;
+      m[r] = mx;
+    }
+#pragma unroll
+    for (int j = 0; j < 16; j++)
+#pragma unroll
+      for (int r = 0; r < R; r++)
+        if (seen[r] >> j & 1) acc[r] += lane_f(w[r], j) * v[j];
+  }
+#pragma unroll
+  for (int r = 0; r < R; r++) {
+    // (each of the four lane groups has all positions)
+    l[r] = row_sum(l[r]);
+    sm_acc[wave][r][lane] = acc[r];
+    if (lane == 0) sm_ml[wave][r] = make_float2(m[r], l[r]);
+  }
+  __syncthreads();
+  if (wave >= rows_in) return;
+  const int r = wave;
+  float M = -INFINITY, L = 0.f;
+#pragma unroll
+  for (int i = 0; i < W; i++) M = fmaxf(M, sm_ml[i][r].x);
+  const float base = M == -INFINITY ? 0.f : M;
+  fe x = {};
+#pragma unroll
+  for (int i = 0; i < W; i++) {
+    const float f = __builtin_amdgcn_exp2f(sm_ml[i][r].x - base);
+    L = fmaf(sm_ml[i][r].y, f, L);
+    x += sm_acc[i][r][lane] * f;
+  }
+  // a parent that is not below its row, on the row's path
+  const bool bad = root >= 0 || root < -1, bad1 = parent > 0 || parent < -1;
+  const int t = drafted(r);
+  const bool broken = t == 0 ? bad : bad1 || (parent == 0 && bad);
+  typedef float feu __attribute__((ext_vector_type(E), aligned(4)));
+  *(reinterpret_cast<feu *>(out(r)) + lane) = broken ? x * NAN : x / L;
+}
+
 // The parts of the rows whose group has several shares, joined. A wave takes
 // neighbouring rows of a group, HD / 4 lanes each, so that it finds its parts once
 // for 256 / HD rows and asks for them in 16 bytes a lane; or four waves do, each
@@ -1066,6 +1192,10 @@ template <int FMT, int HD>
 void launch(const AttendRows &a, hipStream_t st) {
   const Shape s = shape_of(a.kv.sequences, a.kv.rows, a.heads, a.kv.kvh, a.max_len, kTile<FMT>);
   const unsigned blocks = s.blocks;
+  if (FMT == Q3H_KV_F32 && !s.shares && a.kv.rows * s.per_kv <= 2) {
+    hipLaunchKernelGGL((k_attend_few<HD>), dim3(blocks), dim3(384), 0, st, a, s.per_kv);
+    return;
+  }
   if (s.nq == 1)
     hipLaunchKernelGGL((k_attend<FMT, HD, 1>), dim3(blocks), dim3(kThreads), 0, st, a, s);
   else
@@ -1095,7 +1225,7 @@ bool attend_fits(int sequences, int rows, int heads, int kvh, int hd, int fmt, i
       steps_upto(sequences, rows, heads, kvh, max_len, tile) > 0x1p30)
     return false;
   const Shape s = shape_of(sequences, rows, heads, kvh, max_len, tile);
-  return (int64_t)s.blocks * kThreads < most &&
+  return (int64_t)s.blocks * 512 < most &&
          (!s.shares || join_sets(sequences, rows, heads, kvh, hd) * 64 + kThreads < most);
 }
 

@@ -261,6 +261,58 @@ def test_attend_matches_float64(device, case):
         assert (d <= bound[s, :counts[s]]).all()
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("heads,kvh,rows", [(4, 2, 1), (3, 3, 1), (3, 3, 2)])
+@pytest.mark.parametrize("tree", [False, True])
+def test_attend_of_one_or_two_rows(device, hd, heads, kvh, rows, tree):
+    """Single tokens and pairs over short f32 caches, with infinities and NaN where
+    a row does not look, counts of none, bad parents and lengths."""
+    rng = np.random.default_rng(37)
+    lens = np.array([0, 1, 15, 16, 17, 95, 96, 97, 171, 300, 301, 40, 33, 8])
+    n, P = len(lens), 310
+    counts = np.array([rows] * n)
+    counts[4], counts[5] = 0, 1
+    parents = np.array([[-1, -1 + (i % 2)][:rows] for i in range(n)], np.int32)
+    if tree and rows == 2:
+        parents[11], parents[12] = [-1, 1], [0, 0]
+    if tree and rows == 1:
+        parents[11], parents[12] = [0], [-2]
+    k, v = [rng.standard_normal((n, P, kvh, hd)).astype(np.float32) for _ in range(2)]
+    for b in range(n):
+        k[b, lens[b] + rows:, :, 3] = np.nan
+        v[b, lens[b] + rows:, :, 5] = np.inf
+        if tree and rows == 2 and parents[b, 1] == -1:  # row 1 does not see row 0
+            k[b, lens[b]], v[b, lens[b]] = np.nan, -np.inf
+    q = (2 * rng.standard_normal((n, rows, heads, hd))).astype(np.float32)
+    cache = q3h.Cache(device, n, kvh, hd, P, F)
+    fill(cache, k, v, [P] * n)
+    asked = lens.copy()
+    asked[13] = -3
+    out = torch.full((n, rows, heads, hd), 7.0, device="cuda")
+    cache.attend(dev_f(q), dev_i(asked), 302, out=out, counts=dev_i(counts),
+                 parents=dev_i(parents) if tree else None)
+    same = dev_f(q)  # in place
+    cache.attend(same, dev_i(asked), 302, out=same, counts=dev_i(counts),
+                 parents=dev_i(parents) if tree else None)
+    out, same = host(out), host(same)
+    assert np.isnan(out[13]).all()
+    for b in range(13):
+        assert (out[b, counts[b]:] == 7).all() and (same[b, counts[b]:] == q[b, counts[b]:]).all()
+        for t in range(counts[b]):
+            np.testing.assert_array_equal(out[b, t], same[b, t])
+            if tree and (b == 12 or (b == 11 and t == rows - 1)):
+                assert np.isnan(out[b, t]).all()
+                continue
+            if tree and rows == 2 and t == 0 and parents[b, 1] == -1:
+                assert np.isnan(out[b, t]).all()  # it sees its own NaN
+                continue
+            want, bound = ref.attention(
+                q[b:b + 1].astype(np.float64), k[b:b + 1].astype(np.float64),
+                v[b:b + 1].astype(np.float64), [lens[b]], [t + 1],
+                parents[b:b + 1] if tree else None, hd ** -0.5)
+            assert (np.abs(out[b, t] - want[0, t]) <= bound[0, t]).all()
+
+
 @pytest.mark.parametrize("fmt", [F, H, Q])
 @pytest.mark.parametrize("heads", [2, 32])
 def test_unseen_rows_do_not_reach_a_row(device, fmt, heads):
