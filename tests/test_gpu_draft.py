@@ -911,3 +911,31 @@ def test_graphs_that_share_a_workspace(device):
         for (g, q, out, call), w in zip(calls, want):
             assert torch.equal(out, w)
         lens += 20
+
+
+@pytest.mark.parametrize("fmt", [F, H, Q])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("rows,heads", [(1, 2), (3, 10), (40, 6)])
+def test_attend_of_rows_between_boundaries(device, fmt, hd, rows, heads):
+    """Queries and outputs that begin at odd floats, rows an odd number apart; what
+    lies between the rows stays."""
+    rng = np.random.default_rng(38)
+    n, kvh, P, lens = 2, 2, 1100, [1000, 77]
+    cache = q3h.Cache(device, n, kvh, hd, P, fmt)
+    k, v = [rng.standard_normal((n, P, kvh, hd)).astype(np.float32) for _ in range(2)]
+    q = rng.standard_normal((n, rows, heads, hd)).astype(np.float32)
+    fill(cache, k, v, [P] * n)
+
+    def place(ld):
+        buf = torch.full((n * rows * ld + 3,), 9.0, device="cuda")
+        return buf, buf.as_strided((n, rows, heads * hd), (rows * ld, ld, 1), 3)
+
+    (_, tq), (buf, out) = place(heads * hd + 5), place(heads * hd + 7)
+    tq.copy_(dev_f(q).reshape(n, rows, -1))
+    cache.attend(tq, dev_i(lens), 1000, out=out)
+    held = ref.stored(k, fmt).astype(np.float64), ref.stored(v, fmt).astype(np.float64)
+    want, bound = ref.attention(q.astype(np.float64), *held, lens, [rows] * n, None, hd ** -0.5)
+    got = host(out).reshape(want.shape)
+    assert (np.abs(got - want) <= bound).all()
+    out.fill_(9.0)
+    assert (host(buf) == 9).all()
