@@ -289,53 +289,73 @@ __global__ __launch_bounds__(kThreads) void k_cache_append(AppendRows a) {
   }
 }
 
-// 8 elements of a row per thread, keys then values. Memory bound: 32792 positions
-// of 8 heads of 128 from int8, 211 MB of which 168 are written, 55 us (3.8 TB/s; a
-// fill of as much reaches 6.4, a copy 5.0): the rows come in pieces of 128 bytes, a
-// head's positions lying together. Stores that pass the caches took 5 % off;
-// four rows a thread, keys and values in workgroups of their own or loaded
-// together before the first store, changed nothing or cost up to 10 %.
+// 4 elements of kReadRows rows per thread, keys then values. Memory bound: 32792
+// positions of 8 heads of 128 from int8, 211 MB of which 168 are written, 34.7 us
+// (6.1 TB/s). What it takes is that every store instruction writes whole lines, and
+// past the caches: with 8 neighbouring elements a thread, half of each line an
+// instruction, 57.8 us; through the caches 51.5. One row a thread 37.1, four 34.6.
+constexpr int kReadRows = 2;
 template <int FMT, int HD>
 __global__ __launch_bounds__(kThreads) void k_cache_read(KvView kv, const int32_t *starts,
                                                          float *k, float *v) {
-  constexpr int PER = HD / 8;
-  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  const int e = (int)(i % PER) * 8;
-  const int64_t r = i / PER;  // (sequence, row, kv head)
-  const int g = (int)(r % kv.kvh);
-  const int64_t row = r / kv.kvh;
-  if (row >= (int64_t)kv.sequences * kv.rows) return;
-  const int b = (int)(row / kv.rows), t = (int)(row - (int64_t)b * kv.rows);
-  KvSeq s;
-  s.k0 = kv.base + b * kv.seq_bytes;
-  s.max_pos = kv.max_pos;
-  s.len = starts ? starts[b] : 0;
-  s.count = kv.counts ? min(max(kv.counts[b], 0), kv.rows) : kv.rows;
-  if (t >= s.count) return;
-  const bool bad = s.len < 0 || s.len > s.max_pos - s.count;
+  constexpr int PER = HD / 4, SIDE = kThreads / PER;  // threads of a row, rows side by side
+  using KV = std::conditional_t<FMT == Q3H_KV_F32, float,
+                                std::conditional_t<FMT == Q3H_KV_F16, _Float16, uint8_t>>;
+  typedef KV kv4 __attribute__((ext_vector_type(4)));
+  typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+  const int e = (int)(threadIdx.x % PER) * 4;
+  // the workgroup's first row (sequence, position, kv head)
+  const int64_t r0 = (int64_t)blockIdx.x * (SIDE * kReadRows);
+  const int64_t pos0 = r0 / kv.kvh;
+  const int g0 = (int)(r0 - pos0 * kv.kvh), b0 = (int)(pos0 / kv.rows);
+  const uint32_t t0 = (uint32_t)(pos0 - (int64_t)b0 * kv.rows);
+  int64_t at[kReadRows];
+  const char *base[kReadRows];
+  bool there[kReadRows], bad[kReadRows];
+#pragma unroll
+  for (int u = 0; u < kReadRows; u++) {
+    const uint32_t at0 = g0 + u * SIDE + threadIdx.x / PER;
+    const uint32_t pos = at0 / (uint32_t)kv.kvh, g = at0 - pos * kv.kvh;
+    const uint32_t over = (t0 + pos) / (uint32_t)kv.rows;
+    const int b = b0 + (int)over, t = (int)(t0 + pos - over * kv.rows);
+    const int in = min(b, kv.sequences - 1);
+    KvSeq s;
+    s.k0 = kv.base + in * kv.seq_bytes;
+    s.max_pos = kv.max_pos;
+    s.len = starts ? starts[in] : 0;
+    s.count = kv.counts ? min(max(kv.counts[in], 0), kv.rows) : kv.rows;
+    there[u] = b < kv.sequences && t < s.count;
+    bad[u] = s.len < 0 || s.len > s.max_pos - s.count;
+    // (no such row: the first one, which is there)
+    at[u] = kv_row(kv, s, 0, there[u] ? (int)g : 0, there[u] && !bad[u] ? s.len + t : 0);
+    base[u] = s.k0;
+  }
+  const int64_t values = (int64_t)kv.layers * kv.kvh * kv.max_pos;
 #pragma unroll
   for (int part = 0; part < 2; part++) {
     float *dst = part ? v : k;
     if (!dst) continue;
-    float o[8];
-    if (bad) {
-      for (int x = 0; x < 8; x++) o[x] = NAN;
-    } else {
-      const int64_t at = kv_row(kv, s, part, g, s.len + t);
-      if constexpr (FMT == Q3H_KV_Q8) {
-        const uint8_t *p = reinterpret_cast<const uint8_t *>(s.k0) + at * HD + e;
-        const float d = kv_scales(kv, s, HD)[at];
-        for (int x = 0; x < 8; x++) o[x] = kv_byte(p[x]) * d;
-      } else {
-        using KV = std::conditional_t<FMT == Q3H_KV_F16, _Float16, float>;
-        const KV *p = reinterpret_cast<const KV *>(s.k0) + at * HD + e;
-        for (int x = 0; x < 8; x++) o[x] = (float)p[x];
-      }
+    kv4 x[kReadRows];
+    float d[kReadRows];
+#pragma unroll
+    for (int u = 0; u < kReadRows; u++) {
+      const int64_t row = at[u] + part * values;
+      x[u] = *reinterpret_cast<const kv4 *>(reinterpret_cast<const KV *>(base[u]) + row * HD + e);
+      d[u] = FMT == Q3H_KV_Q8 ? reinterpret_cast<const float *>(base[u] + 2 * values * HD)[row] : 1.f;
     }
-    typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
-    float *y = dst + r * HD + e;
-    __builtin_nontemporal_store((f4){o[0], o[1], o[2], o[3]}, reinterpret_cast<f4 *>(y));
-    __builtin_nontemporal_store((f4){o[4], o[5], o[6], o[7]}, reinterpret_cast<f4 *>(y + 4));
+#pragma unroll
+    for (int u = 0; u < kReadRows; u++) {
+      if (!there[u]) continue;
+      f4 o;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        if constexpr (FMT == Q3H_KV_Q8) o[i] = kv_byte(x[u][i]) * d[u];
+        else o[i] = (float)x[u][i];
+        if (bad[u]) o[i] = NAN;
+      }
+      __builtin_nontemporal_store(
+          o, reinterpret_cast<f4 *>(dst + (r0 + u * SIDE + threadIdx.x / PER) * HD + e));
+    }
   }
 }
 
@@ -446,8 +466,8 @@ struct GoAppend {
 template <int FMT, int HD>
 struct GoRead {
   static void go(const KvView &kv, const int32_t *starts, float *k, float *v, hipStream_t st) {
-    const int64_t n = (int64_t)kv.sequences * kv.rows * kv.kvh * (HD / 8);
-    hipLaunchKernelGGL((k_cache_read<FMT, HD>), dim3((unsigned)((n + kThreads - 1) / kThreads)),
+    const int64_t n = (int64_t)kv.sequences * kv.rows * kv.kvh, per = kReadRows * kThreads / (HD / 4);
+    hipLaunchKernelGGL((k_cache_read<FMT, HD>), dim3((unsigned)((n + per - 1) / per)),
                        dim3(kThreads), 0, st, kv, starts, k, v);
   }
 };
