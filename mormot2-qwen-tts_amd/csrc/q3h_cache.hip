@@ -53,9 +53,10 @@ __device__ __forceinline__ int byte_of(float x, float d, double inv) {
   return min(127, max(-127, (int)q)) + 128;
 }
 
-// One head of one row per HD / 8 lanes, 8 elements each: a[i] and b[i] of four
-// pairs that turn together (halves), a's and b's neighbours (interleaved pairs),
-// or elements that do not turn. A wave has 512 / HD heads of a row side by side,
+// One head of one row per HD / 8 lanes, twice four neighbours each, a and b, such
+// that a head's lanes together load and store whole lines: a[i] and b[i] of four
+// pairs that turn together (halves), four pairs of neighbours (interleaved), or
+// elements that do not turn. A wave has 512 / HD heads of a row side by side,
 // kHeads of them one after another with one square root and division for all,
 // and goes over the row's heads with the same turning angles; loads and stores
 // are of 16 bytes a lane (f16: 8, int8: 4). ODD: pairs that are not a multiple of
@@ -65,12 +66,13 @@ __device__ __forceinline__ int byte_of(float x, float d, double inv) {
 // d = fl32(max |y| / 127), byte = rint(y / d).
 //
 // Memory bound over many rows: 3576 rows of 32 + 2 x 8 heads of 128 to f16, 161 MB
-// read and written, 38 us (4.3 TB/s; with a pair a lane, a head over a whole wave,
-// the 64-bit sums of each head made it VALU bound: 60 us). One row: 3.6 us, 496
-// rows of 16 + 2 x 8 heads to int8 7.4 us, which are a launch, the path through
-// the parents and three loads that wait for each other (length, angles, rows).
-constexpr int kHeads = 2;
-template <int FMT, int HD, bool ODD>
+// read and written, 32 us (5.0 TB/s; eight neighbours a lane, half of a line an
+// instruction, 38; a pair a lane, a head over a whole wave, 60: the 64-bit sums of
+// each head made that VALU bound). One row: 3.6 us, 496 rows of 16 + 2 x 8 heads to
+// int8 7.4 us, which are a launch, the path through the parents and three loads that
+// wait for each other (length, angles, rows).
+constexpr int kHeads = 2, kManyRows = 1024;
+template <int FMT, int HD, bool ODD, bool MANY>
 __global__ __launch_bounds__(kThreads) void k_cache_append(AppendRows a) {
   constexpr int G = HD / 8, SIDE = 64 / G;  // lanes of a head, heads side by side
   constexpr int PER = kHeads * SIDE;        // heads of a wave at a time
@@ -90,11 +92,15 @@ __global__ __launch_bounds__(kThreads) void k_cache_append(AppendRows a) {
   const bool rotary = a.table || a.table32;
   const int half = rotary ? a.rot_dim >> 1 : 0;
   // the lane's elements: four from ea, four from eb (ODD: e[i] and e[4 + i])
-  const bool turns = 4 * sub < half, split = rotary && !a.interleaved;
-  int ea = 8 * sub, eb = ea + 4;
+  const bool split = rotary && !a.interleaved;
+  bool turns = 4 * sub < half, turns_b = turns;  // (interleaved: of the first and the last four)
+  int ea = 4 * sub, eb = HD / 2 + ea;
   if (split) {
-    ea = turns ? 4 * sub : a.rot_dim + 2 * (4 * sub - half);
-    eb = turns ? half + 4 * sub : ea + 4;
+    ea = turns ? 4 * sub : a.rot_dim + 4 * sub - half;
+    eb = turns ? half + 4 * sub : ea + (HD - a.rot_dim) / 2;
+  } else {
+    turns = 2 * sub < half;
+    turns_b = HD / 4 + 2 * sub < half;
   }
   int e[ODD ? 8 : 1];
   if constexpr (ODD) {
@@ -108,9 +114,10 @@ __global__ __launch_bounds__(kThreads) void k_cache_append(AppendRows a) {
   double2 cs[4];
 #pragma unroll
   for (int i = 0; i < 4; i++) {
+    const int p = ODD || split ? 4 * sub + i : (i < 2 ? 2 * sub + i : HD / 4 + 2 * sub + i - 2);
     cs[i] = make_double2(1.0, 0.0);
-    if (4 * sub + i < half && !bad) {
-      const size_t at = (size_t)(s.len + depth) * half + 4 * sub + i;
+    if (p < half && !bad) {
+      const size_t at = (size_t)(s.len + depth) * half + p;
       if (a.table) {
         cs[i] = a.table[at];
       } else {
@@ -124,8 +131,8 @@ __global__ __launch_bounds__(kThreads) void k_cache_append(AppendRows a) {
 #pragma unroll
       for (int i = 0; i < 8; i++) x[i] = p[e[ODD ? i : 0]];
     } else {
-      const f4u w0 = *reinterpret_cast<const f4u *>(p + (values ? 8 * sub : ea));
-      const f4u w1 = *reinterpret_cast<const f4u *>(p + (values ? 8 * sub + 4 : eb));
+      const f4u w0 = *reinterpret_cast<const f4u *>(p + (values ? 4 * sub : ea));
+      const f4u w1 = *reinterpret_cast<const f4u *>(p + (values ? HD / 2 + 4 * sub : eb));
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         x[i] = w0[i];
@@ -193,14 +200,15 @@ __global__ __launch_bounds__(kThreads) void k_cache_append(AppendRows a) {
 #pragma unroll
           for (int i = 0; i < 4; i++)
             if (4 * sub + i < half) turn(y[u][i], y[u][4 + i], i);
-        } else if (turns) {
-          if (split) {
+        } else if (split) {
+          if (turns) {
 #pragma unroll
             for (int i = 0; i < 4; i++) turn(y[u][i], y[u][4 + i], i);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 4; i++) turn(y[u][2 * i], y[u][2 * i + 1], i);
           }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            if (i < 2 ? turns : turns_b) turn(y[u][2 * i], y[u][2 * i + 1], i);
         }
 #pragma unroll
         for (int i = 0; i < 8; i++) x[u][i] = (float)y[u][i];
@@ -236,7 +244,7 @@ __global__ __launch_bounds__(kThreads) void k_cache_append(AppendRows a) {
         }
       }
     }
-    const int e_a = values ? 8 * sub : ea, e_b = values ? 8 * sub + 4 : eb;
+    const int e_a = values ? 4 * sub : ea, e_b = values ? HD / 2 + 4 * sub : eb;
 #pragma unroll
     for (int u = 0; u < kHeads; u++) {
       const int j = first + u * SIDE;
@@ -258,7 +266,11 @@ __global__ __launch_bounds__(kThreads) void k_cache_append(AppendRows a) {
           for (int i = 0; i < 8; i++) x[u][i] = NAN;
         }
         put([&](int at, int i) {
-          *reinterpret_cast<f4u *>(o + at) = (f4u){x[u][i], x[u][i + 1], x[u][i + 2], x[u][i + 3]};
+          const f4u y = {x[u][i], x[u][i + 1], x[u][i + 2], x[u][i + 3]};
+          // (MANY: past the caches, 45.6 -> 41.0 us with the read, of the keys and values
+          // too 44.5; few rows stay for the attention that comes next)
+          if constexpr (MANY) __builtin_nontemporal_store(y, reinterpret_cast<f4u *>(o + at));
+          else *reinterpret_cast<f4u *>(o + at) = y;
         }, [&](int at, int i) { o[at] = x[u][i]; });
         continue;
       }
@@ -455,12 +467,14 @@ struct GoAppend {
     // few rows: a wave for each group of heads; many: one workgroup a row, its
     // waves going over the heads with one load of the angles
     const int rows = a.kv.sequences * a.kv.rows;
-    const int side = rows >= 1024 ? 1 : (groups + kThreads / 64 - 1) / (kThreads / 64);
+    const int side = rows >= kManyRows ? 1 : (groups + kThreads / 64 - 1) / (kThreads / 64);
     const dim3 grid(rows, side);
     if ((a.table || a.table32) && a.rot_dim % 8 != 0)
-      hipLaunchKernelGGL((k_cache_append<FMT, HD, true>), grid, dim3(kThreads), 0, st, a);
+      hipLaunchKernelGGL((k_cache_append<FMT, HD, true, false>), grid, dim3(kThreads), 0, st, a);
+    else if (rows >= kManyRows)
+      hipLaunchKernelGGL((k_cache_append<FMT, HD, false, true>), grid, dim3(kThreads), 0, st, a);
     else
-      hipLaunchKernelGGL((k_cache_append<FMT, HD, false>), grid, dim3(kThreads), 0, st, a);
+      hipLaunchKernelGGL((k_cache_append<FMT, HD, false, false>), grid, dim3(kThreads), 0, st, a);
   }
 };
 template <int FMT, int HD>
