@@ -22,19 +22,23 @@
 // each would be half the products; the sums were then 2^-12 off instead of 2^-21.)
 //
 // What bounds it, by how much a share has to do (heads of 128):
-// - one row over 171 positions of an f32 cache, 8 workgroups of 2 or 3 tiles a wave:
-//   9.0 us, a launch and the round trips of one workgroup (lengths, rows, the waves'
-//   meeting);
-// - 32 sequences of one row, 41000 positions of int8 in all, 87 MB: 23.5 us + 4.2 for
-//   the parts, 432 shares of 8 steps, where a workgroup takes 10 us to find its
-//   share, have its first tiles and join its waves, and 1.45 a step. Shares of fewer
-//   steps, or three workgroups a CU at 168 registers (27 us), were slower;
+// - one row over 171 positions of an f16 cache, 8 workgroups of 2 tiles a wave:
+//   6.8 us, a launch and the round trips of one workgroup (lengths, rows, the waves'
+//   meeting); f32: k_attend_few;
+// - 32 sequences of one row, 41000 positions of int8 in all, 87 MB: 23.5-25 us + 4.5
+//   for the parts, 432 shares of 8 steps, where a workgroup takes 10 us to find its
+//   share, have its first tiles and join its waves, and 1.45 a step; the same in f16
+//   168 MB 44 us, in f32 335 MB 77.6 us (4.3 TB/s). Three workgroups a CU at 168
+//   registers (27 us of 23.5), two tiles ahead (29.8 us of 29.1) and loads past the
+//   caches (31.2 of 29.3) were slower;
 // - a tree of 27 rows over 12289 positions of f16, 51 MB: 22 us + 5.2, 224 shares of 7;
-// - 12 trees, 420 rows, 32 query heads over 8, 60000 positions of int8, 141 MB: 129 us
-//   + 11.4, where VALU (300 instructions a wave and tile, 16 scores a lane taking 9
+// - 12 trees, 420 rows, 32 query heads over 8, 60000 positions of int8, 141 MB: 118-129
+//   us + 11.4, where VALU (300 instructions a wave and tile, 16 scores a lane taking 9
 //   each) and matrix instructions (64) take turns more than they overlap: 69 % and
-//   34 % of the time. 260 TFLOP/s of the definition's operations, twice that in
-//   products.
+//   34 % of the time. 270 TFLOP/s of the definition's operations, twice that in
+//   products;
+// - 2 prompts of 1500 rows over 500 positions, 16 heads over 8: f16 101 us, int8 112,
+//   f32 234 (131 of the 154 TFLOP/s of a large f32 product).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
