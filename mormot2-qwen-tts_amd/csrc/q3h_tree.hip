@@ -681,10 +681,27 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
         broken[q] = __shfl((int)p.bad, qt[q]) != 0;
       }
     }
+    // int8: the largest scale of the tile, and whether some are so much smaller
+    // (2^16; a weight's two parts have 39 bits below 2^14) that the maximum has to be
+    // taken of scores and scales together, position by position. A scale's power of
+    // two is taken within 2^-40 .. 2^50: further apart, the factor between two tiles'
+    // sums would leave f32. Weights of larger scales leave f16 and become NaN, a wave
+    // whose scales are all far smaller is known by the largest: both are done again
+    // below.
     float w[NQ][4 * NS], top = 0.f;
+    bool wide = tail;
+    auto power = [](float x) {
+      return (float)std::min(50, std::max(-40, (int)(__float_as_uint(x) >> 23) - 126));
+    };
     if constexpr (Q8) {
+      float low = INFINITY;
 #pragma unroll
-      for (int i = 0; i < 8; i++) top = fmaxf(top, vs[i >> 2][i & 3]);
+      for (int i = 0; i < 8; i++) {
+        top = fmaxf(top, vs[i >> 2][i & 3]);
+        low = fminf(low, vs[i >> 2][i & 3]);
+      }
+      top = rows4_max(top);
+      wide = wide || __any(low < top * 0x1p-16f);
     }
 #pragma unroll
     for (int q = 0; q < NQ; q++) {
@@ -704,21 +721,23 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
           if (broken[q] && d == qt[q]) w[q][i] = NAN;
           if (Q8 && see) vx = fmaxf(vx, vs[i >> 2][i & 3]);
         }
+        if constexpr (Q8) vx = rows4_max(vx);
       }
 #pragma unroll
       for (int i = 0; i < 4 * NS; i++) mx = fmaxf(mx, w[q][i]);
-      mx = rows4_max(mx);
       float off = F32 ? 0.f : -14.f;
-      if constexpr (Q8) {
-        // (of 2^-40 .. 2^50: further apart, the factor between two tiles' sums
-        // would leave f32. Weights of larger scales leave f16 and become NaN, a wave
-        // whose scales are all far smaller is known by the largest: both are done
-        // again below)
-        vx = rows4_max(vx);
-        vmax[q] = fmaxf(vmax[q], vx);
-        off += (float)std::min(50, std::max(-40, (int)(__float_as_uint(vx) >> 23) - 126));
+      if (Q8 && wide) {
+        asm volatile("");
+        mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 4 * NS; i++)
+          mx = fmaxf(mx, fmaf(w[q][i], sfac[q], power(vs[i >> 2][i & 3])));
+        mx = rows4_max(mx) + off;
+      } else {
+        mx = fmaf(rows4_max(mx), sfac[q], Q8 ? off + power(top) : off);
       }
-      mx = fmaxf(m[q], fmaf(mx, sfac[q], off));
+      if constexpr (Q8) vmax[q] = fmaxf(vmax[q], vx);
+      mx = fmaxf(m[q], mx);
       const float base = mx == -INFINITY ? 0.f : mx;
       if (__any(mx > m[q])) {
         const float f = __builtin_amdgcn_exp2f(m[q] - base);

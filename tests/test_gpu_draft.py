@@ -939,3 +939,28 @@ def test_attend_of_rows_between_boundaries(device, fmt, hd, rows, heads):
     assert (np.abs(got - want) <= bound).all()
     out.fill_(9.0)
     assert (host(buf) == 9).all()
+
+
+@pytest.mark.parametrize("fmt", [F, Q])
+@pytest.mark.parametrize("up", [20, 30, 38])
+@pytest.mark.parametrize("heads,length", [(1, 40), (24, 40), (2, 3000)])
+def test_large_values_of_little_weight_cost_no_precision(device, fmt, up, heads, length):
+    """Positions that a row sees, whose values are larger by 2^up and whose weights
+    are smaller by more: the others' sum keeps its precision."""
+    rng = np.random.default_rng(39)
+    hd, P = 64, length + 1
+    q = rng.standard_normal((1, 1, heads, hd)).astype(np.float32)
+    q[..., 0] = 8
+    k = (0.1 * rng.standard_normal((1, P, 1, hd))).astype(np.float32)
+    v = rng.standard_normal((1, P, 1, hd)).astype(np.float32)
+    for j in range(5, P, 19):
+        k[0, j, 0, 0] = -(up + 12) * np.log(2)  # a score of -8 / 8 of it
+        v[0, j] *= 2.0 ** up
+    cache = q3h.Cache(device, 1, 1, hd, P, fmt)
+    fill(cache, k, v, [P])
+    held = ref.stored(k, fmt).astype(np.float64), ref.stored(v, fmt).astype(np.float64)
+    want, bound = ref.attention(q.astype(np.float64), *held, [length], [1], None, 1 / 8)
+    out = host(cache.attend(dev_f(q), dev_i([length]), length, scale=1 / 8))
+    ratio = np.abs(out - want) / bound
+    print(ratio.max(), flush=True)
+    assert (ratio <= 1).all()
