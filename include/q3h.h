@@ -495,8 +495,10 @@ int q3h_cache_read(q3h_cache *c, int layer, int sequences, int rows, const int32
    [..][heads][head_dim], heads a multiple of kv_heads, query head h on kv head
    h / (heads / kv_heads). max_len: no length in lens is above it (the host's
    bound, it sizes the launch; a longer or negative one: NaN rows). scale: 0 for
-   1 / sqrt(head_dim). Products and sums keep f32's precision in every format (an
-   f16 cache's elements below 2^-14 count to 2^-38).
+   1 / sqrt(head_dim). Products and sums keep f32's precision in every format;
+   over f16 and int8 caches that is relative to the row's largest element (an
+   element to which only positions of a weight near 2^-24 add is less exact), and
+   an f16 cache's elements below 2^-14 count to 2^-38.
    Infinities and NaN at positions a row does not see do not reach it. workspace:
    q3h_cache_attend_workspace bytes for the same sequences, rows, heads and max_len
    (of the caller, 256-byte aligned, one for each call that may run at once;
