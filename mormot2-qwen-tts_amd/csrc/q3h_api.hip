@@ -1220,6 +1220,7 @@ extern "C" int q3h_context_time_attention(q3h_context *c, int iters, float *us_p
     const int ldq = NQ + 2 * NKV;
     const bool kv16 = cf.kv_f16 != 0;
     w.ensure(s, 1, attention_splits(s, positions), 0);
+    c->drafted.clear();  // (position len is written)
     check_hip(hipStreamCreateWithFlags(&st, hipStreamNonBlocking), "hipStreamCreate");
     check_hip(hipMemsetAsync(w.qkv, 0, sizeof(float) * ldq, st), "zero");
     launch_prep(c->dev_arr, nullptr, 1, 1, w.rd, st);
