@@ -6,8 +6,10 @@ import gc
 import numpy as np
 import pytest
 
+import draft_ref as ref
 import q3h
-from test_gpu_draft_forward import Setup, rows_of
+from test_gpu_draft_forward import (CASES, DIMS, HD, HEADS, KVH, Model64, Setup, bar, rel,
+                                    rows_of)
 
 pytestmark = pytest.mark.gpu
 
@@ -35,3 +37,79 @@ def test_a_measured_attention_drops_the_tree(device, fmt):
     c.keep([0, 1])
     assert c.length == 4
     s.destroy(c)
+
+
+# ---------------------------------------------------------------------------
+# long contexts
+
+
+def cut(device, s, rows, positions):
+    """Whether the attention of rows over so many positions leaves parts."""
+    c = q3h.Cache(device, 1, KVH, HD, positions, s.fmt)
+    need = c.attend_workspace(1, rows, HEADS, positions - rows)
+    c.destroy()
+    return need > 0
+
+
+def filled(s, c, m, n, seed=3):
+    """n random positions in the context c and in the models m."""
+    rng = np.random.default_rng(seed)
+    k, v = (rng.standard_normal((DIMS["layers"], KVH, n, HD)).astype(np.float32)
+            for _ in range(2))
+    c.fill_kv(k, v)
+    for model in m:
+        for l in range(DIMS["layers"]):
+            a, b = (ref.stored(t[l], s.fmt).astype(np.float64) for t in (k, v))
+            model.cache[l] = [(a[:, p], b[:, p]) for p in range(n)]
+
+
+def drafted_tree(rows, seed):
+    rng = np.random.default_rng(seed)
+    return np.maximum(np.arange(rows) - rng.geometric(0.4, rows), -1).astype(np.int32)
+
+
+LONG = 2304
+LONG_CASES = ["f32", "f16", "int8", "q8_weights_int8", "yarn"]
+
+
+@pytest.mark.parametrize("case", LONG_CASES)
+def test_trees_and_rows_of_long_contexts(device, case):
+    """A tree of each size of group, a path of it kept, then single rows: direct,
+    replayed, of a batch, without allocations, over 1500 positions and more,
+    against float64."""
+    print(f"long {case}", flush=True)
+    s = Setup(device, max_positions=LONG, **CASES[case])
+    own = CASES[case].get("fmt") == q3h.KV_Q8 or "rope" in CASES[case]
+    m, c = Model64(s), s.context(LONG)
+    filled(s, c, [m], 1500)
+    for rows, seed in ((7, 1), (23, 2), (64, 3), (1, 4)):
+        assert cut(device, s, rows, c.length + rows)
+        parents, x = drafted_tree(rows, seed), rows_of(100 + seed, rows)
+        got = c.forward_tree(x, parents, head=s.head)
+        want = m.forward(x, parents)
+        assert rel(got["normed"], want) <= bar(case)
+        assert rel(got["logits"], m.logits(want)) <= bar(case)
+        kept = ref.path(parents, rows - 1)[::-1]
+        c.keep(kept)
+        m.keep(kept)
+        assert c.length == len(m.cache[0])
+        for i, noalloc in enumerate((False, False, True)):
+            assert not own or cut(device, s, 1, c.length + 1)
+            x = rows_of(200 + 10 * seed + i, 1)
+            logits, normed = c.forward(x, head=s.head, noalloc=noalloc)
+            want = m.forward(x)
+            assert rel(normed, want[0]) <= bar(case)
+            assert rel(logits, m.logits(want)[0]) <= bar(case)
+    x = rows_of(300, 20)
+    logits, _ = c.forward(x, head=s.head)  # several rows
+    want = m.forward(x)
+    assert rel(logits, m.logits(want)[-1]) <= bar(case)
+    # a batch whose first context is short: plain launches, then the captured ones
+    d, n = s.context(LONG), Model64(s)
+    filled(s, d, [n], 30)
+    for i in range(3):
+        x = rows_of(400 + i, 2)
+        lg, _ = q3h.forward_batch([d, c], x, [s.head] * 2)
+        assert rel(lg[0], n.logits(n.forward(x[:1]))[0]) <= bar(case)
+        assert rel(lg[1], m.logits(m.forward(x[1:]))[0]) <= bar(case)
+    s.destroy(c, d)
