@@ -116,15 +116,16 @@ bool work_carve(const q3h_stack *s, int rows, int splits, int head_rows, size_t 
                 void *base, size_t cap, Work &w) {
   size_t off = 0;
   bool fits = true;
-  auto carve = [&](void **slot, size_t bytes) {
+  work_fields(s, rows, splits, head_rows, w, [&](void **slot, size_t bytes) {
     off = (off + 255) & ~(size_t)255;
     fits = fits && off + bytes <= cap;
     *slot = fits ? (char *)base + off : nullptr;
     off += bytes;
-  };
-  work_fields(s, rows, splits, head_rows, w, carve);
-  if (tree_bytes) carve((void **)&w.tree, tree_bytes);
-  w.tree_bytes = tree_bytes;
+  });
+  off = (off + 255) & ~(size_t)255;
+  w.carved = true;
+  w.tree_bytes = fits && off < cap ? std::min(tree_bytes, cap - off) : 0;
+  w.tree = w.tree_bytes ? reinterpret_cast<float *>((char *)base + off) : nullptr;
   w.rows_cap = rows;
   w.splits_cap = splits;
   w.head_cap = head_rows;
@@ -273,8 +274,9 @@ static void attend_drafted(const q3h_stack *s, Work &w, int l, int M, int positi
   t.ld_out = NQ;
   t.parents = io.parents;
   t.part = w.tree;
-  require(attend_part_bytes(M / rows, rows, c.heads, c.kv_heads, hd, c.kv_f16, positions) <=
-              w.tree_bytes,
+  t.room = w.tree_bytes;
+  require(w.carved || attend_part_bytes(M / rows, rows, c.heads, c.kv_heads, hd, c.kv_f16,
+                                        positions) <= w.tree_bytes,
           Q3H_E_HIP, "the attention's parts have no room");
   launch_cache_attend(t, hd, c.kv_f16, st);
 }

@@ -179,6 +179,7 @@ struct Work {
   // parts of the attention over drafted rows (q3h_draft.h)
   float *tree = nullptr;
   size_t tree_bytes = 0;
+  bool carved = false;  // by work_carve, with what room there was for the parts
   void ensure_tree(size_t bytes);
   void ensure(const struct ::q3h_stack *s, int rows, int splits, int head_rows);
   void release();
@@ -186,7 +187,8 @@ struct Work {
 
 // w's buffers for (rows, splits, head_rows) carved from [base, base + cap),
 // each at a 256-byte boundary (w owns nothing: never release it); false when
-// they do not fit
+// they do not fit. The parts of the attention over drafted rows take what is left,
+// up to tree_bytes.
 bool work_carve(const struct ::q3h_stack *s, int rows, int splits, int head_rows,
                 size_t tree_bytes, void *base, size_t cap, Work &w);
 // the bytes of Work::tree for a forward of n contexts, rows rows each, over up to

@@ -879,6 +879,7 @@ extern "C" int q3h_cache_attend(q3h_cache *c, const q3h_attend_args *p, void *st
     a.ld_out = p->ld_out;
     a.parents = p->parents;
     a.part = (float *)p->workspace;
+    a.room = need;
     launch_cache_attend(a, cf.head_dim, cf.format, (hipStream_t)stream);
     check_hip(hipGetLastError(), "cache attention kernels");
   });

@@ -125,7 +125,8 @@ struct AttendRows {
   float *out;
   int64_t ld_out;
   const int32_t *parents;
-  float *part;  // attend_part_bytes
+  float *part;
+  size_t room;  // bytes of part: attend_part_bytes, or less (fewer parts then)
 };
 size_t attend_part_bytes(int sequences, int rows, int heads, int kvh, int hd, int fmt,
                          int max_len);

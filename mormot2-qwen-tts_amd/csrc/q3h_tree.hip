@@ -80,9 +80,11 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // workgroup each, so that long and short sequences, full and small groups end
 // together; the shares of a group that has several leave parts, which a second
 // kernel joins. shares: of a short call no group is cut; blocks: workgroups, of
-// shares those that they may come to; parts: that they may leave.
+// shares those that they may come to; parts: that they may leave; workers: how many
+// shares of much work there are, about: kWorkers, fewer where the parts of so many
+// have no room.
 struct Shape {
-  int nq, group, blocks, parts;
+  int nq, group, blocks, parts, workers;
   bool shares;
   int per_kv;       // query heads of a kv head
   uint32_t by_kv;   // ceil(2^32 / per_kv)
@@ -147,8 +149,8 @@ __device__ __forceinline__ Head head_of(const AttendRows &a, const KvSeq &s, con
 // (1544 steps) 26.5 and 29.8; but four rows, 20000 positions in all (1250 steps, 32
 // groups) 20.0 and 18.6, four trees 33 and 29.4.
 constexpr int kWholeSteps = 6, kWorkers = 512;
-__device__ __forceinline__ int share_steps(uint32_t groups, uint32_t steps) {
-  const uint32_t w = steps <= kWorkers / 2 * (groups < 16 ? 7 : 4) ? kWorkers / 2 : kWorkers;
+__device__ __forceinline__ int share_steps(uint32_t groups, uint32_t steps, uint32_t workers) {
+  const uint32_t w = steps <= workers / 2 * (groups < 16 ? 7 : 4) ? workers / 2 : workers;
   const uint32_t n = std::max(w - std::min(groups / 2, w / 2), w / 2);
   return (int)std::max(1u, (steps + n - 1) / n);
 }
@@ -279,7 +281,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
       groups += __builtin_amdgcn_readlane(lane_sums(h.groups), 63) * a.kv.kvh;
       steps += __builtin_amdgcn_readlane(lane_sums(h.steps), 63) * a.kv.kvh;
     }
-    const int most = share_steps(groups, steps), worker = blockIdx.x;
+    const int most = share_steps(groups, steps, shape.workers), worker = blockIdx.x;
     int sum = 0, sum_parts = 0, at = 0, shares = 1, head_parts = 0;
     b = -1;
     for (int base = 0; base < n && (b < 0 || worker == 0); base += 64) {
@@ -1179,7 +1181,9 @@ double steps_upto(int sequences, int rows, int heads, int kvh, int max_len, int 
          ((max_len + rows + tile - 1) / tile);
 }
 
-Shape shape_of(int sequences, int rows, int heads, int kvh, int max_len, int tile) {
+// room: bytes that the parts have
+Shape shape_of(int sequences, int rows, int heads, int kvh, int hd, int max_len, int tile,
+               size_t room) {
   Shape s;
   s.per_kv = heads / kvh;
   s.by_kv = (uint32_t)(((1ull << 32) + s.per_kv - 1) / s.per_kv);
@@ -1195,13 +1199,19 @@ Shape shape_of(int sequences, int rows, int heads, int kvh, int max_len, int til
   // more workgroups the better, down to one step each (8000 positions: 18.5 us with
   // six steps at least, 15.4 with one or two).
   s.shares = steps > kWholeSteps;
-  const int64_t n = std::max<int64_t>(kWorkers - groups / 2, kWorkers / 2);
-  s.blocks = (int)(s.shares ? std::min(n + groups, groups * steps) : groups);
-  // n shares of whole steps and one more a group, or twice n: the most of any number
-  // of groups up to these is at a third of 2 kWorkers
-  s.parts = s.shares ? (int)std::min<int64_t>(
-                           kWorkers + std::min<int64_t>(groups, 2 * kWorkers / 3) / 2 + 2, s.blocks)
-                     : 0;
+  for (int w = s.workers = kWorkers; s.shares && w > 0; w -= kWorkers / 16) {
+    const int64_t n = std::max<int64_t>(w - groups / 2, w / 2);
+    s.workers = w;
+    s.blocks = (int)std::min(n + groups, groups * steps);
+    // n shares of whole steps and one more a group, or twice n: the most of any number
+    // of groups up to these is at a third of 2 w
+    s.parts = (int)std::min<int64_t>(w + std::min<int64_t>(groups, 2 * w / 3) / 2 + 2, s.blocks);
+    if (parts_bytes(s, sequences, hd) <= room) return s;
+  }
+  // short, or no room for the parts of any cut: whole groups
+  s.shares = false;
+  s.blocks = (int)groups;
+  s.parts = 0;
   return s;
 }
 
@@ -1213,7 +1223,8 @@ int64_t join_sets(int sequences, int rows, int heads, int kvh, int hd) {
 
 template <int FMT, int HD>
 void launch(const AttendRows &a, hipStream_t st) {
-  const Shape s = shape_of(a.kv.sequences, a.kv.rows, a.heads, a.kv.kvh, a.max_len, kTile<FMT>);
+  const Shape s = shape_of(a.kv.sequences, a.kv.rows, a.heads, a.kv.kvh, HD, a.max_len, kTile<FMT>,
+                           a.room);
   const unsigned blocks = s.blocks;
   if (FMT == Q3H_KV_F32 && !s.shares && a.kv.rows * s.per_kv <= 2) {
     hipLaunchKernelGGL((k_attend_few<HD>), dim3(blocks), dim3(384), 0, st, a, s.per_kv);
@@ -1236,7 +1247,8 @@ void launch(const AttendRows &a, hipStream_t st) {
 
 size_t attend_part_bytes(int sequences, int rows, int heads, int kvh, int hd, int fmt,
                          int max_len) {
-  return parts_bytes(shape_of(sequences, rows, heads, kvh, max_len, fmt == Q3H_KV_F32 ? 16 : 32),
+  return parts_bytes(shape_of(sequences, rows, heads, kvh, hd, max_len, fmt == Q3H_KV_F32 ? 16 : 32,
+                              SIZE_MAX),
                      sequences, hd);
 }
 
@@ -1247,7 +1259,7 @@ bool attend_fits(int sequences, int rows, int heads, int kvh, int hd, int fmt, i
   if (rows * per_kv * per_kv >= most ||
       steps_upto(sequences, rows, heads, kvh, max_len, tile) > 0x1p30)
     return false;
-  const Shape s = shape_of(sequences, rows, heads, kvh, max_len, tile);
+  const Shape s = shape_of(sequences, rows, heads, kvh, hd, max_len, tile, SIZE_MAX);
   return (int64_t)s.blocks * 512 < most &&
          (!s.shares || join_sets(sequences, rows, heads, kvh, hd) * 64 + kThreads < most);
 }

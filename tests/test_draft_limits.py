@@ -1,0 +1,85 @@
+"""What the host works out before rows of drafts are launched - the room of a
+forward's buffers, counts that a launch or 32 bits hold - on the CPU: a program
+linked to the library with handles filled in by hand (no device is opened)."""
+import os
+import subprocess
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+PKG = os.path.join(ROOT, "mormot2-qwen-tts_amd")
+HIPCC = "/opt/rocm/bin/hipcc"
+
+HEAD = r"""
+#include <algorithm>
+#include <cstdio>
+#include <initializer_list>
+
+#include "q3h.h"
+#include "q3h_api_internal.h"
+#include "q3h_draft.h"
+
+static int bad = 0;
+#define EXPECT(x, ...)                    \
+  do {                                    \
+    if (!(x)) {                           \
+      std::printf("%s: ", #x);            \
+      std::printf(__VA_ARGS__);           \
+      std::printf("\n");                  \
+      bad++;                              \
+    }                                     \
+  } while (0)
+
+// 16 heads over 8 of 128, the layers' widths those of a small talker
+static void dims(q3h_stack &s, int fmt, int max_positions) {
+  s.cfg.layers = 2, s.cfg.hidden = 1024, s.cfg.heads = 16, s.cfg.kv_heads = 8;
+  s.cfg.head_dim = 128, s.cfg.intermediate = 2048, s.cfg.kv_f16 = fmt;
+  s.cfg.max_positions = max_positions;
+  s.ext = true;
+}
+"""
+
+
+def run(tmp_path, body):
+    if not os.path.exists(HIPCC):
+        pytest.skip("no hipcc")
+    src, exe = str(tmp_path / "limits.hip"), str(tmp_path / "limits")
+    with open(src, "w") as f:
+        f.write(HEAD + "int main() {" + body +
+                'std::printf("%d wrong\\n", bad); return bad != 0; }\n')
+    subprocess.run([HIPCC, "-O1", "-std=c++17", "--offload-host-only", "-I",
+                    os.path.join(ROOT, "include"), "-I", os.path.join(PKG, "csrc"), src,
+                    "-L" + PKG, "-l:libq3h.so", "-Wl,-rpath," + PKG, "-o", exe], check=True)
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, r.stdout + r.stderr
+
+
+def test_forwards_without_allocations_fit(tmp_path, q3h):
+    """Every call of up to 64 rows on a stack whose attention leaves parts fits the
+    array at every length, a single row with all the parts that it asks for; the
+    parts end within the array and begin behind the other buffers."""
+    run(tmp_path, r"""
+  static char mem[1];
+  for (int fmt : {Q3H_KV_F32, Q3H_KV_Q8})
+    for (int head : {0, 2048, 4096}) {
+      q3h_stack s;
+      dims(s, fmt, 32768);
+      for (int rows = 1; rows <= Q3H_NOALLOC_MAX_ROWS; rows++) {
+        q3h::Work none;
+        const bool fits = q3h::work_carve(&s, rows, 0, head, 0, mem, Q3H_NOALLOC_SCRATCH_BYTES, none);
+        EXPECT(fits, "%d rows without parts", rows);
+        for (int len : {0, 100, 200, 390, 550, 1000, 3000, 10000, 32768 - rows}) {
+          const size_t want = q3h::tree_bytes(&s, 1, rows, len + rows);
+          q3h::Work w;
+          EXPECT(q3h::work_carve(&s, rows, 0, head, want, mem, Q3H_NOALLOC_SCRATCH_BYTES, w),
+                 "%d rows after %d, format %d, head %d", rows, len, fmt, head);
+          const char *at = (const char *)w.tree;
+          EXPECT(w.tree_bytes <= want && (rows > 1 || w.tree_bytes == want), "%d rows after %d: %zu of %zu",
+                 rows, len, w.tree_bytes, want);
+          EXPECT(w.tree_bytes == 0 || (at > (char *)w.gpart && at + w.tree_bytes <= mem + Q3H_NOALLOC_SCRATCH_BYTES &&
+                                       (at - mem) % 256 == 0), "%d rows after %d", rows, len);
+          EXPECT(want == 0 || w.tree_bytes > 0, "%d rows after %d: no parts", rows, len);
+        }
+      }
+    }
+""")

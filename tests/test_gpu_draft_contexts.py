@@ -113,3 +113,26 @@ def test_trees_and_rows_of_long_contexts(device, case):
         assert rel(lg[0], n.logits(n.forward(x[:1]))[0]) <= bar(case)
         assert rel(lg[1], m.logits(m.forward(x[1:]))[0]) <= bar(case)
     s.destroy(c, d)
+
+
+@pytest.mark.parametrize("case", ["int8", "yarn"])
+@pytest.mark.parametrize("positions", [700, 1500, 4000])
+def test_forwards_without_allocations_at_any_length(device, case, positions):
+    """Up to 64 rows in the device's array, whose room for the attention's parts
+    is less than they ask for: fewer parts, the results of q3h_forward_embeds but
+    for the order of sums."""
+    print(f"noalloc {case} {positions}", flush=True)
+    s = Setup(device, max_positions=4096, **CASES[case])
+    a, b, m = s.context(4096), s.context(4096), Model64(s)
+    for rows in (64, 48, 30, 17, 2):
+        for c in (a, b):
+            filled(s, c, [m] if c is a else [], positions)
+        assert rows == 2 or cut(device, s, rows, positions + rows)
+        x = rows_of(rows, rows)
+        la, na = a.forward(x, head=s.head, noalloc=True)
+        lb, nb = b.forward(x, head=s.head)
+        assert rel(la, lb) <= bar(case) and rel(na, nb) <= bar(case)
+        if rows in (64, 2):
+            want = m.forward(x)
+            assert rel(la, m.logits(want)[-1]) <= bar(case)
+    s.destroy(a, b)
