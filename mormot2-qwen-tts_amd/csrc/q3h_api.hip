@@ -93,7 +93,7 @@ void Work::ensure(const q3h_stack *s, int rows, int splits, int head_rows) {
   rows = std::max(rows, rows_cap);
   splits = std::max(splits, splits_cap);
   head_rows = std::max(head_rows, head_cap);
-  release();
+  release_rows();
   work_fields(s, rows, splits, head_rows, *this,
               [](void **slot, size_t bytes) { *slot = dev_alloc(bytes); });
   rows_cap = rows;  // (only now: after a failed allocation the next call starts anew)
@@ -102,14 +102,15 @@ void Work::ensure(const q3h_stack *s, int rows, int splits, int head_rows) {
   gen++;
 }
 
-void Work::ensure_tree(size_t bytes) {
+void Work::ensure_tree(size_t bytes, size_t most, bool captured) {
   if (bytes <= tree_bytes) return;
+  bytes = std::max(bytes, most);
   dev_free(tree);
   tree = nullptr;
   tree_bytes = 0;
+  if (captured) gen++;
   tree = (float *)dev_alloc(bytes);
   tree_bytes = bytes;
-  gen++;
 }
 
 bool work_carve(const q3h_stack *s, int rows, int splits, int head_rows, size_t tree_bytes,
@@ -133,6 +134,13 @@ bool work_carve(const q3h_stack *s, int rows, int splits, int head_rows, size_t 
 }
 
 void Work::release() {
+  release_rows();
+  dev_free(tree);
+  tree = nullptr;
+  tree_bytes = 0;
+}
+
+void Work::release_rows() {
   dev_free(h);
   dev_free(qkv);
   dev_free(att);
@@ -145,9 +153,6 @@ void Work::release() {
   dev_free(xa.q);
   dev_free(xb.q);
   dev_free(gpart);
-  dev_free(tree);
-  tree = nullptr;
-  tree_bytes = 0;
   x3n = x3a = nullptr;
   xa = QAct{};
   xb = QAct{};
@@ -1308,6 +1313,16 @@ int forward_splits(const q3h_context *c, int rows) {
   return attention_splits(c->s, forward_positions(c, rows));
 }
 
+// the parts of the attention over drafted rows for a forward of `rows` rows over
+// `positions` positions. A buffer that has to grow is made for the context's last
+// position: a context that fills up allocates once for each number of rows above
+// all before it, and keeps its graphs the rest of the time.
+void ensure_parts(q3h_context *c, int rows, int positions, bool drafted = false) {
+  const q3h_stack *s = c->s;
+  c->w.ensure_tree(tree_bytes(s, 1, rows, positions, drafted),
+                   tree_bytes(s, 1, rows, c->max_pos, drafted), s->ext);
+}
+
 // the kernels of a forward: descriptors, layers, head (or final norm), the
 // device length
 void enqueue_forward(q3h_context *c, Work &w, int rows, int positions, int head,
@@ -1475,7 +1490,7 @@ extern "C" int q3h_forward_embeds(q3h_context *c, const float *x, int rows, int 
     check_hip(hipSetDevice(s->dev->ordinal), "hipSetDevice");
     const int head_rows = head >= 0 ? s->heads[head].N : 0;
     c->w.ensure(s, rows, forward_splits(c, rows), head_rows);
-    c->w.ensure_tree(tree_bytes(s, 1, rows, forward_positions(c, rows)));
+    ensure_parts(c, rows, forward_positions(c, rows));
     // one row (a decode step): the forward replayed from a captured graph; a
     // prompt's results through pinned memory where the context has it, or from
     // its second prompt on (the first does not pay for the allocation)
@@ -1494,7 +1509,7 @@ extern "C" int q3h_forward_embeds_probe(q3h_context *c, const float *x, int rows
     check_hip(hipSetDevice(s->dev->ordinal), "hipSetDevice");
     const int head_rows = head >= 0 ? s->heads[head].N : 0;
     c->w.ensure(s, rows, forward_splits(c, rows), head_rows);
-    c->w.ensure_tree(tree_bytes(s, 1, rows, forward_positions(c, rows)));
+    ensure_parts(c, rows, forward_positions(c, rows));
     forward_rows(c, c->w, x, rows, head, logits, normed_last, layer_out, false, normed_rows);
   });
 }
@@ -1669,7 +1684,7 @@ void forward_all_rows(q3h_context *c, const float *x, int rows, const int32_t *p
   const int positions = parents ? c->len + rows : forward_positions(c, rows);
   Work &w = c->w;
   w.ensure(s, rows, parents ? 0 : forward_splits(c, rows), V);
-  w.ensure_tree(tree_bytes(s, 1, rows, positions, parents != nullptr));
+  ensure_parts(c, rows, positions, parents != nullptr);
   // the call's device memory: parents; tokens, scores, their workspace
   size_t need = 0;
   auto take = [&](size_t bytes) {

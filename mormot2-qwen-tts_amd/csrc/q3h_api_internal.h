@@ -180,9 +180,14 @@ struct Work {
   float *tree = nullptr;
   size_t tree_bytes = 0;
   bool carved = false;  // by work_carve, with what room there was for the parts
-  void ensure_tree(size_t bytes);
+  // at least `bytes` of tree, made `most` large when it grows (0: bytes); captured:
+  // whether graphs may hold it (a tree of drafted rows is never captured)
+  void ensure_tree(size_t bytes, size_t most = 0, bool captured = true);
   void ensure(const struct ::q3h_stack *s, int rows, int splits, int head_rows);
   void release();
+
+ private:
+  void release_rows();  // all but tree
 };
 
 // w's buffers for (rows, splits, head_rows) carved from [base, base + cap),

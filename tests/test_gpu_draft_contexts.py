@@ -5,6 +5,7 @@ import gc
 
 import numpy as np
 import pytest
+import torch
 
 import draft_ref as ref
 import q3h
@@ -136,3 +137,27 @@ def test_forwards_without_allocations_at_any_length(device, case, positions):
             want = m.forward(x)
             assert rel(la, m.logits(want)[-1]) <= bar(case)
     s.destroy(a, b)
+
+
+@pytest.mark.parametrize("case", ["f32", "int8"])
+def test_trees_of_a_growing_context_allocate_once(device, case):
+    """The parts of a tree's attention: room for those of the context's last
+    position from the first tree that leaves any."""
+    print(f"growing {case}", flush=True)
+    s = Setup(device, max_positions=4096, **CASES[case])
+    c = s.context(4096)
+    x, parents = rows_of(5, 64), drafted_tree(64, 5)
+    # (the other buffers at their largest: 64 rows, a single row's splits at the end)
+    c.forward_tree(x, parents, head=s.head)
+    filled(s, c, [], 4095)
+    c.forward(x[:1], head=s.head)
+    free = []
+    for n in (700, 900, 1300, 2100, 3000, 4000):
+        filled(s, c, [], n)
+        c.forward_tree(x, parents, head=s.head)
+        c.keep([0])
+        c.forward(x[:1], head=s.head)
+        torch.cuda.synchronize()
+        free.append(torch.cuda.mem_get_info()[0])
+    assert len(set(free)) == 1, free
+    s.destroy(c)
