@@ -176,6 +176,9 @@ size_t tree_bytes(const q3h_stack *s, int n, int rows, int positions, bool draft
   if (!s->ext && !drafted) return 0;
   // single rows: of any length (a captured launch serves many)
   if (rows == 1) positions = c.max_positions;
+  require(attend_fits(n, rows, c.heads, c.kv_heads, c.head_dim, c.kv_f16,
+                      std::max(0, positions - rows)),
+          Q3H_E_CAPACITY, "too many rows, heads and positions for one attention");
   return attend_part_bytes(n, rows, c.heads, c.kv_heads, c.head_dim, c.kv_f16, positions);
 }
 

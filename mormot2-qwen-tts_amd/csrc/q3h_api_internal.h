@@ -198,7 +198,8 @@ bool work_carve(const struct ::q3h_stack *s, int rows, int splits, int head_rows
                 size_t tree_bytes, void *base, size_t cap, Work &w);
 // the bytes of Work::tree for a forward of n contexts, rows rows each, over up to
 // `positions` positions: those of stacks whose every attention is that over
-// drafted rows, or of a drafted tree
+// drafted rows, or of a drafted tree (Q3H_E_CAPACITY where that attention's counts
+// leave 32 bits: what sizes the buffer comes before what is launched)
 size_t tree_bytes(const struct ::q3h_stack *s, int n, int rows, int positions, bool drafted = false);
 
 // attention splits (the partial buffer) for contexts of up to `positions`

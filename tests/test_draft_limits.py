@@ -83,3 +83,30 @@ def test_forwards_without_allocations_fit(tmp_path, q3h):
       }
     }
 """)
+
+
+def test_counts_of_a_forward_beyond_32_bits_are_refused(tmp_path, q3h):
+    """Where a forward's buffers are sized, as q3h_cache_attend refuses its own; the
+    largest that a stack of 32 heads over 8 takes is not refused."""
+    run(tmp_path, r"""
+  auto code = [](const q3h_stack &s, int n, int rows, int positions, bool drafted) {
+    try {
+      q3h::tree_bytes(&s, n, rows, positions, drafted);
+    } catch (const q3h::Error &e) {
+      return e.code;
+    }
+    return 0;
+  };
+  q3h_stack s;
+  dims(s, Q3H_KV_Q8, 65536);
+  s.cfg.heads = 32;
+  EXPECT(code(s, 1, 65536, 65536, false) == 0, "a prompt of all positions");
+  EXPECT(code(s, 256, 1, 65536, false) == 0, "a batch");
+  s.cfg.heads = 4096, s.cfg.kv_heads = 1024;
+  EXPECT(code(s, 1, 65536, 65536, false) == Q3H_E_CAPACITY, "a prompt over 1024 heads");
+  EXPECT(code(s, 65536, 1, 65536, false) == Q3H_E_CAPACITY, "a batch over 1024 heads");
+  s.ext = false;
+  s.cfg.kv_f16 = Q3H_KV_F16;
+  EXPECT(code(s, 65536, 64, 65536, true) == Q3H_E_CAPACITY, "trees");
+  EXPECT(code(s, 65536, 64, 65536, false) == 0, "no attention over drafted rows");
+""")
