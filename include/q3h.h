@@ -534,7 +534,8 @@ int q3h_cache_keep(q3h_cache *c, int sequences, int rows, const int32_t *lens,
                    const int32_t *kept, const int32_t *kept_counts, void *stream);
 
 /* Scores of rows of logits [rows][vocab] (dtype Q3H_F32 or Q3H_BF16, rows ld
-   elements apart, at most 2^20 tokens), computed in f32 from one read of them:
+   elements apart, at most 2^20 tokens; fewer than 2^24 rows, of more than 10233
+   tokens each 10240 of them count as one), computed in f32 from one read of them:
    with lse = log sum exp of a row,
    - logprobs [rows][tokens_per_row]: logit - lse of the given tokens (tokens
      [rows][tokens_per_row]; a token outside [0, vocab): NaN);

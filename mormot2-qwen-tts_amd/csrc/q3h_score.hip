@@ -330,6 +330,10 @@ int score_splits(int vocab) {
   const int per = kThreads * score_width(vocab);
   return (vocab + 7 + per - 1) / per;
 }
+// a launch has fewer than 2^32 threads
+bool score_fits(int rows, int vocab) {
+  return (int64_t)rows * score_splits(vocab) * kThreads < (int64_t)1 << 32;
+}
 static_assert((kMaxVocab + 7 + kThreads * 40 - 1) / (kThreads * 40) * Q3H_TOP_MAX <=
                   kMergeKeys * kThreads,
               "the merge holds every split's keys");
@@ -378,6 +382,8 @@ extern "C" int64_t q3h_token_logprobs_workspace(int rows, int vocab, int top_k) 
   const int rc = guard([&] {
     require(rows >= 0 && vocab > 0 && vocab <= kMaxVocab && top_k >= 0 && top_k <= Q3H_TOP_MAX && top_k <= vocab,
             Q3H_E_ARG, "q3h_token_logprobs_workspace: invalid argument");
+    require(score_fits(rows, vocab), Q3H_E_CAPACITY,
+            "q3h_token_logprobs_workspace: too many rows");
     if (rows > 0) bytes = (int64_t)score_work_bytes(rows, vocab, top_k);
   });
   return rc ? rc : bytes;
@@ -397,8 +403,7 @@ extern "C" int q3h_token_logprobs(q3h_device *dev, const q3h_score_args *p, void
     require(p->logits != nullptr, Q3H_E_ARG, "q3h_token_logprobs: NULL logits");
     require((uintptr_t)p->logits % (p->dtype == Q3H_BF16 ? 2 : 4) == 0, Q3H_E_ARG,
             "q3h_token_logprobs: logits between elements");
-    require((int64_t)p->rows * 128 <= INT32_MAX, Q3H_E_CAPACITY,
-            "q3h_token_logprobs: too many rows");
+    require(score_fits(p->rows, p->vocab), Q3H_E_CAPACITY, "q3h_token_logprobs: too many rows");
     require(p->ld >= p->vocab, Q3H_E_ARG, "q3h_token_logprobs: rows overlap (ld below vocab)");
     require(p->tokens_per_row == 0 || (p->tokens && p->logprobs), Q3H_E_ARG,
             "q3h_token_logprobs: NULL tokens or logprobs");

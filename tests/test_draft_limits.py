@@ -110,3 +110,28 @@ def test_counts_of_a_forward_beyond_32_bits_are_refused(tmp_path, q3h):
   EXPECT(code(s, 65536, 64, 65536, true) == Q3H_E_CAPACITY, "trees");
   EXPECT(code(s, 65536, 64, 65536, false) == 0, "no attention over drafted rows");
 """)
+
+
+def test_scores_of_more_rows_than_a_launch_takes_are_refused(tmp_path, q3h):
+    """2^24 workgroups, several for each row of a large vocabulary."""
+    run(tmp_path, r"""
+  q3h_device dev;
+  dev.ordinal = 0;
+  alignas(256) static float mem[64];
+  static int32_t ints[1];
+  for (int vocab : {100, 10234, 151936, 1 << 20}) {
+    const int per_row = vocab + 7 <= 10240 ? 1 : (vocab + 7 + 10239) / 10240;
+    for (int rows : {((1 << 24) + per_row - 1) / per_row, 1 << 24, 2147483647}) {
+      q3h_score_args a{};
+      a.logits = mem, a.ld = vocab, a.dtype = Q3H_BF16, a.rows = rows, a.vocab = vocab;
+      a.tokens_per_row = 1, a.tokens = ints, a.logprobs = mem;
+      a.workspace = mem, a.workspace_bytes = INT64_MAX;
+      const int rc = q3h_token_logprobs(&dev, &a, nullptr);
+      EXPECT(rc == Q3H_E_CAPACITY, "%d rows of %d: %d (%s)", rows, vocab, rc, q3h_last_error());
+      const long long need = q3h_token_logprobs_workspace(rows, vocab, 0);
+      EXPECT(need == Q3H_E_CAPACITY, "workspace of %d rows of %d: %lld", rows, vocab, need);
+    }
+    const int most = ((1 << 24) - 1) / per_row;
+    EXPECT(q3h_token_logprobs_workspace(most, vocab, 0) >= 0, "workspace of %d rows of %d", most, vocab);
+  }
+""")
