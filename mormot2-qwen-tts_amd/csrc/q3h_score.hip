@@ -102,8 +102,12 @@ __device__ __forceinline__ void block_top(TopSpace &sm, uint64_t *list, int k, K
 
 // The same for logits x(e), first by their values alone: the largest value that k
 // of the 64 groups reach bounds the row's k-th from below, one comparison a logit.
-// Where that leaves more than `list` holds (many logits alike) or bounds nothing
-// (NaN, -infinity), by whole keys. best: the thread's largest logit.
+// Where that leaves more than kShortList (many logits alike: a row of one value, or
+// masked with a finite one down to fewer than k tokens) or bounds nothing (NaN,
+// -infinity), by whole keys, which leave a few hundred of logits alike: ranks are
+// counted for each key against all, 16.3 ms instead of 59 us for the top 64 of 40 rows
+// of 151936 logits alike. best: the thread's largest logit.
+constexpr int kShortList = 1024;
 template <int E, class Logit, class Key, class Emit>
 __device__ __forceinline__ void block_top_logits(TopSpace &sm, uint64_t *list, int k, float best,
                                                  Logit &&x, Key &&key, Emit &&emit) {
@@ -123,13 +127,14 @@ __device__ __forceinline__ void block_top_logits(TopSpace &sm, uint64_t *list, i
   }
   __syncthreads();
   const float bound = sm.value;
+  const int room = min(4 * k * E, kShortList);
   if (bound > -INFINITY) {
     if (best >= bound) {
       int n = 0;
 #pragma unroll
       for (int e = 0; e < E; e++) n += x(e) >= bound;
       int at = atomicAdd(&sm.n, n);
-      if (at + n <= 4 * k * E) {
+      if (at + n <= room) {
 #pragma unroll
         for (int e = 0; e < E; e++)
           if (x(e) >= bound) list[at++] = key(e);
@@ -137,7 +142,7 @@ __device__ __forceinline__ void block_top_logits(TopSpace &sm, uint64_t *list, i
     }
     __syncthreads();
     const int n = sm.n;
-    if (n <= 4 * k * E) {
+    if (n <= room) {
       rank_list(list, n, k, emit);
       return;
     }
