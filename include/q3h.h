@@ -56,7 +56,9 @@ typedef struct {
   int32_t kv_f16;        /* K/V cache in half floats (lm.pas:128-130): 0 or 1; or
                             Q3H_KV_Q8 (2; no reference counterpart): a byte per
                             element and a scale per position and head, f32
-                            activations only */
+                            activations only. Other values are refused; before
+                            there were int8 caches any value but 0, such as a
+                            truth value of -1, chose half floats */
   int32_t act_q8;        /* Q8_0 only: 1 = activations quantized per 32-block
                             (int8 products, ggml vec_dot_q8_0_q8_0); 0 = f32
                             activations times dequantized weights */
