@@ -599,7 +599,8 @@ int q3h_forward_tree(q3h_context *c, const float *x, int rows, const int32_t *pa
 int q3h_context_keep(q3h_context *c, const int32_t *kept, int n);
 /* q3h_forward_embeds of rows whose every position is scored, the logits (of
    every row, nullable) staying on the device otherwise; normed [rows][hidden]
-   nullable. Any stack. */
+   nullable. Any stack. As in every forward with a head, the context's buffers hold
+   rows x head rows logits (f32) from then on. */
 int q3h_forward_score(q3h_context *c, const float *x, int rows, int head,
                       const q3h_row_scores *scores, float *logits, float *normed);
 

@@ -66,7 +66,8 @@ __device__ __forceinline__ int byte_of(float x, float d, double inv) {
 // d = fl32(max |y| / 127), byte = rint(y / d).
 //
 // Memory bound over many rows: 3576 rows of 32 + 2 x 8 heads of 128 to f16, 161 MB
-// read and written, 32 us (5.0 TB/s; eight neighbours a lane, half of a line an
+// read and written, 32 us (5.0 TB/s; turning 20 of the 128 elements, ODD, three times
+// that; eight neighbours a lane, half of a line an
 // instruction, 38; a pair a lane, a head over a whole wave, 60: the 64-bit sums of
 // each head made that VALU bound). One row: 3.6 us, 496 rows of 16 + 2 x 8 heads to
 // int8 7.4 us, which are a launch, the path through the parents and three loads that
@@ -371,6 +372,9 @@ __global__ __launch_bounds__(kThreads) void k_cache_read(KvView kv, const int32_
   }
 }
 
+// 32 sequences of 28 layers of 8 heads of 128, paths of 8 rows: f32 117 MB 29 us
+// (4.1 TB/s), f16 26, int8 29; paths of 32 rows 179, 127 and 113 us; one sequence and
+// a path of 8 5 us, of 32 12-16: bound by a trip to memory a row, one after another.
 // One workgroup per (sequence, layer, kv head, keys or values): the kept rows
 // in ascending order, each to a position at or before its own that no later
 // row comes from, so one row after another is enough; a 4-byte word of a row a

@@ -25,20 +25,20 @@
 // - one row over 171 positions of an f16 cache, 8 workgroups of 2 tiles a wave:
 //   6.8 us, a launch and the round trips of one workgroup (lengths, rows, the waves'
 //   meeting); f32: k_attend_few;
-// - 32 sequences of one row, 41000 positions of int8 in all, 87 MB: 23.5-25 us + 4.5
+// - 32 sequences of one row, 41000 positions of int8 in all, 87 MB: 25-26 us + 4.8
 //   for the parts, 432 shares of 8 steps, where a workgroup takes 10 us to find its
 //   share, have its first tiles and join its waves, and 1.45 a step; the same in f16
 //   168 MB 44 us, in f32 335 MB 77.6 us (4.3 TB/s). Three workgroups a CU at 168
 //   registers (27 us of 23.5), two tiles ahead (29.8 us of 29.1) and loads past the
 //   caches (31.2 of 29.3) were slower;
 // - a tree of 27 rows over 12289 positions of f16, 51 MB: 22 us + 5.2, 224 shares of 7;
-// - 12 trees, 420 rows, 32 query heads over 8, 60000 positions of int8, 141 MB: 118-129
-//   us + 11.4, where VALU (300 instructions a wave and tile, 16 scores a lane taking 9
+// - 12 trees, 420 rows, 32 query heads over 8, 60000 positions of int8, 141 MB: 130-136
+//   us + 11.4 by the box, where VALU (300 instructions a wave and tile, 16 scores a lane taking 9
 //   each) and matrix instructions (64) take turns more than they overlap: 69 % and
-//   34 % of the time. 270 TFLOP/s of the definition's operations, twice that in
+//   34 % of the time. 260 TFLOP/s of the definition's operations, twice that in
 //   products;
-// - 2 prompts of 1500 rows over 500 positions, 16 heads over 8: f16 101 us, int8 112,
-//   f32 234 (131 of the 154 TFLOP/s of a large f32 product).
+// - 2 prompts of 1500 rows over 500 positions, 16 heads over 8: f16 102 us, int8 114,
+//   f32 235 (131 of the 154 TFLOP/s of a large f32 product).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -146,7 +146,8 @@ __device__ __forceinline__ Head head_of(const AttendRows &a, const KvSeq &s, con
 // join has twice the parts otherwise and some of the CUs a second share: one row
 // over 8000 positions of 8 heads 15.4 us, with two 17.3; a tree of 27 over 12289
 // (1544 steps) 26.5 and 29.8; but four rows, 20000 positions in all (1250 steps, 32
-// groups) 20.0 and 18.6, four trees 33 and 29.4.
+// groups) 20.0 and 18.6, four trees 33 and 29.4. (The bound at 16 groups lies between
+// what was measured; nothing sets it closer.)
 constexpr int kWholeSteps = 6, kWorkers = 512;
 __device__ __forceinline__ int share_steps(uint32_t groups, uint32_t steps, uint32_t workers) {
   const uint32_t w = steps <= workers / 2 * (groups < 16 ? 7 : 4) ? workers / 2 : workers;
@@ -1194,7 +1195,8 @@ Shape shape_of(int sequences, int rows, int heads, int kvh, int hd, int max_len,
   const int wk = kWaves / waves;
   const int64_t steps = ((max_len + rows + tile - 1) / tile + wk - 1) / wk;
   // Up to six steps no group is cut: parts cost a second launch, 4 us (one row over
-  // 640 positions of f16: 11.1 us whole, 12.5 cut; 900: 14.4 and 11.9). Beyond, the
+  // 640 positions of f16: 11.1 us whole, 12.5 cut; 900: 14.4 and 11.9; the other formats
+  // take the same number, f32 with half the positions a step). Beyond, the
   // more workgroups the better, down to one step each (8000 positions: 18.5 us with
   // six steps at least, 15.4 with one or two).
   for (int w = steps > kWholeSteps ? kWorkers : 0; w > 0; w -= kWorkers / 16) {
