@@ -171,7 +171,7 @@ type
     scale: single;
     q: PSingle;
     ldq: Int64;
-    out: PSingle;
+    out: PSingle;  // the C field's name; where a mode reserves the word, write &out
     ld_out: Int64;
     lens, counts, parents: PInteger;
     workspace: pointer;
