@@ -80,11 +80,12 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // workgroup each, so that long and short sequences, full and small groups end
 // together; the shares of a group that has several leave parts, which a second
 // kernel joins. shares: of a short call no group is cut; blocks: workgroups, of
-// shares those that they may come to; parts: that they may leave.
+// shares those that they may come to; parts: that they may leave; workers: how many
+// shares of much work there are, about: kWorkers, fewer where the parts of so many
+// have no room.
 struct Shape {
-  int nq, group, blocks, parts;
-  int shares;  // about how many a call of much work has: kWorkers, fewer where the
-               // parts of so many have no room; 0: no group is cut
+  int nq, group, blocks, parts, workers;
+  bool shares;
   int per_kv;       // query heads of a kv head
   uint32_t by_kv;   // ceil(2^32 / per_kv)
   // x / per_kv (attend_fits: x * per_kv < 2^32)
@@ -281,7 +282,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
       groups += __builtin_amdgcn_readlane(lane_sums(h.groups), 63) * a.kv.kvh;
       steps += __builtin_amdgcn_readlane(lane_sums(h.steps), 63) * a.kv.kvh;
     }
-    const int most = share_steps(groups, steps, shape.shares), worker = blockIdx.x;
+    const int most = share_steps(groups, steps, shape.workers), worker = blockIdx.x;
     int sum = 0, sum_parts = 0, at = 0, shares = 1, head_parts = 0;
     b = -1;
     for (int base = 0; base < n && (b < 0 || worker == 0); base += 64) {
@@ -1199,9 +1200,10 @@ Shape shape_of(int sequences, int rows, int heads, int kvh, int hd, int max_len,
   // take the same number, f32 with half the positions a step). Beyond, the
   // more workgroups the better, down to one step each (8000 positions: 18.5 us with
   // six steps at least, 15.4 with one or two).
-  for (int w = steps > kWholeSteps ? kWorkers : 0; w > 0; w -= kWorkers / 16) {
+  s.shares = steps > kWholeSteps;
+  for (int w = s.workers = kWorkers; s.shares && w > 0; w -= kWorkers / 16) {
     const int64_t n = std::max<int64_t>(w - groups / 2, w / 2);
-    s.shares = w;
+    s.workers = w;
     s.blocks = (int)std::min(n + groups, groups * steps);
     // n shares of whole steps and one more a group, or twice n: the most of any number
     // of groups up to these is at a third of 2 w
@@ -1209,7 +1211,7 @@ Shape shape_of(int sequences, int rows, int heads, int kvh, int hd, int max_len,
     if (parts_bytes(s, sequences, hd) <= room) return s;
   }
   // short, or no room for the parts of any cut: whole groups
-  s.shares = 0;
+  s.shares = false;
   s.blocks = (int)groups;
   s.parts = 0;
   return s;
