@@ -84,10 +84,11 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // shares of much work there are, about: kWorkers, fewer where the parts of so many
 // have no room.
 struct Shape {
-  int nq, group, blocks, parts, workers;
+  int nq, group, blocks, parts;
   bool shares;
   int per_kv;       // query heads of a kv head
   uint32_t by_kv;   // ceil(2^32 / per_kv)
+  int workers;
   // x / per_kv (attend_fits: x * per_kv < 2^32)
   __device__ __forceinline__ int drafted(int x) const {
     return per_kv == 1 ? x : (int)__umulhi((uint32_t)x, by_kv);
