@@ -421,6 +421,14 @@ int q3h_codec_destroy(q3h_codec *c);
    max |x| / 127 rounded to f32, byte = x / scale rounded to even, both from 64
    bits. A row with an infinity or NaN reads as NaN. */
 #define Q3H_KV_Q8 2
+/* four bits per element, a step (a byte) per 32 of them and one f32 scale per position
+   and kv head: scale = max |x| / 1785 rounded to f32 (1785 = 7 * 255), step = max |x| of
+   the 32 / (7 scale) rounded up (255 at most), element = x / (step * scale) rounded to
+   even within -7 .. 7, from 64 bits; it stands for element * step * scale. An element is
+   off by at most 1/14 of the largest of its 32 and 1/3570 of the row's largest. A
+   position takes head_dim / 2 + 8 bytes a kv head. A row with an infinity or NaN reads as
+   NaN. */
+#define Q3H_KV_Q4 4
 #define Q3H_TREE_MAX_ROWS 64
 #define Q3H_TOP_MAX 64
 
@@ -456,17 +464,37 @@ typedef struct {
                       factor above 1, else 1 */
 } q3h_rope_config;
 int q3h_rope_create(q3h_device *dev, const q3h_rope_config *cfg, q3h_rope **out);
+/* a table whose pairs turn by positions of several axes (time, height and width of a
+   picture's patches), 1 to 4: pair i by that of axis pair_axes[i], pair_axes
+   [rot_dim / 2] in host memory. Rows get their positions in q3h_cache_append_at; in
+   q3h_cache_append all axes have the row's own. */
+int q3h_rope_create_axes(q3h_device *dev, const q3h_rope_config *cfg, int axes,
+                         const int32_t *pair_axes, q3h_rope **out);
 int q3h_rope_destroy(q3h_rope *r);
 
 /* a K/V cache of several sequences: per sequence keys, then values
    [layers][kv_heads][max_positions][head_dim] in the format (Q3H_KV_*), the
-   layout of a context's cache, then for Q3H_KV_Q8 the scales of the keys and
-   of the values [layers][kv_heads][max_positions]; zeros at first */
+   layout of a context's cache, then for Q3H_KV_Q8 and Q3H_KV_Q4 the scales of the keys and
+   of the values [layers][kv_heads][max_positions], then for Q3H_KV_Q4 their steps, four
+   bytes each; zeros at first */
 typedef struct {
   int32_t sequences, layers, kv_heads, head_dim; /* head_dim 64 or 128 */
   int32_t max_positions, format;
 } q3h_cache_config;
 int q3h_cache_create(q3h_device *dev, const q3h_cache_config *cfg, q3h_cache **out);
+/* a cache whose sequences are made of pages: max_positions of each sequence at most, in
+   `pages` pages of page_positions positions (all layers, keys and values) that sequences
+   take and may share. Which pages a sequence has is kept on the device; all calls on
+   caches take it as any other, a sequence's positions being those that its pages reach
+   (none at first), and rows that would go to a page that another sequence holds too
+   get NaN queries and are not written. */
+#define Q3H_MAX_PAGES (1 << 20)
+typedef struct {
+  q3h_cache_config cache; /* of all sequences up to 2^24 pages, if all were full */
+  int32_t pages;          /* 1 .. Q3H_MAX_PAGES */
+  int32_t page_positions; /* 32, 64, 128 or 256 */
+} q3h_paged_config;
+int q3h_cache_create_paged(q3h_device *dev, const q3h_paged_config *cfg, q3h_cache **out);
 int64_t q3h_cache_bytes(const q3h_cache *c);
 int q3h_cache_destroy(q3h_cache *c);
 
@@ -491,6 +519,13 @@ typedef struct {
   const int32_t *lens, *counts, *parents;
 } q3h_append_args;
 int q3h_cache_append(q3h_cache *c, const q3h_append_args *a, void *stream);
+
+/* q3h_cache_append with positions [axes of the rope][sequences][rows] (device memory) of
+   the rows in place of lens[b] plus depth, which the angles are taken from; the rope is
+   needed. A row with a position outside the rope's table gets NaN queries and is not
+   written. Where the rows go in the cache stays as it is. */
+int q3h_cache_append_at(q3h_cache *c, const q3h_append_args *a, const int32_t *positions,
+                        void *stream);
 
 /* positions starts[b] .. + counts[b] - 1 of a layer (starts nullable: 0) as
    the f32 values that the cache holds: k and v (either nullable)
@@ -534,6 +569,50 @@ int q3h_cache_attend(q3h_cache *c, const q3h_attend_args *a, void *stream);
    kept_counts. A list that is not of that form leaves its sequence as it is. */
 int q3h_cache_keep(q3h_cache *c, int sequences, int rows, const int32_t *lens,
                    const int32_t *kept, const int32_t *kept_counts, void *stream);
+
+/* The pages of a cache of q3h_cache_create_paged, for its first `sequences` sequences. Like
+   the operators above these calls only enqueue kernels, on any stream, and can be
+   captured; but they change what the cache's other calls read, and share scratch memory
+   of the cache: of one cache they run one after another, and not beside a call on
+   its rows. Pages are taken from the lowest free one up, for the sequences in their
+   order, so that the same calls leave the same tables. What only the device holds and is
+   out of range (a negative length, a length beyond a sequence's pages or positions, no
+   such source) leaves its sequence as it is.
+
+   reserve: room for rows to come: sequence b gets the pages that positions lens[b] ..
+   lens[b] + counts[b] - 1 (counts nullable: rows; taken into [0, rows]) lie in and it
+   does not have; lens[b] at most the positions that its pages reach. Pages of that range
+   that other sequences hold too are replaced by its own, the positions before lens[b]
+   copied; if all that hold such a page write to it in this call, the first of them keeps
+   it. ok [sequences] (nullable): 1 where a sequence has all those pages, to itself; 0
+   where there were too few (then it, and the ones behind it that want some, get
+   none) or its arguments are out of range. */
+int q3h_cache_reserve(q3h_cache *c, int sequences, int rows, const int32_t *lens,
+                      const int32_t *counts, int32_t *ok, void *stream);
+/* fork: sequence b becomes the first lens[b] positions of what sequence sources[b] of the
+   cache was before the call (-1: nothing), for all b at once, so that sources may be any
+   assignment (beams that are continued, dropped, reordered). Pages are shared, nothing is
+   copied; what b held before and no sequence holds any more is free. */
+int q3h_cache_fork(q3h_cache *c, int sequences, const int32_t *sources, const int32_t *lens,
+                   void *stream);
+/* release: sequence b keeps the pages that its first lens[b] positions lie in (0: none) */
+int q3h_cache_release(q3h_cache *c, int sequences, const int32_t *lens, void *stream);
+/* compact: the pages in use become pages 0 .. *used - 1 (used: device memory, nullable),
+   with what they hold: those behind that number go, in their order, to the free ones
+   below it, in theirs. */
+int q3h_cache_compact(q3h_cache *c, int32_t *used, void *stream);
+/* copy: positions 0 .. lens[b] - 1 of every layer of sequence sources[b] of src (-1: none)
+   to sequence b of c. Two caches of one device, format, layers, kv heads and head_dim,
+   each in pages or not (a sequence moved out and back, a prompt computed elsewhere);
+   sequence b has the positions already. Pages of c that other sequences hold too stay as
+   they are. */
+int q3h_cache_copy(q3h_cache *c, const q3h_cache *src, int sequences, const int32_t *sources,
+                   const int32_t *lens, void *stream);
+/* the tables as they are, each nullable: table [sequences of the cache]
+   [ceil(max_positions / page_positions)] (-1: no page), counts [sequences] of pages that a
+   sequence holds, refs [pages] of sequences that hold a page */
+int q3h_cache_page_state(const q3h_cache *c, int32_t *table, int32_t *counts, int32_t *refs,
+                         void *stream);
 
 /* Scores of rows of logits [rows][vocab] (dtype Q3H_F32 or Q3H_BF16, rows ld
    elements apart, at most 2^20 tokens; fewer than 2^24 rows, of more than 10233

@@ -860,9 +860,9 @@ extern "C" int q3h_stack_create(q3h_device *dev, const q3h_stack_config *cfg,
     require(c.dtype == Q3H_Q8_0 || w->src_dtype != Q3H_Q8_0, Q3H_E_ARG,
             "q3h_stack_create: an f32 stack takes f32 or BF16 weights");
     require(c.max_positions > 0, Q3H_E_ARG, "q3h_stack_create: max_positions <= 0");
-    require(c.kv_f16 >= Q3H_KV_F32 && c.kv_f16 <= Q3H_KV_Q8, Q3H_E_ARG,
-            "q3h_stack_create: kv_f16 must be Q3H_KV_F32, Q3H_KV_F16 or Q3H_KV_Q8");
-    require(c.kv_f16 != Q3H_KV_Q8 || !c.act_q8, Q3H_E_ARG,
+    require(kv_format(c.kv_f16), Q3H_E_ARG,
+            "q3h_stack_create: kv_f16 must be Q3H_KV_F32, Q3H_KV_F16, Q3H_KV_Q8 or Q3H_KV_Q4");
+    require(!kv_scaled(c.kv_f16) || !c.act_q8, Q3H_E_ARG,
             "q3h_stack_create: act_q8 takes an f32 or f16 cache");
     const int most = attn_max_positions(c.kv_f16 != Q3H_KV_F32);
     require(c.max_positions <= most, Q3H_E_ARG,
@@ -887,7 +887,7 @@ extern "C" int q3h_stack_create(q3h_device *dev, const q3h_stack_config *cfg,
     s = new q3h_stack();
     s->dev = dev;
     s->cfg = c;
-    s->ext = c.kv_f16 == Q3H_KV_Q8;
+    s->ext = kv_scaled(c.kv_f16);
     check_hip(hipStreamCreateWithFlags(&s->stream, hipStreamNonBlocking), "hipStreamCreate");
     const int H = c.hidden, hd = c.head_dim, NQ = c.heads * hd, NKV = c.kv_heads * hd;
     const int I = c.intermediate;
@@ -1054,12 +1054,11 @@ q3h_context *new_context(q3h_stack *s, int max_positions) {
   ctx->max_pos = max_positions;
   try {
     check_hip(hipStreamCreateWithFlags(&ctx->stream, hipStreamNonBlocking), "hipStreamCreate");
-    const size_t n = (size_t)c.layers * c.kv_heads * max_positions * c.head_dim;
-    const size_t esz = kv_elem_bytes(c.kv_f16);
+    const size_t rows = (size_t)c.layers * c.kv_heads * max_positions;
     const size_t bytes = kv_bytes(c.kv_f16, c.layers, c.kv_heads, max_positions, c.head_dim);
-    // keys then values in one allocation: v = k + n elements (int8: then the scales)
+    // keys then values in one allocation (int8 and 4 bits: then the scales)
     ctx->k = dev_alloc(bytes);
-    ctx->v = static_cast<char *>(ctx->k) + n * esz;
+    ctx->v = static_cast<char *>(ctx->k) + rows * kv_row_bytes(c.kv_f16, c.head_dim);
     // zeros: a position is finite before it is first written (the long-context
     // attention reads rows past the context with weight 0)
     check_hip(hipMemset(ctx->k, 0, bytes), "zero K/V");
@@ -1158,9 +1157,9 @@ extern "C" int q3h_context_fill_kv(q3h_context *c, const float *k, const float *
           check_hip(hipMemcpyAsync(st, which ? v : k, n * sizeof(float), hipMemcpyHostToDevice,
                                    c->stream),
                     "fill kv upload");
-          if (cf.kv_f16 == Q3H_KV_Q8)
-            launch_q8_fill(st, (char *)c->k, which, cf.layers, cf.kv_heads, len, cf.head_dim,
-                           c->max_pos, c->stream);
+          if (kv_scaled(cf.kv_f16))
+            launch_scaled_fill(st, (char *)c->k, which, cf.layers, cf.kv_heads, len, cf.head_dim,
+                               cf.kv_f16, c->max_pos, c->stream);
           else
             launch_kv_fill(st, cf.layers, cf.kv_heads, len, cf.head_dim, which ? c->v : c->k,
                            c->max_pos, cf.kv_f16 != 0, c->stream);
@@ -1188,9 +1187,9 @@ extern "C" int q3h_context_read_kv(q3h_context *c, int layer, float *k, float *v
     float *st = (float *)dev_alloc(n * sizeof(float));
     try {
       for (int which = 0; which < 2; which++) {
-        if (cf.kv_f16 == Q3H_KV_Q8)
-          launch_q8_read((const char *)c->k, which, cf.layers, layer, cf.kv_heads, c->len,
-                         cf.head_dim, c->max_pos, st, c->stream);
+        if (kv_scaled(cf.kv_f16))
+          launch_scaled_read((const char *)c->k, which, cf.layers, layer, cf.kv_heads, c->len,
+                             cf.head_dim, cf.kv_f16, c->max_pos, st, c->stream);
         else
           launch_kv_read(which ? c->v : c->k, layer, cf.kv_heads, c->len, cf.head_dim, c->max_pos,
                          cf.kv_f16 != 0, st, c->stream);

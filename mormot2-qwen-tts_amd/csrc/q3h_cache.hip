@@ -53,6 +53,20 @@ __device__ __forceinline__ int byte_of(float x, float d, double inv) {
   return min(127, max(-127, (int)q)) + 128;
 }
 
+// rint(x / d) within -7 .. 7, + 8: an element of the 4-bit format (d: its group's step
+// times the row's scale), the quotient as byte_of takes it
+__device__ __forceinline__ uint32_t nibble_of(float x, double d, double inv) {
+  const double y = (double)x * inv;
+  double q = rint(y);
+  if (fabs(y - q) > 0.5 - 1e-6) q = rint((double)x / d);
+  return (uint32_t)(min(7, max(-7, (int)q)) + 8);
+}
+// the step of a group whose largest is m in a row of scale d: the least whole number of d
+// that 7 of reach m (255 at most)
+__device__ __forceinline__ int step_of(float m, float d) {
+  return d > 0.f ? (int)fmin(255.0, ceil((double)m / (7.0 * (double)d))) : 0;
+}
+
 // One head of one row per HD / 8 lanes, twice four neighbours each, a and b, such
 // that a head's lanes together load and store whole lines: a[i] and b[i] of four
 // pairs that turn together (halves), four pairs of neighbours (interleaved), or
@@ -63,7 +77,9 @@ __device__ __forceinline__ int byte_of(float x, float d, double inv) {
 // four, element by element. Everything up to the f32 row is in 64 bits, so that a
 // byte of the int8 format is that of the definition and not of a rounding
 // before it: y = x / sqrt(sum x^2 / HD + eps) * w; (y0 c - y1 s, y1 c + y0 s);
-// d = fl32(max |y| / 127), byte = rint(y / d).
+// d = fl32(max |y| / 127), byte = rint(y / d); in 4 bits D = fl32(max |y| / 1785), of each
+// 32 elements s = ceil(max |y| / (7 D)), the element rint(y / (s D)): s D is whole steps of
+// D, so that 8 times a step is exact in f16 when it is read.
 //
 // Memory bound over many rows: 3576 rows of 32 + 2 x 8 heads of 128 to f16, 161 MB
 // read and written, 32 us (5.0 TB/s; turning 20 of the 128 elements, ODD, three times
@@ -77,6 +93,8 @@ template <int FMT, int HD, bool ODD, bool MANY>
 __global__ __launch_bounds__(kThreads) void k_cache_append(AppendRows a) {
   constexpr int G = HD / 8, SIDE = 64 / G;  // lanes of a head, heads side by side
   constexpr int PER = kHeads * SIDE;        // heads of a wave at a time
+  __shared__ uint8_t sm_row[FMT == Q3H_KV_Q4 && ODD ? kThreads / 64 : 1][PER]
+                           [FMT == Q3H_KV_Q4 && ODD ? HD : 1];
   const int lane = threadIdx.x & 63, sub = lane & (G - 1), side = lane / G;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int row = blockIdx.x, b = row / a.kv.rows, t = row - b * a.kv.rows;
@@ -84,6 +102,26 @@ __global__ __launch_bounds__(kThreads) void k_cache_append(AppendRows a) {
   if (t >= s.count) return;
   int depth = t;
   bool bad = s.len < 0 || s.len > s.max_pos - s.count;
+  // where the row goes; a page that another sequence holds too is not written to
+  int at_pos = s.len + t;
+  KvSeq place = s;
+  if (a.kv.table && !bad) {
+    const int page = kv_page(a.kv, b, at_pos >> a.kv.page_log2);
+    place.k0 = a.kv.base + page * a.kv.seq_bytes;
+    place.max_pos = 1 << a.kv.page_log2;
+    at_pos &= place.max_pos - 1;
+    bad = a.kv.refs[page] > 1;
+  }
+  // its positions on the axes
+  int axis_pos[kMaxAxes] = {};
+  if (a.places) {
+#pragma unroll
+    for (int i = 0; i < kMaxAxes; i++)
+      if (i < a.n_axes) {
+        axis_pos[i] = a.places[(size_t)i * a.kv.sequences * a.kv.rows + row];
+        bad = bad || (uint32_t)axis_pos[i] >= (uint32_t)a.table_positions;
+      }
+  }
   if (a.parents) {
     const Path path = tree_path(a.parents + (size_t)b * a.kv.rows, a.kv.rows);
     depth = __shfl(path.depth, t);
@@ -118,7 +156,14 @@ __global__ __launch_bounds__(kThreads) void k_cache_append(AppendRows a) {
     const int p = ODD || split ? 4 * sub + i : (i < 2 ? 2 * sub + i : HD / 4 + 2 * sub + i - 2);
     cs[i] = make_double2(1.0, 0.0);
     if (p < half && !bad) {
-      const size_t at = (size_t)(s.len + depth) * half + p;
+      int pos = s.len + depth;
+      if (a.places) {
+        const uint32_t axis = (uint32_t)(a.axes[p >> 5] >> (2 * (p & 31))) & 3u;
+        pos = axis_pos[0];
+#pragma unroll
+        for (int j = 1; j < kMaxAxes; j++) pos = axis == (uint32_t)j ? axis_pos[j] : pos;
+      }
+      const size_t at = (size_t)pos * half + p;
       if (a.table) {
         cs[i] = a.table[at];
       } else {
@@ -216,8 +261,8 @@ __global__ __launch_bounds__(kThreads) void k_cache_append(AppendRows a) {
       }
     }
     // the int8 format: the heads' scales
-    float d[kHeads] = {};
-    double inv[kHeads] = {};
+    [[maybe_unused]] float d[kHeads] = {};
+    [[maybe_unused]] double inv[kHeads] = {};
     if constexpr (FMT == Q3H_KV_Q8) {
       if (values || (group + 1) * PER > a.heads) {
         float m[kHeads];
@@ -246,8 +291,65 @@ __global__ __launch_bounds__(kThreads) void k_cache_append(AppendRows a) {
       }
     }
     const int e_a = values ? 4 * sub : ea, e_b = values ? HD / 2 + 4 * sub : eb;
+    // the 4-bit format: the heads' scales and their groups' steps, lane u * NG + i of a head
+    // those of group i of the u-th one
+    constexpr int NG = HD / 32;
+    int step = 0;
+    double step_inv = 0.0;
+    if constexpr (FMT == Q3H_KV_Q4) {
+      if (values || (group + 1) * PER > a.heads) {
+        float mine = 0.f, dm = 0.f;
+#pragma unroll
+        for (int u = 0; u < kHeads; u++) {
+          float m[NG], most = 0.f;
+          bool finite = true;
+#pragma unroll
+          for (int i = 0; i < 8; i++) finite = finite && fabsf(x[u][i]) < INFINITY;
+#pragma unroll
+          for (int i = 0; i < NG; i++) {
+            m[i] = finite ? 0.f : INFINITY;
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+              const int at = ODD && !values ? e[ODD ? k : 0] : k < 4 ? e_a : e_b;
+              m[i] = fmaxf(m[i], at >> 5 == i ? fabsf(x[u][k]) : 0.f);
+            }
+            m[i] = head_max<G>(m[i]);
+            most = fmaxf(most, m[i]);
+          }
+          d[u] = most;
+#pragma unroll
+          for (int i = 0; i < NG; i++)
+            if (sub == u * NG + i) {
+              mine = m[i];
+              dm = most;
+            }
+        }
+        const float scale = dm == INFINITY ? NAN : (float)((double)dm / 1785.0);
+        step = step_of(mine, scale);
+        step_inv = 1.0 / (step * (double)scale);
+#pragma unroll
+        for (int u = 0; u < kHeads; u++) d[u] = __shfl(scale, side * G + u * NG);
+      }
+    }
 #pragma unroll
     for (int u = 0; u < kHeads; u++) {
+      uint32_t steps = 0, nib[8];
+      if constexpr (FMT == Q3H_KV_Q4) {
+        if (values || (group + 1) * PER > a.heads) {
+          const int from = side * G + u * NG;
+#pragma unroll
+          for (int i = 0; i < NG; i++) steps |= (uint32_t)__shfl(step, from + i) << (8 * i);
+#pragma unroll
+          for (int i = 0; i < 8; i += ODD ? 1 : 4) {
+            const int g = (ODD && !values ? e[ODD ? i : 0] : i < 4 ? e_a : e_b) >> 5;
+            const double by = __shfl(step_inv, from + g);
+            const int n = (int)(steps >> (8 * g) & 255u);
+#pragma unroll
+            for (int k = i; k < (ODD ? i + 1 : i + 4); k++)
+              nib[k] = n > 0 ? nibble_of(x[u][k], n * (double)d[u], by) : 8u;
+          }
+        }
+      }
       const int j = first + u * SIDE;
       if (j >= heads) continue;
       // four(element, values' index) or one(...) of the row
@@ -276,9 +378,34 @@ __global__ __launch_bounds__(kThreads) void k_cache_append(AppendRows a) {
         continue;
       }
       if (bad) continue;
-      const int64_t at = kv_row(a.kv, s, values, values ? j : j - a.heads, s.len + t);
-      if constexpr (FMT == Q3H_KV_Q8) {
-        uint8_t *o = reinterpret_cast<uint8_t *>(s.k0) + at * HD;
+      const int64_t at = kv_row(a.kv, place, values, values ? j : j - a.heads, at_pos);
+      if constexpr (FMT == Q3H_KV_Q4) {
+        uint8_t *o = reinterpret_cast<uint8_t *>(place.k0) + at * (HD / 2);
+        if (ODD && !values) {
+          // (a word's elements are with several lanes)
+          uint8_t *row = sm_row[wave][u * SIDE + side];
+#pragma unroll
+          for (int i = 0; i < 8; i++) row[e[ODD ? i : 0]] = (uint8_t)nib[i];
+          __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+          __builtin_amdgcn_wave_barrier();
+          __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+          uint32_t word = 0;
+#pragma unroll
+          for (int i = 0; i < 8; i++) word |= (uint32_t)row[8 * sub + i] << (4 * i);
+          *reinterpret_cast<uint32_t *>(o + 4 * sub) = word;
+        } else {
+          auto four = [&](int i) {
+            return (uint16_t)(nib[i] | nib[i + 1] << 4 | nib[i + 2] << 8 | nib[i + 3] << 12);
+          };
+          *reinterpret_cast<uint16_t *>(o + e_a / 2) = four(0);
+          *reinterpret_cast<uint16_t *>(o + e_b / 2) = four(4);
+        }
+        if (sub == 0) {
+          kv_scales(a.kv, place, HD / 2)[at] = d[u];
+          kv_steps(a.kv, place, HD / 2)[at] = steps;
+        }
+      } else if constexpr (FMT == Q3H_KV_Q8) {
+        uint8_t *o = reinterpret_cast<uint8_t *>(place.k0) + at * HD;
         const bool some = d[u] > 0.f;  // (not NaN, not 0)
         uint32_t y[8];
 #pragma unroll
@@ -287,11 +414,11 @@ __global__ __launch_bounds__(kThreads) void k_cache_append(AppendRows a) {
           *reinterpret_cast<uint32_t *>(o + at) =
               y[i] | y[i + 1] << 8 | y[i + 2] << 16 | y[i + 3] << 24;
         }, [&](int at, int i) { o[at] = y[i]; });
-        if (sub == 0) kv_scales(a.kv, s, HD)[at] = d[u];
+        if (sub == 0) kv_scales(a.kv, place, HD)[at] = d[u];
       } else {
         using KV = std::conditional_t<FMT == Q3H_KV_F16, _Float16, float>;
         typedef KV kv4 __attribute__((ext_vector_type(4)));
-        KV *o = reinterpret_cast<KV *>(s.k0) + at * HD;
+        KV *o = reinterpret_cast<KV *>(place.k0) + at * HD;
         put([&](int at, int i) {
           *reinterpret_cast<kv4 *>(o + at) =
               (kv4){to_cache<KV>(x[u][i]), to_cache<KV>(x[u][i + 1]), to_cache<KV>(x[u][i + 2]),
@@ -312,9 +439,12 @@ template <int FMT, int HD>
 __global__ __launch_bounds__(kThreads) void k_cache_read(KvView kv, const int32_t *starts,
                                                          float *k, float *v) {
   constexpr int PER = HD / 4, SIDE = kThreads / PER;  // threads of a row, rows side by side
+  constexpr int ROW = kv_row_bytes(FMT, HD);
+  constexpr bool Q4 = FMT == Q3H_KV_Q4;
   using KV = std::conditional_t<FMT == Q3H_KV_F32, float,
                                 std::conditional_t<FMT == Q3H_KV_F16, _Float16, uint8_t>>;
-  typedef KV kv4 __attribute__((ext_vector_type(4)));
+  typedef KV kv4v __attribute__((ext_vector_type(4)));
+  using kv4 = std::conditional_t<Q4, uint16_t, kv4v>;
   typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
   const int e = (int)(threadIdx.x % PER) * 4;
   // the workgroup's first row (sequence, position, kv head)
@@ -333,28 +463,34 @@ __global__ __launch_bounds__(kThreads) void k_cache_read(KvView kv, const int32_
     const int b = b0 + (int)over, t = (int)(t0 + pos - over * kv.rows);
     const int in = min(b, kv.sequences - 1);
     KvSeq s;
-    s.k0 = kv.base + in * kv.seq_bytes;
-    s.max_pos = kv.max_pos;
+    s.k0 = kv.base + (kv.table ? 0 : in * kv.seq_bytes);
+    s.max_pos = kv.table ? kv_room(kv, in) : kv.max_pos;
     s.len = starts ? starts[in] : 0;
     s.count = kv.counts ? min(max(kv.counts[in], 0), kv.rows) : kv.rows;
     there[u] = b < kv.sequences && t < s.count;
     bad[u] = s.len < 0 || s.len > s.max_pos - s.count;
-    // (no such row: the first one, which is there)
-    at[u] = kv_row(kv, s, 0, there[u] ? (int)g : 0, there[u] && !bad[u] ? s.len + t : 0);
+    // (no such row: the first one, which is there, if only as page 0)
+    int p = there[u] && !bad[u] ? s.len + t : 0;
+    s = kv_place(kv, s, in, p);
+    at[u] = kv_row(kv, s, 0, there[u] ? (int)g : 0, p);
     base[u] = s.k0;
   }
-  const int64_t values = (int64_t)kv.layers * kv.kvh * kv.max_pos;
+  const int64_t values =
+      (int64_t)kv.layers * kv.kvh * (kv.table ? 1 << kv.page_log2 : kv.max_pos);
 #pragma unroll
   for (int part = 0; part < 2; part++) {
     float *dst = part ? v : k;
     if (!dst) continue;
     kv4 x[kReadRows];
     float d[kReadRows];
+    [[maybe_unused]] int step[kReadRows];
 #pragma unroll
     for (int u = 0; u < kReadRows; u++) {
       const int64_t row = at[u] + part * values;
-      x[u] = *reinterpret_cast<const kv4 *>(reinterpret_cast<const KV *>(base[u]) + row * HD + e);
-      d[u] = FMT == Q3H_KV_Q8 ? reinterpret_cast<const float *>(base[u] + 2 * values * HD)[row] : 1.f;
+      x[u] = *reinterpret_cast<const kv4 *>(base[u] + row * ROW + e * ROW / HD);
+      const char *scales = base[u] + 2 * values * ROW;
+      d[u] = kv_scaled(FMT) ? reinterpret_cast<const float *>(scales)[row] : 1.f;
+      if constexpr (Q4) step[u] = reinterpret_cast<const uint8_t *>(scales + 8 * values)[4 * row + (e >> 5)];
     }
 #pragma unroll
     for (int u = 0; u < kReadRows; u++) {
@@ -362,7 +498,8 @@ __global__ __launch_bounds__(kThreads) void k_cache_read(KvView kv, const int32_
       f4 o;
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        if constexpr (FMT == Q3H_KV_Q8) o[i] = kv_byte(x[u][i]) * d[u];
+        if constexpr (Q4) o[i] = kv_nibble(x[u], i, step[u]) * d[u];
+        else if constexpr (FMT == Q3H_KV_Q8) o[i] = kv_byte(x[u][i]) * d[u];
         else o[i] = (float)x[u][i];
         if (bad[u]) o[i] = NAN;
       }
@@ -381,7 +518,7 @@ __global__ __launch_bounds__(kThreads) void k_cache_read(KvView kv, const int32_
 // thread (HD = 64 int8: 16 words), the rest of the threads on the scale.
 template <int FMT, int HD>
 __global__ __launch_bounds__(128) void k_cache_keep(KvView kv, const int32_t *kept) {
-  constexpr int WORDS = HD * (FMT == Q3H_KV_F32 ? 4 : FMT == Q3H_KV_F16 ? 2 : 1) / 4;
+  constexpr int ROW = kv_row_bytes(FMT, HD), WORDS = ROW / 4;
   const int b = blockIdx.x, tid = threadIdx.x;
   const KvSeq s = kv_sequence(kv, b);
   const int n = kv.counts[b];
@@ -395,29 +532,45 @@ __global__ __launch_bounds__(128) void k_cache_keep(KvView kv, const int32_t *ke
     last = r;
   }
   if (s.len >= s.max_pos - last) return;
+  // (no row goes to a page that another sequence holds too)
+  if (kv.table)
+    for (int at = s.len >> kv.page_log2; at <= (s.len + n - 1) >> kv.page_log2; at++)
+      if (kv.refs[kv_page(kv, b, at)] > 1) return;
   const int layer = blockIdx.y / (2 * kv.kvh), lg = blockIdx.y - layer * 2 * kv.kvh;
   const int part = lg / kv.kvh, g = lg - part * kv.kvh;
   KvView at = kv;
   at.layer = layer;
-  const int64_t first = kv_row(at, s, part, g, s.len);
-  uint32_t *words = reinterpret_cast<uint32_t *>(s.k0) + first * WORDS;
-  float *scales = kv_scales(at, s, HD) + first;
+  struct Row {
+    uint32_t *words, *scale, *steps;
+  };
+  auto row = [&](int i) {
+    int p = s.len + i;
+    const KvSeq place = kv_place(at, s, b, p);
+    const int64_t r = kv_row(at, place, part, g, p);
+    return Row{reinterpret_cast<uint32_t *>(place.k0) + r * WORDS,
+               reinterpret_cast<uint32_t *>(kv_scales(at, place, ROW)) + r,
+               kv_steps(at, place, ROW) + r};
+  };
   for (int i = 0; i < n; i++) {
     const int r = list[i];
     if (r == i) continue;
-    if (tid < WORDS) words[(int64_t)i * WORDS + tid] = words[(int64_t)r * WORDS + tid];
-    if (FMT == Q3H_KV_Q8 && tid == WORDS) scales[i] = scales[r];
+    const Row from = row(r), to = row(i);
+    if (tid < WORDS) to.words[tid] = from.words[tid];
+    if (kv_scaled(FMT) && tid == WORDS) *to.scale = *from.scale;
+    if (FMT == Q3H_KV_Q4 && tid == WORDS + 1) *to.steps = *from.steps;
   }
 }
 
-// int8 rows from and to f32 [layers][kvh][len][HD], a wave a row
-template <int HD>
-__global__ void k_q8_fill(const float *src, char *k0, int part, int layers, int kvh, int len,
-                          int max_pos) {
+// int8 or 4-bit rows from and to f32 [layers][kvh][len][HD], a wave a row
+template <int FMT, int HD>
+__global__ void k_scaled_fill(const float *src, char *k0, int part, int layers, int kvh, int len,
+                              int max_pos) {
   const int lane = threadIdx.x & 63;
   const int64_t r = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
   if (r >= (int64_t)layers * kvh * len) return;
   const int64_t lg = r / len, at = ((int64_t)part * layers * kvh + lg) * max_pos + (r - lg * len);
+  const int64_t rows = 2 * (int64_t)layers * kvh * max_pos;
+  float *scales = reinterpret_cast<float *>(k0 + rows * kv_row_bytes(FMT, HD));
   float x[HD / 64], m = 0.f;
   bool finite = true;
 #pragma unroll
@@ -427,41 +580,81 @@ __global__ void k_q8_fill(const float *src, char *k0, int part, int layers, int 
     m = fmaxf(m, fabsf(x[e]));
   }
   m = wave_max_dpp(finite ? m : INFINITY);
-  const float d = m == INFINITY ? NAN : (float)((double)m / 127.0);
-  const double inv = 1.0 / (double)d;
+  const float d = m == INFINITY ? NAN : (float)((double)m / (FMT == Q3H_KV_Q4 ? 1785.0 : 127.0));
+  if (lane == 0) scales[at] = d;
+  if constexpr (FMT == Q3H_KV_Q4) {
+    // (a half of the wave has a group of an element)
+    uint32_t steps = 0;
 #pragma unroll
-  for (int e = 0; e < HD / 64; e++)
-    reinterpret_cast<uint8_t *>(k0)[at * HD + 64 * e + lane] = d > 0.f ? byte_of(x[e], d, inv) : 128;
-  if (lane == 0)
-    reinterpret_cast<float *>(k0 + 2 * (int64_t)layers * kvh * max_pos * HD)[at] = d;
+    for (int e = 0; e < HD / 64; e++) {
+      const int step = step_of(half_max_dpp(fabsf(x[e])), d);
+      steps |= ((uint32_t)__shfl(step, 0) | (uint32_t)__shfl(step, 32) << 8) << (16 * e);
+      const double by = step * (double)d;
+      const uint32_t n = step > 0 ? nibble_of(x[e], by, 1.0 / by) : 8u;
+      const uint32_t next = (uint32_t)dpp_i<kQuadXor1>((int)n, 0);
+      if (lane % 2 == 0)
+        reinterpret_cast<uint8_t *>(k0)[at * (HD / 2) + 32 * e + lane / 2] = (uint8_t)(n | next << 4);
+    }
+    if (lane == 0) reinterpret_cast<uint32_t *>(scales + rows)[at] = steps;
+  } else {
+    const double inv = 1.0 / (double)d;
+#pragma unroll
+    for (int e = 0; e < HD / 64; e++)
+      reinterpret_cast<uint8_t *>(k0)[at * HD + 64 * e + lane] = d > 0.f ? byte_of(x[e], d, inv) : 128;
+  }
 }
-template <int HD>
-__global__ void k_q8_read(const char *k0, int part, int layers, int layer, int kvh, int len,
-                          int max_pos, float *dst) {
+template <int FMT, int HD>
+__global__ void k_scaled_read(const char *k0, int part, int layers, int layer, int kvh, int len,
+                              int max_pos, float *dst) {
   const int lane = threadIdx.x & 63;
   const int64_t r = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
   if (r >= (int64_t)kvh * len) return;
   const int64_t g = r / len;
   const int64_t at = (((int64_t)part * layers + layer) * kvh + g) * max_pos + (r - g * len);
-  const float d = reinterpret_cast<const float *>(k0 + 2 * (int64_t)layers * kvh * max_pos * HD)[at];
+  const int64_t rows = 2 * (int64_t)layers * kvh * max_pos;
+  const float *scales = reinterpret_cast<const float *>(k0 + rows * kv_row_bytes(FMT, HD));
+  const float d = scales[at];
 #pragma unroll
-  for (int e = 0; e < HD / 64; e++)
-    dst[r * HD + 64 * e + lane] =
-        kv_byte(reinterpret_cast<const uint8_t *>(k0)[at * HD + 64 * e + lane]) * d;
+  for (int e = 0; e < HD / 64; e++) {
+    if constexpr (FMT == Q3H_KV_Q4) {
+      const int i = 64 * e + lane;
+      dst[r * HD + i] =
+          kv_nibble(reinterpret_cast<const uint8_t *>(k0)[at * (HD / 2) + i / 2], i & 1,
+                    reinterpret_cast<const uint8_t *>(scales + rows)[4 * at + i / 32]) * d;
+    } else {
+      dst[r * HD + 64 * e + lane] =
+          kv_byte(reinterpret_cast<const uint8_t *>(k0)[at * HD + 64 * e + lane]) * d;
+    }
+  }
 }
 
 template <template <int, int> class F, class... A>
-void by_format(int hd, int fmt, A &&...args) {
+void by_scaled(int hd, int fmt, A &&...args) {
   if (hd == 64) {
-    if (fmt == Q3H_KV_F32) F<Q3H_KV_F32, 64>::go(args...);
-    else if (fmt == Q3H_KV_F16) F<Q3H_KV_F16, 64>::go(args...);
-    else F<Q3H_KV_Q8, 64>::go(args...);
+    if (fmt == Q3H_KV_Q8) F<Q3H_KV_Q8, 64>::go(args...);
+    else F<Q3H_KV_Q4, 64>::go(args...);
   } else {
-    if (fmt == Q3H_KV_F32) F<Q3H_KV_F32, 128>::go(args...);
-    else if (fmt == Q3H_KV_F16) F<Q3H_KV_F16, 128>::go(args...);
-    else F<Q3H_KV_Q8, 128>::go(args...);
+    if (fmt == Q3H_KV_Q8) F<Q3H_KV_Q8, 128>::go(args...);
+    else F<Q3H_KV_Q4, 128>::go(args...);
   }
 }
+template <int FMT, int HD>
+struct GoFill {
+  static void go(const float *src, char *k0, bool values, int layers, int kvh, int len,
+                 int max_pos, hipStream_t st) {
+    hipLaunchKernelGGL((k_scaled_fill<FMT, HD>),
+                       dim3((unsigned)(((int64_t)layers * kvh * len + 3) / 4)), dim3(kThreads), 0,
+                       st, src, k0, values, layers, kvh, len, max_pos);
+  }
+};
+template <int FMT, int HD>
+struct GoReadBack {
+  static void go(const char *k0, bool values, int layers, int layer, int kvh, int len,
+                 int max_pos, float *dst, hipStream_t st) {
+    hipLaunchKernelGGL((k_scaled_read<FMT, HD>), dim3((unsigned)(((int64_t)kvh * len + 3) / 4)),
+                       dim3(kThreads), 0, st, k0, values, layers, layer, kvh, len, max_pos, dst);
+  }
+};
 
 template <int FMT, int HD>
 struct GoAppend {
@@ -547,7 +740,9 @@ void check_rows(const q3h_cache *c, int layer, int sequences, int rows, const ch
 // threads of a launch, below what a grid takes
 bool launch_fits(int64_t blocks) { return blocks * kThreads < (int64_t)1 << 32; }
 
-KvView view_of(const q3h_cache *c, int layer, int sequences, int rows, const int32_t *lens,
+}  // namespace
+
+KvView kv_view(const q3h_cache *c, int layer, int sequences, int rows, const int32_t *lens,
                const int32_t *counts) {
   KvView v{};
   v.base = c->data;
@@ -560,10 +755,28 @@ KvView view_of(const q3h_cache *c, int layer, int sequences, int rows, const int
   v.layer = layer;
   v.sequences = sequences;
   v.rows = rows;
+  if (c->pages > 0) {
+    v.table = c->state;
+    v.held = v.table + (size_t)c->cfg.sequences * c->slots;
+    v.refs = v.held + c->cfg.sequences;
+    v.pages = c->pages;
+    v.slots = c->slots;
+    v.page_log2 = c->page_log2;
+  }
   return v;
 }
 
-}  // namespace
+void check_cache_config(const q3h_cache_config &f, const char *who) {
+  require(f.sequences > 0 && f.layers > 0 && f.kv_heads > 0 && f.max_positions > 0, Q3H_E_ARG,
+          std::string(who) + ": non-positive dimension");
+  require(f.sequences <= 65535 && f.kv_heads <= 1024 && f.layers <= 1024 &&
+              f.max_positions <= (1 << 24) && (int64_t)f.layers * f.kv_heads <= 32767,
+          Q3H_E_ARG, std::string(who) + ": too many sequences, layers, heads or positions");
+  require(f.head_dim == 64 || f.head_dim == 128, Q3H_E_ARG,
+          std::string(who) + ": head_dim must be 64 or 128");
+  require(kv_format(f.format), Q3H_E_ARG,
+          std::string(who) + ": format must be Q3H_KV_F32, Q3H_KV_F16, Q3H_KV_Q8 or Q3H_KV_Q4");
+}
 
 DeviceScope::DeviceScope(int ordinal) {
   int now = -1;
@@ -585,26 +798,14 @@ void launch_cache_keep(const KvView &v, const int32_t *kept, int hd, int fmt, hi
   by_format<GoKeep>(hd, fmt, v, kept, st);
 }
 
-void launch_q8_fill(const float *src, char *k0, bool values, int layers, int kvh, int len, int hd,
-                    int max_pos, hipStream_t st) {
-  const dim3 grid((unsigned)(((int64_t)layers * kvh * len + 3) / 4));
-  if (hd == 64)
-    hipLaunchKernelGGL(k_q8_fill<64>, grid, dim3(kThreads), 0, st, src, k0, values, layers, kvh,
-                       len, max_pos);
-  else
-    hipLaunchKernelGGL(k_q8_fill<128>, grid, dim3(kThreads), 0, st, src, k0, values, layers, kvh,
-                       len, max_pos);
+void launch_scaled_fill(const float *src, char *k0, bool values, int layers, int kvh, int len,
+                        int hd, int fmt, int max_pos, hipStream_t st) {
+  by_scaled<GoFill>(hd, fmt, src, k0, values, layers, kvh, len, max_pos, st);
 }
 
-void launch_q8_read(const char *k0, bool values, int layers, int layer, int kvh, int len, int hd,
-                    int max_pos, float *dst, hipStream_t st) {
-  const dim3 grid((unsigned)(((int64_t)kvh * len + 3) / 4));
-  if (hd == 64)
-    hipLaunchKernelGGL(k_q8_read<64>, grid, dim3(kThreads), 0, st, k0, values, layers, layer, kvh,
-                       len, max_pos, dst);
-  else
-    hipLaunchKernelGGL(k_q8_read<128>, grid, dim3(kThreads), 0, st, k0, values, layers, layer,
-                       kvh, len, max_pos, dst);
+void launch_scaled_read(const char *k0, bool values, int layers, int layer, int kvh, int len,
+                        int hd, int fmt, int max_pos, float *dst, hipStream_t st) {
+  by_scaled<GoReadBack>(hd, fmt, k0, values, layers, layer, kvh, len, max_pos, dst, st);
 }
 
 }  // namespace q3h
@@ -614,7 +815,10 @@ using namespace q3h;
 // ---------------------------------------------------------------------------
 // rotary tables
 
-extern "C" int q3h_rope_create(q3h_device *dev, const q3h_rope_config *cfg, q3h_rope **out) {
+namespace {
+
+int create_rope(q3h_device *dev, const q3h_rope_config *cfg, int axes, const int32_t *pair_axes,
+                q3h_rope **out) {
   q3h_rope *r = nullptr;
   double *freq = nullptr;
   int rc = guard([&] {
@@ -645,10 +849,18 @@ extern "C" int q3h_rope_create(q3h_device *dev, const q3h_rope_config *cfg, q3h_
             Q3H_E_ARG, "q3h_rope_create: high_turns > low_turns > 0 is needed");
     require(std::isfinite(c.magnitude) && c.magnitude >= 0.f, Q3H_E_ARG,
             "q3h_rope_create: magnitude must not be negative");
+    require(axes >= 1 && axes <= kMaxAxes, Q3H_E_ARG,
+            "q3h_rope_create_axes: axes must be in [1, 4]");
+    for (int i = 0; pair_axes && i < c.rot_dim / 2; i++)
+      require(pair_axes[i] >= 0 && pair_axes[i] < axes, Q3H_E_ARG,
+              "q3h_rope_create_axes: no axis " + std::to_string(pair_axes[i]));
     DeviceScope scope(dev->ordinal);
     r = new q3h_rope();
     r->dev = dev;
     r->cfg = c;
+    r->axes = axes;
+    for (int i = 0; pair_axes && i < c.rot_dim / 2; i++)
+      r->pair_axes[i / 32] |= (uint64_t)pair_axes[i] << (2 * (i % 32));
     double mag = 1.0;
     const std::vector<double> f = rope_frequencies(c, mag);
     const size_t n = (size_t)c.max_positions * f.size();
@@ -673,6 +885,19 @@ extern "C" int q3h_rope_create(q3h_device *dev, const q3h_rope_config *cfg, q3h_
   return rc;
 }
 
+}  // namespace
+
+extern "C" int q3h_rope_create(q3h_device *dev, const q3h_rope_config *cfg, q3h_rope **out) {
+  return create_rope(dev, cfg, 1, nullptr, out);
+}
+
+extern "C" int q3h_rope_create_axes(q3h_device *dev, const q3h_rope_config *cfg, int axes,
+                                    const int32_t *pair_axes, q3h_rope **out) {
+  if (!pair_axes)
+    return guard([&] { require(false, Q3H_E_ARG, "q3h_rope_create_axes: NULL argument"); });
+  return create_rope(dev, cfg, axes, pair_axes, out);
+}
+
 extern "C" int q3h_rope_destroy(q3h_rope *r) {
   return guard([&] {
     require(r != nullptr, Q3H_E_ARG, "q3h_rope_destroy: NULL table");
@@ -692,15 +917,7 @@ extern "C" int q3h_cache_create(q3h_device *dev, const q3h_cache_config *cfg, q3
   int rc = guard([&] {
     require(dev && cfg && out, Q3H_E_ARG, "q3h_cache_create: NULL argument");
     *out = nullptr;
-    require(cfg->sequences > 0 && cfg->layers > 0 && cfg->kv_heads > 0 && cfg->max_positions > 0,
-            Q3H_E_ARG, "q3h_cache_create: non-positive dimension");
-    require(cfg->sequences <= 65535 && cfg->kv_heads <= 1024 && cfg->layers <= 1024 &&
-                cfg->max_positions <= (1 << 24) && (int64_t)cfg->layers * cfg->kv_heads <= 32767,
-            Q3H_E_ARG, "q3h_cache_create: too many sequences, layers, heads or positions");
-    require(cfg->head_dim == 64 || cfg->head_dim == 128, Q3H_E_ARG,
-            "q3h_cache_create: head_dim must be 64 or 128");
-    require(cfg->format >= Q3H_KV_F32 && cfg->format <= Q3H_KV_Q8, Q3H_E_ARG,
-            "q3h_cache_create: format must be Q3H_KV_F32, Q3H_KV_F16 or Q3H_KV_Q8");
+    check_cache_config(*cfg, "q3h_cache_create");
     DeviceScope scope(dev->ordinal);
     c = new q3h_cache();
     c->dev = dev;
@@ -731,13 +948,16 @@ extern "C" int q3h_cache_destroy(q3h_cache *c) {
     require(c != nullptr, Q3H_E_ARG, "q3h_cache_destroy: NULL cache");
     DeviceScope scope(c->dev->ordinal);
     dev_free(c->data);
+    dev_free(c->state);
     c->dev->bytes -= c->bytes;
     c->dev->stacks--;
     delete c;
   });
 }
 
-extern "C" int q3h_cache_append(q3h_cache *c, const q3h_append_args *p, void *stream) {
+namespace {
+
+int append(q3h_cache *c, const q3h_append_args *p, const int32_t *places, void *stream) {
   return guard([&] {
     require(c && p, Q3H_E_ARG, "q3h_cache_append: NULL argument");
     const q3h_cache_config &cf = c->cfg;
@@ -767,7 +987,7 @@ extern "C" int q3h_cache_append(q3h_cache *c, const q3h_append_args *p, void *st
     }
     DeviceScope scope(c->dev->ordinal);
     AppendRows a{};
-    a.kv = view_of(c, p->layer, p->sequences, p->rows, p->lens, p->counts);
+    a.kv = kv_view(c, p->layer, p->sequences, p->rows, p->lens, p->counts);
     a.heads = p->heads;
     a.q = p->q;
     a.k = p->k;
@@ -784,11 +1004,31 @@ extern "C" int q3h_cache_append(q3h_cache *c, const q3h_append_args *p, void *st
       a.table = p->rope->table;
       a.rot_dim = p->rope->cfg.rot_dim;
       a.interleaved = p->rope->cfg.interleaved;
+      a.places = places;
+      a.axes[0] = p->rope->pair_axes[0];
+      a.axes[1] = p->rope->pair_axes[1];
+      a.n_axes = p->rope->axes;
+      a.table_positions = p->rope->cfg.max_positions;
     }
     a.parents = p->parents;
     launch_cache_append(a, cf.head_dim, cf.format, (hipStream_t)stream);
     check_hip(hipGetLastError(), "cache append kernel");
   });
+}
+
+}  // namespace
+
+extern "C" int q3h_cache_append(q3h_cache *c, const q3h_append_args *p, void *stream) {
+  return append(c, p, nullptr, stream);
+}
+
+extern "C" int q3h_cache_append_at(q3h_cache *c, const q3h_append_args *p,
+                                   const int32_t *positions, void *stream) {
+  if (!positions || (p && !p->rope))
+    return guard([&] {
+      require(false, Q3H_E_ARG, "q3h_cache_append_at: NULL positions or rope");
+    });
+  return append(c, p, positions, stream);
 }
 
 extern "C" int q3h_cache_read(q3h_cache *c, int layer, int sequences, int rows,
@@ -803,7 +1043,7 @@ extern "C" int q3h_cache_read(q3h_cache *c, int layer, int sequences, int rows,
             Q3H_E_CAPACITY, "q3h_cache_read: too many rows");
     DeviceScope scope(c->dev->ordinal);
     by_format<GoRead>(c->cfg.head_dim, c->cfg.format,
-                      view_of(c, layer, sequences, rows, nullptr, counts), starts, k, v,
+                      kv_view(c, layer, sequences, rows, nullptr, counts), starts, k, v,
                       (hipStream_t)stream);
     check_hip(hipGetLastError(), "cache read kernel");
   });
@@ -817,7 +1057,7 @@ extern "C" int q3h_cache_keep(q3h_cache *c, int sequences, int rows, const int32
     if (sequences == 0 || rows == 0) return;
     require(lens && kept && kept_counts, Q3H_E_ARG, "q3h_cache_keep: NULL argument");
     DeviceScope scope(c->dev->ordinal);
-    launch_cache_keep(view_of(c, 0, sequences, rows, lens, kept_counts), kept, c->cfg.head_dim,
+    launch_cache_keep(kv_view(c, 0, sequences, rows, lens, kept_counts), kept, c->cfg.head_dim,
                       c->cfg.format, (hipStream_t)stream);
     check_hip(hipGetLastError(), "cache keep kernel");
   });
@@ -873,7 +1113,7 @@ extern "C" int q3h_cache_attend(q3h_cache *c, const q3h_attend_args *p, void *st
                                     " bytes, 256-byte aligned, is needed");
     DeviceScope scope(c->dev->ordinal);
     AttendRows a{};
-    a.kv = view_of(c, p->layer, p->sequences, p->rows, p->lens, p->counts);
+    a.kv = kv_view(c, p->layer, p->sequences, p->rows, p->lens, p->counts);
     a.heads = p->heads;
     a.max_len = p->max_len;
     a.scale = p->scale != 0.f ? p->scale : 1.0f / std::sqrt((float)cf.head_dim);

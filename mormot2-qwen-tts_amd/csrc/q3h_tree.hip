@@ -212,6 +212,32 @@ __device__ __forceinline__ uint32_t bytes_f16(uint32_t y, uint32_t x, uint32_t s
   return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(b, up, off));
 }
 
+// Elements of the 4-bit format as f16, 2^-19 times what they stand for but the row's
+// scale: (n - 8) * step, a whole number up to 1785, exactly. An element n under zeros is a
+// subnormal, n 2^-24 (in the second place 2^-20), which one packed multiply-add takes
+// with 2^5 step to its place. (Those below 32 steps stay subnormal; what the matrix
+// instructions cut off a product with them is below 2^-29 of the row's largest.)
+struct Steps {
+  uint32_t by, by16, off;  // 2^5 step, 2 step, -2^-16 step, two rows each
+};
+// the bytes of (y, x) at sel's places (each under a byte of zeros)
+__device__ __forceinline__ Steps steps_f16(uint32_t y, uint32_t x, uint32_t sel) {
+  const h2 b = __builtin_bit_cast(h2, __builtin_amdgcn_perm(y, x, sel) | 0x64006400u);  // 1024 + step
+  const h2 up = {(_Float16)32.f, (_Float16)32.f}, off = {(_Float16)-32768.f, (_Float16)-32768.f};
+  const h2 low = {(_Float16)-0x1p-21f, (_Float16)-0x1p-21f}, part = {(_Float16)0x1p-4f, (_Float16)0x1p-4f};
+  const h2 by = __builtin_elementwise_fma(b, up, off);
+  return {__builtin_bit_cast(uint32_t, by), __builtin_bit_cast(uint32_t, by * part),
+          __builtin_bit_cast(uint32_t, by * low)};
+}
+// element c (0 .. 3) of each half of w
+__device__ __forceinline__ uint32_t nibbles_f16(uint32_t w, int c, const Steps &s) {
+  const uint32_t n = (c & 2 ? w >> 8 : w) & (c & 1 ? 0x00f000f0u : 0x000f000fu);
+  return __builtin_bit_cast(
+      uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(h2, n),
+                                          __builtin_bit_cast(h2, c & 1 ? s.by16 : s.by),
+                                          __builtin_bit_cast(h2, s.off)));
+}
+
 template <int FMT, int HD>
 struct Raw;  // a tile's keys and values as loaded
 
@@ -227,19 +253,29 @@ struct Raw<Q3H_KV_Q8, HD> {
   f4 ks[2], vs[2];
 };
 template <int HD>
+struct Raw<Q3H_KV_Q4, HD> {
+  uint32_t k[2][HD / 32];  // HD / 4 elements
+  uint32_t v[8];           // 8 positions of HD / 16 elements
+  uint32_t kw[2];          // the keys' steps
+  u4 vw[2];                // the values' steps of 4 positions
+  f4 ks[2], vs[2];
+};
+template <int HD>
 struct Raw<Q3H_KV_F32, HD> {
   f4 k[HD / 16];
   f4 v[4][HD / 64];
 };
 
 // NQ query tiles a wave share its loads and conversions of K and V.
-template <int FMT, int HD, int NQ>
+// PAGED: the cache's pages, each of whole tiles.
+template <int FMT, int HD, int NQ, bool PAGED>
 __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shape) {
   constexpr int T = kTile<FMT>;
   constexpr int C = HD / 16;           // output tiles; neighbouring elements a lane reads
-  constexpr bool F32 = FMT == Q3H_KV_F32, Q8 = FMT == Q3H_KV_Q8;
+  constexpr bool F32 = FMT == Q3H_KV_F32, Q8 = FMT == Q3H_KV_Q8, Q4 = FMT == Q3H_KV_Q4;
+  constexpr bool SC = kv_scaled(FMT);            // rows with a scale
   constexpr int NS = F32 ? 1 : 2;                // key tiles of 16 in a tile
-  constexpr int ROW = HD * (F32 ? 4 : Q8 ? 1 : 2);  // bytes
+  constexpr int ROW = kv_row_bytes(FMT, HD);     // bytes
   constexpr int LD = HD + 4;  // (rows 4 banks apart)
   // the waves' outputs; before that, with two query tiles a wave, its queries as
   // operands (64 registers: two waves a SIMD would not have them)
@@ -351,35 +387,89 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
   const int here = cut.here, WQ = cut.wq, WK = cut.wk;
   const int wq = wave & (WQ - 1), wk = wave / WQ;
 
-  const char *kbase = s.k0 + kv_row(a.kv, s, 0, g, 0) * ROW;
-  const char *vbase = s.k0 + kv_row(a.kv, s, 1, g, 0) * ROW;
-  const char *ksc = nullptr, *vsc = nullptr;
-  if constexpr (Q8) {
-    ksc = reinterpret_cast<const char *>(kv_scales(a.kv, s, HD) + kv_row(a.kv, s, 0, g, 0));
-    vsc = reinterpret_cast<const char *>(kv_scales(a.kv, s, HD) + kv_row(a.kv, s, 1, g, 0));
+  // Where the keys, the values, their scales and steps of a tile's first position are.
+  // Of pages: those of the wave's tiles in its lanes, 64 at a time.
+  struct Place {
+    const char *k, *v, *ks, *vs, *kw, *vw;
+  };
+  const KvSeq home = PAGED ? KvSeq{s.k0, 1 << a.kv.page_log2, 0, 0} : s;
+  const int64_t key_row = kv_row(a.kv, home, 0, g, 0), value_row = kv_row(a.kv, home, 1, g, 0);
+  Place base{};
+  base.k = home.k0 + key_row * ROW;
+  base.v = home.k0 + value_row * ROW;
+  if constexpr (SC) {
+    base.ks = reinterpret_cast<const char *>(kv_scales(a.kv, home, ROW) + key_row);
+    base.vs = reinterpret_cast<const char *>(kv_scales(a.kv, home, ROW) + value_row);
   }
+  if constexpr (Q4) {
+    base.kw = reinterpret_cast<const char *>(kv_steps(a.kv, home, ROW) + key_row);
+    base.vw = reinterpret_cast<const char *>(kv_steps(a.kv, home, ROW) + value_row);
+  }
+  [[maybe_unused]] int pages = 0, pages_at = -64;
+  auto place = [&](int j0) {
+    Place p = base;
+    int64_t row = j0;
+    int64_t off = 0;
+    if constexpr (PAGED) {
+      const int slot = j0 >> a.kv.page_log2;
+      if ((uint32_t)(slot - pages_at) >= 64u) {
+        pages_at = slot;
+        pages = kv_page(a.kv, b, std::min(slot + lane, a.kv.slots - 1));
+      }
+      off = __builtin_amdgcn_readlane(pages, slot - pages_at) * a.kv.seq_bytes;
+      row = j0 & ((1 << a.kv.page_log2) - 1);
+    }
+    p.k += off + row * ROW;
+    p.v += off + row * ROW;
+    if constexpr (SC) {
+      p.ks += off + row * 4;
+      p.vs += off + row * 4;
+    }
+    if constexpr (Q4) {
+      p.kw += off + row * 4;
+      p.vw += off + row * 4;
+    }
+    return p;
+  };
 
-  auto load_scales = [&](const char *sc, int j0, f4(&d)[2]) {
+  // four bytes for each of positions 4 g4 .. + 3 of the tile's halves
+  auto load_fours = [&](const char *sc, int j0, auto(&d)[2]) {
+    using V = std::remove_reference_t<decltype(d[0])>;
+    typedef V unaligned __attribute__((aligned(4)));
 #pragma unroll
     for (int t = 0; t < 2; t++) {
-      const int j = j0 + 16 * t + 4 * g4;
       if (j0 + T <= cut.end) {
-        d[t] = load<f4u>(sc + 4 * (int64_t)j0, (uint32_t)(64 * t + 16 * g4));
+        d[t] = load<unaligned>(sc, (uint32_t)(64 * t + 16 * g4));
       } else {
 #pragma unroll
-        for (int r = 0; r < 4; r++) d[t][r] = load<float>(sc, 4 * (int64_t)std::min(j + r, last));
+        for (int r = 0; r < 4; r++)
+          d[t][r] = load<std::remove_reference_t<decltype(d[t][r])>>(
+              sc, 4 * std::min(16 * t + 4 * g4 + r, last - j0));
       }
     }
   };
   auto load_k = [&](Raw<FMT, HD> &raw, int tile) {
     const int j0 = tile * T;
-    const char *p = kbase + (int64_t)j0 * ROW;
+    const Place at_tile = place(j0);
+    const char *p = at_tile.k;
 #pragma unroll
     for (int t = 0; t < NS; t++) {
-      const uint32_t at = (uint32_t)(std::min(16 * t + n16, last - j0) * ROW + 16 * g4);
+      const int row = std::min(16 * t + n16, last - j0);
+      const uint32_t at = (uint32_t)(row * ROW + (Q4 ? HD / 8 : 16) * g4);
       if constexpr (F32) {
 #pragma unroll
         for (int i = 0; i < HD / 16; i++) raw.k[i] = load<f4>(p, at + 64 * i);
+      } else if constexpr (Q4) {
+        if constexpr (HD == 128) {
+          const u4 x = load<u4>(p, at);
+#pragma unroll
+          for (int i = 0; i < 4; i++) raw.k[t][i] = x[i];
+        } else {
+          const u2 x = load<u2>(p, at);
+#pragma unroll
+          for (int i = 0; i < 2; i++) raw.k[t][i] = x[i];
+        }
+        raw.kw[t] = load<uint32_t>(at_tile.kw, (uint32_t)(4 * row));
       } else if constexpr (Q8) {
 #pragma unroll
         for (int i = 0; i < HD / 64; i++) raw.k[t][i] = load<u4>(p, at + 64 * i);
@@ -388,11 +478,12 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
         for (int i = 0; i < HD / 32; i++) raw.k[t][i] = load<u4>(p, at + 64 * i);
       }
     }
-    if constexpr (Q8) load_scales(ksc, j0, raw.ks);
+    if constexpr (SC) load_fours(at_tile.ks, j0, raw.ks);
   };
   auto load_v = [&](Raw<FMT, HD> &raw, int tile) {
     const int j0 = tile * T;
-    const char *p = vbase + (int64_t)j0 * ROW;
+    const Place at_tile = place(j0);
+    const char *p = at_tile.v;
 #pragma unroll
     for (int i = 0; i < (F32 ? 4 : 8); i++) {
       const int j = F32 ? 4 * g4 + i : (i >> 2) * 16 + 4 * g4 + (i & 3);
@@ -400,6 +491,9 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
       if constexpr (F32) {
 #pragma unroll
         for (int e = 0; e < HD / 64; e++) raw.v[i][e] = load<f4>(p, at + 16 * e);
+      } else if constexpr (Q4) {
+        if constexpr (HD == 128) raw.v[i] = load<uint32_t>(p, at);
+        else raw.v[i] = load<uint16_t>(p, at);
       } else if constexpr (Q8) {
         if constexpr (HD == 128) raw.v[i] = load<u2>(p, at);
         else raw.v[i / 2][i & 1] = load<uint32_t>(p, at);
@@ -413,8 +507,14 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
         }
       }
     }
-    if constexpr (Q8) load_scales(vsc, j0, raw.vs);
+    if constexpr (SC) load_fours(at_tile.vs, j0, raw.vs);
+    if constexpr (Q4) load_fours(at_tile.vw, j0, raw.vw);
   };
+  // 4 bits: where a key's and a value's group is in its word of steps
+  [[maybe_unused]] const uint32_t key_sel =
+      0x0c000c00u + 0x00010001u * (uint32_t)(HD == 128 ? g4 : g4 >> 1);
+  [[maybe_unused]] const uint32_t value_sel =
+      0x0c040c00u + 0x00010001u * (uint32_t)(n16 >> (HD == 128 ? 2 : 3));
   // word w of the HD / 16 elements of position i of the loaded values
   auto vword = [](const Raw<FMT, HD> &raw, int i, int w) -> uint32_t {
     if constexpr (FMT == Q3H_KV_F16)
@@ -432,16 +532,24 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
   const bool shared = QLDS && WK == 1;
   u4 *const sm_k = reinterpret_cast<u4 *>(sm + QB) + lane, *const sm_v = sm_k + 2 * KI * 64;
   struct Quarter {
-    u4 k[Q8 ? 1 : KN];
+    u4 k[SC ? 1 : KN];
     uint32_t v[8];
+    uint32_t kw;
+    u4 vw[2];
     f4 ks[2], vs[2];
   };
   auto load_quarter = [&](Quarter &raw, int tile) {
     const int j0 = tile * T;
     const int t = wave >> 1, i = (wave & 1) * KN;
-    const char *p = kbase + (int64_t)j0 * ROW;
-    const uint32_t at = (uint32_t)(std::min(16 * t + n16, last - j0) * ROW + 16 * g4);
-    if constexpr (Q8) {
+    const Place at_tile = place(j0);
+    const char *p = at_tile.k;
+    const int row = std::min(16 * t + n16, last - j0);
+    const uint32_t at = (uint32_t)(row * ROW + (Q4 ? HD / 8 : 16) * g4);
+    if constexpr (Q4) {
+#pragma unroll
+      for (int u = 0; u < KN; u++) raw.k[0][u] = load<uint32_t>(p, at + 4 * (i + u));
+      raw.kw = load<uint32_t>(at_tile.kw, (uint32_t)(4 * row));
+    } else if constexpr (Q8) {
       if constexpr (KN == 2) {
         raw.k[0] = load<u4>(p, at + 32 * i);
       } else {
@@ -453,24 +561,30 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
 #pragma unroll
       for (int u = 0; u < KN; u++) raw.k[u] = load<u4>(p, at + 64 * (i + u));
     }
-    p = vbase + (int64_t)j0 * ROW;
+    p = at_tile.v;
     const int word = VN * wave >> (Q8 ? 2 : 1);
 #pragma unroll
     for (int u = 0; u < 8; u++) {
       const int j = (u >> 2) * 16 + 4 * g4 + (u & 3);
-      raw.v[u] = load<uint32_t>(
-          p, (uint32_t)(std::min(j, last - j0) * ROW + n16 * (ROW / 16) + 4 * word));
+      const uint32_t at = (uint32_t)(std::min(j, last - j0) * ROW + n16 * (ROW / 16));
+      if constexpr (Q4) raw.v[u] = load<uint8_t>(p, at + (VN * wave >> 1));
+      else raw.v[u] = load<uint32_t>(p, at + 4 * word);
     }
-    if constexpr (Q8) {
-      load_scales(ksc, j0, raw.ks);
-      load_scales(vsc, j0, raw.vs);
+    if constexpr (SC) {
+      load_fours(at_tile.ks, j0, raw.ks);
+      load_fours(at_tile.vs, j0, raw.vs);
     }
+    if constexpr (Q4) load_fours(at_tile.vw, j0, raw.vw);
   };
   auto store_quarter = [&](const Quarter &raw) {
 #pragma unroll
     for (int u = 0; u < KN; u++) {
       u4 x;
-      if constexpr (Q8) {
+      if constexpr (Q4) {
+        const Steps st = steps_f16(raw.kw, raw.kw, key_sel);
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] = nibbles_f16(raw.k[0][u], e, st);
+      } else if constexpr (Q8) {
 #pragma unroll
         for (int e = 0; e < 2; e++) {
           const uint32_t w = raw.k[0][2 * u + e];
@@ -491,7 +605,11 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
       u4 x;
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        if constexpr (Q8) x[e] = bytes_f16(raw.v[2 * e + 1], raw.v[2 * e], sel);
+        if constexpr (Q4)
+          x[e] = nibbles_f16(raw.v[2 * e] | raw.v[2 * e + 1] << 16, c & 1,
+                             steps_f16(raw.vw[e >> 1][2 * (e & 1) + 1], raw.vw[e >> 1][2 * (e & 1)],
+                                       value_sel));
+        else if constexpr (Q8) x[e] = bytes_f16(raw.v[2 * e + 1], raw.v[2 * e], sel);
         else x[e] = __builtin_amdgcn_perm(raw.v[2 * e + 1], raw.v[2 * e], sel);
       }
       sm_v[c * 64] = x;
@@ -530,6 +648,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
 #pragma unroll
     for (int i = 0; i < HD / 16; i++) {
       const int d = F32 ? 16 * i + 4 * g4
+                    : Q4 ? g4 * (HD / 4) + 4 * i
                     : Q8 ? (i >> 2) * 64 + g4 * 16 + (i & 3) * 4
                          : (i >> 1) * 32 + g4 * 8 + (i & 1) * 4;
       qx[q][i] = load<f4u>(p, 4 * d);
@@ -569,9 +688,10 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
         u4 h, l;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          const f4 x = qx[q][2 * i + (e >> 1)];
+          // (4 bits: elements e and 4 + e of a word)
+          const f4 x = qx[q][2 * i + (Q4 ? 0 : e >> 1)], y = qx[q][2 * i + (Q4 ? 1 : e >> 1)];
           uint32_t hi, lo;
-          split2(x[2 * (e & 1)] * up, x[2 * (e & 1) + 1] * up, hi, lo);
+          split2(x[Q4 ? e : 2 * (e & 1)] * up, y[Q4 ? e : 2 * (e & 1) + 1] * up, hi, lo);
           h[e] = hi;
           l[e] = lo;
         }
@@ -583,7 +703,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
           ql[q][i] = l;
         }
       }
-      sfac[q] = ldexpf(factor, Q8 ? 9 - k : -k);
+      sfac[q] = ldexpf(factor, (Q4 ? 19 : Q8 ? 9 : 0) - k);
     }
   }
 
@@ -634,13 +754,17 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
       for (int i = 0; i < HD / 32; i++)
 #pragma unroll
         for (int t = 0; t < NS; t++) {
-          // int8: the wave at its products goes first, so that the two of a SIMD
+          // int8 (and 4 bits): the wave at its products goes first, so that the two of a SIMD
           // move apart, one's products beside the other's softmax (143.6 -> 140.1
           // us, the prompt in int8 109.6 -> 111.7; f16 trees slower by 0.5 %)
-          if (Q8 && i == 0 && t == 0) __builtin_amdgcn_s_setprio(1);
+          if (SC && i == 0 && t == 0) __builtin_amdgcn_s_setprio(1);
           u4 ka;
           if constexpr (SHARE) {
             ka = sm_k[(t * KI + i) * 64];
+          } else if constexpr (Q4) {
+            const Steps steps = steps_f16(raw.kw[t], raw.kw[t], key_sel);
+#pragma unroll
+            for (int e = 0; e < 4; e++) ka[e] = nibbles_f16(raw.k[t][i], e, steps);
           } else if constexpr (Q8) {
 #pragma unroll
             for (int e = 0; e < 2; e++) {
@@ -661,9 +785,9 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
           }
         }
     }
-    if constexpr (Q8) __builtin_amdgcn_s_setprio(0);
+    if constexpr (SC) __builtin_amdgcn_s_setprio(0);
     f4 ks[2], vs[2];
-    if constexpr (Q8) {
+    if constexpr (SC) {
 #pragma unroll
       for (int t = 0; t < 2; t++) {
         ks[t] = raw.ks[t];
@@ -685,7 +809,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
         broken[q] = __shfl((int)p.bad, qt[q]) != 0;
       }
     }
-    // int8: the largest scale of the tile, and whether some are so much smaller
+    // int8 and 4 bits: the largest scale of the tile, and whether some are so much smaller
     // (2^16; a weight's two parts have 39 bits below 2^14) that the maximum has to be
     // taken of scores and scales together, position by position. A scale's power of
     // two is taken within 2^-40 .. 2^50: further apart, the factor between two tiles'
@@ -697,7 +821,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
     auto power = [](float x) {
       return (float)std::min(50, std::max(-40, (int)(__float_as_uint(x) >> 23) - 126));
     };
-    if constexpr (Q8) {
+    if constexpr (SC) {
       float low = INFINITY;
 #pragma unroll
       for (int i = 0; i < 8; i++) {
@@ -712,7 +836,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
       float mx = -INFINITY, vx = top;
 #pragma unroll
       for (int i = 0; i < 4 * NS; i++)
-        w[q][i] = Q8 ? st[q][i >> 2][i & 3] * ks[i >> 2][i & 3] : st[q][i >> 2][i & 3];
+        w[q][i] = SC ? st[q][i >> 2][i & 3] * ks[i >> 2][i & 3] : st[q][i >> 2][i & 3];
       if (tail) {
         asm volatile("");  // (a branch, so that the other tiles have no selects)
         vx = 0.f;
@@ -723,14 +847,14 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
           w[q][i] = see ? w[q][i] : -INFINITY;
           // a row whose path is broken: NaN at itself, and so in all of it
           if (broken[q] && d == qt[q]) w[q][i] = NAN;
-          if (Q8 && see) vx = fmaxf(vx, vs[i >> 2][i & 3]);
+          if (SC && see) vx = fmaxf(vx, vs[i >> 2][i & 3]);
         }
-        if constexpr (Q8) vx = rows4_max(vx);
+        if constexpr (SC) vx = rows4_max(vx);
       }
 #pragma unroll
       for (int i = 0; i < 4 * NS; i++) mx = fmaxf(mx, w[q][i]);
       float off = F32 ? 0.f : -14.f;
-      if (Q8 && wide) {
+      if (SC && wide) {
         asm volatile("");
         mx = -INFINITY;
 #pragma unroll
@@ -738,9 +862,9 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
           mx = fmaxf(mx, fmaf(w[q][i], sfac[q], power(vs[i >> 2][i & 3])));
         mx = rows4_max(mx) + off;
       } else {
-        mx = fmaf(rows4_max(mx), sfac[q], Q8 ? off + power(top) : off);
+        mx = fmaf(rows4_max(mx), sfac[q], SC ? off + power(top) : off);
       }
-      if constexpr (Q8) vmax[q] = fmaxf(vmax[q], vx);
+      if constexpr (SC) vmax[q] = fmaxf(vmax[q], vx);
       mx = fmaxf(m[q], mx);
       const float base = mx == -INFINITY ? 0.f : mx;
       if (__any(mx > m[q])) {
@@ -754,7 +878,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
       for (int i = 0; i < 4 * NS; i++) {
         const float p = __builtin_amdgcn_exp2f(fmaf(w[q][i], sfac[q], -base));
         l[q] += p;
-        w[q][i] = Q8 ? p * vs[i >> 2][i & 3] : p;
+        w[q][i] = SC ? p * vs[i >> 2][i & 3] : p;
       }
     }
 
@@ -784,12 +908,19 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
       }
 #pragma unroll
       for (int c = 0; c < C; c++) {
-        if (Q8 && c == 0) __builtin_amdgcn_s_setprio(1);
+        if (SC && c == 0) __builtin_amdgcn_s_setprio(1);
         u4 va;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
           if constexpr (SHARE) {
             // (below)
+          } else if constexpr (Q4) {
+            // elements c of positions 2e and 2e + 1
+            const uint32_t w = __builtin_amdgcn_perm(raw.v[2 * e + 1], raw.v[2 * e],
+                                                     c & 4 ? 0x07060302u : 0x05040100u);
+            va[e] = nibbles_f16(w, c & 3,
+                                steps_f16(raw.vw[e >> 1][2 * (e & 1) + 1],
+                                          raw.vw[e >> 1][2 * (e & 1)], value_sel));
           } else if constexpr (Q8) {
             // bytes c of positions 2e and 2e + 1
             va[e] = bytes_f16(vword(raw, 2 * e + 1, c >> 2), vword(raw, 2 * e, c >> 2),
@@ -808,7 +939,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
         }
       }
     }
-    if constexpr (Q8) __builtin_amdgcn_s_setprio(0);
+    if constexpr (SC) __builtin_amdgcn_s_setprio(0);
     if constexpr (!SHARE) {
       if (next < tile1) load_v(raw, next);
     }
@@ -832,14 +963,14 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
   bool nan = false;
 #pragma unroll
   for (int q = 0; q < NQ; q++) {
-    scale[q] = Q8 ? 0x1p9f : 1.f;
+    scale[q] = Q4 ? 0x1p19f : Q8 ? 0x1p9f : 1.f;
     l[q] = rows4_sum(l[q]);
     float zero = 0.f * l[q];
 #pragma unroll
     for (int c = 0; c < C; c++)
 #pragma unroll
       for (int r = 0; r < 4; r++) zero = fmaf(acc[q][c][r], 0.f, zero);
-    nan = nan || (zero != 0.f && !broken[q]) || (Q8 && vmax[q] > 0.f && vmax[q] < 0x1p-56f);
+    nan = nan || (zero != 0.f && !broken[q]) || (SC && vmax[q] > 0.f && vmax[q] < 0x1p-56f);
   }
   // An infinity times one of the parts that a query or a weight is split in is
   // NaN where the product itself is not, and so is an infinity that a row does
@@ -857,17 +988,19 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
       for (int at = tile0 + wk; at < tile1; at += WK)
 #pragma unroll 1
         for (int j = at * T; j < std::min(at * T + T, cut.end); j++) {
-          const float kd = Q8 ? load<float>(ksc, 4 * (int64_t)j) : 1.f;
-          const float vd = Q8 ? load<float>(vsc, 4 * (int64_t)j) : 1.f;
-          auto value = [&](const char *base, int e) {
-            const int64_t off = (int64_t)j * ROW;
-            if constexpr (F32) return load<float>(base, off + 4 * e);
-            else if constexpr (Q8) return kv_byte(load<uint8_t>(base, off + e));
-            else return (float)load<_Float16>(base, off + 2 * e);
+          const Place at_pos = place(j);
+          const float kd = SC ? load<float>(at_pos.ks, 0) : 1.f;
+          const float vd = SC ? load<float>(at_pos.vs, 0) : 1.f;
+          auto value = [&](const char *base, const char *steps, int e) {
+            if constexpr (F32) return load<float>(base, 4 * e);
+            else if constexpr (Q4)
+              return kv_nibble(load<uint8_t>(base, e >> 1), e & 1, load<uint8_t>(steps, e >> 5));
+            else if constexpr (Q8) return kv_byte(load<uint8_t>(base, e));
+            else return (float)load<_Float16>(base, 2 * e);
           };
           float x = 0.f;
 #pragma unroll 1
-          for (int e = 0; e < HD / 4; e++) x = fmaf(p[e], value(kbase, C * 4 * g4 + e), x);
+          for (int e = 0; e < HD / 4; e++) x = fmaf(p[e], value(at_pos.k, at_pos.kw, C * 4 * g4 + e), x);
           x = rows4_sum(x) * kd * a.scale * kLog2e;
           if (!sees(q, j - s.len)) continue;
           if (broken[q]) x = NAN;
@@ -878,7 +1011,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
           for (int c = 0; c < C; c++)
 #pragma unroll
             for (int r = 0; r < 4; r++)
-              acc[q][c][r] = fmaf(acc[q][c][r], f, w * (value(vbase, C * (4 * g4 + r) + c) * vd));
+              acc[q][c][r] = fmaf(acc[q][c][r], f,
+                                  w * (value(at_pos.v, at_pos.vw, C * (4 * g4 + r) + c) * vd));
           ms = mn;
         }
       m[q] = ms;
@@ -962,7 +1096,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
 // (lengths, rows and queries, the waves' meeting): 171 positions, 16 heads over 8,
 // 8.1 us (8.9 on the matrix instructions; 8.6 with four waves, 8.2 with eight), 64
 // such sequences 14.1 (16.5).
-template <int HD>
+template <int HD, bool PAGED>
 __global__ __launch_bounds__(384) void k_attend_few(AttendRows a, int per_kv) {
   constexpr int R = 2, W = 6, E = HD / 64;
   typedef float fe __attribute__((ext_vector_type(E)));
@@ -996,8 +1130,9 @@ __global__ __launch_bounds__(384) void k_attend_few(AttendRows a, int per_kv) {
     return;
   }
   const int end = s.len + s.count, last = end - 1;
-  const char *kbase = s.k0 + kv_row(a.kv, s, 0, g, 0) * (HD * 4);
-  const char *vbase = s.k0 + kv_row(a.kv, s, 1, g, 0) * (HD * 4);
+  const KvSeq home = PAGED ? KvSeq{s.k0, 1 << a.kv.page_log2, 0, 0} : s;
+  const char *kbase = s.k0 + kv_row(a.kv, home, 0, g, 0) * (HD * 4);
+  const char *vbase = s.k0 + kv_row(a.kv, home, 1, g, 0) * (HD * 4);
   f4 q[R][HD / 16];
 #pragma unroll
   for (int r = 0; r < R; r++) {
@@ -1015,7 +1150,11 @@ __global__ __launch_bounds__(384) void k_attend_few(AttendRows a, int per_kv) {
   fe acc[R] = {};
   for (int tile = wave; tile * 16 < end; tile += W) {
     const int j0 = tile * 16;
-    const char *kp = kbase + (int64_t)j0 * (HD * 4), *vp = vbase + (int64_t)j0 * (HD * 4);
+    int64_t off = (int64_t)j0 * (HD * 4);
+    if constexpr (PAGED)
+      off = kv_page(a.kv, b, j0 >> a.kv.page_log2) * a.kv.seq_bytes +
+            (j0 & (home.max_pos - 1)) * (HD * 4);
+    const char *kp = kbase + off, *vp = vbase + off;
     f4 k[HD / 16];
     fe v[16];
 #pragma unroll
@@ -1224,19 +1363,19 @@ int64_t join_sets(int sequences, int rows, int heads, int kvh, int hd) {
   return (int64_t)sequences * kvh * (((int64_t)rows * (heads / kvh) + per - 1) / per);
 }
 
-template <int FMT, int HD>
+template <int FMT, int HD, bool PAGED>
 void launch(const AttendRows &a, hipStream_t st) {
   const Shape s = shape_of(a.kv.sequences, a.kv.rows, a.heads, a.kv.kvh, HD, a.max_len, kTile<FMT>,
                            a.room);
   const unsigned blocks = s.blocks;
   if (FMT == Q3H_KV_F32 && !s.shares && a.kv.rows * s.per_kv <= 2) {
-    hipLaunchKernelGGL((k_attend_few<HD>), dim3(blocks), dim3(384), 0, st, a, s.per_kv);
+    hipLaunchKernelGGL((k_attend_few<HD, PAGED>), dim3(blocks), dim3(384), 0, st, a, s.per_kv);
     return;
   }
   if (s.nq == 1)
-    hipLaunchKernelGGL((k_attend<FMT, HD, 1>), dim3(blocks), dim3(kThreads), 0, st, a, s);
+    hipLaunchKernelGGL((k_attend<FMT, HD, 1, PAGED>), dim3(blocks), dim3(kThreads), 0, st, a, s);
   else
-    hipLaunchKernelGGL((k_attend<FMT, HD, 2>), dim3(blocks), dim3(kThreads), 0, st, a, s);
+    hipLaunchKernelGGL((k_attend<FMT, HD, 2, PAGED>), dim3(blocks), dim3(kThreads), 0, st, a, s);
   if (s.shares) {
     const int64_t sets = join_sets(a.kv.sequences, a.kv.rows, a.heads, a.kv.kvh, HD);
     const int side = sets >= 2048 ? 1 : kWaves;
@@ -1267,16 +1406,26 @@ bool attend_fits(int sequences, int rows, int heads, int kvh, int hd, int fmt, i
          (!s.shares || join_sets(sequences, rows, heads, kvh, hd) * 64 + kThreads < most);
 }
 
+namespace {
+
+template <int FMT, int HD>
+void launch_in(const AttendRows &a, hipStream_t st) {
+  if (a.kv.table) launch<FMT, HD, true>(a, st);
+  else launch<FMT, HD, false>(a, st);
+}
+template <int HD>
+void launch_fmt(const AttendRows &a, int fmt, hipStream_t st) {
+  if (fmt == Q3H_KV_F32) launch_in<Q3H_KV_F32, HD>(a, st);
+  else if (fmt == Q3H_KV_F16) launch_in<Q3H_KV_F16, HD>(a, st);
+  else if (fmt == Q3H_KV_Q8) launch_in<Q3H_KV_Q8, HD>(a, st);
+  else launch_in<Q3H_KV_Q4, HD>(a, st);
+}
+
+}  // namespace
+
 void launch_cache_attend(const AttendRows &a, int hd, int fmt, hipStream_t st) {
-  if (hd == 64) {
-    if (fmt == Q3H_KV_F32) launch<Q3H_KV_F32, 64>(a, st);
-    else if (fmt == Q3H_KV_F16) launch<Q3H_KV_F16, 64>(a, st);
-    else launch<Q3H_KV_Q8, 64>(a, st);
-  } else {
-    if (fmt == Q3H_KV_F32) launch<Q3H_KV_F32, 128>(a, st);
-    else if (fmt == Q3H_KV_F16) launch<Q3H_KV_F16, 128>(a, st);
-    else launch<Q3H_KV_Q8, 128>(a, st);
-  }
+  if (hd == 64) launch_fmt<64>(a, fmt, st);
+  else launch_fmt<128>(a, fmt, st);
 }
 
 }  // namespace q3h

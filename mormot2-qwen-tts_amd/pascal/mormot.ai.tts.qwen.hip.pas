@@ -29,6 +29,8 @@ const
   Q3H_KV_F32 = 0;
   Q3H_KV_F16 = 1;
   Q3H_KV_Q8 = 2;
+  Q3H_KV_Q4 = 4;
+  Q3H_MAX_PAGES = 1 shl 20;
   Q3H_ROPE_PLAIN = 0;
   Q3H_ROPE_LINEAR = 1;
   Q3H_ROPE_YARN = 2;
@@ -152,6 +154,13 @@ type
     sequences, layers, kv_heads, head_dim, max_positions, format: integer;
   end;
   Pq3h_cache_config = ^q3h_cache_config;
+
+  /// a cache in pages that its sequences share
+  q3h_paged_config = record
+    cache: q3h_cache_config;
+    pages, page_positions: integer;
+  end;
+  Pq3h_paged_config = ^q3h_paged_config;
 
   q3h_append_args = record
     layer, sequences, rows, heads: integer;
@@ -292,13 +301,20 @@ function q3h_codec_destroy(c: q3h_codec): integer; cdecl; external LIBQ3H;
 { drafted rows: caches, rotary forms, attention over a tree, token scores }
 function q3h_rope_create(dev: q3h_device; cfg: Pq3h_rope_config;
   out rope: q3h_rope): integer; cdecl; external LIBQ3H;
+function q3h_rope_create_axes(dev: q3h_device; cfg: Pq3h_rope_config;
+  axes: integer; pair_axes: PInteger; out rope: q3h_rope): integer;
+  cdecl; external LIBQ3H;
 function q3h_rope_destroy(r: q3h_rope): integer; cdecl; external LIBQ3H;
 function q3h_cache_create(dev: q3h_device; cfg: Pq3h_cache_config;
+  out cache: q3h_cache): integer; cdecl; external LIBQ3H;
+function q3h_cache_create_paged(dev: q3h_device; cfg: Pq3h_paged_config;
   out cache: q3h_cache): integer; cdecl; external LIBQ3H;
 function q3h_cache_bytes(c: q3h_cache): Int64; cdecl; external LIBQ3H;
 function q3h_cache_destroy(c: q3h_cache): integer; cdecl; external LIBQ3H;
 function q3h_cache_append(c: q3h_cache; a: Pq3h_append_args;
   stream: pointer): integer; cdecl; external LIBQ3H;
+function q3h_cache_append_at(c: q3h_cache; a: Pq3h_append_args;
+  positions: PInteger; stream: pointer): integer; cdecl; external LIBQ3H;
 function q3h_cache_read(c: q3h_cache; layer, sequences, rows: integer;
   starts, counts: PInteger; k, v: PSingle; stream: pointer): integer;
   cdecl; external LIBQ3H;
@@ -309,6 +325,18 @@ function q3h_cache_attend(c: q3h_cache; a: Pq3h_attend_args;
 function q3h_cache_keep(c: q3h_cache; sequences, rows: integer;
   lens, kept, kept_counts: PInteger; stream: pointer): integer;
   cdecl; external LIBQ3H;
+function q3h_cache_reserve(c: q3h_cache; sequences, rows: integer;
+  lens, counts, ok: PInteger; stream: pointer): integer; cdecl; external LIBQ3H;
+function q3h_cache_fork(c: q3h_cache; sequences: integer;
+  sources, lens: PInteger; stream: pointer): integer; cdecl; external LIBQ3H;
+function q3h_cache_release(c: q3h_cache; sequences: integer; lens: PInteger;
+  stream: pointer): integer; cdecl; external LIBQ3H;
+function q3h_cache_compact(c: q3h_cache; used: PInteger;
+  stream: pointer): integer; cdecl; external LIBQ3H;
+function q3h_cache_copy(c, src: q3h_cache; sequences: integer;
+  sources, lens: PInteger; stream: pointer): integer; cdecl; external LIBQ3H;
+function q3h_cache_page_state(c: q3h_cache; table, counts, refs: PInteger;
+  stream: pointer): integer; cdecl; external LIBQ3H;
 function q3h_token_logprobs_workspace(rows, vocab, top_k: integer): Int64;
   cdecl; external LIBQ3H;
 function q3h_token_logprobs(dev: q3h_device; a: Pq3h_score_args;

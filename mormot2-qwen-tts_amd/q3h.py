@@ -24,7 +24,7 @@ Q8_0 = 1
 BF16 = 2
 
 # formats of a K/V cache (Q3H_KV_*)
-KV_F32, KV_F16, KV_Q8 = 0, 1, 2
+KV_F32, KV_F16, KV_Q8, KV_Q4 = 0, 1, 2, 4
 # rotary scalings (Q3H_ROPE_*)
 ROPE_SCALING = {"plain": 0, "linear": 1, "yarn": 2, "bands": 3}
 TREE_MAX_ROWS = 64  # Q3H_TREE_MAX_ROWS
@@ -145,6 +145,11 @@ class CacheConfig(ctypes.Structure):
                 ("sequences", "layers", "kv_heads", "head_dim", "max_positions", "format")]
 
 
+class PagedConfig(ctypes.Structure):
+    _fields_ = [("cache", CacheConfig), ("pages", ctypes.c_int32),
+                ("page_positions", ctypes.c_int32)]
+
+
 # q3h_append_args, q3h_attend_args and q3h_score_args, field by field in the
 # header's order with C's alignment: packed for each call, which takes a quarter of
 # the time that a ctypes structure does (2 us of a call's 8)
@@ -209,15 +214,24 @@ SIGNATURES = {
     "q3h_codec_destroy": (_I, [_P]),
     "q3h_frame_start_text": (_I, [_P, _I, _P, ctypes.POINTER(StartIds), _IP, _I, _IP, _I, _I]),
     "q3h_rope_create": (_I, [_P, ctypes.POINTER(RopeConfig), ctypes.POINTER(_P)]),
+    "q3h_rope_create_axes": (_I, [_P, ctypes.POINTER(RopeConfig), _I, _IP, ctypes.POINTER(_P)]),
     "q3h_rope_destroy": (_I, [_P]),
     "q3h_cache_create": (_I, [_P, ctypes.POINTER(CacheConfig), ctypes.POINTER(_P)]),
+    "q3h_cache_create_paged": (_I, [_P, ctypes.POINTER(PagedConfig), ctypes.POINTER(_P)]),
     "q3h_cache_bytes": (ctypes.c_int64, [_P]),
     "q3h_cache_destroy": (_I, [_P]),
     "q3h_cache_append": (_I, [_P, _P, _P]),
+    "q3h_cache_append_at": (_I, [_P, _P, _P, _P]),
     "q3h_cache_read": (_I, [_P, _I, _I, _I, _P, _P, _P, _P, _P]),
     "q3h_cache_attend_workspace": (ctypes.c_int64, [_P, _I, _I, _I, _I]),
     "q3h_cache_attend": (_I, [_P, _P, _P]),
     "q3h_cache_keep": (_I, [_P, _I, _I, _P, _P, _P, _P]),
+    "q3h_cache_reserve": (_I, [_P, _I, _I, _P, _P, _P, _P]),
+    "q3h_cache_fork": (_I, [_P, _I, _P, _P, _P]),
+    "q3h_cache_release": (_I, [_P, _I, _P, _P]),
+    "q3h_cache_compact": (_I, [_P, _P, _P]),
+    "q3h_cache_copy": (_I, [_P, _P, _I, _P, _P, _P]),
+    "q3h_cache_page_state": (_I, [_P, _P, _P, _P, _P]),
     "q3h_token_logprobs_workspace": (ctypes.c_int64, [_I, _I, _I]),
     "q3h_token_logprobs": (_I, [_P, _P, _P]),
     "q3h_stack_set_rope": (_I, [_P, ctypes.POINTER(RopeConfig)]),
@@ -819,17 +833,27 @@ class Rope:
     in neighbouring pairs (interleaved) or in pairs half of them apart. scaling:
     None, dict(kind="linear", factor=), dict(kind="yarn", factor=, original=,
     beta_fast=32, beta_slow=1), dict(kind="bands", factor=, original=, low=1,
-    high=4); magnitude: on cosine and sine (0: the scaling's own)."""
+    high=4); magnitude: on cosine and sine (0: the scaling's own). axes: the axis of
+    each pair (0 .. 3), whose positions Cache.append gets."""
 
     h = None
 
     def __init__(self, dev, head_dim, max_positions, theta, rot_dim=None, interleaved=False,
-                 scaling=None, magnitude=0.0):
+                 scaling=None, magnitude=0.0, axes=None):
         cfg = _rope_config(head_dim, max_positions, theta, rot_dim, interleaved, scaling,
                            magnitude)
         h = _P()
         L = lib()
-        _check(L.q3h_rope_create(dev.h, ctypes.byref(cfg), ctypes.byref(h)))
+        self.axes = 1
+        if axes is None:
+            _check(L.q3h_rope_create(dev.h, ctypes.byref(cfg), ctypes.byref(h)))
+        else:
+            pairs = [int(x) for x in axes]
+            if len(pairs) != cfg.rot_dim // 2:
+                _bad(f"axes of {len(pairs)} pairs, not of {cfg.rot_dim // 2}")
+            self.axes = max(pairs, default=0) + 1
+            _check(L.q3h_rope_create_axes(dev.h, ctypes.byref(cfg), self.axes,
+                                          (ctypes.c_int32 * len(pairs))(*pairs), ctypes.byref(h)))
         self.dev = dev
         self.h = h
         self._destroy = L.q3h_rope_destroy
@@ -845,25 +869,35 @@ class Rope:
 
 
 class Cache:
-    """A K/V cache of several sequences (q3h_cache_*), in f32, f16 or one byte
-    per element with a scale per position and head (KV_F32, KV_F16, KV_Q8).
-    Calls take rows [sequences][rows][heads][head_dim] for the first sequences of
+    """A K/V cache of several sequences (q3h_cache_*), in f32, f16, one byte
+    per element with a scale per position and head, or four bits with steps for each
+    32 elements too (KV_F32, KV_F16, KV_Q8, KV_Q4). With pages: in that many pages of
+    page_positions positions (32, 64, 128 or 256) that the sequences share (reserve,
+    fork, release, compact). Calls take rows [sequences][rows][heads][head_dim] for the first sequences of
     the cache; lens, counts [sequences] and parents [sequences][rows] are int32
     tensors on the device."""
 
     h = None
 
-    def __init__(self, dev, sequences, kv_heads, head_dim, max_positions, fmt=KV_F32, layers=1):
+    def __init__(self, dev, sequences, kv_heads, head_dim, max_positions, fmt=KV_F32, layers=1,
+                 pages=0, page_positions=64):
         cfg = CacheConfig(sequences, layers, kv_heads, head_dim, max_positions, fmt)
         h = _P()
         L = lib()
-        _check(L.q3h_cache_create(dev.h, ctypes.byref(cfg), ctypes.byref(h)))
+        if pages:
+            paged = PagedConfig(cfg, pages, page_positions)
+            _check(L.q3h_cache_create_paged(dev.h, ctypes.byref(paged), ctypes.byref(h)))
+        else:
+            _check(L.q3h_cache_create(dev.h, ctypes.byref(cfg), ctypes.byref(h)))
         _use_torch()
+        self.pages = pages
+        self.table_shape = (sequences, -(-max_positions // page_positions))
         self.dev = dev
         self.h = h
         self.kv_heads, self.head_dim = kv_heads, head_dim
         self._append, self._read, self._attend = \
             L.q3h_cache_append, L.q3h_cache_read, L.q3h_cache_attend
+        self._append_at = L.q3h_cache_append_at
         self._workspace = L.q3h_cache_attend_workspace
         self._destroy = L.q3h_cache_destroy
 
@@ -872,12 +906,13 @@ class Cache:
         return lib().q3h_cache_bytes(self.h)
 
     def append(self, k, v, lens, counts=None, parents=None, q=None, q_out=None, rope=None,
-               q_norm=None, k_norm=None, eps=1e-6, layer=0):
+               q_norm=None, k_norm=None, eps=1e-6, layer=0, positions=None):
         """Writes the drafted rows k, v at positions lens[b] + row, keys and
         queries normed (q_norm, k_norm) and turned (rope) first. Returns the
         queries (q_out, made when it is None; rows beyond counts as they were),
         None without q. parents: the row each row continues (-1: the sequence
-        itself); None: a chain."""
+        itself); None: a chain. positions [axes of the rope][sequences][rows]: those
+        that the rows are turned by (None: lens[b] plus their depth)."""
         o, hd, i32, f32 = self.dev.ordinal, self.head_dim, _torch.int32, _torch.float32
         n, rows = k.shape[0], k.shape[1]
         pk, ldk = _rows(k, n, rows, self.kv_heads, hd, o, "k")
@@ -897,7 +932,12 @@ class Cache:
             _whole(k_norm, (hd,), o, f32, "k_norm"), eps, turn,
             _whole(lens, (n,), o, i32, "lens"), _whole(counts, (n,), o, i32, "counts"),
             _whole(parents, (n, rows), o, i32, "parents"))
-        _check(self._append(self.h, a, _stream(o)))
+        if positions is None:
+            _check(self._append(self.h, a, _stream(o)))
+        else:
+            at = _whole(positions, (rope.axes if rope is not None else 1, n, rows), o, i32,
+                        "positions")
+            _check(self._append_at(self.h, a, at, _stream(o)))
         return q_out
 
     def read(self, k, v, starts=None, counts=None, layer=0):
@@ -956,6 +996,63 @@ class Cache:
             self.h, n, rows, _whole(lens, (n,), o, i32, "lens"),
             _whole(kept, (n, rows), o, i32, "kept"),
             _whole(kept_counts, (n,), o, i32, "kept_counts"), _stream(o)))
+
+    def reserve(self, lens, rows, counts=None, ok=None):
+        """Pages for positions lens[b] .. lens[b] + counts[b] - 1 (counts None: rows of
+        them), own ones: pages of that range that other sequences hold too are copied.
+        ok [sequences] (None: not wanted) is set to 1 where a sequence has them, 0 where
+        there were too few; returned."""
+        o, i32 = self.dev.ordinal, _torch.int32
+        n = lens.shape[0]
+        _check(lib().q3h_cache_reserve(
+            self.h, n, rows, _whole(lens, (n,), o, i32, "lens"),
+            _whole(counts, (n,), o, i32, "counts"), _whole(ok, (n,), o, i32, "ok"), _stream(o)))
+        return ok
+
+    def fork(self, sources, lens):
+        """Sequence b becomes the first lens[b] positions of what sequence sources[b]
+        was (-1: nothing), for all b at once; pages are shared."""
+        o, i32 = self.dev.ordinal, _torch.int32
+        n = sources.shape[0]
+        _check(lib().q3h_cache_fork(
+            self.h, n, _whole(sources, (n,), o, i32, "sources"),
+            _whole(lens, (n,), o, i32, "lens"), _stream(o)))
+
+    def release(self, lens):
+        """Sequence b keeps the pages of its first lens[b] positions (0: none)."""
+        o = self.dev.ordinal
+        n = lens.shape[0]
+        _check(lib().q3h_cache_release(
+            self.h, n, _whole(lens, (n,), o, _torch.int32, "lens"), _stream(o)))
+
+    def compact(self, used=None):
+        """Moves the pages in use to the front; returns their number (used [1], an
+        int32 tensor on the device, made when it is None)."""
+        o, i32 = self.dev.ordinal, _torch.int32
+        if used is None:
+            used = _torch.empty(1, dtype=i32, device=f"cuda:{o}")
+        _check(lib().q3h_cache_compact(self.h, _whole(used, (1,), o, i32, "used"), _stream(o)))
+        return used
+
+    def copy(self, src, sources, lens):
+        """The first lens[b] positions of sequence sources[b] of another cache (-1:
+        none) to sequence b, which has the room already."""
+        o, i32 = self.dev.ordinal, _torch.int32
+        n = sources.shape[0]
+        _check(lib().q3h_cache_copy(
+            self.h, src.h, n, _whole(sources, (n,), o, i32, "sources"),
+            _whole(lens, (n,), o, i32, "lens"), _stream(o)))
+
+    def page_state(self):
+        """(table [sequences][pages of one at most], counts of pages that a sequence
+        holds, refs: how many sequences hold a page), int32 copies."""
+        o, i32 = self.dev.ordinal, _torch.int32
+        if not self.pages:
+            _bad("not a cache of pages")
+        out = [_torch.empty(shape, dtype=i32, device=f"cuda:{o}") for shape in
+               (self.table_shape, self.table_shape[:1], (self.pages,))]
+        _check(lib().q3h_cache_page_state(self.h, *(t.data_ptr() for t in out), _stream(o)))
+        return tuple(out)
 
     def destroy(self):
         if self.h:
