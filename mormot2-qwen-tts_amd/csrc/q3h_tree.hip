@@ -67,6 +67,15 @@ __device__ __forceinline__ T load(const char *p, int64_t off) {
       reinterpret_cast<uintptr_t>(p) + off);
 }
 
+// the same at a base that is the wave's, an offset of the lane's and one that is known: no
+// address arithmetic
+template <typename T>
+__device__ __forceinline__ T load(const char *p, uint32_t off, int known) {
+  typedef const __attribute__((address_space(1))) char *At;
+  return *reinterpret_cast<const __attribute__((address_space(1))) T *>(
+      reinterpret_cast<At>(reinterpret_cast<uintptr_t>(p)) + off + known);
+}
+
 // positions of a tile
 template <int FMT>
 constexpr int kTile = FMT == Q3H_KV_F32 ? 16 : 32;
@@ -267,8 +276,11 @@ struct Raw<Q3H_KV_F32, HD> {
 };
 
 // NQ query tiles a wave share its loads and conversions of K and V.
-// PAGED: the cache's pages, each of whole tiles.
-template <int FMT, int HD, int NQ, bool PAGED>
+// PAGED: the cache's pages, each of whole tiles. SIDE: up to 8 query rows; the two f16
+// parts of a query and of a weight are columns of one product, 8 apart, instead of two
+// products one after another, and meet in a sum of the lanes (the scores' at each tile,
+// the outputs' at the end).
+template <int FMT, int HD, int NQ, bool PAGED, bool SIDE>
 __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shape) {
   constexpr int T = kTile<FMT>;
   constexpr int C = HD / 16;           // output tiles; neighbouring elements a lane reads
@@ -387,128 +399,140 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
   const int here = cut.here, WQ = cut.wq, WK = cut.wk;
   const int wq = wave & (WQ - 1), wk = wave / WQ;
 
-  // Where the keys, the values, their scales and steps of a tile's first position are.
-  // Of pages: those of the wave's tiles in its lanes, 64 at a time.
-  struct Place {
-    const char *k, *v, *ks, *vs, *kw, *vw;
-  };
+  // Where the keys, the values, their scales and steps of the sequence (its pages) begin.
   const KvSeq home = PAGED ? KvSeq{s.k0, 1 << a.kv.page_log2, 0, 0} : s;
   const int64_t key_row = kv_row(a.kv, home, 0, g, 0), value_row = kv_row(a.kv, home, 1, g, 0);
-  Place base{};
-  base.k = home.k0 + key_row * ROW;
-  base.v = home.k0 + value_row * ROW;
+  const char *kbase = home.k0 + key_row * ROW, *vbase = home.k0 + value_row * ROW;
+  const char *ksc = nullptr, *vsc = nullptr, *kst = nullptr, *vst = nullptr;
   if constexpr (SC) {
-    base.ks = reinterpret_cast<const char *>(kv_scales(a.kv, home, ROW) + key_row);
-    base.vs = reinterpret_cast<const char *>(kv_scales(a.kv, home, ROW) + value_row);
+    ksc = reinterpret_cast<const char *>(kv_scales(a.kv, home, ROW) + key_row);
+    vsc = reinterpret_cast<const char *>(kv_scales(a.kv, home, ROW) + value_row);
   }
   if constexpr (Q4) {
-    base.kw = reinterpret_cast<const char *>(kv_steps(a.kv, home, ROW) + key_row);
-    base.vw = reinterpret_cast<const char *>(kv_steps(a.kv, home, ROW) + value_row);
+    kst = reinterpret_cast<const char *>(kv_steps(a.kv, home, ROW) + key_row);
+    vst = reinterpret_cast<const char *>(kv_steps(a.kv, home, ROW) + value_row);
   }
+  // A position as bytes to its page and its place there (no pages: 0 and itself). The pages
+  // of the wave's next tiles are in its lanes, 64 at a time.
+  struct Place {
+    int64_t page, row;
+    __device__ __forceinline__ const char *in(const char *base, int bytes) const {
+      return base + page + row * bytes;
+    }
+  };
   [[maybe_unused]] int pages = 0, pages_at = -64;
   auto place = [&](int j0) {
-    Place p = base;
-    int64_t row = j0;
-    int64_t off = 0;
-    if constexpr (PAGED) {
-      const int slot = j0 >> a.kv.page_log2;
-      if ((uint32_t)(slot - pages_at) >= 64u) {
-        pages_at = slot;
-        pages = kv_page(a.kv, b, std::min(slot + lane, a.kv.slots - 1));
-      }
-      off = __builtin_amdgcn_readlane(pages, slot - pages_at) * a.kv.seq_bytes;
-      row = j0 & ((1 << a.kv.page_log2) - 1);
+    if constexpr (!PAGED) return Place{0, j0};
+    const int slot = j0 >> a.kv.page_log2;
+    if ((uint32_t)(slot - pages_at) >= 64u) {
+      pages_at = slot;
+      pages = kv_page(a.kv, b, std::min(slot + lane, a.kv.slots - 1));
     }
-    p.k += off + row * ROW;
-    p.v += off + row * ROW;
-    if constexpr (SC) {
-      p.ks += off + row * 4;
-      p.vs += off + row * 4;
-    }
-    if constexpr (Q4) {
-      p.kw += off + row * 4;
-      p.vw += off + row * 4;
-    }
-    return p;
+    return Place{__builtin_amdgcn_readlane(pages, slot - pages_at) * a.kv.seq_bytes,
+                 j0 & ((1 << a.kv.page_log2) - 1)};
   };
 
+  // The loads of a tile: f(true) of a whole one, whose addresses are the lane's own
+  // and the tile's; f(false) of a group's last, where no row behind the last is read.
+  // (Two query tiles of the other formats, whose registers are full, clamp every row:
+  // two sets of loads cost them 2 %, f32 7 %.)
+  constexpr bool BOTH = Q4 || NQ == 1;
+  auto of_tile = [&](int j0, auto &&f) {
+    if constexpr (BOTH) {
+      if (j0 + T <= cut.end) {
+        f(std::true_type());
+        return;
+      }
+    }
+    f(std::false_type());
+  };
   // four bytes for each of positions 4 g4 .. + 3 of the tile's halves
-  auto load_fours = [&](const char *sc, int j0, auto(&d)[2]) {
+  auto load_fours = [&](const char *sc, int j0, auto(&d)[2], auto full) {
     using V = std::remove_reference_t<decltype(d[0])>;
     typedef V unaligned __attribute__((aligned(4)));
 #pragma unroll
     for (int t = 0; t < 2; t++) {
-      if (j0 + T <= cut.end) {
+      if constexpr (decltype(full)::value) {
+        d[t] = load<unaligned>(sc, (uint32_t)(16 * g4), 64 * t);
+      } else if (!BOTH && j0 + T <= cut.end) {
         d[t] = load<unaligned>(sc, (uint32_t)(64 * t + 16 * g4));
       } else {
 #pragma unroll
         for (int r = 0; r < 4; r++)
           d[t][r] = load<std::remove_reference_t<decltype(d[t][r])>>(
-              sc, 4 * std::min(16 * t + 4 * g4 + r, last - j0));
+              sc, 4 * (int64_t)std::min(16 * t + 4 * g4 + r, last - j0));
       }
     }
   };
   auto load_k = [&](Raw<FMT, HD> &raw, int tile) {
     const int j0 = tile * T;
     const Place at_tile = place(j0);
-    const char *p = at_tile.k;
+    of_tile(j0, [&](auto full) {
+      constexpr bool FULL = decltype(full)::value;
 #pragma unroll
-    for (int t = 0; t < NS; t++) {
-      const int row = std::min(16 * t + n16, last - j0);
-      const uint32_t at = (uint32_t)(row * ROW + (Q4 ? HD / 8 : 16) * g4);
-      if constexpr (F32) {
+      for (int t = 0; t < NS; t++) {
+        const char *p = at_tile.in(kbase, ROW) + (FULL ? 16 * t * ROW : 0);
+        const int row = FULL ? n16 : std::min(16 * t + n16, last - j0);
+        const uint32_t at = (uint32_t)(row * ROW + (Q4 ? HD / 8 : 16) * g4);
+        if constexpr (F32) {
 #pragma unroll
-        for (int i = 0; i < HD / 16; i++) raw.k[i] = load<f4>(p, at + 64 * i);
-      } else if constexpr (Q4) {
-        if constexpr (HD == 128) {
-          const u4 x = load<u4>(p, at);
+          for (int i = 0; i < HD / 16; i++) raw.k[i] = load<f4>(p, at, 64 * i);
+        } else if constexpr (Q4) {
+          if constexpr (HD == 128) {
+            const u4 x = load<u4>(p, at, 0);
 #pragma unroll
-          for (int i = 0; i < 4; i++) raw.k[t][i] = x[i];
+            for (int i = 0; i < 4; i++) raw.k[t][i] = x[i];
+          } else {
+            const u2 x = load<u2>(p, at, 0);
+#pragma unroll
+            for (int i = 0; i < 2; i++) raw.k[t][i] = x[i];
+          }
+          raw.kw[t] = load<uint32_t>(at_tile.in(kst, 4), (uint32_t)(4 * row), FULL ? 64 * t : 0);
+        } else if constexpr (Q8) {
+#pragma unroll
+          for (int i = 0; i < HD / 64; i++) raw.k[t][i] = load<u4>(p, at, 64 * i);
         } else {
-          const u2 x = load<u2>(p, at);
 #pragma unroll
-          for (int i = 0; i < 2; i++) raw.k[t][i] = x[i];
+          for (int i = 0; i < HD / 32; i++) raw.k[t][i] = load<u4>(p, at, 64 * i);
         }
-        raw.kw[t] = load<uint32_t>(at_tile.kw, (uint32_t)(4 * row));
-      } else if constexpr (Q8) {
-#pragma unroll
-        for (int i = 0; i < HD / 64; i++) raw.k[t][i] = load<u4>(p, at + 64 * i);
-      } else {
-#pragma unroll
-        for (int i = 0; i < HD / 32; i++) raw.k[t][i] = load<u4>(p, at + 64 * i);
       }
-    }
-    if constexpr (SC) load_fours(at_tile.ks, j0, raw.ks);
+      if constexpr (SC) load_fours(at_tile.in(ksc, 4), j0, raw.ks, full);
+    });
   };
   auto load_v = [&](Raw<FMT, HD> &raw, int tile) {
     const int j0 = tile * T;
     const Place at_tile = place(j0);
-    const char *p = at_tile.v;
+    of_tile(j0, [&](auto full) {
+      constexpr bool FULL = decltype(full)::value;
 #pragma unroll
-    for (int i = 0; i < (F32 ? 4 : 8); i++) {
-      const int j = F32 ? 4 * g4 + i : (i >> 2) * 16 + 4 * g4 + (i & 3);
-      const uint32_t at = (uint32_t)(std::min(j, last - j0) * ROW + n16 * (ROW / 16));
-      if constexpr (F32) {
+      for (int i = 0; i < (F32 ? 4 : 8); i++) {
+        const char *p = at_tile.in(vbase, ROW) + (FULL ? (i >> 2) * 16 * ROW : 0);
+        const int j = (FULL ? 0 : (i >> 2) * 16 + (i & 3)) + 4 * g4;
+        const int known = FULL ? (i & 3) * ROW : 0;
+        const uint32_t at =
+            (uint32_t)((FULL ? j : std::min(j, last - j0)) * ROW + n16 * (ROW / 16));
+        if constexpr (F32) {
 #pragma unroll
-        for (int e = 0; e < HD / 64; e++) raw.v[i][e] = load<f4>(p, at + 16 * e);
-      } else if constexpr (Q4) {
-        if constexpr (HD == 128) raw.v[i] = load<uint32_t>(p, at);
-        else raw.v[i] = load<uint16_t>(p, at);
-      } else if constexpr (Q8) {
-        if constexpr (HD == 128) raw.v[i] = load<u2>(p, at);
-        else raw.v[i / 2][i & 1] = load<uint32_t>(p, at);
-      } else {
-        if constexpr (HD == 128) {
-          raw.v[i] = load<u4>(p, at);
+          for (int e = 0; e < HD / 64; e++) raw.v[i][e] = load<f4>(p, at, known + 16 * e);
+        } else if constexpr (Q4) {
+          if constexpr (HD == 128) raw.v[i] = load<uint32_t>(p, at, known);
+          else raw.v[i] = load<uint16_t>(p, at, known);
+        } else if constexpr (Q8) {
+          if constexpr (HD == 128) raw.v[i] = load<u2>(p, at, known);
+          else raw.v[i / 2][i & 1] = load<uint32_t>(p, at, known);
         } else {
-          const u2 x = load<u2>(p, at);
-          raw.v[i / 2][2 * (i & 1)] = x[0];
-          raw.v[i / 2][2 * (i & 1) + 1] = x[1];
+          if constexpr (HD == 128) {
+            raw.v[i] = load<u4>(p, at, known);
+          } else {
+            const u2 x = load<u2>(p, at, known);
+            raw.v[i / 2][2 * (i & 1)] = x[0];
+            raw.v[i / 2][2 * (i & 1) + 1] = x[1];
+          }
         }
       }
-    }
-    if constexpr (SC) load_fours(at_tile.vs, j0, raw.vs);
-    if constexpr (Q4) load_fours(at_tile.vw, j0, raw.vw);
+      if constexpr (SC) load_fours(at_tile.in(vsc, 4), j0, raw.vs, full);
+      if constexpr (Q4) load_fours(at_tile.in(vst, 4), j0, raw.vw, full);
+    });
   };
   // 4 bits: where a key's and a value's group is in its word of steps
   [[maybe_unused]] const uint32_t key_sel =
@@ -542,39 +566,45 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
     const int j0 = tile * T;
     const int t = wave >> 1, i = (wave & 1) * KN;
     const Place at_tile = place(j0);
-    const char *p = at_tile.k;
-    const int row = std::min(16 * t + n16, last - j0);
-    const uint32_t at = (uint32_t)(row * ROW + (Q4 ? HD / 8 : 16) * g4);
-    if constexpr (Q4) {
+    of_tile(j0, [&](auto full) {
+      constexpr bool FULL = decltype(full)::value;
+      const char *p = at_tile.in(kbase, ROW) + (FULL ? 16 * t * ROW : 0);
+      const int row = FULL ? n16 : std::min(16 * t + n16, last - j0);
+      const uint32_t at = (uint32_t)(row * ROW + (Q4 ? HD / 8 : 16) * g4);
+      if constexpr (Q4) {
 #pragma unroll
-      for (int u = 0; u < KN; u++) raw.k[0][u] = load<uint32_t>(p, at + 4 * (i + u));
-      raw.kw = load<uint32_t>(at_tile.kw, (uint32_t)(4 * row));
-    } else if constexpr (Q8) {
-      if constexpr (KN == 2) {
-        raw.k[0] = load<u4>(p, at + 32 * i);
+        for (int u = 0; u < KN; u++) raw.k[0][u] = load<uint32_t>(p + 4 * i, at, 4 * u);
+        raw.kw = load<uint32_t>(at_tile.in(kst, 4) + (FULL ? 64 * t : 0), (uint32_t)(4 * row), 0);
+      } else if constexpr (Q8) {
+        if constexpr (KN == 2) {
+          raw.k[0] = load<u4>(p + 32 * i, at, 0);
+        } else {
+          const u2 x = load<u2>(p + 8 * i, at, 0);
+          raw.k[0][0] = x[0];
+          raw.k[0][1] = x[1];
+        }
       } else {
-        const u2 x = load<u2>(p, at + 8 * i);
-        raw.k[0][0] = x[0];
-        raw.k[0][1] = x[1];
+#pragma unroll
+        for (int u = 0; u < KN; u++) raw.k[u] = load<u4>(p + 64 * i, at, 64 * u);
       }
-    } else {
+      const int word = VN * wave >> (Q8 ? 2 : 1);
 #pragma unroll
-      for (int u = 0; u < KN; u++) raw.k[u] = load<u4>(p, at + 64 * (i + u));
-    }
-    p = at_tile.v;
-    const int word = VN * wave >> (Q8 ? 2 : 1);
-#pragma unroll
-    for (int u = 0; u < 8; u++) {
-      const int j = (u >> 2) * 16 + 4 * g4 + (u & 3);
-      const uint32_t at = (uint32_t)(std::min(j, last - j0) * ROW + n16 * (ROW / 16));
-      if constexpr (Q4) raw.v[u] = load<uint8_t>(p, at + (VN * wave >> 1));
-      else raw.v[u] = load<uint32_t>(p, at + 4 * word);
-    }
-    if constexpr (SC) {
-      load_fours(at_tile.ks, j0, raw.ks);
-      load_fours(at_tile.vs, j0, raw.vs);
-    }
-    if constexpr (Q4) load_fours(at_tile.vw, j0, raw.vw);
+      for (int u = 0; u < 8; u++) {
+        const char *q = at_tile.in(vbase, ROW) + (FULL ? (u >> 2) * 16 * ROW : 0) +
+                        (Q4 ? VN * wave >> 1 : 4 * word);
+        const int j = (FULL ? 0 : (u >> 2) * 16 + (u & 3)) + 4 * g4;
+        const int known = FULL ? (u & 3) * ROW : 0;
+        const uint32_t v =
+            (uint32_t)((FULL ? j : std::min(j, last - j0)) * ROW + n16 * (ROW / 16));
+        if constexpr (Q4) raw.v[u] = load<uint8_t>(q, v, known);
+        else raw.v[u] = load<uint32_t>(q, v, known);
+      }
+      if constexpr (SC) {
+        load_fours(at_tile.in(ksc, 4), j0, raw.ks, full);
+        load_fours(at_tile.in(vsc, 4), j0, raw.vs, full);
+      }
+      if constexpr (Q4) load_fours(at_tile.in(vst, 4), j0, raw.vw, full);
+    });
   };
   auto store_quarter = [&](const Quarter &raw) {
 #pragma unroll
@@ -625,7 +655,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
   int qrow[NQ], qt[NQ];  // the lane's query row, and the drafted row that it is of
   bool live[NQ];
   f4 qf[F32 ? NQ : 1][HD / 16];
-  u4 qh[F32 || QLDS ? 1 : NQ][HD / 32], ql[F32 || QLDS ? 1 : NQ][HD / 32];
+  u4 qh[F32 || QLDS ? 1 : NQ][HD / 32], ql[F32 || QLDS || SIDE ? 1 : NQ][HD / 32];
   u4 *const qs = reinterpret_cast<u4 *>(sm_acc) + wave * (QW / 4) + lane;
   // the two parts of step i of query tile q
   auto query = [&](int q, int i, int part) -> h8 {
@@ -639,8 +669,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
   f4 qx[NQ][HD / 16];  // as loaded, before the keys and values are on their way
 #pragma unroll
   for (int q = 0; q < NQ; q++) {
-    const int r = first + (wq * NQ + q) * 16 + n16;
-    live[q] = r < rows_in;
+    const int r = first + (wq * NQ + q) * 16 + (SIDE ? n16 & 7 : n16);
+    live[q] = r < rows_in && (!SIDE || n16 < 8);
     qrow[q] = std::min(r, rows_in - 1);
     qt[q] = shape.drafted(qrow[q]);
     const char *p = reinterpret_cast<const char *>(
@@ -695,7 +725,10 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
           h[e] = hi;
           l[e] = lo;
         }
-        if constexpr (QLDS) {
+        if constexpr (SIDE) {
+#pragma unroll
+          for (int e = 0; e < 4; e++) qh[q][i][e] = n16 < 8 ? h[e] : l[e];
+        } else if constexpr (QLDS) {
           qs[(q * (HD / 32) + i) * 2 * 64] = h;
           qs[((q * (HD / 32) + i) * 2 + 1) * 64] = l;
         } else {
@@ -778,14 +811,21 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
           const h8 A = __builtin_bit_cast(h8, ka);
 #pragma unroll
           for (int q = 0; q < NQ; q++) {
-            st[q][t] =
-                __builtin_amdgcn_mfma_f32_16x16x32_f16(A, query(q, i, 1), st[q][t], 0, 0, 0);
+            if constexpr (!SIDE)
+              st[q][t] =
+                  __builtin_amdgcn_mfma_f32_16x16x32_f16(A, query(q, i, 1), st[q][t], 0, 0, 0);
             st[q][t] =
                 __builtin_amdgcn_mfma_f32_16x16x32_f16(A, query(q, i, 0), st[q][t], 0, 0, 0);
           }
         }
     }
     if constexpr (SC) __builtin_amdgcn_s_setprio(0);
+    if constexpr (SIDE) {
+#pragma unroll
+      for (int t = 0; t < NS; t++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) st[0][t][r] += dpp_f<kRowRor8>(st[0][t][r]);
+    }
     f4 ks[2], vs[2];
     if constexpr (SC) {
 #pragma unroll
@@ -900,7 +940,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
         for (int e = 0; e < 4; e++) {
           uint32_t hi, lo;
           split2(w[q][2 * e], w[q][2 * e + 1], hi, lo);
-          hi4[e] = hi;
+          hi4[e] = SIDE && n16 >= 8 ? lo : hi;
           lo4[e] = lo;
         }
         ph[q] = __builtin_bit_cast(h8, hi4);
@@ -934,7 +974,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
         const h8 A = __builtin_bit_cast(h8, va);
 #pragma unroll
         for (int q = 0; q < NQ; q++) {
-          acc[q][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, pl[q], acc[q][c], 0, 0, 0);
+          if constexpr (!SIDE)
+            acc[q][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, pl[q], acc[q][c], 0, 0, 0);
           acc[q][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, ph[q], acc[q][c], 0, 0, 0);
         }
       }
@@ -957,6 +998,12 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
     for (; tile < tile1; tile += WK) step(raw, tile, std::false_type());
   }
 
+  if constexpr (SIDE) {
+#pragma unroll
+    for (int c = 0; c < C; c++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) acc[0][c][r] += dpp_f<kRowRor8>(acc[0][c][r]);
+  }
   // what the outputs are still to be multiplied with; whether any is NaN (or, as
   // good, infinite)
   float scale[NQ];
@@ -989,18 +1036,21 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
 #pragma unroll 1
         for (int j = at * T; j < std::min(at * T + T, cut.end); j++) {
           const Place at_pos = place(j);
-          const float kd = SC ? load<float>(at_pos.ks, 0) : 1.f;
-          const float vd = SC ? load<float>(at_pos.vs, 0) : 1.f;
+          const int64_t four = at_pos.page + 4 * at_pos.row;
+          const float kd = SC ? load<float>(ksc, four) : 1.f;
+          const float vd = SC ? load<float>(vsc, four) : 1.f;
           auto value = [&](const char *base, const char *steps, int e) {
-            if constexpr (F32) return load<float>(base, 4 * e);
+            const int64_t off = at_pos.page + at_pos.row * ROW;
+            if constexpr (F32) return load<float>(base, off + 4 * e);
             else if constexpr (Q4)
-              return kv_nibble(load<uint8_t>(base, e >> 1), e & 1, load<uint8_t>(steps, e >> 5));
-            else if constexpr (Q8) return kv_byte(load<uint8_t>(base, e));
-            else return (float)load<_Float16>(base, 2 * e);
+              return kv_nibble(load<uint8_t>(base, off + (e >> 1)), e & 1,
+                               load<uint8_t>(steps, four + (e >> 5)));
+            else if constexpr (Q8) return kv_byte(load<uint8_t>(base, off + e));
+            else return (float)load<_Float16>(base, off + 2 * e);
           };
           float x = 0.f;
 #pragma unroll 1
-          for (int e = 0; e < HD / 4; e++) x = fmaf(p[e], value(at_pos.k, at_pos.kw, C * 4 * g4 + e), x);
+          for (int e = 0; e < HD / 4; e++) x = fmaf(p[e], value(kbase, kst, C * 4 * g4 + e), x);
           x = rows4_sum(x) * kd * a.scale * kLog2e;
           if (!sees(q, j - s.len)) continue;
           if (broken[q]) x = NAN;
@@ -1012,7 +1062,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
 #pragma unroll
             for (int r = 0; r < 4; r++)
               acc[q][c][r] = fmaf(acc[q][c][r], f,
-                                  w * (value(at_pos.v, at_pos.vw, C * (4 * g4 + r) + c) * vd));
+                                  w * (value(vbase, vst, C * (4 * g4 + r) + c) * vd));
           ms = mn;
         }
       m[q] = ms;
@@ -1372,10 +1422,15 @@ void launch(const AttendRows &a, hipStream_t st) {
     hipLaunchKernelGGL((k_attend_few<HD, PAGED>), dim3(blocks), dim3(384), 0, st, a, s.per_kv);
     return;
   }
-  if (s.nq == 1)
-    hipLaunchKernelGGL((k_attend<FMT, HD, 1, PAGED>), dim3(blocks), dim3(kThreads), 0, st, a, s);
+  // (4 bits, whose conversions leave the matrix instructions no time beside them; the others
+  // keep the order of their sums)
+  constexpr bool SIDE = FMT == Q3H_KV_Q4;
+  if (SIDE && a.kv.rows * s.per_kv <= 8)
+    hipLaunchKernelGGL((k_attend<FMT, HD, 1, PAGED, SIDE>), dim3(blocks), dim3(kThreads), 0, st, a, s);
+  else if (s.nq == 1)
+    hipLaunchKernelGGL((k_attend<FMT, HD, 1, PAGED, false>), dim3(blocks), dim3(kThreads), 0, st, a, s);
   else
-    hipLaunchKernelGGL((k_attend<FMT, HD, 2, PAGED>), dim3(blocks), dim3(kThreads), 0, st, a, s);
+    hipLaunchKernelGGL((k_attend<FMT, HD, 2, PAGED, false>), dim3(blocks), dim3(kThreads), 0, st, a, s);
   if (s.shares) {
     const int64_t sets = join_sets(a.kv.sequences, a.kv.rows, a.heads, a.kv.kvh, HD);
     const int side = sets >= 2048 ? 1 : kWaves;

@@ -23,6 +23,7 @@ constexpr int kQuadXor1 = 0xB1;   // quad_perm [1,0,3,2]
 constexpr int kQuadXor2 = 0x4E;   // quad_perm [2,3,0,1]
 constexpr int kHalfMirror = 0x141;
 constexpr int kRowMirror = 0x140;
+constexpr int kRowRor8 = 0x128;   // row_ror:8
 constexpr int kBcast15 = 0x142;
 constexpr int kBcast31 = 0x143;
 
