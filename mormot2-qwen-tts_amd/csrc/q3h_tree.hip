@@ -91,10 +91,14 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // kernel joins. shares: of a short call no group is cut; blocks: workgroups, of
 // shares those that they may come to; parts: that they may leave; workers: how many
 // shares of much work there are, about: kWorkers, fewer where the parts of so many
-// have no room.
+// have no room. even: the steps of all groups, one behind the other, are cut into
+// shares that differ by a step at most, so that a share may end one group and begin the
+// next (of 4 bits and up to 16 query rows of a kv head, a group a head): the workgroups
+// end together whatever the lengths (32 rows over 1024 .. 4096 positions each 36.7 -> EVEN
+// us, 64 over 4000 .. 16000 216 -> EVEN).
 struct Shape {
   int nq, group, blocks, parts;
-  bool shares;
+  bool shares, even;
   int per_kv;       // query heads of a kv head
   uint32_t by_kv;   // ceil(2^32 / per_kv)
   int workers;
@@ -165,6 +169,17 @@ __device__ __forceinline__ int share_steps(uint32_t groups, uint32_t steps, uint
   const uint32_t n = std::max(w - std::min(groups / 2, w / 2), w / 2);
   return (int)std::max(1u, (steps + n - 1) / n);
 }
+// how many even shares: as share_steps
+__device__ __forceinline__ int even_shares(uint32_t groups, uint32_t steps, uint32_t workers) {
+  return (int)std::min(steps, steps <= workers / 2 * (groups < 16 ? 7 : 4) ? workers / 2 : workers);
+}
+__device__ __forceinline__ int share_start(int i, int shares, int steps) {
+  return (int)((uint64_t)(uint32_t)steps * (uint32_t)i / (uint32_t)shares);
+}
+// the share that step x is in
+__device__ __forceinline__ int share_of(int x, int shares, int steps) {
+  return (int)(((uint64_t)((uint32_t)x + 1) * (uint32_t)shares - 1) / (uint32_t)steps);
+}
 __device__ __forceinline__ KvSeq lane_sequence(const KvSeq &x, int l) {
   KvSeq s;
   const uint64_t p = reinterpret_cast<uint64_t>(x.k0);
@@ -185,10 +200,14 @@ struct Parts {
   float *out;
   float2 *ml;
   int32_t *before, *head, *most;  // [sequences], [sequences], [1]
+  // (even shares: the steps before each sequence, and of one of its heads; how many
+  // shares there are, and of how many steps; of share i parts 2 i, which continues a
+  // group, and 2 i + 1, which begins one)
 };
 inline size_t parts_bytes(const Shape &s, int sequences, int hd) {
   if (!s.shares) return 0;
-  return sizeof(float) * s.parts * s.group * (hd + 2) + sizeof(int32_t) * (2 * (size_t)sequences + 1);
+  return sizeof(float) * s.parts * s.group * (hd + 2) +
+         sizeof(int32_t) * (2 * (size_t)sequences + (s.even ? 2 : 1));
 }
 __device__ __forceinline__ Parts parts_of(const AttendRows &a, const Shape &s, int hd) {
   Parts p;
@@ -307,23 +326,73 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
   const int lane = tid & 63;
   // the workgroup's share: steps step0 .. step1 - 1 of group `first` of kv head g
   // of sequence b; whole: all of the group's, else they leave part `slot`
+  constexpr bool EVEN = Q4 && NQ == 1;
   int b, g, first, step0 = 0, step1 = 0, slot = 0;
   KvSeq s;
   bool whole = true;
   const int n = a.kv.sequences;
+  // (even shares: its steps that are left, of all; 64 sequences' in the lanes)
+  [[maybe_unused]] int even0 = 0, even1 = 0, even_base = 0, even_before = 0, even_upto = 0;
+  KvSeq mine;
+  [[maybe_unused]] Head even_head{0, 0, 0, 0};
+  auto head_at = [&](int i, int most) {
+    if (most == 1 || n > 64) mine = kv_sequence(a.kv, std::min(i, n - 1));
+    return i < n ? head_of(a, mine, shape, T, most) : Head{0, 0, 0, 0};
+  };
+  auto even_load = [&](int base, int before) {
+    even_base = base;
+    even_head = head_at(base + lane, 1);
+    even_upto = before + lane_sums(even_head.steps) * a.kv.kvh;
+    even_before = even_upto - even_head.steps * a.kv.kvh;
+  };
+  // the next piece of the share: the rest of a group, or of the share
+  auto even_next = [&] {
+    while (__builtin_amdgcn_readlane(even_upto, 63) <= even0)
+      even_load(even_base + 64, __builtin_amdgcn_readlane(even_upto, 63));
+    const int f = __builtin_ctzll(__ballot(even_upto > even0));
+    b = even_base + f;
+    s = lane_sequence(mine, f);
+    const int at = even0 - __builtin_amdgcn_readlane(even_before, f);
+    const int own = __builtin_amdgcn_readlane(even_head.steps, f);
+    g = at / own;
+    first = 0;
+    step0 = at - g * own;
+    step1 = std::min(own, step0 + even1 - even0);
+    whole = step1 - step0 == own;
+    slot = 2 * blockIdx.x + (step0 == 0);
+    even0 += step1 - step0;
+  };
   if (!shape.shares) {
     g = blockIdx.x % a.kv.kvh;
     const int bg = blockIdx.x / a.kv.kvh;
     b = bg % n;
     first = bg / n * shape.group;
     s = kv_sequence(a.kv, b);
+  } else if (EVEN) {
+    int groups = 0, steps = 0;
+    for (int base = 0; base < n; base += 64) {
+      even_load(base, steps);
+      groups += __builtin_amdgcn_readlane(lane_sums(even_head.groups), 63) * a.kv.kvh;
+      steps = __builtin_amdgcn_readlane(even_upto, 63);
+      if (blockIdx.x == 0 && tid < 64 && base + lane < n) {
+        const Parts p = parts_of(a, shape, HD);
+        p.before[base + lane] = even_before;
+        p.head[base + lane] = even_head.steps;
+      }
+    }
+    const int shares = even_shares(groups, steps, shape.workers);
+    if (blockIdx.x == 0 && tid == 0) {
+      const Parts p = parts_of(a, shape, HD);
+      p.most[0] = shares;
+      p.most[1] = steps;
+    }
+    if ((int)blockIdx.x >= shares) return;
+    even0 = share_start(blockIdx.x, shares, steps);
+    even1 = share_start(blockIdx.x + 1, shares, steps);
+    if (n > 64) even_load(0, 0);
+    even_next();
   } else {
     // each wave finds it by itself, 64 sequences at a time
-    KvSeq mine;
-    auto head_at = [&](int i, int most) {
-      if (most == 1 || n > 64) mine = kv_sequence(a.kv, std::min(i, n - 1));
-      return i < n ? head_of(a, mine, shape, T, most) : Head{0, 0, 0, 0};
-    };
     Head h{0, 0, 0, 0};
     int groups = 0, steps = 0;
     for (int base = 0; base < n; base += 64) {
@@ -379,9 +448,13 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
       slot += k > 1 ? k : 0;
     }
   }
+  auto piece = [&]() __attribute__((always_inline)) {
   // (as for no share: lengths that change meanwhile)
   if (first >= s.count * per_kv || (!whole && slot >= shape.parts)) return;
-  const int n16 = lane & 15, g4 = lane >> 4;
+  // (even shares: not to be worked out once for all pieces, which costs 70 registers)
+  int own_lane = lane;
+  if constexpr (EVEN) asm volatile("" : "+v"(own_lane));
+  const int n16 = own_lane & 15, g4 = own_lane >> 4;
   const int rows_in = s.count * per_kv;  // query rows of the sequence's kv head
   const size_t row0 = (size_t)b * a.kv.rows;
   if (bad_length(a, s)) {
@@ -555,11 +628,12 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
   constexpr int KI = HD / 32, KN = QLDS ? 2 * KI / kWaves : 1, VN = QLDS ? C / kWaves : 1;
   const bool shared = QLDS && WK == 1;
   u4 *const sm_k = reinterpret_cast<u4 *>(sm + QB) + lane, *const sm_v = sm_k + 2 * KI * 64;
+  // (4 bits: of the values two of a lane's 8 positions, all their elements, so that a
+  // wave makes the factors of those two)
   struct Quarter {
     u4 k[SC ? 1 : KN];
-    uint32_t v[8];
-    uint32_t kw;
-    u4 vw[2];
+    uint32_t v[Q4 ? 2 : 8];
+    uint32_t kw, vw[2];
     f4 ks[2], vs[2];
   };
   auto load_quarter = [&](Quarter &raw, int tile) {
@@ -587,23 +661,33 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
 #pragma unroll
         for (int u = 0; u < KN; u++) raw.k[u] = load<u4>(p + 64 * i, at, 64 * u);
       }
-      const int word = VN * wave >> (Q8 ? 2 : 1);
+      if constexpr (Q4) {
+        const int first = (wave >> 1) * 16 + (wave & 1) * 2;  // (and 4 g4)
 #pragma unroll
-      for (int u = 0; u < 8; u++) {
-        const char *q = at_tile.in(vbase, ROW) + (FULL ? (u >> 2) * 16 * ROW : 0) +
-                        (Q4 ? VN * wave >> 1 : 4 * word);
-        const int j = (FULL ? 0 : (u >> 2) * 16 + (u & 3)) + 4 * g4;
-        const int known = FULL ? (u & 3) * ROW : 0;
-        const uint32_t v =
-            (uint32_t)((FULL ? j : std::min(j, last - j0)) * ROW + n16 * (ROW / 16));
-        if constexpr (Q4) raw.v[u] = load<uint8_t>(q, v, known);
-        else raw.v[u] = load<uint32_t>(q, v, known);
+        for (int u = 0; u < 2; u++) {
+          const int j = FULL ? 4 * g4 : std::min(first + u + 4 * g4, last - j0);
+          const int from = FULL ? first : 0, known = FULL ? u : 0;
+          const uint32_t v = (uint32_t)(j * ROW + n16 * (ROW / 16));
+          if constexpr (HD == 128)
+            raw.v[u] = load<uint32_t>(at_tile.in(vbase, ROW) + from * ROW, v, known * ROW);
+          else
+            raw.v[u] = load<uint16_t>(at_tile.in(vbase, ROW) + from * ROW, v, known * ROW);
+          raw.vw[u] = load<uint32_t>(at_tile.in(vst, 4) + from * 4, (uint32_t)(4 * j), known * 4);
+        }
+      } else {
+        const int word = VN * wave >> (Q8 ? 2 : 1);
+#pragma unroll
+        for (int u = 0; u < 8; u++) {
+          const int j = (u >> 2) * 16 + 4 * g4 + (u & 3);
+          raw.v[u] = load<uint32_t>(
+              at_tile.in(vbase, ROW),
+              (uint32_t)(std::min(j, last - j0) * ROW + n16 * (ROW / 16) + 4 * word));
+        }
       }
       if constexpr (SC) {
         load_fours(at_tile.in(ksc, 4), j0, raw.ks, full);
         load_fours(at_tile.in(vsc, 4), j0, raw.vs, full);
       }
-      if constexpr (Q4) load_fours(at_tile.in(vst, 4), j0, raw.vw, full);
     });
   };
   auto store_quarter = [&](const Quarter &raw) {
@@ -626,23 +710,29 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
       }
       sm_k[(wave * KN + u) * 64] = x;
     }
+    if constexpr (Q4) {
+      const Steps st = steps_f16(raw.vw[1], raw.vw[0], value_sel);
 #pragma unroll
-    for (int u = 0; u < VN; u++) {
-      const int c = VN * wave + u;
-      // (byte or half c of the words)
-      const uint32_t sel = Q8 ? 0x0c040c00u + 0x00010001u * (uint32_t)(c & 3)
-                              : c & 1 ? 0x07060302u : 0x05040100u;
-      u4 x;
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        if constexpr (Q4)
-          x[e] = nibbles_f16(raw.v[2 * e] | raw.v[2 * e + 1] << 16, c & 1,
-                             steps_f16(raw.vw[e >> 1][2 * (e & 1) + 1], raw.vw[e >> 1][2 * (e & 1)],
-                                       value_sel));
-        else if constexpr (Q8) x[e] = bytes_f16(raw.v[2 * e + 1], raw.v[2 * e], sel);
-        else x[e] = __builtin_amdgcn_perm(raw.v[2 * e + 1], raw.v[2 * e], sel);
+      for (int c = 0; c < C; c++) {
+        const uint32_t w =
+            __builtin_amdgcn_perm(raw.v[1], raw.v[0], c & 4 ? 0x07060302u : 0x05040100u);
+        reinterpret_cast<uint32_t *>(sm_v + c * 64)[wave] = nibbles_f16(w, c & 3, st);
       }
-      sm_v[c * 64] = x;
+    } else {
+#pragma unroll
+      for (int u = 0; u < VN; u++) {
+        const int c = VN * wave + u;
+        // (byte or half c of the words)
+        const uint32_t sel = Q8 ? 0x0c040c00u + 0x00010001u * (uint32_t)(c & 3)
+                                : c & 1 ? 0x07060302u : 0x05040100u;
+        u4 x;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          if constexpr (Q8) x[e] = bytes_f16(raw.v[2 * e + 1], raw.v[2 * e], sel);
+          else x[e] = __builtin_amdgcn_perm(raw.v[2 * e + 1], raw.v[2 * e], sel);
+        }
+        sm_v[c * 64] = x;
+      }
     }
   };
   auto barrier = [&] {
@@ -1136,6 +1226,17 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
       *reinterpret_cast<f4u *>(o + e) = x;
     }
   }
+  };
+  if constexpr (EVEN) {
+    for (;;) {
+      piece();
+      if (even0 >= even1) break;
+      even_next();
+      __syncthreads();  // (the waves' meeting place)
+    }
+  } else {
+    piece();
+  }
 }
 
 // One or two query rows of a kv head over an f32 cache, uncut: the f32 matrix
@@ -1293,14 +1394,24 @@ __global__ __launch_bounds__(kThreads) void k_attend_join(AttendRows a, Shape sh
   const int rows_in = s.count * per_kv;
   if (row0 >= rows_in) return;
   const int mine = row0 / shape.group * shape.group;
-  for (int first = 0; first <= mine; first += shape.group) {
-    start += n > 1 ? n : 0;
-    n = (group_steps(a, s, shape, first, rows_in, tile) + most - 1) / most;
+  if (shape.even) {
+    const int steps = parts.most[1], own = parts.head[b];
+    if (start < 0 || own < 1 || start + own > steps || most < 1) return;
+    const int share = share_of(start, most, steps);
+    n = share_of(start + own - 1, most, steps) - share + 1;
+    start = 2 * share;
+    if (n <= 1 || start + 2 * n > shape.parts) return;
+  } else {
+    for (int first = 0; first <= mine; first += shape.group) {
+      start += n > 1 ? n : 0;
+      n = (group_steps(a, s, shape, first, rows_in, tile) + most - 1) / most;
+    }
+    if (n <= 1 || start < 0 || start + n > shape.parts) return;  // (one share: written as it is)
   }
-  if (n <= 1 || start < 0 || start + n > shape.parts) return;  // (one share: written as it is)
   const int sub = lane / (HD / 4), e = lane % (HD / 4) * 4;
   auto part = [&](int i, int r) {
-    return (size_t)(start + i) * shape.group + (std::min(row0 + r, rows_in - 1) - mine);
+    const int at = shape.even ? start + 2 * i + (i == 0) : start + i;
+    return (size_t)at * shape.group + (std::min(row0 + r, rows_in - 1) - mine);
   };
   float M[R], L[R];
   float2 head[R];  // of the first 64 parts
@@ -1366,6 +1477,8 @@ __global__ __launch_bounds__(kThreads) void k_attend_join(AttendRows a, Shape sh
                            (size_t)(g * per_kv + row - t * per_kv) * HD + e) = x / sum;
 }
 
+constexpr int tile_of(int fmt) { return fmt == Q3H_KV_F32 ? 16 : 32; }
+
 // steps of a call at most (a product that can leave 64 bits)
 double steps_upto(int sequences, int rows, int heads, int kvh, int max_len, int tile) {
   return (double)(((int64_t)rows * (heads / kvh) + 15) / 16) * sequences * kvh *
@@ -1373,8 +1486,9 @@ double steps_upto(int sequences, int rows, int heads, int kvh, int max_len, int 
 }
 
 // room: bytes that the parts have
-Shape shape_of(int sequences, int rows, int heads, int kvh, int hd, int max_len, int tile,
+Shape shape_of(int sequences, int rows, int heads, int kvh, int hd, int fmt, int max_len,
                size_t room) {
+  const int tile = tile_of(fmt);
   Shape s;
   s.per_kv = heads / kvh;
   s.by_kv = (uint32_t)(((1ull << 32) + s.per_kv - 1) / s.per_kv);
@@ -1382,6 +1496,7 @@ Shape shape_of(int sequences, int rows, int heads, int kvh, int hd, int max_len,
   s.nq = q_rows > 16 ? 2 : 1;
   const int waves = q_rows > 32 * s.nq ? 4 : q_rows > 16 * s.nq ? 2 : 1;
   s.group = 16 * s.nq * waves;
+  s.even = fmt == Q3H_KV_Q4 && s.nq == 1;
   const int64_t groups = (int64_t)sequences * kvh * ((q_rows + s.group - 1) / s.group);
   const int wk = kWaves / waves;
   const int64_t steps = ((max_len + rows + tile - 1) / tile + wk - 1) / wk;
@@ -1394,14 +1509,15 @@ Shape shape_of(int sequences, int rows, int heads, int kvh, int hd, int max_len,
   for (int w = s.workers = kWorkers; s.shares && w > 0; w -= kWorkers / 16) {
     const int64_t n = std::max<int64_t>(w - groups / 2, w / 2);
     s.workers = w;
-    s.blocks = (int)std::min(n + groups, groups * steps);
+    s.blocks = (int)std::min(s.even ? (int64_t)w : n + groups, groups * steps);
     // n shares of whole steps and one more a group, or twice n: the most of any number
     // of groups up to these is at a third of 2 w
     s.parts = (int)std::min<int64_t>(w + std::min<int64_t>(groups, 2 * w / 3) / 2 + 2, s.blocks);
+    if (s.even) s.parts = 2 * s.blocks;
     if (parts_bytes(s, sequences, hd) <= room) return s;
   }
   // short, or no room for the parts of any cut: whole groups
-  s.shares = false;
+  s.shares = s.even = false;
   s.blocks = (int)groups;
   s.parts = 0;
   return s;
@@ -1415,7 +1531,7 @@ int64_t join_sets(int sequences, int rows, int heads, int kvh, int hd) {
 
 template <int FMT, int HD, bool PAGED>
 void launch(const AttendRows &a, hipStream_t st) {
-  const Shape s = shape_of(a.kv.sequences, a.kv.rows, a.heads, a.kv.kvh, HD, a.max_len, kTile<FMT>,
+  const Shape s = shape_of(a.kv.sequences, a.kv.rows, a.heads, a.kv.kvh, HD, FMT, a.max_len,
                            a.room);
   const unsigned blocks = s.blocks;
   if (FMT == Q3H_KV_F32 && !s.shares && a.kv.rows * s.per_kv <= 2) {
@@ -1444,19 +1560,17 @@ void launch(const AttendRows &a, hipStream_t st) {
 
 size_t attend_part_bytes(int sequences, int rows, int heads, int kvh, int hd, int fmt,
                          int max_len) {
-  return parts_bytes(shape_of(sequences, rows, heads, kvh, hd, max_len, fmt == Q3H_KV_F32 ? 16 : 32,
-                              SIZE_MAX),
-                     sequences, hd);
+  return parts_bytes(shape_of(sequences, rows, heads, kvh, hd, fmt, max_len, SIZE_MAX), sequences, hd);
 }
 
 bool attend_fits(int sequences, int rows, int heads, int kvh, int hd, int fmt, int max_len) {
   const int64_t per_kv = heads / kvh, most = (int64_t)1 << 32;  // threads of a launch: below
-  const int tile = fmt == Q3H_KV_F32 ? 16 : 32;
+  const int tile = tile_of(fmt);
   // (steps in 32 bits, and with them groups and shares)
   if (rows * per_kv * per_kv >= most ||
       steps_upto(sequences, rows, heads, kvh, max_len, tile) > 0x1p30)
     return false;
-  const Shape s = shape_of(sequences, rows, heads, kvh, hd, max_len, tile, SIZE_MAX);
+  const Shape s = shape_of(sequences, rows, heads, kvh, hd, fmt, max_len, SIZE_MAX);
   return (int64_t)s.blocks * 512 < most &&
          (!s.shares || join_sets(sequences, rows, heads, kvh, hd) * 64 + kThreads < most);
 }
