@@ -53,13 +53,14 @@ __device__ __forceinline__ int byte_of(float x, float d, double inv) {
   return min(127, max(-127, (int)q)) + 128;
 }
 
-// rint(x / d) within -7 .. 7, + 8: an element of the 4-bit format (d: its group's step
-// times the row's scale), the quotient as byte_of takes it
-__device__ __forceinline__ uint32_t nibble_of(float x, double d, double inv) {
-  const double y = (double)x * inv;
-  double q = rint(y);
-  if (fabs(y - q) > 0.5 - 1e-6) q = rint((double)x / d);
-  return (uint32_t)(min(7, max(-7, (int)q)) + 8);
+// rint(x / (step d)) within -7 .. 7, + 8: an element of the 4-bit format. The quotient in
+// 32 bits, by a reciprocal (two roundings and an ulp off, 2^-22 of at most 7.5), in 64
+// where that could cross a half, or has left f32.
+__device__ __forceinline__ uint32_t nibble_of(float x, int step, float d, float inv) {
+  const float y = x * inv;
+  float q = rintf(y);
+  if (!(fabsf(y - q) < 0.5f - 4e-6f)) q = (float)rint((double)x / (step * (double)d));
+  return step > 0 ? (uint32_t)(min(7, max(-7, (int)q)) + 8) : 8u;
 }
 // the step of a group whose largest is m in a row of scale d: the least whole number of d
 // that 7 of reach m (255 at most)
@@ -89,7 +90,8 @@ __device__ __forceinline__ int step_of(float m, float d) {
 // int8 7.4 us, which are a launch, the path through the parents and three loads that
 // wait for each other (length, angles, rows).
 constexpr int kHeads = 2, kManyRows = 1024;
-template <int FMT, int HD, bool ODD, bool MANY>
+// PLACED: pages, or positions of several axes (their branches cost the others 4 %).
+template <int FMT, int HD, bool ODD, bool MANY, bool PLACED>
 __global__ __launch_bounds__(kThreads) void k_cache_append(AppendRows a) {
   constexpr int G = HD / 8, SIDE = 64 / G;  // lanes of a head, heads side by side
   constexpr int PER = kHeads * SIDE;        // heads of a wave at a time
@@ -98,29 +100,30 @@ __global__ __launch_bounds__(kThreads) void k_cache_append(AppendRows a) {
   const int lane = threadIdx.x & 63, sub = lane & (G - 1), side = lane / G;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int row = blockIdx.x, b = row / a.kv.rows, t = row - b * a.kv.rows;
-  const KvSeq s = kv_sequence(a.kv, b);
+  const KvSeq s = kv_sequence<PLACED>(a.kv, b);
   if (t >= s.count) return;
   int depth = t;
   bool bad = s.len < 0 || s.len > s.max_pos - s.count;
   // where the row goes; a page that another sequence holds too is not written to
   int at_pos = s.len + t;
   KvSeq place = s;
-  if (a.kv.table && !bad) {
-    const int page = kv_page(a.kv, b, at_pos >> a.kv.page_log2);
-    place.k0 = a.kv.base + page * a.kv.seq_bytes;
-    place.max_pos = 1 << a.kv.page_log2;
-    at_pos &= place.max_pos - 1;
-    bad = a.kv.refs[page] > 1;
-  }
-  // its positions on the axes
-  int axis_pos[kMaxAxes] = {};
-  if (a.places) {
+  [[maybe_unused]] int axis_pos[kMaxAxes] = {};  // its positions on the axes
+  if constexpr (PLACED) {
+    if (a.kv.table && !bad) {
+      const int page = kv_page(a.kv, b, at_pos >> a.kv.page_log2);
+      place.k0 = a.kv.base + page * a.kv.seq_bytes;
+      place.max_pos = 1 << a.kv.page_log2;
+      at_pos &= place.max_pos - 1;
+      bad = a.kv.refs[page] > 1;
+    }
+    if (a.places) {
 #pragma unroll
-    for (int i = 0; i < kMaxAxes; i++)
-      if (i < a.n_axes) {
-        axis_pos[i] = a.places[(size_t)i * a.kv.sequences * a.kv.rows + row];
-        bad = bad || (uint32_t)axis_pos[i] >= (uint32_t)a.table_positions;
-      }
+      for (int i = 0; i < kMaxAxes; i++)
+        if (i < a.n_axes) {
+          axis_pos[i] = a.places[(size_t)i * a.kv.sequences * a.kv.rows + row];
+          bad = bad || (uint32_t)axis_pos[i] >= (uint32_t)a.table_positions;
+        }
+    }
   }
   if (a.parents) {
     const Path path = tree_path(a.parents + (size_t)b * a.kv.rows, a.kv.rows);
@@ -157,7 +160,7 @@ __global__ __launch_bounds__(kThreads) void k_cache_append(AppendRows a) {
     cs[i] = make_double2(1.0, 0.0);
     if (p < half && !bad) {
       int pos = s.len + depth;
-      if (a.places) {
+      if (PLACED && a.places) {
         const uint32_t axis = (uint32_t)(a.axes[p >> 5] >> (2 * (p & 31))) & 3u;
         pos = axis_pos[0];
 #pragma unroll
@@ -291,62 +294,92 @@ __global__ __launch_bounds__(kThreads) void k_cache_append(AppendRows a) {
       }
     }
     const int e_a = values ? 4 * sub : ea, e_b = values ? HD / 2 + 4 * sub : eb;
-    // the 4-bit format: the heads' scales and their groups' steps, lane u * NG + i of a head
-    // those of group i of the u-th one
+    // the 4-bit format: the heads' scales and their groups' steps. Where four neighbours of
+    // a half of a head are with a lane, a group is with 8 lanes, a each and b each, and
+    // lane 2 u + w of them makes the step of the u-th head's a (w 0) or b; elsewhere lane
+    // u * NG + i of a head that of group i.
     constexpr int NG = HD / 32;
-    int step = 0;
-    double step_inv = 0.0;
+    [[maybe_unused]] const bool even = values || !split || a.rot_dim == HD;
+    [[maybe_unused]] int step = 0;
     if constexpr (FMT == Q3H_KV_Q4) {
       if (values || (group + 1) * PER > a.heads) {
         float mine = 0.f, dm = 0.f;
 #pragma unroll
         for (int u = 0; u < kHeads; u++) {
-          float m[NG], most = 0.f;
+          float quad[2];
           bool finite = true;
 #pragma unroll
-          for (int i = 0; i < 8; i++) finite = finite && fabsf(x[u][i]) < INFINITY;
+          for (int w = 0; w < 2; w++) {
+            quad[w] = 0.f;
 #pragma unroll
-          for (int i = 0; i < NG; i++) {
-            m[i] = finite ? 0.f : INFINITY;
-#pragma unroll
-            for (int k = 0; k < 8; k++) {
-              const int at = ODD && !values ? e[ODD ? k : 0] : k < 4 ? e_a : e_b;
-              m[i] = fmaxf(m[i], at >> 5 == i ? fabsf(x[u][k]) : 0.f);
+            for (int i = 4 * w; i < 4 * w + 4; i++) {
+              finite = finite && fabsf(x[u][i]) < INFINITY;
+              quad[w] = fmaxf(quad[w], fabsf(x[u][i]));
             }
-            m[i] = head_max<G>(m[i]);
-            most = fmaxf(most, m[i]);
           }
-          d[u] = most;
-#pragma unroll
-          for (int i = 0; i < NG; i++)
-            if (sub == u * NG + i) {
-              mine = m[i];
-              dm = most;
+          if (!finite) quad[0] = INFINITY;
+          if (!ODD && even) {
+            const float ma = head_max<8>(quad[0]), mb = head_max<8>(quad[1]);
+            d[u] = fmaxf(ma, mb);
+            if (G == 16) d[u] = fmaxf(d[u], dpp_f_keep<kRowRor8>(d[u]));
+            if ((sub & 7) >> 1 == u) {
+              mine = sub & 1 ? mb : ma;
+              dm = d[u];
             }
+          } else {
+            float m[NG];
+            d[u] = 0.f;
+#pragma unroll
+            for (int i = 0; i < NG; i++) {
+              m[i] = finite ? 0.f : INFINITY;
+#pragma unroll
+              for (int k = 0; k < 8; k += ODD ? 1 : 4) {
+                const int at = ODD && !values ? e[ODD ? k : 0] : k < 4 ? e_a : e_b;
+                m[i] = fmaxf(m[i], at >> 5 == i ? (ODD && !values ? fabsf(x[u][k]) : quad[k / 4]) : 0.f);
+              }
+              m[i] = head_max<G>(m[i]);
+              d[u] = fmaxf(d[u], m[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < NG; i++)
+              if (sub == u * NG + i) {
+                mine = m[i];
+                dm = d[u];
+              }
+          }
         }
         const float scale = dm == INFINITY ? NAN : (float)((double)dm / 1785.0);
         step = step_of(mine, scale);
-        step_inv = 1.0 / (step * (double)scale);
 #pragma unroll
-        for (int u = 0; u < kHeads; u++) d[u] = __shfl(scale, side * G + u * NG);
+        for (int u = 0; u < kHeads; u++)
+          d[u] = __shfl(scale, side * G + (!ODD && even ? 2 * u : u * NG));
       }
     }
 #pragma unroll
     for (int u = 0; u < kHeads; u++) {
-      uint32_t steps = 0, nib[8];
+      [[maybe_unused]] uint32_t steps = 0, nib[8];
       if constexpr (FMT == Q3H_KV_Q4) {
         if (values || (group + 1) * PER > a.heads) {
-          const int from = side * G + u * NG;
+          if (!ODD && even) {
 #pragma unroll
-          for (int i = 0; i < NG; i++) steps |= (uint32_t)__shfl(step, from + i) << (8 * i);
+            for (int w = 0; w < 2; w++) {
+              const int n = __shfl(step, (lane & ~7) + 2 * u + w);
+              const float inv = __builtin_amdgcn_rcpf(n * d[u]);
 #pragma unroll
-          for (int i = 0; i < 8; i += ODD ? 1 : 4) {
-            const int g = (ODD && !values ? e[ODD ? i : 0] : i < 4 ? e_a : e_b) >> 5;
-            const double by = __shfl(step_inv, from + g);
-            const int n = (int)(steps >> (8 * g) & 255u);
+              for (int i = 4 * w; i < 4 * w + 4; i++) nib[i] = nibble_of(x[u][i], n, d[u], inv);
+              steps |= (uint32_t)n << (w * (NG / 2) * 8);
+            }
+            if (G == 16) steps |= (uint32_t)dpp_i<kRowRor8>((int)steps, 0) << 8;
+          } else {
+            const int from = side * G + u * NG;
 #pragma unroll
-            for (int k = i; k < (ODD ? i + 1 : i + 4); k++)
-              nib[k] = n > 0 ? nibble_of(x[u][k], n * (double)d[u], by) : 8u;
+            for (int i = 0; i < NG; i++) steps |= (uint32_t)__shfl(step, from + i) << (8 * i);
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+              const int g = (ODD && !values ? e[ODD ? i : 0] : i < 4 ? e_a : e_b) >> 5;
+              const int n = (int)(steps >> (8 * g) & 255u);
+              nib[i] = nibble_of(x[u][i], n, d[u], __builtin_amdgcn_rcpf(n * d[u]));
+            }
           }
         }
       }
@@ -435,7 +468,7 @@ __global__ __launch_bounds__(kThreads) void k_cache_append(AppendRows a) {
 // past the caches: with 8 neighbouring elements a thread, half of each line an
 // instruction, 57.8 us; through the caches 51.5. One row a thread 37.1, four 34.6.
 constexpr int kReadRows = 2;
-template <int FMT, int HD>
+template <int FMT, int HD, bool PAGED>
 __global__ __launch_bounds__(kThreads) void k_cache_read(KvView kv, const int32_t *starts,
                                                          float *k, float *v) {
   constexpr int PER = HD / 4, SIDE = kThreads / PER;  // threads of a row, rows side by side
@@ -463,20 +496,20 @@ __global__ __launch_bounds__(kThreads) void k_cache_read(KvView kv, const int32_
     const int b = b0 + (int)over, t = (int)(t0 + pos - over * kv.rows);
     const int in = min(b, kv.sequences - 1);
     KvSeq s;
-    s.k0 = kv.base + (kv.table ? 0 : in * kv.seq_bytes);
-    s.max_pos = kv.table ? kv_room(kv, in) : kv.max_pos;
+    s.k0 = kv.base + (PAGED ? 0 : in * kv.seq_bytes);
+    s.max_pos = PAGED ? kv_room(kv, in) : kv.max_pos;
     s.len = starts ? starts[in] : 0;
     s.count = kv.counts ? min(max(kv.counts[in], 0), kv.rows) : kv.rows;
     there[u] = b < kv.sequences && t < s.count;
     bad[u] = s.len < 0 || s.len > s.max_pos - s.count;
     // (no such row: the first one, which is there, if only as page 0)
     int p = there[u] && !bad[u] ? s.len + t : 0;
-    s = kv_place(kv, s, in, p);
+    if constexpr (PAGED) s = kv_place(kv, s, in, p);
     at[u] = kv_row(kv, s, 0, there[u] ? (int)g : 0, p);
     base[u] = s.k0;
   }
   const int64_t values =
-      (int64_t)kv.layers * kv.kvh * (kv.table ? 1 << kv.page_log2 : kv.max_pos);
+      (int64_t)kv.layers * kv.kvh * (PAGED ? 1 << kv.page_log2 : kv.max_pos);
 #pragma unroll
   for (int part = 0; part < 2; part++) {
     float *dst = part ? v : k;
@@ -516,11 +549,11 @@ __global__ __launch_bounds__(kThreads) void k_cache_read(KvView kv, const int32_
 // in ascending order, each to a position at or before its own that no later
 // row comes from, so one row after another is enough; a 4-byte word of a row a
 // thread (HD = 64 int8: 16 words), the rest of the threads on the scale.
-template <int FMT, int HD>
+template <int FMT, int HD, bool PAGED>
 __global__ __launch_bounds__(128) void k_cache_keep(KvView kv, const int32_t *kept) {
   constexpr int ROW = kv_row_bytes(FMT, HD), WORDS = ROW / 4;
   const int b = blockIdx.x, tid = threadIdx.x;
-  const KvSeq s = kv_sequence(kv, b);
+  const KvSeq s = kv_sequence<PAGED>(kv, b);
   const int n = kv.counts[b];
   if (n < 1 || n > kv.rows || s.len < 0) return;
   const int32_t *list = kept + (size_t)b * kv.rows;
@@ -533,7 +566,7 @@ __global__ __launch_bounds__(128) void k_cache_keep(KvView kv, const int32_t *ke
   }
   if (s.len >= s.max_pos - last) return;
   // (no row goes to a page that another sequence holds too)
-  if (kv.table)
+  if constexpr (PAGED)
     for (int at = s.len >> kv.page_log2; at <= (s.len + n - 1) >> kv.page_log2; at++)
       if (kv.refs[kv_page(kv, b, at)] > 1) return;
   const int layer = blockIdx.y / (2 * kv.kvh), lg = blockIdx.y - layer * 2 * kv.kvh;
@@ -545,7 +578,7 @@ __global__ __launch_bounds__(128) void k_cache_keep(KvView kv, const int32_t *ke
   };
   auto row = [&](int i) {
     int p = s.len + i;
-    const KvSeq place = kv_place(at, s, b, p);
+    const KvSeq place = PAGED ? kv_place(at, s, b, p) : s;
     const int64_t r = kv_row(at, place, part, g, p);
     return Row{reinterpret_cast<uint32_t *>(place.k0) + r * WORDS,
                reinterpret_cast<uint32_t *>(kv_scales(at, place, ROW)) + r,
@@ -589,8 +622,7 @@ __global__ void k_scaled_fill(const float *src, char *k0, int part, int layers, 
     for (int e = 0; e < HD / 64; e++) {
       const int step = step_of(half_max_dpp(fabsf(x[e])), d);
       steps |= ((uint32_t)__shfl(step, 0) | (uint32_t)__shfl(step, 32) << 8) << (16 * e);
-      const double by = step * (double)d;
-      const uint32_t n = step > 0 ? nibble_of(x[e], by, 1.0 / by) : 8u;
+      const uint32_t n = nibble_of(x[e], step, d, __builtin_amdgcn_rcpf(step * d));
       const uint32_t next = (uint32_t)dpp_i<kQuadXor1>((int)n, 0);
       if (lane % 2 == 0)
         reinterpret_cast<uint8_t *>(k0)[at * (HD / 2) + 32 * e + lane / 2] = (uint8_t)(n | next << 4);
@@ -666,27 +698,38 @@ struct GoAppend {
     const int rows = a.kv.sequences * a.kv.rows;
     const int side = rows >= kManyRows ? 1 : (groups + kThreads / 64 - 1) / (kThreads / 64);
     const dim3 grid(rows, side);
+    if (a.kv.table || a.places) launch<true>(a, rows, grid, st);
+    else launch<false>(a, rows, grid, st);
+  }
+  template <bool PLACED>
+  static void launch(const AppendRows &a, int rows, dim3 grid, hipStream_t st) {
     if ((a.table || a.table32) && a.rot_dim % 8 != 0)
-      hipLaunchKernelGGL((k_cache_append<FMT, HD, true, false>), grid, dim3(kThreads), 0, st, a);
+      hipLaunchKernelGGL((k_cache_append<FMT, HD, true, false, PLACED>), grid, dim3(kThreads), 0, st, a);
     else if (rows >= kManyRows)
-      hipLaunchKernelGGL((k_cache_append<FMT, HD, false, true>), grid, dim3(kThreads), 0, st, a);
+      hipLaunchKernelGGL((k_cache_append<FMT, HD, false, true, PLACED>), grid, dim3(kThreads), 0, st, a);
     else
-      hipLaunchKernelGGL((k_cache_append<FMT, HD, false, false>), grid, dim3(kThreads), 0, st, a);
+      hipLaunchKernelGGL((k_cache_append<FMT, HD, false, false, PLACED>), grid, dim3(kThreads), 0, st, a);
   }
 };
 template <int FMT, int HD>
 struct GoRead {
   static void go(const KvView &kv, const int32_t *starts, float *k, float *v, hipStream_t st) {
     const int64_t n = (int64_t)kv.sequences * kv.rows * kv.kvh, per = kReadRows * kThreads / (HD / 4);
-    hipLaunchKernelGGL((k_cache_read<FMT, HD>), dim3((unsigned)((n + per - 1) / per)),
-                       dim3(kThreads), 0, st, kv, starts, k, v);
+    const dim3 grid((unsigned)((n + per - 1) / per));
+    if (kv.table)
+      hipLaunchKernelGGL((k_cache_read<FMT, HD, true>), grid, dim3(kThreads), 0, st, kv, starts, k, v);
+    else
+      hipLaunchKernelGGL((k_cache_read<FMT, HD, false>), grid, dim3(kThreads), 0, st, kv, starts, k, v);
   }
 };
 template <int FMT, int HD>
 struct GoKeep {
   static void go(const KvView &kv, const int32_t *kept, hipStream_t st) {
-    hipLaunchKernelGGL((k_cache_keep<FMT, HD>), dim3(kv.sequences, kv.layers * 2 * kv.kvh),
-                       dim3(128), 0, st, kv, kept);
+    const dim3 grid(kv.sequences, kv.layers * 2 * kv.kvh);
+    if (kv.table)
+      hipLaunchKernelGGL((k_cache_keep<FMT, HD, true>), grid, dim3(128), 0, st, kv, kept);
+    else
+      hipLaunchKernelGGL((k_cache_keep<FMT, HD, false>), grid, dim3(128), 0, st, kv, kept);
   }
 };
 

@@ -76,6 +76,8 @@ __device__ __forceinline__ int kv_page(const KvView &v, int b, int at) {
   const int page = v.table[(size_t)b * v.slots + at];
   return (uint32_t)page < (uint32_t)v.pages ? page : 0;
 }
+// (PAGED: the view may be of pages)
+template <bool PAGED>
 __device__ __forceinline__ KvSeq kv_sequence(const KvView &v, int b) {
   KvSeq s;
   if (v.rd) {
@@ -85,8 +87,9 @@ __device__ __forceinline__ KvSeq kv_sequence(const KvView &v, int b) {
     s.len = d.pos;
     s.count = d.pos < 0 ? 0 : v.rows;
   } else {
-    s.k0 = v.base + (v.table ? 0 : b * v.seq_bytes);
-    s.max_pos = v.table ? kv_room(v, b) : v.max_pos;
+    const bool pages = PAGED && v.table;
+    s.k0 = v.base + (pages ? 0 : b * v.seq_bytes);
+    s.max_pos = pages ? kv_room(v, b) : v.max_pos;
     s.len = v.lens[b];
     s.count = v.rows;
   }

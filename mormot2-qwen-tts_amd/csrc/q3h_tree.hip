@@ -336,7 +336,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
   KvSeq mine;
   [[maybe_unused]] Head even_head{0, 0, 0, 0};
   auto head_at = [&](int i, int most) {
-    if (most == 1 || n > 64) mine = kv_sequence(a.kv, std::min(i, n - 1));
+    if (most == 1 || n > 64) mine = kv_sequence<PAGED>(a.kv, std::min(i, n - 1));
     return i < n ? head_of(a, mine, shape, T, most) : Head{0, 0, 0, 0};
   };
   auto even_load = [&](int base, int before) {
@@ -367,7 +367,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
     const int bg = blockIdx.x / a.kv.kvh;
     b = bg % n;
     first = bg / n * shape.group;
-    s = kv_sequence(a.kv, b);
+    s = kv_sequence<PAGED>(a.kv, b);
   } else if (EVEN) {
     int groups = 0, steps = 0;
     for (int base = 0; base < n; base += 64) {
@@ -1267,7 +1267,7 @@ __global__ __launch_bounds__(384) void k_attend_few(AttendRows a, int per_kv) {
   const int lane = threadIdx.x & 63, n16 = lane & 15, g4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int b = blockIdx.x / a.kv.kvh, g = blockIdx.x - b * a.kv.kvh;
-  const KvSeq s = kv_sequence(a.kv, b);
+  const KvSeq s = kv_sequence<PAGED>(a.kv, b);
   const int rows_in = s.count * per_kv;
   if (rows_in < 1) return;
   const size_t row0 = (size_t)b * a.kv.rows;
@@ -1387,7 +1387,7 @@ __global__ __launch_bounds__(kThreads) void k_attend_join(AttendRows a, Shape sh
   const int bg = id / sets, row0 = (id - bg * sets) * R;
   const int b = bg / a.kv.kvh, g = bg - b * a.kv.kvh;
   if (b >= a.kv.sequences) return;
-  const KvSeq s = kv_sequence(a.kv, b);
+  const KvSeq s = kv_sequence<true>(a.kv, b);
   const Parts parts = parts_of(a, shape, HD);
   const int most = *parts.most;
   int start = parts.before[b] + g * parts.head[b], n = 1;
