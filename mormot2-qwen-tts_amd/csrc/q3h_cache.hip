@@ -108,13 +108,13 @@ __global__ __launch_bounds__(kThreads) void k_cache_append(AppendRows a) {
   int at_pos = s.len + t;
   KvSeq place = s;
   [[maybe_unused]] int axis_pos[kMaxAxes] = {};  // its positions on the axes
+  [[maybe_unused]] int page = -1;
   if constexpr (PLACED) {
     if (a.kv.table && !bad) {
-      const int page = kv_page(a.kv, b, at_pos >> a.kv.page_log2);
+      page = kv_page(a.kv, b, at_pos >> a.kv.page_log2);
       place.k0 = a.kv.base + page * a.kv.seq_bytes;
       place.max_pos = 1 << a.kv.page_log2;
       at_pos &= place.max_pos - 1;
-      bad = a.kv.refs[page] > 1;
     }
     if (a.places) {
 #pragma unroll
@@ -174,6 +174,10 @@ __global__ __launch_bounds__(kThreads) void k_cache_append(AppendRows a) {
         cs[i] = make_double2(c.x, c.y);
       }
     }
+  }
+  // (known when the rows are stored: who else holds the page is one trip to memory more)
+  if constexpr (PLACED) {
+    if (page >= 0) bad = bad || a.kv.refs[page] > 1;
   }
   auto load8 = [&](const float *p, float (&x)[8], bool values) {
     if (ODD && !values) {

@@ -9,6 +9,7 @@
 // sequences in their order: the outcome does not depend on how the threads run.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <string>
 
 #include "q3h.h"
@@ -35,11 +36,11 @@ struct Book {
   int32_t *next_held;           // [sequences]
   int32_t *wanted;              // [sequences]
   int32_t *copy_from, *copy_to; // [sequences]
-  int32_t *used, *moves;        // [1], [1]
+  int32_t *used, *moves, *come; // [1] each; come is 0 between calls
   int sequences, slots, pages, page_log2, max_pos;
 };
 __host__ __device__ inline size_t book_words(int sequences, int slots, int pages) {
-  return 2 * (size_t)sequences * slots + 5 * (size_t)sequences + 6 * (size_t)pages + 2;
+  return 2 * (size_t)sequences * slots + 5 * (size_t)sequences + 6 * (size_t)pages + 3;
 }
 Book book_of(const q3h_cache *c) {
   const size_t n = c->cfg.sequences, slots = c->slots, pages = c->pages;
@@ -59,6 +60,7 @@ Book book_of(const q3h_cache *c) {
   k.copy_to = k.copy_from + n;
   k.used = k.copy_to + n;
   k.moves = k.used + 1;
+  k.come = k.used + 2;
   k.sequences = c->cfg.sequences;
   k.slots = c->slots;
   k.pages = c->pages;
@@ -109,37 +111,202 @@ __global__ void k_book_clear(Book k) {
     k.table[i] = i < none ? -1 : i >= low && i < low + k.pages ? kNobody : 0;
 }
 
-// Pages for positions lens .. lens + counts - 1 of the first n sequences. One
-// workgroup, `group` lanes (a power of two) a sequence, a slot each: who writes to
-// which shared page (writers, lowest), how many pages each sequence wants, their sums
-// in order, the lowest free pages in order, who gets which.
-__global__ __launch_bounds__(kBook) void k_reserve(Book k, int n, int rows, const int32_t *lens,
-                                                   const int32_t *counts, int32_t *ok, int group) {
+// what a sequence wants: slots first .. end - 1 to be written to, `held` there
+struct Want {
+  int first, end, held, len;
+  bool bad;
+};
+__device__ __forceinline__ Want want_of(const Book &k, int b, int n, int rows, const int32_t *lens,
+                                        const int32_t *counts) {
+  Want w{0, 0, 0, 0, false};
+  if (b >= n) return w;
+  const int c = counts ? min(max(counts[b], 0), rows) : rows, page = 1 << k.page_log2;
+  w.len = lens[b];
+  w.held = k.held[b];
+  w.bad = w.len < 0 || w.len > k.max_pos - c || w.len > (int64_t)w.held << k.page_log2;
+  if (w.bad || c == 0) return w;
+  w.first = w.len >> k.page_log2;
+  w.end = (w.len + c - 1 + page) >> k.page_log2;
+  return w;
+}
+__device__ __forceinline__ void mark_writer(const Book &k, int p, int b) {
+  change(k.writers + p, 1);
+  __hip_atomic_fetch_min(k.lowest + p, b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void forget(const Book &k, int p) {
+  k.writers[p] = 0;
+  k.lowest[p] = kNobody;
+}
+
+// The rows before lens of a page that is replaced, of one (layer, keys or values, kv
+// head), by a wave, 4 KB at a time.
+template <int FMT, int HD>
+__device__ __forceinline__ void copy_tail(const KvView &v, int page, int from, int to, int rows,
+                                          int section) {
+  constexpr int ROW = kv_row_bytes(FMT, HD), AHEAD = 4;
+  const int lane = threadIdx.x & 63;
+  const int64_t all = 2 * (int64_t)v.layers * v.kvh * page, at = (int64_t)section * page;
+  const char *src = v.base + from * v.seq_bytes;
+  char *dst = v.base + to * v.seq_bytes;
+  const u4 *x = reinterpret_cast<const u4 *>(src + at * ROW);
+  u4 *y = reinterpret_cast<u4 *>(dst + at * ROW);
+  // (a scale a row, and a word of steps)
+  const uint32_t *sx = reinterpret_cast<const uint32_t *>(src + all * ROW) + at;
+  uint32_t *sy = reinterpret_cast<uint32_t *>(dst + all * ROW) + at;
+  const int chunks = rows * (ROW / 16);
+  for (int i = lane; i < chunks; i += AHEAD * 64) {
+    u4 r[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; j++) r[j] = x[min(i + j * 64, chunks - 1)];
+#pragma unroll
+    for (int j = 0; j < AHEAD; j++)
+      if (i + j * 64 < chunks) y[i + j * 64] = r[j];
+  }
+  if constexpr (kv_scaled(FMT))
+    for (int i = lane; i < rows; i += 64) {
+      const uint32_t scale = sx[i], steps = FMT == Q3H_KV_Q4 ? sx[all + i] : 0;
+      sy[i] = scale;
+      if constexpr (FMT == Q3H_KV_Q4) sy[all + i] = steps;
+    }
+}
+
+// The workgroups of a launch that all work out the same from the tables: true for the one
+// that comes last, which alone may change them (the others have read what they need).
+__device__ __forceinline__ bool last_to_come(const Book &k) {
+  __shared__ int sm_last;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const int before = __hip_atomic_fetch_add(k.come, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    sm_last = before == (int)gridDim.x - 1;
+    if (sm_last) *k.come = 0;
+  }
+  __syncthreads();
+  return sm_last;
+}
+
+// Pages for positions lens .. lens + counts - 1 of the first n sequences, where a thread
+// each has a slot (`group` a sequence, a power of two up to 64, 1024 in all): what a thread
+// finds stays in its registers, the writers of shared pages are counted in LDS, and the
+// ranks of the pages taken are sums over the threads. Every workgroup does all that, copies
+// its part of the rows before lens of the pages that are replaced, and the one that came
+// last changes the tables: one launch. Bound by the trips to memory that wait for one
+// another (lengths, table, holders) and the barriers, then by the copies.
+template <int FMT, int HD>
+__global__ __launch_bounds__(kBook) void k_reserve(Book k, KvView v, int n, int rows,
+                                                   const int32_t *lens, const int32_t *counts,
+                                                   int32_t *ok, int group) {
+  constexpr int HASH = 2 * kBook;
+  __shared__ int32_t sm_free[kBook], sm_key[HASH], sm_writers[HASH], sm_lowest[HASH];
+  __shared__ int32_t sm_from[kBook], sm_to[kBook], sm_rows[kBook];
+  const int tid = threadIdx.x, lane = tid & 63, page = 1 << k.page_log2;
+  const int sub = lane & (group - 1), lane0 = lane & ~(group - 1), b = tid / group;
+  const uint64_t lanes = group == 64 ? ~0ull : (1ull << group) - 1;
+  constexpr int EACH = 8;
+  auto is_free = [&](int p0, int i) {
+    const int p = p0 + tid * EACH + i;
+    return p < k.pages && k.refs[min(p, k.pages - 1)] == 0;
+  };
+  int mine[EACH];
+#pragma unroll
+  for (int i = 0; i < EACH; i++) mine[i] = is_free(0, i);
+  const Want w = want_of(k, b, n, rows, lens, counts);
+  const int at = w.first + sub;
+  const bool in = at < w.end, there = in && at < w.held;
+  int32_t *const slot = k.table + (size_t)min(b, n - 1) * k.slots + min(at, k.slots - 1);
+  const int old = there ? *slot : -1, holders = there ? k.refs[old] : 0;
+  const bool shared = holders > 1;
+  bool take = in && !there;
+  if (__syncthreads_or(shared)) {
+    for (int i = tid; i < HASH; i += kBook) {
+      sm_key[i] = -1;
+      sm_writers[i] = 0;
+      sm_lowest[i] = kNobody;
+    }
+    __syncthreads();
+    int h = 0;
+    if (shared) {
+      // (at most 1024 pages for 2048 places)
+      for (h = (int)((uint32_t)old * 2654435761u >> 21);; h = (h + 1) & (HASH - 1)) {
+        const int was = atomicCAS(sm_key + h, -1, old);
+        if (was == -1 || was == old) break;
+      }
+      atomicAdd(sm_writers + h, 1);
+      atomicMin(sm_lowest + h, b);
+    }
+    __syncthreads();
+    // (kept: by the first sequence, if all that hold a page write to it)
+    if (shared) take = sm_writers[h] != holders || sm_lowest[h] != b;
+  }
+  int total, found = 0;
+  const int upto = book_sums(take, total), r = upto - take;
+  // the lowest free pages
+  for (int p0 = 0; p0 < k.pages && found < total; p0 += kBook * EACH) {
+    int free = 0, all;
+#pragma unroll
+    for (int i = 0; i < EACH; i++) {
+      if (p0 > 0) mine[i] = is_free(p0, i);
+      free += mine[i];
+    }
+    int rank = found + book_sums(free, all) - free;
+#pragma unroll
+    for (int i = 0; i < EACH; i++)
+      if (mine[i]) {
+        if (rank < total) sm_free[rank] = p0 + tid * EACH + i;
+        rank++;
+      }
+    found += all;
+  }
+  const uint64_t takes = __ballot(take) >> lane0 & lanes;
+  const int wanted = __popcll(takes), last = __shfl(upto, lane0 + group - 1);
+  const bool gets = wanted == 0 || last <= found;
+  const bool changes = last_to_come(k);  // (a barrier: sm_free is whole)
+  const int fresh = take && gets ? sm_free[r] : -1;
+  if (sub == 0) {
+    // (the group's first lane has the first slot)
+    const int tail = fresh >= 0 && old >= 0 ? w.len & (page - 1) : 0;
+    sm_from[b] = old;
+    sm_to[b] = fresh;
+    sm_rows[b] = tail;
+  }
+  if (changes) {
+    if (fresh >= 0) {
+      *slot = fresh;
+      k.refs[fresh] = 1;
+      if (old >= 0) change(k.refs + old, -1);
+    }
+    if (b < n && sub == 0 && gets && wanted > 0 && w.end > w.held) k.held[b] = w.end;
+    if (ok) {
+      __syncthreads();
+      // (a shared page that it keeps is its own if all others have left it)
+      const uint64_t others =
+          __ballot(shared && fresh < 0 && now(k.refs + old) > 1) >> lane0 & lanes;
+      if (b < n && sub == 0) ok[b] = !w.bad && gets && others == 0;
+    }
+  }
+  __syncthreads();
+  const int sections = 2 * v.layers * v.kvh, waves = gridDim.x * kBookWaves;
+  for (int i = blockIdx.x * kBookWaves + __builtin_amdgcn_readfirstlane(tid >> 6); i < n * sections;
+       i += waves) {
+    const int s = i / sections;
+    if (sm_rows[s] > 0) copy_tail<FMT, HD>(v, page, sm_from[s], sm_to[s], sm_rows[s], i - s * sections);
+  }
+}
+
+// The same of any number of slots: one workgroup, `group` lanes (a power of two) a
+// sequence at a time: who writes to which shared page (writers, lowest), how many pages
+// each sequence wants, their sums in order, the lowest free pages in order, who gets which.
+__global__ __launch_bounds__(kBook) void k_reserve_many(Book k, int n, int rows, const int32_t *lens,
+                                                        const int32_t *counts, int32_t *ok,
+                                                        int group) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int sub = lane & (group - 1), lane0 = lane & ~(group - 1);
   const uint64_t lanes = group == 64 ? ~0ull : (1ull << group) - 1;
   const int page = 1 << k.page_log2;
-  struct Want {
-    int first, end, held, len;  // slots to be written to, those that are there
-    bool bad;
-  };
-  auto want = [&](int b) {
-    Want w{0, 0, 0, 0, false};
-    if (b >= n) return w;
-    const int c = counts ? min(max(counts[b], 0), rows) : rows;
-    w.len = lens[b];
-    w.held = k.held[b];
-    w.bad = w.len < 0 || w.len > k.max_pos - c || w.len > (int64_t)w.held << k.page_log2;
-    if (w.bad || c == 0) return w;
-    w.first = w.len >> k.page_log2;
-    w.end = (w.len + c - 1 + page) >> k.page_log2;
-    return w;
-  };
   // f(sequence, what it wants, slot, whether it is one of those) with all lanes of a wave
   auto each = [&](auto &&f) {
     for (int b0 = 0; b0 < n; b0 += kBook / group) {
       const int b = b0 + tid / group;
-      const Want w = want(b);
+      const Want w = want_of(k, b, n, rows, lens, counts);
       int at = w.first + sub;
       do {
         f(b, w, at, at < w.end);
@@ -151,10 +318,7 @@ __global__ __launch_bounds__(kBook) void k_reserve(Book k, int n, int rows, cons
   each([&](int b, const Want &w, int at, bool in) {
     if (in && at < w.held) {
       const int p = *row(b, at);
-      if (k.refs[p] > 1) {
-        change(k.writers + p, 1);
-        __hip_atomic_fetch_min(k.lowest + p, b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      }
+      if (k.refs[p] > 1) mark_writer(k, p, b);
     }
   });
   __syncthreads();
@@ -244,10 +408,6 @@ __global__ __launch_bounds__(kBook) void k_reserve(Book k, int n, int rows, cons
   __syncthreads();
   // what the call has counted is forgotten; whether a sequence has its pages to itself
   bool shared = false;
-  auto forget = [&](int p) {
-    k.writers[p] = 0;
-    k.lowest[p] = kNobody;
-  };
   each([&](int b, const Want &w, int at, bool in) {
     const bool start = at == w.first + sub;
     if (start) shared = false;
@@ -258,63 +418,89 @@ __global__ __launch_bounds__(kBook) void k_reserve(Book k, int n, int rows, cons
     bool others = false;
     if (there) {
       const int p = *row(b, at);
-      forget(p);
+      forget(k, p);
       others = now(k.refs + p) > 1;
     }
     if (gets && b < n)
       for (int r = before + (start ? sub : wanted); r < before + wanted; r += group)
-        if (k.olds[r] >= 0) forget(k.olds[r]);
+        if (k.olds[r] >= 0) forget(k, k.olds[r]);
     shared = shared || (__ballot(others) >> lane0 & lanes) != 0;
     if (ok && b < n && sub == 0) ok[b] = !w.bad && gets && !shared;
   });
 }
 
-// The rows before lens of the pages that k_reserve replaced: a workgroup a (layer, keys or
-// values, kv head).
 template <int FMT, int HD>
 __global__ __launch_bounds__(kThreads) void k_copy_tails(KvView v, Book k, const int32_t *lens) {
-  constexpr int ROW = kv_row_bytes(FMT, HD);
-  const int b = blockIdx.x;
-  const int from = k.copy_from[b], to = k.copy_to[b];
-  if (from < 0) return;
-  const int page = 1 << k.page_log2, rows = lens[b] & (page - 1);
-  const int64_t all = 2 * (int64_t)v.layers * v.kvh * page, at = (int64_t)blockIdx.y * page;
-  const char *src = v.base + from * v.seq_bytes;
-  char *dst = v.base + to * v.seq_bytes;
-  const u4 *x = reinterpret_cast<const u4 *>(src + at * ROW);
-  u4 *y = reinterpret_cast<u4 *>(dst + at * ROW);
-  for (int i = threadIdx.x; i < rows * (ROW / 16); i += kThreads) y[i] = x[i];
-  if constexpr (kv_scaled(FMT)) {
-    // (a scale each, and a word of steps)
-    const uint32_t *sx = reinterpret_cast<const uint32_t *>(src + all * ROW) + at;
-    uint32_t *sy = reinterpret_cast<uint32_t *>(dst + all * ROW) + at;
-    for (int i = threadIdx.x; i < rows; i += kThreads) {
-      sy[i] = sx[i];
-      if constexpr (FMT == Q3H_KV_Q4) sy[all + i] = sx[all + i];
-    }
-  }
+  const int b = blockIdx.x, from = k.copy_from[b];
+  const int section = blockIdx.y * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (from < 0 || section >= 2 * v.layers * v.kvh) return;
+  const int page = 1 << k.page_log2;
+  copy_tail<FMT, HD>(v, page, from, k.copy_to[b], lens[b] & (page - 1), section);
 }
 
-// A fork's table beside the present one, a workgroup a sequence, and who holds which
-// page from now on; then (k_fork_end) in its place.
+// A fork's table: of few slots by one workgroup, its entries in registers between reading
+// and writing (an assignment may be any, so that none is written before all are read); of
+// more in two launches, the table beside the present one first. 128 sequences of 31 slots FORK
+// us.
+constexpr int kForkEach = 16, kForkSlots = kForkEach * kBook;
+struct Forked {
+  int from, now, held;  // (now < 0: as it is)
+};
+__device__ __forceinline__ Forked forked(const Book &k, int b, const int32_t *sources,
+                                         const int32_t *lens) {
+  Forked f{sources[b], 0, k.held[b]};
+  if (f.from >= 0 && f.from < k.sequences) {
+    const int len = lens[b], held = k.held[f.from];
+    f.now = len < 0 || len > (int64_t)held << k.page_log2
+                ? -1
+                : (int)(((int64_t)len + (1 << k.page_log2) - 1) >> k.page_log2);
+  } else if (f.from != -1) {
+    f.now = -1;
+  }
+  return f;
+}
+__device__ __forceinline__ void hold(const Book &k, int was, int is) {
+  if (is == was) return;
+  if (is >= 0) change(k.refs + is, 1);
+  if (was >= 0) change(k.refs + was, -1);
+}
+__global__ __launch_bounds__(kBook) void k_fork_few(Book k, int n, const int32_t *sources,
+                                                    const int32_t *lens) {
+  __shared__ Forked sm[kBook];
+  const int tid = threadIdx.x;
+  if (tid < n) sm[tid] = forked(k, tid, sources, lens);
+  __syncthreads();
+  int is[kForkEach], was[kForkEach];
+#pragma unroll
+  for (int j = 0; j < kForkEach; j++) {
+    const int i = tid + j * kBook, b = i / k.slots, at = i - b * k.slots;
+    is[j] = was[j] = -1;
+    if (b >= n) continue;
+    const Forked f = sm[b];
+    if (f.now < 0) continue;
+    if (at < f.held) was[j] = k.table[i];
+    if (at < f.now) is[j] = k.table[(size_t)f.from * k.slots + at];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kForkEach; j++) {
+    if (is[j] == was[j]) continue;
+    hold(k, was[j], is[j]);
+    k.table[tid + j * kBook] = is[j];
+  }
+  if (tid < n && sm[tid].now >= 0) k.held[tid] = sm[tid].now;
+}
 __global__ __launch_bounds__(kThreads) void k_fork(Book k, const int32_t *sources,
                                                    const int32_t *lens) {
-  const int b = blockIdx.x, from = sources[b], len = lens[b], held = k.held[b];
-  int n = 0;
-  bool bad = from < -1 || from >= k.sequences;
-  if (!bad && from >= 0) {
-    bad = len < 0 || len > (int64_t)k.held[from] << k.page_log2;
-    n = (int)(((int64_t)len + (1 << k.page_log2) - 1) >> k.page_log2);
-  }
-  if (threadIdx.x == 0) k.next_held[b] = bad ? -1 : n;
-  if (bad) return;
-  const int32_t *row = k.table + (size_t)b * k.slots, *src = k.table + (size_t)max(from, 0) * k.slots;
-  for (int i = threadIdx.x; i < max(n, held); i += kThreads) {
-    const int was = i < held ? row[i] : -1, is = i < n ? src[i] : -1;
+  const int b = blockIdx.x;
+  const Forked f = forked(k, b, sources, lens);
+  if (threadIdx.x == 0) k.next_held[b] = f.now;
+  const int32_t *row = k.table + (size_t)b * k.slots,
+                *src = k.table + (size_t)max(f.from, 0) * k.slots;
+  for (int i = threadIdx.x; f.now >= 0 && i < max(f.now, f.held); i += kThreads) {
+    const int was = i < f.held ? row[i] : -1, is = i < f.now ? src[i] : -1;
     k.next[(size_t)b * k.slots + i] = is;
-    if (is == was) continue;
-    if (is >= 0) change(k.refs + is, 1);
-    if (was >= 0) change(k.refs + was, -1);
+    hold(k, was, is);
   }
 }
 __global__ __launch_bounds__(kThreads) void k_fork_end(Book k) {
@@ -338,57 +524,126 @@ __global__ __launch_bounds__(64) void k_release(Book k, const int32_t *lens) {
   if (threadIdx.x == 0) k.held[b] = n;
 }
 
-// Which pages move: the k-th of those in use behind their number (order) to the k-th
-// free one below it (olds); a mover's new place in moved.
-__global__ __launch_bounds__(kBook) void k_compact(Book k, int32_t *used) {
+// Which pages move: the k-th of those in use behind their number to the k-th free one
+// below it. list(k-th, page, whether it moves); returns the pages in use and how many move.
+constexpr int kScan = 8 * kBook;
+template <class F>
+__device__ __forceinline__ int2 compact_lists(const Book &k, F &&list) {
   const int tid = threadIdx.x;
-  constexpr int EACH = 8;
-  int in_use = 0;
-  for (int p0 = 0; p0 < k.pages; p0 += kBook * EACH) {
+  constexpr int EACH = kScan / kBook;
+  int in_use = 0, held[EACH];
+  for (int p0 = 0; p0 < k.pages; p0 += kScan) {
     int here = 0, all;
 #pragma unroll
     for (int i = 0; i < EACH; i++) {
       const int p = p0 + tid * EACH + i;
-      here += p < k.pages && k.refs[min(p, k.pages - 1)] > 0;
+      held[i] = k.refs[min(p, k.pages - 1)];
+      here += p < k.pages && held[i] > 0;
     }
     book_sums(here, all);
     in_use += all;
   }
   int holes = 0, movers = 0;
-  for (int p0 = 0; p0 < k.pages; p0 += kBook * EACH) {
+  for (int p0 = 0; p0 < k.pages; p0 += kScan) {
     int here = 0, all, kind[EACH];
 #pragma unroll
     for (int i = 0; i < EACH; i++) {
       const int p = p0 + tid * EACH + i;
-      const bool in = p < k.pages, held = k.refs[min(p, k.pages - 1)] > 0;
+      if (k.pages > kScan) held[i] = k.refs[min(p, k.pages - 1)];
       // (a hole counts 1, a mover 2^16: 8192 pages at a time)
-      kind[i] = !in ? 0 : p < in_use ? !held : held ? 1 << 16 : 0;
+      kind[i] = p >= k.pages ? 0 : p < in_use ? held[i] <= 0 : held[i] > 0 ? 1 << 16 : 0;
       here += kind[i];
     }
     const int upto = book_sums(here, all) - here;
     int hole = holes + (upto & 0xffff), mover = movers + (upto >> 16);
 #pragma unroll
     for (int i = 0; i < EACH; i++) {
-      if (kind[i] == 1) k.olds[hole++] = p0 + tid * EACH + i;
-      if (kind[i] == 1 << 16) k.order[mover++] = p0 + tid * EACH + i;
+      if (kind[i] == 1) list(hole++, p0 + tid * EACH + i, false);
+      if (kind[i] == 1 << 16) list(mover++, p0 + tid * EACH + i, true);
     }
     holes += all & 0xffff;
     movers += all >> 16;
   }
+  return make_int2(in_use, movers);
+}
+// the contents of pages from[i] to pages to[i], by `all` threads of a launch
+template <int AHEAD>
+__device__ __forceinline__ void move_pages(char *base, int64_t page_bytes, int moves,
+                                           const int32_t *from, const int32_t *to, int64_t first,
+                                           int64_t step) {
+  const int64_t per = page_bytes / 16, all = moves * per;
+  for (int64_t i = first; i < all; i += AHEAD * step) {
+    u4 x[AHEAD];
+    u4 *dst[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; j++) {
+      const int64_t at = min(i + j * step, all - 1), m = at / per, off = at - m * per;
+      dst[j] = reinterpret_cast<u4 *>(base + to[m] * page_bytes) + off;
+      x[j] = reinterpret_cast<const u4 *>(base + from[m] * page_bytes)[off];
+    }
+#pragma unroll
+    for (int j = 0; j < AHEAD; j++)
+      if (i + j * step < all) *dst[j] = x[j];
+  }
+}
+
+// Up to 8192 pages: every workgroup works out the moves, makes its part of them and of
+// the tables' changes, and the last to come changes who holds which page.
+__global__ __launch_bounds__(kBook) void k_compact(Book k, char *base, int64_t page_bytes,
+                                                   int32_t *used) {
+  __shared__ int32_t sm_hole[kScan / 2], sm_mover[kScan / 2];
+  const int tid = threadIdx.x;
+  // (of as many holes below the number in use as there are movers behind it, at most half
+  // of the pages)
+  const int2 n = compact_lists(k, [&](int i, int p, bool moves) { (moves ? sm_mover : sm_hole)[i] = p; });
+  const int in_use = n.x, moves = n.y;
+  if (last_to_come(k)) {
+    for (int i = tid; i < moves; i += kBook) {
+      k.refs[sm_hole[i]] = k.refs[sm_mover[i]];
+      k.refs[sm_mover[i]] = 0;
+    }
+    if (used && tid == 0) *used = in_use;
+  }
+  if (moves == 0) return;
+  const int lane = tid & 63;
+  const int waves = gridDim.x * kBookWaves;
+  for (int b = blockIdx.x * kBookWaves + (tid >> 6); b < k.sequences; b += waves) {
+    const int held = k.held[b];
+    int32_t *row = k.table + (size_t)b * k.slots;
+    for (int i = lane; i < held; i += 64) {
+      const int p = row[i];
+      if (p < in_use) continue;
+      // (its place among the movers, which are in order)
+      int lo = 0, hi = moves - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (sm_mover[mid] < p) lo = mid + 1;
+        else hi = mid;
+      }
+      row[i] = sm_hole[lo];
+    }
+  }
+  move_pages<4>(base, page_bytes, moves, sm_mover, sm_hole, (int64_t)blockIdx.x * kBook + tid,
+                (int64_t)gridDim.x * kBook);
+}
+
+// Any number of pages: one workgroup for the lists, a mover's new place in moved, then the
+// moves and the tables of the sequences.
+__global__ __launch_bounds__(kBook) void k_compact_many(Book k, int32_t *used) {
+  const int2 n = compact_lists(k, [&](int i, int p, bool moves) { (moves ? k.order : k.olds)[i] = p; });
   __syncthreads();
-  for (int i = tid; i < movers; i += kBook) {
+  for (int i = threadIdx.x; i < n.y; i += kBook) {
     const int from = k.order[i], to = k.olds[i];
     k.moved[from] = to;
     k.refs[to] = k.refs[from];
     k.refs[from] = 0;
   }
-  if (tid == 0) {
-    *k.used = in_use;
-    *k.moves = movers;
-    if (used) *used = in_use;
+  if (threadIdx.x == 0) {
+    *k.used = n.x;
+    *k.moves = n.y;
+    if (used) *used = n.x;
   }
 }
-// the pages' contents, and the tables of the sequences that hold them
 __global__ __launch_bounds__(kThreads) void k_move(Book k, char *base, int64_t page_bytes) {
   const int moves = *k.moves, in_use = *k.used;
   for (int b = blockIdx.x; b < k.sequences && moves > 0; b += gridDim.x) {
@@ -399,22 +654,10 @@ __global__ __launch_bounds__(kThreads) void k_move(Book k, char *base, int64_t p
       if (p >= in_use) row[i] = k.moved[p];
     }
   }
-  constexpr int AHEAD = 4;
-  const int64_t per = page_bytes / 16, all = moves * per, step = (int64_t)gridDim.x * kThreads;
-  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < all; i += AHEAD * step) {
-    u4 x[AHEAD];
-    u4 *to[AHEAD];
-#pragma unroll
-    for (int j = 0; j < AHEAD; j++) {
-      const int64_t at = min(i + j * step, all - 1), m = at / per, off = at - m * per;
-      to[j] = reinterpret_cast<u4 *>(base + k.olds[m] * page_bytes) + off;
-      x[j] = reinterpret_cast<const u4 *>(base + k.order[m] * page_bytes)[off];
-    }
-#pragma unroll
-    for (int j = 0; j < AHEAD; j++)
-      if (i + j * step < all) *to[j] = x[j];
-  }
+  move_pages<4>(base, page_bytes, moves, k.order, k.olds, (int64_t)blockIdx.x * kThreads + threadIdx.x,
+                (int64_t)gridDim.x * kThreads);
 }
+
 // The first lens[b] positions of sequence sources[b] of a cache into sequence b of
 // another. A wave takes runs of 32 positions of a (layer, part, kv head), which lie in
 // one piece on both sides, an equal share of all of them.
@@ -510,9 +753,24 @@ __global__ __launch_bounds__(kThreads) void k_page_state(Book k, int32_t *table,
 }
 
 template <int FMT, int HD>
-struct GoTails {
-  static void go(const KvView &v, const Book &k, const int32_t *lens, hipStream_t st) {
-    hipLaunchKernelGGL((k_copy_tails<FMT, HD>), dim3(v.sequences, 2 * v.layers * v.kvh),
+struct GoReserve {
+  static void go(const Book &k, const KvView &v, int n, int rows, const int32_t *lens,
+                 const int32_t *counts, int32_t *ok, hipStream_t st) {
+    // slots of a sequence that the call can touch, up to 64 lanes
+    const int most = ((rows - 1) >> k.page_log2) + 2, sections = 2 * v.layers * v.kvh;
+    int group = 1;
+    while (group < most && group < 64) group *= 2;
+    if (most <= group && n * group <= kBook) {
+      const int64_t waves = (int64_t)n * sections;
+      const unsigned blocks = (unsigned)std::min<int64_t>(256, (waves + kBookWaves - 1) / kBookWaves);
+      hipLaunchKernelGGL((k_reserve<FMT, HD>), dim3(blocks), dim3(kBook), 0, st, k, v, n, rows, lens,
+                         counts, ok, group);
+      return;
+    }
+    hipLaunchKernelGGL(k_reserve_many, dim3(1), dim3(kBook), 0, st, k, n, rows, lens, counts, ok,
+                       group);
+    const int each = kThreads / 64;
+    hipLaunchKernelGGL((k_copy_tails<FMT, HD>), dim3(n, (sections + each - 1) / each),
                        dim3(kThreads), 0, st, v, k, lens);
   }
 };
@@ -526,11 +784,12 @@ struct GoCopy {
 };
 
 void check_pages(const q3h_cache *c, int sequences, const char *who) {
-  require(c != nullptr, Q3H_E_ARG, std::string(who) + ": NULL cache");
-  require(c->pages > 0, Q3H_E_ARG, std::string(who) + ": not a cache of pages");
-  require(sequences >= 0 && sequences <= c->cfg.sequences, Q3H_E_ARG,
-          std::string(who) + ": " + std::to_string(sequences) + " sequences of a cache of " +
-              std::to_string(c->cfg.sequences));
+  if (!c) require(false, Q3H_E_ARG, std::string(who) + ": NULL cache");
+  if (c->pages <= 0) require(false, Q3H_E_ARG, std::string(who) + ": not a cache of pages");
+  if (sequences < 0 || sequences > c->cfg.sequences)
+    require(false, Q3H_E_ARG,
+            std::string(who) + ": " + std::to_string(sequences) + " sequences of a cache of " +
+                std::to_string(c->cfg.sequences));
 }
 
 }  // namespace
@@ -597,16 +856,9 @@ extern "C" int q3h_cache_reserve(q3h_cache *c, int sequences, int rows, const in
     if (sequences == 0) return;
     require(lens != nullptr, Q3H_E_ARG, "q3h_cache_reserve: NULL lens");
     DeviceScope scope(c->dev->ordinal);
-    // slots of a sequence that the call can touch, up to 64 lanes
-    const int most = ((rows - 1) >> c->page_log2) + 2;
-    int group = 1;
-    while (group < most && group < 64) group *= 2;
-    const Book k = book_of(c);
-    hipStream_t st = (hipStream_t)stream;
-    hipLaunchKernelGGL(k_reserve, dim3(1), dim3(kBook), 0, st, k, sequences, rows, lens, counts, ok,
-                       group);
-    const KvView v = kv_view(c, 0, sequences, rows, lens, counts);
-    by_format<GoTails>(c->cfg.head_dim, c->cfg.format, v, k, lens, st);
+    by_format<GoReserve>(c->cfg.head_dim, c->cfg.format, book_of(c),
+                         kv_view(c, 0, sequences, rows, lens, counts), sequences, rows, lens, counts,
+                         ok, (hipStream_t)stream);
     check_hip(hipGetLastError(), "cache reserve kernels");
   });
 }
@@ -620,8 +872,12 @@ extern "C" int q3h_cache_fork(q3h_cache *c, int sequences, const int32_t *source
     DeviceScope scope(c->dev->ordinal);
     const Book k = book_of(c);
     hipStream_t st = (hipStream_t)stream;
-    hipLaunchKernelGGL(k_fork, dim3(sequences), dim3(kThreads), 0, st, k, sources, lens);
-    hipLaunchKernelGGL(k_fork_end, dim3(sequences), dim3(kThreads), 0, st, k);
+    if (sequences <= kBook && (int64_t)sequences * c->slots <= kForkSlots) {
+      hipLaunchKernelGGL(k_fork_few, dim3(1), dim3(kBook), 0, st, k, sequences, sources, lens);
+    } else {
+      hipLaunchKernelGGL(k_fork, dim3(sequences), dim3(kThreads), 0, st, k, sources, lens);
+      hipLaunchKernelGGL(k_fork_end, dim3(sequences), dim3(kThreads), 0, st, k);
+    }
     check_hip(hipGetLastError(), "cache fork kernels");
   });
 }
@@ -644,9 +900,16 @@ extern "C" int q3h_cache_compact(q3h_cache *c, int32_t *used, void *stream) {
     DeviceScope scope(c->dev->ordinal);
     const Book k = book_of(c);
     hipStream_t st = (hipStream_t)stream;
-    hipLaunchKernelGGL(k_compact, dim3(1), dim3(kBook), 0, st, k, used);
-    hipLaunchKernelGGL(k_move, dim3(2048), dim3(kThreads), 0, st, k, c->data,
-                       (int64_t)c->seq_bytes);
+    const int64_t bytes = (int64_t)c->seq_bytes;
+    if (c->pages <= kScan) {
+      // (half of the pages at most move)
+      const int64_t most = c->pages / 2 * bytes / (64 * kBook);
+      const unsigned blocks = (unsigned)std::min<int64_t>(512, std::max<int64_t>(1, most));
+      hipLaunchKernelGGL(k_compact, dim3(blocks), dim3(kBook), 0, st, k, c->data, bytes, used);
+    } else {
+      hipLaunchKernelGGL(k_compact_many, dim3(1), dim3(kBook), 0, st, k, used);
+      hipLaunchKernelGGL(k_move, dim3(2048), dim3(kThreads), 0, st, k, c->data, bytes);
+    }
     check_hip(hipGetLastError(), "cache compact kernels");
   });
 }
@@ -656,9 +919,10 @@ extern "C" int q3h_cache_copy(q3h_cache *c, const q3h_cache *src, int sequences,
   return guard([&] {
     require(c && src, Q3H_E_ARG, "q3h_cache_copy: NULL cache");
     require(c != src, Q3H_E_ARG, "q3h_cache_copy: a cache into itself");
-    require(sequences >= 0 && sequences <= c->cfg.sequences, Q3H_E_ARG,
-            "q3h_cache_copy: " + std::to_string(sequences) + " sequences of a cache of " +
-                std::to_string(c->cfg.sequences));
+    if (sequences < 0 || sequences > c->cfg.sequences)
+      require(false, Q3H_E_ARG,
+              "q3h_cache_copy: " + std::to_string(sequences) + " sequences of a cache of " +
+                  std::to_string(c->cfg.sequences));
     const q3h_cache_config &f = c->cfg, &g = src->cfg;
     require(c->dev->ordinal == src->dev->ordinal, Q3H_E_ARG,
             "q3h_cache_copy: caches of two devices");

@@ -898,6 +898,11 @@ class Cache:
         self._append, self._read, self._attend = \
             L.q3h_cache_append, L.q3h_cache_read, L.q3h_cache_attend
         self._append_at = L.q3h_cache_append_at
+        self._reserve, self._fork, self._release = \
+            L.q3h_cache_reserve, L.q3h_cache_fork, L.q3h_cache_release
+        self._compact, self._copy, self._page_state = \
+            L.q3h_cache_compact, L.q3h_cache_copy, L.q3h_cache_page_state
+        self._device = _torch.device("cuda", dev.ordinal)
         self._workspace = L.q3h_cache_attend_workspace
         self._destroy = L.q3h_cache_destroy
 
@@ -1004,7 +1009,7 @@ class Cache:
         there were too few; returned."""
         o, i32 = self.dev.ordinal, _torch.int32
         n = lens.shape[0]
-        _check(lib().q3h_cache_reserve(
+        _check(self._reserve(
             self.h, n, rows, _whole(lens, (n,), o, i32, "lens"),
             _whole(counts, (n,), o, i32, "counts"), _whole(ok, (n,), o, i32, "ok"), _stream(o)))
         return ok
@@ -1014,7 +1019,7 @@ class Cache:
         was (-1: nothing), for all b at once; pages are shared."""
         o, i32 = self.dev.ordinal, _torch.int32
         n = sources.shape[0]
-        _check(lib().q3h_cache_fork(
+        _check(self._fork(
             self.h, n, _whole(sources, (n,), o, i32, "sources"),
             _whole(lens, (n,), o, i32, "lens"), _stream(o)))
 
@@ -1022,7 +1027,7 @@ class Cache:
         """Sequence b keeps the pages of its first lens[b] positions (0: none)."""
         o = self.dev.ordinal
         n = lens.shape[0]
-        _check(lib().q3h_cache_release(
+        _check(self._release(
             self.h, n, _whole(lens, (n,), o, _torch.int32, "lens"), _stream(o)))
 
     def compact(self, used=None):
@@ -1030,8 +1035,8 @@ class Cache:
         int32 tensor on the device, made when it is None)."""
         o, i32 = self.dev.ordinal, _torch.int32
         if used is None:
-            used = _torch.empty(1, dtype=i32, device=f"cuda:{o}")
-        _check(lib().q3h_cache_compact(self.h, _whole(used, (1,), o, i32, "used"), _stream(o)))
+            used = _torch.empty(1, dtype=i32, device=self._device)
+        _check(self._compact(self.h, _whole(used, (1,), o, i32, "used"), _stream(o)))
         return used
 
     def copy(self, src, sources, lens):
@@ -1039,20 +1044,23 @@ class Cache:
         none) to sequence b, which has the room already."""
         o, i32 = self.dev.ordinal, _torch.int32
         n = sources.shape[0]
-        _check(lib().q3h_cache_copy(
+        _check(self._copy(
             self.h, src.h, n, _whole(sources, (n,), o, i32, "sources"),
             _whole(lens, (n,), o, i32, "lens"), _stream(o)))
 
     def page_state(self):
         """(table [sequences][pages of one at most], counts of pages that a sequence
         holds, refs: how many sequences hold a page), int32 copies."""
-        o, i32 = self.dev.ordinal, _torch.int32
         if not self.pages:
             _bad("not a cache of pages")
-        out = [_torch.empty(shape, dtype=i32, device=f"cuda:{o}") for shape in
-               (self.table_shape, self.table_shape[:1], (self.pages,))]
-        _check(lib().q3h_cache_page_state(self.h, *(t.data_ptr() for t in out), _stream(o)))
-        return tuple(out)
+        n, slots = self.table_shape
+        table, counts, refs = _torch.empty(
+            n * slots + n + self.pages, dtype=_torch.int32, device=self._device).split(
+                (n * slots, n, self.pages))
+        at = table.data_ptr()
+        _check(self._page_state(self.h, at, at + 4 * n * slots, at + 4 * n * (slots + 1),
+                                _stream(self.dev.ordinal)))
+        return table.view(n, slots), counts, refs
 
     def destroy(self):
         if self.h:
