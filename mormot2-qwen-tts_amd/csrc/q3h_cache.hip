@@ -107,7 +107,7 @@ __global__ __launch_bounds__(kThreads) void k_cache_append(AppendRows a) {
   // where the row goes; a page that another sequence holds too is not written to
   int at_pos = s.len + t;
   KvSeq place = s;
-  [[maybe_unused]] int axis_pos[kMaxAxes] = {};  // its positions on the axes
+  [[maybe_unused]] int axis_pos = 0;  // its position on axis lane % 4
   [[maybe_unused]] int page = -1;
   if constexpr (PLACED) {
     if (a.kv.table && !bad) {
@@ -117,12 +117,9 @@ __global__ __launch_bounds__(kThreads) void k_cache_append(AppendRows a) {
       at_pos &= place.max_pos - 1;
     }
     if (a.places) {
-#pragma unroll
-      for (int i = 0; i < kMaxAxes; i++)
-        if (i < a.n_axes) {
-          axis_pos[i] = a.places[(size_t)i * a.kv.sequences * a.kv.rows + row];
-          bad = bad || (uint32_t)axis_pos[i] >= (uint32_t)a.table_positions;
-        }
+      const int axis = lane % kMaxAxes < a.n_axes ? lane % kMaxAxes : 0;
+      axis_pos = a.places[(size_t)axis * a.kv.sequences * a.kv.rows + row];
+      bad = bad || __any((uint32_t)axis_pos >= (uint32_t)a.table_positions);
     }
   }
   if (a.parents) {
@@ -153,20 +150,27 @@ __global__ __launch_bounds__(kThreads) void k_cache_append(AppendRows a) {
       e[4 + i] = split && p < half ? half + p : e[i] + 1;
     }
   }
+  [[maybe_unused]] int axis_at[4];
+  if constexpr (PLACED) {
+    // the axes of the lane's pairs, two bits each: of four neighbours, or twice two
+    auto fields = [&](int p) { return (uint32_t)(a.axes[p >> 5] >> (2 * (p & 31))); };
+    const uint32_t two = fields(ODD || split ? 4 * sub : 2 * sub),
+                   more = ODD || split ? two >> 4 : fields(HD / 4 + 2 * sub);
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      axis_at[i] = __shfl(axis_pos, (int)((i < 2 ? two >> (2 * i) : more >> (2 * i - 4)) & 3u));
+  }
   double2 cs[4];
 #pragma unroll
   for (int i = 0; i < 4; i++) {
     const int p = ODD || split ? 4 * sub + i : (i < 2 ? 2 * sub + i : HD / 4 + 2 * sub + i - 2);
     cs[i] = make_double2(1.0, 0.0);
     if (p < half && !bad) {
-      int pos = s.len + depth;
-      if (PLACED && a.places) {
-        const uint32_t axis = (uint32_t)(a.axes[p >> 5] >> (2 * (p & 31))) & 3u;
-        pos = axis_pos[0];
-#pragma unroll
-        for (int j = 1; j < kMaxAxes; j++) pos = axis == (uint32_t)j ? axis_pos[j] : pos;
+      size_t at = (size_t)(s.len + depth) * half + p;
+      if constexpr (PLACED) {
+        // (lanes 0 .. 3 have the positions; a table has at most 2^30 pairs)
+        if (a.places) at = (uint32_t)axis_at[i] * (uint32_t)half + (uint32_t)p;
       }
-      const size_t at = (size_t)pos * half + p;
       if (a.table) {
         cs[i] = a.table[at];
       } else {
@@ -718,7 +722,8 @@ struct GoAppend {
 template <int FMT, int HD>
 struct GoRead {
   static void go(const KvView &kv, const int32_t *starts, float *k, float *v, hipStream_t st) {
-    const int64_t n = (int64_t)kv.sequences * kv.rows * kv.kvh, per = kReadRows * kThreads / (HD / 4);
+    const int64_t n = (int64_t)kv.sequences * kv.rows * kv.kvh;
+    const int64_t per = (int64_t)kReadRows * kThreads / (HD / 4);
     const dim3 grid((unsigned)((n + per - 1) / per));
     if (kv.table)
       hipLaunchKernelGGL((k_cache_read<FMT, HD, true>), grid, dim3(kThreads), 0, st, kv, starts, k, v);
