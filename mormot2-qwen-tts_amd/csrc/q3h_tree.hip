@@ -537,9 +537,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
       }
     }
   };
-  auto load_k = [&](Raw<FMT, HD> &raw, int tile) {
+  auto load_k = [&](Raw<FMT, HD> &raw, int tile, const Place &at_tile) {
     const int j0 = tile * T;
-    const Place at_tile = place(j0);
     of_tile(j0, [&](auto full) {
       constexpr bool FULL = decltype(full)::value;
 #pragma unroll
@@ -572,9 +571,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
       if constexpr (SC) load_fours(at_tile.in(ksc, 4), j0, raw.ks, full);
     });
   };
-  auto load_v = [&](Raw<FMT, HD> &raw, int tile) {
+  auto load_v = [&](Raw<FMT, HD> &raw, int tile, const Place &at_tile) {
     const int j0 = tile * T;
-    const Place at_tile = place(j0);
     of_tile(j0, [&](auto full) {
       constexpr bool FULL = decltype(full)::value;
 #pragma unroll
@@ -781,8 +779,9 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
     if (shared) {
       load_quarter(quarter, tile);
     } else {
-      load_k(raw, tile);
-      load_v(raw, tile);
+      const Place at_tile = place(tile * T);
+      load_k(raw, tile, at_tile);
+      load_v(raw, tile, at_tile);
     }
   }
 
@@ -924,10 +923,12 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
         vs[t] = raw.vs[t];
       }
     }
+    [[maybe_unused]] Place at_next{0, 0};
     if constexpr (SHARE) {
       if (next < tile1) load_quarter(raw, next);
-    } else {
-      if (next < tile1) load_k(raw, next);
+    } else if (next < tile1) {
+      at_next = place(next * T);
+      load_k(raw, next, at_next);
     }
 
     if (tail && a.parents && !paths) {
@@ -1072,7 +1073,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
     }
     if constexpr (SC) __builtin_amdgcn_s_setprio(0);
     if constexpr (!SHARE) {
-      if (next < tile1) load_v(raw, next);
+      if (next < tile1) load_v(raw, next, at_next);
     }
   };
   if (shared) {
