@@ -94,8 +94,8 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // have no room. even: the steps of all groups, one behind the other, are cut into
 // shares that differ by a step at most, so that a share may end one group and begin the
 // next (of 4 bits and up to 16 query rows of a kv head, a group a head): the workgroups
-// end together whatever the lengths (32 rows over 1024 .. 4096 positions each 36.7 -> EVEN
-// us, 64 over 4000 .. 16000 216 -> EVEN).
+// end together whatever the lengths (32 rows over 1024 .. 4096 positions
+// each 36.7 us with a head's shares by themselves, 35.3 so; 64 over 4000 .. 16000 216 and 182).
 struct Shape {
   int nq, group, blocks, parts;
   bool shares, even;
@@ -154,6 +154,60 @@ __device__ __forceinline__ Head head_of(const AttendRows &a, const KvSeq &s, con
     h.parts += k > 1 ? k : 0;
   }
   return h;
+}
+// inclusive sums over the lanes
+__device__ __forceinline__ int lane_sums(int x) { return wave_prefix_sum_i(x); }
+__device__ __forceinline__ int lanes_sum(int x) {
+  return __builtin_amdgcn_readlane(lane_sums(x), 63);
+}
+// the same by all lanes, a group each
+__device__ __forceinline__ Head head_of_lanes(const AttendRows &a, const KvSeq &s,
+                                              const Shape &shape, int tile, int most) {
+  const int rows_in = s.count * shape.per_kv;
+  int steps = 0, shares = 0, parts = 0;
+  for (int first = (int)(threadIdx.x & 63) * shape.group; first < rows_in;
+       first += 64 * shape.group) {
+    const int n = group_steps(a, s, shape, first, rows_in, tile), k = (n + most - 1) / most;
+    steps += n;
+    shares += k;
+    parts += k > 1 ? k : 0;
+  }
+  return {(rows_in + shape.group - 1) / shape.group, lanes_sum(steps), lanes_sum(shares),
+          lanes_sum(parts)};
+}
+// (A prompt has many groups. One after another for every wave of both kernels, to find
+// what is its own, 2 prompts of 1500 rows with 24 groups each took 33 us more of 147, f16,
+// of which 18 in the join, whose 24000 waves do little else.)
+// A head's group: the one that is(its first row, the shares up to its end) holds of. Its
+// steps, its shares, and the shares and parts before it (none: first behind the rows).
+struct Group {
+  int first, steps, shares, shares_before, parts_before;
+};
+template <class F>
+__device__ __forceinline__ Group find_group(const AttendRows &a, const KvSeq &s,
+                                            const Shape &shape, int rows_in, int tile, int most,
+                                            F &&is) {
+  if (rows_in <= shape.group) {
+    const int n = group_steps(a, s, shape, 0, rows_in, tile), k = (n + most - 1) / most;
+    return is(0, k) ? Group{0, n, k, 0, 0} : Group{rows_in, 0, 0, 0, 0};
+  }
+  int shares = 0, parts = 0;
+  for (int base = 0; base < rows_in; base += 64 * shape.group) {
+    const int first = base + (int)(threadIdx.x & 63) * shape.group;
+    const int n = first < rows_in ? group_steps(a, s, shape, first, rows_in, tile) : 0;
+    const int k = (n + most - 1) / most, p = k > 1 ? k : 0;
+    const int upto = shares + lane_sums(k), parts_upto = parts + lane_sums(p);
+    const uint64_t hit = __ballot(first < rows_in && is(first, upto));
+    if (hit) {
+      const int f = __builtin_ctzll(hit);
+      return {base + f * shape.group, __builtin_amdgcn_readlane(n, f),
+              __builtin_amdgcn_readlane(k, f), __builtin_amdgcn_readlane(upto - k, f),
+              __builtin_amdgcn_readlane(parts_upto - p, f)};
+    }
+    shares = __builtin_amdgcn_readlane(upto, 63);
+    parts = __builtin_amdgcn_readlane(parts_upto, 63);
+  }
+  return {rows_in, 0, 0, 0, 0};
 }
 // The steps of a share at most, from all heads' groups and steps. Rounding up
 // costs half a share a group: the shares come to about two for each CU, what it
@@ -219,9 +273,6 @@ __device__ __forceinline__ Parts parts_of(const AttendRows &a, const Shape &s, i
   p.most = p.head + a.kv.sequences;
   return p;
 }
-// inclusive sums over the lanes
-__device__ __forceinline__ int lane_sums(int x) { return wave_prefix_sum_i(x); }
-
 // two floats rounded to f16 and what is left of them
 __device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t &lo) {
   const h2 h = __builtin_convertvector((f2){x, y}, h2);
@@ -337,6 +388,16 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
   [[maybe_unused]] Head even_head{0, 0, 0, 0};
   auto head_at = [&](int i, int most) {
     if (most == 1 || n > 64) mine = kv_sequence<PAGED>(a.kv, std::min(i, n - 1));
+    // (few sequences of many groups: a group a lane)
+    const int here = __builtin_amdgcn_readfirstlane(std::min(n - i + lane, 64));
+    if (!EVEN && a.kv.rows * per_kv > 2 * here * shape.group) {
+      Head h{0, 0, 0, 0};
+      for (int f = 0; f < here; f++) {
+        const Head x = head_of_lanes(a, lane_sequence(mine, f), shape, T, most);
+        if (lane == f) h = x;
+      }
+      return h;
+    }
     return i < n ? head_of(a, mine, shape, T, most) : Head{0, 0, 0, 0};
   };
   auto even_load = [&](int base, int before) {
@@ -432,21 +493,16 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
     g = at / shares;
     at -= g * shares;
     slot += g * head_parts;
-    const int rows_in = s.count * per_kv;
-    for (first = 0; first < rows_in; first += shape.group) {
-      const int own = group_steps(a, s, shape, first, rows_in, T), k = (own + most - 1) / most;
-      if (at < k) {
-        // k shares that differ by a step at most
-        const int q = own / k, longer = own - q * k;
-        step0 = at * q + std::min(at, longer);
-        step1 = step0 + q + (at < longer);
-        whole = k == 1;
-        slot += at;
-        break;
-      }
-      at -= k;
-      slot += k > 1 ? k : 0;
-    }
+    const Group own = find_group(a, s, shape, s.count * per_kv, T, most,
+                                 [&](int, int upto) { return upto > at; });
+    first = own.first;
+    at -= own.shares_before;
+    slot += own.parts_before + at;
+    whole = own.shares == 1;
+    // shares that differ by a step at most
+    const int q = own.steps / std::max(own.shares, 1), longer = own.steps - q * own.shares;
+    step0 = at * q + std::min(at, longer);
+    step1 = step0 + q + (at < longer);
   }
   auto piece = [&]() __attribute__((always_inline)) {
   // (as for no share: lengths that change meanwhile)
@@ -1403,10 +1459,10 @@ __global__ __launch_bounds__(kThreads) void k_attend_join(AttendRows a, Shape sh
     start = 2 * share;
     if (n <= 1 || start + 2 * n > shape.parts) return;
   } else {
-    for (int first = 0; first <= mine; first += shape.group) {
-      start += n > 1 ? n : 0;
-      n = (group_steps(a, s, shape, first, rows_in, tile) + most - 1) / most;
-    }
+    const Group own = find_group(a, s, shape, rows_in, tile, most,
+                                 [&](int first, int) { return first == mine; });
+    start += own.parts_before;
+    n = own.shares;
     if (n <= 1 || start < 0 || start + n > shape.parts) return;  // (one share: written as it is)
   }
   const int sub = lane / (HD / 4), e = lane % (HD / 4) * 4;
