@@ -510,6 +510,9 @@ __global__ __launch_bounds__(kThreads) void k_cache_read(KvView kv, const int32_
     s.count = kv.counts ? min(max(kv.counts[in], 0), kv.rows) : kv.rows;
     there[u] = b < kv.sequences && t < s.count;
     bad[u] = s.len < 0 || s.len > s.max_pos - s.count;
+    // (nothing is loaded for rows behind a sequence's: 16 sequences of up to 2051 int8
+    // rows in pages, an eighth of them there, 24.8 -> 19.0 us)
+    if (u == kReadRows - 1 && !there[0] && !there[u]) return;
     // (no such row: the first one, which is there, if only as page 0)
     int p = there[u] && !bad[u] ? s.len + t : 0;
     if constexpr (PAGED) s = kv_place(kv, s, in, p);
