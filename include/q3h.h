@@ -55,8 +55,9 @@ typedef struct {
   int32_t dtype;         /* storage: Q3H_F32 or Q3H_Q8_0 (weights and heads) */
   int32_t kv_f16;        /* K/V cache in half floats (lm.pas:128-130): 0 or 1; or
                             Q3H_KV_Q8 (2; no reference counterpart): a byte per
-                            element and a scale per position and head, f32
-                            activations only. Other values are refused; before
+                            element and a scale per position and head, or
+                            Q3H_KV_Q4 (4): four bits per element with steps and
+                            a scale, both f32 activations only. Other values are refused; before
                             there were int8 caches any value but 0, such as a
                             truth value of -1, chose half floats */
   int32_t act_q8;        /* Q8_0 only: 1 = activations quantized per 32-block
@@ -171,7 +172,7 @@ int q3h_forward_embeds(q3h_context *c, const float *x, int rows, int head,
    buffers of the call (they grow with rows and, for fewer than 16 rows of
    an f32-activation stack over more than 256 positions, with the decode
    attention's splits) must fit the array: otherwise
-   Q3H_E_CAPACITY and nothing is computed. With an int8 cache or rotary
+   Q3H_E_CAPACITY and nothing is computed. With an int8 or 4-bit cache or rotary
    positions of q3h_stack_set_rope they grow with rows alone: the attention's
    partial sums take what the others leave, and where that is less than
    q3h_forward_embeds uses (16 heads over 8, an f32 cache: 33 to 64 rows over
@@ -539,7 +540,7 @@ int q3h_cache_read(q3h_cache *c, int layer, int sequences, int rows, const int32
    h / (heads / kv_heads). max_len: no length in lens is above it (the host's
    bound, it sizes the launch; a longer or negative one: NaN rows). scale: 0 for
    1 / sqrt(head_dim). Products and sums keep f32's precision in every format;
-   over f16 and int8 caches that is relative to the row's largest element (an
+   over f16, int8 and 4-bit caches that is relative to the row's largest element (an
    element to which only positions of a weight near 2^-24 add is less exact), and
    an f16 cache's elements below 2^-14 count to 2^-38.
    Infinities and NaN at positions a row does not see do not reach it. workspace:
@@ -566,13 +567,15 @@ int q3h_cache_attend(q3h_cache *c, const q3h_attend_args *a, void *stream);
    holds kept_counts[b] row numbers, each above the one before (a path from a
    root down); row kept[b][i], at position lens[b] + kept[b][i], goes to
    position lens[b] + i, in every layer. The caller's lengths grow by
-   kept_counts. A list that is not of that form leaves its sequence as it is. */
+   kept_counts. A list that is not of that form leaves its sequence as it is, and so
+   does one whose rows would go to a page that another sequence holds too. */
 int q3h_cache_keep(q3h_cache *c, int sequences, int rows, const int32_t *lens,
                    const int32_t *kept, const int32_t *kept_counts, void *stream);
 
 /* The pages of a cache of q3h_cache_create_paged, for its first `sequences` sequences. Like
    the operators above these calls only enqueue kernels, on any stream, and can be
-   captured; but they change what the cache's other calls read, and share scratch memory
+   captured (the order in which they run is the caller's to keep, also of two graphs);
+   but they change what the cache's other calls read, and share scratch memory
    of the cache: of one cache they run one after another, and not beside a call on
    its rows. Pages are taken from the lowest free one up, for the sequences in their
    order, so that the same calls leave the same tables. What only the device holds and is
@@ -650,7 +653,7 @@ int q3h_token_logprobs(q3h_device *dev, const q3h_score_args *a, void *stream);
    context of a stack with f32 activations: before the first context or frame
    (Q3H_E_STATE); head_dim and max_positions as the stack's. rope_theta of the
    stack's configuration is not used then. Contexts of such a stack, and of one
-   with an int8 cache, take the same calls as any other (prompts of
+   with an int8 or 4-bit cache, take the same calls as any other (prompts of
    q3h_frame_start_batch each by itself; not q3h_context_time_attention). */
 int q3h_stack_set_rope(q3h_stack *s, const q3h_rope_config *cfg);
 

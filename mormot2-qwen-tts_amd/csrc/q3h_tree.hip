@@ -406,10 +406,13 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
     even_upto = before + lane_sums(even_head.steps) * a.kv.kvh;
     even_before = even_upto - even_head.steps * a.kv.kvh;
   };
-  // the next piece of the share: the rest of a group, or of the share
+  // the next piece of the share: the rest of a group, or of the share (false: there is
+  // none, where lengths change while the kernel runs)
   auto even_next = [&] {
-    while (__builtin_amdgcn_readlane(even_upto, 63) <= even0)
+    while (__builtin_amdgcn_readlane(even_upto, 63) <= even0) {
+      if (even_base + 64 >= n) return false;
       even_load(even_base + 64, __builtin_amdgcn_readlane(even_upto, 63));
+    }
     const int f = __builtin_ctzll(__ballot(even_upto > even0));
     b = even_base + f;
     s = lane_sequence(mine, f);
@@ -422,6 +425,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
     whole = step1 - step0 == own;
     slot = 2 * blockIdx.x + (step0 == 0);
     even0 += step1 - step0;
+    return true;
   };
   if (!shape.shares) {
     g = blockIdx.x % a.kv.kvh;
@@ -451,7 +455,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
     even0 = share_start(blockIdx.x, shares, steps);
     even1 = share_start(blockIdx.x + 1, shares, steps);
     if (n > 64) even_load(0, 0);
-    even_next();
+    if (!even_next()) return;
   } else {
     // each wave finds it by itself, 64 sequences at a time
     Head h{0, 0, 0, 0};
@@ -1287,8 +1291,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
   if constexpr (EVEN) {
     for (;;) {
       piece();
-      if (even0 >= even1) break;
-      even_next();
+      if (even0 >= even1 || !even_next()) break;
       __syncthreads();  // (the waves' meeting place)
     }
   } else {

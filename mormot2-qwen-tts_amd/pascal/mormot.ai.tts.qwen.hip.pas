@@ -67,8 +67,8 @@ type
     layers, hidden, heads, kv_heads, head_dim, intermediate: integer;
     rms_eps, rope_theta: single;
     dtype: integer;         // Q3H_F32 or Q3H_Q8_0
-    kv_f16: integer;        // K/V cache in half floats (lm.pas:128-130), or Q3H_KV_Q8;
-                            // Ord() of a boolean: -1, a LongBool's True, is refused
+    kv_f16: integer;        // K/V cache in half floats (lm.pas:128-130), or Q3H_KV_Q8,
+                            // or Q3H_KV_Q4; Ord() of a boolean: -1, a LongBool's True, is refused
     act_q8: integer;        // Q8_0 only: activations quantized per 32-block
     max_positions: integer;
   end;

@@ -277,9 +277,30 @@ ATTEND = [
 @pytest.mark.parametrize("case,page", [(i, page) for i, c in enumerate(ATTEND)
                                        for page in (0, 32, 64, 256) if page or c[0] == N])
 def test_attend_matches_float64(device, case, page):
-    fmt, hd, heads, kvh, rows, lens, tree = ATTEND[case]
-    print("attend", ATTEND[case], page, flush=True)
-    rng = np.random.default_rng(100 + case)
+    check_attend(device, ATTEND[case], page, 100 + case)
+
+
+# more sequences than a wave has lanes, and heads of more groups of rows than that
+LARGE = [
+    (N, 64, 4, 2, 1, [2500 - 7 * i for i in range(70)], False),
+    (N, 128, 4, 2, 3, [1200 - 9 * i for i in range(130)], True),
+    (N, 64, 2, 1, 2100, [100], False),
+    (H, 64, 2, 1, 4200, [30], False),
+    (Q, 64, 8, 1, 1200, [300, 0], False),
+    (F, 64, 4, 1, 700, [0, 900, 20], False),
+]
+
+
+@pytest.mark.parametrize("page", [0, 32])
+@pytest.mark.parametrize("case", range(len(LARGE)))
+def test_attend_of_many(device, case, page):
+    check_attend(device, LARGE[case], page, 200 + case)
+
+
+def check_attend(device, case, page, seed):
+    fmt, hd, heads, kvh, rows, lens, tree = case
+    print("attend", case, page, flush=True)
+    rng = np.random.default_rng(seed)
     n, P = len(lens), max(lens) + rows + 3
     lens = np.array(lens)
     counts = np.array([max(1, rows - i * 3) for i in range(n)])
