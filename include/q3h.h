@@ -176,8 +176,8 @@ int q3h_forward_embeds(q3h_context *c, const float *x, int rows, int head,
    positions of q3h_stack_set_rope they grow with rows alone: the attention's
    partial sums take what the others leave, and where that is less than
    q3h_forward_embeds uses (16 heads over 8, an f32 cache: 33 to 64 rows over
-   more than 130 to 310 positions, 17 to 32 over 1480 to 1730; an int8 one:
-   over twice as many or more), the positions are cut into fewer pieces: the
+   more than 130 to 310 positions, 17 to 32 over 1480 to 1730; an int8 or
+   4-bit one: over twice as many or more), the positions are cut into fewer pieces: the
    results differ in the order of those sums. Every call on one GPU shares that
    GPU's array, which keeps the last call's contents (no kernel reads a
    buffer before writing it); calls on one device are serialized by a lock

@@ -88,7 +88,11 @@ __device__ __forceinline__ int step_of(float m, float d) {
 // instruction, 38; a pair a lane, a head over a whole wave, 60: the 64-bit sums of
 // each head made that VALU bound). One row: 3.6 us, 496 rows of 16 + 2 x 8 heads to
 // int8 7.4 us, which are a launch, the path through the parents and three loads that
-// wait for each other (length, angles, rows).
+// wait for each other (length, angles, rows). The 3576 rows to 4 bits 31 us (150 MB, 4.9
+// TB/s; the steps, 64-bit quotients next to a half, and elements joined by neighbouring
+// lanes are 250 instructions a wave more than f16's 470, and it waits for half of its time
+// all the same); over pages and with positions of three axes 35: two more loads before the
+// rows go out, the position of a pair's axis and the page.
 constexpr int kHeads = 2, kManyRows = 1024;
 // PLACED: pages, or positions of several axes (their branches cost the others 4 %).
 template <int FMT, int HD, bool ODD, bool MANY, bool PLACED>
@@ -554,8 +558,9 @@ __global__ __launch_bounds__(kThreads) void k_cache_read(KvView kv, const int32_
 }
 
 // 32 sequences of 28 layers of 8 heads of 128, paths of 8 rows: f32 117 MB 29 us
-// (4.1 TB/s), f16 26, int8 29; paths of 32 rows 179, 127 and 113 us; one sequence and
-// a path of 8 5 us, of 32 12-16: bound by a trip to memory a row, one after another.
+// (4.1 TB/s), f16 26, int8 29, 4 bits 32; paths of 32 rows 179, 127 and 113 us; one sequence
+// and a path of 8 5 us, of 32 12-16: bound by a trip to memory a row, one after another.
+// In pages two, the row's page first (f16 49, int8 54, 4 bits 62 us; one sequence 10).
 // One workgroup per (sequence, layer, kv head, keys or values): the kept rows
 // in ascending order, each to a position at or before its own that no later
 // row comes from, so one row after another is enough; a 4-byte word of a row a

@@ -190,7 +190,11 @@ __device__ __forceinline__ bool last_to_come(const Book &k) {
 // ranks of the pages taken are sums over the threads. Every workgroup does all that, copies
 // its part of the rows before lens of the pages that are replaced, and the one that came
 // last changes the tables: one launch. Bound by the trips to memory that wait for one
-// another (lengths, table, holders) and the barriers, then by the copies.
+// another (lengths, table, holders) and the barriers, then by the copies: 4 sequences 5.3 us,
+// 16 of up to 33 pages 5.6, four beams of a shared page 7.3 and 128 of 16 prompts, where the
+// rows of 112 pages are copied in 5 layers of 4 bits, 29 MB read and written, 16.4. (In two
+// launches, one workgroup and then the copies, fork and reserve of the four beams 16.8 us,
+// 10.7 so.)
 template <int FMT, int HD>
 __global__ __launch_bounds__(kBook) void k_reserve(Book k, KvView v, int n, int rows,
                                                    const int32_t *lens, const int32_t *counts,
@@ -292,7 +296,8 @@ __global__ __launch_bounds__(kBook) void k_reserve(Book k, KvView v, int n, int 
   }
 }
 
-// The same of any number of slots: one workgroup, `group` lanes (a power of two) a
+// The same of any number of slots (32 sequences of up to 64 pages at once 13.3 us,
+// and a launch for the copies): one workgroup, `group` lanes (a power of two) a
 // sequence at a time: who writes to which shared page (writers, lowest), how many pages
 // each sequence wants, their sums in order, the lowest free pages in order, who gets which.
 __global__ __launch_bounds__(kBook) void k_reserve_many(Book k, int n, int rows, const int32_t *lens,
@@ -440,8 +445,8 @@ __global__ __launch_bounds__(kThreads) void k_copy_tails(KvView v, Book k, const
 
 // A fork's table: of few slots by one workgroup, its entries in registers between reading
 // and writing (an assignment may be any, so that none is written before all are read); of
-// more in two launches, the table beside the present one first. 128 sequences of 31 slots FORK
-// us.
+// more in two launches, the table beside the present one first. 4 sequences of two slots 3.4
+// us, 128 of 31 5.2: a chain of four trips to memory.
 constexpr int kForkEach = 16, kForkSlots = kForkEach * kBook;
 struct Forked {
   int from, now, held;  // (now < 0: as it is)
@@ -588,7 +593,9 @@ __device__ __forceinline__ void move_pages(char *base, int64_t page_bytes, int m
 }
 
 // Up to 8192 pages: every workgroup works out the moves, makes its part of them and of
-// the tables' changes, and the last to come changes who holds which page.
+// the tables' changes, and the last to come changes who holds which page. Nothing to move:
+// 6.4 us, a scan of all pages by every workgroup before its first load; 164 of 64 positions
+// and 2 layers of int8, 89 MB read and written, 20.
 __global__ __launch_bounds__(kBook) void k_compact(Book k, char *base, int64_t page_bytes,
                                                    int32_t *used) {
   __shared__ int32_t sm_hole[kScan / 2], sm_mover[kScan / 2];
@@ -660,7 +667,8 @@ __global__ __launch_bounds__(kThreads) void k_move(Book k, char *base, int64_t p
 
 // The first lens[b] positions of sequence sources[b] of a cache into sequence b of
 // another. A wave takes runs of 32 positions of a (layer, part, kv head), which lie in
-// one piece on both sides, an equal share of all of them.
+// one piece on both sides, an equal share of all of them. 8 sequences, 10300
+// positions of 2 layers of int8, 87 MB read and written: 19 us (4.6 TB/s).
 template <int FMT, int HD>
 __global__ __launch_bounds__(kThreads) void k_copy(KvView to, KvView from, const int32_t *sources,
                                                    int src_sequences) {

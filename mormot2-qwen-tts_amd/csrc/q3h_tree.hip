@@ -20,6 +20,10 @@
 // instructions. An int8 row's scale is a factor of the position: it multiplies
 // the score, and the weight that the values are summed with. (One f16 part of
 // each would be half the products; the sums were then 2^-12 off instead of 2^-21.)
+// In 4 bits an element is a whole number up to 1785 of its row's scale, exact in f16
+// too: the same kernel, where two elements take three instructions from nibbles to f16.
+// A cache in pages is read a tile at a time, whose page is found once, from 64 of the
+// table's entries in the wave's lanes.
 //
 // What bounds it, by how much a share has to do (heads of 128):
 // - one row over 171 positions of an f16 cache, 8 workgroups of 2 tiles a wave:
@@ -37,8 +41,15 @@
 //   each) and matrix instructions (64) take turns more than they overlap: 69 % and
 //   34 % of the time. 260 TFLOP/s of the definition's operations, twice that in
 //   products;
-// - 2 prompts of 1500 rows over 500 positions, 16 heads over 8: f16 102 us, int8 114,
-//   f32 235 (131 of the 154 TFLOP/s of a large f32 product).
+// - 2 prompts of 1500 rows over 500 and 125 positions, 16 heads over 8, 26 GFLOP: f16 112
+//   us, int8 130, 4 bits 132, f32 354 (both over 500: VALU 45 % and matrix instructions 23 %
+//   of the time, 1.6 waves a SIMD on average);
+// - 32 sequences of one row, 82000 positions of 4 bits in pages of 64, 95 MB: 35 us + 4.8.
+//   Of a wave's 343 instructions a tile 182 make f16 of
+//   nibbles; 12 us are a share's beginning, end and the join, 2 the pages, a step 0.9. 64
+//   sequences of 4000 .. 16000 positions 178 (4.1 TB/s; int8 291 at 4.65). One row over 171
+//   positions 7.6, over 8000 13.6;
+// - the 12 trees in 4 bits 140 + 12: the conversions of int8 (130) with a step more.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

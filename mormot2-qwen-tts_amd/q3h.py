@@ -873,9 +873,9 @@ class Cache:
     per element with a scale per position and head, or four bits with steps for each
     32 elements too (KV_F32, KV_F16, KV_Q8, KV_Q4). With pages: in that many pages of
     page_positions positions (32, 64, 128 or 256) that the sequences share (reserve,
-    fork, release, compact). Calls take rows [sequences][rows][heads][head_dim] for the first sequences of
-    the cache; lens, counts [sequences] and parents [sequences][rows] are int32
-    tensors on the device."""
+    fork, release, compact). Calls take rows [sequences][rows][heads][head_dim] for the
+    first sequences of the cache; lens, counts [sequences] and parents
+    [sequences][rows] are int32 tensors on the device."""
 
     h = None
 
