@@ -340,15 +340,15 @@ template <int HD>
 struct Raw<Q3H_KV_Q8, HD> {
   u4 k[2][HD / 64];
   u2 v[8 * HD / 128];  // 8 positions of HD / 16 bytes
-  f4 ks[2], vs[2];
+  float scale;         // (of_row)
 };
 template <int HD>
 struct Raw<Q3H_KV_Q4, HD> {
   uint32_t k[2][HD / 32];  // HD / 4 elements
   uint32_t v[8];           // 8 positions of HD / 16 elements
   uint32_t kw[2];          // the keys' steps
-  u4 vw[2];                // the values' steps of 4 positions
-  f4 ks[2], vs[2];
+  uint32_t vw;             // a value's steps (of_row)
+  float scale;
 };
 template <int HD>
 struct Raw<Q3H_KV_F32, HD> {
@@ -590,24 +590,19 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
     }
     f(std::false_type());
   };
-  // four bytes for each of positions 4 g4 .. + 3 of the tile's halves
-  auto load_fours = [&](const char *sc, int j0, auto(&d)[2], auto full) {
-    using V = std::remove_reference_t<decltype(d[0])>;
-    typedef V unaligned __attribute__((aligned(4)));
-#pragma unroll
-    for (int t = 0; t < 2; t++) {
-      if constexpr (decltype(full)::value) {
-        d[t] = load<unaligned>(sc, (uint32_t)(16 * g4), 64 * t);
-      } else if (!BOTH && j0 + T <= cut.end) {
-        d[t] = load<unaligned>(sc, (uint32_t)(64 * t + 16 * g4));
-      } else {
-#pragma unroll
-        for (int r = 0; r < 4; r++)
-          d[t][r] = load<std::remove_reference_t<decltype(d[t][r])>>(
-              sc, 4 * (int64_t)std::min(16 * t + 4 * g4 + r, last - j0));
-      }
-    }
+  // What a row of 16 lanes needs of the scales, the 8 positions of its scores' keys and the
+  // same of the values, in one lane each (of_row: position 16 t + 4 g4 + r at lane 4 t + r,
+  // of the values 8 behind): one load of four bytes, where all in every lane are four of 16,
+  // which the address path takes as many cycles for as for 16 different bytes a lane; an
+  // operand that another lane of the row holds costs nothing.
+  const int of_row = 16 * (n16 >> 2 & 1) + 4 * g4 + (n16 & 3);
+  const char *const sc_row = SC ? (n16 < 8 ? ksc : vsc) : nullptr;
+  auto load_scales = [&](const Place &at_tile, int j0, auto full) {
+    const int row = decltype(full)::value ? of_row : std::min(of_row, last - j0);
+    return load<float>(sc_row, at_tile.page + 4 * (at_tile.row + row));
   };
+  auto key_scale = [](float scale, int i) { return row_lane(scale, i); };
+  auto value_scale = [](float scale, int i) { return row_lane(scale, 8 + i); };
   auto load_k = [&](Raw<FMT, HD> &raw, int tile, const Place &at_tile) {
     const int j0 = tile * T;
     of_tile(j0, [&](auto full) {
@@ -639,7 +634,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
           for (int i = 0; i < HD / 32; i++) raw.k[t][i] = load<u4>(p, at, 64 * i);
         }
       }
-      if constexpr (SC) load_fours(at_tile.in(ksc, 4), j0, raw.ks, full);
+      if constexpr (SC) raw.scale = load_scales(at_tile, j0, full);
     });
   };
   auto load_v = [&](Raw<FMT, HD> &raw, int tile, const Place &at_tile) {
@@ -672,8 +667,9 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
           }
         }
       }
-      if constexpr (SC) load_fours(at_tile.in(vsc, 4), j0, raw.vs, full);
-      if constexpr (Q4) load_fours(at_tile.in(vst, 4), j0, raw.vw, full);
+      if constexpr (Q4)
+        raw.vw = load<uint32_t>(at_tile.in(vst, 4),
+                                (uint32_t)(4 * (FULL ? of_row : std::min(of_row, last - j0))), 0);
     });
   };
   // 4 bits: where a key's and a value's group is in its word of steps
@@ -703,7 +699,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
     u4 k[SC ? 1 : KN];
     uint32_t v[Q4 ? 2 : 8];
     uint32_t kw, vw[2];
-    f4 ks[2], vs[2];
+    float scale;
   };
   auto load_quarter = [&](Quarter &raw, int tile) {
     const int j0 = tile * T;
@@ -753,10 +749,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
               (uint32_t)(std::min(j, last - j0) * ROW + n16 * (ROW / 16) + 4 * word));
         }
       }
-      if constexpr (SC) {
-        load_fours(at_tile.in(ksc, 4), j0, raw.ks, full);
-        load_fours(at_tile.in(vsc, 4), j0, raw.vs, full);
-      }
+      if constexpr (SC) raw.scale = load_scales(at_tile, j0, full);
     });
   };
   auto store_quarter = [&](const Quarter &raw) {
@@ -986,14 +979,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
 #pragma unroll
         for (int r = 0; r < 4; r++) st[0][t][r] += dpp_f<kRowRor8>(st[0][t][r]);
     }
-    f4 ks[2], vs[2];
-    if constexpr (SC) {
-#pragma unroll
-      for (int t = 0; t < 2; t++) {
-        ks[t] = raw.ks[t];
-        vs[t] = raw.vs[t];
-      }
-    }
+    float scales = 0.f;
+    if constexpr (SC) scales = raw.scale;
     [[maybe_unused]] Place at_next{0, 0};
     if constexpr (SHARE) {
       if (next < tile1) load_quarter(raw, next);
@@ -1027,8 +1014,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
       float low = INFINITY;
 #pragma unroll
       for (int i = 0; i < 8; i++) {
-        top = fmaxf(top, vs[i >> 2][i & 3]);
-        low = fminf(low, vs[i >> 2][i & 3]);
+        top = fmaxf(top, value_scale(scales, i));
+        low = fminf(low, value_scale(scales, i));
       }
       top = rows4_max(top);
       wide = wide || __any(low < top * 0x1p-16f);
@@ -1038,18 +1025,19 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
       float mx = -INFINITY, vx = top;
 #pragma unroll
       for (int i = 0; i < 4 * NS; i++)
-        w[q][i] = SC ? st[q][i >> 2][i & 3] * ks[i >> 2][i & 3] : st[q][i >> 2][i & 3];
+        w[q][i] = SC ? st[q][i >> 2][i & 3] * key_scale(scales, i) : st[q][i >> 2][i & 3];
       if (tail) {
         asm volatile("");  // (a branch, so that the other tiles have no selects)
         vx = 0.f;
 #pragma unroll
         for (int i = 0; i < 4 * NS; i++) {
           const int d = j0 + (i >> 2) * 16 + 4 * g4 + (i & 3) - s.len;
+          [[maybe_unused]] const float own = SC ? value_scale(scales, i) : 0.f;
           const bool see = sees(q, d);
           w[q][i] = see ? w[q][i] : -INFINITY;
           // a row whose path is broken: NaN at itself, and so in all of it
           if (broken[q] && d == qt[q]) w[q][i] = NAN;
-          if (SC && see) vx = fmaxf(vx, vs[i >> 2][i & 3]);
+          if (SC && see) vx = fmaxf(vx, own);
         }
         if constexpr (SC) vx = rows4_max(vx);
       }
@@ -1061,7 +1049,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
         mx = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 4 * NS; i++)
-          mx = fmaxf(mx, fmaf(w[q][i], sfac[q], power(vs[i >> 2][i & 3])));
+          mx = fmaxf(mx, fmaf(w[q][i], sfac[q], power(value_scale(scales, i))));
         mx = rows4_max(mx) + off;
       } else {
         mx = fmaf(rows4_max(mx), sfac[q], SC ? off + power(top) : off);
@@ -1080,7 +1068,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
       for (int i = 0; i < 4 * NS; i++) {
         const float p = __builtin_amdgcn_exp2f(fmaf(w[q][i], sfac[q], -base));
         l[q] += p;
-        w[q][i] = SC ? p * vs[i >> 2][i & 3] : p;
+        w[q][i] = SC ? p * value_scale(scales, i) : p;
       }
     }
 
@@ -1121,8 +1109,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
             const uint32_t w = __builtin_amdgcn_perm(raw.v[2 * e + 1], raw.v[2 * e],
                                                      c & 4 ? 0x07060302u : 0x05040100u);
             va[e] = nibbles_f16(w, c & 3,
-                                steps_f16(raw.vw[e >> 1][2 * (e & 1) + 1],
-                                          raw.vw[e >> 1][2 * (e & 1)], value_sel));
+                                steps_f16(row_lane_i(raw.vw, 2 * e + 1),
+                                          row_lane_i(raw.vw, 2 * e), value_sel));
           } else if constexpr (Q8) {
             // bytes c of positions 2e and 2e + 1
             va[e] = bytes_f16(vword(raw, 2 * e + 1, c >> 2), vword(raw, 2 * e, c >> 2),

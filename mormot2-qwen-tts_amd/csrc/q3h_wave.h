@@ -26,6 +26,25 @@ constexpr int kRowMirror = 0x140;
 constexpr int kRowRor8 = 0x128;   // row_ror:8
 constexpr int kBcast15 = 0x142;
 constexpr int kBcast31 = 0x143;
+constexpr int kRowBcast = 0x150;  // row_newbcast:0, .. + 15: a lane of the row of 16
+
+// lane i (known when it is compiled, 0 .. 15) of the row of 16, in all of it (all lanes
+// active): an operand of the instruction that takes it
+__device__ __forceinline__ int row_lane_i(int v, int i) {
+  switch (i) {
+#define Q3H_ROW_LANE(n) \
+  case n: return __builtin_amdgcn_update_dpp(0, v, kRowBcast + n, 0xf, 0xf, true);
+    Q3H_ROW_LANE(0) Q3H_ROW_LANE(1) Q3H_ROW_LANE(2) Q3H_ROW_LANE(3)
+    Q3H_ROW_LANE(4) Q3H_ROW_LANE(5) Q3H_ROW_LANE(6) Q3H_ROW_LANE(7)
+    Q3H_ROW_LANE(8) Q3H_ROW_LANE(9) Q3H_ROW_LANE(10) Q3H_ROW_LANE(11)
+    Q3H_ROW_LANE(12) Q3H_ROW_LANE(13) Q3H_ROW_LANE(14)
+#undef Q3H_ROW_LANE
+  }
+  return __builtin_amdgcn_update_dpp(0, v, kRowBcast + 15, 0xf, 0xf, true);
+}
+__device__ __forceinline__ float row_lane(float v, int i) {
+  return __builtin_bit_cast(float, row_lane_i(__builtin_bit_cast(int, v), i));
+}
 
 // sum over the 64 lanes, returned in every lane (all lanes must be active)
 __device__ __forceinline__ float wave_sum_dpp(float v) {
