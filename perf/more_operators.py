@@ -285,7 +285,9 @@ def _prepare_own(case, x, state):
     dev = state["dev"] = q3h.Device(0)
     op, n, page = case["op"], case["n"], case["page"]
     if op == "beams":
-        cache = state["cache"] = _own_cache(case, dev, n * case["width"], case["len"] + 1, page)
+        # (a page's positions at least: so many rows are read of each sequence)
+        cache = state["cache"] = _own_cache(case, dev, n * case["width"],
+                                            max(case["len"] + 1, page), page)
         _own_fill(case, cache, x["k"], x["v"], x["lens"])
         state["ok"] = torch.zeros(n * case["width"], dtype=torch.int32, device="cuda")
         return
