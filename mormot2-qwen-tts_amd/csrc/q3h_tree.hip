@@ -42,14 +42,16 @@
 //   34 % of the time. 260 TFLOP/s of the definition's operations, twice that in
 //   products;
 // - 2 prompts of 1500 rows over 500 and 125 positions, 16 heads over 8, 26 GFLOP: f16 112
-//   us, int8 130, 4 bits 132, f32 354 (both over 500: VALU 45 % and matrix instructions 23 %
+//   us, int8 126, 4 bits 130, f32 354 (both over 500: VALU 45 % and matrix instructions 23 %
 //   of the time, 1.6 waves a SIMD on average);
 // - 32 sequences of one row, 82000 positions of 4 bits in pages of 64, 95 MB: 35 us + 4.8.
 //   Of a wave's 343 instructions a tile 182 make f16 of
 //   nibbles; 12 us are a share's beginning, end and the join, 2 the pages, a step 0.9. 64
 //   sequences of 4000 .. 16000 positions 178 (4.1 TB/s; int8 291 at 4.65). One row over 171
 //   positions 7.6, over 8000 13.6;
-// - the 12 trees in 4 bits 140 + 12: the conversions of int8 (130) with a step more.
+// - the 12 trees in 4 bits 141 + 12: the conversions of int8 (130) with a step more. A step of
+//   four waves takes 5700 cycles, two workgroups on a CU: scores 1240, the next loads 740,
+//   softmax 1700, values 1250, conversions and barriers 780; alone on a CU 5100.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -594,7 +596,9 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
   // same of the values, in one lane each (of_row: position 16 t + 4 g4 + r at lane 4 t + r,
   // of the values 8 behind): one load of four bytes, where all in every lane are four of 16,
   // which the address path takes as many cycles for as for 16 different bytes a lane; an
-  // operand that another lane of the row holds costs nothing.
+  // operand that another lane of the row holds costs nothing, and 15 registers are free (12
+  // trees in int8 189 -> 183 us, in 4 bits 199 -> 193, launched one behind another; prompts
+  // 131 -> 126).
   const int of_row = 16 * (n16 >> 2 & 1) + 4 * g4 + (n16 & 3);
   const char *const sc_row = SC ? (n16 < 8 ? ksc : vsc) : nullptr;
   auto load_scales = [&](const Place &at_tile, int j0, auto full) {
