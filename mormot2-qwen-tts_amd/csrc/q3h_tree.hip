@@ -375,6 +375,11 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
   // the waves' outputs; before that, with two query tiles a wave, its queries as
   // operands (64 registers: two waves a SIMD would not have them)
   constexpr bool QLDS = NQ > 1 && !F32;
+  // on their way there loaded by whole rows, not as the operands have them, where every
+  // lane's 16 bytes are a line of their own: a tree of 27 rows over 12289 positions of f16 in
+  // pages 28.4 -> 27.3 us; not over int8 and 4 bits (2 prompts of 1500 rows 93.0 -> 94.8, 12
+  // trees 126.5 -> 128)
+  constexpr bool QROWS = QLDS && FMT == Q3H_KV_F16;
   constexpr int QW = NQ * (HD / 32) * 2 * 256;  // words of a wave's queries
   // with four waves side by side also a tile's keys and values as operands, each
   // wave's quarter
@@ -829,19 +834,15 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
     live[q] = r < rows_in && (!SIDE || n16 < 8);
     qrow[q] = std::min(r, rows_in - 1);
     qt[q] = shape.drafted(qrow[q]);
-    // (into LDS: four lanes a row, 64 neighbouring bytes an instruction, or 32 of each 64;
-    // as the operands have them every lane's 16 bytes are a line of their own: a tree of 27
-    // rows over 12289 positions of f16 in pages 28.4 -> 27.3 us, 12 trees of 4 bits 141 ->
-    // 139, in pages of 64 201 -> 205 one behind another, the others the same)
-    const int from = QLDS ? std::min(first + (wq * NQ + q) * 16 + (own_lane >> 2), rows_in - 1)
-                          : qrow[q],
-              t = QLDS ? shape.drafted(from) : qt[q];
+    // (QROWS: four lanes a row, 64 neighbouring bytes an instruction)
+    const int from = QROWS ? std::min(first + (wq * NQ + q) * 16 + (own_lane >> 2), rows_in - 1)
+                           : qrow[q],
+              t = QROWS ? shape.drafted(from) : qt[q];
     const char *p = reinterpret_cast<const char *>(
         a.q + (row0 + t) * a.ldq + (size_t)(g * per_kv + from - t * per_kv) * HD);
 #pragma unroll
     for (int i = 0; i < HD / 16; i++) {
-      const int d = QLDS ? Q4 ? 32 * (i >> 1) + 8 * (own_lane & 3) + 4 * (i & 1)
-                              : 16 * i + 4 * (own_lane & 3)
+      const int d = QROWS ? 16 * i + 4 * (own_lane & 3)
                     : F32 ? 16 * i + 4 * g4
                     : Q4 ? g4 * (HD / 4) + 4 * i
                     : Q8 ? (i >> 2) * 64 + g4 * 16 + (i & 3) * 4
@@ -874,44 +875,32 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
       for (int i = 0; i < HD / 16; i++)
 #pragma unroll
         for (int e = 0; e < 4; e++) m = fmaxf(m, fabsf(qx[q][i][e]));
-      m = QLDS ? quad_max_dpp(m) : rows4_max(m);
+      m = QROWS ? quad_max_dpp(m) : rows4_max(m);
       // m * 2^k in [2^13, 2^14) (rows below 2^-113: less); infinities and NaN stay
       // what they are
       const int k = m > 0.f && m < INFINITY ? std::min(126, 140 - (int)(__float_as_uint(m) >> 23)) : 0;
       const float up = sign * __uint_as_float((uint32_t)(127 + k) << 23);
-      if constexpr (QLDS) {
+      if constexpr (QROWS) {
         // (as operands: 16 bytes of lane 16 g4 + row for each of (step, part))
-        const int row = own_lane >> 2, seg = own_lane & 3;
-        char *const to = reinterpret_cast<char *>(sm_acc) + wave * QW * 4 + q * (HD / 32) * 2048;
+        char *const to = reinterpret_cast<char *>(qs - lane + 64 * 2 * (HD / 32) * q +
+                                                  16 * (own_lane >> 1 & 1) + (own_lane >> 2)) +
+                         8 * (own_lane & 1);
 #pragma unroll
-        for (int i = 0; i < HD / 16; i += 2) {
-          u4 h, l;
+        for (int i = 0; i < HD / 16; i++) {
+          u2 h, l;
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const f4 x = qx[q][i + (Q4 ? 0 : e >> 1)], y = qx[q][i + (Q4 ? 1 : e >> 1)];
+          for (int e = 0; e < 2; e++) {
             uint32_t hi, lo;
-            split2(x[Q4 ? e : 2 * (e & 1)] * up, y[Q4 ? e : 2 * (e & 1) + 1] * up, hi, lo);
+            split2(qx[q][i][2 * e] * up, qx[q][i][2 * e + 1] * up, hi, lo);
             h[e] = hi;
             l[e] = lo;
           }
-          if constexpr (Q4) {
-            const int g = HD == 128 ? i >> 1 : i + (seg >> 1), at = HD == 128 ? seg : seg & 1;
-            u4 *const o = reinterpret_cast<u4 *>(to + at * 2048 + (16 * g + row) * 16);
-            o[0] = h;
-            o[64] = l;
-          } else {
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-              const int at = Q8 ? (i >> 2) * 2 + (seg >> 1) : i >> 1,
-                        g = Q8 ? (i & 2) + u : 2 * u + (seg >> 1);
-              u2 *const o = reinterpret_cast<u2 *>(to + at * 2048 + (16 * g + row) * 16 + 8 * (seg & 1));
-              o[0] = (u2){h[2 * u], h[2 * u + 1]};
-              o[128] = (u2){l[2 * u], l[2 * u + 1]};
-            }
-          }
+          u2 *const o = reinterpret_cast<u2 *>(to + (i >> 1) * 2048 + (i & 1) * 512);
+          o[0] = h;
+          o[128] = l;
         }
         asm volatile("" ::: "memory");
-        sfac[q] = ldexpf(factor, (Q4 ? 19 : Q8 ? 9 : 0) - __shfl(k, 4 * n16));
+        sfac[q] = ldexpf(factor, -__shfl(k, 4 * n16));
         continue;
       }
 #pragma unroll
@@ -929,6 +918,9 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
         if constexpr (SIDE) {
 #pragma unroll
           for (int e = 0; e < 4; e++) qh[q][i][e] = n16 < 8 ? h[e] : l[e];
+        } else if constexpr (QLDS) {
+          qs[(q * (HD / 32) + i) * 2 * 64] = h;
+          qs[((q * (HD / 32) + i) * 2 + 1) * 64] = l;
         } else {
           qh[q][i] = h;
           ql[q][i] = l;
