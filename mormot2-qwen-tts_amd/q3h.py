@@ -884,16 +884,17 @@ class Cache:
         cfg = CacheConfig(sequences, layers, kv_heads, head_dim, max_positions, fmt)
         h = _P()
         L = lib()
+        _use_torch()
+        self.dev = dev
+        self._destroy = L.q3h_cache_destroy
         if pages:
             paged = PagedConfig(cfg, pages, page_positions)
             _check(L.q3h_cache_create_paged(dev.h, ctypes.byref(paged), ctypes.byref(h)))
         else:
             _check(L.q3h_cache_create(dev.h, ctypes.byref(cfg), ctypes.byref(h)))
-        _use_torch()
+        self.h = h  # (from here on __del__ gives it back)
         self.pages = pages
-        self.table_shape = (sequences, -(-max_positions // page_positions))
-        self.dev = dev
-        self.h = h
+        self.table_shape = (sequences, -(-max_positions // page_positions)) if pages else None
         self.kv_heads, self.head_dim = kv_heads, head_dim
         self._append, self._read, self._attend = \
             L.q3h_cache_append, L.q3h_cache_read, L.q3h_cache_attend
@@ -904,7 +905,6 @@ class Cache:
             L.q3h_cache_compact, L.q3h_cache_copy, L.q3h_cache_page_state
         self._device = _torch.device("cuda", dev.ordinal)
         self._workspace = L.q3h_cache_attend_workspace
-        self._destroy = L.q3h_cache_destroy
 
     @property
     def bytes(self):
