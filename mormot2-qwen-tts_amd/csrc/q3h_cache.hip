@@ -877,43 +877,39 @@ using namespace q3h;
 
 namespace {
 
-int create_rope(q3h_device *dev, const q3h_rope_config *cfg, int axes, const int32_t *pair_axes,
-                q3h_rope **out) {
+int create_rope(const char *who, q3h_device *dev, const q3h_rope_config *cfg, int axes,
+                const int32_t *pair_axes, q3h_rope **out) {
   q3h_rope *r = nullptr;
   double *freq = nullptr;
+  auto need = [&](bool fine, const std::string &what) {
+    require(fine, Q3H_E_ARG, who + (": " + what));
+  };
   int rc = guard([&] {
-    require(dev && cfg && out, Q3H_E_ARG, "q3h_rope_create: NULL argument");
+    need(dev && cfg && out, "NULL argument");
     *out = nullptr;
     const q3h_rope_config &c = *cfg;
-    require(c.head_dim == 64 || c.head_dim == 128, Q3H_E_ARG,
-            "q3h_rope_create: head_dim must be 64 or 128");
-    require(c.rot_dim >= 2 && c.rot_dim <= c.head_dim && c.rot_dim % 2 == 0, Q3H_E_ARG,
-            "q3h_rope_create: rot_dim must be even and in [2, head_dim]");
-    require(c.interleaved == 0 || c.interleaved == 1, Q3H_E_ARG,
-            "q3h_rope_create: interleaved must be 0 or 1");
-    require(c.max_positions > 0 && c.max_positions <= (1 << 24), Q3H_E_ARG,
-            "q3h_rope_create: max_positions must be in [1, 2^24]");
-    require(c.theta > 1.f && std::isfinite(c.theta), Q3H_E_ARG,
-            "q3h_rope_create: theta must be above 1");
-    require(c.scaling >= Q3H_ROPE_PLAIN && c.scaling <= Q3H_ROPE_BANDS, Q3H_E_ARG,
-            "q3h_rope_create: no scaling " + std::to_string(c.scaling));
-    require(c.scaling == Q3H_ROPE_PLAIN || (c.factor > 0.f && std::isfinite(c.factor)), Q3H_E_ARG,
-            "q3h_rope_create: factor must be above 0");
-    require(c.scaling < Q3H_ROPE_YARN || c.original_positions > 0, Q3H_E_ARG,
-            "q3h_rope_create: original_positions must be above 0");
-    require(c.scaling != Q3H_ROPE_YARN ||
-                (c.beta_fast > c.beta_slow && c.beta_slow > 0.f && std::isfinite(c.beta_fast)),
-            Q3H_E_ARG, "q3h_rope_create: beta_fast > beta_slow > 0 is needed");
-    require(c.scaling != Q3H_ROPE_BANDS ||
-                (c.high_turns > c.low_turns && c.low_turns > 0.f && std::isfinite(c.high_turns)),
-            Q3H_E_ARG, "q3h_rope_create: high_turns > low_turns > 0 is needed");
-    require(std::isfinite(c.magnitude) && c.magnitude >= 0.f, Q3H_E_ARG,
-            "q3h_rope_create: magnitude must not be negative");
-    require(axes >= 1 && axes <= kMaxAxes, Q3H_E_ARG,
-            "q3h_rope_create_axes: axes must be in [1, 4]");
+    need(c.head_dim == 64 || c.head_dim == 128, "head_dim must be 64 or 128");
+    need(c.rot_dim >= 2 && c.rot_dim <= c.head_dim && c.rot_dim % 2 == 0,
+         "rot_dim must be even and in [2, head_dim]");
+    need(c.interleaved == 0 || c.interleaved == 1, "interleaved must be 0 or 1");
+    need(c.max_positions > 0 && c.max_positions <= (1 << 24), "max_positions must be in [1, 2^24]");
+    need(c.theta > 1.f && std::isfinite(c.theta), "theta must be above 1");
+    need(c.scaling >= Q3H_ROPE_PLAIN && c.scaling <= Q3H_ROPE_BANDS,
+         "no scaling " + std::to_string(c.scaling));
+    need(c.scaling == Q3H_ROPE_PLAIN || (c.factor > 0.f && std::isfinite(c.factor)),
+         "factor must be above 0");
+    need(c.scaling < Q3H_ROPE_YARN || c.original_positions > 0,
+         "original_positions must be above 0");
+    need(c.scaling != Q3H_ROPE_YARN ||
+             (c.beta_fast > c.beta_slow && c.beta_slow > 0.f && std::isfinite(c.beta_fast)),
+         "beta_fast > beta_slow > 0 is needed");
+    need(c.scaling != Q3H_ROPE_BANDS ||
+             (c.high_turns > c.low_turns && c.low_turns > 0.f && std::isfinite(c.high_turns)),
+         "high_turns > low_turns > 0 is needed");
+    need(std::isfinite(c.magnitude) && c.magnitude >= 0.f, "magnitude must not be negative");
+    need(axes >= 1 && axes <= kMaxAxes, "axes must be in [1, 4]");
     for (int i = 0; pair_axes && i < c.rot_dim / 2; i++)
-      require(pair_axes[i] >= 0 && pair_axes[i] < axes, Q3H_E_ARG,
-              "q3h_rope_create_axes: no axis " + std::to_string(pair_axes[i]));
+      need(pair_axes[i] >= 0 && pair_axes[i] < axes, "no axis " + std::to_string(pair_axes[i]));
     DeviceScope scope(dev->ordinal);
     r = new q3h_rope();
     r->dev = dev;
@@ -948,14 +944,14 @@ int create_rope(q3h_device *dev, const q3h_rope_config *cfg, int axes, const int
 }  // namespace
 
 extern "C" int q3h_rope_create(q3h_device *dev, const q3h_rope_config *cfg, q3h_rope **out) {
-  return create_rope(dev, cfg, 1, nullptr, out);
+  return create_rope("q3h_rope_create", dev, cfg, 1, nullptr, out);
 }
 
 extern "C" int q3h_rope_create_axes(q3h_device *dev, const q3h_rope_config *cfg, int axes,
                                     const int32_t *pair_axes, q3h_rope **out) {
   if (!pair_axes)
     return guard([&] { require(false, Q3H_E_ARG, "q3h_rope_create_axes: NULL argument"); });
-  return create_rope(dev, cfg, axes, pair_axes, out);
+  return create_rope("q3h_rope_create_axes", dev, cfg, axes, pair_axes, out);
 }
 
 extern "C" int q3h_rope_destroy(q3h_rope *r) {
@@ -1017,33 +1013,34 @@ extern "C" int q3h_cache_destroy(q3h_cache *c) {
 
 namespace {
 
-int append(q3h_cache *c, const q3h_append_args *p, const int32_t *places, void *stream) {
+int append(const char *who, q3h_cache *c, const q3h_append_args *p, const int32_t *places,
+           void *stream) {
   return guard([&] {
-    require(c && p, Q3H_E_ARG, "q3h_cache_append: NULL argument");
+    auto need = [&](bool fine, const char *what, int code = Q3H_E_ARG) {
+      if (!fine) require(false, code, who + std::string(": ") + what);
+    };
+    need(c && p, "NULL argument");
     const q3h_cache_config &cf = c->cfg;
-    check_rows(c, p->layer, p->sequences, p->rows, "q3h_cache_append");
-    require(p->heads >= 0 && p->heads <= 4096, Q3H_E_ARG, "q3h_cache_append: bad heads");
+    check_rows(c, p->layer, p->sequences, p->rows, who);
+    need(p->heads >= 0 && p->heads <= 4096, "bad heads");
     if (p->sequences == 0 || p->rows == 0) return;
-    require(p->k && p->v && p->lens, Q3H_E_ARG, "q3h_cache_append: NULL k, v or lens");
-    require(p->heads == 0 || (p->q && p->q_out), Q3H_E_ARG, "q3h_cache_append: NULL q or q_out");
+    need(p->k && p->v && p->lens, "NULL k, v or lens");
+    need(p->heads == 0 || (p->q && p->q_out), "NULL q or q_out");
     const int64_t wq = (int64_t)p->heads * cf.head_dim, wk = (int64_t)cf.kv_heads * cf.head_dim;
-    require(p->ldk >= wk && p->ldv >= wk && (p->heads == 0 || (p->ldq >= wq && p->ld_out >= wq)),
-            Q3H_E_ARG, "q3h_cache_append: rows overlap (a row distance below the row's width)");
-    require(p->heads == 0 || p->q_out != p->q || p->ldq == p->ld_out, Q3H_E_ARG,
-            "q3h_cache_append: in place with another row distance");
-    require((p->q_norm == nullptr && p->k_norm == nullptr) || p->eps >= 0.f, Q3H_E_ARG,
-            "q3h_cache_append: eps must not be negative");
-    require(!p->parents || p->rows <= Q3H_TREE_MAX_ROWS, Q3H_E_CAPACITY,
-            "q3h_cache_append: a tree has at most 64 rows");
-    require(launch_fits((int64_t)p->sequences * p->rows), Q3H_E_CAPACITY,
-            "q3h_cache_append: too many rows");
+    need(p->ldk >= wk && p->ldv >= wk && (p->heads == 0 || (p->ldq >= wq && p->ld_out >= wq)),
+         "rows overlap (a row distance below the row's width)");
+    need(p->heads == 0 || p->q_out != p->q || p->ldq == p->ld_out,
+         "in place with another row distance");
+    need((p->q_norm == nullptr && p->k_norm == nullptr) || p->eps >= 0.f,
+         "eps must not be negative");
+    need(!p->parents || p->rows <= Q3H_TREE_MAX_ROWS, "a tree has at most 64 rows",
+         Q3H_E_CAPACITY);
+    need(launch_fits((int64_t)p->sequences * p->rows), "too many rows", Q3H_E_CAPACITY);
     if (p->rope) {
-      require(p->rope->dev->ordinal == c->dev->ordinal, Q3H_E_ARG,
-              "q3h_cache_append: rope of another device");
-      require(p->rope->cfg.head_dim == cf.head_dim, Q3H_E_ARG,
-              "q3h_cache_append: rope of another head_dim");
-      require(p->rope->cfg.max_positions >= cf.max_positions, Q3H_E_ARG,
-              "q3h_cache_append: the rope table has fewer positions than the cache");
+      need(p->rope->dev->ordinal == c->dev->ordinal, "rope of another device");
+      need(p->rope->cfg.head_dim == cf.head_dim, "rope of another head_dim");
+      need(p->rope->cfg.max_positions >= cf.max_positions,
+           "the rope table has fewer positions than the cache");
     }
     DeviceScope scope(c->dev->ordinal);
     AppendRows a{};
@@ -1079,7 +1076,7 @@ int append(q3h_cache *c, const q3h_append_args *p, const int32_t *places, void *
 }  // namespace
 
 extern "C" int q3h_cache_append(q3h_cache *c, const q3h_append_args *p, void *stream) {
-  return append(c, p, nullptr, stream);
+  return append("q3h_cache_append", c, p, nullptr, stream);
 }
 
 extern "C" int q3h_cache_append_at(q3h_cache *c, const q3h_append_args *p,
@@ -1088,7 +1085,7 @@ extern "C" int q3h_cache_append_at(q3h_cache *c, const q3h_append_args *p,
     return guard([&] {
       require(false, Q3H_E_ARG, "q3h_cache_append_at: NULL positions or rope");
     });
-  return append(c, p, positions, stream);
+  return append("q3h_cache_append_at", c, p, positions, stream);
 }
 
 extern "C" int q3h_cache_read(q3h_cache *c, int layer, int sequences, int rows,
