@@ -1013,8 +1013,9 @@ extern "C" int q3h_cache_destroy(q3h_cache *c) {
 
 namespace {
 
-int append(const char *who, q3h_cache *c, const q3h_append_args *p, const int32_t *places,
-           void *stream) {
+// placed: by positions of the rows (places)
+int append(const char *who, q3h_cache *c, const q3h_append_args *p, bool placed,
+           const int32_t *places, void *stream) {
   return guard([&] {
     auto need = [&](bool fine, const char *what, int code = Q3H_E_ARG) {
       if (!fine) require(false, code, who + std::string(": ") + what);
@@ -1024,6 +1025,7 @@ int append(const char *who, q3h_cache *c, const q3h_append_args *p, const int32_
     check_rows(c, p->layer, p->sequences, p->rows, who);
     need(p->heads >= 0 && p->heads <= 4096, "bad heads");
     if (p->sequences == 0 || p->rows == 0) return;
+    need(!placed || (places && p->rope), "NULL positions or rope");
     need(p->k && p->v && p->lens, "NULL k, v or lens");
     need(p->heads == 0 || (p->q && p->q_out), "NULL q or q_out");
     const int64_t wq = (int64_t)p->heads * cf.head_dim, wk = (int64_t)cf.kv_heads * cf.head_dim;
@@ -1076,16 +1078,12 @@ int append(const char *who, q3h_cache *c, const q3h_append_args *p, const int32_
 }  // namespace
 
 extern "C" int q3h_cache_append(q3h_cache *c, const q3h_append_args *p, void *stream) {
-  return append("q3h_cache_append", c, p, nullptr, stream);
+  return append("q3h_cache_append", c, p, false, nullptr, stream);
 }
 
 extern "C" int q3h_cache_append_at(q3h_cache *c, const q3h_append_args *p,
                                    const int32_t *positions, void *stream) {
-  if (!positions || (p && !p->rope))
-    return guard([&] {
-      require(false, Q3H_E_ARG, "q3h_cache_append_at: NULL positions or rope");
-    });
-  return append("q3h_cache_append_at", c, p, positions, stream);
+  return append("q3h_cache_append_at", c, p, true, positions, stream);
 }
 
 extern "C" int q3h_cache_read(q3h_cache *c, int layer, int sequences, int rows,

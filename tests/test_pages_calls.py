@@ -121,6 +121,20 @@ PARTS = {
   expect("no config", "q3h_rope_create", Q3H_E_ARG, q3h_rope_create(&dev, nullptr, &ro));
   expect("axes", "q3h_rope_create_axes", Q3H_E_ARG, q3h_rope_create_axes(&dev, &r, 5, axes, &ro));
 """,
+    # nothing to write: as q3h_cache_append takes it, without positions
+    "nothing to write": r"""
+  q3h_append_args a = good;
+  a.rows = 0;
+  a.q = a.k = a.v = nullptr, a.q_out = nullptr, a.lens = nullptr;
+  expect("no rows", at, Q3H_OK, q3h_cache_append_at(&c, &a, nullptr, 0));
+  expect("no rows", plain, Q3H_OK, q3h_cache_append(&c, &a, 0));
+  a.rope = nullptr;
+  expect("no rows or rope", at, Q3H_OK, q3h_cache_append_at(&c, &a, nullptr, 0));
+  a.rows = 10, a.sequences = 0;
+  expect("no sequences", at, Q3H_OK, q3h_cache_append_at(&c, &a, nullptr, 0));
+  a.layer = 2;
+  expect("no sequences of no layer", at, Q3H_E_ARG, q3h_cache_append_at(&c, &a, nullptr, 0));
+""",
 }
 
 
