@@ -456,7 +456,8 @@ __device__ __forceinline__ Forked forked(const Book &k, int b, const int32_t *so
   Forked f{sources[b], 0, k.held[b]};
   if (f.from >= 0 && f.from < k.sequences) {
     const int len = lens[b], held = k.held[f.from];
-    f.now = len < 0 || len > (int64_t)held << k.page_log2
+    // (the last page can reach behind the cache's positions)
+    f.now = len < 0 || len > k.max_pos || len > (int64_t)held << k.page_log2
                 ? -1
                 : (int)(((int64_t)len + (1 << k.page_log2) - 1) >> k.page_log2);
   } else if (f.from != -1) {

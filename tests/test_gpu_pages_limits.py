@@ -1,4 +1,5 @@
-"""Caches in pages at the edges of what their calls take: calls without rows."""
+"""Caches in pages at the edges of what their calls take: lengths between a cache's last
+position and the end of its last page, calls without rows."""
 import gc
 
 import numpy as np
@@ -16,6 +17,36 @@ def no_handles_left():
     """Handles that a refusal's traceback still holds go before the device does."""
     yield
     gc.collect()
+
+
+@pytest.mark.parametrize("sequences", [4, 1500])
+@pytest.mark.parametrize("positions,page", [(100, 32), (97, 64), (1, 256), (129, 128)])
+def test_fork_beyond_the_cache(device, sequences, positions, page):
+    """A length that the source's last page reaches and the cache's positions do not leaves
+    its sequence as it is: of few sequences in one launch, of many in two."""
+    print(f"fork of {sequences} sequences of {positions} in pages of {page}", flush=True)
+    slots = -(-positions // page)
+    cache = q3h.Cache(device, sequences, 1, 64, positions, q3h.KV_F16, pages=3 * slots,
+                      page_positions=page)
+    zero = np.zeros(sequences, int)
+    counts = zero.copy()
+    counts[:2] = positions, 1
+    cache.reserve(dev_i(zero), positions, counts=dev_i(counts))
+    before = [t.cpu().numpy() for t in cache.page_state()]
+    assert before[1][:2].tolist() == [slots, 1]
+    most = slots * page
+    for length in (positions + 1, most, most + 1, 2 ** 31 - 1):
+        sources, lens = np.full(sequences, -2), zero.copy()
+        sources[:3], lens[:3] = 0, length
+        cache.fork(dev_i(sources), dev_i(lens))
+        for was, now in zip(before, cache.page_state()):
+            np.testing.assert_array_equal(was, now.cpu().numpy(), err_msg=str(length))
+    sources, lens = np.full(sequences, -2), zero.copy()
+    sources[1], lens[1] = 0, positions
+    cache.fork(dev_i(sources), dev_i(lens))
+    table, held, refs = [t.cpu().numpy() for t in cache.page_state()]
+    np.testing.assert_array_equal(table[1], table[0])
+    assert held[1] == slots and (refs[table[0]] == 2).all()
 
 
 def test_append_of_no_rows_at_positions(device):
