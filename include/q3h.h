@@ -426,9 +426,11 @@ int q3h_codec_destroy(q3h_codec *c);
    and kv head: scale = max |x| / 1785 rounded to f32 (1785 = 7 * 255), step = max |x| of
    the 32 / (7 scale) rounded up (255 at most), element = x / (step * scale) rounded to
    even within -7 .. 7, from 64 bits; it stands for element * step * scale. An element is
-   off by at most 1/14 of the largest of its 32 and 1/3570 of the row's largest. A
-   position takes head_dim / 2 + 8 bytes a kv head. A row with an infinity or NaN reads as
-   NaN. */
+   off by at most 1/14 of the largest of its 32 plus 1/3570 of the row's largest, and by
+   f32's roundings of the scale and the product beside that: 2^-23 of the row's largest, or
+   2.6e-42 where that is more (a row under 1.2e-42 reads as zeros). A row, the key or the
+   value of a position and kv head, takes head_dim / 2 + 8 bytes. A row with an infinity
+   or NaN reads as NaN. */
 #define Q3H_KV_Q4 4
 #define Q3H_TREE_MAX_ROWS 64
 #define Q3H_TOP_MAX 64
