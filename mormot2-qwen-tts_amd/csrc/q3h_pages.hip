@@ -443,11 +443,14 @@ __global__ __launch_bounds__(kThreads) void k_copy_tails(KvView v, Book k, const
   copy_tail<FMT, HD>(v, page, from, k.copy_to[b], lens[b] & (page - 1), section);
 }
 
-// A fork's table: of few slots by one workgroup, its entries in registers between reading
-// and writing (an assignment may be any, so that none is written before all are read); of
-// more in two launches, the table beside the present one first. 4 sequences of two slots 3.4
-// us, 128 of 31 5.2: a chain of four trips to memory.
-constexpr int kForkEach = 16, kForkSlots = kForkEach * kBook;
+// A fork's table: of up to 4096 entries (and 1024 sequences) by one workgroup, four of them a
+// thread in registers between reading and writing (an assignment may be any, so that none is
+// written before all are read); of more in two launches, the table beside the present one
+// first. A chain of four trips to memory, in a graph: 4 sequences of two slots 2.6 us (two
+// launches 5.0), 128 of 16 3.4 (5.2), 1024 of 4 4.2 (5.7), 64 of 64 4.1 (5.1), 256 of 17 in
+// two 5.4. With sixteen entries a thread, each asked for in turn, 64 of two took 4.1 us, and
+// 512 of 32 in one launch 10.0 (two 5.2).
+constexpr int kForkEach = 4, kForkSlots = kForkEach * kBook;
 struct Forked {
   int from, now, held;  // (now < 0: as it is)
 };

@@ -1,11 +1,13 @@
 """Caches in pages at the edges of what their calls take: lengths between a cache's last
-position and the end of its last page, calls without rows."""
+position and the end of its last page, calls without rows, tables of just the size that is
+forked in one launch and of more."""
 import gc
 
 import numpy as np
 import pytest
 import torch
 
+import pages_ref as pref
 import q3h
 from test_gpu_draft import dev_i
 
@@ -60,3 +62,30 @@ def test_append_of_no_rows_at_positions(device):
             q = cache.append(x, x, dev_i(np.zeros(n)), q=x, rope=rope, positions=at)
             assert q.shape == x.shape
             cache.append(x, x, dev_i(np.zeros(n)), rope=rope)
+
+
+@pytest.mark.parametrize("n,slots", [(1024, 4), (1023, 5), (1025, 3), (64, 64), (65, 64), (63, 65),
+                                     (1, 4096), (1, 4097), (3, 1365), (300, 40)])
+def test_forks_of_any_size(device, n, slots):
+    """Any assignment of sequences, a few times over, against lists."""
+    print(f"fork of {n} sequences of {slots} pages", flush=True)
+    rng = np.random.default_rng(n + slots)
+    P, pages = 32 * slots, n * slots + 5
+    cache = q3h.Cache(device, n, 1, 64, P, q3h.KV_Q4, pages=pages, page_positions=32)
+    model = pref.Pages(n, pages, 32, P)
+    counts = rng.integers(0, P + 1, n)
+    counts[rng.integers(0, n)] = P
+    cache.reserve(dev_i(np.zeros(n)), P, counts=dev_i(counts))
+    model.reserve([0] * n, counts.tolist())
+    for m in (n, n, max(1, n // 2), n):
+        sources = rng.integers(-1, n, m)
+        sources[rng.random(m) < 0.3] = 0
+        own = rng.random(m) < 0.3
+        sources[own] = np.arange(m)[own]
+        room = np.array([len(model.lists[s]) * 32 if s >= 0 else 0 for s in sources])
+        lens = np.where(rng.random(m) < 0.5, room, (room * rng.random(m)).astype(int))
+        cache.fork(dev_i(sources), dev_i(lens))
+        model.fork(sources.tolist(), lens.tolist())
+        for got, want in zip(cache.page_state(),
+                             (model.table(), [len(x) for x in model.lists], model.refs())):
+            np.testing.assert_array_equal(got.cpu().numpy(), want)
