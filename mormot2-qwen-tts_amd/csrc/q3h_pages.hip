@@ -194,7 +194,10 @@ __device__ __forceinline__ bool last_to_come(const Book &k) {
 // 16 of up to 33 pages 5.6, four beams of a shared page 7.3 and 128 of 16 prompts, where the
 // rows of 112 pages are copied in 5 layers of 4 bits, 29 MB read and written, 16.4. (In two
 // launches, one workgroup and then the copies, fork and reserve of the four beams 16.8 us,
-// 10.7 so.)
+// 10.7 so.) At its largest, 1024 slots, it is still the faster form: 512 beams of 256 prompts
+// 8 us (two launches 12), 64 sequences that take 15 pages each 8.3 with the release before
+// (12.0); it is the threads and LDS that end there. Few free pages behind many used ones cost
+// a scan by every workgroup: 16 pages, 99000 of 100000 in use, 54 us (57 in two launches).
 template <int FMT, int HD>
 __global__ __launch_bounds__(kBook) void k_reserve(Book k, KvView v, int n, int rows,
                                                    const int32_t *lens, const int32_t *counts,
@@ -296,10 +299,12 @@ __global__ __launch_bounds__(kBook) void k_reserve(Book k, KvView v, int n, int 
   }
 }
 
-// The same of any number of slots (32 sequences of up to 64 pages at once 13.3 us,
-// and a launch for the copies): one workgroup, `group` lanes (a power of two) a
-// sequence at a time: who writes to which shared page (writers, lowest), how many pages
-// each sequence wants, their sums in order, the lowest free pages in order, who gets which.
+// The same of any number of slots, and a launch for the copies: one workgroup, `group`
+// lanes (a power of two) a sequence at a time: who writes to which shared page (writers,
+// lowest), how many pages each sequence wants, their sums in order, the lowest free pages in
+// order, who gets which. A pass over the slots for each, of one workgroup's trips to memory:
+// 32 sequences of up to 64 pages at once 13.3 us, 1024 beams of 512 prompts 17.5 with the
+// copies, 2048 of 1024 30, 256 sequences of 15 pages that they have already 16.7.
 __global__ __launch_bounds__(kBook) void k_reserve_many(Book k, int n, int rows, const int32_t *lens,
                                                         const int32_t *counts, int32_t *ok,
                                                         int group) {
@@ -599,7 +604,12 @@ __device__ __forceinline__ void move_pages(char *base, int64_t page_bytes, int m
 // Up to 8192 pages: every workgroup works out the moves, makes its part of them and of
 // the tables' changes, and the last to come changes who holds which page. Nothing to move:
 // 6.4 us, a scan of all pages by every workgroup before its first load; 164 of 64 positions
-// and 2 layers of int8, 89 MB read and written, 20.
+// and 2 layers of int8, 89 MB read and written, 20. Against one workgroup and a launch for the
+// moves, with few workgroups (pages of 2.5 KB, nothing to move / half of them): 1024 pages 4.6
+// / 7.5 us (5.9 / 7.5), 4096 6.5 / 9.6 (7.1 / 11.7), 8192 9.2 / 13.8 (8.7 / 16.2); with 512
+// of them nothing to move of 512 pages of 7.3 MB 10.0 (5.6) and of 8192 of 135 KB 13.7 (8.7),
+// half of the 512 moved, 3.8 GB read and written, 774 (791). What moves in earnest decides for
+// one launch; the lists in LDS end at 8192.
 __global__ __launch_bounds__(kBook) void k_compact(Book k, char *base, int64_t page_bytes,
                                                    int32_t *used) {
   __shared__ int32_t sm_hole[kScan / 2], sm_mover[kScan / 2];
@@ -639,7 +649,8 @@ __global__ __launch_bounds__(kBook) void k_compact(Book k, char *base, int64_t p
 }
 
 // Any number of pages: one workgroup for the lists, a mover's new place in moved, then the
-// moves and the tables of the sequences.
+// moves and the tables of the sequences. The scan of the holders is the time: 16384 pages,
+// nothing to move, 20 us, 100000 101.
 __global__ __launch_bounds__(kBook) void k_compact_many(Book k, int32_t *used) {
   const int2 n = compact_lists(k, [&](int i, int p, bool moves) { (moves ? k.order : k.olds)[i] = p; });
   __syncthreads();

@@ -40,7 +40,8 @@
 //   us + 11.4 by the box, where VALU (300 instructions a wave and tile, 16 scores a lane taking 9
 //   each) and matrix instructions (64) take turns more than they overlap: 69 % and
 //   34 % of the time. 260 TFLOP/s of the definition's operations, twice that in
-//   products;
+//   products (traced, each kernel by itself; one behind the other they take less: the
+//   same trees in 4 bits 138-147 + 12 traced, both together 133);
 // - 2 prompts of 1500 rows over 500 and 125 positions, 16 heads over 8, 26 GFLOP: f16 112
 //   us, int8 126, 4 bits 130, f32 354 (both over 500: VALU 45 % and matrix instructions 23 %
 //   of the time, 1.6 waves a SIMD on average);
@@ -49,9 +50,9 @@
 //   nibbles; 12 us are a share's beginning, end and the join, 2 the pages, a step 0.9. 64
 //   sequences of 4000 .. 16000 positions 178 (4.1 TB/s; int8 291 at 4.65). One row over 171
 //   positions 7.6, over 8000 13.6;
-// - the 12 trees in 4 bits 141 + 12: the conversions of int8 (130) with a step more. A step of
-//   four waves takes 5700 cycles, two workgroups on a CU: scores 1240, the next loads 740,
-//   softmax 1700, values 1250, conversions and barriers 780; alone on a CU 5100.
+// - the 12 trees in 4 bits 133 with the join: the conversions of int8 with a step more. A step
+//   of four waves takes 5640 cycles, two workgroups on a CU: scores 1250, the next loads 590,
+//   softmax 1750, values 1280, conversions and barriers 770; alone on a CU 4930.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -377,8 +378,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
   constexpr bool QLDS = NQ > 1 && !F32;
   // on their way there loaded by whole rows, not as the operands have them, where every
   // lane's 16 bytes are a line of their own: a tree of 27 rows over 12289 positions of f16 in
-  // pages 28.4 -> 27.3 us; not over int8 and 4 bits (2 prompts of 1500 rows 93.0 -> 94.8, 12
-  // trees 126.5 -> 128)
+  // pages 28.4 -> 27.3 us; not over int8 and 4 bits (2 prompts of up to 1500 rows 93.0 -> 94.8,
+  // 12 trees, 420 rows, 126.5 -> 128)
   constexpr bool QROWS = QLDS && FMT == Q3H_KV_F16;
   constexpr int QW = NQ * (HD / 32) * 2 * 256;  // words of a wave's queries
   // with four waves side by side also a tile's keys and values as operands, each
@@ -602,7 +603,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(AttendRows a, Shape shap
   // of the values 8 behind): one load of four bytes, where all in every lane are four of 16,
   // which the address path takes as many cycles for as for 16 different bytes a lane; an
   // operand that another lane of the row holds costs nothing, and 15 registers are free (12
-  // trees in int8 189 -> 183 us, in 4 bits 199 -> 193, launched one behind another; prompts
+  // full trees, 768 rows with the join, in int8 189 -> 183 us, in 4 bits 199 -> 193; prompts
   // 131 -> 126).
   const int of_row = 16 * (n16 >> 2 & 1) + 4 * g4 + (n16 & 3);
   const char *const sc_row = SC ? (n16 < 8 ? ksc : vsc) : nullptr;
