@@ -851,6 +851,8 @@ class Rope:
             pairs = [int(x) for x in axes]
             if len(pairs) != cfg.rot_dim // 2:
                 _bad(f"axes of {len(pairs)} pairs, not of {cfg.rot_dim // 2}")
+            if not all(0 <= x < 4 for x in pairs):  # (32 bits would make others of some)
+                _bad(f"axes {sorted(set(pairs))}, not of 0 .. 3")
             self.axes = max(pairs, default=0) + 1
             _check(L.q3h_rope_create_axes(dev.h, ctypes.byref(cfg), self.axes,
                                           (ctypes.c_int32 * len(pairs))(*pairs), ctypes.byref(h)))

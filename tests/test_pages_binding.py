@@ -1,5 +1,6 @@
-"""The binding's handles of caches, without a device: a library in its place that counts
+"""The binding's handles of caches and rotary tables, without a device: a library in its place that counts
 what it makes and takes back."""
+import ctypes
 import gc
 import types
 
@@ -7,7 +8,7 @@ import pytest
 
 
 class Library:
-    """The entry points that a cache's handle is made and destroyed with."""
+    """The entry points that a handle is made and destroyed with."""
 
     def __init__(self, real):
         self.real, self.made, self.live, self.lacks = real, 0, set(), None
@@ -23,11 +24,18 @@ class Library:
         out._obj.value = self.made
         return 0
 
-    q3h_cache_create = q3h_cache_create_paged = _make
+    q3h_cache_create = q3h_cache_create_paged = q3h_rope_create = _make
+
+    def q3h_rope_create_axes(self, dev, cfg, axes, pairs, out):
+        axes = ctypes.c_int(axes).value  # (what reaches it)
+        fine = 1 <= axes <= 4 and all(0 <= x < axes for x in pairs)
+        return self._make(dev, cfg, out) if fine else -1
 
     def q3h_cache_destroy(self, h):
         self.live.remove(h.value)
         return 0
+
+    q3h_rope_destroy = q3h_cache_destroy
 
 
 @pytest.fixture
@@ -73,3 +81,17 @@ def test_caches_in_pages_know_their_tables(q3h, library):
     del cache
     gc.collect()
     assert library.made == 1 and not library.live
+
+
+def test_axes_that_there_are_not(q3h, library):
+    """An axis outside 0 .. 3 is refused, one that 32 bits would make another of as well."""
+    for axis in (-1, 4, 2 ** 31, 2 ** 32, 2 ** 32 + 1, -2 ** 32):
+        with pytest.raises(q3h.Q3HError) as e:
+            q3h.Rope(DEV, 64, 100, 1e4, axes=[axis] * 32)
+        assert e.value.code == q3h.E_ARG
+        with pytest.raises(q3h.Q3HError) as e:
+            q3h.Rope(DEV, 64, 100, 1e4, axes=[3] * 31 + [axis])
+        assert e.value.code == q3h.E_ARG
+    assert library.made == 0
+    rope = q3h.Rope(DEV, 64, 100, 1e4, axes=[i % 4 for i in range(32)])
+    assert rope.axes == 4 and library.made == 1
